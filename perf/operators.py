@@ -258,7 +258,8 @@ def _plain_plan(s):
     b = grown[r, (pos // page).clamp(min=0)].long()
     slots = torch.where(here & (b >= 0), b * page + pos % page, -1)
     taken = torch.minimum(want.sum(), tail - head)
-    info = torch.stack([head + taken, tail + back.sum(), cu[-1], want.sum() - taken])
+    turn = (head + taken) // n_blocks * n_blocks  # the head stays inside the ring
+    info = torch.stack([head + taken - turn, tail + back.sum() - turn, cu[-1], want.sum() - taken])
     seq = torch.where(ends, 0, ctx + come)
     return {"cu": cu.int(), "seq": seq.int(), "pos": pos.int(), "slots": slots.int(), "info": info.int(), "tables": tables, "ring": ring}
 
