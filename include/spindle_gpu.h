@@ -52,6 +52,7 @@ typedef int32_t sg_status;
 #define SG_Q8_0 8
 #define SG_Q4_K 12
 #define SG_Q6_K 14
+#define SG_BF16 30 /* activations of the paged cache and log-probability calls only */
 
 /* Weight layouts (sg_mat.layout).  GGUF: the file's rows, verbatim.
  * TILED16: the same bytes permuted once at upload by sg_repack_tiled16 so that
@@ -538,6 +539,114 @@ SG_API sg_status sg_pipe_send(const float *d_src, uint64_t n, uint64_t n_max, vo
                               void *stream);
 SG_API sg_status sg_pipe_recv(float *d_dst, uint64_t n, uint64_t n_max, void *d_recv, void *d_comm, void *d_peer_comm,
                               void *stream);
+
+/* ---- Paged KV cache in 4 bits, and token log probabilities -----------------------
+ *
+ * For serving many requests from one cache (the reference keeps one f16 cache
+ * per chat).  One step is sg_kv4_plan (block tables and slot maps from the
+ * requests' lengths), per layer sg_kv4_append of the new K/V rows and
+ * sg_kv4_attention of the new queries, and after the LM head sg_logprobs; every
+ * call takes its lengths and tables from device memory, so a step can be
+ * captured once and replayed.
+ *
+ * The cache is n_blocks blocks of `page` positions (a power of two, 16..1024);
+ * position p of a request whose block table says block b for p / page lies in
+ * slot b * page + p % page.  K and V rows of n_kv_heads x head_dim (64, 128 or
+ * 256) values are held in groups of 32 along head_dim as m + s * c: c of 4 bits,
+ * m = f16(min), s = f16((max - m) / 15), 20 bytes per group.  data:
+ * sg_kv4_bytes(c) device bytes, 16-byte aligned; one sg_kv4 per layer. */
+typedef struct {
+    uint32_t head_dim, n_kv_heads, page, n_blocks;
+    uint8_t *data;
+} sg_kv4;
+/* 0 for a shape that is not supported (n_blocks * page must be below 2^31). */
+SG_API uint64_t sg_kv4_bytes(const sg_kv4 *c);
+
+/* Block tables and slot maps of one step, from the lengths, on the device.
+ * Request i holds d_ctx[i] positions; d_new[i] >= 0 more come, or, if negative,
+ * it ends.  Free blocks stand in the ring d_ring[n_blocks] from d_cursor[0] to
+ * d_cursor[1] (indices modulo n_blocks; a new cache: the ring 0, 1, 2, ... and
+ * the cursor {0, n_blocks}).  Requests take blocks from its front in request
+ * order, and the blocks of ending requests (table entries that are blocks)
+ * go to its back; their table rows stay as they are, and a row is used again from
+ * d_ctx = 0.
+ *   d_tables [n_req] rows of width entries, ld_tables apart: entries below
+ *     ceil(ctx / page) are kept, those that the new positions need are written
+ *     (-1 where the ring is empty), the others stay;
+ *   d_cu [n_req + 1]: first new position of each request in the packed order;
+ *   d_seq [n_req]: ctx + new (0 for a request that ends);
+ *   d_pos, d_slots [max_tokens]: each new position's place in its request and
+ *     its slot, -1 where it has none; past the last new position both are -1;
+ *   d_info [4]: the next step's cursor (2), the sum of new, and the number of
+ *     blocks that were wanted and not there.  d_info must not be d_cursor.
+ * max_tokens at least the sum of the positive d_new.  Calling it again with the
+ * same cursor writes the same. */
+SG_API sg_status sg_kv4_plan(uint32_t page, uint32_t n_blocks, uint64_t n_req, const int32_t *d_ctx, const int32_t *d_new,
+                             int32_t *d_tables, uint64_t ld_tables, uint64_t width, int32_t *d_ring,
+                             const int32_t *d_cursor, int32_t *d_cu, int32_t *d_seq, int32_t *d_pos, int32_t *d_slots,
+                             uint64_t max_tokens, int32_t *d_info, void *stream);
+
+/* Quantizes n_tok K and V rows into their slots (negative or out of range: the
+ * row is left out; no two rows may have the same slot).  type SG_F32, SG_F16 or
+ * SG_BF16; element (t, h, d) of K at d_k[t * k_tok + h * k_head + d], V likewise.
+ * Values are clamped to f16's finite range and NaN counts as 0, so that the cache
+ * holds finite numbers only; d_nonfinite (optional) counts the groups that had an
+ * infinity or a NaN.  sg_kv4_read gives back the values of given slots as
+ * [n_tok][n_kv_heads][head_dim] of `type`, 16-byte aligned, zeros for no slot. */
+SG_API sg_status sg_kv4_append(const sg_kv4 *c, int32_t type, const void *d_k, uint64_t k_tok, uint64_t k_head,
+                               const void *d_v, uint64_t v_tok, uint64_t v_head, const int32_t *d_slots, uint64_t n_tok,
+                               int32_t *d_nonfinite, void *stream);
+SG_API sg_status sg_kv4_read(const sg_kv4 *c, int32_t type, const int32_t *d_slots, uint64_t n_tok, void *d_k, void *d_v,
+                             void *stream);
+
+/* Grouped-query attention of the new tokens over the cache, causal: token t of
+ * request i (cu[i] <= t < cu[i + 1]) stands at position seq[i] - (cu[i + 1] - t)
+ * and sees the positions up to its own, the last `window` of them if window > 0;
+ * the positions of table entries that are no block are not seen.  Query head hq
+ * reads KV head hq / (n_heads / n_kv_heads).  out = softmax(scale * q.k) v in
+ * q's type; lse (optional, f32 [n_tok][n_heads]) = ln of the softmax's sum, for
+ * joining with attention over other keys.  A token that sees nothing, or belongs
+ * to no request, gets zeros and lse = -infinity.  q and out: element (t, h, d) at
+ * [t * tok stride + h * head stride + d].  scale 0: 1 / sqrt(head_dim).  max_new:
+ * an upper bound of a request's new tokens (0: n_tok).  scratch:
+ * sg_kv4_attention_scratch_bytes() bytes, 256-byte aligned, zeroed once by
+ * sg_kv4_attention_scratch_init; calls that overlap on the GPU need one each. */
+typedef struct {
+    int32_t type;                     /* of q and out: SG_F32, SG_F16 or SG_BF16 */
+    uint32_t n_heads;
+    uint64_t n_tok, n_req;
+    const void *q;
+    uint64_t q_tok, q_head;
+    void *out;
+    uint64_t o_tok, o_head;
+    float *lse;
+    const int32_t *cu, *seq, *tables; /* as sg_kv4_plan writes them */
+    uint64_t ld_tables, width;
+    float scale;
+    uint32_t window;
+    uint64_t max_new;
+    void *scratch;
+    uint64_t scratch_bytes;
+} sg_kv4_attn;
+SG_API uint64_t sg_kv4_attention_scratch_bytes(void);
+SG_API sg_status sg_kv4_attention_scratch_init(void *d_scratch, uint64_t bytes, void *stream);
+SG_API sg_status sg_kv4_attention(const sg_kv4 *c, const sg_kv4_attn *a, void *stream);
+
+/* Log probabilities of given tokens: for each of the rows (d_logits + r * ld,
+ * vocab values of `type` SG_F32, SG_F16 or SG_BF16)
+ *   logprob = ln softmax(x)[tokens[r]], entropy = -sum p ln p (nats),
+ *   rank = how many tokens come before the given one when sorted by falling
+ *   logit, equal ones by rising id, and the first `top` <= SG_LOGPROBS_TOP_MAX
+ *   tokens of that order with their log probabilities ([rows][top]; ids first
+ *   the likeliest).  top <= vocab <= 2^30.
+ * A tokens[r] outside 0..vocab-1 (d_tokens NULL: all of them) gets logprob NaN
+ * and rank -1.  A row of minus infinities only has logprobs -infinity and
+ * entropy 0.  A NaN or an infinity in a row makes its probabilities NaN; NaN
+ * sorts before everything. */
+#define SG_LOGPROBS_TOP_MAX 64
+SG_API sg_status sg_logprobs(int32_t type, const void *d_logits, uint64_t ld, uint64_t rows, uint64_t vocab,
+                             const int32_t *d_tokens, float *d_logprob, float *d_entropy, int32_t *d_rank, uint64_t top,
+                             int32_t *d_top_ids, float *d_top_logprobs, void *stream);
 
 /* ---- the reference's synthetic benchmark kernels ----------------------------
  * Prototypes driven by the reference's early benchmark (main.rs), not by its

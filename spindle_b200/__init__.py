@@ -11,6 +11,9 @@ Host-side mirror of the reference's kernel API (WiseHax/spindle 1.1.0, src/):
   matmul_rows_float        quant_multi.rs:232-273 (float path, shared decode)
   Moe, moe_forward         smollm_chat.rs:1178-1382
   moe_forward_batch        smollm_chat.rs:928-1174
+and, beyond the reference, what serving many requests needs (kv4.py): Kv4Cache,
+kv4_plan, kv4_append, kv4_read, kv4_attention (a paged KV cache in 4 bits) and
+logprobs.
 Every call goes through the C ABI of include/spindle_gpu.h (libspindle_b200.so);
 torch tensors are only the device-memory plumbing.  There is no CPU path: a
 missing library or a failed call raises.
@@ -429,3 +432,8 @@ def decode_choice(choice):
     ids = [int(v) for v in c[4:4 + n]]
     w = c[4 + MOE_MAX_USED:4 + MOE_MAX_USED + n].view(torch.float32).tolist()
     return ids, w
+
+
+# ---- paged 4-bit KV cache and token log probabilities (serving many requests)
+from .kv4 import (Kv4Cache, Kv4Plan, LogProbs, kv4_append, kv4_attention, kv4_attention_scratch, kv4_plan, kv4_read,  # noqa: E402,F401
+                  logprobs)

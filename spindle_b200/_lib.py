@@ -63,6 +63,20 @@ class SgMoeEp(C.Structure):
                 ("recv_slots", C.c_uint64), ("recv", C.c_void_p * TP_MAX_RANKS), ("comm", C.c_void_p)]
 
 
+class SgKv4(C.Structure):
+    _fields_ = [("head_dim", C.c_uint32), ("n_kv_heads", C.c_uint32), ("page", C.c_uint32), ("n_blocks", C.c_uint32),
+                ("data", C.c_void_p)]
+
+
+class SgKv4Attn(C.Structure):
+    _fields_ = [("type", C.c_int32), ("n_heads", C.c_uint32), ("n_tok", C.c_uint64), ("n_req", C.c_uint64),
+                ("q", C.c_void_p), ("q_tok", C.c_uint64), ("q_head", C.c_uint64),
+                ("out", C.c_void_p), ("o_tok", C.c_uint64), ("o_head", C.c_uint64), ("lse", C.c_void_p),
+                ("cu", C.c_void_p), ("seq", C.c_void_p), ("tables", C.c_void_p),
+                ("ld_tables", C.c_uint64), ("width", C.c_uint64), ("scale", C.c_float), ("window", C.c_uint32),
+                ("max_new", C.c_uint64), ("scratch", C.c_void_p), ("scratch_bytes", C.c_uint64)]
+
+
 P, U64, I32 = C.c_void_p, C.c_uint64, C.c_int32
 
 # name -> (restype, argtypes); every function the header declares.
@@ -136,6 +150,14 @@ SIGNATURES = {
     "sg_pipe_recv": (I32, [P, U64, U64, P, P, P, P]),
     "sg_model_batch_scratch_bytes": (U64, [P, U64]),
     "sg_model_batch_prepare": (I32, [P, U64, P, U64, P]),
+    "sg_kv4_bytes": (U64, [C.POINTER(SgKv4)]),
+    "sg_kv4_plan": (I32, [C.c_uint32, C.c_uint32, U64, P, P, P, U64, U64, P, P, P, P, P, P, U64, P, P]),
+    "sg_kv4_append": (I32, [C.POINTER(SgKv4), I32, P, U64, U64, P, U64, U64, P, U64, P, P]),
+    "sg_kv4_read": (I32, [C.POINTER(SgKv4), I32, P, U64, P, P, P]),
+    "sg_kv4_attention_scratch_bytes": (U64, []),
+    "sg_kv4_attention_scratch_init": (I32, [P, U64, P]),
+    "sg_kv4_attention": (I32, [C.POINTER(SgKv4), C.POINTER(SgKv4Attn), P]),
+    "sg_logprobs": (I32, [I32, P, U64, U64, U64, P, P, P, P, U64, P, P, P]),
     "sg_forward_batch": (I32, [P, P, U64, P, P, P, U64, U64, P, U64, P, P]),
 }
 

@@ -14,6 +14,8 @@
 #include "gemv_tiled.cuh"
 #include "gemv_list.cuh"
 #include "kernels.cuh"
+#include "kv4.cuh"
+#include "logprobs.cuh"
 #include "moe.cuh"
 #include "decode.cuh"
 #include "gemv_float.cuh"
@@ -2391,6 +2393,158 @@ sg_status sg_forward_ep(const sg_model *m, const sg_moe_ep *eps, int32_t *d_stat
                         uint64_t scratch_bytes, float *d_hidden, float *d_logits, int64_t *d_token, void *stream) {
     if (!eps) return SG_ERR_INVALID;
     return forward_one(m, eps, d_state, d_kv, d_scratch, scratch_bytes, d_hidden, d_logits, d_token, stream);
+}
+
+}  // extern "C"
+
+// ---- paged 4-bit KV cache, token log probabilities ----------------------------
+
+namespace {
+
+bool page_ok(uint32_t page) { return page >= 16 && page <= 1024 && (page & (page - 1)) == 0; }
+uint32_t log2_of(uint32_t v) { return 31u - (uint32_t)__builtin_clz(v); }
+// element size of an activation type, 0: not one
+uint32_t act_bytes(int32_t type) { return type == SG_F32 ? 4 : type == SG_F16 || type == SG_BF16 ? 2 : 0; }
+
+sg_status check_kv4(const sg_kv4 *c, bool data) {
+    if (!c) return SG_ERR_INVALID;
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return SG_ERR_SHAPE;
+    if (!page_ok(c->page) || !c->n_kv_heads || c->n_kv_heads > 65535 || !c->n_blocks ||
+        (uint64_t)c->n_blocks * c->page >= 1ull << 31)
+        return SG_ERR_SHAPE;
+    if (!data) return SG_OK;
+    if (!c->data) return SG_ERR_INVALID;
+    return aligned(c->data, 16) ? SG_OK : SG_ERR_ALIGN;
+}
+
+Kv4Cache kv4_of(const sg_kv4 *c) { return {c->data, c->n_blocks, log2_of(c->page), c->n_kv_heads}; }
+
+}  // namespace
+
+extern "C" {
+
+uint64_t sg_kv4_bytes(const sg_kv4 *c) {
+    return check_kv4(c, false) ? 0 : (uint64_t)c->n_blocks * c->n_kv_heads * (c->page / 16) * 20 * c->head_dim;
+}
+
+sg_status sg_kv4_plan(uint32_t page, uint32_t n_blocks, uint64_t n_req, const int32_t *d_ctx, const int32_t *d_new,
+                      int32_t *d_tables, uint64_t ld_tables, uint64_t width, int32_t *d_ring, const int32_t *d_cursor,
+                      int32_t *d_cu, int32_t *d_seq, int32_t *d_pos, int32_t *d_slots, uint64_t max_tokens,
+                      int32_t *d_info, void *stream) {
+    if (!page_ok(page) || !n_blocks || (uint64_t)n_blocks * page >= 1ull << 31) return SG_ERR_SHAPE;
+    if (!d_ring || !d_cursor || !d_cu || !d_info || d_info == d_cursor || (max_tokens && (!d_pos || !d_slots)) ||
+        (n_req && (!d_ctx || !d_new || !d_tables || !d_seq)))
+        return SG_ERR_INVALID;
+    if (n_req >= 1ull << 31 || max_tokens >= 1ull << 31 || width >= 1ull << 31 || (n_req > 1 && ld_tables < width))
+        return SG_ERR_INVALID;
+    DevInfo *di;
+    if (sg_status st = dev_info(&di)) return st;
+    const Kv4PlanArgs a = {d_ctx, d_new, d_tables, ld_tables, d_ring, d_cursor, d_cu, d_seq, d_pos, d_slots, d_info,
+                           (uint32_t)n_req, (uint32_t)max_tokens, (uint32_t)width, log2_of(page), n_blocks};
+    const uint64_t want = (max_tokens + KV4_PLAN_THREADS - 1) / KV4_PLAN_THREADS;
+    const uint32_t grid = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(want, di->sms));
+    kv4_plan_kernel<<<grid, KV4_PLAN_THREADS, 0, (cudaStream_t)stream>>>(a);
+    CK(cudaGetLastError());
+    return SG_OK;
+}
+
+sg_status sg_kv4_append(const sg_kv4 *c, int32_t type, const void *d_k, uint64_t k_tok, uint64_t k_head, const void *d_v,
+                        uint64_t v_tok, uint64_t v_head, const int32_t *d_slots, uint64_t n_tok, int32_t *d_nonfinite,
+                        void *stream) {
+    if (sg_status st = check_kv4(c, true)) return st;
+    const uint32_t es = act_bytes(type);
+    if (!es) return SG_ERR_DTYPE;
+    if (n_tok == 0) return SG_OK;
+    if (!d_k || !d_v || !d_slots || n_tok >= 1ull << 31) return SG_ERR_INVALID;
+    if (!aligned(d_k, es) || !aligned(d_v, es)) return SG_ERR_ALIGN;
+    DevInfo *di;
+    if (sg_status st = dev_info(&di)) return st;
+    const uint64_t m = 16 / es - 1;
+    const bool vec = aligned(d_k, 16) && aligned(d_v, 16) && !((k_tok | k_head | v_tok | v_head) & m);
+    const Kv4RowArgs a = {kv4_of(c), d_k, d_v, k_tok, k_head, v_tok, v_head, nullptr, nullptr, d_slots, d_nonfinite,
+                          (uint32_t)n_tok};
+    const uint64_t lanes = n_tok * c->n_kv_heads * (c->head_dim / 32) * 8;
+    const uint32_t grid = (uint32_t)std::min<uint64_t>((lanes + KV4_ROW_THREADS - 1) / KV4_ROW_THREADS, (uint64_t)di->sms * 64);
+    kv4_append_kernel_for(type, c->head_dim, vec)<<<grid, KV4_ROW_THREADS, 0, (cudaStream_t)stream>>>(a);
+    CK(cudaGetLastError());
+    return SG_OK;
+}
+
+sg_status sg_kv4_read(const sg_kv4 *c, int32_t type, const int32_t *d_slots, uint64_t n_tok, void *d_k, void *d_v,
+                      void *stream) {
+    if (sg_status st = check_kv4(c, true)) return st;
+    if (!act_bytes(type)) return SG_ERR_DTYPE;
+    if (n_tok == 0) return SG_OK;
+    if (!d_k || !d_v || !d_slots || n_tok >= 1ull << 31) return SG_ERR_INVALID;
+    if (!aligned(d_k, 16) || !aligned(d_v, 16)) return SG_ERR_ALIGN;
+    DevInfo *di;
+    if (sg_status st = dev_info(&di)) return st;
+    const Kv4RowArgs a = {kv4_of(c), nullptr, nullptr, 0, 0, 0, 0, d_k, d_v, d_slots, nullptr, (uint32_t)n_tok};
+    const uint64_t lanes = n_tok * c->n_kv_heads * (c->head_dim / 32) * 8;
+    const uint32_t grid = (uint32_t)std::min<uint64_t>((lanes + KV4_ROW_THREADS - 1) / KV4_ROW_THREADS, (uint64_t)di->sms * 64);
+    kv4_read_kernel_for(type, c->head_dim)<<<grid, KV4_ROW_THREADS, 0, (cudaStream_t)stream>>>(a);
+    CK(cudaGetLastError());
+    return SG_OK;
+}
+
+uint64_t sg_kv4_attention_scratch_bytes(void) { return KV4_SCRATCH_BYTES; }
+
+sg_status sg_kv4_attention_scratch_init(void *d_scratch, uint64_t bytes, void *stream) {
+    if (!d_scratch || bytes < KV4_SCRATCH_BYTES) return SG_ERR_INVALID;
+    if (!aligned(d_scratch, 256)) return SG_ERR_ALIGN;
+    CK(cudaMemsetAsync(d_scratch, 0, KV4_SCRATCH_BYTES, (cudaStream_t)stream));
+    return SG_OK;
+}
+
+sg_status sg_kv4_attention(const sg_kv4 *c, const sg_kv4_attn *p, void *stream) {
+    if (sg_status st = check_kv4(c, true)) return st;
+    if (!p) return SG_ERR_INVALID;
+    const uint32_t es = act_bytes(p->type);
+    if (!es) return SG_ERR_DTYPE;
+    if (!p->n_heads || p->n_heads % c->n_kv_heads || p->n_heads > 65535) return SG_ERR_SHAPE;
+    if (p->n_tok == 0) return SG_OK;
+    if (!p->q || !p->out || !p->scratch || p->scratch_bytes < KV4_SCRATCH_BYTES || p->n_tok >= 1ull << 31 ||
+        p->n_req >= 1ull << 31 || !(p->scale - p->scale == 0.0f) ||
+        (p->n_req && (!p->cu || !p->seq || (p->width && !p->tables))))
+        return SG_ERR_INVALID;
+    if (p->width * c->page >= 1ull << 31 || p->width >= 1ull << 31 || (p->n_req > 1 && p->ld_tables < p->width))
+        return SG_ERR_INVALID;
+    if (!aligned(p->q, es) || !aligned(p->out, es) || !aligned(p->scratch, 256) || !aligned(p->lse, 4)) return SG_ERR_ALIGN;
+    DevInfo *di;
+    if (sg_status st = dev_info(&di)) return st;
+    Kv4AttnArgs a = {};
+    a.c = kv4_of(c);
+    a.q = p->q, a.out = p->out, a.lse = p->lse;
+    a.q_tok = p->q_tok, a.q_head = p->q_head, a.o_tok = p->o_tok, a.o_head = p->o_head;
+    a.cu = p->cu, a.seq = p->seq, a.tables = p->tables, a.ld_tables = p->ld_tables;
+    a.width = (uint32_t)p->width, a.n_req = (uint32_t)p->n_req, a.n_tok = (uint32_t)p->n_tok;
+    a.n_heads = p->n_heads, a.group = p->n_heads / c->n_kv_heads, a.window = p->window;
+    a.max_new = (uint32_t)(p->max_new && p->max_new < p->n_tok ? p->max_new : p->n_tok);
+    a.scale = p->scale == 0.0f ? 1.0f / sqrtf((float)c->head_dim) : p->scale;
+    a.scratch = (uint8_t *)p->scratch;
+    cudaError_t e = cudaSuccess;
+    sg_status st = kv4_attention_launch(a, p->type, c->head_dim, di->sms, (cudaStream_t)stream, &e);
+    return st == SG_ERR_CUDA ? cuda_fail(e, "kv4_attention") : st;
+}
+
+sg_status sg_logprobs(int32_t type, const void *d_logits, uint64_t ld, uint64_t rows, uint64_t vocab,
+                      const int32_t *d_tokens, float *d_logprob, float *d_entropy, int32_t *d_rank, uint64_t top,
+                      int32_t *d_top_ids, float *d_top_logprobs, void *stream) {
+    const uint32_t es = act_bytes(type);
+    if (!es) return SG_ERR_DTYPE;
+    if (!vocab || vocab > 1ull << 30 || top > SG_LOGPROBS_TOP_MAX || top > vocab) return SG_ERR_SHAPE;
+    if (rows == 0) return SG_OK;
+    if (!d_logits || !d_logprob || !d_entropy || !d_rank || (top && (!d_top_ids || !d_top_logprobs)) ||
+        rows >= 1ull << 31 || (rows > 1 && ld < vocab))
+        return SG_ERR_INVALID;
+    if (!aligned(d_logits, es)) return SG_ERR_ALIGN;
+    DevInfo *di;
+    if (sg_status st = dev_info(&di)) return st;
+    const LogprobsArgs a = {d_logits, ld, (uint32_t)rows, (uint32_t)vocab, (uint32_t)top, d_tokens,
+                            d_logprob, d_entropy, d_rank, d_top_ids, d_top_logprobs};
+    cudaError_t e = cudaSuccess;
+    sg_status st = logprobs_launch(a, type, di->sms, (cudaStream_t)stream, &e);
+    return st == SG_ERR_CUDA ? cuda_fail(e, "logprobs") : st;
 }
 
 }  // extern "C"

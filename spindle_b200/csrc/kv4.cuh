@@ -1,0 +1,92 @@
+// kv4.cuh — the paged KV cache held in 4 bits: layout, and the launch
+// interfaces of the plan, append, read and attention kernels.
+//
+// The cache is n_blocks blocks of `page` positions.  For one KV head a block is
+// page / 16 tiles of 16 positions, TILE = 20 * D bytes each, one after the
+// other; the heads of a block follow each other.  With D = head_dim and G =
+// D / 32 groups of 32 values (a value is m + s * c: c a code of 4 bits, s and m
+// f16), a tile holds
+//   K codes   [16 positions][D / 2 bytes]
+//   V codes   [8 pairs of positions][D bytes]
+//   K scales  [8 pairs][G][2] f16        K minima  [16 positions][G] f16
+//   V scales  [8 pairs][G][2] f16        V minima  [8 pairs][G][2] f16
+// so that one bulk copy brings everything a warp needs of 16 positions, and each
+// lane's part of an m16n8k16 operand is whole aligned words:
+//   K: the word kv4_word(j, g, 4) of a position holds the values d = 32 g + 8 j + n
+//      in its nibbles n = 0..7 (lane j of a quad has all groups side by side);
+//   V: the word kv4_word(j, g, 8) of a pair holds d = 32 g + 4 j + n in the
+//      nibbles n = 0..3 of its low half for the even position and of its high
+//      half for the odd one (the two halves of an f16x2 register after a mask).
+#pragma once
+
+#include "common.cuh"
+
+namespace sg {
+
+// Word index of (lane part j of J, group g) inside a position's or pair's codes;
+// four groups of one j are 16 bytes.
+__host__ __device__ constexpr uint32_t kv4_word(uint32_t j, uint32_t g, uint32_t J, uint32_t G) {
+    return G < 4 ? j * G + g : ((g / 4) * J + j) * 4 + g % 4;
+}
+
+template <int D>
+struct Kv4Tile {
+    static constexpr uint32_t G = D / 32;
+    static constexpr uint32_t KROW = D / 2, VROW = D;           // bytes of a position's K codes, of a pair's V codes
+    static constexpr uint32_t VC = 8 * D, KS = 16 * D, KM = 17 * D, VS = 18 * D, VM = 19 * D, BYTES = 20 * D;
+};
+
+struct Kv4Cache {
+    uint8_t *data;
+    uint32_t n_blocks, page_shift;  // page = 1 << page_shift positions
+    uint32_t heads;
+};
+
+struct Kv4PlanArgs {
+    const int32_t *ctx, *add;
+    int32_t *tables;
+    uint64_t ld_tables;
+    int32_t *ring;
+    const int32_t *cursor;
+    int32_t *cu, *seq, *pos, *slots, *info;
+    uint32_t n_req, max_tok, width, page_shift, n_blocks;
+};
+
+struct Kv4RowArgs {
+    Kv4Cache c;
+    const void *k, *v;                 // append: the rows
+    uint64_t k_tok, k_head, v_tok, v_head;  // strides in elements
+    void *k_out, *v_out;               // read: [n_tok][heads][D]
+    const int32_t *slots;
+    int32_t *nonfinite;
+    uint32_t n_tok;
+};
+
+struct Kv4AttnArgs {
+    Kv4Cache c;
+    const void *q;
+    void *out;
+    float *lse;
+    uint64_t q_tok, q_head, o_tok, o_head;  // strides in elements
+    const int32_t *cu, *seq, *tables;
+    uint64_t ld_tables;
+    uint32_t width, n_req, n_tok, n_heads, group, window, max_new;
+    float scale;
+    uint8_t *scratch;
+};
+
+constexpr int KV4_PLAN_THREADS = 1024;
+__global__ void kv4_plan_kernel(const __grid_constant__ Kv4PlanArgs a);
+
+typedef void (*kv4_row_fn)(const Kv4RowArgs);
+// type: SG_F32, SG_F16 or SG_BF16; vec: rows and strides allow 16-byte loads
+kv4_row_fn kv4_append_kernel_for(int32_t type, uint32_t d, bool vec);
+kv4_row_fn kv4_read_kernel_for(int32_t type, uint32_t d);
+constexpr int KV4_ROW_THREADS = 256;
+
+// Attention scratch: partial results of requests whose positions are spread over
+// several CTAs, and their arrival counters (zero between calls).
+constexpr uint64_t KV4_SCRATCH_BYTES = 8ull << 20;
+sg_status kv4_attention_launch(const Kv4AttnArgs &a, int32_t type, uint32_t d, int sms, cudaStream_t s, cudaError_t *err);
+
+}  // namespace sg

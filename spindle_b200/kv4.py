@@ -1,0 +1,236 @@
+"""Paged KV cache held in 4 bits, for serving many requests: block tables and
+slot maps from request lengths (kv4_plan), rows quantized into the cache
+(kv4_append) and read back (kv4_read), grouped-query attention over it
+(kv4_attention), and token log probabilities (logprobs), through the C ABI
+(sg_kv4_*, sg_logprobs).  The reference keeps one f16 cache per chat
+(smollm_chat.rs:2924-2972); nothing here changes that path (Decoder).
+
+One serving step: plan, then per layer append and attend, then the LM head and
+logprobs.  All lengths, tables and slots stay on the device."""
+import contextlib
+import ctypes as C
+
+import torch
+
+from . import _lib
+from ._lib import SgKv4, SgKv4Attn
+
+LOGPROBS_TOP_MAX = 64
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+
+
+def _s(stream):
+    return (stream if stream is not None else torch.cuda.current_stream()).cuda_stream
+
+
+def _on(stream):
+    """What a call allocates belongs to the stream that it runs on."""
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+
+
+def _type(t, what):
+    try:
+        return _TYPES[t.dtype]
+    except KeyError:
+        raise TypeError("%s must be float32, float16 or bfloat16" % what) from None
+
+
+def _i32(t, what, shape=None):
+    if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
+        raise TypeError("%s must be a contiguous int32 CUDA tensor" % what)
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError("%s must have the shape %s" % (what, shape))
+    return t.data_ptr()
+
+
+class Kv4Cache:
+    """n_blocks blocks of `page` positions of n_kv_heads x head_dim K and V
+    values in 4 bits (one per layer; 20 bytes per 32 values).  data:
+    the device bytes (a uint8 CUDA tensor of Kv4Cache.bytes_for), allocated if None.
+    nonfinite counts the groups of 32 appended values that had an infinity or a NaN."""
+
+    def __init__(self, n_blocks, n_kv_heads, head_dim, page=64, device=None, data=None):
+        self.n_blocks, self.n_kv_heads, self.head_dim, self.page = n_blocks, n_kv_heads, head_dim, page
+        need = self.bytes_for(n_blocks, n_kv_heads, head_dim, page)
+        if data is None:
+            data = torch.zeros(need, dtype=torch.uint8, device=device or "cuda")
+        if data.dtype != torch.uint8 or not data.is_cuda or not data.is_contiguous() or data.numel() < need:
+            raise ValueError("data must be a contiguous uint8 CUDA tensor of %d bytes" % need)
+        self.data = data
+        self.nonfinite = torch.zeros(1, dtype=torch.int32, device=data.device)
+        self.desc = SgKv4(head_dim, n_kv_heads, page, n_blocks, data.data_ptr())
+        self._c = C.byref(self.desc)
+
+    @staticmethod
+    def bytes_for(n_blocks, n_kv_heads, head_dim, page):
+        n = _lib.load().sg_kv4_bytes(C.byref(SgKv4(head_dim, n_kv_heads, page, n_blocks, None)))
+        if not n:
+            raise _lib.SgError(3, "kv4_bytes")
+        return n
+
+
+class Kv4Plan:
+    """What kv4_plan writes, for up to n_req requests and max_tokens new
+    positions a step: cu [n_req + 1], seq [n_req], pos and slots [max_tokens],
+    and info [4] (the next step's cursor, the sum of the new positions, the
+    blocks that were wanted and not there).  It also keeps a ring of all blocks,
+    free to begin with, and the cursor, for callers without their own."""
+
+    def __init__(self, n_req, max_tokens, page, n_blocks, device="cuda"):
+        new = lambda n: torch.empty(n, dtype=torch.int32, device=device)  # noqa: E731
+        self.n_req, self.max_tokens, self.page, self.n_blocks = n_req, max_tokens, page, n_blocks
+        self.cu, self.seq, self.pos, self.slots = new(n_req + 1), new(n_req), new(max_tokens), new(max_tokens)
+        self.ring = torch.arange(n_blocks, dtype=torch.int32, device=device)
+        self._infos = [torch.tensor([0, n_blocks, 0, 0], dtype=torch.int32, device=device) for _ in range(2)]
+        self._turn = 0
+        self._out = (self.cu.data_ptr(), self.seq.data_ptr(), self.pos.data_ptr(), self.slots.data_ptr())
+
+    @property
+    def info(self):
+        return self._infos[self._turn]
+
+
+def kv4_plan(plan, ctx, new, tables, ring=None, cursor=None, stream=None):
+    """Block tables and slot maps of one step (sg_kv4_plan): ctx and new int32
+    [n_req] (positions held, positions to come; new < 0: the request ends), tables
+    int32 [n_req, width], updated in place.  ring and cursor: the free blocks
+    (int32 [n_blocks] and [2 or more]); None: the plan's own, carried from call to
+    call.  Fills and returns plan."""
+    n = ctx.numel()
+    if n != plan.n_req:
+        raise ValueError("the plan is made for %d requests" % plan.n_req)
+    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != n or (tables.numel() and tables.stride(1) != 1):
+        raise ValueError("tables must be int32 [n_req, width] with contiguous rows")
+    if (ring is None) != (cursor is None):
+        raise ValueError("ring and cursor come together")
+    own = cursor is None
+    if own:
+        ring, cursor = plan.ring, plan.info
+    elif ring.numel() != plan.n_blocks or cursor.numel() < 2:
+        raise ValueError("ring must have n_blocks entries and cursor two")
+    turn = plan._turn ^ 1
+    info = plan._infos[turn]
+    cu, seq, pos, slots = plan._out
+    st = _lib.load().sg_kv4_plan(plan.page, plan.n_blocks, n, _i32(ctx, "ctx"), _i32(new, "new", (n,)), tables.data_ptr(),
+                                 tables.stride(0), tables.shape[1], _i32(ring, "ring"), _i32(cursor, "cursor"), cu, seq, pos,
+                                 slots, plan.max_tokens, info.data_ptr(), _s(stream))
+    if st:
+        _lib.check(st, "kv4_plan")
+    plan._turn = turn
+    return plan
+
+
+def _rows(cache, t, what):
+    if t.dim() != 3 or t.shape[1] != cache.n_kv_heads or t.shape[2] != cache.head_dim or t.stride(2) != 1:
+        raise ValueError("%s must be [n_tok, %d, %d] with contiguous rows" % (what, cache.n_kv_heads, cache.head_dim))
+
+
+def kv4_append(cache, k, v, slots, stream=None):
+    """Quantizes the rows k, v [n_tok, n_kv_heads, head_dim] (float32, float16 or
+    bfloat16, any token and head strides) into their slots (int32 [n_tok], as
+    kv4_plan makes them; negative: the row is left out)."""
+    _rows(cache, k, "k")
+    _rows(cache, v, "v")
+    if v.dtype != k.dtype or v.shape[0] != k.shape[0]:
+        raise ValueError("k and v must have one type and one number of rows")
+    n = k.shape[0]
+    st = _lib.load().sg_kv4_append(cache._c, _type(k, "k"), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                                   v.stride(1), _i32(slots, "slots", (n,)), n, cache.nonfinite.data_ptr(), _s(stream))
+    if st:
+        _lib.check(st, "kv4_append")
+
+
+def kv4_read(cache, slots, out=None, dtype=torch.float16, stream=None):
+    """The values that the cache holds at the given slots (int32 [n_tok]): (k, v),
+    [n_tok, n_kv_heads, head_dim] of dtype each, or into out = (k, v)."""
+    n = slots.numel()
+    if out is None:
+        with _on(stream):
+            out = tuple(torch.empty(n, cache.n_kv_heads, cache.head_dim, dtype=dtype, device=slots.device)
+                        for _ in range(2))
+    k, v = out
+    for t in out:
+        _rows(cache, t, "out")
+        if t.shape[0] != n or t.dtype != k.dtype or not t.is_contiguous():
+            raise ValueError("out must be two contiguous tensors of one type with a row per slot")
+    st = _lib.load().sg_kv4_read(cache._c, _type(k, "out"), _i32(slots, "slots"), n, k.data_ptr(), v.data_ptr(), _s(stream))
+    if st:
+        _lib.check(st, "kv4_read")
+    return out
+
+
+def kv4_attention_scratch(device="cuda", stream=None):
+    """Scratch of kv4_attention: kept by the caller, one for calls that may overlap on the GPU."""
+    L = _lib.load()
+    with _on(stream):
+        t = torch.empty(L.sg_kv4_attention_scratch_bytes(), dtype=torch.uint8, device=device)
+    _lib.check(L.sg_kv4_attention_scratch_init(t.data_ptr(), t.numel(), _s(stream)), "kv4_attention_scratch_init")
+    return t
+
+
+def kv4_attention(cache, q, cu, seq, tables, scale=None, window=0, max_new=0, out=None, lse=None, scratch=None, stream=None):
+    """Grouped-query attention of new tokens over the cache (sg_kv4_attention): q
+    [n_tok, n_heads, head_dim] (float32, float16 or bfloat16), cu [n_req + 1] and
+    seq [n_req] int32 as kv4_plan makes them, tables int32 [n_req, width].  Token t
+    of a request sees the positions up to its own, the last `window` of them if
+    window > 0.  max_new: an upper bound of a request's new tokens, if the caller
+    knows one.  lse: optional float32 [n_tok, n_heads] to fill with the log of the
+    softmax's sum.  Returns out, [n_tok, n_heads, head_dim] of q's type."""
+    n = seq.numel()
+    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.stride(2) != 1:
+        raise ValueError("q must be [n_tok, n_heads, %d] with contiguous rows" % cache.head_dim)
+    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != n or (tables.numel() and tables.stride(1) != 1):
+        raise ValueError("tables must be int32 [n_req, width] with contiguous rows")
+    if out is None:
+        with _on(stream):
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        raise ValueError("out must have q's shape and type, and contiguous rows")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()):
+        raise ValueError("lse must be a contiguous float32 [n_tok, n_heads]")
+    if scratch is None:
+        scratch = kv4_attention_scratch(q.device, stream)
+    a = SgKv4Attn(_type(q, "q"), q.shape[1], q.shape[0], n, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(),
+                  out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), _i32(cu, "cu", (n + 1,)),
+                  _i32(seq, "seq"), tables.data_ptr(), tables.stride(0), tables.shape[1], 0.0 if scale is None else scale,
+                  window, max_new, scratch.data_ptr(), scratch.numel())
+    st = _lib.load().sg_kv4_attention(cache._c, C.byref(a), _s(stream))
+    if st:
+        _lib.check(st, "kv4_attention")
+    return out
+
+
+class LogProbs:
+    """What logprobs returns, for `rows` rows: logprob and entropy float32 [rows],
+    rank int32 [rows], top_ids int32 and top_logprobs float32 [rows, top]."""
+
+    def __init__(self, rows, top=0, device="cuda"):
+        f = lambda *n: torch.empty(*n, dtype=torch.float32, device=device)  # noqa: E731
+        i = lambda *n: torch.empty(*n, dtype=torch.int32, device=device)  # noqa: E731
+        self.rows, self.top = rows, top
+        self.logprob, self.entropy, self.rank = f(rows), f(rows), i(rows)
+        self.top_ids, self.top_logprobs = i(rows, top), f(rows, top)
+        self._p = [t.data_ptr() for t in (self.logprob, self.entropy, self.rank, self.top_ids, self.top_logprobs)]
+
+
+def logprobs(logits, tokens=None, top=0, out=None, stream=None):
+    """Log probabilities of the given tokens under softmax(logits) (sg_logprobs):
+    logits [rows, vocab] float32, float16 or bfloat16 with contiguous rows, tokens
+    int32 [rows] or None, top up to 64 alternatives.  Returns a LogProbs (out, if
+    given): the log probability and the rank (0: the likeliest) of each given
+    token, the entropy in nats, and the `top` likeliest tokens."""
+    if logits.dim() != 2 or (logits.numel() and logits.stride(1) != 1) or not logits.is_cuda:
+        raise ValueError("logits must be a CUDA tensor [rows, vocab] with contiguous rows")
+    rows, vocab = logits.shape
+    if out is None:
+        with _on(stream):
+            out = LogProbs(rows, top, logits.device)
+    elif out.rows != rows or out.top != top:
+        raise ValueError("out is made for %d rows and top %d" % (out.rows, out.top))
+    lp, ent, rank, ids, tops = out._p
+    st = _lib.load().sg_logprobs(_type(logits, "logits"), logits.data_ptr(), logits.stride(0), rows, vocab,
+                                 None if tokens is None else _i32(tokens, "tokens", (rows,)), lp, ent, rank, top, ids, tops,
+                                 _s(stream))
+    if st:
+        _lib.check(st, "logprobs")
+    return out
