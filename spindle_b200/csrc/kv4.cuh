@@ -73,6 +73,8 @@ struct Kv4AttnArgs {
     uint32_t width, n_req, n_tok, n_heads, group, window, max_new;
     float scale;
     uint8_t *scratch;
+    bool vec_out;  // output rows allow 16-byte stores
+    bool last;     // this launch's requests are the last ones
 };
 
 constexpr int KV4_PLAN_THREADS = 1024;
