@@ -2522,6 +2522,8 @@ sg_status sg_kv4_attention(const sg_kv4 *c, const sg_kv4_attn *p, void *stream) 
     a.max_new = (uint32_t)(p->max_new && p->max_new < p->n_tok ? p->max_new : p->n_tok);
     a.scale = p->scale == 0.0f ? 1.0f / sqrtf((float)c->head_dim) : p->scale;
     a.scratch = (uint8_t *)p->scratch;
+    a.block_bytes = (uint64_t)c->n_kv_heads * (c->page / 16) * 20 * c->head_dim;
+    a.vec_q = aligned(p->q, 16) && !((p->q_tok | p->q_head) & (16 / es - 1));
     a.vec_out = aligned(p->out, 16) && !((p->o_tok | p->o_head) & (16 / es - 1));
     cudaError_t e = cudaSuccess;
     sg_status st = kv4_attention_launch(a, p->type, c->head_dim, di->sms, (cudaStream_t)stream, &e);

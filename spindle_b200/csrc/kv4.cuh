@@ -73,7 +73,8 @@ struct Kv4AttnArgs {
     uint32_t width, n_req, n_tok, n_heads, group, window, max_new;
     float scale;
     uint8_t *scratch;
-    bool vec_out;  // output rows allow 16-byte stores
+    uint64_t block_bytes;  // of one block, all heads
+    bool vec_q, vec_out;  // the rows allow 16-byte accesses
     bool last;     // this launch's requests are the last ones
 };
 

@@ -19,9 +19,10 @@
 //   q.k   = sum_g s_g (q_g . c_g) + sum_g m_g sum(q_g)
 //   sum_t p_t v_t = sum_t (p_t s_tg) c_t + sum_t p_t m_tg
 // where the scales s_g are applied in f32 to the small results on the K side and
-// to p on the V side.  The sixteen rows of an operand hold the eight query rows
-// twice: the f16 rounding of a number above, the f16 rounding of what that left
-// below (about 22 bits together), for p, p s and an f32 q.  A 16-bit q is exact
+// to p on the V side.  The codes are the 16-row operand (16 positions for the
+// scores, 16 values of a position for the sums), the eight query rows the 8-wide
+// one; p, p s and an f32 q go in as the f16 rounding and, in a second product,
+// the rounding of what that left (about 22 bits together).  A 16-bit q is exact
 // after scaling by a power of two.  So every product is as good as one in f32.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -67,10 +68,48 @@ __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
     return d;
 }
 
+__device__ __forceinline__ uint32_t fma_h2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+// Any half of a larger than b's: both hold f16 numbers that are not negative.
+__device__ __forceinline__ bool any_gt_h2(uint32_t a, uint32_t b) { return __vmaxu2(a, b) != b; }
+
+// d = a b, d += a b
+__device__ __forceinline__ void mma16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void mma8_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(b0), "f"(0.0f));
+}
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// An 8 x 8 matrix of 16-bit numbers, a row per four lanes, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+    return d;
+}
+
+// Four neighbouring values of an output row.
+template <typename T>
+__device__ __forceinline__ void put4(T *out, float x, float y, float z, float w, bool vec) {
+    alignas(16) T v[4] = {Act<T>::put(x), Act<T>::put(y), Act<T>::put(z), Act<T>::put(w)};
+    if (vec) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<const uint4 *>(v);
+        else *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<const uint2 *>(v);
+    } else {
+        out[0] = v[0], out[1] = v[1], out[2] = v[2], out[3] = v[3];
+    }
 }
 
 // N words of shared memory (8- or 16-byte aligned).
@@ -102,9 +141,11 @@ __device__ __forceinline__ void lds_codes(uint32_t (&w)[G], const uint8_t *row, 
 }
 
 constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
-constexpr float P_SHIFT = 10.0f;  // weights are held as 2^10 p: small ones keep their bits in f16
+// Weights are held as 2^P_SHIFT p with p below 2^LAG; V scales are brought below 2^5, so that a product
+// stays inside f16's range above and keeps 30 bits below its largest.
+constexpr float P_SHIFT = 2.0f, LAG = 8.0f;
 constexpr int ROWS = 8;
-constexpr uint32_t MAX_REQ = 2048;  // requests of one launch (their prefix sums are in shared memory)
+constexpr uint32_t MAX_REQ = 1024;  // requests of one launch (their steps are in shared memory)
 constexpr uint32_t MAX_CTAS = 320;
 
 template <int D>
@@ -117,39 +158,39 @@ struct Cfg {
     static constexpr uint32_t STAGE_BYTES = TILES * Kv4Tile<D>::BYTES;
     static constexpr uint32_t PART_BYTES = ROWS * D * 4 + 2 * ROWS * 4;  // rows, m, l
     static constexpr uint32_t RING = WARPS * STAGES * STAGE_BYTES;
-    static constexpr uint32_t SMEM = RING + WARPS * PART_BYTES + (MAX_REQ + 1) * 8 + WARPS * STAGES * 8 + 1024;
+    static constexpr uint32_t SMEM = RING + WARPS * PART_BYTES + (MAX_REQ + 1) * 8 + MAX_REQ * 16 + WARPS * STAGES * 8 + 1024 + (MAX_CTAS + 2) * ROWS * 4;
     static_assert(STAGES * STAGE_BYTES >= PART_BYTES, "a warp's last partial result lies in its ring");
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 constexpr uint32_t PART_MAX = Cfg<256>::PART_BYTES;
 static_assert(4096 + (uint64_t)MAX_CTAS * 2 * PART_MAX <= KV4_SCRATCH_BYTES, "scratch");
 
-// The steps of one request, the same for each of its heads and row tiles.
+// One request: its steps are the same for each of its heads and row tiles.
 struct Req {
-    int32_t tok0, nq, seq;      // first packed token, new tokens, positions
-    uint32_t s0, steps, tiles;  // first step, steps (at least one where there are rows), row tiles
+    int32_t tok0, nq, seq;  // first packed token, new tokens, positions (as given: seq - nq is the first new one's place)
+    uint32_t s0;            // first step
 };
 
 template <int STEP>
-__device__ __forceinline__ Req req_of(const Kv4AttnArgs &a, uint32_t i) {
+__device__ __forceinline__ Req req_of(const Kv4AttnArgs &a, uint32_t i, uint32_t &steps) {
     Req r;
     r.tok0 = max(a.cu[i], 0);
     r.nq = max(min(a.cu[i + 1], (int32_t)a.n_tok) - r.tok0, 0);
+    r.seq = max(a.seq[i], 0);
     const int64_t cap = (int64_t)a.width << a.c.page_shift;
-    const int32_t seq = max(a.seq[i], 0);
-    r.seq = seq < cap ? seq : (int32_t)cap;
+    const int32_t end = r.seq < cap ? r.seq : (int32_t)cap;
     int32_t lo = 0;
-    if (a.window && seq - r.nq + 1 > (int64_t)a.window) lo = seq - r.nq + 1 - (int32_t)a.window;
-    r.s0 = min(lo, r.seq) / STEP;
-    const uint32_t s1 = (r.seq + STEP - 1) / STEP;
-    r.steps = r.nq ? max(1u, s1 - min(s1, r.s0)) : 0;
-    r.tiles = (uint32_t)(((uint64_t)r.nq * a.group + ROWS - 1) / ROWS);
+    if (a.window && r.seq - r.nq + 1 > (int64_t)a.window) lo = r.seq - r.nq + 1 - (int32_t)a.window;
+    const uint32_t s1 = (end + STEP - 1) / STEP;
+    r.s0 = min((uint32_t)lo / STEP, s1);
+    steps = r.nq ? max(1u, s1 - r.s0) : 0;  // at least one where there are rows to write
     return r;
 }
 
 struct Seg {
     Req r;
-    uint32_t req, head, tile;
+    int32_t end;  // positions that the table has room for
+    uint32_t req, head, tile, steps;
     uint64_t begin;  // its first step among all steps
 };
 
@@ -166,10 +207,12 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
     uint8_t *ring_all = smem;
     float *first_all = reinterpret_cast<float *>(smem + C::RING);
     uint64_t *pre = reinterpret_cast<uint64_t *>(smem + C::RING + WARPS * C::PART_BYTES);  // [n_req + 1] steps before each request
-    uint64_t *bars = pre + MAX_REQ + 1;
+    Req *reqs = reinterpret_cast<Req *>(pre + MAX_REQ + 1);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(reqs + MAX_REQ);
     uint64_t *seg_begin = bars + WARPS * STAGES;                      // [2 * WARPS] the partials' segments, ~0: none
     uint64_t *scan_s = seg_begin + 2 * WARPS;                         // [WARPS + 1]
     uint32_t *flag_s = reinterpret_cast<uint32_t *>(scan_s + WARPS + 1);
+    float *weight_s = reinterpret_cast<float *>(flag_s + 2), *ml_s = weight_s + MAX_CTAS * ROWS;  // of the joins
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, quad = lane & 3;
 
     if (lane == 0)
@@ -177,13 +220,17 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
     fence_mbar_init();
     if (tid < 2 * WARPS) seg_begin[tid] = ~0ull;
 
+    auto tiles_of = [&](const Req &r) { return ((uint32_t)r.nq * a.group + ROWS - 1) / ROWS; };
+
     // steps before each request
     uint64_t total = 0;
     for (uint32_t r0 = 0; r0 < a.n_req; r0 += WARPS * 32) {
         uint64_t v = 0;
         if (r0 + tid < a.n_req) {
-            const Req r = req_of<STEP>(a, r0 + tid);
-            v = (uint64_t)r.steps * r.tiles * a.c.heads;
+            uint32_t steps;
+            const Req r = req_of<STEP>(a, r0 + tid, steps);
+            reqs[r0 + tid] = r;
+            v = (uint64_t)steps * tiles_of(r) * a.c.heads;
         }
         uint64_t inc = v;
 #pragma unroll
@@ -235,178 +282,205 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
         }
         Seg s;
         s.req = x;
-        s.r = req_of<STEP>(a, x);
-        const uint64_t rem = idx - pre[x], k = rem / s.r.steps;
-        s.head = (uint32_t)(k / s.r.tiles);
-        s.tile = (uint32_t)(k % s.r.tiles);
-        s.begin = pre[x] + k * s.r.steps;
+        s.r = reqs[x];
+        const uint32_t tiles = tiles_of(s.r);
+        const uint64_t rem = idx - pre[x], all = pre[x + 1] - pre[x];
+        s.end = (int32_t)min((int64_t)s.r.seq, (int64_t)a.width << a.c.page_shift);
+        s.steps = max(1u, (uint32_t)(s.end + STEP - 1) / STEP - s.r.s0);
+        uint64_t k;
+        if (all >> 32) k = rem / s.steps;
+        else k = (uint32_t)rem / s.steps;
+        s.head = tiles == 1 ? (uint32_t)k : (uint32_t)(k / tiles);
+        s.tile = (uint32_t)k - s.head * tiles;
+        s.begin = pre[x] + k * s.steps;
         return s;
     };
 
-    // ---- the copies: one step at a time, the table entries read a step ahead ----
-    uint64_t p_idx = w0, p_end = w0;
-    const int32_t *p_row = nullptr;
-    uint32_t p_head = 0, p_step = 0;
-    int32_t p_seq = 0, p_blk[TILES];
+    // ---- the copies: a step at a time, the table entries of 32 pages in the lanes ----
+    const uint32_t n = (uint32_t)(w1 - w0);
+    uint32_t p_i = 0, p_end = 0, p_t = 0, p_page = 0, p_req = 0, p_head = 0;
+    int32_t p_blk = -1, p_seq = 0;
     bool dead = false;  // a wait ran out: no further copies
-    auto fetch = [&]() {
-        if (p_idx >= w1) return;
-        if (p_idx >= p_end) {
-            const Seg s = seg_at(p_idx);
-            p_end = s.begin + s.r.steps;
-            p_row = a.tables + (uint64_t)s.req * a.ld_tables;
-            p_head = s.head;
-            p_step = s.r.s0 + (uint32_t)(p_idx - s.begin);
-            p_seq = s.r.seq;
-        }
-#pragma unroll
-        for (int i = 0; i < TILES; i++) {
-            const uint32_t t = p_step * STEP + i * 16;
-            p_blk[i] = (int32_t)t < p_seq ? __ldg(p_row + (t >> a.c.page_shift)) : -1;
-        }
+    auto pages = [&]() {
+        p_page = p_t >> a.c.page_shift;
+        const uint64_t page = (uint64_t)p_page + lane;
+        p_blk = (int64_t)(page << a.c.page_shift) < p_seq ? __ldg(a.tables + (uint64_t)p_req * a.ld_tables + page) : -1;
     };
-    // returns a bit per tile that is there
+    // copies the next step into a stage; returns a bit per tile that is there
     auto issue = [&](uint32_t stage) -> uint32_t {
-        if (p_idx >= w1) return 0;
+        if (p_i >= n) return 0;
+        if (p_i == p_end) {
+            const Seg s = seg_at(w0 + p_i);
+            p_end = (uint32_t)min((uint64_t)n, s.begin + s.steps - w0);
+            p_req = s.req, p_head = s.head, p_seq = s.end;
+            p_t = (s.r.s0 + (uint32_t)(w0 + p_i - s.begin)) * STEP;
+            pages();
+        }
+        uint8_t *dst = ring + stage * C::STAGE_BYTES;
         uint32_t there = 0;
-#pragma unroll
-        for (int i = 0; i < TILES; i++) there |= ((uint32_t)p_blk[i] < a.c.n_blocks) << i;
-        if (lane == 0 && !dead) {
-            mbar_arrive_expect_tx(&bar[stage], __popc(there) * L::BYTES);
-            uint8_t *dst = ring + stage * C::STAGE_BYTES;
+        const uint32_t shift = a.c.page_shift;
+        const uint64_t head_off = ((uint64_t)p_head << (shift - 4)) * L::BYTES;
+        if ((1u << shift) >= STEP) {  // the step lies in one page
+            if ((p_t >> shift) - p_page >= 32) pages();
+            const uint32_t blk = (uint32_t)__shfl_sync(~0u, p_blk, (p_t >> shift) - p_page);
+            there = blk < a.c.n_blocks ? (1u << TILES) - 1 : 0;
+            if (lane == 0 && !dead) {
+                mbar_arrive_expect_tx(&bar[stage], there ? C::STAGE_BYTES : 0);
+                if (there)
+                    bulk_g2s(dst, a.c.data + blk * a.block_bytes + head_off + ((p_t & ((1u << shift) - 1)) >> 4) * L::BYTES, C::STAGE_BYTES,
+                             &bar[stage]);
+            }
+        } else {  // a page per tile
+            uint32_t blk[TILES];
 #pragma unroll
             for (int i = 0; i < TILES; i++) {
-                if (!(there >> i & 1)) continue;
-                const uint32_t t = p_step * STEP + i * 16, at = (t & ((1u << a.c.page_shift) - 1)) >> 4;
-                const uint8_t *src = a.c.data + ((((uint64_t)p_blk[i] * a.c.heads + p_head) << (a.c.page_shift - 4)) + at) * (uint64_t)L::BYTES;
-                bulk_g2s(dst + i * L::BYTES, src, L::BYTES, &bar[stage]);
+                if ((p_t >> 4) + i - p_page >= 32) {
+                    p_t += 16 * i;
+                    pages();
+                    p_t -= 16 * i;
+                }
+                blk[i] = (uint32_t)__shfl_sync(~0u, p_blk, (p_t >> 4) + i - p_page);
+                there |= (blk[i] < a.c.n_blocks) << i;
+            }
+            if (lane == 0 && !dead) {
+                mbar_arrive_expect_tx(&bar[stage], __popc(there) * L::BYTES);
+#pragma unroll
+                for (int i = 0; i < TILES; i++)
+                    if (there >> i & 1) bulk_g2s(dst + i * L::BYTES, a.c.data + blk[i] * a.block_bytes + head_off, L::BYTES, &bar[stage]);
             }
         }
-        p_idx++;
-        p_step++;
+        p_i++;
+        p_t += STEP;
         return there;
     };
-    uint32_t there[STAGES];
+    uint32_t there = 0;  // the bits of the steps in the ring, the next one's lowest
 #pragma unroll
-    for (int s = 0; s < STAGES; s++) {
-        fetch();
-        there[s] = issue(s);
-    }
-    fetch();
+    for (int s = 0; s < STAGES; s++) there |= issue(s) << (s * TILES);
 
     // ---- the steps ----
-    uint32_t qa[2 * G][QR], qs[G == 8 ? 2 : 1];
-    float o[4 * G][4], om[4];
-    float m = -INFINITY, l = 0.0f, cs = 0.0f;
-    int32_t lo_t = 0, hi_t = 0, full_lo = 0, full_hi = 0;
-    int32_t kexp = 15;        // of group lane % G: V scales are multiplied by 2^kexp
-    float vlim = -1.0f;       // and are at most this
-    uint32_t kmul[G];         // f16x2 of each group's 2^kexp
-    uint64_t seg_end = w0;
-    Seg seg;
-    uint32_t phase = 0, stage = 0;
+    // Operands: scores are K codes (16 positions) times query rows (8), sums V codes (16 values) times weights
+    // (8 rows), so that a lane of quad `quad` has rows 2 quad and 2 quad + 1 of every result.
+    uint32_t qb[2 * G][QR], qs[G == 8 ? 2 : 1];
+    float o[2 * G][4], om[4];
+    float m[2], l[2], cs[2];
+    int32_t lo_t[2], hi_t[2], full_lo = 0, full_hi = 0;  // positions [lo, hi) that a row sees; that all rows see
+    int32_t kexp = 15;   // of group lane % G: V scales are multiplied by 2^kexp
+    uint32_t vlim2 = 0;  // and are at most this (f16x2)
+    uint32_t kmul[G];    // f16x2 of each group's 2^kexp
+    uint32_t c_end = 0, phase = 0, stage = 0;
+    int32_t t0 = 0, held_end = 0;  // the step's first position, the positions held
+    const uint32_t half_sel = gid & 1 ? 0x7632u : 0x5410u;
 
-    // the rows' sums in values: lane holds row gid, d = 32 g + 8 quad + 0..7 of each group in r[g]
-    auto rows_of = [&](float (&r)[G][8]) {
+    // the sums as values: rows 2 quad + i, d = 32 g + 4 gid + n in r[g][i][n]
+    auto rows_of = [&](float (&r)[G][2][4]) {
 #pragma unroll
         for (int g = 0; g < G; g++) {
             const int k = __shfl_sync(~0u, kexp, g);
-            const float f = __uint_as_float((uint32_t)(127 + 24 - k) << 23);
-            const int src = (lane & 28) | (g >> 1);
-            const float mn = (g & 1) ? __shfl_sync(~0u, om[1] + om[3], src) : __shfl_sync(~0u, om[0] + om[2], src);
+            const float f = __uint_as_float((uint32_t)(127 + 24 - k) << 23), f16 = f * 0.0625f;  // odd nibbles came in 16-fold
 #pragma unroll
-            for (int n = 0; n < 4; n++) {
-                const float fn = n & 1 ? f * 0.0625f : f;
-                r[g][n] = fmaf(o[4 * g + n][0] + o[4 * g + n][2], fn, mn);
-                r[g][4 + n] = fmaf(o[4 * g + n][1] + o[4 * g + n][3], fn, mn);
+            for (int i = 0; i < 2; i++) {
+                const float mn = __shfl_sync(~0u, om[i], 4 * g + quad);
+                r[g][i][0] = fmaf(o[2 * g][i], f, mn);
+                r[g][i][1] = fmaf(o[2 * g][2 + i], f16, mn);
+                r[g][i][2] = fmaf(o[2 * g + 1][i], f, mn);
+                r[g][i][3] = fmaf(o[2 * g + 1][2 + i], f16, mn);
             }
         }
     };
-    auto put_part = [&](float *part, const float (&r)[G][8]) {
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-            float4 *p = reinterpret_cast<float4 *>(part + gid * D + g * 32 + quad * 8);
-            p[0] = make_float4(r[g][0], r[g][1], r[g][2], r[g][3]);
-            p[1] = make_float4(r[g][4], r[g][5], r[g][6], r[g][7]);
-        }
-        if (quad == 0) part[ROWS * D + gid] = m, part[ROWS * D + ROWS + gid] = l;
-    };
     auto lse_of = [](float mm, float ll) { return ll == 0.0f ? -INFINITY : (mm - P_SHIFT + log2f(ll)) * LN2; };
 
-    for (uint64_t idx = w0; idx < w1; idx++) {
-        if (idx >= seg_end) {
+    for (uint32_t idx = 0; idx < n; idx++, t0 += STEP) {
+        if (idx == c_end) {
             // a new segment: its query rows as operand registers
-            seg = seg_at(idx);
-            seg_end = seg.begin + seg.r.steps;
+            const Seg seg = seg_at(w0 + idx);
+            c_end = (uint32_t)min((uint64_t)n, seg.begin + seg.steps - w0);
+            t0 = (int32_t)(seg.r.s0 + (uint32_t)(w0 + idx - seg.begin)) * STEP;
+            held_end = seg.end;
             const uint32_t row = seg.tile * ROWS + gid, tok = row / a.group, hq = seg.head * a.group + row % a.group;
             const bool live = tok < (uint32_t)seg.r.nq;
             const T *q = (const T *)a.q + (uint64_t)(seg.r.tok0 + (live ? tok : 0)) * a.q_tok + hq * a.q_head + quad * 8;
-            float x[G][8], amax = 0.0f;
+            alignas(16) T raw[G][8];
+            if (a.vec_q) {
+#pragma unroll
+                for (int g = 0; g < G; g++)
+#pragma unroll
+                    for (int k = 0; k < (int)sizeof(T) / 2; k++)
+                        reinterpret_cast<uint4 *>(raw[g])[k] = __ldg(reinterpret_cast<const uint4 *>(q + g * 32) + k);
+            } else {
+#pragma unroll
+                for (int g = 0; g < G; g++)
+#pragma unroll
+                    for (int k = 0; k < 8; k++) raw[g][k] = q[g * 32 + k];
+            }
+            float amax = 0.0f;
 #pragma unroll
             for (int g = 0; g < G; g++)
 #pragma unroll
-                for (int n = 0; n < 8; n++) {
-                    x[g][n] = live ? Act<T>::get(q[g * 32 + n]) : 0.0f;
-                    amax = fmaxf(amax, fabsf(x[g][n]));
-                }
+                for (int k = 0; k < 8; k++) amax = fmaxf(amax, live ? fabsf(Act<T>::get(raw[g][k])) : 0.0f);
             amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
             // q * 2^(14 - e) is below 2^15 in f16; e is kept where 2^(14 - e) and 2^(e + 10) are f32 numbers
             const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 116);
-            const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-            cs = a.scale * LOG2E * __uint_as_float((uint32_t)(127 + 10 + e) << 23);
+            const float up = copysignf(__uint_as_float((uint32_t)(127 + 14 - e) << 23), a.scale);
+            const float cs_row = fabsf(a.scale) * LOG2E * __uint_as_float((uint32_t)(127 + 10 + e) << 23);
             float sum[G];
 #pragma unroll
             for (int g = 0; g < G; g++) {
+                float x[8];
                 sum[g] = 0.0f;
 #pragma unroll
-                for (int n = 0; n < 8; n++) sum[g] += x[g][n];
+                for (int k = 0; k < 8; k++) {
+                    x[k] = live ? Act<T>::get(raw[g][k]) : 0.0f;
+                    sum[g] += x[k];
+                }
                 sum[g] += __shfl_xor_sync(~0u, sum[g], 1);
                 sum[g] += __shfl_xor_sync(~0u, sum[g], 2);
                 sum[g] *= up * 0.015625f;
-                // nibbles (0, 4), (1, 5), (2, 6), (3, 7) make the four K registers; those of odd n are 16 c
+                // nibbles (0, 4), (1, 5), (2, 6), (3, 7) make the four K registers; those of odd ones are 16 c
 #pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    const float f = n & 1 ? up * 0.0625f : up, x0 = x[g][n] * f, x1 = x[g][n + 4] * f;
+                for (int k = 0; k < 4; k++) {
+                    const float f = k & 1 ? up * 0.0625f : up, x0 = x[k] * f, x1 = x[k + 4] * f;
                     const uint32_t hi = pack_h2(x0, x1);
-                    const int ks = 2 * g + (n >> 1), at = n & 1;
+                    qb[2 * g + (k >> 1)][k & 1] = hi;
                     if constexpr (Q32) {
                         const float2 h = unpack_h2(hi);
-                        qa[ks][2 * at] = hi;
-                        qa[ks][2 * at + 1] = pack_h2(x0 - h.x, x1 - h.y);
-                    } else {
-                        qa[ks][at] = hi;
+                        qb[2 * g + (k >> 1)][2 + (k & 1)] = pack_h2(x0 - h.x, x1 - h.y);
                     }
                 }
             }
             // sums of the query's groups against the K minima: column k holds group k % G, first the f16
             // rounding, then what it left
-            {
-                constexpr int KK = G == 8 ? 16 : 8;
 #pragma unroll
-                for (int w = 0; w < KK / 8; w++) {
-                    float v[2];
+            for (int w = 0; w < (G == 8 ? 2 : 1); w++) {
+                float v[2];
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const uint32_t k = w * 8 + quad * 2 + i, part = k / G, gg = k % G;
-                        float s = 0.0f;
+                for (int i = 0; i < 2; i++) {
+                    const uint32_t k = w * 8 + quad * 2 + i, part = k / G, gg = k % G;
+                    float s = 0.0f;
 #pragma unroll
-                        for (int g = 0; g < G; g++) s = (uint32_t)g == gg ? sum[g] : s;
-                        const float h = __half2float(__float2half_rn(s));
-                        v[i] = part == 0 ? h : part == 1 ? s - h : 0.0f;
-                    }
-                    qs[w] = pack_h2(v[0], v[1]);
+                    for (int g = 0; g < G; g++) s = (uint32_t)g == gg ? sum[g] : s;
+                    const float h = __half2float(__float2half_rn(s));
+                    v[i] = part == 0 ? h : part == 1 ? s - h : 0.0f;
                 }
+                qs[w] = pack_h2(v[0], v[1]);
             }
             // what this row sees, and what every row of the tile sees
-            const int64_t place = (int64_t)a.seq[seg.req] - seg.r.nq + tok;
-            hi_t = live ? (int32_t)min(place + 1, (int64_t)seg.r.seq) : 0;
-            lo_t = a.window && place + 1 > (int64_t)a.window ? (int32_t)(place + 1 - a.window) : 0;
-            full_hi = __reduce_min_sync(~0u, live ? hi_t : 0x7fffffff);
-            full_lo = __reduce_max_sync(~0u, live ? lo_t : 0);
-            m = -INFINITY, l = 0.0f, kexp = 15, vlim = -1.0f;
+            const int64_t place = (int64_t)seg.r.seq - seg.r.nq + tok;
+            const int32_t hi_row = live ? (int32_t)max((int64_t)0, min(place + 1, (int64_t)seg.end)) : 0;
+            const int32_t lo_row = a.window && place + 1 > (int64_t)a.window ? (int32_t)(place + 1 - a.window) : 0;
+            full_hi = __reduce_min_sync(~0u, live ? hi_row : 0x7fffffff);
+            full_lo = __reduce_max_sync(~0u, live ? lo_row : 0);
 #pragma unroll
-            for (int i = 0; i < 4 * G; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+            for (int i = 0; i < 2; i++) {
+                const int src = (2 * quad + i) * 4;
+                cs[i] = __shfl_sync(~0u, cs_row, src);
+                hi_t[i] = __shfl_sync(~0u, hi_row, src);
+                lo_t[i] = __shfl_sync(~0u, lo_row, src);
+                m[i] = -INFINITY, l[i] = 0.0f;
+            }
+            kexp = 15, vlim2 = 0x13FF13FFu;  // the f16 below 2^-10
+#pragma unroll
+            for (int i = 0; i < 2 * G; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
             om[0] = om[1] = om[2] = om[3] = 0.0f;
 #pragma unroll
             for (int g = 0; g < G; g++) kmul[g] = 0x78007800u;  // 2^15
@@ -418,130 +492,145 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
         }
         dead = __any_sync(~0u, dead);
         const uint8_t *buf = ring + stage * C::STAGE_BYTES;
-        const int32_t t0 = (int32_t)(seg.r.s0 + (uint32_t)(idx - seg.begin)) * STEP;
-        const uint32_t here = there[0];
+        const uint32_t here = there & ((1u << TILES) - 1);
         // whole: every row sees every position of the step
         const bool whole = here == (1u << TILES) - 1 && t0 >= full_lo && t0 + STEP <= full_hi;
 
-        // scores
+        // scores: s[i][2 p + r] of position 16 i + gid + 8 p and row 2 quad + r
         float s[TILES][4];
 #pragma unroll
         for (int i = 0; i < TILES; i++) {
             const uint8_t *tile = buf + i * L::BYTES;
+            uint32_t w0_[G], w1_[G], ks0[G], ks1[G];
+            lds_codes<G, 4>(w0_, tile + gid * L::KROW, quad);
+            lds_codes<G, 4>(w1_, tile + (gid + 8) * L::KROW, quad);
+            lds_words<G>(ks0, tile + L::KS + (gid >> 1) * (G * 4));
+            lds_words<G>(ks1, tile + L::KS + (4 + (gid >> 1)) * (G * 4));
+            constexpr int KMW = G == 2 ? 0 : G == 4 ? 1 : 3;
+            const uint32_t km0 = *reinterpret_cast<const uint32_t *>(tile + L::KM + gid * (G * 2) + (quad & KMW) * 4);
+            const uint32_t km1 = *reinterpret_cast<const uint32_t *>(tile + L::KM + (gid + 8) * (G * 2) + (quad & KMW) * 4);
+            float c[4];
+            if constexpr (G == 8) mma16_first(c, km0, km1, km0, km1, qs[0], qs[1]);
+            else mma8_first(c, km0, km1, qs[0]);
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                uint32_t w[G], ks[G];
-                lds_codes<G, 4>(w, tile + (8 * j + gid) * L::KROW, quad);
-                lds_words<G>(ks, tile + L::KS + (4 * j + quad) * (G * 4));
-                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                if constexpr (G == 8) {
-                    const uint32_t km = *reinterpret_cast<const uint32_t *>(tile + L::KM + ((8 * j + gid) * G + 2 * quad) * 2);
-                    mma16(c, qs[0], 0, qs[1], 0, km, km);
-                } else {
-                    const uint32_t km = *reinterpret_cast<const uint32_t *>(tile + L::KM + ((8 * j + gid) * G + (G == 4 ? (quad & 1) * 2 : 0)) * 2);
-                    asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
-                        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                        : "r"(qs[0]), "r"(0), "r"(km));
-                }
-                float s0 = c[0] * 0x1p-18f, s1 = c[1] * 0x1p-18f;
+            for (int k = 0; k < 4; k++) s[i][k] = c[k] * 0x1p-18f;
 #pragma unroll
-                for (int g = 0; g < G; g++) {
-                    const uint32_t h = w[g] >> 8;
-                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if constexpr (Q32) {
-                        mma16(d, qa[2 * g][0], qa[2 * g][1], qa[2 * g][2], qa[2 * g][3], w[g] & 0x000F000Fu, w[g] & 0x00F000F0u);
-                        mma16(d, qa[2 * g + 1][0], qa[2 * g + 1][1], qa[2 * g + 1][2], qa[2 * g + 1][3], h & 0x000F000Fu, h & 0x00F000F0u);
-                        d[0] += d[2], d[1] += d[3];
-                    } else {
-                        mma16(d, qa[2 * g][0], 0, qa[2 * g][1], 0, w[g] & 0x000F000Fu, w[g] & 0x00F000F0u);
-                        mma16(d, qa[2 * g + 1][0], 0, qa[2 * g + 1][1], 0, h & 0x000F000Fu, h & 0x00F000F0u);
-                    }
-                    const float2 sc = unpack_h2(ks[g]);
-                    s0 = fmaf(d[0], sc.x, s0);
-                    s1 = fmaf(d[1], sc.y, s1);
+            for (int g = 0; g < G; g++) {
+                const uint32_t h0 = w0_[g] >> 8, h1 = w1_[g] >> 8;
+                float d[4];
+                mma16_first(d, w0_[g] & 0x000F000Fu, w1_[g] & 0x000F000Fu, w0_[g] & 0x00F000F0u, w1_[g] & 0x00F000F0u, qb[2 * g][0], qb[2 * g][1]);
+                mma16(d, h0 & 0x000F000Fu, h1 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x00F000F0u, qb[2 * g + 1][0], qb[2 * g + 1][1]);
+                if constexpr (Q32) {
+                    mma16(d, w0_[g] & 0x000F000Fu, w1_[g] & 0x000F000Fu, w0_[g] & 0x00F000F0u, w1_[g] & 0x00F000F0u, qb[2 * g][2], qb[2 * g][3]);
+                    mma16(d, h0 & 0x000F000Fu, h1 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x00F000F0u, qb[2 * g + 1][2], qb[2 * g + 1][3]);
                 }
-                s[i][2 * j] = s0, s[i][2 * j + 1] = s1;
+                // scales of positions gid (even or odd in its pair) for two groups in one register
+                if (g % 2 == 0) {
+                    ks0[g] = __byte_perm(ks0[g], ks0[g + 1], half_sel);
+                    ks1[g] = __byte_perm(ks1[g], ks1[g + 1], half_sel);
+                }
+                const float2 sc0 = unpack_h2(ks0[g & ~1]), sc1 = unpack_h2(ks1[g & ~1]);
+                const float a0 = g & 1 ? sc0.y : sc0.x, a1 = g & 1 ? sc1.y : sc1.x;
+                s[i][0] = fmaf(d[0], a0, s[i][0]), s[i][1] = fmaf(d[1], a0, s[i][1]);
+                s[i][2] = fmaf(d[2], a1, s[i][2]), s[i][3] = fmaf(d[3], a1, s[i][3]);
             }
         }
-        // positions that a row does not see, and the running maximum
-        float top = m;
+        // positions that a row does not see, and the reference of the weights: a running maximum that follows
+        // the true one only when it is 2^LAG behind, so that the sums are seldom rescaled
+        if (!whole) {
 #pragma unroll
-        for (int i = 0; i < TILES; i++)
+            for (int i = 0; i < TILES; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                s[i][j] *= cs;
-                if (!whole) {
-                    const int32_t t = t0 + i * 16 + (j >> 1) * 8 + quad * 2 + (j & 1);
-                    if (t < lo_t || t >= hi_t || !(here >> i & 1)) s[i][j] = -INFINITY;
+                for (int k = 0; k < 4; k++) {
+                    const int32_t t = t0 + i * 16 + gid + (k >> 1) * 8;
+                    if (t < lo_t[k & 1] || t >= hi_t[k & 1] || !(here >> i & 1)) s[i][k] = -INFINITY;
                 }
-                top = fmaxf(top, s[i][j]);
-            }
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-        if (__any_sync(~0u, top > m)) {
-            const float f = m == top ? 1.0f : ex2(m - top);
-            m = top;
-            l *= f;
-#pragma unroll
-            for (int i = 0; i < 4 * G; i++) o[i][0] *= f, o[i][1] *= f, o[i][2] *= f, o[i][3] *= f;
-            om[0] *= f, om[1] *= f, om[2] *= f, om[3] *= f;
         }
-        const float shift = m == -INFINITY ? 0.0f : P_SHIFT - m;
+        float top[2];
+        bool behind = false;
 #pragma unroll
-        for (int i = 0; i < TILES; i++)
+        for (int r = 0; r < 2; r++) {
+            top[r] = fmaxf(s[0][r], s[0][2 + r]);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                s[i][j] = ex2(s[i][j] + shift);
-                l += s[i][j];
+            for (int i = 1; i < TILES; i++) top[r] = fmaxf(top[r], fmaxf(s[i][r], s[i][2 + r]));
+            top[r] *= cs[r];
+            behind |= top[r] > m[r] + LAG;
+        }
+        if (__any_sync(~0u, behind)) {
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) top[r] = fmaxf(top[r], __shfl_xor_sync(~0u, top[r], off));
+                const float mm = fmaxf(m[r], top[r]), f = m[r] == mm ? 1.0f : ex2(m[r] - mm);
+                m[r] = mm;
+                l[r] *= f;
+#pragma unroll
+                for (int i = 0; i < 2 * G; i++) o[i][r] *= f, o[i][2 + r] *= f;
+                om[r] *= f;
             }
+        }
+        const float sh0 = m[0] == -INFINITY ? 0.0f : P_SHIFT - m[0], sh1 = m[1] == -INFINITY ? 0.0f : P_SHIFT - m[1];
 
         // values
 #pragma unroll
         for (int i = 0; i < TILES; i++) {
             const uint8_t *tile = buf + i * L::BYTES;
+            // the weights, and as f16 rounding and rest, turned so that a lane has positions 2 quad + (0, 1) + 8 j of row gid
+            uint32_t ph[2], pl[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float p0 = ex2(fmaf(s[i][2 * j], cs[0], sh0)), p1 = ex2(fmaf(s[i][2 * j + 1], cs[1], sh1));
+                l[0] += p0, l[1] += p1;
+                ph[j] = pack_h2(p0, p1);
+                const float2 h = unpack_h2(ph[j]);
+                pl[j] = transpose8(pack_h2(p0 - h.x, p1 - h.y));
+                ph[j] = transpose8(ph[j]);
+            }
             // positions of this tile that are held; the others' scales and minima may be anything
-            const int32_t held = here >> i & 1 ? seg.r.seq - (t0 + i * 16) : 0;
+            const int32_t held = here >> i & 1 ? held_end - (t0 + i * 16) : 0;
             const bool part = held < 16;
             // a V scale larger than any before: the group's sums move to a new power of two
-            float vmax = 0.0f;
-            {
-                constexpr int N = G * 8 / 32 ? G * 8 / 32 : 1;
+            constexpr int N = G == 8 ? 2 : 1;  // the tile's 8 G words of scales, lane l's of group l % G
+            uint32_t vw[N];
+            bool above = false;
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                const uint32_t at = (lane + 32 * k) % (G * 8);
+                vw[k] = *reinterpret_cast<const uint32_t *>(tile + L::VS + at * 4);
+                if (part) {
+                    const int32_t t = (int32_t)(at / G) * 2;
+                    vw[k] &= t + 1 < held ? 0xffffffffu : t < held ? 0xffffu : 0u;
+                }
+                above |= any_gt_h2(vw[k], vlim2);
+            }
+            if (__any_sync(~0u, above)) {
+                float vmax = 0.0f;
 #pragma unroll
                 for (int k = 0; k < N; k++) {
-                    const uint32_t at = (lane + 32 * k) % (G * 8), pos = at / G * 2;
-                    const float2 v = unpack_h2(*reinterpret_cast<const uint32_t *>(tile + L::VS + at * 4));
-                    if ((int32_t)pos < held) vmax = fmaxf(vmax, v.x);
-                    if ((int32_t)pos + 1 < held) vmax = fmaxf(vmax, v.y);
+                    const float2 v = unpack_h2(vw[k]);
+                    vmax = fmaxf(vmax, fmaxf(v.x, v.y));
                 }
-            }
-            if (__any_sync(~0u, vmax > vlim)) {
 #pragma unroll
                 for (int off = G; off < 32; off <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(~0u, vmax, off));
-                if (vmax > vlim) {
-                    // 2^kexp times the largest scale is below 2^5 (kexp at most 15, f16's largest power)
-                    const int k = min(15, 4 - ((int)(__float_as_uint(vmax) >> 23) - 127));
-                    vlim = __uint_as_float((uint32_t)(127 + 5 - k) << 23) * 0.99999994f;
-                    const int old = kexp;
-                    kexp = min(k, kexp);
-                    vmax = __uint_as_float((uint32_t)(127 + kexp - old) << 23);
-                } else {
-                    vmax = 1.0f;
-                }
+                // 2^kexp times the largest scale is below 2^5 (kexp at most 15, f16's largest power of two)
+                const int k = min(kexp, 4 - ((int)(__float_as_uint(vmax) >> 23) - 127));
+                vmax = __uint_as_float((uint32_t)(127 + k - kexp) << 23);
+                kexp = k;
+                vlim2 = (uint32_t)((15 + 5 - k) << 10) * 0x10001u - 0x10001u;  // the f16 below 2^(5 - k)
 #pragma unroll
                 for (int g = 0; g < G; g++) {
                     const float f = __shfl_sync(~0u, vmax, g);
-                    const int k = __shfl_sync(~0u, kexp, g);
-                    kmul[g] = (uint32_t)(15 + k) << 10 | (uint32_t)(15 + k) << 26;
+                    const int kg = __shfl_sync(~0u, kexp, g);
+                    kmul[g] = (uint32_t)(15 + kg) << 10 | (uint32_t)(15 + kg) << 26;
 #pragma unroll
-                    for (int n = 0; n < 4; n++)
-                        o[4 * g + n][0] *= f, o[4 * g + n][1] *= f, o[4 * g + n][2] *= f, o[4 * g + n][3] *= f;
+                    for (int k2 = 0; k2 < 4; k2++) o[2 * g][k2] *= f, o[2 * g + 1][k2] *= f;
                 }
             }
-            uint32_t vs[2][G], vm[2], v[2][G], ph[2], pl[2];
+            uint32_t vs[2][G], vm[2], v[2][G];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 lds_words<G>(vs[j], tile + L::VS + (4 * j + quad) * (G * 4));
-                vm[j] = gid < G ? *reinterpret_cast<const uint32_t *>(tile + L::VM + ((4 * j + quad) * G + (G == 8 ? gid : gid % G)) * 4) : 0u;
+                vm[j] = *reinterpret_cast<const uint32_t *>(tile + L::VM + ((4 * j + quad) * G + gid % G) * 4);
                 lds_codes<G, 8>(v[j], tile + L::VC + (4 * j + quad) * L::VROW, gid);
                 if (part) {
                     const int32_t t = 8 * j + 2 * quad;
@@ -550,71 +639,65 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
 #pragma unroll
                     for (int g = 0; g < G; g++) vs[j][g] &= mask;
                 }
-                ph[j] = pack_h2(s[i][2 * j], s[i][2 * j + 1]);
-                const float2 h = unpack_h2(ph[j]);
-                pl[j] = pack_h2(s[i][2 * j] - h.x, s[i][2 * j + 1] - h.y);
             }
-            mma16(om, ph[0], pl[0], ph[1], pl[1], vm[0], vm[1]);
+            // row gid of the minima's product is group gid % G
+            mma16(om, vm[0], 0, vm[1], 0, ph[0], ph[1]);
+            mma16(om, vm[0], 0, vm[1], 0, pl[0], pl[1]);
 #pragma unroll
             for (int g = 0; g < G; g++) {
                 uint32_t hi[2], lo[2];
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    const float2 sc = unpack_h2(mul_h2(vs[j][g], kmul[g]));
-                    hi[j] = pack_h2(s[i][2 * j] * sc.x, s[i][2 * j + 1] * sc.y);
-                    const float2 h = unpack_h2(hi[j]);
-                    lo[j] = pack_h2(fmaf(s[i][2 * j], sc.x, -h.x), fmaf(s[i][2 * j + 1], sc.y, -h.y));
+                    // (ph + pl) sc as the f16 rounding of ph sc and the rest
+                    const uint32_t sc = mul_h2(vs[j][g], kmul[g]);
+                    hi[j] = mul_h2(ph[j], sc);
+                    lo[j] = fma_h2(pl[j], sc, fma_h2(ph[j], sc, hi[j] ^ 0x80008000u));
                 }
-                const uint32_t w0_ = v[0][g], w1_ = v[1][g], h0 = w0_ >> 8, h1 = w1_ >> 8;
-                mma16(o[4 * g], hi[0], lo[0], hi[1], lo[1], w0_ & 0x000F000Fu, w1_ & 0x000F000Fu);
-                mma16(o[4 * g + 1], hi[0], lo[0], hi[1], lo[1], w0_ & 0x00F000F0u, w1_ & 0x00F000F0u);
-                mma16(o[4 * g + 2], hi[0], lo[0], hi[1], lo[1], h0 & 0x000F000Fu, h1 & 0x000F000Fu);
-                mma16(o[4 * g + 3], hi[0], lo[0], hi[1], lo[1], h0 & 0x00F000F0u, h1 & 0x00F000F0u);
+                const uint32_t h0 = v[0][g] >> 8, h1 = v[1][g] >> 8;
+                mma16(o[2 * g], v[0][g] & 0x000F000Fu, v[0][g] & 0x00F000F0u, v[1][g] & 0x000F000Fu, v[1][g] & 0x00F000F0u, hi[0], hi[1]);
+                mma16(o[2 * g], v[0][g] & 0x000F000Fu, v[0][g] & 0x00F000F0u, v[1][g] & 0x000F000Fu, v[1][g] & 0x00F000F0u, lo[0], lo[1]);
+                mma16(o[2 * g + 1], h0 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x000F000Fu, h1 & 0x00F000F0u, hi[0], hi[1]);
+                mma16(o[2 * g + 1], h0 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x000F000Fu, h1 & 0x00F000F0u, lo[0], lo[1]);
             }
         }
 
         // the stage is read: the next copy into it
         __syncwarp();
-#pragma unroll
-        for (int k = 0; k + 1 < STAGES; k++) there[k] = there[k + 1];
-        there[STAGES - 1] = issue(stage);
-        fetch();
+        there = there >> TILES | issue(stage) << ((STAGES - 1) * TILES);
         if (++stage == STAGES) stage = 0, phase ^= 1;
 
-        if (idx + 1 == seg_end || idx + 1 == w1) {
+        if (idx + 1 == c_end) {
             // the end of the segment, or of this warp's part of it
-            l += __shfl_xor_sync(~0u, l, 1);
-            l += __shfl_xor_sync(~0u, l, 2);
-            float r[G][8];
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) {
+                l[0] += __shfl_xor_sync(~0u, l[0], off);
+                l[1] += __shfl_xor_sync(~0u, l[1], off);
+            }
+            float r[G][2][4];
             rows_of(r);
-            const bool begins = seg.begin >= w0, ends = seg_end <= w1;
-            if (begins && ends) {
-                const uint32_t row = seg.tile * ROWS + gid, tok = row / a.group, hq = seg.head * a.group + row % a.group;
-                if (tok < (uint32_t)seg.r.nq) {
-                    const uint64_t t = (uint64_t)seg.r.tok0 + tok;
-                    T *out = (T *)a.out + t * a.o_tok + hq * a.o_head + quad * 8;
-                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const Seg seg = seg_at(w0 + idx);
+            const bool begins = seg.begin >= w0, ends = seg.begin + seg.steps <= w1;
+            // a part that began before this warp (at most one) and one that goes on after it (at most one) are left for the joins
+            float *part = begins ? reinterpret_cast<float *>(ring) : first_all + warp * (C::PART_BYTES / 4);
+            if (lane == 0 && !(begins && ends)) seg_begin[2 * warp + begins] = seg.begin;
 #pragma unroll
-                    for (int g = 0; g < G; g++) {
-                        alignas(16) T y[8];
+            for (int i = 0; i < 2; i++) {
+                const uint32_t tr = 2 * quad + i;
+                if (!(begins && ends)) {
 #pragma unroll
-                        for (int n = 0; n < 8; n++) y[n] = Act<T>::put(r[g][n] * inv);
-                        if (a.vec_out) {
-#pragma unroll
-                            for (int k = 0; k < (int)sizeof(T) / 2; k++)
-                                reinterpret_cast<uint4 *>(out + g * 32)[k] = reinterpret_cast<const uint4 *>(y)[k];
-                        } else {
-#pragma unroll
-                            for (int n = 0; n < 8; n++) out[g * 32 + n] = y[n];
-                        }
-                    }
-                    if (a.lse && quad == 0) a.lse[t * a.n_heads + hq] = lse_of(m, l);
+                    for (int g = 0; g < G; g++)
+                        *reinterpret_cast<float4 *>(part + tr * D + g * 32 + gid * 4) = make_float4(r[g][i][0], r[g][i][1], r[g][i][2], r[g][i][3]);
+                    if (gid == 0) part[ROWS * D + tr] = m[i], part[ROWS * D + ROWS + tr] = l[i];
+                    continue;
                 }
-            } else {
-                // at most one part that began before this warp, and one that goes on after it
-                const uint32_t k = begins ? 1 : 0;
-                put_part(k ? reinterpret_cast<float *>(ring) : first_all + warp * (C::PART_BYTES / 4), r);
-                if (lane == 0) seg_begin[2 * warp + k] = seg.begin;
+                const uint32_t row = seg.tile * ROWS + tr, tok = row / a.group, hq = seg.head * a.group + row % a.group;
+                if (tok >= (uint32_t)seg.r.nq) continue;
+                const uint64_t t = (uint64_t)seg.r.tok0 + tok;
+                T *out = (T *)a.out + t * a.o_tok + hq * a.o_head + gid * 4;
+                const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+#pragma unroll
+                for (int g = 0; g < G; g++) put4(out + g * 32, r[g][i][0] * inv, r[g][i][1] * inv, r[g][i][2] * inv, r[g][i][3] * inv, a.vec_out);
+                if (a.lse && gid == 0) a.lse[t * a.n_heads + hq] = lse_of(m[i], l[i]);
             }
         }
     }
@@ -640,41 +723,62 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
         uint32_t k1 = k0 + 1;
         while (k1 < 2 * WARPS && (seg_begin[k1] == sb || seg_begin[k1] == ~0ull)) k1++;
         const Seg sg_ = seg_at(sb);
-        const uint64_t se = sb + sg_.r.steps;
+        const uint64_t se = sb + sg_.steps;
         const bool all_here = sb >= c0 && se <= c1;
         const uint32_t cb = (uint32_t)(sb / cta_chunk), ce = (uint32_t)((se - 1) / cta_chunk);
-        // joins the rows of n partial results, a thread per value
-        auto join_out = [&](uint32_t n, auto part, auto ld, bool final_, float *dst) {
-            for (uint32_t e = tid; e < ROWS * D; e += WARPS * 32) {
-                const uint32_t row = e / D, d = e % D;
+        // Joins the rows of n partial results: the weights of each row by a warp, then a thread per four values
+        // with several of the parts' loads in flight.
+        auto join_out = [&](uint32_t n, auto part, auto ld4, auto ld, bool final_, float *dst) {
+            for (uint32_t row = warp; row < ROWS; row += WARPS) {
                 float mm = -INFINITY;
+                for (uint32_t i = lane; i < n; i += 32) {
+                    const float *p = part(i);
+                    const float v = p ? ld(p + ROWS * D + row) : -INFINITY;
+                    weight_s[i * ROWS + row] = v;
+                    mm = fmaxf(mm, v);
+                }
+#pragma unroll
+                for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(~0u, mm, o));
+                float ll = 0.0f;
+                for (uint32_t i = lane; i < n; i += 32) {
+                    const float *p = part(i);
+                    const float mi = weight_s[i * ROWS + row], w = !p ? 0.0f : mi == mm ? 1.0f : ex2(mi - mm);
+                    weight_s[i * ROWS + row] = w;
+                    if (p) ll = fmaf(w, ld(p + ROWS * D + ROWS + row), ll);
+                }
+#pragma unroll
+                for (int o = 16; o; o >>= 1) ll += __shfl_xor_sync(~0u, ll, o);
+                if (lane == 0) ml_s[row] = mm, ml_s[ROWS + row] = ll;
+            }
+            __syncthreads();
+            for (uint32_t e = tid * 4; e < ROWS * D; e += WARPS * 128) {
+                const uint32_t row = e / D, d = e % D;
+                float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
                 for (uint32_t i = 0; i < n; i++) {
                     const float *p = part(i);
-                    if (p) mm = fmaxf(mm, ld(p + ROWS * D + row));
+                    const float w = weight_s[i * ROWS + row];
+                    const float4 v = p ? ld4(p + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    acc.x = fmaf(w, v.x, acc.x), acc.y = fmaf(w, v.y, acc.y), acc.z = fmaf(w, v.z, acc.z), acc.w = fmaf(w, v.w, acc.w);
                 }
-                float acc = 0.0f, ll = 0.0f;
-                for (uint32_t i = 0; i < n; i++) {
-                    const float *p = part(i);
-                    if (!p) continue;
-                    const float mi = ld(p + ROWS * D + row), w = mi == mm ? 1.0f : ex2(mi - mm);
-                    acc = fmaf(w, ld(p + e), acc);
-                    ll = fmaf(w, ld(p + ROWS * D + ROWS + row), ll);
-                }
+                const float mm = ml_s[row], ll = ml_s[ROWS + row];
                 if (!final_) {
-                    dst[e] = acc;
+                    *reinterpret_cast<float4 *>(dst + e) = acc;
                     if (d == 0) dst[ROWS * D + row] = mm, dst[ROWS * D + ROWS + row] = ll;
                     continue;
                 }
                 const uint32_t rr = sg_.tile * ROWS + row, tok = rr / a.group, hq = sg_.head * a.group + rr % a.group;
                 if (tok >= (uint32_t)sg_.r.nq) continue;
                 const uint64_t t = (uint64_t)sg_.r.tok0 + tok;
-                ((T *)a.out)[t * a.o_tok + hq * a.o_head + d] = Act<T>::put(ll == 0.0f ? 0.0f : acc / ll);
+                const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+                put4((T *)a.out + t * a.o_tok + hq * a.o_head + d, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv, a.vec_out);
                 if (a.lse && d == 0) a.lse[t * a.n_heads + hq] = lse_of(mm, ll);
             }
         };
         auto in_smem = [&](uint32_t i) -> const float * { return seg_begin[k0 + i] == sb ? slot(k0 + i) : nullptr; };
         float *mine = parts + (uint64_t)(blockIdx.x * 2 + (sb < c0 ? 0 : 1)) * PART;
-        join_out(k1 - k0, in_smem, [](const float *p) { return *p; }, all_here, mine);
+        join_out(k1 - k0, in_smem, [](const float *p) { return *reinterpret_cast<const float4 *>(p); },
+                 [](const float *p) { return *p; }, all_here, mine);
         if (!all_here) {
             __threadfence();
             __syncthreads();
@@ -687,10 +791,11 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
             if (*flag_s) {
                 __threadfence();
                 auto in_scratch = [&](uint32_t i) -> const float * { return parts + (uint64_t)((cb + i) * 2 + (i ? 0 : 1)) * PART; };
-                join_out(ce - cb + 1, in_scratch, [](const float *p) { return __ldcg(p); }, true, nullptr);
+                join_out(ce - cb + 1, in_scratch, [](const float *p) { return __ldcg(reinterpret_cast<const float4 *>(p)); },
+                         [](const float *p) { return __ldcg(p); }, true, nullptr);
             }
-            __syncthreads();
         }
+        __syncthreads();
         k0 = k1;
     }
 }
