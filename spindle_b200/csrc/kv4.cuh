@@ -75,7 +75,8 @@ struct Kv4AttnArgs {
     uint8_t *scratch;
     uint64_t block_bytes;  // of one block, all heads
     bool vec_q, vec_out;  // the rows allow 16-byte accesses
-    bool last;     // this launch's requests are the last ones
+    bool last;            // this launch's requests are the last ones
+    uint32_t head0, n_kv; // and its KV heads
 };
 
 constexpr int KV4_PLAN_THREADS = 1024;

@@ -27,6 +27,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "kv4.cuh"
 
 namespace sg {
@@ -68,14 +70,17 @@ __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
     return d;
 }
 
+// a b + c, a b - c
 __device__ __forceinline__ uint32_t fma_h2(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t d;
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
     return d;
 }
-// Any half of a larger than b's: both hold f16 numbers that are not negative.
-__device__ __forceinline__ bool any_gt_h2(uint32_t a, uint32_t b) { return __vmaxu2(a, b) != b; }
-
+__device__ __forceinline__ uint32_t fms_h2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("{\n .reg .b32 t;\n neg.f16x2 t, %3;\n fma.rn.f16x2 %0, %1, %2, t;\n}" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
 // d = a b, d += a b
 __device__ __forceinline__ void mma16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
@@ -147,6 +152,7 @@ constexpr float P_SHIFT = 2.0f, LAG = 8.0f;
 constexpr int ROWS = 8;
 constexpr uint32_t MAX_REQ = 1024;  // requests of one launch (their steps are in shared memory)
 constexpr uint32_t MAX_CTAS = 320;
+constexpr uint32_t MIN_WARPS = 4;   // warps that a CTA uses at least, where the steps are few
 
 template <int D>
 struct Cfg {
@@ -158,7 +164,9 @@ struct Cfg {
     static constexpr uint32_t STAGE_BYTES = TILES * Kv4Tile<D>::BYTES;
     static constexpr uint32_t PART_BYTES = ROWS * D * 4 + 2 * ROWS * 4;  // rows, m, l
     static constexpr uint32_t RING = WARPS * STAGES * STAGE_BYTES;
-    static constexpr uint32_t SMEM = RING + WARPS * PART_BYTES + (MAX_REQ + 1) * 8 + MAX_REQ * 16 + WARPS * STAGES * 8 + 1024 + (MAX_CTAS + 2) * ROWS * 4;
+    static constexpr int SEGS = STAGES + 1;
+    static constexpr uint32_t SMEM = RING + WARPS * PART_BYTES + (MAX_REQ + 1) * 4 + MAX_REQ * 16 + WARPS * (STAGES * 8 + (SEGS + 2) * 40 + 4) + 512;
+    static_assert(WARPS <= 16, "a lane per partial result");
     static_assert(STAGES * STAGE_BYTES >= PART_BYTES, "a warp's last partial result lies in its ring");
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
@@ -190,8 +198,8 @@ __device__ __forceinline__ Req req_of(const Kv4AttnArgs &a, uint32_t i, uint32_t
 struct Seg {
     Req r;
     int32_t end;  // positions that the table has room for
-    uint32_t req, head, tile, steps;
-    uint64_t begin;  // its first step among all steps
+    uint32_t req, head, tile;
+    uint32_t begin, steps;  // its first step among all steps, its steps
 };
 
 }  // namespace
@@ -206,74 +214,75 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring_all = smem;
     float *first_all = reinterpret_cast<float *>(smem + C::RING);
-    uint64_t *pre = reinterpret_cast<uint64_t *>(smem + C::RING + WARPS * C::PART_BYTES);  // [n_req + 1] steps before each request
-    Req *reqs = reinterpret_cast<Req *>(pre + MAX_REQ + 1);
-    uint64_t *bars = reinterpret_cast<uint64_t *>(reqs + MAX_REQ);
-    uint64_t *seg_begin = bars + WARPS * STAGES;                      // [2 * WARPS] the partials' segments, ~0: none
-    uint64_t *scan_s = seg_begin + 2 * WARPS;                         // [WARPS + 1]
-    uint32_t *flag_s = reinterpret_cast<uint32_t *>(scan_s + WARPS + 1);
-    float *weight_s = reinterpret_cast<float *>(flag_s + 2), *ml_s = weight_s + MAX_CTAS * ROWS;  // of the joins
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::RING + WARPS * C::PART_BYTES);
+    Req *reqs = reinterpret_cast<Req *>(bars + WARPS * STAGES);       // [n_req]
+    Seg *segs_all = reinterpret_cast<Seg *>(reqs + MAX_REQ);          // [WARPS][SEGS] the segments in a warp's ring
+    Seg *part_seg = segs_all + WARPS * C::SEGS;                       // [2 * WARPS] the partial results' segments
+    uint32_t *pre = reinterpret_cast<uint32_t *>(part_seg + 2 * WARPS);  // [n_req + 1] steps before each request
+    uint32_t *seg_begin = pre + MAX_REQ + 1;                          // [32] the partials' segments, NONE: no partial
+    uint32_t *scan_s = seg_begin + 32;                                // [WARPS]
+    uint32_t *flag_s = scan_s + WARPS;                                // [2]
+    constexpr uint32_t NONE = 0xffffffffu;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, quad = lane & 3;
 
     if (lane == 0)
         for (int s = 0; s < STAGES; s++) mbar_init(&bars[warp * STAGES + s], 1);
     fence_mbar_init();
-    if (tid < 2 * WARPS) seg_begin[tid] = ~0ull;
+    if (tid < 32) seg_begin[tid] = NONE;
 
     auto tiles_of = [&](const Req &r) { return ((uint32_t)r.nq * a.group + ROWS - 1) / ROWS; };
 
+    const uint32_t spare = !a.last ? a.n_tok : a.n_req ? (uint32_t)max(a.cu[a.n_req], 0) : 0;  // first token of no request
+
     // steps before each request
-    uint64_t total = 0;
+    uint32_t total = 0;
     for (uint32_t r0 = 0; r0 < a.n_req; r0 += WARPS * 32) {
-        uint64_t v = 0;
+        uint32_t v = 0;
         if (r0 + tid < a.n_req) {
             uint32_t steps;
             const Req r = req_of<STEP>(a, r0 + tid, steps);
             reqs[r0 + tid] = r;
-            v = (uint64_t)steps * tiles_of(r) * a.c.heads;
+            v = steps * tiles_of(r) * a.n_kv;
         }
-        uint64_t inc = v;
+        uint32_t inc = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t u = __shfl_up_sync(~0u, inc, o);
+            const uint32_t u = __shfl_up_sync(~0u, inc, o);
             if (lane >= (uint32_t)o) inc += u;
         }
         if (lane == 31) scan_s[warp] = inc;
         __syncthreads();
-        uint64_t base = total, all = 0;
-        for (int w = 0; w < WARPS; w++) {
-            if ((uint32_t)w < warp) base += scan_s[w];
-            all += scan_s[w];
-        }
-        if (r0 + tid < a.n_req) pre[r0 + tid] = base + inc - v;
-        total += all;
+        const uint32_t w = lane < WARPS ? scan_s[lane] : 0;
+        const uint32_t base = __reduce_add_sync(~0u, lane < warp ? w : 0);
+        if (r0 + tid < a.n_req) pre[r0 + tid] = total + base + inc - v;
+        total += __reduce_add_sync(~0u, w);
         __syncthreads();
     }
     if (tid == 0) pre[a.n_req] = total;
     __syncthreads();
 
     // tokens of no request
-    {
-        const uint32_t t0 = !a.last ? a.n_tok : a.n_req ? (uint32_t)max(a.cu[a.n_req], 0) : 0;
-        const uint64_t n = t0 < a.n_tok ? (uint64_t)(a.n_tok - t0) * a.n_heads * D : 0;
-        for (uint64_t e = (uint64_t)blockIdx.x * (WARPS * 32) + tid; e < n; e += (uint64_t)gridDim.x * (WARPS * 32)) {
-            const uint64_t row = e / D, t = t0 + row / a.n_heads, h = row % a.n_heads;
-            ((T *)a.out)[t * a.o_tok + h * a.o_head + e % D] = Act<T>::put(0.0f);
-            if (a.lse && e % D == 0) a.lse[t * a.n_heads + h] = -INFINITY;
+    if (spare < a.n_tok) {
+        const uint32_t rows = (a.n_tok - spare) * a.n_heads;
+        for (uint32_t row = blockIdx.x * WARPS + warp; row < rows; row += gridDim.x * WARPS) {
+            const uint32_t t = spare + row / a.n_heads, h = row % a.n_heads;
+            if (h / a.group - a.head0 >= a.n_kv) continue;
+            for (uint32_t d = lane; d < D; d += 32) ((T *)a.out)[t * a.o_tok + h * a.o_head + d] = Act<T>::put(0.0f);
+            if (a.lse && lane == 0) a.lse[(uint64_t)t * a.n_heads + h] = -INFINITY;
         }
     }
 
-    // this warp's stretch [w0, w1) of the steps; fewer warps a CTA where there is little to do
-    const uint64_t per_cta = (total + gridDim.x - 1) / gridDim.x;
-    const uint32_t nw = (uint32_t)min((uint64_t)WARPS, max((uint64_t)1, per_cta));
-    const uint64_t chunk = (per_cta + nw - 1) / nw, cta_chunk = chunk * nw;
-    const uint64_t w0 = min(total, blockIdx.x * cta_chunk + (uint64_t)min(warp, nw) * chunk);
-    const uint64_t w1 = warp < nw ? min(total, w0 + chunk) : w0;
+    // this warp's stretch of the steps, n from w0 on, in the CTA's [c0, c1); fewer warps a CTA where there is little to do
+    const uint32_t per_cta = (total + gridDim.x - 1) / gridDim.x, nw = min((uint32_t)WARPS, max((uint32_t)MIN_WARPS, per_cta));
+    const uint32_t chunk = (per_cta + nw - 1) / nw, cta_chunk = chunk * nw;
+    const uint32_t c0 = min(total, blockIdx.x * cta_chunk), c1 = min(total, c0 + cta_chunk);
+    const uint32_t w0 = min(c1, c0 + min(warp, nw) * chunk), n = min(c1, w0 + chunk) - w0;
 
     uint8_t *ring = ring_all + warp * (STAGES * C::STAGE_BYTES);
     uint64_t *bar = bars + warp * STAGES;
 
-    auto seg_at = [&](uint64_t idx) {
+    // The segment of a step; steps * row tiles * heads of a request fit in 32 bits.
+    auto seg_at = [&](uint32_t idx) {
         uint32_t x = 0, y = a.n_req;
         while (y - x > 1) {
             const uint32_t m = (x + y) >> 1;
@@ -283,22 +292,19 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
         Seg s;
         s.req = x;
         s.r = reqs[x];
-        const uint32_t tiles = tiles_of(s.r);
-        const uint64_t rem = idx - pre[x], all = pre[x + 1] - pre[x];
+        const uint32_t tiles = max(1u, tiles_of(s.r));
         s.end = (int32_t)min((int64_t)s.r.seq, (int64_t)a.width << a.c.page_shift);
         s.steps = max(1u, (uint32_t)(s.end + STEP - 1) / STEP - s.r.s0);
-        uint64_t k;
-        if (all >> 32) k = rem / s.steps;
-        else k = (uint32_t)rem / s.steps;
-        s.head = tiles == 1 ? (uint32_t)k : (uint32_t)(k / tiles);
-        s.tile = (uint32_t)k - s.head * tiles;
+        const uint32_t k = (idx - pre[x]) / s.steps, h = tiles == 1 ? k : k / tiles;
+        s.head = a.head0 + min(h, a.n_kv - 1);
+        s.tile = k - h * tiles;
         s.begin = pre[x] + k * s.steps;
         return s;
     };
 
     // ---- the copies: a step at a time, the table entries of 32 pages in the lanes ----
-    const uint32_t n = (uint32_t)(w1 - w0);
-    uint32_t p_i = 0, p_end = 0, p_t = 0, p_page = 0, p_req = 0, p_head = 0;
+    Seg *segs = segs_all + warp * C::SEGS;
+    uint32_t p_i = 0, p_end = 0, p_seg = 0, p_t = 0, p_page = 0, p_req = 0, p_head = 0;
     int32_t p_blk = -1, p_seq = 0;
     bool dead = false;  // a wait ran out: no further copies
     auto pages = [&]() {
@@ -311,9 +317,11 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
         if (p_i >= n) return 0;
         if (p_i == p_end) {
             const Seg s = seg_at(w0 + p_i);
-            p_end = (uint32_t)min((uint64_t)n, s.begin + s.steps - w0);
+            if (lane == 0) segs[p_seg] = s;
+            if (++p_seg == C::SEGS) p_seg = 0;
+            p_end = min(n, s.begin + s.steps - w0);
             p_req = s.req, p_head = s.head, p_seq = s.end;
-            p_t = (s.r.s0 + (uint32_t)(w0 + p_i - s.begin)) * STEP;
+            p_t = (s.r.s0 + (w0 + p_i - s.begin)) * STEP;
             pages();
         }
         uint8_t *dst = ring + stage * C::STAGE_BYTES;
@@ -354,20 +362,19 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
         return there;
     };
     uint32_t there = 0;  // the bits of the steps in the ring, the next one's lowest
-#pragma unroll
-    for (int s = 0; s < STAGES; s++) there |= issue(s) << (s * TILES);
 
     // ---- the steps ----
     // Operands: scores are K codes (16 positions) times query rows (8), sums V codes (16 values) times weights
     // (8 rows), so that a lane of quad `quad` has rows 2 quad and 2 quad + 1 of every result.
     uint32_t qb[2 * G][QR], qs[G == 8 ? 2 : 1];
     float o[2 * G][4], om[4];
-    float m[2], l[2], cs[2];
+    float m[2], sh[2], cs[2];  // the weights' reference and its shift; what a score is multiplied by
+    const uint32_t ones = gid == 0 ? 0x3C003C00u : 0u;
     int32_t lo_t[2], hi_t[2], full_lo = 0, full_hi = 0;  // positions [lo, hi) that a row sees; that all rows see
     int32_t kexp = 15;   // of group lane % G: V scales are multiplied by 2^kexp
     uint32_t vlim2 = 0;  // and are at most this (f16x2)
     uint32_t kmul[G];    // f16x2 of each group's 2^kexp
-    uint32_t c_end = 0, phase = 0, stage = 0;
+    uint32_t c_end = 0, c_seg = 0, phase = 0, stage = 0;
     int32_t t0 = 0, held_end = 0;  // the step's first position, the positions held
     const uint32_t half_sel = gid & 1 ? 0x7632u : 0x5410u;
 
@@ -389,12 +396,15 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
     };
     auto lse_of = [](float mm, float ll) { return ll == 0.0f ? -INFINITY : (mm - P_SHIFT + log2f(ll)) * LN2; };
 
-    for (uint32_t idx = 0; idx < n; idx++, t0 += STEP) {
+    // the first STAGES turns only start copies
+    for (uint32_t turn = 0; turn < n + STAGES; turn++) {
+        const uint32_t idx = turn - STAGES;
+        if (turn >= STAGES) {
         if (idx == c_end) {
             // a new segment: its query rows as operand registers
-            const Seg seg = seg_at(w0 + idx);
-            c_end = (uint32_t)min((uint64_t)n, seg.begin + seg.steps - w0);
-            t0 = (int32_t)(seg.r.s0 + (uint32_t)(w0 + idx - seg.begin)) * STEP;
+            const Seg &seg = segs[c_seg];
+            c_end = min(n, seg.begin + seg.steps - w0);
+            t0 = (int32_t)(seg.r.s0 + (w0 + idx - seg.begin)) * STEP;
             held_end = seg.end;
             const uint32_t row = seg.tile * ROWS + gid, tok = row / a.group, hq = seg.head * a.group + row % a.group;
             const bool live = tok < (uint32_t)seg.r.nq;
@@ -412,34 +422,39 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
 #pragma unroll
                     for (int k = 0; k < 8; k++) raw[g][k] = q[g * 32 + k];
             }
-            float amax = 0.0f;
+            // q * 2^(14 - e) is below 2^15 in f16; e is kept where 2^(14 - e) and 2^(e + 10) are f32 numbers.
+            // A row that is no row stands in with the values of the first one.
+            int e;
+            if constexpr (Q32) {
+                float amax = 0.0f;
+#pragma unroll
+                for (int g = 0; g < G; g++)
+#pragma unroll
+                    for (int k = 0; k < 8; k++) amax = fmaxf(amax, fabsf(raw[g][k]));
+                amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
+                e = (int)(__float_as_uint(amax) >> 23) - 127;
+            } else {
+                uint32_t amax = 0;  // the bits without the sign have the order of the values
+#pragma unroll
+                for (int g = 0; g < G; g++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) amax = __vmaxu2(amax, reinterpret_cast<const uint32_t *>(raw[g])[k] & 0x7FFF7FFFu);
+                amax = __vmaxu2(amax, amax >> 16);
+                amax = __vmaxu2(amax, __shfl_xor_sync(~0u, amax, 1));
+                amax = __vmaxu2(amax, __shfl_xor_sync(~0u, amax, 2)) & 0x7FFFu;
+                e = std::is_same<T, __half>::value ? (int)(amax >> 10) - 15 : (int)(amax >> 7) - 127;
+            }
+            e = min(max(e, -100), 116);
+            const float up = copysignf(__uint_as_float((uint32_t)(127 + 14 - e) << 23), a.scale);
+            const float cs_row = fabsf(a.scale) * LOG2E * __uint_as_float((uint32_t)(127 + 10 + e) << 23);
+            const float up16 = up * 0.0625f;
 #pragma unroll
             for (int g = 0; g < G; g++)
 #pragma unroll
-                for (int k = 0; k < 8; k++) amax = fmaxf(amax, live ? fabsf(Act<T>::get(raw[g][k])) : 0.0f);
-            amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
-            // q * 2^(14 - e) is below 2^15 in f16; e is kept where 2^(14 - e) and 2^(e + 10) are f32 numbers
-            const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 116);
-            const float up = copysignf(__uint_as_float((uint32_t)(127 + 14 - e) << 23), a.scale);
-            const float cs_row = fabsf(a.scale) * LOG2E * __uint_as_float((uint32_t)(127 + 10 + e) << 23);
-            float sum[G];
-#pragma unroll
-            for (int g = 0; g < G; g++) {
-                float x[8];
-                sum[g] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    x[k] = live ? Act<T>::get(raw[g][k]) : 0.0f;
-                    sum[g] += x[k];
-                }
-                sum[g] += __shfl_xor_sync(~0u, sum[g], 1);
-                sum[g] += __shfl_xor_sync(~0u, sum[g], 2);
-                sum[g] *= up * 0.015625f;
                 // nibbles (0, 4), (1, 5), (2, 6), (3, 7) make the four K registers; those of odd ones are 16 c
-#pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const float f = k & 1 ? up * 0.0625f : up, x0 = x[k] * f, x1 = x[k + 4] * f;
+                    const float f = k & 1 ? up16 : up, x0 = Act<T>::get(raw[g][k]) * f, x1 = Act<T>::get(raw[g][k + 4]) * f;
                     const uint32_t hi = pack_h2(x0, x1);
                     qb[2 * g + (k >> 1)][k & 1] = hi;
                     if constexpr (Q32) {
@@ -447,22 +462,33 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
                         qb[2 * g + (k >> 1)][2 + (k & 1)] = pack_h2(x0 - h.x, x1 - h.y);
                     }
                 }
-            }
-            // sums of the query's groups against the K minima: column k holds group k % G, first the f16
-            // rounding, then what it left
+            // The sums of the query's groups, for the K minima: the product with codes of 1, in units of 2^-24.
+            // Column k of the operand holds group k % G, first the f16 rounding, then what it left.
+            {
+                float sum[2] = {0.0f, 0.0f};
+                uint32_t hi[2], lo[2];
 #pragma unroll
-            for (int w = 0; w < (G == 8 ? 2 : 1); w++) {
-                float v[2];
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const uint32_t k = w * 8 + quad * 2 + i, part = k / G, gg = k % G;
-                    float s = 0.0f;
-#pragma unroll
-                    for (int g = 0; g < G; g++) s = (uint32_t)g == gg ? sum[g] : s;
-                    const float h = __half2float(__float2half_rn(s));
-                    v[i] = part == 0 ? h : part == 1 ? s - h : 0.0f;
+                for (int g = 0; g < G; g++) {
+                    float d[4];
+                    constexpr uint32_t C0 = 0x00010001u, C1 = 0x00100010u;
+                    mma16_first(d, C0, C0, C1, C1, qb[2 * g][0], qb[2 * g][1]);
+                    mma16(d, C0, C0, C1, C1, qb[2 * g + 1][0], qb[2 * g + 1][1]);
+                    if constexpr (Q32) {
+                        mma16(d, C0, C0, C1, C1, qb[2 * g][2], qb[2 * g][3]);
+                        mma16(d, C0, C0, C1, C1, qb[2 * g + 1][2], qb[2 * g + 1][3]);
+                    }
+                    if ((int)(gid % G) == g) sum[0] = d[0], sum[1] = d[1];
                 }
-                qs[w] = pack_h2(v[0], v[1]);
+                const float f = 0x1p18f;  // 2^24 of the codes' unit, 2^-6 to stay inside f16
+                hi[0] = pack_h2(sum[0] * f, sum[1] * f);
+                const float2 h = unpack_h2(hi[0]);
+                lo[0] = pack_h2(fmaf(sum[0], f, -h.x), fmaf(sum[1], f, -h.y));
+                if constexpr (G == 8) {
+                    qs[0] = transpose8(hi[0]);
+                    qs[1] = transpose8(lo[0]);
+                } else {
+                    qs[0] = transpose8(gid < G ? hi[0] : gid < 2 * G ? lo[0] : 0u);
+                }
             }
             // what this row sees, and what every row of the tile sees
             const int64_t place = (int64_t)seg.r.seq - seg.r.nq + tok;
@@ -476,7 +502,7 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
                 cs[i] = __shfl_sync(~0u, cs_row, src);
                 hi_t[i] = __shfl_sync(~0u, hi_row, src);
                 lo_t[i] = __shfl_sync(~0u, lo_row, src);
-                m[i] = -INFINITY, l[i] = 0.0f;
+                m[i] = -INFINITY, sh[i] = 0.0f;
             }
             kexp = 15, vlim2 = 0x13FF13FFu;  // the f16 below 2^-10
 #pragma unroll
@@ -491,7 +517,7 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
             if (lane == 0) atomicExch(&g_dev_status, (unsigned)DEV_TIMEOUT_TMA);
         }
         dead = __any_sync(~0u, dead);
-        const uint8_t *buf = ring + stage * C::STAGE_BYTES;
+        uint8_t *buf = ring + stage * C::STAGE_BYTES;
         const uint32_t here = there & ((1u << TILES) - 1);
         // whole: every row sees every position of the step
         const bool whole = here == (1u << TILES) - 1 && t0 >= full_lo && t0 + STEP <= full_hi;
@@ -545,6 +571,19 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
                     const int32_t t = t0 + i * 16 + gid + (k >> 1) * 8;
                     if (t < lo_t[k & 1] || t >= hi_t[k & 1] || !(here >> i & 1)) s[i][k] = -INFINITY;
                 }
+            // the scales and minima of positions that are not held may be anything: zeros in their place
+#pragma unroll 1
+            for (int i = 0; i < TILES; i++) {
+                const int32_t held = here >> i & 1 ? held_end - (t0 + i * 16) : 0;
+                if (held >= 16) continue;
+                for (uint32_t k = lane; k < 16 * G; k += 32) {
+                    const int32_t t = (int32_t)(k % (8 * G) / G) * 2;
+                    uint32_t *w = reinterpret_cast<uint32_t *>(buf + i * L::BYTES + L::VS) + k;  // V scales, then V minima
+                    *w &= t + 1 < held ? 0xffffffffu : t < held ? 0xffffu : 0u;
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into this stage
+            __syncwarp();
         }
         float top[2];
         bool behind = false;
@@ -563,53 +602,25 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
                 for (int off = 4; off < 32; off <<= 1) top[r] = fmaxf(top[r], __shfl_xor_sync(~0u, top[r], off));
                 const float mm = fmaxf(m[r], top[r]), f = m[r] == mm ? 1.0f : ex2(m[r] - mm);
                 m[r] = mm;
-                l[r] *= f;
 #pragma unroll
                 for (int i = 0; i < 2 * G; i++) o[i][r] *= f, o[i][2 + r] *= f;
-                om[r] *= f;
+                om[r] *= f, om[2 + r] *= f;
+                sh[r] = mm == -INFINITY ? 0.0f : P_SHIFT - mm;
             }
         }
-        const float sh0 = m[0] == -INFINITY ? 0.0f : P_SHIFT - m[0], sh1 = m[1] == -INFINITY ? 0.0f : P_SHIFT - m[1];
 
-        // values
-#pragma unroll
-        for (int i = 0; i < TILES; i++) {
-            const uint8_t *tile = buf + i * L::BYTES;
-            // the weights, and as f16 rounding and rest, turned so that a lane has positions 2 quad + (0, 1) + 8 j of row gid
-            uint32_t ph[2], pl[2];
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const float p0 = ex2(fmaf(s[i][2 * j], cs[0], sh0)), p1 = ex2(fmaf(s[i][2 * j + 1], cs[1], sh1));
-                l[0] += p0, l[1] += p1;
-                ph[j] = pack_h2(p0, p1);
-                const float2 h = unpack_h2(ph[j]);
-                pl[j] = transpose8(pack_h2(p0 - h.x, p1 - h.y));
-                ph[j] = transpose8(ph[j]);
-            }
-            // positions of this tile that are held; the others' scales and minima may be anything
-            const int32_t held = here >> i & 1 ? held_end - (t0 + i * 16) : 0;
-            const bool part = held < 16;
-            // a V scale larger than any before: the group's sums move to a new power of two
-            constexpr int N = G == 8 ? 2 : 1;  // the tile's 8 G words of scales, lane l's of group l % G
-            uint32_t vw[N];
-            bool above = false;
+        // a V scale larger than any before: the group's sums move to a new power of two
+        {
+            constexpr int N = TILES * (G == 8 ? 2 : 1);  // the 8 G words of a tile's scales, lane l's of group l % G
+            uint32_t vw[N], wmax = vlim2;
 #pragma unroll
             for (int k = 0; k < N; k++) {
-                const uint32_t at = (lane + 32 * k) % (G * 8);
-                vw[k] = *reinterpret_cast<const uint32_t *>(tile + L::VS + at * 4);
-                if (part) {
-                    const int32_t t = (int32_t)(at / G) * 2;
-                    vw[k] &= t + 1 < held ? 0xffffffffu : t < held ? 0xffffu : 0u;
-                }
-                above |= any_gt_h2(vw[k], vlim2);
+                vw[k] = *reinterpret_cast<const uint32_t *>(buf + (k % TILES) * L::BYTES + L::VS + (lane + 32 * (k / TILES)) % (G * 8) * 4);
+                wmax = __vmaxu2(wmax, vw[k]);
             }
-            if (__any_sync(~0u, above)) {
-                float vmax = 0.0f;
-#pragma unroll
-                for (int k = 0; k < N; k++) {
-                    const float2 v = unpack_h2(vw[k]);
-                    vmax = fmaxf(vmax, fmaxf(v.x, v.y));
-                }
+            if (__any_sync(~0u, wmax != vlim2)) {
+                const float2 v = unpack_h2(wmax);  // at least the limit, which is below 2^(5 - kexp)
+                float vmax = fmaxf(v.x, v.y);
 #pragma unroll
                 for (int off = G; off < 32; off <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(~0u, vmax, off));
                 // 2^kexp times the largest scale is below 2^5 (kexp at most 15, f16's largest power of two)
@@ -626,23 +637,32 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
                     for (int k2 = 0; k2 < 4; k2++) o[2 * g][k2] *= f, o[2 * g + 1][k2] *= f;
                 }
             }
+        }
+
+        // values
+#pragma unroll
+        for (int i = 0; i < TILES; i++) {
+            const uint8_t *tile = buf + i * L::BYTES;
+            // the weights, and as f16 rounding and rest, turned so that a lane has positions 2 quad + (0, 1) + 8 j of row gid
+            uint32_t ph[2], pl[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float p0 = ex2(fmaf(s[i][2 * j], cs[0], sh[0])), p1 = ex2(fmaf(s[i][2 * j + 1], cs[1], sh[1]));
+                ph[j] = pack_h2(p0, p1);
+                const float2 h = unpack_h2(ph[j]);
+                pl[j] = transpose8(pack_h2(p0 - h.x, p1 - h.y));
+                ph[j] = transpose8(ph[j]);
+            }
             uint32_t vs[2][G], vm[2], v[2][G];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 lds_words<G>(vs[j], tile + L::VS + (4 * j + quad) * (G * 4));
                 vm[j] = *reinterpret_cast<const uint32_t *>(tile + L::VM + ((4 * j + quad) * G + gid % G) * 4);
                 lds_codes<G, 8>(v[j], tile + L::VC + (4 * j + quad) * L::VROW, gid);
-                if (part) {
-                    const int32_t t = 8 * j + 2 * quad;
-                    const uint32_t mask = t + 1 < held ? 0xffffffffu : t < held ? 0xffffu : 0u;
-                    vm[j] &= mask;
-#pragma unroll
-                    for (int g = 0; g < G; g++) vs[j][g] &= mask;
-                }
             }
-            // row gid of the minima's product is group gid % G
-            mma16(om, vm[0], 0, vm[1], 0, ph[0], ph[1]);
-            mma16(om, vm[0], 0, vm[1], 0, pl[0], pl[1]);
+            // row gid of this product is the minima of group gid % G, row 8 the sum of the weights
+            mma16(om, vm[0], ones, vm[1], ones, ph[0], ph[1]);
+            mma16(om, vm[0], ones, vm[1], ones, pl[0], pl[1]);
 #pragma unroll
             for (int g = 0; g < G; g++) {
                 uint32_t hi[2], lo[2];
@@ -651,7 +671,7 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
                     // (ph + pl) sc as the f16 rounding of ph sc and the rest
                     const uint32_t sc = mul_h2(vs[j][g], kmul[g]);
                     hi[j] = mul_h2(ph[j], sc);
-                    lo[j] = fma_h2(pl[j], sc, fma_h2(ph[j], sc, hi[j] ^ 0x80008000u));
+                    lo[j] = fma_h2(pl[j], sc, fms_h2(ph[j], sc, hi[j]));
                 }
                 const uint32_t h0 = v[0][g] >> 8, h1 = v[1][g] >> 8;
                 mma16(o[2 * g], v[0][g] & 0x000F000Fu, v[0][g] & 0x00F000F0u, v[1][g] & 0x000F000Fu, v[1][g] & 0x00F000F0u, hi[0], hi[1]);
@@ -661,25 +681,23 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
             }
         }
 
-        // the stage is read: the next copy into it
+        t0 += STEP;
+        }
+        // the stage is read (or empty): the next copy into it
         __syncwarp();
         there = there >> TILES | issue(stage) << ((STAGES - 1) * TILES);
-        if (++stage == STAGES) stage = 0, phase ^= 1;
+        if (++stage == STAGES) stage = 0, phase ^= turn >= STAGES;
 
-        if (idx + 1 == c_end) {
+        if (turn >= STAGES && idx + 1 == c_end) {
             // the end of the segment, or of this warp's part of it
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) {
-                l[0] += __shfl_xor_sync(~0u, l[0], off);
-                l[1] += __shfl_xor_sync(~0u, l[1], off);
-            }
+            const float l[2] = {__shfl_sync(~0u, om[2], quad), __shfl_sync(~0u, om[3], quad)};
             float r[G][2][4];
             rows_of(r);
-            const Seg seg = seg_at(w0 + idx);
-            const bool begins = seg.begin >= w0, ends = seg.begin + seg.steps <= w1;
+            const Seg &seg = segs[c_seg];
+            const bool begins = seg.begin >= w0, ends = seg.begin + seg.steps <= w0 + n;
             // a part that began before this warp (at most one) and one that goes on after it (at most one) are left for the joins
             float *part = begins ? reinterpret_cast<float *>(ring) : first_all + warp * (C::PART_BYTES / 4);
-            if (lane == 0 && !(begins && ends)) seg_begin[2 * warp + begins] = seg.begin;
+            if (lane == 0 && !(begins && ends)) seg_begin[2 * warp + begins] = seg.begin, part_seg[2 * warp + begins] = seg;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const uint32_t tr = 2 * quad + i;
@@ -699,6 +717,7 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
                 for (int g = 0; g < G; g++) put4(out + g * 32, r[g][i][0] * inv, r[g][i][1] * inv, r[g][i][2] * inv, r[g][i][3] * inv, a.vec_out);
                 if (a.lse && gid == 0) a.lse[t * a.n_heads + hq] = lse_of(m[i], l[i]);
             }
+            if (++c_seg == C::SEGS) c_seg = 0;
         }
     }
     if (dead) {  // copies still in flight must not land in memory that is used for something else
@@ -706,97 +725,135 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
     }
     __syncthreads();
 
-    // ---- joining the CTA's partial results, segment by segment ----
+    // ---- joining the CTA's partial results: a warp per (segment, row), a lane per part for the weights ----
     uint32_t *counters = reinterpret_cast<uint32_t *>(a.scratch);
     float *parts = reinterpret_cast<float *>(a.scratch + 4096);
-    constexpr uint32_t PART = C::PART_BYTES / 4;
-    auto slot = [&](uint32_t k) -> const float * {
-        return k & 1 ? reinterpret_cast<const float *>(ring_all + (k >> 1) * (STAGES * C::STAGE_BYTES)) : first_all + (k >> 1) * PART;
-    };
-    const uint64_t c0 = min(total, blockIdx.x * cta_chunk), c1 = min(total, c0 + cta_chunk);
-    for (uint32_t k0 = 0; k0 < 2 * WARPS;) {
-        const uint64_t sb = seg_begin[k0];
-        if (sb == ~0ull) {
-            k0++;
-            continue;
+    constexpr uint32_t PART = C::PART_BYTES / 4, V = D / 32;
+    // The row's values in a lane: V of them, in twos (D = 64) or fours, 32 lanes apart.
+    constexpr uint32_t W = V < 4 ? V : 4;
+    auto at_of = [&](uint32_t k) { return k / W * (W * 32) + lane * W + k % W; };
+    auto get_row = [&](float (&x)[V], const float *p) {
+        if constexpr (W == 2) {
+            const float2 y = *reinterpret_cast<const float2 *>(p + lane * 2);
+            x[0] = y.x, x[1] = y.y;
+        } else {
+#pragma unroll
+            for (int k = 0; k < (int)V; k += 4) {
+                const float4 y = *reinterpret_cast<const float4 *>(p + k * 32 + lane * 4);
+                x[k] = y.x, x[k + 1] = y.y, x[k + 2] = y.z, x[k + 3] = y.w;
+            }
         }
-        uint32_t k1 = k0 + 1;
-        while (k1 < 2 * WARPS && (seg_begin[k1] == sb || seg_begin[k1] == ~0ull)) k1++;
-        const Seg sg_ = seg_at(sb);
-        const uint64_t se = sb + sg_.steps;
-        const bool all_here = sb >= c0 && se <= c1;
-        const uint32_t cb = (uint32_t)(sb / cta_chunk), ce = (uint32_t)((se - 1) / cta_chunk);
-        // Joins the rows of n partial results: the weights of each row by a warp, then a thread per four values
-        // with several of the parts' loads in flight.
-        auto join_out = [&](uint32_t n, auto part, auto ld4, auto ld, bool final_, float *dst) {
-            for (uint32_t row = warp; row < ROWS; row += WARPS) {
-                float mm = -INFINITY;
-                for (uint32_t i = lane; i < n; i += 32) {
-                    const float *p = part(i);
-                    const float v = p ? ld(p + ROWS * D + row) : -INFINITY;
-                    weight_s[i * ROWS + row] = v;
-                    mm = fmaxf(mm, v);
-                }
+    };
+    auto warp_max = [](float v) {
 #pragma unroll
-                for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(~0u, mm, o));
-                float ll = 0.0f;
-                for (uint32_t i = lane; i < n; i += 32) {
-                    const float *p = part(i);
-                    const float mi = weight_s[i * ROWS + row], w = !p ? 0.0f : mi == mm ? 1.0f : ex2(mi - mm);
-                    weight_s[i * ROWS + row] = w;
-                    if (p) ll = fmaf(w, ld(p + ROWS * D + ROWS + row), ll);
-                }
+        for (int off = 16; off; off >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, off));
+        return v;
+    };
+    auto warp_sum = [](float v) {
 #pragma unroll
-                for (int o = 16; o; o >>= 1) ll += __shfl_xor_sync(~0u, ll, o);
-                if (lane == 0) ml_s[row] = mm, ml_s[ROWS + row] = ll;
-            }
-            __syncthreads();
-            for (uint32_t e = tid * 4; e < ROWS * D; e += WARPS * 128) {
-                const uint32_t row = e / D, d = e % D;
-                float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                for (uint32_t i = 0; i < n; i++) {
-                    const float *p = part(i);
-                    const float w = weight_s[i * ROWS + row];
-                    const float4 v = p ? ld4(p + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    acc.x = fmaf(w, v.x, acc.x), acc.y = fmaf(w, v.y, acc.y), acc.z = fmaf(w, v.z, acc.z), acc.w = fmaf(w, v.w, acc.w);
-                }
-                const float mm = ml_s[row], ll = ml_s[ROWS + row];
-                if (!final_) {
-                    *reinterpret_cast<float4 *>(dst + e) = acc;
-                    if (d == 0) dst[ROWS * D + row] = mm, dst[ROWS * D + ROWS + row] = ll;
-                    continue;
-                }
-                const uint32_t rr = sg_.tile * ROWS + row, tok = rr / a.group, hq = sg_.head * a.group + rr % a.group;
-                if (tok >= (uint32_t)sg_.r.nq) continue;
-                const uint64_t t = (uint64_t)sg_.r.tok0 + tok;
-                const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-                put4((T *)a.out + t * a.o_tok + hq * a.o_head + d, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv, a.vec_out);
-                if (a.lse && d == 0) a.lse[t * a.n_heads + hq] = lse_of(mm, ll);
-            }
-        };
-        auto in_smem = [&](uint32_t i) -> const float * { return seg_begin[k0 + i] == sb ? slot(k0 + i) : nullptr; };
-        float *mine = parts + (uint64_t)(blockIdx.x * 2 + (sb < c0 ? 0 : 1)) * PART;
-        join_out(k1 - k0, in_smem, [](const float *p) { return *reinterpret_cast<const float4 *>(p); },
-                 [](const float *p) { return *p; }, all_here, mine);
-        if (!all_here) {
+        for (int off = 16; off; off >>= 1) v += __shfl_xor_sync(~0u, v, off);
+        return v;
+    };
+    const uint32_t mine = seg_begin[lane];  // the parts, in order; a segment's are neighbours
+    const uint32_t valid = __ballot_sync(~0u, mine != NONE), before = valid & ((1u << lane) - 1);
+    if (!valid) return;
+    const uint32_t prev = __shfl_sync(~0u, mine, before ? 31 - __clz(before) : 0);
+    const uint32_t leads = __ballot_sync(~0u, mine != NONE && (!before || prev != mine));
+    // the segments that other CTAs have parts of too: the one that began before this CTA, the one that goes on after it
+    const Seg &edge0 = part_seg[__ffs(valid) - 1], &edge1 = part_seg[31 - __clz(valid)];
+    const bool has0 = edge0.begin < c0, has1 = edge1.begin >= c0 && edge1.begin + edge1.steps > c1;
+    // First the parts in this CTA, segment by segment; then, in the CTA that comes last to a segment, those of all CTAs.
+#pragma unroll 1
+    for (uint32_t pass = 0; pass < 2; pass++) {
+        if (pass) {
+            if (!has0 && !has1) return;
             __threadfence();
             __syncthreads();
-            if (tid == 0) {
-                const uint32_t before = atomicAdd(&counters[cb], 1u);
-                *flag_s = before == ce - cb;
-                if (before == ce - cb) counters[cb] = 0;
+            if (tid < 2) {
+                flag_s[tid] = 0;
+                if (tid ? has1 : has0) {
+                    const Seg &sg_ = tid ? edge1 : edge0;
+                    const uint32_t cb = sg_.begin / cta_chunk, ce = (sg_.begin + sg_.steps - 1) / cta_chunk;
+                    const uint32_t arrived = atomicAdd(&counters[cb], 1u);
+                    flag_s[tid] = arrived == ce - cb;
+                    if (arrived == ce - cb) counters[cb] = 0;  // nobody else comes: ready for the next call
+                }
             }
             __syncthreads();
-            if (*flag_s) {
-                __threadfence();
-                auto in_scratch = [&](uint32_t i) -> const float * { return parts + (uint64_t)((cb + i) * 2 + (i ? 0 : 1)) * PART; };
-                join_out(ce - cb + 1, in_scratch, [](const float *p) { return __ldcg(reinterpret_cast<const float4 *>(p)); },
-                         [](const float *p) { return __ldcg(p); }, true, nullptr);
-            }
+            __threadfence();
         }
-        __syncthreads();
-        k0 = k1;
+        const uint32_t units = pass ? 2 * ROWS : __popc(leads) * ROWS;
+#pragma unroll 1
+        for (uint32_t u = warp; u < units; u += WARPS) {
+            const uint32_t row = u % ROWS;
+            uint32_t these = 0, count = 32, cb = 0;
+            const Seg *of;
+            if (pass == 0) {
+                uint32_t lead = leads;
+                for (uint32_t k = u / ROWS; k; k--) lead &= lead - 1;
+                const uint32_t rest = lead & (lead - 1);
+                these = valid & (rest ? (rest & (0u - rest)) - 1 : ~0u) & ~((lead & (0u - lead)) - 1);
+                of = part_seg + __ffs(lead) - 1;
+            } else {
+                if (!flag_s[u / ROWS]) continue;
+                of = u / ROWS ? &edge1 : &edge0;
+                cb = of->begin / cta_chunk;
+                count = (of->begin + of->steps - 1) / cta_chunk - cb + 1;
+            }
+            // part i of the segment, or none
+            auto part = [&](uint32_t i) -> const float * {
+                if (pass) return i < count ? parts + (uint64_t)((cb + i) * 2 + (i ? 0 : 1)) * PART : nullptr;
+                if (!(these >> i & 1)) return nullptr;
+                return i & 1 ? reinterpret_cast<const float *>(ring_all + (i >> 1) * (STAGES * C::STAGE_BYTES)) : first_all + (i >> 1) * PART;
+            };
+            // 32 parts at a time: a lane per part for maximum and sum, then their values, several loads in flight
+            float mm = -INFINITY, ll = 0.0f, acc[V] = {};
+#pragma unroll 1
+            for (uint32_t i0 = 0; i0 < count; i0 += 32) {
+                const float *p = part(i0 + lane);
+                const float mi = p ? p[ROWS * D + row] : -INFINITY, li = p ? p[ROWS * D + ROWS + row] : 0.0f;
+                const float top = fmaxf(mm, warp_max(mi)), f = mm == top ? 1.0f : ex2(mm - top), w = !p ? 0.0f : mi == top ? 1.0f : ex2(mi - top);
+                mm = top;
+                ll = fmaf(w, li, ll * f);
+#pragma unroll
+                for (int v = 0; v < (int)V; v++) acc[v] *= f;
+                constexpr int N = V == 8 ? 4 : 8;
+                for (uint32_t left = __ballot_sync(~0u, p != nullptr); left;) {
+                    float x[N][V], wq[N];
+#pragma unroll
+                    for (int k = 0; k < N; k++) {
+                        const int i = left ? __ffs(left) - 1 : -1;
+                        const float *q = reinterpret_cast<const float *>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(p), i & 31));
+                        wq[k] = __shfl_sync(~0u, w, i & 31);
+#pragma unroll
+                        for (int v = 0; v < (int)V; v++) x[k][v] = 0.0f;
+                        if (i >= 0) get_row(x[k], q + row * D);
+                        left &= left - 1;
+                    }
+#pragma unroll
+                    for (int k = 0; k < N; k++)
+#pragma unroll
+                        for (int v = 0; v < (int)V; v++) acc[v] = fmaf(wq[k], x[k][v], acc[v]);
+                }
+            }
+            ll = warp_sum(ll);
+            const Seg &sg_ = *of;
+            if (pass == 0 && (sg_.begin < c0 || sg_.begin + sg_.steps > c1)) {
+                float *dst = parts + (uint64_t)(blockIdx.x * 2 + (sg_.begin < c0 ? 0 : 1)) * PART;
+#pragma unroll
+                for (int k = 0; k < (int)V; k++) dst[row * D + at_of(k)] = acc[k];
+                if (lane == 0) dst[ROWS * D + row] = mm, dst[ROWS * D + ROWS + row] = ll;
+                continue;
+            }
+            const uint32_t rr = sg_.tile * ROWS + row, tok = rr / a.group, hq = sg_.head * a.group + rr % a.group;
+            if (tok >= (uint32_t)sg_.r.nq) continue;
+            const uint64_t t = (uint64_t)sg_.r.tok0 + tok;
+            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+            T *out = (T *)a.out + t * a.o_tok + hq * a.o_head;
+#pragma unroll
+            for (int k = 0; k < (int)V; k++) out[at_of(k)] = Act<T>::put(acc[k] * inv);
+            if (a.lse && lane == 0) a.lse[t * a.n_heads + hq] = lse_of(mm, ll);
+        }
     }
 }
 
@@ -812,16 +869,22 @@ sg_status launch(const Kv4AttnArgs &a0, int sms, cudaStream_t s, cudaError_t *er
         if ((*err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM)) != cudaSuccess) return SG_ERR_CUDA;
         ready[dev & 63] = true;
     }
-    const uint32_t grid = (uint32_t)sms < MAX_CTAS ? (uint32_t)sms : MAX_CTAS;
-    // MAX_REQ requests a launch; the tokens of no request are those after the last one's
-    for (uint32_t r0 = 0; r0 == 0 || r0 < a0.n_req; r0 += MAX_REQ) {
-        Kv4AttnArgs a = a0;
-        a.n_req = a0.n_req - r0 < MAX_REQ ? a0.n_req - r0 : MAX_REQ;
-        if (r0) a.cu += r0, a.seq += r0, a.tables += (uint64_t)r0 * a.ld_tables;
-        a.last = r0 + a.n_req == a0.n_req;
-        fn<<<grid, Cfg<D>::WARPS * 32, Cfg<D>::SMEM, s>>>(a);
-        if ((*err = cudaGetLastError()) != cudaSuccess) return SG_ERR_CUDA;
-    }
+    const uint32_t grid = (uint32_t)sms < MAX_CTAS ? (uint32_t)sms : MAX_CTAS, all = a0.c.heads;
+    // MAX_REQ requests a launch, and as many heads as keep the number of steps below 2^32
+    const uint64_t rows = (uint64_t)a0.n_tok * a0.group / ROWS + a0.n_req, steps = (((uint64_t)a0.width << a0.c.page_shift) + Cfg<D>::STEP - 1) / Cfg<D>::STEP + 1;
+    const uint64_t heads = (1ull << 31) / (rows * steps);
+    if (heads == 0) return SG_ERR_SHAPE;
+    for (uint32_t r0 = 0; r0 == 0 || r0 < a0.n_req; r0 += MAX_REQ)
+        for (uint32_t h0 = 0; h0 < all; h0 += (uint32_t)(heads < all ? heads : all)) {
+            Kv4AttnArgs a = a0;
+            a.n_req = a0.n_req - r0 < MAX_REQ ? a0.n_req - r0 : MAX_REQ;
+            if (r0) a.cu += r0, a.seq += r0, a.tables += (uint64_t)r0 * a.ld_tables;
+            a.last = r0 + a.n_req == a0.n_req;
+            a.head0 = h0;
+            a.n_kv = (uint32_t)(all - h0 < heads ? all - h0 : heads);
+            fn<<<grid, Cfg<D>::WARPS * 32, Cfg<D>::SMEM, s>>>(a);
+            if ((*err = cudaGetLastError()) != cudaSuccess) return SG_ERR_CUDA;
+        }
     return SG_OK;
 }
 
