@@ -151,13 +151,13 @@ constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
 constexpr float P_SHIFT = 2.0f, LAG = 8.0f;
 constexpr int ROWS = 8;
 constexpr uint32_t MAX_REQ = 1024;  // requests of one launch (their steps are in shared memory)
-constexpr uint32_t MAX_CTAS = 320;
+constexpr uint32_t MAX_CTAS = 192;
 constexpr uint32_t MIN_WARPS = 4;   // warps that a CTA uses at least, where the steps are few
 
-template <int D>
+template <typename T, int D>
 struct Cfg {
-    // D = 256 holds 128 sums a lane: 8 warps of at most 255 registers, steps of one tile
-    static constexpr int WARPS = D == 256 ? 8 : 12;
+    // As many warps as their sums and query registers leave room for (65536 registers): 128 a lane for 16 of them
+    static constexpr int WARPS = D == 256 ? 8 : D == 128 && sizeof(T) == 4 ? 12 : 16;
     static constexpr int TILES = D == 256 ? 1 : 2;
     static constexpr int STAGES = D == 256 ? 3 : 2;
     static constexpr int STEP = TILES * 16;
@@ -165,13 +165,16 @@ struct Cfg {
     static constexpr uint32_t PART_BYTES = ROWS * D * 4 + 2 * ROWS * 4;  // rows, m, l
     static constexpr uint32_t RING = WARPS * STAGES * STAGE_BYTES;
     static constexpr int SEGS = STAGES + 1;
-    static constexpr uint32_t SMEM = RING + WARPS * PART_BYTES + (MAX_REQ + 1) * 4 + MAX_REQ * 16 + WARPS * (STAGES * 8 + (SEGS + 2) * 40 + 4) + 512;
+    static constexpr uint32_t SMEM = RING + (MAX_REQ + 1) * 4 + MAX_REQ * 16 + WARPS * (STAGES * 8 + 2 * 8 + (SEGS + 2) * 40 + 4) + 512;
     static_assert(WARPS <= 16, "a lane per partial result");
     static_assert(STAGES * STAGE_BYTES >= PART_BYTES, "a warp's last partial result lies in its ring");
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
-constexpr uint32_t PART_MAX = Cfg<256>::PART_BYTES;
-static_assert(4096 + (uint64_t)MAX_CTAS * 2 * PART_MAX <= KV4_SCRATCH_BYTES, "scratch");
+// Scratch: arrival counters, two partial results a CTA for the segments that go over its ends, and one a warp for a
+// segment that ends in the middle of the warp's work.
+constexpr uint64_t PART_MAX = Cfg<float, 256>::PART_BYTES;
+static_assert(4096 + MAX_CTAS * (2 + 8) * PART_MAX <= KV4_SCRATCH_BYTES, "scratch");
+static_assert(4096 + (uint64_t)MAX_CTAS * (2 + 16) * Cfg<__half, 128>::PART_BYTES <= KV4_SCRATCH_BYTES, "scratch");
 
 // One request: its steps are the same for each of its heads and row tiles.
 struct Req {
@@ -205,17 +208,17 @@ struct Seg {
 }  // namespace
 
 template <typename T, int D>
-__global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
+__global__ void __launch_bounds__(Cfg<T, D>::WARPS * 32, 1) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
     using L = Kv4Tile<D>;
-    using C = Cfg<D>;
+    using C = Cfg<T, D>;
     constexpr int G = L::G, TILES = C::TILES, STAGES = C::STAGES, STEP = C::STEP, WARPS = C::WARPS;
     constexpr bool Q32 = sizeof(T) == 4;
     constexpr int QR = Q32 ? 4 : 2;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring_all = smem;
-    float *first_all = reinterpret_cast<float *>(smem + C::RING);
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::RING + WARPS * C::PART_BYTES);
-    Req *reqs = reinterpret_cast<Req *>(bars + WARPS * STAGES);       // [n_req]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::RING);
+    const float **part_at = reinterpret_cast<const float **>(bars + WARPS * STAGES);  // [2 * WARPS] the partial results
+    Req *reqs = reinterpret_cast<Req *>(part_at + 2 * WARPS);         // [n_req]
     Seg *segs_all = reinterpret_cast<Seg *>(reqs + MAX_REQ);          // [WARPS][SEGS] the segments in a warp's ring
     Seg *part_seg = segs_all + WARPS * C::SEGS;                       // [2 * WARPS] the partial results' segments
     uint32_t *pre = reinterpret_cast<uint32_t *>(part_seg + 2 * WARPS);  // [n_req + 1] steps before each request
@@ -304,64 +307,72 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
 
     // ---- the copies: a step at a time, the table entries of 32 pages in the lanes ----
     Seg *segs = segs_all + warp * C::SEGS;
-    uint32_t p_i = 0, p_end = 0, p_seg = 0, p_t = 0, p_page = 0, p_req = 0, p_head = 0;
-    int32_t p_blk = -1, p_seq = 0;
+    uint32_t p_left = n, p_run = 0, p_end = 0, p_seg = 0, p_t = 0, p_page = 0;  // steps left; left in this page; in this segment
+    int32_t p_blk = -1;
+    const uint8_t *p_src = nullptr;
+    uint32_t p_there = 0;
     bool dead = false;  // a wait ran out: no further copies
-    auto pages = [&]() {
-        p_page = p_t >> a.c.page_shift;
-        const uint64_t page = (uint64_t)p_page + lane;
-        p_blk = (int64_t)(page << a.c.page_shift) < p_seq ? __ldg(a.tables + (uint64_t)p_req * a.ld_tables + page) : -1;
+    // the step at p_t begins a page or a segment: where its positions lie
+    auto locate = [&]() {
+        const uint32_t shift = a.c.page_shift;
+        bool load = (p_t >> shift) - p_page >= 32;
+        if (p_end == 0) {
+            const uint32_t idx = w0 + n - p_left;
+            const Seg s = seg_at(idx);
+            if (lane == 0) segs[p_seg] = s;
+            if (++p_seg == C::SEGS) p_seg = 0;
+            p_end = min(p_left, s.begin + s.steps - idx);
+            p_t = (s.r.s0 + (idx - s.begin)) * STEP;
+            load = true;
+        }
+        const Seg &s = segs[p_seg ? p_seg - 1 : C::SEGS - 1];
+        if (load) {
+            __syncwarp();
+            p_page = p_t >> shift;
+            const uint64_t page = (uint64_t)p_page + lane;
+            p_blk = (int64_t)(page << shift) < s.end ? __ldg(a.tables + (uint64_t)s.req * a.ld_tables + page) : -1;
+        }
+        const uint32_t blk = (uint32_t)__shfl_sync(~0u, p_blk, (p_t >> shift) - p_page), at = p_t & ((1u << shift) - 1);
+        p_there = blk < a.c.n_blocks;
+        p_src = a.c.data + blk * a.block_bytes + (((uint64_t)s.head << (shift - 4)) + (at >> 4)) * L::BYTES;
+        p_run = min(p_end, max(1u, ((1u << shift) - at) / STEP));
     };
     // copies the next step into a stage; returns a bit per tile that is there
     auto issue = [&](uint32_t stage) -> uint32_t {
-        if (p_i >= n) return 0;
-        if (p_i == p_end) {
-            const Seg s = seg_at(w0 + p_i);
-            if (lane == 0) segs[p_seg] = s;
-            if (++p_seg == C::SEGS) p_seg = 0;
-            p_end = min(n, s.begin + s.steps - w0);
-            p_req = s.req, p_head = s.head, p_seq = s.end;
-            p_t = (s.r.s0 + (w0 + p_i - s.begin)) * STEP;
-            pages();
-        }
+        if (p_left == 0) return 0;
+        if (p_run == 0) locate();
         uint8_t *dst = ring + stage * C::STAGE_BYTES;
-        uint32_t there = 0;
-        const uint32_t shift = a.c.page_shift;
-        const uint64_t head_off = ((uint64_t)p_head << (shift - 4)) * L::BYTES;
-        if ((1u << shift) >= STEP) {  // the step lies in one page
-            if ((p_t >> shift) - p_page >= 32) pages();
-            const uint32_t blk = (uint32_t)__shfl_sync(~0u, p_blk, (p_t >> shift) - p_page);
-            there = blk < a.c.n_blocks ? (1u << TILES) - 1 : 0;
+        uint32_t there = p_there;
+        if (TILES == 1 || a.c.page_shift > 4) {  // the step lies in one page
+            there = p_there ? (1u << TILES) - 1 : 0;
             if (lane == 0 && !dead) {
                 mbar_arrive_expect_tx(&bar[stage], there ? C::STAGE_BYTES : 0);
-                if (there)
-                    bulk_g2s(dst, a.c.data + blk * a.block_bytes + head_off + ((p_t & ((1u << shift) - 1)) >> 4) * L::BYTES, C::STAGE_BYTES,
-                             &bar[stage]);
+                if (there) bulk_g2s(dst, p_src, C::STAGE_BYTES, &bar[stage]);
             }
         } else {  // a page per tile
-            uint32_t blk[TILES];
-#pragma unroll
-            for (int i = 0; i < TILES; i++) {
-                if ((p_t >> 4) + i - p_page >= 32) {
-                    p_t += 16 * i;
-                    pages();
-                    p_t -= 16 * i;
-                }
-                blk[i] = (uint32_t)__shfl_sync(~0u, p_blk, (p_t >> 4) + i - p_page);
-                there |= (blk[i] < a.c.n_blocks) << i;
-            }
+            const uint8_t *src0 = p_src;
+            p_t += 16;
+            locate();
+            p_t -= 16;
+            there |= p_there << 1;
             if (lane == 0 && !dead) {
                 mbar_arrive_expect_tx(&bar[stage], __popc(there) * L::BYTES);
-#pragma unroll
-                for (int i = 0; i < TILES; i++)
-                    if (there >> i & 1) bulk_g2s(dst + i * L::BYTES, a.c.data + blk[i] * a.block_bytes + head_off, L::BYTES, &bar[stage]);
+                if (there & 1) bulk_g2s(dst, src0, L::BYTES, &bar[stage]);
+                if (there & 2) bulk_g2s(dst + L::BYTES, p_src, L::BYTES, &bar[stage]);
             }
         }
-        p_i++;
+        p_left--, p_end--, p_run--;
+        p_src += C::STAGE_BYTES;
         p_t += STEP;
         return there;
     };
     uint32_t there = 0;  // the bits of the steps in the ring, the next one's lowest
+#pragma unroll 1
+    for (int s = 0; s < STAGES; s++) there |= issue(s) << (s * TILES);
+
+    uint32_t *counters = reinterpret_cast<uint32_t *>(a.scratch);
+    float *parts = reinterpret_cast<float *>(a.scratch + 4096);
+    constexpr uint32_t PART = C::PART_BYTES / 4;
 
     // ---- the steps ----
     // Operands: scores are K codes (16 positions) times query rows (8), sums V codes (16 values) times weights
@@ -396,10 +407,7 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
     };
     auto lse_of = [](float mm, float ll) { return ll == 0.0f ? -INFINITY : (mm - P_SHIFT + log2f(ll)) * LN2; };
 
-    // the first STAGES turns only start copies
-    for (uint32_t turn = 0; turn < n + STAGES; turn++) {
-        const uint32_t idx = turn - STAGES;
-        if (turn >= STAGES) {
+    for (uint32_t idx = 0; idx < n; idx++, t0 += STEP) {
         if (idx == c_end) {
             // a new segment: its query rows as operand registers
             const Seg &seg = segs[c_seg];
@@ -516,7 +524,6 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
             dead = true;
             if (lane == 0) atomicExch(&g_dev_status, (unsigned)DEV_TIMEOUT_TMA);
         }
-        dead = __any_sync(~0u, dead);
         uint8_t *buf = ring + stage * C::STAGE_BYTES;
         const uint32_t here = there & ((1u << TILES) - 1);
         // whole: every row sees every position of the step
@@ -681,14 +688,12 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
             }
         }
 
-        t0 += STEP;
-        }
-        // the stage is read (or empty): the next copy into it
+        // the stage is read: the next copy into it
         __syncwarp();
         there = there >> TILES | issue(stage) << ((STAGES - 1) * TILES);
-        if (++stage == STAGES) stage = 0, phase ^= turn >= STAGES;
+        if (++stage == STAGES) stage = 0, phase ^= 1;
 
-        if (turn >= STAGES && idx + 1 == c_end) {
+        if (idx + 1 == c_end) {
             // the end of the segment, or of this warp's part of it
             const float l[2] = {__shfl_sync(~0u, om[2], quad), __shfl_sync(~0u, om[3], quad)};
             float r[G][2][4];
@@ -696,8 +701,12 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
             const Seg &seg = segs[c_seg];
             const bool begins = seg.begin >= w0, ends = seg.begin + seg.steps <= w0 + n;
             // a part that began before this warp (at most one) and one that goes on after it (at most one) are left for the joins
-            float *part = begins ? reinterpret_cast<float *>(ring) : first_all + warp * (C::PART_BYTES / 4);
-            if (lane == 0 && !(begins && ends)) seg_begin[2 * warp + begins] = seg.begin, part_seg[2 * warp + begins] = seg;
+            float *part = idx + 1 == n ? reinterpret_cast<float *>(ring) : parts + (uint64_t)(2 * MAX_CTAS + blockIdx.x * WARPS + warp) * PART;
+            if (lane == 0 && !(begins && ends)) {
+                seg_begin[2 * warp + begins] = seg.begin;
+                part_seg[2 * warp + begins] = seg;
+                part_at[2 * warp + begins] = part;
+            }
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const uint32_t tr = 2 * quad + i;
@@ -726,9 +735,7 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
     __syncthreads();
 
     // ---- joining the CTA's partial results: a warp per (segment, row), a lane per part for the weights ----
-    uint32_t *counters = reinterpret_cast<uint32_t *>(a.scratch);
-    float *parts = reinterpret_cast<float *>(a.scratch + 4096);
-    constexpr uint32_t PART = C::PART_BYTES / 4, V = D / 32;
+    constexpr uint32_t V = D / 32;
     // The row's values in a lane: V of them, in twos (D = 64) or fours, 32 lanes apart.
     constexpr uint32_t W = V < 4 ? V : 4;
     auto at_of = [&](uint32_t k) { return k / W * (W * 32) + lane * W + k % W; };
@@ -786,49 +793,45 @@ __global__ void __launch_bounds__(Cfg<D>::WARPS * 32, 1) kv4_attn_kernel(const _
 #pragma unroll 1
         for (uint32_t u = warp; u < units; u += WARPS) {
             const uint32_t row = u % ROWS;
-            uint32_t these = 0, count = 32, cb = 0;
+            uint32_t at = 0, count, cb = 0;  // pass 0: the first part's slot; its first CTA
             const Seg *of;
             if (pass == 0) {
                 uint32_t lead = leads;
                 for (uint32_t k = u / ROWS; k; k--) lead &= lead - 1;
-                const uint32_t rest = lead & (lead - 1);
-                these = valid & (rest ? (rest & (0u - rest)) - 1 : ~0u) & ~((lead & (0u - lead)) - 1);
-                of = part_seg + __ffs(lead) - 1;
+                const uint32_t rest = lead & (lead - 1), these = valid & (rest ? (rest & (0u - rest)) - 1 : ~0u) & ~((lead & (0u - lead)) - 1);
+                at = __ffs(lead) - 1;
+                of = part_seg + at;
+                count = __popc(these);  // the first warp's slot, then the even slots of the warps after it
             } else {
                 if (!flag_s[u / ROWS]) continue;
                 of = u / ROWS ? &edge1 : &edge0;
                 cb = of->begin / cta_chunk;
                 count = (of->begin + of->steps - 1) / cta_chunk - cb + 1;
             }
-            // part i of the segment, or none
             auto part = [&](uint32_t i) -> const float * {
-                if (pass) return i < count ? parts + (uint64_t)((cb + i) * 2 + (i ? 0 : 1)) * PART : nullptr;
-                if (!(these >> i & 1)) return nullptr;
-                return i & 1 ? reinterpret_cast<const float *>(ring_all + (i >> 1) * (STAGES * C::STAGE_BYTES)) : first_all + (i >> 1) * PART;
+                return pass ? parts + (uint64_t)((cb + i) * 2 + (i ? 0 : 1)) * PART : part_at[i ? (at & ~1u) + 2 * i : at];
             };
             // 32 parts at a time: a lane per part for maximum and sum, then their values, several loads in flight
             float mm = -INFINITY, ll = 0.0f, acc[V] = {};
 #pragma unroll 1
             for (uint32_t i0 = 0; i0 < count; i0 += 32) {
-                const float *p = part(i0 + lane);
-                const float mi = p ? p[ROWS * D + row] : -INFINITY, li = p ? p[ROWS * D + ROWS + row] : 0.0f;
-                const float top = fmaxf(mm, warp_max(mi)), f = mm == top ? 1.0f : ex2(mm - top), w = !p ? 0.0f : mi == top ? 1.0f : ex2(mi - top);
+                const bool in = i0 + lane < count;
+                const float *p = part(in ? i0 + lane : 0) + row * D;
+                const float mi = in ? p[ROWS * D - row * D + row] : -INFINITY, li = p[ROWS * D + ROWS - row * D + row];
+                const float top = fmaxf(mm, warp_max(mi)), f = mm == top ? 1.0f : ex2(mm - top), w = !in ? 0.0f : mi == top ? 1.0f : ex2(mi - top);
                 mm = top;
                 ll = fmaf(w, li, ll * f);
 #pragma unroll
                 for (int v = 0; v < (int)V; v++) acc[v] *= f;
                 constexpr int N = V == 8 ? 4 : 8;
-                for (uint32_t left = __ballot_sync(~0u, p != nullptr); left;) {
+                const uint32_t m = min(32u, count - i0);
+                for (uint32_t i = 0; i < m; i += N) {
                     float x[N][V], wq[N];
 #pragma unroll
                     for (int k = 0; k < N; k++) {
-                        const int i = left ? __ffs(left) - 1 : -1;
-                        const float *q = reinterpret_cast<const float *>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(p), i & 31));
-                        wq[k] = __shfl_sync(~0u, w, i & 31);
-#pragma unroll
-                        for (int v = 0; v < (int)V; v++) x[k][v] = 0.0f;
-                        if (i >= 0) get_row(x[k], q + row * D);
-                        left &= left - 1;
+                        const uint32_t src = min(i + k, m - 1);
+                        wq[k] = i + k < m ? __shfl_sync(~0u, w, src) : 0.0f;
+                        get_row(x[k], part(i0 + src) + row * D);
                     }
 #pragma unroll
                     for (int k = 0; k < N; k++)
@@ -866,12 +869,12 @@ sg_status launch(const Kv4AttnArgs &a0, int sms, cudaStream_t s, cudaError_t *er
     int dev = 0;
     if ((*err = cudaGetDevice(&dev)) != cudaSuccess) return SG_ERR_CUDA;
     if (!ready[dev & 63]) {
-        if ((*err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM)) != cudaSuccess) return SG_ERR_CUDA;
+        if ((*err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<T, D>::SMEM)) != cudaSuccess) return SG_ERR_CUDA;
         ready[dev & 63] = true;
     }
     const uint32_t grid = (uint32_t)sms < MAX_CTAS ? (uint32_t)sms : MAX_CTAS, all = a0.c.heads;
     // MAX_REQ requests a launch, and as many heads as keep the number of steps below 2^32
-    const uint64_t rows = (uint64_t)a0.n_tok * a0.group / ROWS + a0.n_req, steps = (((uint64_t)a0.width << a0.c.page_shift) + Cfg<D>::STEP - 1) / Cfg<D>::STEP + 1;
+    const uint64_t rows = (uint64_t)a0.n_tok * a0.group / ROWS + a0.n_req, steps = (((uint64_t)a0.width << a0.c.page_shift) + Cfg<T, D>::STEP - 1) / Cfg<T, D>::STEP + 1;
     const uint64_t heads = (1ull << 31) / (rows * steps);
     if (heads == 0) return SG_ERR_SHAPE;
     for (uint32_t r0 = 0; r0 == 0 || r0 < a0.n_req; r0 += MAX_REQ)
@@ -882,7 +885,7 @@ sg_status launch(const Kv4AttnArgs &a0, int sms, cudaStream_t s, cudaError_t *er
             a.last = r0 + a.n_req == a0.n_req;
             a.head0 = h0;
             a.n_kv = (uint32_t)(all - h0 < heads ? all - h0 : heads);
-            fn<<<grid, Cfg<D>::WARPS * 32, Cfg<D>::SMEM, s>>>(a);
+            fn<<<grid, Cfg<T, D>::WARPS * 32, Cfg<T, D>::SMEM, s>>>(a);
             if ((*err = cudaGetLastError()) != cudaSuccess) return SG_ERR_CUDA;
         }
     return SG_OK;
