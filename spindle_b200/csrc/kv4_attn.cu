@@ -53,6 +53,10 @@ struct Act<__nv_bfloat16> {
     static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
 };
 
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -156,16 +160,17 @@ constexpr uint32_t MIN_WARPS = 4;   // warps that a CTA uses at least, where the
 
 template <typename T, int D>
 struct Cfg {
-    // As many warps as their sums and query registers leave room for (65536 registers): 128 a lane for 16 of them
-    static constexpr int WARPS = D == 256 ? 8 : D == 128 && sizeof(T) == 4 ? 12 : 16;
+    // As many warps as their sums and query registers leave room for (65536 registers), and one that copies
+    static constexpr int WARPS = D == 256 ? 7 : D == 64 ? 15 : 11;
+    static constexpr int THREADS = (WARPS + 1) * 32;
     static constexpr int TILES = D == 256 ? 1 : 2;
-    static constexpr int STAGES = D == 256 ? 3 : 2;
+    static constexpr int STAGES = D == 256 ? 4 : D == 64 ? 4 : 3;
     static constexpr int STEP = TILES * 16;
     static constexpr uint32_t STAGE_BYTES = TILES * Kv4Tile<D>::BYTES;
     static constexpr uint32_t PART_BYTES = ROWS * D * 4 + 2 * ROWS * 4;  // rows, m, l
     static constexpr uint32_t RING = WARPS * STAGES * STAGE_BYTES;
     static constexpr int SEGS = STAGES + 1;
-    static constexpr uint32_t SMEM = RING + (MAX_REQ + 1) * 4 + MAX_REQ * 16 + WARPS * (STAGES * 8 + 2 * 8 + (SEGS + 2) * 40 + 4) + 512;
+    static constexpr uint32_t SMEM = RING + (MAX_REQ + 1) * 4 + MAX_REQ * 16 + WARPS * (STAGES * 20 + 2 * 8 + (SEGS + 2) * 40 + 4) + 512;
     static_assert(WARPS <= 16, "a lane per partial result");
     static_assert(STAGES * STAGE_BYTES >= PART_BYTES, "a warp's last partial result lies in its ring");
     static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -208,28 +213,29 @@ struct Seg {
 }  // namespace
 
 template <typename T, int D>
-__global__ void __launch_bounds__(Cfg<T, D>::WARPS * 32, 1) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
+__global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
     using L = Kv4Tile<D>;
     using C = Cfg<T, D>;
-    constexpr int G = L::G, TILES = C::TILES, STAGES = C::STAGES, STEP = C::STEP, WARPS = C::WARPS;
+    constexpr int G = L::G, TILES = C::TILES, STAGES = C::STAGES, STEP = C::STEP, WARPS = C::WARPS, THREADS = C::THREADS;
     constexpr bool Q32 = sizeof(T) == 4;
     constexpr int QR = Q32 ? 4 : 2;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring_all = smem;
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::RING);
-    const float **part_at = reinterpret_cast<const float **>(bars + WARPS * STAGES);  // [2 * WARPS] the partial results
+    uint64_t *frees = bars + WARPS * STAGES;                          // a stage's copy has landed; a stage may be written
+    const float **part_at = reinterpret_cast<const float **>(frees + WARPS * STAGES);  // [2 * WARPS] the partial results
     Req *reqs = reinterpret_cast<Req *>(part_at + 2 * WARPS);         // [n_req]
     Seg *segs_all = reinterpret_cast<Seg *>(reqs + MAX_REQ);          // [WARPS][SEGS] the segments in a warp's ring
     Seg *part_seg = segs_all + WARPS * C::SEGS;                       // [2 * WARPS] the partial results' segments
     uint32_t *pre = reinterpret_cast<uint32_t *>(part_seg + 2 * WARPS);  // [n_req + 1] steps before each request
     uint32_t *seg_begin = pre + MAX_REQ + 1;                          // [32] the partials' segments, NONE: no partial
-    uint32_t *scan_s = seg_begin + 32;                                // [WARPS]
-    uint32_t *flag_s = scan_s + WARPS;                                // [2]
+    uint32_t *scan_s = seg_begin + 32;                                // [WARPS + 1]
+    uint32_t *flag_s = scan_s + WARPS + 1;                            // [2]
+    uint32_t *there_s = flag_s + 2;                                   // [WARPS][STAGES] a bit per tile of a stage that is there
     constexpr uint32_t NONE = 0xffffffffu;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, quad = lane & 3;
 
-    if (lane == 0)
-        for (int s = 0; s < STAGES; s++) mbar_init(&bars[warp * STAGES + s], 1);
+    for (uint32_t i = tid; i < 2 * WARPS * STAGES; i += THREADS) mbar_init(&bars[i], 1);
     fence_mbar_init();
     if (tid < 32) seg_begin[tid] = NONE;
 
@@ -239,7 +245,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::WARPS * 32, 1) kv4_attn_kernel(cons
 
     // steps before each request
     uint32_t total = 0;
-    for (uint32_t r0 = 0; r0 < a.n_req; r0 += WARPS * 32) {
+    for (uint32_t r0 = 0; r0 < a.n_req; r0 += THREADS) {
         uint32_t v = 0;
         if (r0 + tid < a.n_req) {
             uint32_t steps;
@@ -255,7 +261,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::WARPS * 32, 1) kv4_attn_kernel(cons
         }
         if (lane == 31) scan_s[warp] = inc;
         __syncthreads();
-        const uint32_t w = lane < WARPS ? scan_s[lane] : 0;
+        const uint32_t w = lane <= WARPS ? scan_s[lane] : 0;
         const uint32_t base = __reduce_add_sync(~0u, lane < warp ? w : 0);
         if (r0 + tid < a.n_req) pre[r0 + tid] = total + base + inc - v;
         total += __reduce_add_sync(~0u, w);
@@ -267,7 +273,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::WARPS * 32, 1) kv4_attn_kernel(cons
     // tokens of no request
     if (spare < a.n_tok) {
         const uint32_t rows = (a.n_tok - spare) * a.n_heads;
-        for (uint32_t row = blockIdx.x * WARPS + warp; row < rows; row += gridDim.x * WARPS) {
+        for (uint32_t row = blockIdx.x * (WARPS + 1) + warp; row < rows; row += gridDim.x * (WARPS + 1)) {
             const uint32_t t = spare + row / a.n_heads, h = row % a.n_heads;
             if (h / a.group - a.head0 >= a.n_kv) continue;
             for (uint32_t d = lane; d < D; d += 32) ((T *)a.out)[t * a.o_tok + h * a.o_head + d] = Act<T>::put(0.0f);
@@ -275,14 +281,17 @@ __global__ void __launch_bounds__(Cfg<T, D>::WARPS * 32, 1) kv4_attn_kernel(cons
         }
     }
 
-    // this warp's stretch of the steps, n from w0 on, in the CTA's [c0, c1); fewer warps a CTA where there is little to do
+    // the CTA's stretch [c0, c1) of the steps, and a warp's, n from w0 on; fewer warps a CTA where there is little to do.
+    // The copying warp's lanes stand for one warp each.
     const uint32_t per_cta = (total + gridDim.x - 1) / gridDim.x, nw = min((uint32_t)WARPS, max((uint32_t)MIN_WARPS, per_cta));
     const uint32_t chunk = (per_cta + nw - 1) / nw, cta_chunk = chunk * nw;
     const uint32_t c0 = min(total, blockIdx.x * cta_chunk), c1 = min(total, c0 + cta_chunk);
-    const uint32_t w0 = min(c1, c0 + min(warp, nw) * chunk), n = min(c1, w0 + chunk) - w0;
+    const uint32_t who = warp < WARPS ? warp : min(lane, (uint32_t)WARPS - 1);
+    const uint32_t w0 = min(c1, c0 + min(who, nw) * chunk), n = min(c1, w0 + chunk) - w0;
 
-    uint8_t *ring = ring_all + warp * (STAGES * C::STAGE_BYTES);
-    uint64_t *bar = bars + warp * STAGES;
+    uint8_t *ring = ring_all + who * (STAGES * C::STAGE_BYTES);
+    uint64_t *bar = bars + who * STAGES, *free_bar = frees + who * STAGES;
+    Seg *segs = segs_all + who * C::SEGS;
 
     // The segment of a step; steps * row tiles * heads of a request fit in 32 bits.
     auto seg_at = [&](uint32_t idx) {
@@ -305,70 +314,69 @@ __global__ void __launch_bounds__(Cfg<T, D>::WARPS * 32, 1) kv4_attn_kernel(cons
         return s;
     };
 
-    // ---- the copies: a step at a time, the table entries of 32 pages in the lanes ----
-    Seg *segs = segs_all + warp * C::SEGS;
-    uint32_t p_left = n, p_run = 0, p_end = 0, p_seg = 0, p_t = 0, p_page = 0;  // steps left; left in this page; in this segment
-    int32_t p_blk = -1;
-    const uint8_t *p_src = nullptr;
-    uint32_t p_there = 0;
-    bool dead = false;  // a wait ran out: no further copies
-    // the step at p_t begins a page or a segment: where its positions lie
-    auto locate = [&]() {
+    if (warp == WARPS) {
+        // ---- the copies: every lane keeps one warp's ring full ----
+        uint32_t left = lane < WARPS ? n : 0, end = 0, seg_at_ = 0, t = 0, stage = 0, phase = 1;
         const uint32_t shift = a.c.page_shift;
-        bool load = (p_t >> shift) - p_page >= 32;
-        if (p_end == 0) {
-            const uint32_t idx = w0 + n - p_left;
-            const Seg s = seg_at(idx);
-            if (lane == 0) segs[p_seg] = s;
-            if (++p_seg == C::SEGS) p_seg = 0;
-            p_end = min(p_left, s.begin + s.steps - idx);
-            p_t = (s.r.s0 + (idx - s.begin)) * STEP;
-            load = true;
-        }
-        const Seg &s = segs[p_seg ? p_seg - 1 : C::SEGS - 1];
-        if (load) {
-            __syncwarp();
-            p_page = p_t >> shift;
-            const uint64_t page = (uint64_t)p_page + lane;
-            p_blk = (int64_t)(page << shift) < s.end ? __ldg(a.tables + (uint64_t)s.req * a.ld_tables + page) : -1;
-        }
-        const uint32_t blk = (uint32_t)__shfl_sync(~0u, p_blk, (p_t >> shift) - p_page), at = p_t & ((1u << shift) - 1);
-        p_there = blk < a.c.n_blocks;
-        p_src = a.c.data + blk * a.block_bytes + (((uint64_t)s.head << (shift - 4)) + (at >> 4)) * L::BYTES;
-        p_run = min(p_end, max(1u, ((1u << shift) - at) / STEP));
-    };
-    // copies the next step into a stage; returns a bit per tile that is there
-    auto issue = [&](uint32_t stage) -> uint32_t {
-        if (p_left == 0) return 0;
-        if (p_run == 0) locate();
-        uint8_t *dst = ring + stage * C::STAGE_BYTES;
-        uint32_t there = p_there;
-        if (TILES == 1 || a.c.page_shift > 4) {  // the step lies in one page
-            there = p_there ? (1u << TILES) - 1 : 0;
-            if (lane == 0 && !dead) {
+        const int32_t *row = nullptr;
+        const uint8_t *base = nullptr;
+        int32_t blk = -1, next = -1, held = 0;
+        uint64_t since = 0;
+        while (__any_sync(~0u, left)) {
+            const bool go = left && mbar_try_wait(&free_bar[stage], phase);
+            if (!__any_sync(~0u, go)) {
+                // nobody took anything: the warps always come on, so that a long wait is an error
+                if (!since) since = globaltimer_ns();
+                else if (globaltimer_ns() - since > 2 * WAIT_LIMIT_NS) {
+                    if (lane == 0) atomicExch(&g_dev_status, (unsigned)DEV_TIMEOUT_TMA);
+                    break;
+                }
+                continue;
+            }
+            since = 0;
+            if (!go) continue;
+            if (end == 0) {  // a new segment
+                const uint32_t idx = w0 + n - left;
+                const Seg s = seg_at(idx);
+                segs[seg_at_] = s;
+                if (++seg_at_ == C::SEGS) seg_at_ = 0;
+                end = min(left, s.begin + s.steps - idx);
+                t = (s.r.s0 + (idx - s.begin)) * STEP;
+                held = s.end;
+                row = a.tables + (uint64_t)s.req * a.ld_tables;
+                base = a.c.data + ((uint64_t)s.head << (shift - 4)) * L::BYTES;
+                blk = (int32_t)t < held ? __ldg(row + (t >> shift)) : -1;
+                const int64_t u = ((int64_t)(t >> shift) + 1) << shift;
+                next = u < held ? __ldg(row + (t >> shift) + 1) : -1;
+            }
+            // the next table entry is read a page ahead
+            auto turn_page = [&](uint32_t page) {
+                blk = next;
+                next = ((int64_t)page + 1) << shift < held ? __ldg(row + page + 1) : -1;
+            };
+            uint8_t *dst = ring + stage * C::STAGE_BYTES;
+            const uint32_t at = (t & ((1u << shift) - 1)) >> 4;
+            uint32_t there = (uint32_t)blk < a.c.n_blocks;
+            const uint8_t *src = base + (uint32_t)blk * a.block_bytes + at * L::BYTES;
+            if (TILES == 1 || shift > 4) {  // the step lies in one page
+                if (there) there = (1u << TILES) - 1;
+                there_s[who * STAGES + stage] = there;
                 mbar_arrive_expect_tx(&bar[stage], there ? C::STAGE_BYTES : 0);
-                if (there) bulk_g2s(dst, p_src, C::STAGE_BYTES, &bar[stage]);
-            }
-        } else {  // a page per tile
-            const uint8_t *src0 = p_src;
-            p_t += 16;
-            locate();
-            p_t -= 16;
-            there |= p_there << 1;
-            if (lane == 0 && !dead) {
+                if (there) bulk_g2s(dst, src, C::STAGE_BYTES, &bar[stage]);
+            } else {  // a page per tile
+                turn_page((t >> shift) + 1);
+                there |= ((uint32_t)blk < a.c.n_blocks) << 1;
+                there_s[who * STAGES + stage] = there;
                 mbar_arrive_expect_tx(&bar[stage], __popc(there) * L::BYTES);
-                if (there & 1) bulk_g2s(dst, src0, L::BYTES, &bar[stage]);
-                if (there & 2) bulk_g2s(dst + L::BYTES, p_src, L::BYTES, &bar[stage]);
+                if (there & 1) bulk_g2s(dst, src, L::BYTES, &bar[stage]);
+                if (there & 2) bulk_g2s(dst + L::BYTES, base + (uint32_t)blk * a.block_bytes, L::BYTES, &bar[stage]);
             }
+            t += STEP;
+            if ((t & ((1u << shift) - 1)) == 0) turn_page(t >> shift);
+            left--, end--;
+            if (++stage == STAGES) stage = 0, phase ^= 1;
         }
-        p_left--, p_end--, p_run--;
-        p_src += C::STAGE_BYTES;
-        p_t += STEP;
-        return there;
-    };
-    uint32_t there = 0;  // the bits of the steps in the ring, the next one's lowest
-#pragma unroll 1
-    for (int s = 0; s < STAGES; s++) there |= issue(s) << (s * TILES);
+    }
 
     uint32_t *counters = reinterpret_cast<uint32_t *>(a.scratch);
     float *parts = reinterpret_cast<float *>(a.scratch + 4096);
@@ -407,7 +415,13 @@ __global__ void __launch_bounds__(Cfg<T, D>::WARPS * 32, 1) kv4_attn_kernel(cons
     };
     auto lse_of = [](float mm, float ll) { return ll == 0.0f ? -INFINITY : (mm - P_SHIFT + log2f(ll)) * LN2; };
 
-    for (uint32_t idx = 0; idx < n; idx++, t0 += STEP) {
+    bool dead = false;  // a wait ran out
+    const uint32_t n_mine = warp < WARPS ? n : 0;
+    for (uint32_t idx = 0; idx < n_mine; idx++, t0 += STEP) {
+        if (!dead && !mbar_wait_bounded(&bar[stage], phase, WAIT_LIMIT_NS)) {
+            dead = true;
+            if (lane == 0) atomicExch(&g_dev_status, (unsigned)DEV_TIMEOUT_TMA);
+        }
         if (idx == c_end) {
             // a new segment: its query rows as operand registers
             const Seg &seg = segs[c_seg];
@@ -520,12 +534,8 @@ __global__ void __launch_bounds__(Cfg<T, D>::WARPS * 32, 1) kv4_attn_kernel(cons
             for (int g = 0; g < G; g++) kmul[g] = 0x78007800u;  // 2^15
         }
 
-        if (!dead && !mbar_wait_bounded(&bar[stage], phase, WAIT_LIMIT_NS)) {
-            dead = true;
-            if (lane == 0) atomicExch(&g_dev_status, (unsigned)DEV_TIMEOUT_TMA);
-        }
         uint8_t *buf = ring + stage * C::STAGE_BYTES;
-        const uint32_t here = there & ((1u << TILES) - 1);
+        const uint32_t here = there_s[warp * STAGES + stage];
         // whole: every row sees every position of the step
         const bool whole = here == (1u << TILES) - 1 && t0 >= full_lo && t0 + STEP <= full_hi;
 
@@ -688,9 +698,9 @@ __global__ void __launch_bounds__(Cfg<T, D>::WARPS * 32, 1) kv4_attn_kernel(cons
             }
         }
 
-        // the stage is read: the next copy into it
+        // the stage is read: it may be written again
         __syncwarp();
-        there = there >> TILES | issue(stage) << ((STAGES - 1) * TILES);
+        if (lane == 0) mbar_arrive(&free_bar[stage]);
         if (++stage == STAGES) stage = 0, phase ^= 1;
 
         if (idx + 1 == c_end) {
@@ -730,7 +740,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::WARPS * 32, 1) kv4_attn_kernel(cons
         }
     }
     if (dead) {  // copies still in flight must not land in memory that is used for something else
-        for (int s = 0; s < STAGES; s++) mbar_wait_bounded(&bar[s], phase, WAIT_LIMIT_NS / 20);
+        for (int s = 0; s < STAGES; s++) mbar_wait_bounded(&bar[s], s < (int)stage ? phase ^ 1 : phase, WAIT_LIMIT_NS / 20);
     }
     __syncthreads();
 
@@ -791,7 +801,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::WARPS * 32, 1) kv4_attn_kernel(cons
         }
         const uint32_t units = pass ? 2 * ROWS : __popc(leads) * ROWS;
 #pragma unroll 1
-        for (uint32_t u = warp; u < units; u += WARPS) {
+        for (uint32_t u = warp; u < units; u += WARPS + 1) {
             const uint32_t row = u % ROWS;
             uint32_t at = 0, count, cb = 0;  // pass 0: the first part's slot; its first CTA
             const Seg *of;
@@ -885,7 +895,7 @@ sg_status launch(const Kv4AttnArgs &a0, int sms, cudaStream_t s, cudaError_t *er
             a.last = r0 + a.n_req == a0.n_req;
             a.head0 = h0;
             a.n_kv = (uint32_t)(all - h0 < heads ? all - h0 : heads);
-            fn<<<grid, Cfg<T, D>::WARPS * 32, Cfg<T, D>::SMEM, s>>>(a);
+            fn<<<grid, Cfg<T, D>::THREADS, Cfg<T, D>::SMEM, s>>>(a);
             if ((*err = cudaGetLastError()) != cudaSuccess) return SG_ERR_CUDA;
         }
     return SG_OK;
