@@ -1,24 +1,119 @@
 // logprobs.cu — log probabilities of given tokens with entropy, rank and the
-// likeliest alternatives, one CTA per row.
+// likeliest alternatives, in one pass over the logits.
 //
 //   m = max x, z = sum e^(x - m), logprob = x_tok - m - ln z,
 //   entropy = ln z - sum (x - m) e^(x - m) / z,
 //   rank = how many tokens come before the given one when sorted by falling
 //   logit, equal ones by rising index; the alternatives are the first of that order.
+//
+// A row belongs to a cluster of CTAs (one where the rows alone fill the device),
+// each with a stretch of it.  A thread reads 64 bytes at a time, takes their
+// maximum, and adds to its running m, z and sum of (x - m) e^(x - m); what bounds
+// it is reading the row.  The alternatives cost the pass nothing but keeping the
+// maximum of each thread's UNITS stretches: with t the top-th largest of the maxima
+// of 128 groups of four threads, every alternative is at least t (each of `top`
+// groups has one that is), and only about top elements are; the few stretches that
+// reach t are read again and their elements sorted by counting.  Where that
+// collects too many (a row of equal logits, say) or a NaN is about, the exact
+// top-th key comes from four passes of 8 bits each, and ties are taken in index
+// order.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <utility>
 
 #include "logprobs.cuh"
 
 namespace sg {
 
+namespace cg = cooperative_groups;
+
 namespace {
 
-constexpr int THREADS = 1024;
+constexpr uint32_t THREADS = 512, WARPS = THREADS / 32, GROUPS = THREADS / 4;
+constexpr uint32_t LOADS = 4;    // 16-byte loads of a thread in flight
+constexpr uint32_t UNITS = 16;   // stretches of a thread whose maxima are kept; one more for the row's ragged ends
+constexpr uint32_t CAP = 1536;   // candidates that are sorted by counting
+constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
 
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+struct El;
+template <>
+struct El<float> {
+    static constexpr uint32_t N = 4, NEG = 0xFF800000u;  // values of 16 bytes; minus infinities
+    static __device__ __forceinline__ float2 two(const uint32_t *r, int i) { return make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])); }
+    static __device__ __forceinline__ float get(float v) { return v; }
+};
+template <>
+struct El<__half> {
+    static constexpr uint32_t N = 8, NEG = 0xFC00FC00u;
+    static __device__ __forceinline__ float2 two(const uint32_t *r, int i) { return __half22float2(reinterpret_cast<const __half2 *>(r)[i]); }
+    static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
+};
+template <>
+struct El<__nv_bfloat16> {
+    static constexpr uint32_t N = 8, NEG = 0xFF80FF80u;
+    static __device__ __forceinline__ float2 two(const uint32_t *r, int i) { return make_float2(__uint_as_float(r[i] << 16), __uint_as_float(r[i] & 0xFFFF0000u)); }
+    static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
+};
+
+template <typename T, int W>
+__device__ __forceinline__ float max_of(const uint32_t (&r)[W]) {
+    if constexpr (sizeof(T) == 4) {
+        float m = __uint_as_float(r[0]);
+#pragma unroll
+        for (int i = 1; i < W; i++) m = fmaxf(m, __uint_as_float(r[i]));
+        return m;
+    } else {
+        uint32_t m = r[0];
+#pragma unroll
+        for (int i = 1; i < W; i++) {
+            if constexpr (sizeof(T) == 2 && El<T>::NEG == El<__half>::NEG) asm("max.f16x2 %0, %0, %1;" : "+r"(m) : "r"(r[i]));
+            else asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(r[i]));
+        }
+        const float2 f = El<T>::two(&m, 0);
+        return fmaxf(f.x, f.y);
+    }
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// The larger one, NaN if either is.
+__device__ __forceinline__ float max_nan(float x, float y) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(x), "f"(y));
+    return d;
+}
+// Two f32 operations in one instruction.
+__device__ __forceinline__ uint64_t two_f32(float x, float y) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+    return d;
+}
+__device__ __forceinline__ float2 two_of(uint64_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
 
 // Order of falling logits, equal ones by rising index, as one number (larger
 // comes first).  NaN counts as larger than everything; the zeros are equal.
@@ -26,93 +121,351 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     const uint32_t b = __float_as_uint(x + 0.0f);
     return x == x ? (b & 0x80000000u ? ~b : b | 0x80000000u) : 0xfffffffeu;
 }
+constexpr uint32_t ORDER_NEG_INF = 0x007fffffu;
+__device__ __forceinline__ float value_of(uint32_t o) {
+    return o == 0xfffffffeu ? NAN : __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t i) { return (uint64_t)order_of(x) << 32 | (uint32_t)~i; }
 
+// Running maximum, sum of 2^t and sum of t 2^t over t = (x - m) log2 e.
 struct Sum {
-    float m, z, zx;  // running max, sum e^(x-m), sum (x-m) e^(x-m)
+    float m, z, zt;
 };
 
-// A term whose weight is zero counts nothing, whatever its distance.
+// A sum that has nothing yet changes nothing, whatever its maximum.
 __device__ __forceinline__ Sum join(Sum a, Sum b) {
     if (b.m > a.m) {
         const Sum t = a;
         a = b;
         b = t;
     }
-    if (b.z == 0.0f && b.m == b.m) return a;
-    const float d = b.m - a.m, w = d == 0.0f ? 1.0f : expf(d);  // equal infinities: no difference
-    a.z += b.z * w;
-    a.zx += w == 0.0f ? 0.0f : (b.zx + d * b.z) * w;
+    if (b.z == 0.0f) return a;
+    const float d = b.m == a.m ? 0.0f : (b.m - a.m) * LOG2E, w = ex2(d);
+    a.z = fmaf(b.z, w, a.z);
+    a.zt += w == 0.0f ? 0.0f : (b.zt + d * b.z) * w;
     return a;
 }
 
+struct Shared {
+    Sum sum[WARPS], all[8];
+    uint32_t ahead[WARPS], all_ahead[8];
+    uint32_t gmax[GROUPS];
+    uint32_t count, threshold, found;
+    uint32_t warp_count[WARPS];
+    union {
+        uint64_t cand[CAP];
+        uint32_t hist[256];
+    };
+    uint64_t top[8 * LP_TOP_MAX];  // the CTAs' alternatives, in the first CTA
+    float unit[UNITS + 1][THREADS];
+};
+
 template <typename T>
-__global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogprobsArgs a) {
-    __shared__ Sum sum_s[32];
-    __shared__ uint64_t key_s[32];
-    __shared__ uint32_t cnt_s[32];
-    const uint32_t tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-    for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const T *x = (const T *)a.logits + (uint64_t)row * a.ld;
-        const int32_t tok = a.tokens ? a.tokens[row] : -1;
-        const bool given = tok >= 0 && (uint32_t)tok < a.vocab;
-        const uint64_t kt = given ? key_of(to_f32(x[tok]), tok) : ~0ull;
-        Sum s = {-INFINITY, 0.0f, 0.0f};
-        uint32_t ahead = 0;
-        for (uint32_t i = tid; i < a.vocab; i += THREADS) {
-            const float v = to_f32(x[i]);
-            ahead += key_of(v, i) > kt;
-            s = join(s, Sum{v, v == -INFINITY ? 0.0f : 1.0f, 0.0f});
+__global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs a) {
+    constexpr uint32_t N = El<T>::N;
+    extern __shared__ __align__(16) uint8_t smem[];
+    Shared &s = *reinterpret_cast<Shared *>(smem);
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t parts = cluster.num_blocks(), part = cluster.block_rank();
+    auto started = cluster.barrier_arrive();  // waited for before another CTA's memory is written
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t row = blockIdx.x / parts;
+    const T *x = (const T *)a.logits + (uint64_t)row * a.ld;
+    const int32_t tok = a.tokens ? a.tokens[row] : -1;
+    const bool given = tok >= 0 && (uint32_t)tok < a.vocab;
+    const float xt = given ? El<T>::get(x[tok]) : INFINITY;
+
+    // the row: `head` values up to the first 16-byte boundary, whole 16-byte words, the rest
+    const uint32_t head = min(a.vocab, (uint32_t)((16 - ((uintptr_t)x & 15)) & 15) / (uint32_t)sizeof(T));
+    const uint32_t words = (a.vocab - head) / N, tail = a.vocab - head - words * N;
+    const uint32_t v0 = (uint32_t)((uint64_t)words * part / parts), v1 = (uint32_t)((uint64_t)words * (part + 1) / parts);
+    const uint32_t begin = part == 0 ? 0 : head + v0 * N, end = part + 1 == parts ? a.vocab : head + v1 * N;  // this CTA's values
+    const uint4 *xv = reinterpret_cast<const uint4 *>(x + head);
+    const uint32_t turns = (v1 - v0 + LOADS * THREADS - 1) / (LOADS * THREADS), per_unit = (turns + UNITS - 1) / UNITS;
+
+    Sum sum = {-INFINITY, 0.0f, 0.0f};
+    uint64_t z2 = 0, zt2 = 0;  // the pair of sums at sum.m
+    uint32_t ahead = 0;
+    float tmax = -INFINITY, umax = -INFINITY;
+    uint32_t unit = 0, in_unit = 0;
+    // one load's worth: W words of a thread that start at element `at` (words LOADS * THREADS apart)
+    auto add = [&](const uint32_t (&r)[LOADS * 4], uint32_t v) {
+        const float m = max_of<T>(r);
+        umax = fmaxf(umax, m);
+        if (m > sum.m) {
+            const float d = (sum.m - m) * LOG2E, w = ex2(d);
+            const float2 z = two_of(z2), zt = two_of(zt2);
+            zt2 = two_f32(z.x == 0.0f ? 0.0f : (zt.x + d * z.x) * w, z.y == 0.0f ? 0.0f : (zt.y + d * z.y) * w);
+            z2 = two_f32(z.x * w, z.y * w);
+            sum.m = m;
         }
-        for (int o = 16; o; o >>= 1) {
-            s = join(s, Sum{__shfl_xor_sync(~0u, s.m, o), __shfl_xor_sync(~0u, s.z, o), __shfl_xor_sync(~0u, s.zx, o)});
-            ahead += __shfl_xor_sync(~0u, ahead, o);
+        const float ref = sum.m == -INFINITY ? 0.0f : sum.m;  // where all is masked so far the terms are 0
+        const uint64_t nm = two_f32(-ref, -ref), l2 = two_f32(LOG2E, LOG2E);
+#pragma unroll
+        for (int i = 0; i < (int)(LOADS * N / 2); i++) {
+            const float2 f = El<T>::two(r, i), t = two_of(mul2(add2(two_f32(f.x, f.y), nm), l2));
+            const float t0 = max_nan(t.x, -200.0f), t1 = max_nan(t.y, -200.0f);  // 2^-200 is 0 in f32, and 0 * -200 too
+            const uint64_t e = two_f32(ex2(t0), ex2(t1));
+            z2 = add2(z2, e);
+            zt2 = fma2(e, two_f32(t0, t1), zt2);
         }
-        if (lane == 0) sum_s[wid] = s, cnt_s[wid] = ahead;
-        __syncthreads();
-        s = sum_s[0], ahead = cnt_s[0];
-        for (int w = 1; w < 32; w++) s = join(s, sum_s[w]), ahead += cnt_s[w];
-        const bool none = s.m == -INFINITY && s.z == 0.0f;  // a row whose mask leaves nothing
-        const float lz = s.m == INFINITY ? NAN : logf(s.z);  // an infinite logit leaves no probabilities
-        if (tid == 0) {
-            a.logprob[row] = !given ? NAN : none ? -INFINITY : to_f32(x[tok]) - s.m - lz;
-            a.entropy[row] = none ? 0.0f : lz - s.zx / s.z;
-            a.rank[row] = given ? (int32_t)ahead : -1;
+        if (m >= xt) {
+#pragma unroll
+            for (int j = 0; j < (int)LOADS; j++)
+#pragma unroll
+                for (int i = 0; i < (int)(N / 2); i++) {
+                    const float2 f = El<T>::two(r + 4 * j, i);
+                    const uint32_t at = head + (v + j * THREADS) * N + 2 * i;
+                    ahead += f.x > xt || (f.x == xt && at < (uint32_t)tok);
+                    ahead += f.y > xt || (f.y == xt && at + 1 < (uint32_t)tok);
+                }
         }
-        uint64_t last = ~0ull;
-        for (uint32_t k = 0; k < a.top; k++) {
-            uint64_t best = 0;
-            for (uint32_t i = tid; i < a.vocab; i += THREADS) {
-                const uint64_t q = key_of(to_f32(x[i]), i);
-                if (q < last && q > best) best = q;
-            }
-            for (int o = 16; o; o >>= 1) {
-                const uint64_t q = __shfl_xor_sync(~0u, best, o);
-                best = q > best ? q : best;
-            }
-            __syncthreads();
-            if (lane == 0) key_s[wid] = best;
-            __syncthreads();
-            for (int w = 0; w < 32; w++) best = key_s[w] > best ? key_s[w] : best;
-            last = best;
-            if (tid == 0) {
-                const uint32_t id = ~(uint32_t)best;
-                a.top_ids[(uint64_t)row * a.top + k] = (int32_t)id;
-                a.top_logprobs[(uint64_t)row * a.top + k] = none ? -INFINITY : to_f32(x[id]) - s.m - lz;
-            }
+    };
+    for (uint32_t turn = 0; turn < turns; turn++) {
+        const uint32_t v = v0 + turn * LOADS * THREADS + tid;
+        uint32_t r[LOADS * 4];
+#pragma unroll
+        for (int j = 0; j < (int)LOADS; j++) {
+            const uint4 w = v + j * THREADS < v1 ? __ldg(xv + v + j * THREADS) : make_uint4(El<T>::NEG, El<T>::NEG, El<T>::NEG, El<T>::NEG);
+            r[4 * j] = w.x, r[4 * j + 1] = w.y, r[4 * j + 2] = w.z, r[4 * j + 3] = w.w;
         }
-        __syncthreads();
+        add(r, v);
+        if (++in_unit == per_unit || turn + 1 == turns) {
+            s.unit[unit][tid] = umax;
+            tmax = fmaxf(tmax, umax);
+            umax = -INFINITY;
+            unit++, in_unit = 0;
+        }
     }
+    const uint32_t units = unit;
+    // the ragged ends, a value per thread: the head in the first CTA, the tail in the last
+    const uint32_t n_head = part == 0 ? head : 0, n_edge = n_head + (part + 1 == parts ? tail : 0);
+    const uint32_t edge = tid < n_head ? tid : a.vocab - tail + (tid - n_head);
+    if (tid < n_edge) {
+        const float f = El<T>::get(x[edge]);
+        const float2 z = two_of(z2), zt = two_of(zt2);
+        const Sum one = {f, f == -INFINITY ? 0.0f : 1.0f, 0.0f};
+        const Sum got = join(Sum{sum.m, z.x + z.y, zt.x + zt.y}, one);
+        sum.m = got.m, z2 = two_f32(got.z, 0.0f), zt2 = two_f32(got.zt, 0.0f);
+        ahead += f > xt || (f == xt && edge < (uint32_t)tok);
+        umax = f;
+        tmax = fmaxf(tmax, f);
+    }
+    s.unit[UNITS][tid] = umax;
+    {
+        const float2 z = two_of(z2), zt = two_of(zt2);
+        sum.z = z.x + z.y, sum.zt = zt.x + zt.y;
+    }
+
+    // the CTA's sums
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        sum = join(sum, Sum{__shfl_xor_sync(~0u, sum.m, o), __shfl_xor_sync(~0u, sum.z, o), __shfl_xor_sync(~0u, sum.zt, o)});
+        ahead += __shfl_xor_sync(~0u, ahead, o);
+    }
+    if (lane == 0) s.sum[warp] = sum, s.ahead[warp] = ahead;
+    if (tid == 0) s.count = 0, s.found = 0, s.threshold = 0;
+    if (a.top) {
+        float g = fmaxf(tmax, __shfl_xor_sync(~0u, tmax, 1));
+        g = fmaxf(g, __shfl_xor_sync(~0u, g, 2));
+        if ((tid & 3) == 0) s.gmax[tid >> 2] = order_of(g);
+    }
+    __syncthreads();
+    sum = s.sum[0], ahead = s.ahead[0];
+#pragma unroll 1
+    for (uint32_t w = 1; w < WARPS; w++) sum = join(sum, s.sum[w]), ahead += s.ahead[w];
+    const bool odd = sum.z != sum.z;  // a NaN, or infinities that cancel
+
+    if (odd && given) {  // the comparisons above saw no NaN: count again by keys
+        const uint64_t kt = key_of(xt, (uint32_t)tok);
+        uint32_t n = 0;
+        for (uint32_t i = begin + tid; i < end; i += THREADS) n += key_of(El<T>::get(x[i]), i) > kt;
+        n = __reduce_add_sync(~0u, n);
+        __syncthreads();
+        if (lane == 0) s.ahead[warp] = n;
+        __syncthreads();
+        ahead = 0;
+        for (uint32_t w = 0; w < WARPS; w++) ahead += s.ahead[w];
+    }
+    cluster.barrier_wait(std::move(started));
+    if (tid == 0) {
+        Shared &first = *cluster.map_shared_rank(&s, 0);
+        first.all[part] = sum;
+        first.all_ahead[part] = ahead;
+    }
+
+    // ---- the alternatives in this CTA's stretch: at most `want`, into the first CTA's list ----
+    const uint32_t k = a.top, want = min(k, end - begin);
+    if (k) {
+        uint64_t *list = cluster.map_shared_rank(&s.top[0], 0) + part * k;
+        bool exact = odd;
+        uint32_t n = 0;
+        if (!odd) {
+            // the top-th largest of the groups' maxima
+            if (tid < GROUPS) {
+                const uint32_t mine = s.gmax[tid];
+                uint32_t before = 0;
+#pragma unroll 8
+                for (uint32_t g = 0; g < GROUPS; g += 4) {
+                    const uint4 o = *reinterpret_cast<const uint4 *>(&s.gmax[g]);
+                    before += (o.x > mine || (o.x == mine && g < tid)) + (o.y > mine || (o.y == mine && g + 1 < tid));
+                    before += (o.z > mine || (o.z == mine && g + 2 < tid)) + (o.w > mine || (o.w == mine && g + 3 < tid));
+                }
+                if (before == k - 1) s.threshold = mine;
+            }
+            __syncthreads();
+            // a threshold of minus infinity: all that is larger, and below as many of those that are not as can be needed
+            const uint32_t t = s.threshold, least = t <= ORDER_NEG_INF ? ORDER_NEG_INF + 1 : t;
+            auto push = [&](float f, uint32_t i) {
+                if (order_of(f) < least) return;
+                const uint32_t c = atomicAdd(&s.count, 1u);
+                if (c < CAP) s.cand[c] = key_of(f, i);
+            };
+            if (order_of(tmax) >= least) {
+                for (uint32_t u = 0; u < units; u++) {
+                    if (order_of(s.unit[u][tid]) < least) continue;
+                    for (uint32_t turn = u * per_unit; turn < min(turns, (u + 1) * per_unit); turn++)
+                        for (uint32_t j = 0; j < LOADS; j++) {
+                            const uint32_t v = v0 + (turn * LOADS + j) * THREADS + tid;
+                            if (v >= v1) break;
+                            const uint4 w = xv[v];
+                            const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for (int i = 0; i < (int)(N / 2); i++) {
+                                const float2 f = El<T>::two(r, i);
+                                push(f.x, head + v * N + 2 * i);
+                                push(f.y, head + v * N + 2 * i + 1);
+                            }
+                        }
+                }
+                if (tid < n_edge) push(s.unit[UNITS][tid], edge);
+            }
+            __syncthreads();
+            n = s.count;
+            if (t <= ORDER_NEG_INF && n < want) {
+                // of the first n + want values of the stretch at least want are minus infinities, or all of them are there
+                for (uint32_t i = begin + tid; i < min(end, begin + n + want); i += THREADS) {
+                    const float f = El<T>::get(x[i]);
+                    if (f != -INFINITY) continue;
+                    const uint32_t c = atomicAdd(&s.count, 1u);
+                    if (c < CAP) s.cand[c] = key_of(f, i);
+                }
+                __syncthreads();
+                n = s.count;
+            }
+            exact = n > CAP;
+        }
+        if (exact) {
+            // the want-th largest order, 8 bits at a time
+            uint32_t prefix = 0, need = want;
+            for (int shift = 24; shift >= 0; shift -= 8) {
+                __syncthreads();
+                if (tid < 256) s.hist[tid] = 0;
+                __syncthreads();
+                for (uint32_t i = begin + tid; i < end; i += THREADS) {
+                    const uint32_t o = order_of(El<T>::get(x[i]));
+                    if (shift == 24 || (o >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s.hist[(o >> shift) & 255], 1u);
+                }
+                __syncthreads();
+                if (tid == 0) {
+                    uint32_t left = need;
+                    int b = 255;
+                    while (b > 0 && s.hist[b] < left) left -= s.hist[b--];
+                    s.threshold = prefix | (uint32_t)b << shift;
+                    s.count = left;
+                }
+                __syncthreads();
+                prefix = s.threshold, need = s.count;
+            }
+            // the larger ones in any order; of the equal ones the first `need`
+            __syncthreads();
+            if (tid == 0) s.count = 0;
+            __syncthreads();
+            uint32_t taken = 0;
+            for (uint32_t i0 = begin; i0 < end; i0 += THREADS) {
+                const uint32_t i = i0 + tid;
+                const float f = i < end ? El<T>::get(x[i]) : -INFINITY;
+                const uint32_t o = order_of(f);
+                if (i < end && o > prefix) s.cand[atomicAdd(&s.count, 1u)] = key_of(f, i);  // fewer than want
+                if (taken >= need) continue;
+                const uint32_t same = __ballot_sync(~0u, i < end && o == prefix);
+                __syncthreads();
+                if (lane == 0) s.warp_count[warp] = __popc(same);
+                __syncthreads();
+                uint32_t at = taken, all = 0;
+                for (uint32_t w = 0; w < WARPS; w++) at += w < warp ? s.warp_count[w] : 0, all += s.warp_count[w];
+                at += __popc(same & ((1u << lane) - 1));
+                if (same >> lane & 1 && at < need) s.cand[atomicAdd(&s.count, 1u)] = key_of(f, i);
+                taken += all;
+            }
+            __syncthreads();
+            n = s.count;
+        }
+        // the best of the candidates, each at its place (any number of them is at least want)
+        for (uint32_t c = tid; c < n; c += THREADS) {
+            const uint64_t mine = s.cand[c];
+            uint32_t before = 0;
+            for (uint32_t j = 0; j < n; j++) before += s.cand[j] > mine;
+            if (before < want) list[before] = mine;
+        }
+        if (tid >= want && tid < k) list[tid] = 0;
+    }
+    cluster.sync();
+    if (part) return;
+
+    // ---- the row's results, in the first CTA ----
+    sum = s.all[0], ahead = s.all_ahead[0];
+    for (uint32_t p = 1; p < parts; p++) sum = join(sum, s.all[p]), ahead += s.all_ahead[p];
+    const bool none = sum.m == -INFINITY && sum.z == 0.0f;        // a row whose mask leaves nothing
+    const float lz = sum.m == INFINITY ? NAN : log2f(sum.z) * LN2;  // an infinite logit leaves no probabilities
+    if (tid == 0) {
+        a.logprob[row] = !given ? NAN : none ? -INFINITY : xt - sum.m - lz;
+        a.entropy[row] = none ? 0.0f : lz - sum.zt / sum.z * LN2;
+        a.rank[row] = given ? (int32_t)ahead : -1;
+    }
+    for (uint32_t c = tid; c < parts * k; c += THREADS) {
+        const uint64_t mine = s.top[c];
+        uint32_t before = parts == 1 ? c : 0;
+        if (parts > 1)
+            for (uint32_t j = 0; j < parts * k; j++) before += s.top[j] > mine;
+        if (mine && before < k) {
+            a.top_ids[(uint64_t)row * k + before] = (int32_t)~(uint32_t)mine;
+            a.top_logprobs[(uint64_t)row * k + before] = none ? -INFINITY : value_of((uint32_t)(mine >> 32)) - sum.m - lz;
+        }
+    }
+}
+
+template <typename T>
+cudaError_t launch(const LogprobsArgs &a, int sms, cudaStream_t s) {
+    auto fn = logprobs_kernel<T>;
+    static bool ready[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (!ready[dev & 63]) {
+        if ((e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared))) != cudaSuccess) return e;
+        ready[dev & 63] = true;
+    }
+    // as many CTAs a row as the device has room for two per SM, at most 8, and at least a turn of loads for each
+    uint32_t parts = 1;
+    while (parts < 8 && a.rows * parts * 2 <= (uint32_t)sms * 2 && a.vocab >= 2 * parts * THREADS * El<T>::N) parts *= 2;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(a.rows * parts);
+    c.blockDim = dim3(THREADS);
+    c.dynamicSmemBytes = sizeof(Shared);
+    c.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {parts, 1, 1};
+    c.attrs = at;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, fn, a);
 }
 
 }  // namespace
 
 sg_status logprobs_launch(const LogprobsArgs &a, int32_t type, int sms, cudaStream_t s, cudaError_t *err) {
-    const uint32_t grid = a.rows < (uint32_t)sms * 2 ? a.rows : (uint32_t)sms * 2;
-    if (type == SG_F32) logprobs_kernel<float><<<grid, THREADS, 0, s>>>(a);
-    else if (type == SG_F16) logprobs_kernel<__half><<<grid, THREADS, 0, s>>>(a);
-    else logprobs_kernel<__nv_bfloat16><<<grid, THREADS, 0, s>>>(a);
-    *err = cudaGetLastError();
+    *err = type == SG_F32 ? launch<float>(a, sms, s) : type == SG_F16 ? launch<__half>(a, sms, s) : launch<__nv_bfloat16>(a, sms, s);
     return *err == cudaSuccess ? SG_OK : SG_ERR_CUDA;
 }
 

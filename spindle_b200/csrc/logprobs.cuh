@@ -15,7 +15,7 @@ struct LogprobsArgs {
     float *top_logprobs;
 };
 
-constexpr int LP_TOP_MAX = SG_LOGPROBS_TOP_MAX;
+constexpr uint32_t LP_TOP_MAX = SG_LOGPROBS_TOP_MAX;
 
 sg_status logprobs_launch(const LogprobsArgs &a, int32_t type, int sms, cudaStream_t s, cudaError_t *err);
 

@@ -19,8 +19,9 @@ LOGPROBS_TOP_MAX = 64
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 
 
-def _s(stream):
-    return (stream if stream is not None else torch.cuda.current_stream()).cuda_stream
+def _s(stream, t):
+    """The handle of the stream that a call on t's device runs on."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device()) if stream is None else stream.cuda_stream
 
 
 def _on(stream):
@@ -113,7 +114,7 @@ def kv4_plan(plan, ctx, new, tables, ring=None, cursor=None, stream=None):
     cu, seq, pos, slots = plan._out
     st = _lib.load().sg_kv4_plan(plan.page, plan.n_blocks, n, _i32(ctx, "ctx"), _i32(new, "new", (n,)), tables.data_ptr(),
                                  tables.stride(0), tables.shape[1], _i32(ring, "ring"), _i32(cursor, "cursor"), cu, seq, pos,
-                                 slots, plan.max_tokens, info.data_ptr(), _s(stream))
+                                 slots, plan.max_tokens, info.data_ptr(), _s(stream, tables))
     if st:
         _lib.check(st, "kv4_plan")
     plan._turn = turn
@@ -135,7 +136,7 @@ def kv4_append(cache, k, v, slots, stream=None):
         raise ValueError("k and v must have one type and one number of rows")
     n = k.shape[0]
     st = _lib.load().sg_kv4_append(cache._c, _type(k, "k"), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                                   v.stride(1), _i32(slots, "slots", (n,)), n, cache.nonfinite.data_ptr(), _s(stream))
+                                   v.stride(1), _i32(slots, "slots", (n,)), n, cache.nonfinite.data_ptr(), _s(stream, k))
     if st:
         _lib.check(st, "kv4_append")
 
@@ -153,7 +154,7 @@ def kv4_read(cache, slots, out=None, dtype=torch.float16, stream=None):
         _rows(cache, t, "out")
         if t.shape[0] != n or t.dtype != k.dtype or not t.is_contiguous():
             raise ValueError("out must be two contiguous tensors of one type with a row per slot")
-    st = _lib.load().sg_kv4_read(cache._c, _type(k, "out"), _i32(slots, "slots"), n, k.data_ptr(), v.data_ptr(), _s(stream))
+    st = _lib.load().sg_kv4_read(cache._c, _type(k, "out"), _i32(slots, "slots"), n, k.data_ptr(), v.data_ptr(), _s(stream, k))
     if st:
         _lib.check(st, "kv4_read")
     return out
@@ -164,7 +165,7 @@ def kv4_attention_scratch(device="cuda", stream=None):
     L = _lib.load()
     with _on(stream):
         t = torch.empty(L.sg_kv4_attention_scratch_bytes(), dtype=torch.uint8, device=device)
-    _lib.check(L.sg_kv4_attention_scratch_init(t.data_ptr(), t.numel(), _s(stream)), "kv4_attention_scratch_init")
+    _lib.check(L.sg_kv4_attention_scratch_init(t.data_ptr(), t.numel(), _s(stream, t)), "kv4_attention_scratch_init")
     return t
 
 
@@ -194,7 +195,7 @@ def kv4_attention(cache, q, cu, seq, tables, scale=None, window=0, max_new=0, ou
                   out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), _i32(cu, "cu", (n + 1,)),
                   _i32(seq, "seq"), tables.data_ptr(), tables.stride(0), tables.shape[1], 0.0 if scale is None else scale,
                   window, max_new, scratch.data_ptr(), scratch.numel())
-    st = _lib.load().sg_kv4_attention(cache._c, C.byref(a), _s(stream))
+    st = _lib.load().sg_kv4_attention(cache._c, C.byref(a), _s(stream, q))
     if st:
         _lib.check(st, "kv4_attention")
     return out
@@ -230,7 +231,7 @@ def logprobs(logits, tokens=None, top=0, out=None, stream=None):
     lp, ent, rank, ids, tops = out._p
     st = _lib.load().sg_logprobs(_type(logits, "logits"), logits.data_ptr(), logits.stride(0), rows, vocab,
                                  None if tokens is None else _i32(tokens, "tokens", (rows,)), lp, ent, rank, top, ids, tops,
-                                 _s(stream))
+                                 _s(stream, logits))
     if st:
         _lib.check(st, "logprobs")
     return out
