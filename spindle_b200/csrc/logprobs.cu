@@ -21,7 +21,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <utility>
+#include <type_traits>
 
 #include "logprobs.cuh"
 
@@ -33,8 +33,9 @@ namespace {
 
 constexpr uint32_t THREADS = 512, WARPS = THREADS / 32, GROUPS = THREADS / 4;
 constexpr uint32_t LOADS = 4;    // 16-byte loads of a thread in flight
-constexpr uint32_t UNITS = 16;   // stretches of a thread whose maxima are kept; one more for the row's ragged ends
+constexpr uint32_t UNITS = 8;    // stretches of a thread whose maxima are kept; one more for the row's ragged ends
 constexpr uint32_t CAP = 1536;   // candidates that are sorted by counting
+constexpr float LAG = 8.0f;
 constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
 
 template <typename T>
@@ -50,43 +51,80 @@ struct El<__half> {
     static constexpr uint32_t N = 8, NEG = 0xFC00FC00u;
     static __device__ __forceinline__ float2 two(const uint32_t *r, int i) { return __half22float2(reinterpret_cast<const __half2 *>(r)[i]); }
     static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half inf() { return __ushort_as_half(0x7C00); }
 };
 template <>
 struct El<__nv_bfloat16> {
     static constexpr uint32_t N = 8, NEG = 0xFF80FF80u;
     static __device__ __forceinline__ float2 two(const uint32_t *r, int i) { return make_float2(__uint_as_float(r[i] << 16), __uint_as_float(r[i] & 0xFFFF0000u)); }
     static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 inf() { return __ushort_as_bfloat16(0x7F80); }
 };
 
+// The larger one, NaN if either is.
+__device__ __forceinline__ float max_nan(float x, float y) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(x), "f"(y));
+    return d;
+}
+// Of two pairs of 16-bit values: 1 where x > y, or x >= y, else 0; their sums.
+template <typename T>
+__device__ __forceinline__ uint32_t more2(uint32_t x, uint32_t y, bool equal_too) {
+    uint32_t d;
+    if constexpr (std::is_same<T, __half>::value) {
+        if (equal_too) asm("set.ge.f16x2.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y));
+        else asm("set.gt.f16x2.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y));
+    } else {
+        if (equal_too) asm("set.ge.bf16x2.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y));
+        else asm("set.gt.bf16x2.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y));
+    }
+    return d;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t add2_16(uint32_t x, uint32_t y) {
+    uint32_t d;
+    if constexpr (std::is_same<T, __half>::value) asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y));
+    else asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y));
+    return d;
+}
+
+// The largest of a thread's values, NaN if one is.
 template <typename T, int W>
 __device__ __forceinline__ float max_of(const uint32_t (&r)[W]) {
     if constexpr (sizeof(T) == 4) {
         float m = __uint_as_float(r[0]);
 #pragma unroll
-        for (int i = 1; i < W; i++) m = fmaxf(m, __uint_as_float(r[i]));
+        for (int i = 1; i < W; i++) m = max_nan(m, __uint_as_float(r[i]));
         return m;
     } else {
         uint32_t m = r[0];
 #pragma unroll
         for (int i = 1; i < W; i++) {
-            if constexpr (sizeof(T) == 2 && El<T>::NEG == El<__half>::NEG) asm("max.f16x2 %0, %0, %1;" : "+r"(m) : "r"(r[i]));
-            else asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(r[i]));
+            if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(m) : "r"(r[i]));
+            else asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(r[i]));
         }
         const float2 f = El<T>::two(&m, 0);
-        return fmaxf(f.x, f.y);
+        return max_nan(f.x, f.y);
     }
+}
+
+// The smallest of a thread's 16-bit values (none of them a NaN).
+template <typename T, int W>
+__device__ __forceinline__ float least_of(const uint32_t (&r)[W]) {
+    uint32_t m = r[0];
+#pragma unroll
+    for (int i = 1; i < W; i++) {
+        if constexpr (std::is_same<T, __half>::value) asm("min.f16x2 %0, %0, %1;" : "+r"(m) : "r"(r[i]));
+        else asm("min.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(r[i]));
+    }
+    const float2 f = El<T>::two(&m, 0);
+    return fminf(f.x, f.y);
 }
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-// The larger one, NaN if either is.
-__device__ __forceinline__ float max_nan(float x, float y) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(x), "f"(y));
-    return d;
 }
 // Two f32 operations in one instruction.
 __device__ __forceinline__ uint64_t two_f32(float x, float y) {
@@ -127,7 +165,7 @@ __device__ __forceinline__ float value_of(uint32_t o) {
 }
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t i) { return (uint64_t)order_of(x) << 32 | (uint32_t)~i; }
 
-// Running maximum, sum of 2^t and sum of t 2^t over t = (x - m) log2 e.
+// A reference near the running maximum (or minus infinity), sum of 2^t and sum of t 2^t over t = (x - m) log2 e.
 struct Sum {
     float m, z, zt;
 };
@@ -146,6 +184,19 @@ __device__ __forceinline__ Sum join(Sum a, Sum b) {
     return a;
 }
 
+// The sums of N neighbouring lanes together.
+template <int N>
+__device__ __forceinline__ Sum join_lanes(Sum a) {
+    float m = a.m;
+#pragma unroll
+    for (int o = 1; o < N; o <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    const float d = a.m == m ? 0.0f : (a.m - m) * LOG2E, w = ex2(d);
+    float z = a.z == 0.0f ? 0.0f : a.z * w, zt = a.z == 0.0f || w == 0.0f ? 0.0f : (a.zt + d * a.z) * w;
+#pragma unroll
+    for (int o = 1; o < N; o <<= 1) z += __shfl_xor_sync(~0u, z, o), zt += __shfl_xor_sync(~0u, zt, o);
+    return {m, z, zt};
+}
+
 struct Shared {
     Sum sum[WARPS], all[8];
     uint32_t ahead[WARPS], all_ahead[8];
@@ -160,6 +211,24 @@ struct Shared {
     float unit[UNITS + 1][THREADS];
 };
 
+// A row, or a CTA's part of it: `head` values up to the first 16-byte boundary, whole 16-byte words (this CTA's are
+// v0..v1), the rest.
+template <typename T>
+struct Row {
+    const T *x;
+    uint32_t head, tail, v0, v1, turns;
+    __device__ __forceinline__ Row(const LogprobsArgs &a, uint32_t row, uint32_t part, uint32_t parts) {
+        constexpr uint32_t N = El<T>::N;
+        x = (const T *)a.logits + (uint64_t)row * a.ld;
+        head = min(a.vocab, (uint32_t)((16 - ((uintptr_t)x & 15)) & 15) / (uint32_t)sizeof(T));
+        const uint32_t words = (a.vocab - head) / N;
+        tail = a.vocab - head - words * N;
+        v0 = (uint32_t)((uint64_t)words * part / parts), v1 = (uint32_t)((uint64_t)words * (part + 1) / parts);
+        turns = (v1 - v0 + LOADS * THREADS - 1) / (LOADS * THREADS);
+    }
+    __device__ __forceinline__ const uint4 *words() const { return reinterpret_cast<const uint4 *>(x + head); }
+};
+
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs a) {
     constexpr uint32_t N = El<T>::N;
@@ -167,21 +236,25 @@ __global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs
     Shared &s = *reinterpret_cast<Shared *>(smem);
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t parts = cluster.num_blocks(), part = cluster.block_rank();
-    auto started = cluster.barrier_arrive();  // waited for before another CTA's memory is written
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t row = blockIdx.x / parts;
-    const T *x = (const T *)a.logits + (uint64_t)row * a.ld;
+    const uint32_t row0 = blockIdx.x / parts, rows_apart = gridDim.x / parts;
+
+    if (parts > 1) cluster.sync();  // another CTA's memory may be written from here on
+
+    for (uint32_t row = row0; row < a.rows; row += rows_apart) {
+    const Row<T> R(a, row, part, parts);
+    const T *x = R.x;
+    const uint4 *xv = R.words();
+    const uint32_t head = R.head, tail = R.tail, v0 = R.v0, v1 = R.v1, turns = R.turns, per_unit = (turns + UNITS - 1) / UNITS;
     const int32_t tok = a.tokens ? a.tokens[row] : -1;
     const bool given = tok >= 0 && (uint32_t)tok < a.vocab;
     const float xt = given ? El<T>::get(x[tok]) : INFINITY;
-
-    // the row: `head` values up to the first 16-byte boundary, whole 16-byte words, the rest
-    const uint32_t head = min(a.vocab, (uint32_t)((16 - ((uintptr_t)x & 15)) & 15) / (uint32_t)sizeof(T));
-    const uint32_t words = (a.vocab - head) / N, tail = a.vocab - head - words * N;
-    const uint32_t v0 = (uint32_t)((uint64_t)words * part / parts), v1 = (uint32_t)((uint64_t)words * (part + 1) / parts);
+    uint32_t xt2 = 0;  // twice, in the logits' type
+    if constexpr (sizeof(T) == 2) {
+        const T v = given ? x[tok] : El<T>::inf();
+        xt2 = (uint32_t)*reinterpret_cast<const uint16_t *>(&v) * 0x10001u;
+    }
     const uint32_t begin = part == 0 ? 0 : head + v0 * N, end = part + 1 == parts ? a.vocab : head + v1 * N;  // this CTA's values
-    const uint4 *xv = reinterpret_cast<const uint4 *>(x + head);
-    const uint32_t turns = (v1 - v0 + LOADS * THREADS - 1) / (LOADS * THREADS), per_unit = (turns + UNITS - 1) / UNITS;
 
     Sum sum = {-INFINITY, 0.0f, 0.0f};
     uint64_t z2 = 0, zt2 = 0;  // the pair of sums at sum.m
@@ -192,33 +265,74 @@ __global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs
     auto add = [&](const uint32_t (&r)[LOADS * 4], uint32_t v) {
         const float m = max_of<T>(r);
         umax = fmaxf(umax, m);
-        if (m > sum.m) {
+        // the reference follows the maximum when that is LAG above it
+        if (m > sum.m + LAG) {
             const float d = (sum.m - m) * LOG2E, w = ex2(d);
             const float2 z = two_of(z2), zt = two_of(zt2);
             zt2 = two_f32(z.x == 0.0f ? 0.0f : (zt.x + d * z.x) * w, z.y == 0.0f ? 0.0f : (zt.y + d * z.y) * w);
             z2 = two_f32(z.x * w, z.y * w);
             sum.m = m;
         }
-        const float ref = sum.m == -INFINITY ? 0.0f : sum.m;  // where all is masked so far the terms are 0
-        const uint64_t nm = two_f32(-ref, -ref), l2 = two_f32(LOG2E, LOG2E);
+        const float ref = sum.m == -INFINITY ? 0.0f : -sum.m;
+        const uint64_t nm = two_f32(ref, ref), l2 = two_f32(LOG2E, LOG2E);
+        // t of masked values is held at -200, whose 2^t is 0 in f32, so that its product with t is 0 too
+        auto terms = [&](bool masked) {
 #pragma unroll
-        for (int i = 0; i < (int)(LOADS * N / 2); i++) {
-            const float2 f = El<T>::two(r, i), t = two_of(mul2(add2(two_f32(f.x, f.y), nm), l2));
-            const float t0 = max_nan(t.x, -200.0f), t1 = max_nan(t.y, -200.0f);  // 2^-200 is 0 in f32, and 0 * -200 too
-            const uint64_t e = two_f32(ex2(t0), ex2(t1));
-            z2 = add2(z2, e);
-            zt2 = fma2(e, two_f32(t0, t1), zt2);
-        }
-        if (m >= xt) {
-#pragma unroll
-            for (int j = 0; j < (int)LOADS; j++)
-#pragma unroll
-                for (int i = 0; i < (int)(N / 2); i++) {
-                    const float2 f = El<T>::two(r + 4 * j, i);
-                    const uint32_t at = head + (v + j * THREADS) * N + 2 * i;
-                    ahead += f.x > xt || (f.x == xt && at < (uint32_t)tok);
-                    ahead += f.y > xt || (f.y == xt && at + 1 < (uint32_t)tok);
+            for (int i = 0; i < (int)(LOADS * N / 2); i++) {
+                const float2 f = El<T>::two(r, i);
+                uint64_t t = mul2(add2(two_f32(f.x, f.y), nm), l2);
+                float2 tt = two_of(t);
+                if (masked) {
+                    tt.x = fmaxf(tt.x, -200.0f), tt.y = fmaxf(tt.y, -200.0f);
+                    t = two_f32(tt.x, tt.y);
                 }
+                const uint64_t e = two_f32(ex2(tt.x), ex2(tt.y));
+                z2 = add2(z2, e);
+                zt2 = fma2(e, t, zt2);
+            }
+        };
+        if (m != m) z2 = two_f32(NAN, NAN);
+        else if (m == -INFINITY) ;  // nothing to add
+        else if (sizeof(T) == 4 || !(least_of<T>(r) > -3e38f)) terms(true);
+        else terms(false);
+        if (m >= xt) {
+            // the values before the given token count when equal, those after it do not
+            const uint32_t at0 = head + v * N, at1 = at0 + (LOADS - 1) * THREADS * N;
+            if (v + (LOADS - 1) * THREADS < v1 && (at1 + N <= (uint32_t)tok || at0 > (uint32_t)tok)) {
+                const bool equal_too = at0 < (uint32_t)tok;
+                if constexpr (sizeof(T) == 4) {
+                    if (equal_too) {
+#pragma unroll
+                        for (int i = 0; i < (int)(LOADS * 4); i++) ahead += __uint_as_float(r[i]) >= xt;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < (int)(LOADS * 4); i++) ahead += __uint_as_float(r[i]) > xt;
+                    }
+                } else {
+                    uint32_t n2 = 0;
+                    if (equal_too) {
+#pragma unroll
+                        for (int i = 0; i < (int)(LOADS * 4); i++) n2 = add2_16<T>(n2, more2<T>(r[i], xt2, true));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < (int)(LOADS * 4); i++) n2 = add2_16<T>(n2, more2<T>(r[i], xt2, false));
+                    }
+                    const float2 n = El<T>::two(&n2, 0);
+                    ahead += (uint32_t)(n.x + n.y);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < (int)LOADS; j++) {
+                    const uint32_t at = head + (v + j * THREADS) * N;
+                    if (v + j * THREADS >= v1) continue;
+#pragma unroll
+                    for (int i = 0; i < (int)(N / 2); i++) {
+                        const float2 f = El<T>::two(r + 4 * j, i);
+                        ahead += f.x > xt || (f.x == xt && at + 2 * i < (uint32_t)tok);
+                        ahead += f.y > xt || (f.y == xt && at + 2 * i + 1 < (uint32_t)tok);
+                    }
+                }
+            }
         }
     };
     for (uint32_t turn = 0; turn < turns; turn++) {
@@ -244,7 +358,7 @@ __global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs
     if (tid < n_edge) {
         const float f = El<T>::get(x[edge]);
         const float2 z = two_of(z2), zt = two_of(zt2);
-        const Sum one = {f, f == -INFINITY ? 0.0f : 1.0f, 0.0f};
+        const Sum one = {f, f == -INFINITY ? 0.0f : f - f + 1.0f, 0.0f};
         const Sum got = join(Sum{sum.m, z.x + z.y, zt.x + zt.y}, one);
         sum.m = got.m, z2 = two_f32(got.z, 0.0f), zt2 = two_f32(got.zt, 0.0f);
         ahead += f > xt || (f == xt && edge < (uint32_t)tok);
@@ -258,11 +372,8 @@ __global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs
     }
 
     // the CTA's sums
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        sum = join(sum, Sum{__shfl_xor_sync(~0u, sum.m, o), __shfl_xor_sync(~0u, sum.z, o), __shfl_xor_sync(~0u, sum.zt, o)});
-        ahead += __shfl_xor_sync(~0u, ahead, o);
-    }
+    sum = join_lanes<32>(sum);
+    ahead = __reduce_add_sync(~0u, ahead);
     if (lane == 0) s.sum[warp] = sum, s.ahead[warp] = ahead;
     if (tid == 0) s.count = 0, s.found = 0, s.threshold = 0;
     if (a.top) {
@@ -271,9 +382,8 @@ __global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs
         if ((tid & 3) == 0) s.gmax[tid >> 2] = order_of(g);
     }
     __syncthreads();
-    sum = s.sum[0], ahead = s.ahead[0];
-#pragma unroll 1
-    for (uint32_t w = 1; w < WARPS; w++) sum = join(sum, s.sum[w]), ahead += s.ahead[w];
+    sum = join_lanes<WARPS>(s.sum[lane % WARPS]);
+    ahead = __reduce_add_sync(~0u, lane < WARPS ? s.ahead[lane] : 0u);
     const bool odd = sum.z != sum.z;  // a NaN, or infinities that cancel
 
     if (odd && given) {  // the comparisons above saw no NaN: count again by keys
@@ -287,7 +397,6 @@ __global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs
         ahead = 0;
         for (uint32_t w = 0; w < WARPS; w++) ahead += s.ahead[w];
     }
-    cluster.barrier_wait(std::move(started));
     if (tid == 0) {
         Shared &first = *cluster.map_shared_rank(&s, 0);
         first.all[part] = sum;
@@ -302,28 +411,31 @@ __global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs
         uint32_t n = 0;
         if (!odd) {
             // the top-th largest of the groups' maxima
-            if (tid < GROUPS) {
-                const uint32_t mine = s.gmax[tid];
-                uint32_t before = 0;
-#pragma unroll 8
-                for (uint32_t g = 0; g < GROUPS; g += 4) {
-                    const uint4 o = *reinterpret_cast<const uint4 *>(&s.gmax[g]);
-                    before += (o.x > mine || (o.x == mine && g < tid)) + (o.y > mine || (o.y == mine && g + 1 < tid));
-                    before += (o.z > mine || (o.z == mine && g + 2 < tid)) + (o.w > mine || (o.w == mine && g + 3 < tid));
+            {
+                const uint32_t mine = s.gmax[tid >> 2];
+                uint32_t more = 0, same = 0;
+#pragma unroll
+                for (uint32_t g = 0; g < GROUPS / 4; g += 4) {  // four threads, a quarter of the groups each
+                    const uint4 o = *reinterpret_cast<const uint4 *>(&s.gmax[(tid & 3) * 4 + g * 4]);
+                    more += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+                    same += (o.x == mine) + (o.y == mine) + (o.z == mine) + (o.w == mine);
                 }
-                if (before == k - 1) s.threshold = mine;
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) more += __shfl_xor_sync(~0u, more, o), same += __shfl_xor_sync(~0u, same, o);
+                if (more < k && more + same >= k) s.threshold = mine;
             }
             __syncthreads();
             // a threshold of minus infinity: all that is larger, and below as many of those that are not as can be needed
             const uint32_t t = s.threshold, least = t <= ORDER_NEG_INF ? ORDER_NEG_INF + 1 : t;
+            const float floor_x = value_of(least);
             auto push = [&](float f, uint32_t i) {
-                if (order_of(f) < least) return;
+                if (!(f >= floor_x)) return;
                 const uint32_t c = atomicAdd(&s.count, 1u);
                 if (c < CAP) s.cand[c] = key_of(f, i);
             };
-            if (order_of(tmax) >= least) {
+            if (tmax >= floor_x) {
                 for (uint32_t u = 0; u < units; u++) {
-                    if (order_of(s.unit[u][tid]) < least) continue;
+                    if (s.unit[u][tid] < floor_x) continue;
                     for (uint32_t turn = u * per_unit; turn < min(turns, (u + 1) * per_unit); turn++)
                         for (uint32_t j = 0; j < LOADS; j++) {
                             const uint32_t v = v0 + (turn * LOADS + j) * THREADS + tid;
@@ -410,16 +522,21 @@ __global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs
         }
         if (tid >= want && tid < k) list[tid] = 0;
     }
-    cluster.sync();
-    if (part) return;
+    if (parts > 1) {
+        cluster.sync();
+        if (part) return;  // a cluster has one row
+    } else {
+        __syncthreads();
+    }
 
     // ---- the row's results, in the first CTA ----
     sum = s.all[0], ahead = s.all_ahead[0];
     for (uint32_t p = 1; p < parts; p++) sum = join(sum, s.all[p]), ahead += s.all_ahead[p];
-    const bool none = sum.m == -INFINITY && sum.z == 0.0f;        // a row whose mask leaves nothing
+    const bool none = sum.m == -INFINITY && sum.z == 0.0f;          // a row whose mask leaves nothing
     const float lz = sum.m == INFINITY ? NAN : log2f(sum.z) * LN2;  // an infinite logit leaves no probabilities
+    auto logprob_of = [&](float v) { return none ? -INFINITY : v - sum.m - lz; };
     if (tid == 0) {
-        a.logprob[row] = !given ? NAN : none ? -INFINITY : xt - sum.m - lz;
+        a.logprob[row] = given ? logprob_of(xt) : NAN;
         a.entropy[row] = none ? 0.0f : lz - sum.zt / sum.z * LN2;
         a.rank[row] = given ? (int32_t)ahead : -1;
     }
@@ -430,8 +547,10 @@ __global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs
             for (uint32_t j = 0; j < parts * k; j++) before += s.top[j] > mine;
         if (mine && before < k) {
             a.top_ids[(uint64_t)row * k + before] = (int32_t)~(uint32_t)mine;
-            a.top_logprobs[(uint64_t)row * k + before] = none ? -INFINITY : value_of((uint32_t)(mine >> 32)) - sum.m - lz;
+            a.top_logprobs[(uint64_t)row * k + before] = logprob_of(value_of((uint32_t)(mine >> 32)));
         }
+    }
+    __syncthreads();
     }
 }
 
@@ -450,7 +569,7 @@ cudaError_t launch(const LogprobsArgs &a, int sms, cudaStream_t s) {
     uint32_t parts = 1;
     while (parts < 8 && a.rows * parts * 2 <= (uint32_t)sms * 2 && a.vocab >= 2 * parts * THREADS * El<T>::N) parts *= 2;
     cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(a.rows * parts);
+    c.gridDim = dim3(parts > 1 || a.rows < (uint32_t)sms * 2 ? a.rows * parts : sms * 2);
     c.blockDim = dim3(THREADS);
     c.dynamicSmemBytes = sizeof(Shared);
     c.stream = s;
