@@ -31,7 +31,7 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr uint32_t THREADS = 512, WARPS = THREADS / 32, GROUPS = THREADS / 4;
+constexpr uint32_t GROUPS = 128;  // of a CTA's threads, by their maxima
 constexpr uint32_t LOADS = 4;    // 16-byte loads of a thread in flight
 constexpr uint32_t UNITS = 8;    // stretches of a thread whose maxima are kept; one more for the row's ragged ends
 constexpr uint32_t CAP = 1536;   // candidates that are sorted by counting
@@ -197,7 +197,9 @@ __device__ __forceinline__ Sum join_lanes(Sum a) {
     return {m, z, zt};
 }
 
+template <uint32_t THREADS>
 struct Shared {
+    static constexpr uint32_t WARPS = THREADS / 32;
     Sum sum[WARPS], all[8];
     uint32_t ahead[WARPS], all_ahead[8];
     uint32_t gmax[GROUPS];
@@ -213,7 +215,7 @@ struct Shared {
 
 // A row, or a CTA's part of it: `head` values up to the first 16-byte boundary, whole 16-byte words (this CTA's are
 // v0..v1), the rest.
-template <typename T>
+template <typename T, uint32_t THREADS>
 struct Row {
     const T *x;
     uint32_t head, tail, v0, v1, turns;
@@ -229,9 +231,10 @@ struct Row {
     __device__ __forceinline__ const uint4 *words() const { return reinterpret_cast<const uint4 *>(x + head); }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs a) {
-    constexpr uint32_t N = El<T>::N;
+template <typename T, uint32_t THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const LogprobsArgs a) {
+    using Shared = Shared<THREADS>;
+    constexpr uint32_t N = El<T>::N, WARPS = THREADS / 32, PER_GROUP = THREADS / GROUPS;
     extern __shared__ __align__(16) uint8_t smem[];
     Shared &s = *reinterpret_cast<Shared *>(smem);
     cg::cluster_group cluster = cg::this_cluster();
@@ -242,7 +245,7 @@ __global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs
     if (parts > 1) cluster.sync();  // another CTA's memory may be written from here on
 
     for (uint32_t row = row0; row < a.rows; row += rows_apart) {
-    const Row<T> R(a, row, part, parts);
+    const Row<T, THREADS> R(a, row, part, parts);
     const T *x = R.x;
     const uint4 *xv = R.words();
     const uint32_t head = R.head, tail = R.tail, v0 = R.v0, v1 = R.v1, turns = R.turns, per_unit = (turns + UNITS - 1) / UNITS;
@@ -377,9 +380,10 @@ __global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs
     if (lane == 0) s.sum[warp] = sum, s.ahead[warp] = ahead;
     if (tid == 0) s.count = 0, s.found = 0, s.threshold = 0;
     if (a.top) {
-        float g = fmaxf(tmax, __shfl_xor_sync(~0u, tmax, 1));
-        g = fmaxf(g, __shfl_xor_sync(~0u, g, 2));
-        if ((tid & 3) == 0) s.gmax[tid >> 2] = order_of(g);
+        float g = tmax;
+#pragma unroll
+        for (int o = 1; o < (int)PER_GROUP; o <<= 1) g = fmaxf(g, __shfl_xor_sync(~0u, g, o));
+        if (tid % PER_GROUP == 0) s.gmax[tid / PER_GROUP] = order_of(g);
     }
     __syncthreads();
     sum = join_lanes<WARPS>(s.sum[lane % WARPS]);
@@ -412,16 +416,16 @@ __global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs
         if (!odd) {
             // the top-th largest of the groups' maxima
             {
-                const uint32_t mine = s.gmax[tid >> 2];
+                const uint32_t mine = s.gmax[tid / PER_GROUP];
                 uint32_t more = 0, same = 0;
 #pragma unroll
-                for (uint32_t g = 0; g < GROUPS / 4; g += 4) {  // four threads, a quarter of the groups each
-                    const uint4 o = *reinterpret_cast<const uint4 *>(&s.gmax[(tid & 3) * 4 + g * 4]);
+                for (uint32_t g = 0; g < GROUPS; g += 4 * PER_GROUP) {  // the group's threads share the others
+                    const uint4 o = *reinterpret_cast<const uint4 *>(&s.gmax[tid % PER_GROUP * 4 + g]);
                     more += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
                     same += (o.x == mine) + (o.y == mine) + (o.z == mine) + (o.w == mine);
                 }
 #pragma unroll
-                for (int o = 1; o < 4; o <<= 1) more += __shfl_xor_sync(~0u, more, o), same += __shfl_xor_sync(~0u, same, o);
+                for (int o = 1; o < (int)PER_GROUP; o <<= 1) more += __shfl_xor_sync(~0u, more, o), same += __shfl_xor_sync(~0u, same, o);
                 if (more < k && more + same >= k) s.threshold = mine;
             }
             __syncthreads();
@@ -472,7 +476,7 @@ __global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs
             uint32_t prefix = 0, need = want;
             for (int shift = 24; shift >= 0; shift -= 8) {
                 __syncthreads();
-                if (tid < 256) s.hist[tid] = 0;
+                for (uint32_t i = tid; i < 256; i += THREADS) s.hist[i] = 0;
                 __syncthreads();
                 for (uint32_t i = begin + tid; i < end; i += THREADS) {
                     const uint32_t o = order_of(El<T>::get(x[i]));
@@ -554,24 +558,22 @@ __global__ void __launch_bounds__(THREADS, 2) logprobs_kernel(const LogprobsArgs
     }
 }
 
-template <typename T>
-cudaError_t launch(const LogprobsArgs &a, int sms, cudaStream_t s) {
-    auto fn = logprobs_kernel<T>;
+template <typename T, uint32_t THREADS>
+cudaError_t launch_as(const LogprobsArgs &a, uint32_t parts, uint32_t grid, cudaStream_t s) {
+    auto fn = logprobs_kernel<T, THREADS>;
+    constexpr size_t smem = sizeof(Shared<THREADS>);
     static bool ready[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (!ready[dev & 63]) {
-        if ((e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared))) != cudaSuccess) return e;
+        if ((e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
         ready[dev & 63] = true;
     }
-    // as many CTAs a row as the device has room for two per SM, at most 8, and at least a turn of loads for each
-    uint32_t parts = 1;
-    while (parts < 8 && a.rows * parts * 2 <= (uint32_t)sms * 2 && a.vocab >= 2 * parts * THREADS * El<T>::N) parts *= 2;
     cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(parts > 1 || a.rows < (uint32_t)sms * 2 ? a.rows * parts : sms * 2);
+    c.gridDim = dim3(grid);
     c.blockDim = dim3(THREADS);
-    c.dynamicSmemBytes = sizeof(Shared);
+    c.dynamicSmemBytes = smem;
     c.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -579,6 +581,17 @@ cudaError_t launch(const LogprobsArgs &a, int sms, cudaStream_t s) {
     c.attrs = at;
     c.numAttrs = 1;
     return cudaLaunchKernelEx(&c, fn, a);
+}
+
+template <typename T>
+cudaError_t launch(const LogprobsArgs &a, int sms, cudaStream_t s) {
+    // Many rows: four CTAs of 256 threads an SM, so that the steps at the end of a row, which wait for one another,
+    // run beside the others' reading.  Fewer: CTAs of 512, two an SM, and as many of them a row as the device has
+    // room for, at most 8, while each has a turn of loads.
+    if (a.rows >= (uint32_t)sms * 2) return launch_as<T, 256>(a, 1, a.rows < (uint32_t)sms * 4 ? a.rows : sms * 4, s);
+    uint32_t parts = 1;
+    while (parts < 8 && a.rows * parts <= (uint32_t)sms && a.vocab >= 2 * parts * 512 * El<T>::N) parts *= 2;
+    return launch_as<T, 512>(a, parts, a.rows * parts, s);
 }
 
 }  // namespace
