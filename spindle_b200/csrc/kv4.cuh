@@ -91,6 +91,9 @@ constexpr int KV4_ROW_THREADS = 256;
 // Attention scratch: partial results of requests whose positions are spread over
 // several CTAs, and their arrival counters (zero between calls).
 constexpr uint64_t KV4_SCRATCH_BYTES = 16ull << 20;
+// The tensor-core kernel for many rows a head, and whether it is the faster one.
+cudaError_t kv4_prefill_launch(const Kv4AttnArgs &a, int32_t type, uint32_t d, cudaStream_t s);
+bool kv4_prefill_pays(const Kv4AttnArgs &a, int32_t type, uint32_t d, int sms);
 sg_status kv4_attention_launch(const Kv4AttnArgs &a, int32_t type, uint32_t d, int sms, cudaStream_t s, cudaError_t *err);
 
 }  // namespace sg

@@ -909,6 +909,10 @@ sg_status pick(const Kv4AttnArgs &a, uint32_t d, int sms, cudaStream_t s, cudaEr
 }  // namespace
 
 sg_status kv4_attention_launch(const Kv4AttnArgs &a, int32_t type, uint32_t d, int sms, cudaStream_t s, cudaError_t *err) {
+    if (kv4_prefill_pays(a, type, d, sms)) {
+        *err = kv4_prefill_launch(a, type, d, s);
+        return *err == cudaSuccess ? SG_OK : SG_ERR_CUDA;
+    }
     return type == SG_F32 ? pick<float>(a, d, sms, s, err) : type == SG_F16 ? pick<__half>(a, d, sms, s, err) : pick<__nv_bfloat16>(a, d, sms, s, err);
 }
 

@@ -1,0 +1,600 @@
+// kv4_prefill.cu — attention over the paged 4-bit KV cache for many query rows
+// per KV head (prompt chunks, large verify batches), f16 and bf16: what bounds it
+// is the tensor cores, so the products run on tcgen05 with the sums in TMEM.
+//
+// A CTA has NQ tiles of 128 query rows (a row is a (token, head of the group)
+// pair) of one request and KV head, and goes over the positions NK at a time:
+//   - warps of 128 threads per tile: a thread per row takes its scores from
+//     TMEM, keeps the running maximum and sum, and puts its weights back in f16;
+//   - ND threads turn the codes into f16 operands in shared memory, two buffers;
+//   - one thread issues the tensor products: the next scores before this step's
+//     sums, so that the tensor cores work while the weights are made.
+// The scores are as good as f32: with K values m + s c (16-bit s and m, a code c)
+// s c goes in as its f16 rounding and the exact rest, and the minima as 16 more
+// columns against the sums of the query's groups (f16 rounding and rest).  V
+// values and weights are rounded to f16 once each.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "kv4.cuh"
+
+namespace sg {
+
+namespace {
+
+constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
+constexpr float P_SHIFT = 6.0f, LAG = 8.0f;  // weights are held as 2^6 p, p below 2^8: inside f16's range
+
+template <int D>
+struct Pre {
+    static constexpr int G = D / 32;
+    static constexpr int NQ = D == 256 ? 1 : 2, NK = D == 256 ? 32 : 64;
+    static constexpr int ND = D == 256 ? 256 : 128;                 // threads that make operands
+    static constexpr int THREADS = 128 * NQ + ND + 32;
+    static constexpr int GV = NK * G / ND;                          // groups of V that one of them makes
+    static constexpr int KI = NK * 4 * (G == 8 ? 2 : 1) / ND;       // positions of K
+    static constexpr uint32_t SBO_Q = (D / 8 + 2) * 128, SBO_K = D / 8 * 128, SBO_M = 256, SBO_V = NK * 16 + 16;
+    static constexpr uint32_t Q_BYTES = 16 * SBO_Q;                 // 128 rows
+    static constexpr uint32_t K_BYTES = NK / 8 * SBO_K, M_BYTES = NK / 8 * SBO_M, V_BYTES = D / 8 * SBO_V;
+    static constexpr uint32_t BUF = 2 * K_BYTES + M_BYTES + V_BYTES;
+    static constexpr uint32_t SMEM = NQ * Q_BYTES + 2 * BUF + 256;
+    // TMEM columns: scores, weights (two f16 a column), sums
+    static constexpr uint32_t S_COL = 0, P_COL = 128, O_COL = 256;
+    static_assert(GV >= 1 && KI >= 1 && SMEM <= 227 * 1024, "shapes");
+};
+
+__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t sbo) {
+    // K-major, no swizzle: core matrices of 8 rows x 16 bytes, 128 bytes apart along K, sbo apart along the rows
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(128u >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | (1ull << 46);
+}
+constexpr uint32_t idesc(uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((128u >> 4) << 24); }  // f16 x f16 -> f32, M = 128
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t add) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b),
+                 "r"(id), "r"(add)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t add) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b),
+                 "r"(id), "r"(add)
+                 : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void arrive(uint64_t *bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory"); }
+
+// 32 columns of this thread's lane
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t hneg2(uint32_t a) {
+    uint32_t d;
+    asm("neg.f16x2 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// The four pairs of a word's codes as f16 numbers: nibbles (0, 4), (1, 5), (2, 6), (3, 7).
+__device__ __forceinline__ void codes(uint32_t w, uint32_t (&c)[4]) {
+    const uint32_t h = w >> 8;
+    c[0] = hsub2((w & 0x000F000Fu) | 0x64006400u, 0x64006400u);  // 1024 + c
+    c[1] = hsub2((w & 0x00F000F0u) | 0x54005400u, 0x54005400u);  // 64 + c
+    c[2] = hsub2((h & 0x000F000Fu) | 0x64006400u, 0x64006400u);
+    c[3] = hsub2((h & 0x00F000F0u) | 0x54005400u, 0x54005400u);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) {
+    if constexpr (std::is_same<T, __half>::value) return __half2float(v);
+    else return __bfloat162float(v);
+}
+template <typename T>
+__device__ __forceinline__ T from_f32(float v) {
+    if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
+    else return __float2bfloat16_rn(v);
+}
+
+template <int N>
+__device__ __forceinline__ void ldg_words(uint32_t (&w)[N], const uint8_t *p) {
+    if constexpr (N == 1) w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
+    else if constexpr (N == 2) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
+        w[0] = v.x, w[1] = v.y;
+    } else {
+        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    }
+}
+
+}  // namespace
+
+template <typename T, int D>
+__global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
+    using L = Kv4Tile<D>;
+    using C = Pre<D>;
+    constexpr int G = C::G, NQ = C::NQ, NK = C::NK, ND = C::ND, GV = C::GV, KI = C::KI;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t *q_s = smem, *buf_s = smem + NQ * C::Q_BYTES;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(buf_s + 2 * C::BUF);
+    uint64_t *kv_full = bars, *kv_free = bars + 2, *s_full = bars + 4, *s_free = bars + 6, *p_full = bars + 8, *pv_done = bars + 10;
+    uint64_t *drain = bars + 12;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 13);
+    volatile uint32_t *dead = tmem_slot + 1;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t req = blockIdx.z, head = blockIdx.y;
+
+    // tokens of no request: zeros, and no sum
+    if (a.last && req == 0) {
+        const uint32_t spare = min((uint32_t)max(a.cu[a.n_req], 0), a.n_tok), all = (a.n_tok - spare) * a.n_heads;
+        for (uint32_t r = (blockIdx.y * gridDim.x + blockIdx.x) * (C::THREADS / 32) + warp; r < all; r += gridDim.x * gridDim.y * (C::THREADS / 32)) {
+            const uint64_t t = spare + r / a.n_heads, h = r % a.n_heads;
+            for (uint32_t d = lane; d < D; d += 32) ((T *)a.out)[t * a.o_tok + h * a.o_head + d] = from_f32<T>(0.0f);
+            if (a.lse && lane == 0) a.lse[t * a.n_heads + h] = -INFINITY;
+        }
+    }
+
+    // this CTA's rows; the requests' last tiles, which see most, come first
+    const int32_t tok0 = max(a.cu[req], 0), nq = max(min(a.cu[req + 1], (int32_t)a.n_tok) - tok0, 0);
+    const uint32_t rows = (uint32_t)nq * a.group, tile = gridDim.x - 1 - blockIdx.x, row0 = tile * (128 * NQ);
+    if (row0 >= rows) return;
+    const uint32_t halves = min((uint32_t)NQ, (rows - row0 + 127) / 128);
+    const int32_t seq = max(a.seq[req], 0);
+    const int32_t end = (int32_t)min((int64_t)seq, (int64_t)a.width << a.c.page_shift);
+    const uint32_t last_row = min(rows, row0 + 128 * NQ) - 1;
+    const int64_t first_place = (int64_t)seq - nq + row0 / a.group, last_place = (int64_t)seq - nq + last_row / a.group;
+    const int32_t see_lo = a.window && first_place + 1 > (int64_t)a.window ? (int32_t)(first_place + 1 - a.window) : 0;
+    const int32_t see_hi = (int32_t)max((int64_t)0, min(last_place + 1, (int64_t)end));
+    const int32_t k0 = min(see_lo, see_hi) / NK, k1 = (see_hi + NK - 1) / NK;
+    const uint32_t n = (uint32_t)max(k1 - k0, 0);  // steps
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&kv_full[i], ND);
+            mbar_init(&kv_free[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&s_free[i], 128);
+            mbar_init(&p_full[i], 128);
+            mbar_init(&pv_done[i], 1);
+        }
+        mbar_init(drain, 1);
+        fence_mbar_init();
+        *dead = 0;
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+
+    // ---- the query rows, a thread each: scaled by a power of two, in the order of the K operand, and their groups' sums ----
+    float cs = 0.0f;
+    if (tid < 128 * NQ) {
+        const uint32_t r = row0 + tid, rr = min(r, rows - 1), tok = rr / a.group, hq = head * a.group + rr % a.group;
+        const T *q = (const T *)a.q + (uint64_t)(tok0 + tok) * a.q_tok + hq * a.q_head;
+        auto load8 = [&](uint32_t c, float (&x)[8]) {
+            alignas(16) T v[8];
+            if (a.vec_q) {
+                *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(q + c * 8));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = q[c * 8 + i];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = to_f32(v[i]);
+        };
+        float amax = 0.0f, x[8];
+        for (int c = 0; c < D / 8; c++) {
+            load8(c, x);
+#pragma unroll
+            for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[i]));
+        }
+        // q * 2^(6 - e) is below 2^7; the K operand is half of s c
+        const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 116);
+        const float up = copysignf(__uint_as_float((uint32_t)(127 + 6 - e) << 23), a.scale);
+        cs = fabsf(a.scale) * LOG2E * 2.0f * __uint_as_float((uint32_t)(127 - 6 + e) << 23);
+        uint8_t *dst = q_s + tid / 128 * C::Q_BYTES + tid % 128 / 8 * C::SBO_Q + tid % 8 * 16;
+        float sum[G];
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            sum[g] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                load8(g * 4 + c, x);
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] *= up, sum[g] += x[i];
+                *reinterpret_cast<uint4 *>(dst + (g * 4 + c) * 128) = make_uint4(pack2(x[0], x[4]), pack2(x[1], x[5]), pack2(x[2], x[6]), pack2(x[3], x[7]));
+            }
+            sum[g] *= 0.5f;
+        }
+        // 16 columns: the sums' f16 roundings, what those left, zeros
+        __half col[16];
+#pragma unroll
+        for (int k = 0; k < 16; k++) {
+            const float s = sum[k % G], h = __half2float(__float2half_rn(s));
+            col[k] = __float2half_rn(k < G ? s : k < 2 * G ? s - h : 0.0f);
+        }
+        *reinterpret_cast<uint4 *>(dst + D / 8 * 128) = *reinterpret_cast<const uint4 *>(col);
+        *reinterpret_cast<uint4 *>(dst + (D / 8 + 1) * 128) = *reinterpret_cast<const uint4 *>(col + 8);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+        if (*dead) return;
+        if (!mbar_wait_bounded(bar, parity, WAIT_LIMIT_NS)) {
+            *dead = 1;
+            atomicExch(&g_dev_status, (unsigned)DEV_TIMEOUT_TMA);
+        }
+    };
+
+    if (warp == (128 * NQ + ND) / 32) {
+        // ---- the tensor products ----
+        if (lane == 0) {
+            const uint32_t qa = smem_u32(q_s), ba = smem_u32(buf_s);
+            auto scores = [&](uint32_t i) {
+                const uint32_t b = i & 1, k = ba + b * C::BUF;
+                wait(&kv_full[b], i >> 1 & 1);
+                for (uint32_t h = 0; h < halves; h++) {
+                    wait(&s_free[h], (i & 1) ^ 1);
+                    fence_after();
+                    if (*dead) continue;
+                    const uint32_t d = tmem + C::S_COL + h * NK, qh = qa + h * C::Q_BYTES;
+#pragma unroll 1
+                    for (uint32_t c = 0; c < D / 8; c += 2) {
+                        const uint64_t qd = smem_desc(qh + c * 128, C::SBO_Q);
+                        mma_ss(d, qd, smem_desc(k + c * 128, C::SBO_K), idesc(NK), c != 0);
+                        mma_ss(d, qd, smem_desc(k + C::K_BYTES + c * 128, C::SBO_K), idesc(NK), 1);
+                    }
+                    mma_ss(d, smem_desc(qh + D / 8 * 128, C::SBO_Q), smem_desc(k + 2 * C::K_BYTES, C::SBO_M), idesc(NK), 1);
+                    commit(&s_full[h]);
+                }
+            };
+            if (n) scores(0);
+            for (uint32_t i = 0; i < n; i++) {
+                if (i + 1 < n) scores(i + 1);
+                const uint32_t b = i & 1, v = ba + b * C::BUF + 2 * C::K_BYTES + C::M_BYTES;
+                for (uint32_t h = 0; h < halves; h++) {
+                    wait(&p_full[h], i & 1);
+                    fence_after();
+                    if (*dead) continue;
+                    const uint32_t d = tmem + C::O_COL + h * D, p = tmem + C::P_COL + h * (NK / 2);
+#pragma unroll 1
+                    for (uint32_t c = 0; c < NK / 16; c++) mma_ts(d, p + c * 8, smem_desc(v + c * 256, C::SBO_V), idesc(D), i != 0 || c != 0);
+                    commit(&pv_done[h]);
+                }
+                if (!*dead) commit(&kv_free[b]);
+            }
+            if (*dead) {  // what is still running must end before its memory goes
+                commit(drain);
+                mbar_wait_bounded(drain, 0, WAIT_LIMIT_NS / 10);
+            }
+        }
+        __syncwarp();
+    } else if (tid >= 128 * NQ) {
+        // ---- the operands of a step from the cache: its codes are read a step ahead, its table entries two ----
+        const uint32_t dt = tid - 128 * NQ, dw = dt >> 5, x8 = lane & 7, y4 = lane >> 3;
+        // K: positions of this thread (its word part j = y4); V: the 8 positions tb, word part x8, groups from gq * GV on
+        constexpr int HALF = G == 8 ? 2 : 1;
+        const uint32_t ka = HALF == 2 ? dw / (NK / 8) : 0;  // D = 256: which half of the groups
+        auto kpos = [&](int i) { return HALF == 2 ? dw % (NK / 8) * 8 + x8 : (uint32_t)(i * (ND / 32) + dw) * 8 + x8; };
+        const uint32_t vi = dw * 4 + y4, tb = vi % (NK / 8), gq = vi / (NK / 8);
+        const int32_t *table = a.tables + (uint64_t)req * a.ld_tables;
+        const uint32_t shift = a.c.page_shift;
+        auto entry = [&](int32_t pos) { return pos < end ? __ldg(table + (pos >> shift)) : -1; };
+        auto tile_of = [&](int32_t blk, int32_t pos) {
+            return a.c.data + (uint32_t)blk * a.block_bytes + ((((uint64_t)head << (shift - 4)) + ((pos & ((1 << shift) - 1)) >> 4)) * L::BYTES);
+        };
+        constexpr int KG = G < 4 ? G : 4;  // groups of a K item
+        int32_t kb[KI], vb;
+        uint32_t kr[KI][KG], ks[KI][KG], km[KI][KG / 2], vr[4][GV], vs[4][GV], vm[4][GV];
+        bool k_ok[KI], v_ok;
+        auto entries = [&](uint32_t i) {
+            const int32_t t = (k0 + (int32_t)i) * NK;
+#pragma unroll
+            for (int j = 0; j < KI; j++) kb[j] = entry(t + kpos(j));
+            vb = entry(t + tb * 8);
+        };
+        auto load = [&](uint32_t i) {
+            const int32_t t = (k0 + (int32_t)i) * NK;
+#pragma unroll
+            for (int j = 0; j < KI; j++) {
+                const int32_t pos = t + kpos(j);
+                const uint32_t p = pos & 15;
+                k_ok[j] = pos < end && (uint32_t)kb[j] < a.c.n_blocks;
+                if (k_ok[j]) {
+                    const uint8_t *tl = tile_of(kb[j], pos);
+                    ldg_words<KG>(kr[j], tl + p * L::KROW + (G < 4 ? y4 * G : (ka * 4 + y4) * 4) * 4);
+                    ldg_words<KG>(ks[j], tl + L::KS + (p >> 1) * (G * 4) + ka * 16);
+                    ldg_words<KG / 2>(km[j], tl + L::KM + p * (G * 2) + ka * 8);
+                }
+            }
+            const int32_t pos = t + tb * 8;
+            v_ok = pos < end && (uint32_t)vb < a.c.n_blocks;
+            if (v_ok) {
+                const uint8_t *tl = tile_of(vb, pos);
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const uint32_t pair = ((pos & 15) >> 1) + q, g0 = gq * GV;
+                    ldg_words<GV>(vr[q], tl + L::VC + pair * L::VROW + kv4_word(x8, g0, 8, G) * 4);
+                    ldg_words<GV>(vs[q], tl + L::VS + (pair * G + g0) * 4);
+                    ldg_words<GV>(vm[q], tl + L::VM + (pair * G + g0) * 4);
+                }
+            }
+        };
+        if (n) {
+            entries(0);
+            load(0);
+            if (n > 1) entries(1);
+        }
+        for (uint32_t i = 0; i < n; i++) {
+            const uint32_t b = i & 1;
+            wait(&kv_free[b], (i >> 1 & 1) ^ 1);
+            uint8_t *k_hi = buf_s + b * C::BUF, *k_lo = k_hi + C::K_BYTES, *k_m = k_lo + C::K_BYTES, *v_t = k_m + C::M_BYTES;
+            const int32_t t = (k0 + (int32_t)i) * NK;
+#pragma unroll
+            for (int j = 0; j < KI; j++) {
+                const uint32_t pos = kpos(j);
+                uint8_t *hi = k_hi + (pos >> 3) * C::SBO_K + (pos & 7) * 16, *lo = k_lo + (pos >> 3) * C::SBO_K + (pos & 7) * 16;
+#pragma unroll
+                for (int g = 0; g < KG; g++) {
+                    uint32_t c[4], h[4], l[4];
+                    // the position's scale twice, halved
+                    uint32_t s = k_ok[j] ? __byte_perm(ks[j][g], 0, pos & 1 ? 0x3232 : 0x1010) : 0u;
+                    s = hmul2(s, 0x38003800u);
+                    codes(k_ok[j] ? kr[j][g] : 0u, c);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) h[k] = hmul2(c[k], s), l[k] = hfma2(c[k], s, hneg2(h[k]));
+                    const uint32_t chunk = ((G < 4 ? g : ka * 4 + g) * 4 + y4) * 128;
+                    *reinterpret_cast<uint4 *>(hi + chunk) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4 *>(lo + chunk) = make_uint4(l[0], l[1], l[2], l[3]);
+                }
+                if (y4 == 0) {
+                    // the minima: groups 0..G-1 and again, against the sums' roundings and rests
+                    uint8_t *m = k_m + (pos >> 3) * C::SBO_M + (pos & 7) * 16;
+                    uint32_t w[KG / 2];
+#pragma unroll
+                    for (int g = 0; g < KG / 2; g++) w[g] = k_ok[j] ? km[j][g] : 0u;
+                    if constexpr (G == 2) {
+                        *reinterpret_cast<uint4 *>(m) = make_uint4(w[0], w[0], 0u, 0u);
+                        *reinterpret_cast<uint4 *>(m + 128) = make_uint4(0u, 0u, 0u, 0u);
+                    } else if constexpr (G == 4) {
+                        *reinterpret_cast<uint4 *>(m) = make_uint4(w[0], w[1], w[0], w[1]);
+                        *reinterpret_cast<uint4 *>(m + 128) = make_uint4(0u, 0u, 0u, 0u);
+                    } else {
+                        *reinterpret_cast<uint2 *>(m + ka * 8) = make_uint2(w[0], w[1]);
+                        *reinterpret_cast<uint2 *>(m + 128 + ka * 8) = make_uint2(w[0], w[1]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < GV; g++) {
+                uint32_t val[4][4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int32_t p = t + (int32_t)tb * 8 + 2 * q;
+                    const uint32_t mask = !v_ok || p >= end ? 0u : p + 1 >= end ? 0xFFFFu : 0xFFFFFFFFu;
+                    const uint32_t s = vs[q][g] & mask, m = vm[q][g] & mask;
+                    uint32_t c[4];
+                    codes(vr[q][g], c);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) val[k][q] = hfma2(c[k], s, m);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t d = 32 * (gq * GV + g) + 4 * x8 + k;
+                    *reinterpret_cast<uint4 *>(v_t + (d >> 3) * C::SBO_V + tb * 128 + (d & 7) * 16) = make_uint4(val[k][0], val[k][1], val[k][2], val[k][3]);
+                }
+            }
+            if (i + 1 < n) {
+                load(i + 1);
+                if (i + 2 < n) entries(i + 2);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            arrive(&kv_full[b]);
+        }
+    } else if (tid < 128 * halves) {
+        // ---- the weights: a thread per row ----
+        const uint32_t h = tid >> 7, row = row0 + tid, rr = min(row, rows - 1);
+        const bool live = row < rows;
+        const uint32_t mine = tmem + ((warp & 3) << 21);  // this warp's 32 lanes
+        const int64_t place = (int64_t)seq - nq + rr / a.group;
+        const int32_t hi_t = live ? (int32_t)max((int64_t)0, min(place + 1, (int64_t)end)) : 0;
+        const int32_t lo_t = a.window && place + 1 > (int64_t)a.window ? (int32_t)(place + 1 - a.window) : 0;
+        const int32_t *table = a.tables + (uint64_t)req * a.ld_tables;
+        float m = -INFINITY, l = 0.0f;
+        for (uint32_t i = 0; i < n; i++) {
+            const int32_t t0 = (k0 + (int32_t)i) * NK;
+            wait(&s_full[h], i & 1);
+            __syncwarp();
+            fence_after();
+            uint32_t s[NK / 32][32];
+#pragma unroll
+            for (int c = 0; c < NK / 32; c++) tmem_ld32(mine + C::S_COL + h * NK + c * 32, s[c]);
+            fence_before();
+            arrive(&s_free[h]);
+            // the pages of this step that are there, a bit per 16 positions
+            uint32_t there = 0;
+            if (t0 < end) {
+                for (int c = 0; c < NK / 16; c++) there |= (uint32_t)(t0 + 16 * c < end && (uint32_t)__ldg(table + ((t0 + 16 * c) >> a.c.page_shift)) < a.c.n_blocks) << c;
+            }
+            float top = -INFINITY;
+            if (t0 < lo_t || t0 + NK > hi_t || there != (1u << (NK / 16)) - 1) {
+#pragma unroll
+                for (int c = 0; c < NK; c++)
+                    if (t0 + c < lo_t || t0 + c >= hi_t || !(there >> (c / 16) & 1)) s[c / 32][c % 32] = 0xFF800000u;
+            }
+#pragma unroll
+            for (int c = 0; c < NK; c++) top = fmaxf(top, __uint_as_float(s[c / 32][c % 32]));
+            top *= cs;
+            // the reference of the weights follows the maximum when that is 2^LAG above it
+            const bool up = top > m + LAG;
+            float f = 1.0f;
+            if (up) {
+                f = ex2(m - top);
+                m = top;
+                l *= f;
+            }
+            const float shift = m == -INFINITY ? 0.0f : P_SHIFT - m;
+            uint32_t p[NK / 2];
+            float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NK; c += 2) {
+                const float p0 = ex2(fmaf(__uint_as_float(s[c / 32][c % 32]), cs, shift)), p1 = ex2(fmaf(__uint_as_float(s[c / 32][c % 32 + 1]), cs, shift));
+                l0 += p0, l1 += p1;
+                p[c / 2] = pack2(p0, p1);
+            }
+            l += l0 + l1;
+            if (i) {
+                wait(&pv_done[h], (i - 1) & 1);
+                __syncwarp();
+                fence_after();
+                if (__any_sync(~0u, up)) {
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(mine + C::O_COL + h * D + c, o);
+#pragma unroll
+                        for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                        tmem_st16(mine + C::O_COL + h * D + c, o);
+                        tmem_st16(mine + C::O_COL + h * D + c + 16, o + 16);
+                    }
+                }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < NK / 2; c += 16) tmem_st16(mine + C::P_COL + h * (NK / 2) + c, p + c);
+            tmem_st_wait();
+            fence_before();
+            arrive(&p_full[h]);
+        }
+        // ---- the results ----
+        if (n) {
+            wait(&pv_done[h], (n - 1) & 1);
+            __syncwarp();
+            fence_after();
+        }
+        const uint32_t tok = rr / a.group, hq = head * a.group + rr % a.group;
+        const uint64_t t = (uint64_t)tok0 + tok;
+        T *out = (T *)a.out + t * a.o_tok + hq * a.o_head;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            __syncwarp();
+            if (n) tmem_ld32(mine + C::O_COL + h * D + c, o);
+            if (live) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 8) {
+                    alignas(16) T y[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) y[j] = from_f32<T>(l == 0.0f ? 0.0f : __uint_as_float(o[k + j]) * inv);
+                    if (a.vec_out) {
+                        *reinterpret_cast<uint4 *>(out + c + k) = *reinterpret_cast<const uint4 *>(y);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) out[c + k + j] = y[j];
+                    }
+                }
+            }
+        }
+        if (live && a.lse) a.lse[t * a.n_heads + hq] = l == 0.0f ? -INFINITY : (m - P_SHIFT + log2f(l)) * LN2;
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+namespace {
+
+template <typename T, int D>
+cudaError_t launch(const Kv4AttnArgs &a, cudaStream_t s) {
+    using C = Pre<D>;
+    auto fn = kv4_prefill_kernel<T, D>;
+    static bool ready[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (!ready[dev & 63]) {
+        if ((e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) != cudaSuccess) return e;
+        ready[dev & 63] = true;
+    }
+    const uint32_t tiles = (uint32_t)(((uint64_t)a.max_new * a.group + 128 * C::NQ - 1) / (128 * C::NQ));
+    for (uint32_t r0 = 0; r0 < a.n_req; r0 += 32768) {
+        Kv4AttnArgs b = a;
+        b.n_req = a.n_req - r0 < 32768 ? a.n_req - r0 : 32768;
+        b.last = r0 + b.n_req == a.n_req;
+        b.cu += r0, b.seq += r0, b.tables += (uint64_t)r0 * a.ld_tables;
+        fn<<<dim3(tiles, a.c.heads, b.n_req), C::THREADS, C::SMEM, s>>>(b);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t kv4_prefill_launch(const Kv4AttnArgs &a, int32_t type, uint32_t d, cudaStream_t s) {
+    if (type == SG_F16) return d == 64 ? launch<__half, 64>(a, s) : d == 128 ? launch<__half, 128>(a, s) : launch<__half, 256>(a, s);
+    return d == 64 ? launch<__nv_bfloat16, 64>(a, s) : d == 128 ? launch<__nv_bfloat16, 128>(a, s) : launch<__nv_bfloat16, 256>(a, s);
+}
+
+bool kv4_prefill_pays(const Kv4AttnArgs &a, int32_t type, uint32_t d, int sms) {
+    if (type == SG_F32 || a.n_req == 0) return false;
+    // Device cycles per cached position, both measured on a long context of heads of 128: the tensor-core kernel
+    // takes 26 a wave of its CTAs (256 rows each, 128 where a head has 256 values), the other one 0.007 a row.
+    const uint64_t per = d == 256 ? 128 : 256, rows = (uint64_t)a.n_tok * a.group;
+    const uint64_t ctas = (rows / per + a.n_req) * a.c.heads, waves = (ctas + sms - 1) / sms;
+    return rows * a.c.heads * 7 > waves * 26000;
+}
+
+}  // namespace sg
