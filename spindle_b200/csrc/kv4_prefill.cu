@@ -51,15 +51,21 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t sbo) {
 }
 constexpr uint32_t idesc(uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((128u >> 4) << 24); }  // f16 x f16 -> f32, M = 128
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t add) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b),
-                 "r"(id), "r"(add)
-                 : "memory");
+// d (+)= a b: the first product of a sum and the others
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool add) {
+    if (add) asm volatile("{\n .reg .pred p;\n setp.eq.b32 p, 0, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(id) : "memory");
+    else asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, 0, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(id) : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t add) {
     asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b),
                  "r"(id), "r"(add)
                  : "memory");
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ void commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -276,46 +282,58 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
     };
 
     if (warp == (128 * NQ + ND) / 32) {
-        // ---- the tensor products ----
-        if (lane == 0) {
-            const uint32_t qa = smem_u32(q_s), ba = smem_u32(buf_s);
-            auto scores = [&](uint32_t i) {
-                const uint32_t b = i & 1, k = ba + b * C::BUF;
-                wait(&kv_full[b], i >> 1 & 1);
-                for (uint32_t h = 0; h < halves; h++) {
-                    wait(&s_free[h], (i & 1) ^ 1);
-                    fence_after();
-                    if (*dead) continue;
-                    const uint32_t d = tmem + C::S_COL + h * NK, qh = qa + h * C::Q_BYTES;
+        // ---- the tensor products: the warp goes together, one lane issues ----
+        const uint32_t base = smem_u32(smem), tm = __shfl_sync(~0u, tmem, 0);
+        const uint64_t q_desc = smem_desc(base, C::SBO_Q), k_desc = smem_desc(base + NQ * C::Q_BYTES, C::SBO_K),
+                       m_desc = smem_desc(base + NQ * C::Q_BYTES + 2 * C::K_BYTES, C::SBO_M),
+                       v_desc = smem_desc(base + NQ * C::Q_BYTES + 2 * C::K_BYTES + C::M_BYTES, C::SBO_V);
+        auto scores = [&](uint32_t i) {
+            const uint32_t b = i & 1;
+            const uint64_t off = b * (C::BUF >> 4);
+            wait(&kv_full[b], i >> 1 & 1);
 #pragma unroll 1
+            for (uint32_t h = 0; h < halves; h++) {
+                wait(&s_free[h], (i & 1) ^ 1);
+                __syncwarp();
+                fence_after();
+                if (elect_one() && !*dead) {
+                    const uint32_t d = tm + C::S_COL + h * NK;
+                    const uint64_t qd = q_desc + h * (C::Q_BYTES >> 4), kd = k_desc + off;
+#pragma unroll
                     for (uint32_t c = 0; c < D / 8; c += 2) {
-                        const uint64_t qd = smem_desc(qh + c * 128, C::SBO_Q);
-                        mma_ss(d, qd, smem_desc(k + c * 128, C::SBO_K), idesc(NK), c != 0);
-                        mma_ss(d, qd, smem_desc(k + C::K_BYTES + c * 128, C::SBO_K), idesc(NK), 1);
+                        mma_ss(d, qd + c * 8, kd + c * 8, idesc(NK), c != 0);
+                        mma_ss(d, qd + c * 8, kd + (C::K_BYTES >> 4) + c * 8, idesc(NK), true);
                     }
-                    mma_ss(d, smem_desc(qh + D / 8 * 128, C::SBO_Q), smem_desc(k + 2 * C::K_BYTES, C::SBO_M), idesc(NK), 1);
+                    mma_ss(d, qd + D, m_desc + off, idesc(NK), true);
                     commit(&s_full[h]);
                 }
-            };
-            if (n) scores(0);
-            for (uint32_t i = 0; i < n; i++) {
-                if (i + 1 < n) scores(i + 1);
-                const uint32_t b = i & 1, v = ba + b * C::BUF + 2 * C::K_BYTES + C::M_BYTES;
-                for (uint32_t h = 0; h < halves; h++) {
-                    wait(&p_full[h], i & 1);
-                    fence_after();
-                    if (*dead) continue;
-                    const uint32_t d = tmem + C::O_COL + h * D, p = tmem + C::P_COL + h * (NK / 2);
+                __syncwarp();
+            }
+        };
+        if (n) scores(0);
 #pragma unroll 1
-                    for (uint32_t c = 0; c < NK / 16; c++) mma_ts(d, p + c * 8, smem_desc(v + c * 256, C::SBO_V), idesc(D), i != 0 || c != 0);
+        for (uint32_t i = 0; i < n; i++) {
+            if (i + 1 < n) scores(i + 1);
+            const uint32_t b = i & 1;
+            const uint64_t vd = v_desc + b * (C::BUF >> 4);
+#pragma unroll 1
+            for (uint32_t h = 0; h < halves; h++) {
+                wait(&p_full[h], i & 1);
+                __syncwarp();
+                fence_after();
+                if (elect_one() && !*dead) {
+                    const uint32_t d = tm + C::O_COL + h * D, p = tm + C::P_COL + h * (NK / 2);
+#pragma unroll
+                    for (uint32_t c = 0; c < NK / 16; c++) mma_ts(d, p + c * 8, vd + c * 16, idesc(D), c ? 1u : i);
                     commit(&pv_done[h]);
+                    if (h + 1 == halves) commit(&kv_free[b]);
                 }
-                if (!*dead) commit(&kv_free[b]);
+                __syncwarp();
             }
-            if (*dead) {  // what is still running must end before its memory goes
-                commit(drain);
-                mbar_wait_bounded(drain, 0, WAIT_LIMIT_NS / 10);
-            }
+        }
+        if (*dead && lane == 0) {  // what is still running must end before its memory goes
+            commit(drain);
+            mbar_wait_bounded(drain, 0, WAIT_LIMIT_NS / 10);
         }
         __syncwarp();
     } else if (tid >= 128 * NQ) {
