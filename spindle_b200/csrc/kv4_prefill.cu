@@ -168,9 +168,10 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *q_s = smem, *buf_s = smem + NQ * C::Q_BYTES;
     uint64_t *bars = reinterpret_cast<uint64_t *>(buf_s + 2 * C::BUF);
-    uint64_t *kv_full = bars, *kv_free = bars + 2, *s_full = bars + 4, *s_free = bars + 6, *p_full = bars + 8, *pv_done = bars + 10;
-    uint64_t *drain = bars + 12;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 13);
+    // operands made and free again, by buffer; scores there and taken, weights there and used, by tile of rows
+    uint64_t *k_full = bars, *k_free = bars + 2, *v_full = bars + 4, *v_free = bars + 6;
+    uint64_t *s_full = bars + 8, *s_free = bars + 10, *p_full = bars + 12, *pv_done = bars + 14, *drain = bars + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 17);
     volatile uint32_t *dead = tmem_slot + 1;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t req = blockIdx.z, head = blockIdx.y;
@@ -201,8 +202,10 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
 
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&kv_full[i], ND);
-            mbar_init(&kv_free[i], 1);
+            mbar_init(&k_full[i], ND);
+            mbar_init(&k_free[i], 1);
+            mbar_init(&v_full[i], ND);
+            mbar_init(&v_free[i], 1);
             mbar_init(&s_full[i], 1);
             mbar_init(&s_free[i], 128);
             mbar_init(&p_full[i], 128);
@@ -290,7 +293,7 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
         auto scores = [&](uint32_t i) {
             const uint32_t b = i & 1;
             const uint64_t off = b * (C::BUF >> 4);
-            wait(&kv_full[b], i >> 1 & 1);
+            wait(&k_full[b], i >> 1 & 1);
 #pragma unroll 1
             for (uint32_t h = 0; h < halves; h++) {
                 wait(&s_free[h], (i & 1) ^ 1);
@@ -306,6 +309,7 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
                     }
                     mma_ss(d, qd + D, m_desc + off, idesc(NK), true);
                     commit(&s_full[h]);
+                    if (h + 1 == halves) commit(&k_free[b]);
                 }
                 __syncwarp();
             }
@@ -316,6 +320,7 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
             if (i + 1 < n) scores(i + 1);
             const uint32_t b = i & 1;
             const uint64_t vd = v_desc + b * (C::BUF >> 4);
+            wait(&v_full[b], i >> 1 & 1);
 #pragma unroll 1
             for (uint32_t h = 0; h < halves; h++) {
                 wait(&p_full[h], i & 1);
@@ -326,7 +331,7 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
 #pragma unroll
                     for (uint32_t c = 0; c < NK / 16; c++) mma_ts(d, p + c * 8, vd + c * 16, idesc(D), c ? 1u : i);
                     commit(&pv_done[h]);
-                    if (h + 1 == halves) commit(&kv_free[b]);
+                    if (h + 1 == halves) commit(&v_free[b]);
                 }
                 __syncwarp();
             }
@@ -394,7 +399,7 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
         }
         for (uint32_t i = 0; i < n; i++) {
             const uint32_t b = i & 1;
-            wait(&kv_free[b], (i >> 1 & 1) ^ 1);
+            wait(&k_free[b], (i >> 1 & 1) ^ 1);
             uint8_t *k_hi = buf_s + b * C::BUF, *k_lo = k_hi + C::K_BYTES, *k_m = k_lo + C::K_BYTES, *v_t = k_m + C::M_BYTES;
             const int32_t t = (k0 + (int32_t)i) * NK;
 #pragma unroll
@@ -432,6 +437,9 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
                     }
                 }
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            arrive(&k_full[b]);
+            wait(&v_free[b], (i >> 1 & 1) ^ 1);
 #pragma unroll
             for (int g = 0; g < GV; g++) {
                 uint32_t val[4][4];
@@ -451,12 +459,12 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
                     *reinterpret_cast<uint4 *>(v_t + (d >> 3) * C::SBO_V + tb * 128 + (d & 7) * 16) = make_uint4(val[k][0], val[k][1], val[k][2], val[k][3]);
                 }
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            arrive(&v_full[b]);
             if (i + 1 < n) {
                 load(i + 1);
                 if (i + 2 < n) entries(i + 2);
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            arrive(&kv_full[b]);
         }
     } else if (tid < 128 * halves) {
         // ---- the weights: a thread per row ----
