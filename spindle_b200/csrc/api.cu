@@ -2440,7 +2440,8 @@ sg_status sg_kv4_plan(uint32_t page, uint32_t n_blocks, uint64_t n_req, const in
     DevInfo *di;
     if (sg_status st = dev_info(&di)) return st;
     const Kv4PlanArgs a = {d_ctx, d_new, d_tables, ld_tables, d_ring, d_cursor, d_cu, d_seq, d_pos, d_slots, d_info,
-                           (uint32_t)n_req, (uint32_t)max_tokens, (uint32_t)width, log2_of(page), n_blocks};
+                           (uint32_t)n_req, (uint32_t)max_tokens, (uint32_t)width, log2_of(page), n_blocks,
+                           aligned(d_pos, 16) && aligned(d_slots, 16)};
     const uint64_t want = (max_tokens + KV4_PLAN_THREADS - 1) / KV4_PLAN_THREADS;
     const uint32_t grid = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(want, di->sms));
     kv4_plan_kernel<<<grid, KV4_PLAN_THREADS, 0, (cudaStream_t)stream>>>(a);
@@ -2461,12 +2462,16 @@ sg_status sg_kv4_append(const sg_kv4 *c, int32_t type, const void *d_k, uint64_t
     if (sg_status st = dev_info(&di)) return st;
     const uint64_t m = 16 / es - 1;
     const bool vec = aligned(d_k, 16) && aligned(d_v, 16) && !((k_tok | k_head | v_tok | v_head) & m);
-    const Kv4RowArgs a = {kv4_of(c), d_k, d_v, k_tok, k_head, v_tok, v_head, nullptr, nullptr, d_slots, d_nonfinite,
-                          (uint32_t)n_tok};
-    const uint64_t lanes = n_tok * c->n_kv_heads * (c->head_dim / 32) * 8;
-    const uint32_t grid = (uint32_t)std::min<uint64_t>((lanes + KV4_ROW_THREADS - 1) / KV4_ROW_THREADS, (uint64_t)di->sms * 64);
-    kv4_append_kernel_for(type, c->head_dim, vec)<<<grid, KV4_ROW_THREADS, 0, (cudaStream_t)stream>>>(a);
-    CK(cudaGetLastError());
+    // a lane per sixteen values, fewer than 2^31 of them a launch
+    const uint64_t per_tok = (uint64_t)c->n_kv_heads * (c->head_dim / 8), step = std::max<uint64_t>(1, (1ull << 30) / per_tok);
+    for (uint64_t t = 0; t < n_tok; t += step) {
+        const uint64_t n = std::min(step, n_tok - t);
+        const Kv4RowArgs a = {kv4_of(c), (const uint8_t *)d_k + t * k_tok * es, (const uint8_t *)d_v + t * v_tok * es, k_tok, k_head,
+                              v_tok, v_head, nullptr, nullptr, d_slots + t, d_nonfinite, (uint32_t)(n * per_tok)};
+        const uint32_t grid = (uint32_t)std::min<uint64_t>((a.lanes + KV4_ROW_THREADS - 1) / KV4_ROW_THREADS, (uint64_t)di->sms * 64);
+        kv4_append_kernel_for(type, c->head_dim, vec)<<<grid, KV4_ROW_THREADS, 0, (cudaStream_t)stream>>>(a);
+        CK(cudaGetLastError());
+    }
     return SG_OK;
 }
 
@@ -2479,11 +2484,16 @@ sg_status sg_kv4_read(const sg_kv4 *c, int32_t type, const int32_t *d_slots, uin
     if (!aligned(d_k, 16) || !aligned(d_v, 16)) return SG_ERR_ALIGN;
     DevInfo *di;
     if (sg_status st = dev_info(&di)) return st;
-    const Kv4RowArgs a = {kv4_of(c), nullptr, nullptr, 0, 0, 0, 0, d_k, d_v, d_slots, nullptr, (uint32_t)n_tok};
-    const uint64_t lanes = n_tok * c->n_kv_heads * (c->head_dim / 32) * 8;
-    const uint32_t grid = (uint32_t)std::min<uint64_t>((lanes + KV4_ROW_THREADS - 1) / KV4_ROW_THREADS, (uint64_t)di->sms * 64);
-    kv4_read_kernel_for(type, c->head_dim)<<<grid, KV4_ROW_THREADS, 0, (cudaStream_t)stream>>>(a);
-    CK(cudaGetLastError());
+    const uint64_t es = act_bytes(type), row = (uint64_t)c->n_kv_heads * c->head_dim;
+    const uint64_t per_tok = (uint64_t)c->n_kv_heads * (c->head_dim / 8), step = std::max<uint64_t>(1, (1ull << 30) / per_tok);
+    for (uint64_t t = 0; t < n_tok; t += step) {
+        const uint64_t n = std::min(step, n_tok - t);
+        const Kv4RowArgs a = {kv4_of(c), nullptr, nullptr, 0, 0, 0, 0, (uint8_t *)d_k + t * row * es, (uint8_t *)d_v + t * row * es,
+                              d_slots + t, nullptr, (uint32_t)(n * per_tok)};
+        const uint32_t grid = (uint32_t)std::min<uint64_t>((a.lanes + KV4_ROW_THREADS - 1) / KV4_ROW_THREADS, (uint64_t)di->sms * 64);
+        kv4_read_kernel_for(type, c->head_dim)<<<grid, KV4_ROW_THREADS, 0, (cudaStream_t)stream>>>(a);
+        CK(cudaGetLastError());
+    }
     return SG_OK;
 }
 

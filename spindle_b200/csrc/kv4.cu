@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(KV4_PLAN_THREADS) kv4_plan_kernel(const __grid
     const uint32_t tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const uint32_t page = 1u << a.page_shift;
     const uint32_t head = (uint32_t)a.cursor[0], tail = (uint32_t)a.cursor[1], free_blocks = tail - head;
-    const uint32_t per = (a.max_tok + gridDim.x - 1) / gridDim.x;
+    const uint32_t per = ((a.max_tok + gridDim.x - 1) / gridDim.x + 3) & ~3u;
     const uint32_t t0 = min(a.max_tok, blockIdx.x * per), t1 = min(a.max_tok, t0 + per);
     uint32_t base_come = 0, base_want = 0, base_back = 0;
 
@@ -115,29 +115,44 @@ __global__ void __launch_bounds__(KV4_PLAN_THREADS) kv4_plan_kernel(const __grid
                 at += __popc(is);
             }
         }
-        // this CTA's new positions among these requests
+        // this CTA's new positions among these requests, four neighbours a thread: one search, and a table entry
+        // looked up again where the request or the page changes
         const uint32_t lo = max(t0, base_come), hi = min(t1, base_come + total_s[0]);
-        for (uint32_t t = lo + tid; t < hi; t += KV4_PLAN_THREADS) {
-            uint32_t x = 0, y = n;  // the last request with cu <= t
+        for (uint32_t q = (lo & ~3u) + tid * 4; q < hi; q += KV4_PLAN_THREADS * 4) {
+            uint32_t x = 0, y = n;  // the last request with cu <= the first position
+            const uint32_t first = max(q, lo), last = min(q + 4, hi);
             while (y - x > 1) {
                 const uint32_t m = (x + y) >> 1;
-                if (cu_s[m] <= t) x = m;
+                if (cu_s[m] <= first) x = m;
                 else y = m;
             }
-            const uint32_t c = (uint32_t)ctx_s[x], pos = c + (t - cu_s[x]);
-            const uint32_t have = min((c + page - 1) >> a.page_shift, a.width), j = pos >> a.page_shift;
-            int32_t *row = a.tables + (uint64_t)(r0 + x) * a.ld_tables;
-            int32_t block = -1;
-            if (j >= a.width) {
-            } else if (j < have) {
-                block = row[j];
-            } else {
-                const uint32_t k = want_s[x] + j - have;
-                if (k < free_blocks) block = a.ring[(head + k) % a.n_blocks];
-                if ((pos & (page - 1)) == 0) row[j] = block;
+            int32_t block = -1, pos4[4], slot4[4];
+            uint32_t known = ~0u;  // the page that block is of
+            for (uint32_t t = first; t < last; t++) {
+                while (x + 1 < n && cu_s[x + 1] <= t) x++, known = ~0u;
+                const uint32_t c = (uint32_t)ctx_s[x], pos = c + (t - cu_s[x]), j = pos >> a.page_shift;
+                if (j != known) {
+                    const uint32_t have = min((c + page - 1) >> a.page_shift, a.width);
+                    int32_t *row = a.tables + (uint64_t)(r0 + x) * a.ld_tables;
+                    block = -1;
+                    if (j < have) {
+                        block = row[j];
+                    } else if (j < a.width) {
+                        const uint32_t k = want_s[x] + j - have;
+                        if (k < free_blocks) block = a.ring[(head + k) % a.n_blocks];
+                        if ((pos & (page - 1)) == 0) row[j] = block;
+                    }
+                    known = j;
+                }
+                pos4[t & 3] = (int32_t)pos;
+                slot4[t & 3] = (uint32_t)block < a.n_blocks ? block * (int32_t)page + (int32_t)(pos & (page - 1)) : -1;
             }
-            a.pos[t] = (int32_t)pos;
-            a.slots[t] = (uint32_t)block < a.n_blocks ? block * (int32_t)page + (int32_t)(pos & (page - 1)) : -1;
+            if (a.vec && last - first == 4) {
+                *reinterpret_cast<int4 *>(a.pos + q) = make_int4(pos4[0], pos4[1], pos4[2], pos4[3]);
+                *reinterpret_cast<int4 *>(a.slots + q) = make_int4(slot4[0], slot4[1], slot4[2], slot4[3]);
+            } else {
+                for (uint32_t t = first; t < last; t++) a.pos[t] = pos4[t & 3], a.slots[t] = slot4[t & 3];
+            }
         }
         base_come += total_s[0];
         base_want += total_s[1];
@@ -158,90 +173,110 @@ __global__ void __launch_bounds__(KV4_PLAN_THREADS) kv4_plan_kernel(const __grid
 
 // ---- append -------------------------------------------------------------------
 //
-// Four lanes per group of 32 values, eight values each: lane j's eight are the
-// K word (j, g), and the two V half words (2j, g) and (2j + 1, g).
+// Two lanes per group of 32 values, sixteen values each: lane i's are the K words
+// j = 2 i and 2 i + 1 of the group, and its V half words 4 i .. 4 i + 3.
 //   m = f16(min), s = f16((max - m) * f32(1/15)), c = rint(clamp((x - m) * (1 / s), 0, 15))
 // with x clamped to f16's finite range and NaN counted as 0, so that the cache
 // holds finite numbers only; groups that had such a value are counted.  Every
 // step is one rounded f32 operation, so the codes can be reproduced bit for bit.
+// What bounds it is the arithmetic (about 8 instructions a value), hence sixteen
+// values a lane: the place of a row in the cache is worked out half as often.
+
+// The larger and the smaller one, NaN if either is.
+__device__ __forceinline__ float max_nan(float x, float y) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(x), "f"(y));
+    return d;
+}
+__device__ __forceinline__ float min_nan(float x, float y) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(x), "f"(y));
+    return d;
+}
+
+// Which sixteen values a lane has: token t, head h, K or V, group g, half i of it.
+struct Place {
+    uint32_t t, h, g, i;
+    bool is_v;
+};
+template <int D>
+__device__ __forceinline__ Place place_of(uint32_t f, uint32_t heads) {
+    constexpr uint32_t G = D / 32;
+    const uint32_t per_tok = heads * G * 4;  // lanes of a token: K's, then V's, head by head, two a group
+    const uint32_t t = f / per_tok, u = f - t * per_tok, hv = u / (2 * G);
+    return {t, hv >= heads ? hv - heads : hv, u / 2 % G, u % 2, hv >= heads};
+}
+// The tile of a slot, and the position inside it.
+template <int D>
+__device__ __forceinline__ uint8_t *tile_of(const Kv4Cache &c, int32_t slot, uint32_t h, uint32_t &p) {
+    const uint32_t at = (uint32_t)slot & ((1u << c.page_shift) - 1);
+    p = at & 15;
+    return c.data + ((((uint64_t)((uint32_t)slot >> c.page_shift) * c.heads + h) << (c.page_shift - 4)) + (at >> 4)) * (uint64_t)Kv4Tile<D>::BYTES;
+}
+
 template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(KV4_ROW_THREADS) kv4_append_kernel(const __grid_constant__ Kv4RowArgs a) {
     using L = Kv4Tile<D>;
     constexpr uint32_t G = L::G;
-    const uint64_t n = (uint64_t)a.n_tok * a.c.heads * G * 2;  // groups: K's and V's of a row side by side
-    for (uint64_t i0 = ((uint64_t)blockIdx.x * KV4_ROW_THREADS + threadIdx.x) >> 2; i0 < ((n + 7) & ~7ull);
-         i0 += (uint64_t)gridDim.x * KV4_ROW_THREADS >> 2) {
-        const bool live = i0 < n;
-        const uint64_t i = live ? i0 : n - 1;
-        const uint32_t j = threadIdx.x & 3, g = (uint32_t)(i % G), is_v = (uint32_t)(i / G) & 1;
-        const uint64_t row = i / (2 * G);
-        const uint32_t h = (uint32_t)(row % a.c.heads);
-        const uint64_t t = row / a.c.heads;
-        const int32_t slot = a.slots[t];
-        const T *src = (const T *)(is_v ? a.v : a.k) + t * (is_v ? a.v_tok : a.k_tok) + h * (is_v ? a.v_head : a.k_head) +
-                       g * 32 + j * 8;
-        float x[8];
+    for (uint32_t f = blockIdx.x * KV4_ROW_THREADS + threadIdx.x; f - threadIdx.x % 32 < a.lanes; f += gridDim.x * KV4_ROW_THREADS) {
+        const bool live = f < a.lanes;
+        const Place q = place_of<D>(live ? f : a.lanes - 1, a.c.heads);
+        const int32_t slot = a.slots[q.t];
+        const T *src = (const T *)(q.is_v ? a.v : a.k) + q.t * (q.is_v ? a.v_tok : a.k_tok) + q.h * (q.is_v ? a.v_head : a.k_head) +
+                       q.g * 32 + q.i * 16;
+        alignas(16) T raw[16];
         if (VEC) {
-            alignas(16) T raw[8];
-            constexpr int W = sizeof(T) * 8 / 16;
 #pragma unroll
-            for (int w = 0; w < W; w++) reinterpret_cast<uint4 *>(raw)[w] = __ldg(reinterpret_cast<const uint4 *>(src) + w);
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = Conv<T>::get(raw[e]);
+            for (int w = 0; w < (int)sizeof(T); w++) reinterpret_cast<uint4 *>(raw)[w] = __ldg(reinterpret_cast<const uint4 *>(src) + w);
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = Conv<T>::get(src[e]);
+            for (int e = 0; e < 16; e++) raw[e] = src[e];
         }
-        float lo = x[0], hi = x[0], odd = 0.0f;
+        float x[16];
 #pragma unroll
-        for (int e = 0; e < 8; e++) odd = fmaf(x[e], 0.0f, odd);  // NaN when a value is not finite
-        bool bad = !(odd == 0.0f);
+        for (int e = 0; e < 16; e++) x[e] = Conv<T>::get(raw[e]);
+        float lo = x[0], hi = x[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) lo = min_nan(lo, x[e]), hi = max_nan(hi, x[e]);
+        const bool bad = !(lo >= -3.4028235e38f && hi <= 3.4028235e38f);  // a NaN or an infinity
         if (bad) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = x[e] == x[e] ? x[e] : 0.0f;
+            for (int e = 0; e < 16; e++) x[e] = x[e] == x[e] ? x[e] : 0.0f;
             lo = hi = x[0];
-        }
 #pragma unroll
-        for (int e = 1; e < 8; e++) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]);
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            for (int e = 1; e < 16; e++) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]);
         }
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 1));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
         lo = fminf(fmaxf(lo, -65504.0f), 65504.0f);
         hi = fminf(fmaxf(hi, -65504.0f), 65504.0f);
         const __half mh = __float2half_rn(lo + 0.0f);  // + 0: no negative zero
         const float m = __half2float(mh);
         const __half sh = __float2half_rn(__fmul_rn(fmaxf(hi - m, 0.0f), 1.0f / 15.0f));
         const float s = __half2float(sh), r = s > 0.0f ? __frcp_rn(s) : 0.0f;
-        uint32_t word = 0;
+        uint32_t word[2] = {0, 0};
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float y = fminf(fmaxf(x[e], -65504.0f), 65504.0f);
-            const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(y, m), r), 0.0f), 15.0f);
-            word |= (uint32_t)__float2int_rn(c) << (4 * e);
+        for (int e = 0; e < 16; e++) {
+            // to an unsigned number, below 0 and NaN to 0; a value beyond the clamped ends falls on their codes
+            const uint32_t c = min(__float2uint_rn(__fmul_rn(__fsub_rn(x[e], m), r)), 15u);
+            word[e / 8] += c << (4 * (e % 8));
         }
-        const unsigned any = __ballot_sync(0xffffffffu, bad && live) >> (threadIdx.x & 28) & 0xf;
+        const unsigned any = __ballot_sync(0xffffffffu, bad && live) >> (threadIdx.x & 30) & 3;
         if (!live || slot < 0 || (uint32_t)(slot >> a.c.page_shift) >= a.c.n_blocks) continue;
-        if (any && j == 0 && a.nonfinite) atomicAdd(a.nonfinite, 1);
-        const uint32_t at = (uint32_t)slot & ((1u << a.c.page_shift) - 1), p = at & 15;
-        uint8_t *tile = a.c.data + ((((uint64_t)(slot >> a.c.page_shift) * a.c.heads + h) << (a.c.page_shift - 4)) + (at >> 4)) *
-                                       (uint64_t)L::BYTES;
-        const uint32_t pair = ((p >> 1) * G + g) * 2 + (p & 1);
-        if (is_v) {
+        if (any && q.i == 0 && a.nonfinite) atomicAdd(a.nonfinite, 1);
+        uint32_t p;
+        uint8_t *tile = tile_of<D>(a.c, slot, q.h, p);
+        const uint32_t pair = ((p >> 1) * G + q.g) * 2 + (p & 1);
+        if (q.is_v) {
             uint8_t *v = tile + L::VC + (p >> 1) * L::VROW + (p & 1) * 2;
-            *reinterpret_cast<uint16_t *>(v + kv4_word(2 * j, g, 8, G) * 4) = (uint16_t)word;
-            *reinterpret_cast<uint16_t *>(v + kv4_word(2 * j + 1, g, 8, G) * 4) = (uint16_t)(word >> 16);
-            if (j == 0) {
-                reinterpret_cast<__half *>(tile + L::VS)[pair] = sh;
-                reinterpret_cast<__half *>(tile + L::VM)[pair] = mh;
-            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) *reinterpret_cast<uint16_t *>(v + kv4_word(4 * q.i + k, q.g, 8, G) * 4) = (uint16_t)(word[k / 2] >> (k % 2 * 16));
+            reinterpret_cast<__half *>(tile + (q.i ? L::VM : L::VS))[pair] = q.i ? mh : sh;
         } else {
-            *reinterpret_cast<uint32_t *>(tile + p * L::KROW + kv4_word(j, g, 4, G) * 4) = word;
-            if (j == 0) {
-                reinterpret_cast<__half *>(tile + L::KS)[pair] = sh;
-                reinterpret_cast<__half *>(tile + L::KM)[p * G + g] = mh;
-            }
+#pragma unroll
+            for (int k = 0; k < 2; k++) *reinterpret_cast<uint32_t *>(tile + p * L::KROW + kv4_word(2 * q.i + k, q.g, 4, G) * 4) = word[k];
+            if (q.i) reinterpret_cast<__half *>(tile + L::KM)[p * G + q.g] = mh;
+            else reinterpret_cast<__half *>(tile + L::KS)[pair] = sh;
         }
     }
 }
@@ -252,41 +287,38 @@ template <typename T, int D>
 __global__ void __launch_bounds__(KV4_ROW_THREADS) kv4_read_kernel(const __grid_constant__ Kv4RowArgs a) {
     using L = Kv4Tile<D>;
     constexpr uint32_t G = L::G;
-    const uint64_t n = (uint64_t)a.n_tok * a.c.heads * G * 8;  // 8 values each: 4 lanes of K, 4 of V per group
-    for (uint64_t i = (uint64_t)blockIdx.x * KV4_ROW_THREADS + threadIdx.x; i < n; i += (uint64_t)gridDim.x * KV4_ROW_THREADS) {
-        const uint32_t j = (uint32_t)i & 3, g = (uint32_t)(i / 4 % G), is_v = (uint32_t)(i / (4 * G)) & 1;
-        const uint64_t row = i / (8 * G), t = row / a.c.heads;
-        const uint32_t h = (uint32_t)(row % a.c.heads);
-        const int32_t slot = a.slots[t];
-        alignas(16) T y[8];
-        if (slot < 0 || (uint32_t)(slot >> a.c.page_shift) >= a.c.n_blocks) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) y[e] = Conv<T>::put(0.0f);
-        } else {
-            const uint32_t at = (uint32_t)slot & ((1u << a.c.page_shift) - 1), p = at & 15;
-            const uint8_t *tile = a.c.data + ((((uint64_t)(slot >> a.c.page_shift) * a.c.heads + h) << (a.c.page_shift - 4)) + (at >> 4)) *
-                                                 (uint64_t)L::BYTES;
-            const uint32_t pair = ((p >> 1) * G + g) * 2 + (p & 1);
-            uint32_t word;
-            float s, m;
-            if (is_v) {
+    for (uint32_t f = blockIdx.x * KV4_ROW_THREADS + threadIdx.x; f < a.lanes; f += gridDim.x * KV4_ROW_THREADS) {
+        const Place q = place_of<D>(f, a.c.heads);
+        const int32_t slot = a.slots[q.t];
+        uint32_t word[2] = {0, 0};
+        float s = 0.0f, m = 0.0f;
+        if (slot >= 0 && (uint32_t)(slot >> a.c.page_shift) < a.c.n_blocks) {
+            uint32_t p;
+            const uint8_t *tile = tile_of<D>(a.c, slot, q.h, p);
+            const uint32_t pair = ((p >> 1) * G + q.g) * 2 + (p & 1);
+            if (q.is_v) {
                 const uint8_t *v = tile + L::VC + (p >> 1) * L::VROW + (p & 1) * 2;
-                word = *reinterpret_cast<const uint16_t *>(v + kv4_word(2 * j, g, 8, G) * 4) |
-                       (uint32_t) * reinterpret_cast<const uint16_t *>(v + kv4_word(2 * j + 1, g, 8, G) * 4) << 16;
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    word[k / 2] |= (uint32_t) * reinterpret_cast<const uint16_t *>(v + kv4_word(4 * q.i + k, q.g, 8, G) * 4) << (k % 2 * 16);
                 s = __half2float(reinterpret_cast<const __half *>(tile + L::VS)[pair]);
                 m = __half2float(reinterpret_cast<const __half *>(tile + L::VM)[pair]);
             } else {
-                word = *reinterpret_cast<const uint32_t *>(tile + p * L::KROW + kv4_word(j, g, 4, G) * 4);
+#pragma unroll
+                for (int k = 0; k < 2; k++) word[k] = *reinterpret_cast<const uint32_t *>(tile + p * L::KROW + kv4_word(2 * q.i + k, q.g, 4, G) * 4);
                 s = __half2float(reinterpret_cast<const __half *>(tile + L::KS)[pair]);
-                m = __half2float(reinterpret_cast<const __half *>(tile + L::KM)[p * G + g]);
+                m = __half2float(reinterpret_cast<const __half *>(tile + L::KM)[p * G + q.g]);
             }
-#pragma unroll
-            for (int e = 0; e < 8; e++) y[e] = Conv<T>::put(fmaf(s, (float)(word >> (4 * e) & 15u), m));
         }
-        uint4 *dst = reinterpret_cast<uint4 *>((T *)(is_v ? a.v_out : a.k_out) + row * D + g * 32 + j * 8);
-        constexpr int W = sizeof(T) * 8 / 16;
+        alignas(16) T y[16];
 #pragma unroll
-        for (int w = 0; w < W; w++) dst[w] = reinterpret_cast<const uint4 *>(y)[w];
+        for (int e = 0; e < 16; e++) {
+            const float c = __uint_as_float((word[e / 8] >> (4 * (e % 8)) & 15u) | 0x4B000000u) - 8388608.0f;  // 2^23 + c
+            y[e] = Conv<T>::put(fmaf(s, c, m));
+        }
+        uint4 *dst = reinterpret_cast<uint4 *>((T *)(q.is_v ? a.v_out : a.k_out) + ((uint64_t)q.t * a.c.heads + q.h) * D + q.g * 32 + q.i * 16);
+#pragma unroll
+        for (int w = 0; w < (int)sizeof(T); w++) dst[w] = reinterpret_cast<const uint4 *>(y)[w];
     }
 }
 

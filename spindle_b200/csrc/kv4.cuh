@@ -50,6 +50,7 @@ struct Kv4PlanArgs {
     const int32_t *cursor;
     int32_t *cu, *seq, *pos, *slots, *info;
     uint32_t n_req, max_tok, width, page_shift, n_blocks;
+    bool vec;  // pos and slots allow 16-byte stores
 };
 
 struct Kv4RowArgs {
@@ -59,7 +60,7 @@ struct Kv4RowArgs {
     void *k_out, *v_out;               // read: [n_tok][heads][D]
     const int32_t *slots;
     int32_t *nonfinite;
-    uint32_t n_tok;
+    uint32_t lanes;  // tokens * heads * D / 8: a lane per sixteen values of K or V
 };
 
 struct Kv4AttnArgs {

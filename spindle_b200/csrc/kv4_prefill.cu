@@ -39,7 +39,7 @@ struct Pre {
     static constexpr uint32_t Q_BYTES = 16 * SBO_Q;                 // 128 rows
     static constexpr uint32_t K_BYTES = NK / 8 * SBO_K, M_BYTES = NK / 8 * SBO_M, V_BYTES = D / 8 * SBO_V;
     static constexpr uint32_t BUF = 2 * K_BYTES + M_BYTES + V_BYTES;
-    static constexpr uint32_t SMEM = NQ * Q_BYTES + 2 * BUF + 256;
+    static constexpr uint32_t SMEM = NQ * Q_BYTES + 2 * BUF + 256;  // and the barriers
     // TMEM columns: scores, weights (two f16 a column), sums
     static constexpr uint32_t S_COL = 0, P_COL = 128, O_COL = 256;
     static_assert(GV >= 1 && KI >= 1 && SMEM <= 227 * 1024, "shapes");
@@ -173,6 +173,7 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
     uint64_t *s_full = bars + 8, *s_free = bars + 10, *p_full = bars + 12, *pv_done = bars + 14, *drain = bars + 16;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 17);
     volatile uint32_t *dead = tmem_slot + 1;
+    uint32_t *there_s = tmem_slot + 2;  // [4] of steps: a byte per 16 positions, 1 where they are there
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t req = blockIdx.z, head = blockIdx.y;
 
@@ -206,7 +207,7 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
             mbar_init(&k_free[i], 1);
             mbar_init(&v_full[i], ND);
             mbar_init(&v_free[i], 1);
-            mbar_init(&s_full[i], 1);
+            mbar_init(&s_full[i], 2);  // the products' end, and the issuing lane's own word on what it saw
             mbar_init(&s_free[i], 128);
             mbar_init(&p_full[i], 128);
             mbar_init(&pv_done[i], 1);
@@ -309,6 +310,7 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
                     }
                     mma_ss(d, qd + D, m_desc + off, idesc(NK), true);
                     commit(&s_full[h]);
+                    arrive(&s_full[h]);
                     if (h + 1 == halves) commit(&k_free[b]);
                 }
                 __syncwarp();
@@ -359,13 +361,12 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
         int32_t kb[KI], vb;
         uint32_t kr[KI][KG], ks[KI][KG], km[KI][KG / 2], vr[4][GV], vs[4][GV], vm[4][GV];
         bool k_ok[KI], v_ok;
-        auto entries = [&](uint32_t i) {
-            const int32_t t = (k0 + (int32_t)i) * NK;
+        auto entries_k = [&](uint32_t i) {
 #pragma unroll
-            for (int j = 0; j < KI; j++) kb[j] = entry(t + kpos(j));
-            vb = entry(t + tb * 8);
+            for (int j = 0; j < KI; j++) kb[j] = entry((k0 + (int32_t)i) * NK + kpos(j));
         };
-        auto load = [&](uint32_t i) {
+        auto entries_v = [&](uint32_t i) { vb = entry((k0 + (int32_t)i) * NK + tb * 8); };
+        auto load_k = [&](uint32_t i) {
             const int32_t t = (k0 + (int32_t)i) * NK;
 #pragma unroll
             for (int j = 0; j < KI; j++) {
@@ -379,7 +380,9 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
                     ldg_words<KG / 2>(km[j], tl + L::KM + p * (G * 2) + ka * 8);
                 }
             }
-            const int32_t pos = t + tb * 8;
+        };
+        auto load_v = [&](uint32_t i) {
+            const int32_t pos = (k0 + (int32_t)i) * NK + tb * 8;
             v_ok = pos < end && (uint32_t)vb < a.c.n_blocks;
             if (v_ok) {
                 const uint8_t *tl = tile_of(vb, pos);
@@ -393,9 +396,9 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
             }
         };
         if (n) {
-            entries(0);
-            load(0);
-            if (n > 1) entries(1);
+            entries_k(0), entries_v(0);
+            load_k(0), load_v(0);
+            if (n > 1) entries_k(1), entries_v(1);
         }
         for (uint32_t i = 0; i < n; i++) {
             const uint32_t b = i & 1;
@@ -438,7 +441,16 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            if (y4 == 0 && ka == 0) {
+#pragma unroll
+                for (int j = 0; j < KI; j++)
+                    if ((kpos(j) & 15) == 0) reinterpret_cast<uint8_t *>(there_s + (i & 3))[kpos(j) / 16] = k_ok[j];
+            }
             arrive(&k_full[b]);
+            if (i + 1 < n) {
+                load_k(i + 1);
+                if (i + 2 < n) entries_k(i + 2);
+            }
             wait(&v_free[b], (i >> 1 & 1) ^ 1);
 #pragma unroll
             for (int g = 0; g < GV; g++) {
@@ -462,8 +474,8 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             arrive(&v_full[b]);
             if (i + 1 < n) {
-                load(i + 1);
-                if (i + 2 < n) entries(i + 2);
+                load_v(i + 1);
+                if (i + 2 < n) entries_v(i + 2);
             }
         }
     } else if (tid < 128 * halves) {
@@ -474,7 +486,7 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
         const int64_t place = (int64_t)seq - nq + rr / a.group;
         const int32_t hi_t = live ? (int32_t)max((int64_t)0, min(place + 1, (int64_t)end)) : 0;
         const int32_t lo_t = a.window && place + 1 > (int64_t)a.window ? (int32_t)(place + 1 - a.window) : 0;
-        const int32_t *table = a.tables + (uint64_t)req * a.ld_tables;
+        constexpr uint32_t ALL = NK == 64 ? 0x01010101u : 0x0101u;
         float m = -INFINITY, l = 0.0f;
         for (uint32_t i = 0; i < n; i++) {
             const int32_t t0 = (k0 + (int32_t)i) * NK;
@@ -484,18 +496,14 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
             uint32_t s[NK / 32][32];
 #pragma unroll
             for (int c = 0; c < NK / 32; c++) tmem_ld32(mine + C::S_COL + h * NK + c * 32, s[c]);
+            const uint32_t there = there_s[i & 3];
             fence_before();
             arrive(&s_free[h]);
-            // the pages of this step that are there, a bit per 16 positions
-            uint32_t there = 0;
-            if (t0 < end) {
-                for (int c = 0; c < NK / 16; c++) there |= (uint32_t)(t0 + 16 * c < end && (uint32_t)__ldg(table + ((t0 + 16 * c) >> a.c.page_shift)) < a.c.n_blocks) << c;
-            }
             float top = -INFINITY;
-            if (t0 < lo_t || t0 + NK > hi_t || there != (1u << (NK / 16)) - 1) {
+            if (t0 < lo_t || t0 + NK > hi_t || (there & ALL) != ALL) {
 #pragma unroll
                 for (int c = 0; c < NK; c++)
-                    if (t0 + c < lo_t || t0 + c >= hi_t || !(there >> (c / 16) & 1)) s[c / 32][c % 32] = 0xFF800000u;
+                    if (t0 + c < lo_t || t0 + c >= hi_t || !(there >> (c / 16 * 8) & 1)) s[c / 32][c % 32] = 0xFF800000u;
             }
 #pragma unroll
             for (int c = 0; c < NK; c++) top = fmaxf(top, __uint_as_float(s[c / 32][c % 32]));
