@@ -449,3 +449,75 @@ def test_refusals(dev):
         sg.kv4_plan(p, z, z, torch.zeros(2, 2, device=dev))
     with pytest.raises(ValueError):
         sg.kv4_plan(p, z, z, torch.zeros(2, 2, dtype=torch.int32, device=dev), ring=p.ring)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,group,d,page", [(4, 8, 64, 16), (4, 8, 128, 64), (4, 8, 256, 16), (2, 7, 128, 32), (1, 16, 64, 128)])
+@pytest.mark.parametrize("window", [0, 1, 50, 300])
+def test_attention_many_rows(dev, dtype, heads, group, d, page, window):
+    # enough rows for the tensor-core kernel: chunks against a context and without one, a request without new
+    # tokens, rows that see nothing (no positions held, more new tokens than positions), blocks that are missing
+    lens, news = [700, 300, 0, 40, 129, 65], [260, 300, 5, 60, 0, 1]
+    assert sum(news) * heads * group * 7 > 26000
+    missing = [(0, 0), (0, 2)] if page < 128 else [(0, 1)]
+    cache, tables, full, cu, seq, g = case(dev, lens, news, heads, d, page, window + d, extra_width=1, missing=missing)
+    n = sum(news) + 2                                                   # two tokens of no request
+    q = torch.randn(n, heads * group, d, device=dev, generator=g).to(dtype)
+    lse = torch.empty(n, heads * group, device=dev)
+    out = sg.kv4_attention(cache, q, cu, seq, tables, window=window, lse=lse, max_new=300)
+    check(dev, cache, tables, full, cu, seq, q, d ** -0.5, window, out, lse)
+    assert (out[sum(news):] == 0).all() and torch.isneginf(lse[sum(news):]).all()
+    assert torch.equal(sg.kv4_attention(cache, q, cu, seq, tables, window=window), out)
+    sg.device_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attention_many_rows_strides_and_scales(dev, dtype):
+    heads, group, d, page = 2, 4, 128, 16
+    lens, news = [600, 513], [500, 513]
+    cache, tables, full, cu, seq, g = case(dev, lens, news, heads, d, page, 77)
+    n, hq = sum(news), heads * group
+    qkv = torch.randn(n, hq + 2 * heads, d, device=dev, generator=g)
+    qkv[3, 1] *= 1e-4
+    qkv[4, 2] = 0
+    qkv[5, 3] *= 100.0
+    qkv = qkv.to(dtype)
+    for scale in (d ** -0.5, -0.03):
+        o = torch.full((hq, n, d + 1), 7.0, dtype=dtype, device=dev)    # heads first, odd rows
+        lse = torch.empty(n, hq, device=dev)
+        got = sg.kv4_attention(cache, qkv[:, :hq], cu, seq, tables, scale=scale, lse=lse, out=o.transpose(0, 1)[..., :d])
+        check(dev, cache, tables, full, cu, seq, qkv[:, :hq], scale, 0, got, lse)
+        assert (o[..., d] == 7.0).all()
+        odd = torch.empty(n * hq * d + 1, dtype=dtype, device=dev)[1:].view(n, hq, d).copy_(qkv[:, :hq])
+        assert torch.equal(sg.kv4_attention(cache, odd, cu, seq, tables, scale=scale), got)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_many_requests(dev, dtype):
+    # more requests than one launch of the streaming kernel takes, of no and of a few tokens; and many short chunks
+    g = torch.Generator().manual_seed(1)
+    for n_req, most in [(2100, 1), (60, 24)]:
+        lens = torch.randint(0, 40, (n_req,), generator=g).tolist()
+        news = [min(x, int(torch.randint(0, most + 1, (1,), generator=g))) for x in lens]
+        heads, group, d, page = 1, 4, 64, 16
+        cache, tables, full, cu, seq, gg = case(dev, lens, news, heads, d, page, n_req)
+        q = torch.randn(sum(news), heads * group, d, device=dev, generator=gg).to(dtype)
+        lse = torch.empty(sum(news), heads * group, device=dev)
+        out = sg.kv4_attention(cache, q, cu, seq, tables, lse=lse, max_new=most)
+        for i in range(0, n_req, 97 if most == 1 else 7):               # some of them
+            a, b = cu[i].item(), cu[i + 1].item()
+            if a < b:
+                check(dev, cache, tables[i:i + 1], full[i:i + 1], ints([0, b - a], dev), seq[i:i + 1], q[a:b], d ** -0.5, 0, out[a:b], lse[a:b])
+
+
+def test_scratch_of_one_stream_serves_every_kernel(dev):
+    # calls of different shapes one after another on one scratch
+    scratch = sg.kv4_attention_scratch(dev)
+    for k in range(3):
+        for dtype, heads, group, d, lens, news in [(torch.float32, 2, 4, 128, [3000], [1]), (torch.float16, 1, 8, 256, [5000, 3], [2, 3]),
+                                                   (torch.bfloat16, 4, 8, 64, [400], [300])]:
+            cache, tables, full, cu, seq, g = case(dev, lens, news, heads, d, 32, k)
+            q = torch.randn(sum(news), heads * group, d, device=dev, generator=g).to(dtype)
+            lse = torch.empty(sum(news), heads * group, device=dev)
+            out = sg.kv4_attention(cache, q, cu, seq, tables, lse=lse, scratch=scratch)
+            check(dev, cache, tables, full, cu, seq, q, d ** -0.5, 0, out, lse)
