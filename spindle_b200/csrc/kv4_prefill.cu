@@ -4,11 +4,12 @@
 //
 // A CTA has NQ tiles of 128 query rows (a row is a (token, head of the group)
 // pair) of one request and KV head, and goes over the positions NK at a time:
-//   - warps of 128 threads per tile: a thread per row takes its scores from
-//     TMEM, keeps the running maximum and sum, and puts its weights back in f16;
-//   - ND threads turn the codes into f16 operands in shared memory, two buffers;
-//   - one thread issues the tensor products: the next scores before this step's
-//     sums, so that the tensor cores work while the weights are made.
+//   - 128 threads per tile: a thread per row takes its scores from TMEM, keeps the
+//     running maximum and sum, and puts its weights, in f16, where the scores were;
+//   - ND threads turn the codes into f16 operands in shared memory (K, and V twice);
+//   - one thread issues the tensor products, a tile's sums and its next scores when
+//     its weights are there: the tensor cores work for one tile while the weights
+//     of the other are made.
 // The scores are as good as f32: with K values m + s c (16-bit s and m, a code c)
 // s c goes in as its f16 rounding and the exact rest, and the minima as 16 more
 // columns against the sums of the query's groups (f16 rounding and rest).  V
@@ -30,18 +31,20 @@ constexpr float P_SHIFT = 6.0f, LAG = 8.0f;  // weights are held as 2^6 p, p bel
 template <int D>
 struct Pre {
     static constexpr int G = D / 32;
-    static constexpr int NQ = D == 256 ? 1 : 2, NK = D == 256 ? 32 : 64;
-    static constexpr int ND = D == 256 ? 256 : 128;                 // threads that make operands
+    // Products of 128 rows by 128 positions run at twice the rate of those by 64 (73 cycles against 59); what a head of
+    // 256 leaves of the shared memory and of TMEM is one tile of rows and 64 positions.
+    static constexpr int NQ = D == 256 ? 1 : 2, NK = D == 256 ? 64 : 128;
+    static constexpr int ND = 256;                                  // threads that make operands
     static constexpr int THREADS = 128 * NQ + ND + 32;
     static constexpr int GV = NK * G / ND;                          // groups of V that one of them makes
-    static constexpr int KI = NK * 4 * (G == 8 ? 2 : 1) / ND;       // positions of K
+    static constexpr int KI = NK * 4 * (G == 8 ? 2 : 1) / ND;       // items of K: a position's part of four groups (two)
     static constexpr uint32_t SBO_Q = (D / 8 + 2) * 128, SBO_K = D / 8 * 128, SBO_M = 256, SBO_V = NK * 16 + 16;
     static constexpr uint32_t Q_BYTES = 16 * SBO_Q;                 // 128 rows
     static constexpr uint32_t K_BYTES = NK / 8 * SBO_K, M_BYTES = NK / 8 * SBO_M, V_BYTES = D / 8 * SBO_V;
-    static constexpr uint32_t BUF = 2 * K_BYTES + M_BYTES + V_BYTES;
-    static constexpr uint32_t SMEM = NQ * Q_BYTES + 2 * BUF + 256;  // and the barriers
-    // TMEM columns: scores, weights (two f16 a column), sums
-    static constexpr uint32_t S_COL = 0, P_COL = 128, O_COL = 256;
+    static constexpr uint32_t K_AT = NQ * Q_BYTES, M_AT = K_AT + 2 * K_BYTES, V_AT = M_AT + M_BYTES, BAR_AT = V_AT + 2 * V_BYTES;
+    static constexpr uint32_t SMEM = BAR_AT + 256;
+    // TMEM columns: scores, whose place the weights take (two f16 a column), and sums
+    static constexpr uint32_t S_COL = 0, O_COL = 256;
     static_assert(GV >= 1 && KI >= 1 && SMEM <= 227 * 1024, "shapes");
 };
 
@@ -166,14 +169,14 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
     using C = Pre<D>;
     constexpr int G = C::G, NQ = C::NQ, NK = C::NK, ND = C::ND, GV = C::GV, KI = C::KI;
     extern __shared__ __align__(128) uint8_t smem[];
-    uint8_t *q_s = smem, *buf_s = smem + NQ * C::Q_BYTES;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(buf_s + 2 * C::BUF);
-    // operands made and free again, by buffer; scores there and taken, weights there and used, by tile of rows
-    uint64_t *k_full = bars, *k_free = bars + 2, *v_full = bars + 4, *v_free = bars + 6;
-    uint64_t *s_full = bars + 8, *s_free = bars + 10, *p_full = bars + 12, *pv_done = bars + 14, *drain = bars + 16;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 17);
+    uint8_t *q_s = smem;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::BAR_AT);
+    // operands made and free again (V by buffer); scores and weights there and sums done, by tile of rows
+    uint64_t *k_full = bars, *k_free = bars + 1, *v_full = bars + 2, *v_free = bars + 4;
+    uint64_t *s_full = bars + 6, *p_full = bars + 8, *pv_done = bars + 10, *drain = bars + 12;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 13);
     volatile uint32_t *dead = tmem_slot + 1;
-    uint32_t *there_s = tmem_slot + 2;  // [4] of steps: a byte per 16 positions, 1 where they are there
+    uint32_t *there_s = tmem_slot + 2;  // [4][2] of steps: a byte per 16 positions, 1 where they are there
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t req = blockIdx.z, head = blockIdx.y;
 
@@ -202,16 +205,16 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
     const uint32_t n = (uint32_t)max(k1 - k0, 0);  // steps
 
     if (tid == 0) {
+        mbar_init(k_full, ND);
+        mbar_init(k_free, 1);
         for (int i = 0; i < 2; i++) {
-            mbar_init(&k_full[i], ND);
-            mbar_init(&k_free[i], 1);
             mbar_init(&v_full[i], ND);
             mbar_init(&v_free[i], 1);
             mbar_init(&s_full[i], 2);  // the products' end, and the issuing lane's own word on what it saw
-            mbar_init(&s_free[i], 128);
             mbar_init(&p_full[i], 128);
             mbar_init(&pv_done[i], 1);
         }
+        for (int i = 0; i < 8; i++) there_s[i] = 0x01010101u;
         mbar_init(drain, 1);
         fence_mbar_init();
         *dead = 0;
@@ -288,54 +291,49 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
     if (warp == (128 * NQ + ND) / 32) {
         // ---- the tensor products: the warp goes together, one lane issues ----
         const uint32_t base = smem_u32(smem), tm = __shfl_sync(~0u, tmem, 0);
-        const uint64_t q_desc = smem_desc(base, C::SBO_Q), k_desc = smem_desc(base + NQ * C::Q_BYTES, C::SBO_K),
-                       m_desc = smem_desc(base + NQ * C::Q_BYTES + 2 * C::K_BYTES, C::SBO_M),
-                       v_desc = smem_desc(base + NQ * C::Q_BYTES + 2 * C::K_BYTES + C::M_BYTES, C::SBO_V);
-        auto scores = [&](uint32_t i) {
-            const uint32_t b = i & 1;
-            const uint64_t off = b * (C::BUF >> 4);
-            wait(&k_full[b], i >> 1 & 1);
+        const uint64_t q_desc = smem_desc(base, C::SBO_Q), k_desc = smem_desc(base + C::K_AT, C::SBO_K),
+                       m_desc = smem_desc(base + C::M_AT, C::SBO_M), v_desc = smem_desc(base + C::V_AT, C::SBO_V);
+        // step i: for each tile of rows the sums of step i - 1, then the scores of step i in the weights' place
+#pragma unroll 1
+        for (uint32_t i = 0; i <= n && n; i++) {
+            const uint32_t b = (i - 1) & 1;
+            if (i) wait(&v_full[b], (i - 1) >> 1 & 1);
 #pragma unroll 1
             for (uint32_t h = 0; h < halves; h++) {
-                wait(&s_free[h], (i & 1) ^ 1);
-                __syncwarp();
-                fence_after();
-                if (elect_one() && !*dead) {
-                    const uint32_t d = tm + C::S_COL + h * NK;
-                    const uint64_t qd = q_desc + h * (C::Q_BYTES >> 4), kd = k_desc + off;
+                if (i) {
+                    wait(&p_full[h], (i - 1) & 1);
+                    __syncwarp();
+                    fence_after();
+                    if (elect_one() && !*dead) {
+                        const uint32_t d = tm + C::O_COL + h * D, p = tm + C::S_COL + h * NK;
+                        const uint64_t vd = v_desc + b * (C::V_BYTES >> 4);
 #pragma unroll
-                    for (uint32_t c = 0; c < D / 8; c += 2) {
-                        mma_ss(d, qd + c * 8, kd + c * 8, idesc(NK), c != 0);
-                        mma_ss(d, qd + c * 8, kd + (C::K_BYTES >> 4) + c * 8, idesc(NK), true);
+                        for (uint32_t c = 0; c < NK / 16; c++) mma_ts(d, p + c * 8, vd + c * 16, idesc(D), c ? 1u : i - 1);
+                        if (h + 1 == halves) commit(&v_free[b]);
+                        commit(&pv_done[h]);
                     }
-                    mma_ss(d, qd + D, m_desc + off, idesc(NK), true);
-                    commit(&s_full[h]);
-                    arrive(&s_full[h]);
-                    if (h + 1 == halves) commit(&k_free[b]);
+                    __syncwarp();
                 }
-                __syncwarp();
-            }
-        };
-        if (n) scores(0);
-#pragma unroll 1
-        for (uint32_t i = 0; i < n; i++) {
-            if (i + 1 < n) scores(i + 1);
-            const uint32_t b = i & 1;
-            const uint64_t vd = v_desc + b * (C::BUF >> 4);
-            wait(&v_full[b], i >> 1 & 1);
-#pragma unroll 1
-            for (uint32_t h = 0; h < halves; h++) {
-                wait(&p_full[h], i & 1);
-                __syncwarp();
-                fence_after();
-                if (elect_one() && !*dead) {
-                    const uint32_t d = tm + C::O_COL + h * D, p = tm + C::P_COL + h * (NK / 2);
+                if (i < n) {
+                    if (i) wait(&pv_done[h], (i - 1) & 1);  // the weights are read
+                    if (h == 0) wait(k_full, i & 1);
+                    __syncwarp();
+                    fence_after();
+                    if (elect_one() && !*dead) {
+                        const uint32_t d = tm + C::S_COL + h * NK;
+                        const uint64_t qd = q_desc + h * (C::Q_BYTES >> 4);
 #pragma unroll
-                    for (uint32_t c = 0; c < NK / 16; c++) mma_ts(d, p + c * 8, vd + c * 16, idesc(D), c ? 1u : i);
-                    commit(&pv_done[h]);
-                    if (h + 1 == halves) commit(&v_free[b]);
+                        for (uint32_t c = 0; c < D / 8; c += 2) {
+                            mma_ss(d, qd + c * 8, k_desc + c * 8, idesc(NK), c != 0);
+                            mma_ss(d, qd + c * 8, k_desc + (C::K_BYTES >> 4) + c * 8, idesc(NK), true);
+                        }
+                        mma_ss(d, qd + D, m_desc, idesc(NK), true);
+                        commit(&s_full[h]);
+                        arrive(&s_full[h]);
+                        if (h + 1 == halves) commit(k_free);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
         }
         if (*dead && lane == 0) {  // what is still running must end before its memory goes
@@ -346,10 +344,10 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
     } else if (tid >= 128 * NQ) {
         // ---- the operands of a step from the cache: its codes are read a step ahead, its table entries two ----
         const uint32_t dt = tid - 128 * NQ, dw = dt >> 5, x8 = lane & 7, y4 = lane >> 3;
-        // K: positions of this thread (its word part j = y4); V: the 8 positions tb, word part x8, groups from gq * GV on
-        constexpr int HALF = G == 8 ? 2 : 1;
-        const uint32_t ka = HALF == 2 ? dw / (NK / 8) : 0;  // D = 256: which half of the groups
-        auto kpos = [&](int i) { return HALF == 2 ? dw % (NK / 8) * 8 + x8 : (uint32_t)(i * (ND / 32) + dw) * 8 + x8; };
+        // K: item j of this thread is word part y4 of the groups from 4 ka(j) on, at position kpos(j); V: the eight
+        // positions tb, word part x8, groups from gq * GV on
+        auto kpos = [&](int j) { return (uint32_t)(j * (ND / 32) + dw) % (NK / 8) * 8 + x8; };
+        auto ka = [&](int j) { return (uint32_t)(j * (ND / 32) + dw) / (NK / 8); };
         const uint32_t vi = dw * 4 + y4, tb = vi % (NK / 8), gq = vi / (NK / 8);
         const int32_t *table = a.tables + (uint64_t)req * a.ld_tables;
         const uint32_t shift = a.c.page_shift;
@@ -375,9 +373,9 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
                 k_ok[j] = pos < end && (uint32_t)kb[j] < a.c.n_blocks;
                 if (k_ok[j]) {
                     const uint8_t *tl = tile_of(kb[j], pos);
-                    ldg_words<KG>(kr[j], tl + p * L::KROW + (G < 4 ? y4 * G : (ka * 4 + y4) * 4) * 4);
-                    ldg_words<KG>(ks[j], tl + L::KS + (p >> 1) * (G * 4) + ka * 16);
-                    ldg_words<KG / 2>(km[j], tl + L::KM + p * (G * 2) + ka * 8);
+                    ldg_words<KG>(kr[j], tl + p * L::KROW + (G < 4 ? y4 * G : (ka(j) * 4 + y4) * 4) * 4);
+                    ldg_words<KG>(ks[j], tl + L::KS + (p >> 1) * (G * 4) + ka(j) * 16);
+                    ldg_words<KG / 2>(km[j], tl + L::KM + p * (G * 2) + ka(j) * 8);
                 }
             }
         };
@@ -402,8 +400,8 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
         }
         for (uint32_t i = 0; i < n; i++) {
             const uint32_t b = i & 1;
-            wait(&k_free[b], (i >> 1 & 1) ^ 1);
-            uint8_t *k_hi = buf_s + b * C::BUF, *k_lo = k_hi + C::K_BYTES, *k_m = k_lo + C::K_BYTES, *v_t = k_m + C::M_BYTES;
+            wait(k_free, (i & 1) ^ 1);
+            uint8_t *k_hi = smem + C::K_AT, *k_lo = k_hi + C::K_BYTES, *k_m = smem + C::M_AT, *v_t = smem + C::V_AT + b * C::V_BYTES;
             const int32_t t = (k0 + (int32_t)i) * NK;
 #pragma unroll
             for (int j = 0; j < KI; j++) {
@@ -418,7 +416,7 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
                     codes(k_ok[j] ? kr[j][g] : 0u, c);
 #pragma unroll
                     for (int k = 0; k < 4; k++) h[k] = hmul2(c[k], s), l[k] = hfma2(c[k], s, hneg2(h[k]));
-                    const uint32_t chunk = ((G < 4 ? g : ka * 4 + g) * 4 + y4) * 128;
+                    const uint32_t chunk = ((G < 4 ? g : ka(j) * 4 + g) * 4 + y4) * 128;
                     *reinterpret_cast<uint4 *>(hi + chunk) = make_uint4(h[0], h[1], h[2], h[3]);
                     *reinterpret_cast<uint4 *>(lo + chunk) = make_uint4(l[0], l[1], l[2], l[3]);
                 }
@@ -435,18 +433,18 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
                         *reinterpret_cast<uint4 *>(m) = make_uint4(w[0], w[1], w[0], w[1]);
                         *reinterpret_cast<uint4 *>(m + 128) = make_uint4(0u, 0u, 0u, 0u);
                     } else {
-                        *reinterpret_cast<uint2 *>(m + ka * 8) = make_uint2(w[0], w[1]);
-                        *reinterpret_cast<uint2 *>(m + 128 + ka * 8) = make_uint2(w[0], w[1]);
+                        *reinterpret_cast<uint2 *>(m + ka(j) * 8) = make_uint2(w[0], w[1]);
+                        *reinterpret_cast<uint2 *>(m + 128 + ka(j) * 8) = make_uint2(w[0], w[1]);
                     }
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            if (y4 == 0 && ka == 0) {
+            if (y4 == 0) {
 #pragma unroll
                 for (int j = 0; j < KI; j++)
-                    if ((kpos(j) & 15) == 0) reinterpret_cast<uint8_t *>(there_s + (i & 3))[kpos(j) / 16] = k_ok[j];
+                    if ((kpos(j) & 15) == 0 && ka(j) == 0) reinterpret_cast<uint8_t *>(there_s + (i & 3) * 2)[kpos(j) / 16] = k_ok[j];
             }
-            arrive(&k_full[b]);
+            arrive(k_full);
             if (i + 1 < n) {
                 load_k(i + 1);
                 if (i + 2 < n) entries_k(i + 2);
@@ -486,65 +484,73 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
         const int64_t place = (int64_t)seq - nq + rr / a.group;
         const int32_t hi_t = live ? (int32_t)max((int64_t)0, min(place + 1, (int64_t)end)) : 0;
         const int32_t lo_t = a.window && place + 1 > (int64_t)a.window ? (int32_t)(place + 1 - a.window) : 0;
-        constexpr uint32_t ALL = NK == 64 ? 0x01010101u : 0x0101u;
+        const uint32_t s_at = mine + C::S_COL + h * NK, o_at = mine + C::O_COL + h * D;
         float m = -INFINITY, l = 0.0f;
         for (uint32_t i = 0; i < n; i++) {
             const int32_t t0 = (k0 + (int32_t)i) * NK;
-            wait(&s_full[h], i & 1);
+            wait(&s_full[h], i & 1);  // and the sums of the step before are done
             __syncwarp();
             fence_after();
-            uint32_t s[NK / 32][32];
+            const uint2 there = *reinterpret_cast<const uint2 *>(there_s + (i & 3) * 2);
+            const bool whole = t0 >= lo_t && t0 + NK <= hi_t && (there.x & there.y) == 0x01010101u;
+            auto masked = [&](uint32_t (&s)[32], int c) {
+                if (whole) return;
 #pragma unroll
-            for (int c = 0; c < NK / 32; c++) tmem_ld32(mine + C::S_COL + h * NK + c * 32, s[c]);
-            const uint32_t there = there_s[i & 3];
-            fence_before();
-            arrive(&s_free[h]);
+                for (int k = 0; k < 32; k++) {
+                    const int32_t t = c + k;
+                    if (t0 + t < lo_t || t0 + t >= hi_t || !((t < 64 ? there.x : there.y) >> (t / 16 % 4 * 8) & 1)) s[k] = 0xFF800000u;
+                }
+            };
+            // 32 scores at a time, twice: for the maximum, and for the weights
             float top = -INFINITY;
-            if (t0 < lo_t || t0 + NK > hi_t || (there & ALL) != ALL) {
 #pragma unroll
-                for (int c = 0; c < NK; c++)
-                    if (t0 + c < lo_t || t0 + c >= hi_t || !(there >> (c / 16 * 8) & 1)) s[c / 32][c % 32] = 0xFF800000u;
+            for (int c = 0; c < NK; c += 32) {
+                uint32_t s[32];
+                __syncwarp();
+                tmem_ld32(s_at + c, s);
+                masked(s, c);
+                float t1 = __uint_as_float(s[0]), t2 = __uint_as_float(s[1]);
+#pragma unroll
+                for (int k = 2; k < 32; k += 2) t1 = fmaxf(t1, __uint_as_float(s[k])), t2 = fmaxf(t2, __uint_as_float(s[k + 1]));
+                top = fmaxf(top, fmaxf(t1, t2));
             }
-#pragma unroll
-            for (int c = 0; c < NK; c++) top = fmaxf(top, __uint_as_float(s[c / 32][c % 32]));
             top *= cs;
             // the reference of the weights follows the maximum when that is 2^LAG above it
             const bool up = top > m + LAG;
-            float f = 1.0f;
-            if (up) {
-                f = ex2(m - top);
-                m = top;
-                l *= f;
-            }
-            const float shift = m == -INFINITY ? 0.0f : P_SHIFT - m;
-            uint32_t p[NK / 2];
-            float l0 = 0.0f, l1 = 0.0f;
-#pragma unroll
-            for (int c = 0; c < NK; c += 2) {
-                const float p0 = ex2(fmaf(__uint_as_float(s[c / 32][c % 32]), cs, shift)), p1 = ex2(fmaf(__uint_as_float(s[c / 32][c % 32 + 1]), cs, shift));
-                l0 += p0, l1 += p1;
-                p[c / 2] = pack2(p0, p1);
-            }
-            l += l0 + l1;
-            if (i) {
-                wait(&pv_done[h], (i - 1) & 1);
-                __syncwarp();
-                fence_after();
-                if (__any_sync(~0u, up)) {
+            if (__any_sync(~0u, up)) {
+                const float f = up ? ex2(m - top) : 1.0f;
+                if (up) m = top, l *= f;
+                if (i) {
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         uint32_t o[32];
-                        tmem_ld32(mine + C::O_COL + h * D + c, o);
+                        __syncwarp();
+                        tmem_ld32(o_at + c, o);
 #pragma unroll
                         for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                        tmem_st16(mine + C::O_COL + h * D + c, o);
-                        tmem_st16(mine + C::O_COL + h * D + c + 16, o + 16);
+                        tmem_st16(o_at + c, o);
+                        tmem_st16(o_at + c + 16, o + 16);
                     }
                 }
             }
-            __syncwarp();
+            const float shift = m == -INFINITY ? 0.0f : P_SHIFT - m;
+            float l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
-            for (int c = 0; c < NK / 2; c += 16) tmem_st16(mine + C::P_COL + h * (NK / 2) + c, p + c);
+            for (int c = 0; c < NK; c += 32) {
+                uint32_t s[32], p[16];
+                __syncwarp();
+                tmem_ld32(s_at + c, s);
+                masked(s, c);
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) {
+                    const float p0 = ex2(fmaf(__uint_as_float(s[k]), cs, shift)), p1 = ex2(fmaf(__uint_as_float(s[k + 1]), cs, shift));
+                    l0 += p0, l1 += p1;
+                    p[k / 2] = pack2(p0, p1);
+                }
+                __syncwarp();
+                tmem_st16(s_at + c / 2, p);  // over scores that are taken
+            }
+            l += l0 + l1;
             tmem_st_wait();
             fence_before();
             arrive(&p_full[h]);
