@@ -630,11 +630,13 @@ cudaError_t kv4_prefill_launch(const Kv4AttnArgs &a, int32_t type, uint32_t d, c
 
 bool kv4_prefill_pays(const Kv4AttnArgs &a, int32_t type, uint32_t d, int sms) {
     if (type == SG_F32 || a.n_req == 0) return false;
-    // Device cycles per cached position, both measured on a long context of heads of 128: the tensor-core kernel
-    // takes 26 a wave of its CTAs (256 rows each, 128 where a head has 256 values), the other one 0.007 a row.
+    // Rows (of all heads and requests) a wave of its CTAs from which this kernel is the faster one.  Measured in bf16
+    // over 500 to 8000 positions: heads of 128 at 6656 rows a wave 85 us against 65 in the streaming kernel, at 8192
+    // 126 against 143, at 13312 78 against 105; heads of 64 cross at the same place (69 against 46, 100 against 95, 60
+    // against 73); heads of 256, whose tiles are half as tall, at 5216 73 against 65 and at 6656 112 against 119.
     const uint64_t per = d == 256 ? 128 : 256, rows = (uint64_t)a.n_tok * a.group;
     const uint64_t ctas = (rows / per + a.n_req) * a.c.heads, waves = (ctas + sms - 1) / sms;
-    return rows * a.c.heads * 7 > waves * 26000;
+    return rows * a.c.heads > waves * (d == 256 ? 5700 : 7700);
 }
 
 }  // namespace sg
