@@ -156,7 +156,7 @@ constexpr float P_SHIFT = 2.0f, LAG = 8.0f;
 constexpr int ROWS = 8;
 constexpr uint32_t MAX_REQ = 1024;  // requests of one launch (their steps are in shared memory)
 constexpr uint32_t MAX_CTAS = 192;
-constexpr uint32_t MIN_WARPS = 4;   // warps that a CTA uses at least, where the steps are few
+constexpr uint32_t MIN_WARPS = 7;   // warps that a CTA uses at least, where the steps are few
 
 template <typename T, int D>
 struct Cfg {

@@ -36,12 +36,23 @@ def _type(t, what):
         raise TypeError("%s must be float32, float16 or bfloat16" % what) from None
 
 
-def _i32(t, what, shape=None):
-    if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
+def _i32(t, what, n=None):
+    if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous():
         raise TypeError("%s must be a contiguous int32 CUDA tensor" % what)
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError("%s must have the shape %s" % (what, shape))
+    if n is not None and t.numel() != n:
+        raise ValueError("%s must have %d entries" % (what, n))
     return t.data_ptr()
+
+
+def _tables(t, n):
+    """Pointer, row stride and width of a block table for n requests."""
+    if t.dtype is not torch.int32 or t.dim() != 2 or not t.is_cuda:
+        raise ValueError("tables must be an int32 CUDA tensor [n_req, width]")
+    rows, width = t.shape
+    ld, one = t.stride()
+    if rows != n or (one != 1 and width > 1 and rows):
+        raise ValueError("tables must be int32 [%d, width] with contiguous rows" % n)
+    return t.data_ptr(), ld, width
 
 
 class Kv4Cache:
@@ -59,6 +70,7 @@ class Kv4Cache:
             raise ValueError("data must be a contiguous uint8 CUDA tensor of %d bytes" % need)
         self.data = data
         self.nonfinite = torch.zeros(1, dtype=torch.int32, device=data.device)
+        self._nonfinite = self.nonfinite.data_ptr()
         self.desc = SgKv4(head_dim, n_kv_heads, page, n_blocks, data.data_ptr())
         self._c = C.byref(self.desc)
 
@@ -100,8 +112,7 @@ def kv4_plan(plan, ctx, new, tables, ring=None, cursor=None, stream=None):
     n = ctx.numel()
     if n != plan.n_req:
         raise ValueError("the plan is made for %d requests" % plan.n_req)
-    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != n or (tables.numel() and tables.stride(1) != 1):
-        raise ValueError("tables must be int32 [n_req, width] with contiguous rows")
+    table, ld, width = _tables(tables, n)
     if (ring is None) != (cursor is None):
         raise ValueError("ring and cursor come together")
     own = cursor is None
@@ -112,8 +123,8 @@ def kv4_plan(plan, ctx, new, tables, ring=None, cursor=None, stream=None):
     turn = plan._turn ^ 1
     info = plan._infos[turn]
     cu, seq, pos, slots = plan._out
-    st = _lib.load().sg_kv4_plan(plan.page, plan.n_blocks, n, _i32(ctx, "ctx"), _i32(new, "new", (n,)), tables.data_ptr(),
-                                 tables.stride(0), tables.shape[1], _i32(ring, "ring"), _i32(cursor, "cursor"), cu, seq, pos,
+    st = _lib.load().sg_kv4_plan(plan.page, plan.n_blocks, n, _i32(ctx, "ctx"), _i32(new, "new", n), table,
+                                 ld, width, _i32(ring, "ring"), _i32(cursor, "cursor"), cu, seq, pos,
                                  slots, plan.max_tokens, info.data_ptr(), _s(stream, tables))
     if st:
         _lib.check(st, "kv4_plan")
@@ -122,21 +133,23 @@ def kv4_plan(plan, ctx, new, tables, ring=None, cursor=None, stream=None):
 
 
 def _rows(cache, t, what):
-    if t.dim() != 3 or t.shape[1] != cache.n_kv_heads or t.shape[2] != cache.head_dim or t.stride(2) != 1:
-        raise ValueError("%s must be [n_tok, %d, %d] with contiguous rows" % (what, cache.n_kv_heads, cache.head_dim))
+    """Number, token and head stride of rows of the cache's heads."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != cache.n_kv_heads or shape[2] != cache.head_dim or stride[2] != 1 or not t.is_cuda:
+        raise ValueError("%s must be a CUDA tensor [n_tok, %d, %d] with contiguous rows" % (what, cache.n_kv_heads, cache.head_dim))
+    return shape[0], stride[0], stride[1]
 
 
 def kv4_append(cache, k, v, slots, stream=None):
     """Quantizes the rows k, v [n_tok, n_kv_heads, head_dim] (float32, float16 or
     bfloat16, any token and head strides) into their slots (int32 [n_tok], as
     kv4_plan makes them; negative: the row is left out)."""
-    _rows(cache, k, "k")
-    _rows(cache, v, "v")
-    if v.dtype != k.dtype or v.shape[0] != k.shape[0]:
+    n, kt, kh = _rows(cache, k, "k")
+    nv, vt, vh = _rows(cache, v, "v")
+    if v.dtype is not k.dtype or nv != n:
         raise ValueError("k and v must have one type and one number of rows")
-    n = k.shape[0]
-    st = _lib.load().sg_kv4_append(cache._c, _type(k, "k"), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                                   v.stride(1), _i32(slots, "slots", (n,)), n, cache.nonfinite.data_ptr(), _s(stream, k))
+    st = _lib.load().sg_kv4_append(cache._c, _type(k, "k"), k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _i32(slots, "slots", n), n,
+                                   cache._nonfinite, _s(stream, k))
     if st:
         _lib.check(st, "kv4_append")
 
@@ -150,10 +163,9 @@ def kv4_read(cache, slots, out=None, dtype=torch.float16, stream=None):
             out = tuple(torch.empty(n, cache.n_kv_heads, cache.head_dim, dtype=dtype, device=slots.device)
                         for _ in range(2))
     k, v = out
-    for t in out:
-        _rows(cache, t, "out")
-        if t.shape[0] != n or t.dtype != k.dtype or not t.is_contiguous():
-            raise ValueError("out must be two contiguous tensors of one type with a row per slot")
+    if (_rows(cache, k, "out")[0] != n or _rows(cache, v, "out")[0] != n or v.dtype is not k.dtype or not k.is_contiguous() or
+            not v.is_contiguous()):
+        raise ValueError("out must be two contiguous tensors of one type with a row per slot")
     st = _lib.load().sg_kv4_read(cache._c, _type(k, "out"), _i32(slots, "slots"), n, k.data_ptr(), v.data_ptr(), _s(stream, k))
     if st:
         _lib.check(st, "kv4_read")
@@ -178,23 +190,23 @@ def kv4_attention(cache, q, cu, seq, tables, scale=None, window=0, max_new=0, ou
     knows one.  lse: optional float32 [n_tok, n_heads] to fill with the log of the
     softmax's sum.  Returns out, [n_tok, n_heads, head_dim] of q's type."""
     n = seq.numel()
-    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.stride(2) != 1:
-        raise ValueError("q must be [n_tok, n_heads, %d] with contiguous rows" % cache.head_dim)
-    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != n or (tables.numel() and tables.stride(1) != 1):
-        raise ValueError("tables must be int32 [n_req, width] with contiguous rows")
+    shape, stride = q.shape, q.stride()
+    if len(shape) != 3 or shape[2] != cache.head_dim or stride[2] != 1 or not q.is_cuda:
+        raise ValueError("q must be a CUDA tensor [n_tok, n_heads, %d] with contiguous rows" % cache.head_dim)
+    table, ld, width = _tables(tables, n)
     if out is None:
         with _on(stream):
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+    ostride = out.stride()
+    if out.shape != shape or out.dtype is not q.dtype or ostride[2] != 1:
         raise ValueError("out must have q's shape and type, and contiguous rows")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()):
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != shape[:2] or not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous float32 [n_tok, n_heads]")
     if scratch is None:
         scratch = kv4_attention_scratch(q.device, stream)
-    a = SgKv4Attn(_type(q, "q"), q.shape[1], q.shape[0], n, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(),
-                  out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), _i32(cu, "cu", (n + 1,)),
-                  _i32(seq, "seq"), tables.data_ptr(), tables.stride(0), tables.shape[1], 0.0 if scale is None else scale,
-                  window, max_new, scratch.data_ptr(), scratch.numel())
+    a = SgKv4Attn(_type(q, "q"), shape[1], shape[0], n, q.data_ptr(), stride[0], stride[1], out.data_ptr(), ostride[0], ostride[1],
+                  None if lse is None else lse.data_ptr(), _i32(cu, "cu", n + 1), _i32(seq, "seq"), table, ld, width,
+                  0.0 if scale is None else scale, window, max_new, scratch.data_ptr(), scratch.numel())
     st = _lib.load().sg_kv4_attention(cache._c, C.byref(a), _s(stream, q))
     if st:
         _lib.check(st, "kv4_attention")
@@ -220,17 +232,18 @@ def logprobs(logits, tokens=None, top=0, out=None, stream=None):
     int32 [rows] or None, top up to 64 alternatives.  Returns a LogProbs (out, if
     given): the log probability and the rank (0: the likeliest) of each given
     token, the entropy in nats, and the `top` likeliest tokens."""
-    if logits.dim() != 2 or (logits.numel() and logits.stride(1) != 1) or not logits.is_cuda:
+    shape, stride = logits.shape, logits.stride()
+    if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1) or not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor [rows, vocab] with contiguous rows")
-    rows, vocab = logits.shape
+    rows, vocab = shape
     if out is None:
         with _on(stream):
             out = LogProbs(rows, top, logits.device)
     elif out.rows != rows or out.top != top:
         raise ValueError("out is made for %d rows and top %d" % (out.rows, out.top))
     lp, ent, rank, ids, tops = out._p
-    st = _lib.load().sg_logprobs(_type(logits, "logits"), logits.data_ptr(), logits.stride(0), rows, vocab,
-                                 None if tokens is None else _i32(tokens, "tokens", (rows,)), lp, ent, rank, top, ids, tops,
+    st = _lib.load().sg_logprobs(_type(logits, "logits"), logits.data_ptr(), stride[0], rows, vocab,
+                                 None if tokens is None else _i32(tokens, "tokens", rows), lp, ent, rank, top, ids, tops,
                                  _s(stream, logits))
     if st:
         _lib.check(st, "logprobs")
