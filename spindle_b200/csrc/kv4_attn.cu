@@ -417,14 +417,18 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
 
     bool dead = false;  // a wait ran out
     const uint32_t n_mine = warp < WARPS ? n : 0;
-    for (uint32_t idx = 0; idx < n_mine; idx++, t0 += STEP) {
+    auto landed = [&]() {
         if (!dead && !mbar_wait_bounded(&bar[stage], phase, WAIT_LIMIT_NS)) {
             dead = true;
             if (lane == 0) atomicExch(&g_dev_status, (unsigned)DEV_TIMEOUT_TMA);
         }
+    };
+    for (uint32_t idx = 0; idx < n_mine; idx++, t0 += STEP) {
+        if (idx) landed();
         if (idx == c_end) {
-            // a new segment: its query rows as operand registers
-            const Seg &seg = segs[c_seg];
+            // a new segment: its query rows as operand registers; the first one's while its copies are on their way (the
+            // others come with theirs)
+            const Seg seg = idx ? segs[c_seg] : seg_at(w0);
             c_end = min(n, seg.begin + seg.steps - w0);
             t0 = (int32_t)(seg.r.s0 + (w0 + idx - seg.begin)) * STEP;
             held_end = seg.end;
@@ -534,6 +538,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
             for (int g = 0; g < G; g++) kmul[g] = 0x78007800u;  // 2^15
         }
 
+        if (!idx) landed();
         uint8_t *buf = ring + stage * C::STAGE_BYTES;
         const uint32_t here = there_s[warp * STAGES + stage];
         // whole: every row sees every position of the step
