@@ -12,18 +12,22 @@
 // rows) meet in shared memory at the end of the CTA, and those that span CTAs in
 // scratch, where the last CTA to arrive joins them, always in position order.
 //
-// Arithmetic.  All products are m16n8k16 f16 tensor operations with f32 sums,
-// and the cache's codes go into them as they are: a code c masked out of its
-// word is the f16 number c * 2^-24 (or c * 2^-20), exact, so a pair of values
-// costs one AND.  With a value m + s c, per group g of 32 values
-//   q.k   = sum_g s_g (q_g . c_g) + sum_g m_g sum(q_g)
-//   sum_t p_t v_t = sum_t (p_t s_tg) c_t + sum_t p_t m_tg
-// where the scales s_g are applied in f32 to the small results on the K side and
-// to p on the V side.  The codes are the 16-row operand (16 positions for the
-// scores, 16 values of a position for the sums), the eight query rows the 8-wide
-// one; p, p s and an f32 q go in as the f16 rounding and, in a second product,
-// the rounding of what that left (about 22 bits together).  A 16-bit q is exact
-// after scaling by a power of two.  So every product is as good as one in f32.
+// Arithmetic.  All products are m16n8k16 f16 tensor operations with f32 sums, the
+// codes the 16-row operand (16 positions for the scores, 16 values of a position
+// for the sums), the eight query rows the 8-wide one.  A code becomes an exact f16
+// number with a mask into the mantissa of 1024 or 64 and a subtraction, two values
+// at a time.  (Masked alone it is a subnormal number, exact too, but the tensor
+// cores add such products with ten bits less.)  With a value m + s c, per group g of
+// 32 values
+//   q.k = sum_g s_g (q_g . c_g) + sum_g m_g sum(q_g)
+// with the scales applied in f32 to the small results, and q and its sums as f16
+// rounding and, in a second product, the rounding of what that left (about 22 bits
+// together; a 16-bit q is exact after scaling by a power of two).  The weights p are
+// held the same way.  For 16-bit types the V values are made in f16, one rounding
+// each.  For f32
+//   sum_t p_t v_t = sum_t (p_t s_tg) (c_t - 8) + sum_t p_t (m_tg + 8 s_tg)
+// with p s and m + 8 s in two f16 parts again: around the middle of the codes the
+// long sums stay small, so that nothing of them cancels.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -85,6 +89,28 @@ __device__ __forceinline__ uint32_t fms_h2(uint32_t a, uint32_t b, uint32_t c) {
     asm("{\n .reg .b32 t;\n neg.f16x2 t, %3;\n fma.rn.f16x2 %0, %1, %2, t;\n}" : "=r"(d) : "r"(a), "r"(b), "r"(c));
     return d;
 }
+__device__ __forceinline__ uint32_t add_h2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t sub_h2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+// The codes c - OFF of a word as f16 pairs: nibbles (0, 4), (1, 5), (2, 6), (3, 7).
+template <int OFF>
+__device__ __forceinline__ void codes_h2(uint32_t w, uint32_t (&c)[4]) {
+    constexpr uint32_t M0 = 0x64006400u, M1 = 0x54005400u;  // 1024 and 64, whose units are the nibbles' lowest bits
+    constexpr uint32_t O0 = M0 + OFF * 0x00010001u, O1 = M1 + OFF * 0x00100010u;
+    const uint32_t h = w >> 8;
+    c[0] = sub_h2((w & 0x000F000Fu) | M0, O0);
+    c[1] = sub_h2((w & 0x00F000F0u) | M1, O1);
+    c[2] = sub_h2((h & 0x000F000Fu) | M0, O0);
+    c[3] = sub_h2((h & 0x00F000F0u) | M1, O1);
+}
+
 // d = a b, d += a b
 __device__ __forceinline__ void mma16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
@@ -150,8 +176,8 @@ __device__ __forceinline__ void lds_codes(uint32_t (&w)[G], const uint8_t *row, 
 }
 
 constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
-// Weights are held as 2^P_SHIFT p with p below 2^LAG; V scales are brought below 2^5, so that a product
-// stays inside f16's range above and keeps 30 bits below its largest.
+// Weights are held as 2^P_SHIFT p with p below 2^LAG; in f32 the V scales are brought below 2^5, so that a
+// product stays inside f16's range above and keeps 30 bits below its largest.
 constexpr float P_SHIFT = 2.0f, LAG = 8.0f;
 constexpr int ROWS = 8;
 constexpr uint32_t MAX_REQ = 1024;  // requests of one launch (their steps are in shared memory)
@@ -388,7 +414,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
     uint32_t qb[2 * G][QR], qs[G == 8 ? 2 : 1];
     float o[2 * G][4], om[4];
     float m[2], sh[2], cs[2];  // the weights' reference and its shift; what a score is multiplied by
-    const uint32_t ones = gid == 0 ? 0x3C003C00u : 0u;
+    float l[2];
     int32_t lo_t[2], hi_t[2], full_lo = 0, full_hi = 0;  // positions [lo, hi) that a row sees; that all rows see
     int32_t kexp = 15;   // of group lane % G: V scales are multiplied by 2^kexp
     uint32_t vlim2 = 0;  // and are at most this (f16x2)
@@ -401,15 +427,15 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
     auto rows_of = [&](float (&r)[G][2][4]) {
 #pragma unroll
         for (int g = 0; g < G; g++) {
-            const int k = __shfl_sync(~0u, kexp, g);
-            const float f = __uint_as_float((uint32_t)(127 + 24 - k) << 23), f16 = f * 0.0625f;  // odd nibbles came in 16-fold
+            const float f = Q32 ? __uint_as_float((uint32_t)(127 - __shfl_sync(~0u, kexp, g)) << 23) : 1.0f;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const float mn = __shfl_sync(~0u, om[i], 4 * g + quad);
+                // (the middles came in halved)
+                const float mn = Q32 ? 2.0f * __shfl_sync(~0u, om[i] + om[2 + i], 4 * g + quad) : 0.0f;
                 r[g][i][0] = fmaf(o[2 * g][i], f, mn);
-                r[g][i][1] = fmaf(o[2 * g][2 + i], f16, mn);
+                r[g][i][1] = fmaf(o[2 * g][2 + i], f, mn);
                 r[g][i][2] = fmaf(o[2 * g + 1][i], f, mn);
-                r[g][i][3] = fmaf(o[2 * g + 1][2 + i], f16, mn);
+                r[g][i][3] = fmaf(o[2 * g + 1][2 + i], f, mn);
             }
         }
     };
@@ -448,7 +474,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
 #pragma unroll
                     for (int k = 0; k < 8; k++) raw[g][k] = q[g * 32 + k];
             }
-            // q * 2^(14 - e) is below 2^15 in f16; e is kept where 2^(14 - e) and 2^(e + 10) are f32 numbers.
+            // q * 2^(14 - e) is below 2^15 in f16; e is kept where that power and its inverse are f32 numbers.
             // A row that is no row stands in with the values of the first one.
             int e;
             if constexpr (Q32) {
@@ -473,14 +499,13 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
             }
             e = min(max(e, -100), 116);
             const float up = copysignf(__uint_as_float((uint32_t)(127 + 14 - e) << 23), a.scale);
-            const float cs_row = fabsf(a.scale) * LOG2E * __uint_as_float((uint32_t)(127 + 10 + e) << 23);
-            const float up16 = up * 0.0625f;
+            const float cs_row = fabsf(a.scale) * LOG2E * __uint_as_float((uint32_t)(127 - 14 + e) << 23);
 #pragma unroll
             for (int g = 0; g < G; g++)
 #pragma unroll
-                // nibbles (0, 4), (1, 5), (2, 6), (3, 7) make the four K registers; those of odd ones are 16 c
+                // nibbles (0, 4), (1, 5), (2, 6), (3, 7) make the four K registers
                 for (int k = 0; k < 4; k++) {
-                    const float f = k & 1 ? up16 : up, x0 = Act<T>::get(raw[g][k]) * f, x1 = Act<T>::get(raw[g][k + 4]) * f;
+                    const float x0 = Act<T>::get(raw[g][k]) * up, x1 = Act<T>::get(raw[g][k + 4]) * up;
                     const uint32_t hi = pack_h2(x0, x1);
                     qb[2 * g + (k >> 1)][k & 1] = hi;
                     if constexpr (Q32) {
@@ -488,7 +513,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
                         qb[2 * g + (k >> 1)][2 + (k & 1)] = pack_h2(x0 - h.x, x1 - h.y);
                     }
                 }
-            // The sums of the query's groups, for the K minima: the product with codes of 1, in units of 2^-24.
+            // The sums of the query's groups, for the K minima: the product with ones.
             // Column k of the operand holds group k % G, first the f16 rounding, then what it left.
             {
                 float sum[2] = {0.0f, 0.0f};
@@ -496,16 +521,16 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
 #pragma unroll
                 for (int g = 0; g < G; g++) {
                     float d[4];
-                    constexpr uint32_t C0 = 0x00010001u, C1 = 0x00100010u;
-                    mma16_first(d, C0, C0, C1, C1, qb[2 * g][0], qb[2 * g][1]);
-                    mma16(d, C0, C0, C1, C1, qb[2 * g + 1][0], qb[2 * g + 1][1]);
+                    constexpr uint32_t ONE = 0x3C003C00u;
+                    mma16_first(d, ONE, ONE, ONE, ONE, qb[2 * g][0], qb[2 * g][1]);
+                    mma16(d, ONE, ONE, ONE, ONE, qb[2 * g + 1][0], qb[2 * g + 1][1]);
                     if constexpr (Q32) {
-                        mma16(d, C0, C0, C1, C1, qb[2 * g][2], qb[2 * g][3]);
-                        mma16(d, C0, C0, C1, C1, qb[2 * g + 1][2], qb[2 * g + 1][3]);
+                        mma16(d, ONE, ONE, ONE, ONE, qb[2 * g][2], qb[2 * g][3]);
+                        mma16(d, ONE, ONE, ONE, ONE, qb[2 * g + 1][2], qb[2 * g + 1][3]);
                     }
                     if ((int)(gid % G) == g) sum[0] = d[0], sum[1] = d[1];
                 }
-                const float f = 0x1p18f;  // 2^24 of the codes' unit, 2^-6 to stay inside f16
+                const float f = 0x1p-6f;  // inside f16's range
                 hi[0] = pack_h2(sum[0] * f, sum[1] * f);
                 const float2 h = unpack_h2(hi[0]);
                 lo[0] = pack_h2(fmaf(sum[0], f, -h.x), fmaf(sum[1], f, -h.y));
@@ -528,7 +553,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
                 cs[i] = __shfl_sync(~0u, cs_row, src);
                 hi_t[i] = __shfl_sync(~0u, hi_row, src);
                 lo_t[i] = __shfl_sync(~0u, lo_row, src);
-                m[i] = -INFINITY, sh[i] = 0.0f;
+                m[i] = -INFINITY, sh[i] = 0.0f, l[i] = 0.0f;
             }
             kexp = 15, vlim2 = 0x13FF13FFu;  // the f16 below 2^-10
 #pragma unroll
@@ -561,16 +586,18 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
             if constexpr (G == 8) mma16_first(c, km0, km1, km0, km1, qs[0], qs[1]);
             else mma8_first(c, km0, km1, qs[0]);
 #pragma unroll
-            for (int k = 0; k < 4; k++) s[i][k] = c[k] * 0x1p-18f;
+            for (int k = 0; k < 4; k++) s[i][k] = c[k] * 0x1p6f;
 #pragma unroll
             for (int g = 0; g < G; g++) {
-                const uint32_t h0 = w0_[g] >> 8, h1 = w1_[g] >> 8;
+                uint32_t ca[4], cb[4];
+                codes_h2<0>(w0_[g], ca);
+                codes_h2<0>(w1_[g], cb);
                 float d[4];
-                mma16_first(d, w0_[g] & 0x000F000Fu, w1_[g] & 0x000F000Fu, w0_[g] & 0x00F000F0u, w1_[g] & 0x00F000F0u, qb[2 * g][0], qb[2 * g][1]);
-                mma16(d, h0 & 0x000F000Fu, h1 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x00F000F0u, qb[2 * g + 1][0], qb[2 * g + 1][1]);
+                mma16_first(d, ca[0], cb[0], ca[1], cb[1], qb[2 * g][0], qb[2 * g][1]);
+                mma16(d, ca[2], cb[2], ca[3], cb[3], qb[2 * g + 1][0], qb[2 * g + 1][1]);
                 if constexpr (Q32) {
-                    mma16(d, w0_[g] & 0x000F000Fu, w1_[g] & 0x000F000Fu, w0_[g] & 0x00F000F0u, w1_[g] & 0x00F000F0u, qb[2 * g][2], qb[2 * g][3]);
-                    mma16(d, h0 & 0x000F000Fu, h1 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x00F000F0u, qb[2 * g + 1][2], qb[2 * g + 1][3]);
+                    mma16(d, ca[0], cb[0], ca[1], cb[1], qb[2 * g][2], qb[2 * g][3]);
+                    mma16(d, ca[2], cb[2], ca[3], cb[3], qb[2 * g + 1][2], qb[2 * g + 1][3]);
                 }
                 // scales of positions gid (even or odd in its pair) for two groups in one register
                 if (g % 2 == 0) {
@@ -627,12 +654,13 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
 #pragma unroll
                 for (int i = 0; i < 2 * G; i++) o[i][r] *= f, o[i][2 + r] *= f;
                 om[r] *= f, om[2 + r] *= f;
+                l[r] *= f;
                 sh[r] = mm == -INFINITY ? 0.0f : P_SHIFT - mm;
             }
         }
 
         // a V scale larger than any before: the group's sums move to a new power of two
-        {
+        if constexpr (Q32) {
             constexpr int N = TILES * (G == 8 ? 2 : 1);  // the 8 G words of a tile's scales, lane l's of group l % G
             uint32_t vw[N], wmax = vlim2;
 #pragma unroll
@@ -670,36 +698,60 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const float p0 = ex2(fmaf(s[i][2 * j], cs[0], sh[0])), p1 = ex2(fmaf(s[i][2 * j + 1], cs[1], sh[1]));
+                l[0] += p0, l[1] += p1;
                 ph[j] = pack_h2(p0, p1);
                 const float2 h = unpack_h2(ph[j]);
                 pl[j] = transpose8(pack_h2(p0 - h.x, p1 - h.y));
                 ph[j] = transpose8(ph[j]);
             }
-            uint32_t vs[2][G], vm[2], v[2][G];
+            uint32_t vs[2][G], v[2][G];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 lds_words<G>(vs[j], tile + L::VS + (4 * j + quad) * (G * 4));
-                vm[j] = *reinterpret_cast<const uint32_t *>(tile + L::VM + ((4 * j + quad) * G + gid % G) * 4);
                 lds_codes<G, 8>(v[j], tile + L::VC + (4 * j + quad) * L::VROW, gid);
             }
-            // row gid of this product is the minima of group gid % G, row 8 the sum of the weights
-            mma16(om, vm[0], ones, vm[1], ones, ph[0], ph[1]);
-            mma16(om, vm[0], ones, vm[1], ones, pl[0], pl[1]);
-#pragma unroll
-            for (int g = 0; g < G; g++) {
-                uint32_t hi[2], lo[2];
+            if constexpr (Q32) {
+                // row gid of this product is half the middle m + 8 s of group gid % G, row 8 + gid what its f16 rounding left
+                uint32_t mid[2], rest[2];
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    // (ph + pl) sc as the f16 rounding of ph sc and the rest
-                    const uint32_t sc = mul_h2(vs[j][g], kmul[g]);
-                    hi[j] = mul_h2(ph[j], sc);
-                    lo[j] = fma_h2(pl[j], sc, fms_h2(ph[j], sc, hi[j]));
+                    const uint32_t at = ((4 * j + quad) * G + gid % G) * 4;
+                    const uint32_t x = mul_h2(*reinterpret_cast<const uint32_t *>(tile + L::VS + at), 0x44004400u);  // 4 s
+                    const uint32_t y = mul_h2(*reinterpret_cast<const uint32_t *>(tile + L::VM + at), 0x38003800u);  // m / 2
+                    mid[j] = add_h2(x, y);
+                    const uint32_t yy = sub_h2(mid[j], x);
+                    rest[j] = add_h2(sub_h2(x, sub_h2(mid[j], yy)), sub_h2(y, yy));  // exactly x + y - mid
                 }
-                const uint32_t h0 = v[0][g] >> 8, h1 = v[1][g] >> 8;
-                mma16(o[2 * g], v[0][g] & 0x000F000Fu, v[0][g] & 0x00F000F0u, v[1][g] & 0x000F000Fu, v[1][g] & 0x00F000F0u, hi[0], hi[1]);
-                mma16(o[2 * g], v[0][g] & 0x000F000Fu, v[0][g] & 0x00F000F0u, v[1][g] & 0x000F000Fu, v[1][g] & 0x00F000F0u, lo[0], lo[1]);
-                mma16(o[2 * g + 1], h0 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x000F000Fu, h1 & 0x00F000F0u, hi[0], hi[1]);
-                mma16(o[2 * g + 1], h0 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x000F000Fu, h1 & 0x00F000F0u, lo[0], lo[1]);
+                mma16(om, mid[0], rest[0], mid[1], rest[1], ph[0], ph[1]);
+                mma16(om, mid[0], rest[0], mid[1], rest[1], pl[0], pl[1]);
+            }
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                uint32_t c0[4], c1[4], bh[2], bl[2];
+                if constexpr (Q32) {
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        // (ph + pl) sc as the f16 rounding of ph sc and the rest
+                        const uint32_t sc = mul_h2(vs[j][g], kmul[g]);
+                        bh[j] = mul_h2(ph[j], sc);
+                        bl[j] = fma_h2(pl[j], sc, fms_h2(ph[j], sc, bh[j]));
+                    }
+                    codes_h2<8>(v[0][g], c0);
+                    codes_h2<8>(v[1][g], c1);
+                } else {
+                    // the values themselves
+                    codes_h2<0>(v[0][g], c0);
+                    codes_h2<0>(v[1][g], c1);
+                    const uint32_t m0 = *reinterpret_cast<const uint32_t *>(tile + L::VM + (quad * G + g) * 4);
+                    const uint32_t m1 = *reinterpret_cast<const uint32_t *>(tile + L::VM + ((4 + quad) * G + g) * 4);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) c0[k] = fma_h2(c0[k], vs[0][g], m0), c1[k] = fma_h2(c1[k], vs[1][g], m1);
+                    bh[0] = ph[0], bh[1] = ph[1], bl[0] = pl[0], bl[1] = pl[1];
+                }
+                mma16(o[2 * g], c0[0], c0[1], c1[0], c1[1], bh[0], bh[1]);
+                mma16(o[2 * g], c0[0], c0[1], c1[0], c1[1], bl[0], bl[1]);
+                mma16(o[2 * g + 1], c0[2], c0[3], c1[2], c1[3], bh[0], bh[1]);
+                mma16(o[2 * g + 1], c0[2], c0[3], c1[2], c1[3], bl[0], bl[1]);
             }
         }
 
@@ -710,7 +762,11 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
 
         if (idx + 1 == c_end) {
             // the end of the segment, or of this warp's part of it
-            const float l[2] = {__shfl_sync(~0u, om[2], quad), __shfl_sync(~0u, om[3], quad)};
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) {
+                l[0] += __shfl_xor_sync(~0u, l[0], off);
+                l[1] += __shfl_xor_sync(~0u, l[1], off);
+            }
             float r[G][2][4];
             rows_of(r);
             const Seg &seg = segs[c_seg];
