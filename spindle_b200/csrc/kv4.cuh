@@ -36,6 +36,37 @@ struct Kv4Tile {
     static constexpr uint32_t VC = 8 * D, KS = 16 * D, KM = 17 * D, VS = 18 * D, VM = 19 * D, BYTES = 20 * D;
 };
 
+// The codes of a word as f16 pairs, c - OFF of the nibbles (0, 4), (1, 5), (2, 6), (3, 7): a nibble in the lowest
+// mantissa bits of 1024, or four bits up in those of 64, less that number.  The masks and numbers are kept in registers
+// that the compiler does not see through, so that mask and insertion are one instruction (which takes one immediate).
+struct Kv4Codes {
+    uint32_t k0, k1, m0, m1;
+    __device__ __forceinline__ Kv4Codes() {
+        asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(k0));
+        asm volatile("mov.b32 %0, 0x00F000F0;" : "=r"(k1));
+        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(m0));
+        asm volatile("mov.b32 %0, 0x54005400;" : "=r"(m1));
+    }
+    static __device__ __forceinline__ uint32_t put(uint32_t w, uint32_t k, uint32_t m) {
+        uint32_t d;
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(w), "r"(k), "r"(m));  // (w & k) | m
+        return d;
+    }
+    static __device__ __forceinline__ uint32_t less(uint32_t a, uint32_t b) {
+        uint32_t d;
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
+    template <int OFF>
+    __device__ __forceinline__ void get(uint32_t w, uint32_t (&c)[4]) const {
+        const uint32_t o0 = OFF ? 0x64006400u + OFF * 0x00010001u : m0, o1 = OFF ? 0x54005400u + OFF * 0x00100010u : m1, h = w >> 8;
+        c[0] = less(put(w, k0, m0), o0);
+        c[1] = less(put(w, k1, m1), o1);
+        c[2] = less(put(h, k0, m0), o0);
+        c[3] = less(put(h, k1, m1), o1);
+    }
+};
+
 struct Kv4Cache {
     uint8_t *data;
     uint32_t n_blocks, page_shift;  // page = 1 << page_shift positions

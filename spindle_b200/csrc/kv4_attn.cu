@@ -23,8 +23,8 @@
 // with the scales applied in f32 to the small results, and q and its sums as f16
 // rounding and, in a second product, the rounding of what that left (about 22 bits
 // together; a 16-bit q is exact after scaling by a power of two).  The weights p are
-// held the same way.  For 16-bit types the V values are made in f16, one rounding
-// each.  For f32
+// held the same way (for bf16 without the rest).  For 16-bit types the V values are
+// made in f16, one rounding each.  For f32
 //   sum_t p_t v_t = sum_t (p_t s_tg) (c_t - 8) + sum_t p_t (m_tg + 8 s_tg)
 // with p s and m + 8 s in two f16 parts again: around the middle of the codes the
 // long sums stay small, so that nothing of them cancels.
@@ -99,18 +99,6 @@ __device__ __forceinline__ uint32_t sub_h2(uint32_t a, uint32_t b) {
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
-// The codes c - OFF of a word as f16 pairs: nibbles (0, 4), (1, 5), (2, 6), (3, 7).
-template <int OFF>
-__device__ __forceinline__ void codes_h2(uint32_t w, uint32_t (&c)[4]) {
-    constexpr uint32_t M0 = 0x64006400u, M1 = 0x54005400u;  // 1024 and 64, whose units are the nibbles' lowest bits
-    constexpr uint32_t O0 = M0 + OFF * 0x00010001u, O1 = M1 + OFF * 0x00100010u;
-    const uint32_t h = w >> 8;
-    c[0] = sub_h2((w & 0x000F000Fu) | M0, O0);
-    c[1] = sub_h2((w & 0x00F000F0u) | M1, O1);
-    c[2] = sub_h2((h & 0x000F000Fu) | M0, O0);
-    c[3] = sub_h2((h & 0x00F000F0u) | M1, O1);
-}
-
 // d = a b, d += a b
 __device__ __forceinline__ void mma16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
@@ -245,6 +233,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
     constexpr int G = L::G, TILES = C::TILES, STAGES = C::STAGES, STEP = C::STEP, WARPS = C::WARPS, THREADS = C::THREADS;
     constexpr bool Q32 = sizeof(T) == 4;
     constexpr int QR = Q32 ? 4 : 2;
+    constexpr bool REST = !std::is_same<T, __nv_bfloat16>::value;  // what the weights' f16 rounding leaves is far below bf16
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring_all = smem;
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::RING);
@@ -409,6 +398,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
     constexpr uint32_t PART = C::PART_BYTES / 4;
 
     // ---- the steps ----
+    const Kv4Codes codes;
     // Operands: scores are K codes (16 positions) times query rows (8), sums V codes (16 values) times weights
     // (8 rows), so that a lane of quad `quad` has rows 2 quad and 2 quad + 1 of every result.
     uint32_t qb[2 * G][QR], qs[G == 8 ? 2 : 1];
@@ -590,8 +580,8 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
 #pragma unroll
             for (int g = 0; g < G; g++) {
                 uint32_t ca[4], cb[4];
-                codes_h2<0>(w0_[g], ca);
-                codes_h2<0>(w1_[g], cb);
+                codes.get<0>(w0_[g], ca);
+                codes.get<0>(w1_[g], cb);
                 float d[4];
                 mma16_first(d, ca[0], cb[0], ca[1], cb[1], qb[2 * g][0], qb[2 * g][1]);
                 mma16(d, ca[2], cb[2], ca[3], cb[3], qb[2 * g + 1][0], qb[2 * g + 1][1]);
@@ -700,14 +690,17 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
                 const float p0 = ex2(fmaf(s[i][2 * j], cs[0], sh[0])), p1 = ex2(fmaf(s[i][2 * j + 1], cs[1], sh[1]));
                 l[0] += p0, l[1] += p1;
                 ph[j] = pack_h2(p0, p1);
-                const float2 h = unpack_h2(ph[j]);
-                pl[j] = transpose8(pack_h2(p0 - h.x, p1 - h.y));
+                if constexpr (REST) {
+                    const float2 h = unpack_h2(ph[j]);
+                    pl[j] = transpose8(pack_h2(p0 - h.x, p1 - h.y));
+                }
                 ph[j] = transpose8(ph[j]);
             }
-            uint32_t vs[2][G], v[2][G];
+            uint32_t vs[2][G], vm[2][G], v[2][G];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 lds_words<G>(vs[j], tile + L::VS + (4 * j + quad) * (G * 4));
+                if constexpr (!Q32) lds_words<G>(vm[j], tile + L::VM + (4 * j + quad) * (G * 4));
                 lds_codes<G, 8>(v[j], tile + L::VC + (4 * j + quad) * L::VROW, gid);
             }
             if constexpr (Q32) {
@@ -736,22 +729,21 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
                         bh[j] = mul_h2(ph[j], sc);
                         bl[j] = fma_h2(pl[j], sc, fms_h2(ph[j], sc, bh[j]));
                     }
-                    codes_h2<8>(v[0][g], c0);
-                    codes_h2<8>(v[1][g], c1);
+                    codes.get<8>(v[0][g], c0);
+                    codes.get<8>(v[1][g], c1);
                 } else {
                     // the values themselves
-                    codes_h2<0>(v[0][g], c0);
-                    codes_h2<0>(v[1][g], c1);
-                    const uint32_t m0 = *reinterpret_cast<const uint32_t *>(tile + L::VM + (quad * G + g) * 4);
-                    const uint32_t m1 = *reinterpret_cast<const uint32_t *>(tile + L::VM + ((4 + quad) * G + g) * 4);
+                    codes.get<0>(v[0][g], c0);
+                    codes.get<0>(v[1][g], c1);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) c0[k] = fma_h2(c0[k], vs[0][g], m0), c1[k] = fma_h2(c1[k], vs[1][g], m1);
-                    bh[0] = ph[0], bh[1] = ph[1], bl[0] = pl[0], bl[1] = pl[1];
+                    for (int k = 0; k < 4; k++) c0[k] = fma_h2(c0[k], vs[0][g], vm[0][g]), c1[k] = fma_h2(c1[k], vs[1][g], vm[1][g]);
+                    bh[0] = ph[0], bh[1] = ph[1];
+                    if constexpr (REST) bl[0] = pl[0], bl[1] = pl[1];
                 }
                 mma16(o[2 * g], c0[0], c0[1], c1[0], c1[1], bh[0], bh[1]);
-                mma16(o[2 * g], c0[0], c0[1], c1[0], c1[1], bl[0], bl[1]);
+                if constexpr (REST) mma16(o[2 * g], c0[0], c0[1], c1[0], c1[1], bl[0], bl[1]);
                 mma16(o[2 * g + 1], c0[2], c0[3], c1[2], c1[3], bh[0], bh[1]);
-                mma16(o[2 * g + 1], c0[2], c0[3], c1[2], c1[3], bl[0], bl[1]);
+                if constexpr (REST) mma16(o[2 * g + 1], c0[2], c0[3], c1[2], c1[3], bl[0], bl[1]);
             }
         }
 

@@ -109,11 +109,6 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
-__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-}
 __device__ __forceinline__ uint32_t hneg2(uint32_t a) {
     uint32_t d;
     asm("neg.f16x2 %0, %1;" : "=r"(d) : "r"(a));
@@ -123,15 +118,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-// The four pairs of a word's codes as f16 numbers: nibbles (0, 4), (1, 5), (2, 6), (3, 7).
-__device__ __forceinline__ void codes(uint32_t w, uint32_t (&c)[4]) {
-    const uint32_t h = w >> 8;
-    c[0] = hsub2((w & 0x000F000Fu) | 0x64006400u, 0x64006400u);  // 1024 + c
-    c[1] = hsub2((w & 0x00F000F0u) | 0x54005400u, 0x54005400u);  // 64 + c
-    c[2] = hsub2((h & 0x000F000Fu) | 0x64006400u, 0x64006400u);
-    c[3] = hsub2((h & 0x00F000F0u) | 0x54005400u, 0x54005400u);
-}
-
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -343,6 +329,7 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
         __syncwarp();
     } else if (tid >= 128 * NQ) {
         // ---- the operands of a step from the cache: its codes are read a step ahead, its table entries two ----
+        const Kv4Codes codes;
         const uint32_t dt = tid - 128 * NQ, dw = dt >> 5, x8 = lane & 7, y4 = lane >> 3;
         // K: item j of this thread is word part y4 of the groups from 4 ka(j) on, at position kpos(j); V: the eight
         // positions tb, word part x8, groups from gq * GV on
@@ -413,7 +400,7 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
                     // the position's scale twice, halved
                     uint32_t s = k_ok[j] ? __byte_perm(ks[j][g], 0, pos & 1 ? 0x3232 : 0x1010) : 0u;
                     s = hmul2(s, 0x38003800u);
-                    codes(k_ok[j] ? kr[j][g] : 0u, c);
+                    codes.get<0>(k_ok[j] ? kr[j][g] : 0u, c);
 #pragma unroll
                     for (int k = 0; k < 4; k++) h[k] = hmul2(c[k], s), l[k] = hfma2(c[k], s, hneg2(h[k]));
                     const uint32_t chunk = ((G < 4 ? g : ka(j) * 4 + g) * 4 + y4) * 128;
@@ -459,7 +446,7 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
                     const uint32_t mask = !v_ok || p >= end ? 0u : p + 1 >= end ? 0xFFFFu : 0xFFFFFFFFu;
                     const uint32_t s = vs[q][g] & mask, m = vm[q][g] & mask;
                     uint32_t c[4];
-                    codes(vr[q][g], c);
+                    codes.get<0>(vr[q][g], c);
 #pragma unroll
                     for (int k = 0; k < 4; k++) val[k][q] = hfma2(c[k], s, m);
                 }
