@@ -12,6 +12,12 @@
 // rows) meet in shared memory at the end of the CTA, and those that span CTAs in
 // scratch, where the last CTA to arrive joins them, always in position order.
 //
+// Measured (device time): one token each of 64 requests of 2048 to 8192 positions, 32 query and 4 KV heads of 128,
+// bf16: 58 us, 3.7 TB/s (57 % of the measured copy rate); one request of 131071 positions, 32 and 8 heads, f16: 53
+// us, 3.2 TB/s; 1037 positions: 13 us; 16 requests of 9 tokens at 2050 positions in f32: 34 us.  What bounds it is
+// issuing instructions, about 600 for 32 positions of eight rows, of which the codes take 290 and the tensor products
+// 34 to 66; starting and joining take about 12 us of a call.
+//
 // Arithmetic.  All products are m16n8k16 f16 tensor operations with f32 sums, the
 // codes the 16-row operand (16 positions for the scores, 16 values of a position
 // for the sums), the eight query rows the 8-wide one.  A code becomes an exact f16
@@ -170,7 +176,7 @@ constexpr float P_SHIFT = 2.0f, LAG = 8.0f;
 constexpr int ROWS = 8;
 constexpr uint32_t MAX_REQ = 1024;  // requests of one launch (their steps are in shared memory)
 constexpr uint32_t MAX_CTAS = 192;
-constexpr uint32_t MIN_WARPS = 7;   // warps that a CTA uses at least, where the steps are few
+constexpr uint32_t MIN_WARPS = 7;   // warps that a CTA uses at least where the steps are few (264 steps: 13.0 us; 4: 13.6, 2: 15.0)
 
 template <typename T, int D>
 struct Cfg {

@@ -14,6 +14,11 @@
 // s c goes in as its f16 rounding and the exact rest, and the minima as 16 more
 // columns against the sums of the query's groups (f16 rounding and rest).  V
 // values and weights are rounded to f16 once each.
+//
+// Two chunks of 1024 and 768 tokens against up to 8100 positions, 32 query and 4 KV heads of 128, bf16: 374 us, 500
+// TFLOP/s of the 186 GFLOP that attention has (30 % of the measured matrix rate; with the rests of K and the minima
+// the products are 1.56 times that).  A step of 128 positions takes a tile 6100 cycles, of which its own thread-per-row
+// work is 3600 and the products of both tiles 3700; the last wave of CTAs is part empty (224 CTAs on 148 SMs).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
