@@ -47,7 +47,7 @@ __device__ __forceinline__ uint32_t warp_scan(uint32_t v, uint32_t lane) {
 // one new position that is a multiple of the page, so the thread of that
 // position writes the table entry, and everyone else computes the block from the
 // ring without reading it back.  A decode step of 64 requests is a launch (5 us); 1.5 million positions of 509
-// requests 13 us, 1.1 TB/s of positions and slots, bound by the searches and the scan that every CTA repeats.
+// requests 13 to 14 us, 1 TB/s of positions and slots, bound by the searches and the scan that every CTA repeats.
 __global__ void __launch_bounds__(KV4_PLAN_THREADS) kv4_plan_kernel(const __grid_constant__ Kv4PlanArgs a) {
     __shared__ uint32_t cu_s[KV4_PLAN_THREADS + 1], want_s[KV4_PLAN_THREADS];
     __shared__ int32_t ctx_s[KV4_PLAN_THREADS];
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(KV4_PLAN_THREADS) kv4_plan_kernel(const __grid
 // with x clamped to f16's finite range and NaN counted as 0, so that the cache
 // holds finite numbers only; groups that had such a value are counted.  Every
 // step is one rounded f32 operation, so the codes can be reproduced bit for bit.
-// What bounds it is the arithmetic (about 8 instructions a value), hence sixteen
+// What bounds it is the arithmetic (19 instructions a value by the counters), hence sixteen
 // values a lane: the place of a row in the cache is worked out half as often.
 // 24001 rows of 8 heads of 128 in bf16: 44 us, 2.9 TB/s (45 % of the measured copy rate); 32 rows are a launch.
 
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(KV4_ROW_THREADS) kv4_append_kernel(const __gri
 
 // ---- read ---------------------------------------------------------------------
 // The values of given slots, m + s * c rounded once; a slot that is no slot reads as zeros.  The rows above to f16:
-// 32 us, 4.0 TB/s, bound by unpacking.
+// 32 us, 4.0 TB/s, bound by unpacking (13 instructions a value).
 template <typename T, int D>
 __global__ void __launch_bounds__(KV4_ROW_THREADS) kv4_read_kernel(const __grid_constant__ Kv4RowArgs a) {
     using L = Kv4Tile<D>;
