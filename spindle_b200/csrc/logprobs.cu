@@ -462,16 +462,19 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
             }
             __syncthreads();
             n = s.count;
-            if (t <= ORDER_NEG_INF && n < want) {
-                // of the first n + want values of the stretch at least want are minus infinities, or all of them are there
-                for (uint32_t i = begin + tid; i < min(end, begin + n + want); i += THREADS) {
-                    const float f = El<T>::get(x[i]);
-                    if (f != -INFINITY) continue;
-                    const uint32_t c = atomicAdd(&s.count, 1u);
-                    if (c < CAP) s.cand[c] = key_of(f, i);
+            if (t <= ORDER_NEG_INF) {
+                __syncthreads();  // every thread has read the count before one adds to it: all go the same way
+                if (n < want) {
+                    // of the first n + want values of the stretch at least want are minus infinities, or all of them are there
+                    for (uint32_t i = begin + tid; i < min(end, begin + n + want); i += THREADS) {
+                        const float f = El<T>::get(x[i]);
+                        if (f != -INFINITY) continue;
+                        const uint32_t c = atomicAdd(&s.count, 1u);
+                        if (c < CAP) s.cand[c] = key_of(f, i);
+                    }
+                    __syncthreads();
+                    n = s.count;
                 }
-                __syncthreads();
-                n = s.count;
             }
             exact = n > CAP;
         }
