@@ -944,7 +944,7 @@ sg_status launch(const Kv4AttnArgs &a0, int sms, cudaStream_t s, cudaError_t *er
     const uint32_t grid = (uint32_t)sms < MAX_CTAS ? (uint32_t)sms : MAX_CTAS, all = a0.c.heads;
     // MAX_REQ requests a launch, and as many heads as keep the number of steps below 2^32
     const uint64_t rows = (uint64_t)a0.n_tok * a0.group / ROWS + a0.n_req, steps = (((uint64_t)a0.width << a0.c.page_shift) + Cfg<T, D>::STEP - 1) / Cfg<T, D>::STEP + 1;
-    const uint64_t heads = (1ull << 31) / (rows * steps);
+    const uint64_t heads = (1ull << 31) / (rows ? rows * steps : 1);  // (no requests and a few tokens of none: no rows)
     if (heads == 0) return SG_ERR_SHAPE;
     for (uint32_t r0 = 0; r0 == 0 || r0 < a0.n_req; r0 += MAX_REQ)
         for (uint32_t h0 = 0; h0 < all; h0 += (uint32_t)(heads < all ? heads : all)) {
