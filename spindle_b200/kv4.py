@@ -36,18 +36,27 @@ def _type(t, what):
         raise TypeError("%s must be float32, float16 or bfloat16" % what) from None
 
 
-def _i32(t, what, n=None):
-    if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous():
-        raise TypeError("%s must be a contiguous int32 CUDA tensor" % what)
+def _dev(t, what):
+    """The index of t's GPU, which has to be the current one: the kernels run there, and
+    every tensor of a call has to lie there."""
+    d = t.get_device()
+    if d < 0 or d != torch._C._cuda_getDevice():
+        raise ValueError("%s must be a tensor of the current CUDA device" % what)
+    return d
+
+
+def _i32(t, what, dev, n=None):
+    if t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous():
+        raise TypeError("%s must be a contiguous int32 tensor of the same CUDA device" % what)
     if n is not None and t.numel() != n:
         raise ValueError("%s must have %d entries" % (what, n))
     return t.data_ptr()
 
 
-def _tables(t, n):
+def _tables(t, n, dev):
     """Pointer, row stride and width of a block table for n requests."""
-    if t.dtype is not torch.int32 or t.dim() != 2 or not t.is_cuda:
-        raise ValueError("tables must be an int32 CUDA tensor [n_req, width]")
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.get_device() != dev:
+        raise ValueError("tables must be an int32 tensor [n_req, width] of the same CUDA device")
     rows, width = t.shape
     ld, one = t.stride()
     if rows != n or (one != 1 and width > 1 and rows):
@@ -68,7 +77,7 @@ class Kv4Cache:
             data = torch.zeros(need, dtype=torch.uint8, device=device or "cuda")
         if data.dtype != torch.uint8 or not data.is_cuda or not data.is_contiguous() or data.numel() < need:
             raise ValueError("data must be a contiguous uint8 CUDA tensor of %d bytes" % need)
-        self.data = data
+        self.data, self.dev = data, data.get_device()
         self.nonfinite = torch.zeros(1, dtype=torch.int32, device=data.device)
         self._nonfinite = self.nonfinite.data_ptr()
         self.desc = SgKv4(head_dim, n_kv_heads, page, n_blocks, data.data_ptr())
@@ -96,6 +105,7 @@ class Kv4Plan:
         self.ring = torch.arange(n_blocks, dtype=torch.int32, device=device)
         self._infos = [torch.tensor([0, n_blocks, 0, 0], dtype=torch.int32, device=device) for _ in range(2)]
         self._turn = 0
+        self.dev = self.ring.get_device()
         self._out = (self.cu.data_ptr(), self.seq.data_ptr(), self.pos.data_ptr(), self.slots.data_ptr())
 
     @property
@@ -112,7 +122,10 @@ def kv4_plan(plan, ctx, new, tables, ring=None, cursor=None, stream=None):
     n = ctx.numel()
     if n != plan.n_req:
         raise ValueError("the plan is made for %d requests" % plan.n_req)
-    table, ld, width = _tables(tables, n)
+    dev = _dev(tables, "tables")
+    if plan.dev != dev:
+        raise ValueError("the plan must lie on the same CUDA device")
+    table, ld, width = _tables(tables, n, dev)
     if (ring is None) != (cursor is None):
         raise ValueError("ring and cursor come together")
     own = cursor is None
@@ -123,8 +136,8 @@ def kv4_plan(plan, ctx, new, tables, ring=None, cursor=None, stream=None):
     turn = plan._turn ^ 1
     info = plan._infos[turn]
     cu, seq, pos, slots = plan._out
-    st = _lib.load().sg_kv4_plan(plan.page, plan.n_blocks, n, _i32(ctx, "ctx"), _i32(new, "new", n), table,
-                                 ld, width, _i32(ring, "ring"), _i32(cursor, "cursor"), cu, seq, pos,
+    st = _lib.load().sg_kv4_plan(plan.page, plan.n_blocks, n, _i32(ctx, "ctx", dev), _i32(new, "new", dev, n), table,
+                                 ld, width, _i32(ring, "ring", dev), _i32(cursor, "cursor", dev), cu, seq, pos,
                                  slots, plan.max_tokens, info.data_ptr(), _s(stream, tables))
     if st:
         _lib.check(st, "kv4_plan")
@@ -135,8 +148,9 @@ def kv4_plan(plan, ctx, new, tables, ring=None, cursor=None, stream=None):
 def _rows(cache, t, what):
     """Number, token and head stride of rows of the cache's heads."""
     shape, stride = t.shape, t.stride()
-    if len(shape) != 3 or shape[1] != cache.n_kv_heads or shape[2] != cache.head_dim or stride[2] != 1 or not t.is_cuda:
-        raise ValueError("%s must be a CUDA tensor [n_tok, %d, %d] with contiguous rows" % (what, cache.n_kv_heads, cache.head_dim))
+    if len(shape) != 3 or shape[1] != cache.n_kv_heads or shape[2] != cache.head_dim or stride[2] != 1 or t.get_device() != cache.dev:
+        raise ValueError("%s must be a tensor [n_tok, %d, %d] with contiguous rows on the cache's CUDA device" %
+                         (what, cache.n_kv_heads, cache.head_dim))
     return shape[0], stride[0], stride[1]
 
 
@@ -144,11 +158,12 @@ def kv4_append(cache, k, v, slots, stream=None):
     """Quantizes the rows k, v [n_tok, n_kv_heads, head_dim] (float32, float16 or
     bfloat16, any token and head strides) into their slots (int32 [n_tok], as
     kv4_plan makes them; negative: the row is left out)."""
+    dev = _dev(k, "k")
     n, kt, kh = _rows(cache, k, "k")
     nv, vt, vh = _rows(cache, v, "v")
     if v.dtype is not k.dtype or nv != n:
         raise ValueError("k and v must have one type and one number of rows")
-    st = _lib.load().sg_kv4_append(cache._c, _type(k, "k"), k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _i32(slots, "slots", n), n,
+    st = _lib.load().sg_kv4_append(cache._c, _type(k, "k"), k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _i32(slots, "slots", dev, n), n,
                                    cache._nonfinite, _s(stream, k))
     if st:
         _lib.check(st, "kv4_append")
@@ -157,7 +172,7 @@ def kv4_append(cache, k, v, slots, stream=None):
 def kv4_read(cache, slots, out=None, dtype=torch.float16, stream=None):
     """The values that the cache holds at the given slots (int32 [n_tok]): (k, v),
     [n_tok, n_kv_heads, head_dim] of dtype each, or into out = (k, v)."""
-    n = slots.numel()
+    n, dev = slots.numel(), _dev(slots, "slots")
     if out is None:
         with _on(stream):
             out = tuple(torch.empty(n, cache.n_kv_heads, cache.head_dim, dtype=dtype, device=slots.device)
@@ -166,7 +181,7 @@ def kv4_read(cache, slots, out=None, dtype=torch.float16, stream=None):
     if (_rows(cache, k, "out")[0] != n or _rows(cache, v, "out")[0] != n or v.dtype is not k.dtype or not k.is_contiguous() or
             not v.is_contiguous()):
         raise ValueError("out must be two contiguous tensors of one type with a row per slot")
-    st = _lib.load().sg_kv4_read(cache._c, _type(k, "out"), _i32(slots, "slots"), n, k.data_ptr(), v.data_ptr(), _s(stream, k))
+    st = _lib.load().sg_kv4_read(cache._c, _type(k, "out"), _i32(slots, "slots", dev), n, k.data_ptr(), v.data_ptr(), _s(stream, k))
     if st:
         _lib.check(st, "kv4_read")
     return out
@@ -177,6 +192,8 @@ def kv4_attention_scratch(device="cuda", stream=None):
     L = _lib.load()
     with _on(stream):
         t = torch.empty(L.sg_kv4_attention_scratch_bytes(), dtype=torch.uint8, device=device)
+    if not t.is_cuda:
+        raise ValueError("scratch must be CUDA memory")
     _lib.check(L.sg_kv4_attention_scratch_init(t.data_ptr(), t.numel(), _s(stream, t)), "kv4_attention_scratch_init")
     return t
 
@@ -191,21 +208,24 @@ def kv4_attention(cache, q, cu, seq, tables, scale=None, window=0, max_new=0, ou
     softmax's sum.  Returns out, [n_tok, n_heads, head_dim] of q's type."""
     n = seq.numel()
     shape, stride = q.shape, q.stride()
-    if len(shape) != 3 or shape[2] != cache.head_dim or stride[2] != 1 or not q.is_cuda:
-        raise ValueError("q must be a CUDA tensor [n_tok, n_heads, %d] with contiguous rows" % cache.head_dim)
-    table, ld, width = _tables(tables, n)
+    dev = _dev(q, "q")
+    if len(shape) != 3 or shape[2] != cache.head_dim or stride[2] != 1 or dev != cache.dev:
+        raise ValueError("q must be a tensor [n_tok, n_heads, %d] with contiguous rows on the cache's CUDA device" % cache.head_dim)
+    table, ld, width = _tables(tables, n, dev)
     if out is None:
         with _on(stream):
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
     ostride = out.stride()
-    if out.shape != shape or out.dtype is not q.dtype or ostride[2] != 1:
-        raise ValueError("out must have q's shape and type, and contiguous rows")
-    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != shape[:2] or not lse.is_contiguous()):
-        raise ValueError("lse must be a contiguous float32 [n_tok, n_heads]")
+    if out.shape != shape or out.dtype is not q.dtype or ostride[2] != 1 or out.get_device() != dev:
+        raise ValueError("out must have q's shape, type and device, and contiguous rows")
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != shape[:2] or not lse.is_contiguous() or lse.get_device() != dev):
+        raise ValueError("lse must be a contiguous float32 [n_tok, n_heads] on q's device")
     if scratch is None:
         scratch = kv4_attention_scratch(q.device, stream)
+    elif not scratch.is_contiguous() or scratch.get_device() != dev:
+        raise ValueError("scratch must be a contiguous tensor on q's device")
     a = SgKv4Attn(_type(q, "q"), shape[1], shape[0], n, q.data_ptr(), stride[0], stride[1], out.data_ptr(), ostride[0], ostride[1],
-                  None if lse is None else lse.data_ptr(), _i32(cu, "cu", n + 1), _i32(seq, "seq"), table, ld, width,
+                  None if lse is None else lse.data_ptr(), _i32(cu, "cu", dev, n + 1), _i32(seq, "seq", dev), table, ld, width,
                   0.0 if scale is None else scale, window, max_new, scratch.data_ptr(), scratch.numel())
     st = _lib.load().sg_kv4_attention(cache._c, C.byref(a), _s(stream, q))
     if st:
@@ -223,6 +243,7 @@ class LogProbs:
         self.rows, self.top = rows, top
         self.logprob, self.entropy, self.rank = f(rows), f(rows), i(rows)
         self.top_ids, self.top_logprobs = i(rows, top), f(rows, top)
+        self.dev = self.rank.get_device()
         self._p = [t.data_ptr() for t in (self.logprob, self.entropy, self.rank, self.top_ids, self.top_logprobs)]
 
 
@@ -233,17 +254,20 @@ def logprobs(logits, tokens=None, top=0, out=None, stream=None):
     given): the log probability and the rank (0: the likeliest) of each given
     token, the entropy in nats, and the `top` likeliest tokens."""
     shape, stride = logits.shape, logits.stride()
-    if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1) or not logits.is_cuda:
-        raise ValueError("logits must be a CUDA tensor [rows, vocab] with contiguous rows")
+    dev = _dev(logits, "logits")
+    if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
+        raise ValueError("logits must be a tensor [rows, vocab] with contiguous rows")
     rows, vocab = shape
     if out is None:
         with _on(stream):
             out = LogProbs(rows, top, logits.device)
     elif out.rows != rows or out.top != top:
         raise ValueError("out is made for %d rows and top %d" % (out.rows, out.top))
+    elif out.dev != dev:
+        raise ValueError("out must lie on the logits' device")
     lp, ent, rank, ids, tops = out._p
     st = _lib.load().sg_logprobs(_type(logits, "logits"), logits.data_ptr(), stride[0], rows, vocab,
-                                 None if tokens is None else _i32(tokens, "tokens", rows), lp, ent, rank, top, ids, tops,
+                                 None if tokens is None else _i32(tokens, "tokens", dev, rows), lp, ent, rank, top, ids, tops,
                                  _s(stream, logits))
     if st:
         _lib.check(st, "logprobs")
