@@ -276,7 +276,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
         if (m > sum.m + LAG) {
             const float d = (sum.m - m) * LOG2E, w = ex2(d);
             const float2 z = two_of(z2), zt = two_of(zt2);
-            zt2 = two_f32(z.x == 0.0f ? 0.0f : (zt.x + d * z.x) * w, z.y == 0.0f ? 0.0f : (zt.y + d * z.y) * w);
+            // (where w is 0, d and d z may be minus infinity: the first sum, or one over a mask's large finite numbers)
+            zt2 = two_f32(w == 0.0f ? 0.0f : (zt.x + d * z.x) * w, w == 0.0f ? 0.0f : (zt.y + d * z.y) * w);
             z2 = two_f32(z.x * w, z.y * w);
             sum.m = m;
         }

@@ -38,3 +38,31 @@ def test_fewer_allowed_than_alternatives(dev, dtype, rows, vocab):
     assert torch.equal(torch.isneginf(got.top_logprobs), ~fin)
     # distances up to 16 (half a unit in the last place each), a sum of at most 20 terms, its logarithm
     assert ((got.top_logprobs.double() - lp).abs()[fin] <= (16 + 8 * 16 + 20) * 2.0 ** -24).all()
+
+
+def finite_masks(dev, dtype, rows, vocab, mask, places):
+    """Rows of one large finite number but for a few likely tokens in given places; in 64 bits the masked ones
+    have probability 0.  Returns logits, tokens, and log probability, entropy and alternatives in 64 bits."""
+    x = torch.full((rows, vocab), mask, device=dev, dtype=dtype)
+    at = torch.tensor([(p + 37 * r) % vocab for r in range(rows) for p in places], device=dev).view(rows, -1)
+    x.scatter_(1, at, (torch.arange(len(places), device=dev) * 0.5 - 1).to(dtype).expand(rows, -1))
+    few = x.gather(1, at).double()
+    lp = few.log_softmax(1)
+    return x, at, lp, -(lp.exp() * lp).sum(1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(1, 151936), (65, 151936), (900, 70001)])
+@pytest.mark.parametrize("mask", ["lowest", -1e38, -1e37, -1e9])
+def test_large_finite_masks(dev, dtype, rows, vocab, mask):
+    # the allowed tokens come a thread's second turn or later: its sum moves from the mask's value to theirs
+    low = float(torch.finfo(dtype).min)
+    mask = low if mask == "lowest" else max(mask, low)
+    places = [vocab - 5, vocab - 70, vocab - 3000, vocab // 2 + 9000, vocab - 9001]
+    x, at, lp, ent = finite_masks(dev, dtype, rows, vocab, mask, places)
+    got = sg.logprobs(x, at[:, 2].int().contiguous(), top=5)
+    # values below 2 apart: a few units in the last place of 1 for distances, exponentials, five terms and the logarithm
+    tol = (16 + 8 * 2 + 5) * 2.0 ** -24
+    assert (got.entropy.double() - ent).abs().max() <= tol
+    assert (got.logprob.double() - lp[:, 2]).abs().max() <= tol
+    assert torch.equal(got.top_ids.long(), at.flip(1)) and (got.rank == 2).all()
