@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
         };
         if (m != m) z2 = two_f32(NAN, NAN);
         else if (m == -INFINITY) ;  // nothing to add
-        else if (sizeof(T) == 4 || !(least_of<T>(r) > -3e38f)) terms(true);
+        else if (sizeof(T) == 4 || !(least_of<T>(r) - sum.m > -1e38f)) terms(true);  // (t inside f32's range)
         else terms(false);
         if (m >= xt) {
             // the values before the given token count when equal, those after it do not

@@ -66,3 +66,29 @@ def test_large_finite_masks(dev, dtype, rows, vocab, mask):
     assert (got.entropy.double() - ent).abs().max() <= tol
     assert (got.logprob.double() - lp[:, 2]).abs().max() <= tol
     assert torch.equal(got.top_ids.long(), at.flip(1)) and (got.rank == 2).all()
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 151936), (65, 151936), (900, 70001)])
+@pytest.mark.parametrize("part", [0.7, 0.8])
+def test_large_finite_masks_below_bf16s_lowest(dev, rows, vocab, part):
+    # masks whose distance times log2 e is past f32's range, in a type that reads them sixteen values at a time
+    places = [vocab - 5, vocab - 70, vocab - 3000, vocab // 2 + 9000, vocab - 9001]
+    x, at, lp, ent = finite_masks(dev, torch.bfloat16, rows, vocab, part * torch.finfo(torch.bfloat16).min, places)
+    x[:, ::7] = x[0, 0] * 0.9                                    # more than one of them
+    x.scatter_(1, at, (torch.arange(5, device=dev) * 0.5 - 1).bfloat16().expand(rows, -1))
+    got = sg.logprobs(x, at[:, 2].int().contiguous(), top=5)
+    tol = (16 + 8 * 2 + 5) * 2.0 ** -24
+    assert (got.entropy.double() - ent).abs().max() <= tol
+    assert (got.logprob.double() - lp[:, 2]).abs().max() <= tol
+    assert torch.equal(got.top_ids.long(), at.flip(1)) and (got.rank == 2).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_huge_logit_after_ordinary_ones(dev, dtype):
+    vocab = 151936
+    g = torch.Generator(device=dev).manual_seed(7)
+    x = torch.randn(3, vocab, device=dev, generator=g).to(dtype)
+    for r, at in enumerate((vocab - 9, vocab // 2, 100000)):
+        x[r, at] = torch.finfo(dtype).max
+    got = sg.logprobs(x, torch.tensor([vocab - 9, vocab // 2, 100000], dtype=torch.int32, device=dev), top=1)
+    assert (got.entropy == 0).all() and (got.logprob == 0).all() and (got.rank == 0).all()
