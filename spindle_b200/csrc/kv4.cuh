@@ -67,6 +67,12 @@ struct Kv4Codes {
     }
 };
 
+// A result in f16.  It is a mean of values that are finite in f16, so its true value is, but the weights' sum is 1 only up
+// to their rounding (2^-12 of it in the kernel for many rows): what that carries past the end of the range stays there.
+__device__ __forceinline__ __half kv4_f16(float v) {
+    return __float2half_rn(fabsf(v) > 65504.0f ? copysignf(65504.0f, v) : v);
+}
+
 struct Kv4Cache {
     uint8_t *data;
     uint32_t n_blocks, page_shift;  // page = 1 << page_shift positions

@@ -55,7 +55,7 @@ struct Act<float> {
 template <>
 struct Act<__half> {
     static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
-    static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ __half put(float v) { return kv4_f16(v); }
 };
 template <>
 struct Act<__nv_bfloat16> {

@@ -136,7 +136,7 @@ __device__ __forceinline__ float to_f32(T v) {
 }
 template <typename T>
 __device__ __forceinline__ T from_f32(float v) {
-    if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
+    if constexpr (std::is_same<T, __half>::value) return kv4_f16(v);
     else return __float2bfloat16_rn(v);
 }
 

@@ -61,3 +61,21 @@ def test_tensors_of_another_device_are_refused(dev):
         with pytest.raises((ValueError, TypeError)):
             sg.logprobs(*args, out=out)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("heads,group,new", [(2, 4, 3), (2, 4, 300), (4, 8, 900)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_means_of_f16s_largest_number(dev, d, heads, group, new):
+    # V equal to +-65504 in some groups: a mean of it is that number, whatever the weights' rounding (which shows most
+    # where one position that comes late has nearly all the weight, hence the scale)
+    page, length, scale = 16, 1000, 4 * d ** -0.5
+    cache = sg.Kv4Cache(63, heads, d, page, device=dev)
+    g = torch.Generator(device=dev).manual_seed(new)
+    k, v = (torch.randn(length, heads, d, device=dev, generator=g) for _ in range(2))
+    v[..., :32], v[..., 32:64] = 65504.0, -65504.0
+    sg.kv4_append(cache, k, v, torch.arange(length, dtype=torch.int32, device=dev))
+    tables = torch.arange(63, dtype=torch.int32, device=dev)[None]
+    for dtype in TYPES:
+        q = torch.randn(new, heads * group, d, device=dev, generator=g).to(dtype)
+        out = sg.kv4_attention(cache, q, ints([0, new], dev), ints([length], dev), tables, scale=scale)
+        check(dev, cache, tables, tables.cpu(), ints([0, new], dev), ints([length], dev), q, scale, 0, out, None)
