@@ -553,7 +553,8 @@ SG_API sg_status sg_pipe_recv(float *d_dst, uint64_t n, uint64_t n_max, void *d_
  * position p of a request whose block table says block b for p / page lies in
  * slot b * page + p % page.  K and V rows of n_kv_heads x head_dim (64, 128 or
  * 256) values are held in groups of 32 along head_dim as m + s * c: c of 4 bits,
- * m = f16(min), s = f16((max - m) / 15), 20 bytes per group.  data:
+ * m = f16(min), s = f16((max - m) / 15) (the next smaller f16 where m + 15 s would
+ * be infinite in f16), 20 bytes per group.  data:
  * sg_kv4_bytes(c) device bytes, 16-byte aligned; one sg_kv4 per layer. */
 typedef struct {
     uint32_t head_dim, n_kv_heads, page, n_blocks;
@@ -590,7 +591,7 @@ SG_API sg_status sg_kv4_plan(uint32_t page, uint32_t n_blocks, uint64_t n_req, c
  * row is left out; no two rows may have the same slot).  type SG_F32, SG_F16 or
  * SG_BF16; element (t, h, d) of K at d_k[t * k_tok + h * k_head + d], V likewise.
  * Values are clamped to f16's finite range and NaN counts as 0, so that the cache
- * holds finite numbers only; d_nonfinite (optional) counts the groups that had an
+ * holds numbers that are finite in f16 only; d_nonfinite (optional) counts the groups that had an
  * infinity or a NaN.  sg_kv4_read gives back the values of given slots as
  * [n_tok][n_kv_heads][head_dim] of `type`, 16-byte aligned, zeros for no slot. */
 SG_API sg_status sg_kv4_append(const sg_kv4 *c, int32_t type, const void *d_k, uint64_t k_tok, uint64_t k_head,

@@ -177,8 +177,9 @@ __global__ void __launch_bounds__(KV4_PLAN_THREADS) kv4_plan_kernel(const __grid
 // Two lanes per group of 32 values, sixteen values each: lane i's are the K words
 // j = 2 i and 2 i + 1 of the group, and its V half words 4 i .. 4 i + 3.
 //   m = f16(min), s = f16((max - m) * f32(1/15)), c = rint(clamp((x - m) * (1 / s), 0, 15))
-// with x clamped to f16's finite range and NaN counted as 0, so that the cache
-// holds finite numbers only; groups that had such a value are counted.  Every
+// with x clamped to f16's finite range, NaN counted as 0, and s the next smaller
+// f16 where m + 15 s >= 65520, which is infinity in f16, so that the cache holds
+// finite numbers only; groups that had an infinity or a NaN are counted.  Every
 // step is one rounded f32 operation, so the codes can be reproduced bit for bit.
 // What bounds it is the arithmetic (19 instructions a value by the counters), hence sixteen
 // values a lane: the place of a row in the cache is worked out half as often.
@@ -254,7 +255,9 @@ __global__ void __launch_bounds__(KV4_ROW_THREADS) kv4_append_kernel(const __gri
         hi = fminf(fmaxf(hi, -65504.0f), 65504.0f);
         const __half mh = __float2half_rn(lo + 0.0f);  // + 0: no negative zero
         const float m = __half2float(mh);
-        const __half sh = __float2half_rn(__fmul_rn(fmaxf(hi - m, 0.0f), 1.0f / 15.0f));
+        __half sh = __float2half_rn(__fmul_rn(fmaxf(hi - m, 0.0f), 1.0f / 15.0f));
+        // a step that was rounded up so far that the largest value would be infinite in f16: the next smaller one
+        if (fmaf(15.0f, __half2float(sh), m) >= 65520.0f) sh = __ushort_as_half(__half_as_ushort(sh) - 1);
         const float s = __half2float(sh), r = s > 0.0f ? __frcp_rn(s) : 0.0f;
         uint32_t word[2] = {0, 0};
 #pragma unroll

@@ -79,3 +79,82 @@ def test_attention_means_of_f16s_largest_number(dev, d, heads, group, new):
         q = torch.randn(new, heads * group, d, device=dev, generator=g).to(dtype)
         out = sg.kv4_attention(cache, q, ints([0, new], dev), ints([length], dev), tables, scale=scale)
         check(dev, cache, tables, tables.cpu(), ints([0, new], dev), ints([length], dev), q, scale, 0, out, None)
+
+
+def finite_quantized(x):
+    """kv4_util.quantized with the step that keeps a group's largest value finite in f16: one f16 step
+    less where m + 15 s, in f32, is 65520 or more."""
+    x = torch.nan_to_num(x.float(), nan=0.0, posinf=U.F16_MAX, neginf=-U.F16_MAX).clamp(-U.F16_MAX, U.F16_MAX)
+    g = x.unflatten(-1, (x.shape[-1] // 32, 32))
+    m = g.amin(-1, keepdim=True).half().float()
+    s = ((g.amax(-1, keepdim=True) - m).clamp(min=0) * torch.tensor(1.0 / 15.0)).half()
+    less = (s.view(torch.int16) - 1).view(torch.float16)
+    s = torch.where(m.double() + 15 * s.double() >= 65520.0 - 2.0 ** -9, less, s).float()
+    r = torch.where(s > 0, torch.tensor(1.0) / s, torch.zeros(()))
+    c = torch.round(((g - m) * r).clamp(0, 15))
+    return (m.double() + s.double() * c.double()).flatten(-2)
+
+
+def full_range(n, heads, d, dtype, seed):
+    """Rows whose groups reach f16's ends: from 0 or a little above to infinity, from one infinity to the other, and ordinary ones."""
+    g = torch.Generator().manual_seed(seed)
+    inf = float("inf")
+    x = torch.randn(n, heads, d, generator=g)
+    x[0, 0, :32] = x[0, 0, :32].abs()
+    x[0, 0, 3] = inf                     # 0.. to the largest
+    x[1, 0, :32], x[1, 0, 9] = 0.0, 65504.0
+    x[2, 0, :32] = 14.0
+    x[2, 0, 31] = inf
+    x[3, 0, 32:64] = x[3, 0, 32:64] * 100
+    x[3, 0, 40], x[3, 0, 41] = inf, -inf
+    x[4, 0, 5], x[4, 0, 6] = -inf, 60000.0
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,heads,page", [(64, 1, 16), (128, 2, 32), (256, 1, 64)])
+def test_append_holds_what_is_finite_in_f16(dev, dtype, d, heads, page):
+    n = 40
+    x = full_range(n, heads, d, dtype, d)
+    cache = sg.Kv4Cache(64 // page + 2, heads, d, page, device=dev)
+    slots = torch.arange(n, dtype=torch.int32, device=dev)
+    sg.kv4_append(cache, x.to(dev), x.to(dev), slots)
+    want = finite_quantized(x.float())
+    for out_type in TYPES:
+        for t in sg.kv4_read(cache, slots, dtype=out_type):
+            assert torch.isfinite(t).all()
+            assert torch.equal(t.cpu(), want.float().to(out_type))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group,new", [(2, 3), (8, 300), (8, 1500)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_over_the_whole_range_of_f16(dev, dtype, group, new, d):
+    # a few positions with such rows among ordinary ones: finite results, right against 64 bits, and the rows that do not
+    # see those positions have the bits that they have without them
+    heads, page, length = 2, 16, 1600
+    cache, ref = (sg.Kv4Cache(length // page, heads, d, page, device=dev) for _ in range(2))
+    slots = torch.arange(length, dtype=torch.int32, device=dev)
+    g = torch.Generator(device=dev).manual_seed(5)
+    k = torch.randn(length, heads, d, device=dev, generator=g)
+    v = torch.randn(length, heads, d, device=dev, generator=g)
+    sg.kv4_append(ref, k, v, slots)
+    at = length - 10
+    k[at:at + 5, :1] = full_range(5, 1, d, torch.float32, 1).to(dev)
+    v[at:at + 5, :1] = full_range(5, 1, d, torch.float32, 2).to(dev)
+    sg.kv4_append(cache, k, v, slots)
+    tables = torch.arange(length // page, dtype=torch.int32, device=dev)[None]
+    q = torch.randn(new, heads * group, d, device=dev, generator=g).to(dtype)
+    cu, seq = ints([0, new], dev), ints([length], dev)
+    out = sg.kv4_attention(cache, q, cu, seq, tables)
+    check(dev, cache, tables, tables.cpu(), cu, seq, q, d ** -0.5, 0, out, None)
+    want = sg.kv4_attention(ref, q, cu, seq, tables)
+    before = torch.arange(length - new, length, device=dev) < at
+    assert torch.equal(out[:, group:], want[:, group:])
+    if before.any() and dtype != torch.float32:
+        assert torch.equal(out[before], want[before])
+    elif before.any():
+        # f32 holds the sums of a group at a power of two for its largest scale, 2^14 times the ordinary ones here: a
+        # position's weight times value is off by up to 8 * 2^-25 * 2^6 of the largest weight, 1600 of them over a sum
+        # of weights that is at least 25 for these scores
+        assert (out[before] - want[before]).abs().max() <= 1600 * 8 * 2.0 ** -19 / 25
