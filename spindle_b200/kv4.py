@@ -95,30 +95,31 @@ class Kv4Plan:
     """What kv4_plan writes, for up to n_req requests and max_tokens new
     positions a step: cu [n_req + 1], seq [n_req], pos and slots [max_tokens],
     and info [4] (the next step's cursor, the sum of the new positions, the
-    blocks that were wanted and not there).  It also keeps a ring of all blocks,
-    free to begin with, and the cursor, for callers without their own."""
+    blocks that were wanted and not there; of the last call).  It also keeps a ring
+    of all blocks, free to begin with, and the cursor, for callers without their own."""
 
     def __init__(self, n_req, max_tokens, page, n_blocks, device="cuda"):
         new = lambda n: torch.empty(n, dtype=torch.int32, device=device)  # noqa: E731
         self.n_req, self.max_tokens, self.page, self.n_blocks = n_req, max_tokens, page, n_blocks
         self.cu, self.seq, self.pos, self.slots = new(n_req + 1), new(n_req), new(max_tokens), new(max_tokens)
         self.ring = torch.arange(n_blocks, dtype=torch.int32, device=device)
-        self._infos = [torch.tensor([0, n_blocks, 0, 0], dtype=torch.int32, device=device) for _ in range(2)]
-        self._turn = 0
+        # two a kind, as a call reads a cursor and writes the next: of the own ring, and of rings that are given
+        infos = torch.tensor([[0, n_blocks, 0, 0]] * 4, dtype=torch.int32, device=device).unbind()
+        self._infos, self._given = infos[:2], infos[2:]
+        self._turn = self._given_turn = 0
+        self._captured = False  # a graph holds the own ring's cursor: it stays where it is
+        self.info = self._infos[0]
         self.dev = self.ring.get_device()
         self._out = (self.cu.data_ptr(), self.seq.data_ptr(), self.pos.data_ptr(), self.slots.data_ptr())
-
-    @property
-    def info(self):
-        return self._infos[self._turn]
 
 
 def kv4_plan(plan, ctx, new, tables, ring=None, cursor=None, stream=None):
     """Block tables and slot maps of one step (sg_kv4_plan): ctx and new int32
     [n_req] (positions held, positions to come; new < 0: the request ends), tables
     int32 [n_req, width], updated in place.  ring and cursor: the free blocks
-    (int32 [n_blocks] and [2 or more]); None: the plan's own, carried from call to
-    call.  Fills and returns plan."""
+    (int32 [n_blocks] and [2 or more]; info[:2] is the next call's cursor); None: the
+    plan's own, carried from call to call, replays of captured calls among them.
+    Fills and returns plan."""
     n = ctx.numel()
     if n != plan.n_req:
         raise ValueError("the plan is made for %d requests" % plan.n_req)
@@ -130,18 +131,34 @@ def kv4_plan(plan, ctx, new, tables, ring=None, cursor=None, stream=None):
         raise ValueError("ring and cursor come together")
     own = cursor is None
     if own:
-        ring, cursor = plan.ring, plan.info
+        turn = plan._turn ^ 1
+        ring, cursor, info = plan.ring, plan._infos[plan._turn], plan._infos[turn]
     elif ring.numel() != plan.n_blocks or cursor.numel() < 2:
         raise ValueError("ring must have n_blocks entries and cursor two")
-    turn = plan._turn ^ 1
-    info = plan._infos[turn]
+    else:
+        turn = plan._given_turn ^ 1
+        if plan._given[turn].data_ptr() == cursor.data_ptr():
+            turn ^= 1
+        info = plan._given[turn]
     cu, seq, pos, slots = plan._out
     st = _lib.load().sg_kv4_plan(plan.page, plan.n_blocks, n, _i32(ctx, "ctx", dev), _i32(new, "new", dev, n), table,
                                  ld, width, _i32(ring, "ring", dev), _i32(cursor, "cursor", dev), cu, seq, pos,
                                  slots, plan.max_tokens, info.data_ptr(), _s(stream, tables))
     if st:
         _lib.check(st, "kv4_plan")
-    plan._turn = turn
+    if not own:
+        plan._given_turn = turn
+    else:
+        with _on(stream):
+            if plan._captured or torch.cuda.is_current_stream_capturing():
+                # a replay reads the cursor where the captured call did: the next one goes there, from now on for
+                # the calls outside the graph too
+                cursor = plan._infos[plan._turn]
+                cursor.copy_(info)
+                plan._captured, info = True, cursor
+            else:
+                plan._turn = turn
+    plan.info = info
     return plan
 
 

@@ -158,3 +158,51 @@ def test_attention_over_the_whole_range_of_f16(dev, dtype, group, new, d):
         # position's weight times value is off by up to 8 * 2^-25 * 2^6 of the largest weight, 1600 of them over a sum
         # of weights that is at least 25 for these scores
         assert (out[before] - want[before]).abs().max() <= 1600 * 8 * 2.0 ** -19 / 25
+
+
+def test_plan_captured_with_its_own_ring(dev):
+    # a captured plan on the plan's own ring goes on from replay to replay, over page ends, and calls outside the graph go on from there
+    n, page, n_blocks, width = 3, 16, 40, 12
+    plan = sg.Kv4Plan(n, 8, page, n_blocks, device=dev)
+    tables = torch.full((n, width), -1, dtype=torch.int32, device=dev)
+    ctx, new = ints([0] * n, dev), ints([1, 2, 0], dev)
+    side = torch.cuda.Stream()
+    want_t, ring, head, tail = [[-1] * width for _ in range(n)], list(range(n_blocks)), 0, n_blocks
+    lens, graph = [0] * n, None
+    for t in range(70):
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            if t == 3:
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=side):
+                    sg.kv4_plan(plan, ctx, new, tables)
+            if graph is None or t % 10 == 9:
+                sg.kv4_plan(plan, ctx, new, tables)
+            else:
+                graph.replay()
+        torch.cuda.synchronize()
+        want = U.plan(lens, [1, 2, 0], want_t, ring, head, tail, page, n_blocks, 8)
+        assert [x.tolist() for x in (plan.cu, plan.seq, plan.pos, plan.slots, plan.info)] == [list(x) for x in want], t
+        assert tables.tolist() == want_t and plan.ring.tolist() == ring, t
+        head, tail = want[4][:2]
+        lens = want[1]
+        ctx.copy_(plan.seq)
+    del graph
+
+
+def test_plan_own_and_given_rings_apart(dev):
+    # calls with a ring and cursor of the caller leave the plan's own ones as they are, and infos feed the next call
+    plan = sg.Kv4Plan(1, 40, 16, 6, device=dev)
+    tables = [torch.full((1, 8), -1, dtype=torch.int32, device=dev) for _ in range(2)]
+    ring, cursor = torch.arange(6, dtype=torch.int32, device=dev).flip(0).contiguous(), ints([2, 8], dev)
+    want_t, want_r, at = [[[-1] * 8], [[-1] * 8]], [list(range(6)), ring.tolist()], [(0, 6), (2, 8)]
+    for step, (own, ctx) in enumerate([(True, 0), (False, 0), (False, 20), (True, 20), (False, 40), (True, 40)]):
+        k = 0 if own else 1
+        got = sg.kv4_plan(plan, ints([ctx], dev), ints([20], dev), tables[k], *(() if own else (ring, cursor)))
+        want = U.plan([ctx], [20], want_t[k], want_r[k], *at[k], 16, 6, 40)
+        assert got.info.tolist() == list(want[4]) and tables[k].tolist() == want_t[k], step
+        at[k] = want[4][:2]
+        if not own:
+            cursor = got.info                              # the tensor itself, or a copy of it
+            if step == 1:
+                cursor = cursor[:2].clone()
