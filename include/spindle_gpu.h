@@ -579,7 +579,9 @@ SG_API uint64_t sg_kv4_bytes(const sg_kv4 *c);
  *   d_pos, d_slots [max_tokens]: each new position's place in its request and
  *     its slot, -1 where it has none; past the last new position both are -1;
  *   d_info [4]: the next step's cursor (2), the sum of new, and the number of
- *     blocks that were wanted and not there.  d_info must not be d_cursor.
+ *     blocks that were wanted and not there.
+ * Nothing that is written may overlap d_ctx, d_new or d_cursor, but d_seq may be
+ * d_ctx, to carry the lengths on in place.
  * max_tokens at least the sum of the positive d_new.  Calling it again with the
  * same cursor writes the same. */
 SG_API sg_status sg_kv4_plan(uint32_t page, uint32_t n_blocks, uint64_t n_req, const int32_t *d_ctx, const int32_t *d_new,

@@ -2403,6 +2403,9 @@ namespace {
 
 bool page_ok(uint32_t page) { return page >= 16 && page <= 1024 && (page & (page - 1)) == 0; }
 uint32_t log2_of(uint32_t v) { return 31u - (uint32_t)__builtin_clz(v); }
+bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
+    return na && nb && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
 // element size of an activation type, 0: not one
 uint32_t act_bytes(int32_t type) { return type == SG_F32 ? 4 : type == SG_F16 || type == SG_BF16 ? 2 : 0; }
 
@@ -2437,15 +2440,31 @@ sg_status sg_kv4_plan(uint32_t page, uint32_t n_blocks, uint64_t n_req, const in
         return SG_ERR_INVALID;
     if (n_req >= 1ull << 31 || max_tokens >= 1ull << 31 || width >= 1ull << 31 || (n_req > 1 && ld_tables < width))
         return SG_ERR_INVALID;
+    // Every CTA reads the lengths and the cursor while others write: nothing written may lie there, but for the new lengths
+    // in the place of the old ones.
+    const bool in_place = d_seq == d_ctx && n_req;
+    const struct { const void *p; uint64_t n; } in[3] = {{d_ctx, n_req * 4}, {d_new, n_req * 4}, {d_cursor, 8}},
+        out[7] = {{d_cu, n_req * 4 + 4}, {d_seq, n_req * 4}, {d_pos, max_tokens * 4}, {d_slots, max_tokens * 4}, {d_info, 16},
+                  {d_ring, (uint64_t)n_blocks * 4}, {d_tables, n_req && width ? ((n_req - 1) * ld_tables + width) * 4 : 0}};
+    for (int i = 0; i < 3; i++)
+        for (int o = 0; o < 7; o++)
+            if (overlap(in[i].p, in[i].n, out[o].p, out[o].n) && !(in_place && i == 0 && o == 1)) return SG_ERR_INVALID;
     DevInfo *di;
     if (sg_status st = dev_info(&di)) return st;
-    const Kv4PlanArgs a = {d_ctx, d_new, d_tables, ld_tables, d_ring, d_cursor, d_cu, d_seq, d_pos, d_slots, d_info,
-                           (uint32_t)n_req, (uint32_t)max_tokens, (uint32_t)width, log2_of(page), n_blocks,
-                           aligned(d_pos, 16) && aligned(d_slots, 16)};
+    Kv4PlanArgs a = {d_ctx, d_new, d_tables, ld_tables, d_ring, d_cursor, d_cu, d_seq, d_pos, d_slots, d_info,
+                     (uint32_t)n_req, (uint32_t)max_tokens, (uint32_t)width, log2_of(page), n_blocks,
+                     aligned(d_pos, 16) && aligned(d_slots, 16), true};
     const uint64_t want = (max_tokens + KV4_PLAN_THREADS - 1) / KV4_PLAN_THREADS;
     const uint32_t grid = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(want, di->sms));
+    // lengths in place with several CTAs: first the positions, then, in one CTA, the lengths
+    a.lengths = !in_place || grid == 1;
     kv4_plan_kernel<<<grid, KV4_PLAN_THREADS, 0, (cudaStream_t)stream>>>(a);
     CK(cudaGetLastError());
+    if (!a.lengths) {
+        a.lengths = true, a.max_tok = 0;
+        kv4_plan_kernel<<<1, KV4_PLAN_THREADS, 0, (cudaStream_t)stream>>>(a);
+        CK(cudaGetLastError());
+    }
     return SG_OK;
 }
 

@@ -48,6 +48,7 @@ __device__ __forceinline__ uint32_t warp_scan(uint32_t v, uint32_t lane) {
 // position writes the table entry, and everyone else computes the block from the
 // ring without reading it back.  A decode step of 64 requests is a launch (5 us); 1.5 million positions of 509
 // requests 13 to 14 us, 1 TB/s of positions and slots, bound by the searches and the scan that every CTA repeats.
+// Where the new lengths take the place of the old ones, which every CTA reads, a second launch of one CTA writes them.
 __global__ void __launch_bounds__(KV4_PLAN_THREADS) kv4_plan_kernel(const __grid_constant__ Kv4PlanArgs a) {
     __shared__ uint32_t cu_s[KV4_PLAN_THREADS + 1], want_s[KV4_PLAN_THREADS];
     __shared__ int32_t ctx_s[KV4_PLAN_THREADS];
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(KV4_PLAN_THREADS) kv4_plan_kernel(const __grid
         ctx_s[tid] = (int32_t)ctx;
         const uint32_t back_at = base_back + warp_s[2][wid] + s2 - back;
         if (tid == 0) cu_s[KV4_PLAN_THREADS] = base_come + total_s[0];
-        if (blockIdx.x == 0 && r < a.n_req) {
+        if (blockIdx.x == 0 && r < a.n_req && a.lengths) {
             a.cu[r] = (int32_t)c0;
             a.seq[r] = ends ? 0 : (int32_t)(ctx + come);
         }
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(KV4_PLAN_THREADS) kv4_plan_kernel(const __grid
         __syncthreads();
     }
     for (uint32_t t = max(t0, min(base_come, t1)) + tid; t < t1; t += KV4_PLAN_THREADS) a.pos[t] = a.slots[t] = -1;
-    if (blockIdx.x == 0 && tid == 0) {
+    if (blockIdx.x == 0 && tid == 0 && a.lengths) {
         const uint32_t taken = min(base_want, free_blocks);
         a.cu[a.n_req] = (int32_t)base_come;
         const uint32_t turn = (head + taken) / a.n_blocks * a.n_blocks;  // the head stays inside the ring

@@ -88,6 +88,7 @@ struct Kv4PlanArgs {
     int32_t *cu, *seq, *pos, *slots, *info;
     uint32_t n_req, max_tok, width, page_shift, n_blocks;
     bool vec;  // pos and slots allow 16-byte stores
+    bool lengths;  // this launch writes cu, seq and info
 };
 
 struct Kv4RowArgs {

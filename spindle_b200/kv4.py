@@ -115,7 +115,8 @@ class Kv4Plan:
 
 def kv4_plan(plan, ctx, new, tables, ring=None, cursor=None, stream=None):
     """Block tables and slot maps of one step (sg_kv4_plan): ctx and new int32
-    [n_req] (positions held, positions to come; new < 0: the request ends), tables
+    [n_req] (positions held, positions to come; new < 0: the request ends; ctx may
+    be plan.seq, to carry the lengths on in place), tables
     int32 [n_req, width], updated in place.  ring and cursor: the free blocks
     (int32 [n_blocks] and [2 or more]; info[:2] is the next call's cursor); None: the
     plan's own, carried from call to call, replays of captured calls among them.

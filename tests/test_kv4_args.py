@@ -42,3 +42,23 @@ def test_a_gpu_that_is_not_the_current_one(monkeypatch):
         kv4._i32(on(1, 3, dtype=torch.int32), "x", 0)
     with pytest.raises(ValueError):
         kv4._tables(on(1, 2, 2, dtype=torch.int32), 2, 0)
+
+
+def test_plan_refuses_overlapping_memory():
+    # what a plan writes must not lie where it reads (addresses only: refused before a launch)
+    import ctypes as C
+
+    from spindle_b200 import _lib
+    L = _lib.load()
+    p = lambda k: C.c_void_p(0x100000 + k)  # noqa: E731
+    at = dict(ctx=0x1000, new=0x2000, tables=0x3000, ring=0x4000, cursor=0x5000, cu=0x6000, seq=0x7000, pos=0x8000, slots=0x9000, info=0xa000)
+
+    def plan(**kw):
+        a = {k: p(v) for k, v in dict(at, **kw).items()}
+        return L.sg_kv4_plan(64, 8, 10, a["ctx"], a["new"], a["tables"], 4, 4, a["ring"], a["cursor"], a["cu"], a["seq"], a["pos"],
+                             a["slots"], 10, a["info"], None)
+    sizes = dict(cu=44, seq=40, pos=40, slots=40, info=16, ring=32, tables=160)
+    for read, n in (("ctx", 40), ("new", 40), ("cursor", 8)):
+        for out, m in sizes.items():
+            assert plan(**{out: at[read] + n - 4}) == 1, (read, out)
+            assert plan(**{out: at[read] - m + 4}) == 1, (read, out)

@@ -1,4 +1,6 @@
 """The paged 4-bit KV cache on the GPU at the edges of what its entry points take."""
+import random
+
 import pytest
 import torch
 
@@ -206,3 +208,42 @@ def test_plan_own_and_given_rings_apart(dev):
             cursor = got.info                              # the tensor itself, or a copy of it
             if step == 1:
                 cursor = cursor[:2].clone()
+
+
+@pytest.mark.parametrize("n_req,most,page,n_blocks", [(3, 9, 16, 40), (5, 5000, 1024, 64), (1500, 40, 16, 20000), (64, 300, 64, 2000)])
+def test_plan_lengths_in_place(dev, n_req, most, page, n_blocks):
+    # plan.seq as the next call's lengths: steps of one CTA and of many
+    rng = random.Random(n_req)
+    width = (4 * most + page - 1) // page + 3
+    cap = n_req * most + 5
+    plan = sg.Kv4Plan(n_req, cap, page, n_blocks, device=dev)
+    plan.seq.zero_()
+    tables = torch.full((n_req, width), -1, dtype=torch.int32, device=dev)
+    want_t, ring, at, ctx = [[-1] * width for _ in range(n_req)], list(range(n_blocks)), (0, n_blocks), [0] * n_req
+    for step in range(4):
+        new = [-1 if step and rng.random() < 0.2 else rng.choice([0, 1, most]) for _ in range(n_req)]
+        sg.kv4_plan(plan, plan.seq, ints(new, dev), tables)
+        want = U.plan(ctx, new, want_t, ring, *at, page, n_blocks, cap)
+        for a, b in zip((plan.cu, plan.seq, plan.pos, plan.slots, plan.info), want):
+            assert a.tolist() == list(b)
+        assert tables.tolist() == want_t and plan.ring.tolist() == ring
+        at, ctx = want[4][:2], want[1]
+
+
+def test_plan_refuses_what_it_would_overwrite(dev):
+    plan = sg.Kv4Plan(2, 4, 16, 4, device=dev)
+    z, t = ints([0, 0], dev), torch.full((2, 2), -1, dtype=torch.int32, device=dev)
+    for ctx, new in ((plan.cu[:2], z), (plan.cu[1:], z), (z, plan.seq), (plan.pos[2:], z), (z, plan.slots[:2]), (plan.ring[1:3], z),
+                     (t[0], z), (z, t[1])):
+        with pytest.raises(sg.SgError):
+            sg.kv4_plan(plan, ctx, new, t)
+    for cursor in (plan.cu, plan.seq, plan.pos, plan.ring):
+        with pytest.raises(sg.SgError):
+            sg.kv4_plan(plan, z, z, t, plan.ring, cursor)
+    sg.kv4_plan(plan, z, z, t)
+    # side by side in one buffer is fine
+    buf = torch.zeros(16, dtype=torch.int32, device=dev)
+    buf[4:6] = ints([0, 4], dev)
+    plan.ring = torch.arange(4, dtype=torch.int32, device=dev)
+    sg.kv4_plan(plan, buf[0:2], buf[2:4], buf[12:16].view(2, 2), plan.ring, buf[4:6])
+    assert plan.seq.tolist() == [0, 0]
