@@ -33,7 +33,11 @@
 // made in f16, one rounding each.  For f32
 //   sum_t p_t v_t = sum_t (p_t s_tg) (c_t - 8) + sum_t p_t (m_tg + 8 s_tg)
 // with p s and m + 8 s in two f16 parts again: around the middle of the codes the
-// long sums stay small, so that nothing of them cancels.
+// long sums stay small, so that nothing of them cancels.  The tensor cores cut off
+// what does not fit a sum's f32, always towards zero, which over a long stretch of
+// small weights after a large one adds up to more than f32 has to lose (4.6e-5 after 4096 positions, 3.1e-6
+// now): so f32 sums the products of 16 positions apart and adds them by rounded f32 additions
+// (16 requests of 9 tokens: 36.7 -> 38.5 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -120,6 +124,15 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// c += d, rounded to nearest, two numbers an instruction.
+__device__ __forceinline__ void add4(float (&c)[4], const float (&d)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; k += 2)
+        asm("{\n .reg .b64 x, y;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %3};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+            : "+f"(c[k]), "+f"(c[k + 1])
+            : "f"(d[k]), "f"(d[k + 1]));
 }
 
 // An 8 x 8 matrix of 16-bit numbers, a row per four lanes, transposed.
@@ -686,6 +699,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
         }
 
         // values
+        float ls[2];  // the step's weights: one rounding of the long sums a step
 #pragma unroll
         for (int i = 0; i < TILES; i++) {
             const uint8_t *tile = buf + i * L::BYTES;
@@ -694,7 +708,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const float p0 = ex2(fmaf(s[i][2 * j], cs[0], sh[0])), p1 = ex2(fmaf(s[i][2 * j + 1], cs[1], sh[1]));
-                l[0] += p0, l[1] += p1;
+                ls[0] = i + j ? ls[0] + p0 : p0, ls[1] = i + j ? ls[1] + p1 : p1;
                 ph[j] = pack_h2(p0, p1);
                 if constexpr (REST) {
                     const float2 h = unpack_h2(ph[j]);
@@ -721,8 +735,10 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
                     const uint32_t yy = sub_h2(mid[j], x);
                     rest[j] = add_h2(sub_h2(x, sub_h2(mid[j], yy)), sub_h2(y, yy));  // exactly x + y - mid
                 }
-                mma16(om, mid[0], rest[0], mid[1], rest[1], ph[0], ph[1]);
-                mma16(om, mid[0], rest[0], mid[1], rest[1], pl[0], pl[1]);
+                float d[4];
+                mma16_first(d, mid[0], rest[0], mid[1], rest[1], ph[0], ph[1]);
+                mma16(d, mid[0], rest[0], mid[1], rest[1], pl[0], pl[1]);
+                add4(om, d);
             }
 #pragma unroll
             for (int g = 0; g < G; g++) {
@@ -746,12 +762,24 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
                     bh[0] = ph[0], bh[1] = ph[1];
                     if constexpr (REST) bl[0] = pl[0], bl[1] = pl[1];
                 }
-                mma16(o[2 * g], c0[0], c0[1], c1[0], c1[1], bh[0], bh[1]);
-                if constexpr (REST) mma16(o[2 * g], c0[0], c0[1], c1[0], c1[1], bl[0], bl[1]);
-                mma16(o[2 * g + 1], c0[2], c0[3], c1[2], c1[3], bh[0], bh[1]);
-                if constexpr (REST) mma16(o[2 * g + 1], c0[2], c0[3], c1[2], c1[3], bl[0], bl[1]);
+                if constexpr (Q32) {
+                    float d[4];
+                    mma16_first(d, c0[0], c0[1], c1[0], c1[1], bh[0], bh[1]);
+                    mma16(d, c0[0], c0[1], c1[0], c1[1], bl[0], bl[1]);
+                    add4(o[2 * g], d);
+                    mma16_first(d, c0[2], c0[3], c1[2], c1[3], bh[0], bh[1]);
+                    mma16(d, c0[2], c0[3], c1[2], c1[3], bl[0], bl[1]);
+                    add4(o[2 * g + 1], d);
+                } else {
+                    mma16(o[2 * g], c0[0], c0[1], c1[0], c1[1], bh[0], bh[1]);
+                    if constexpr (REST) mma16(o[2 * g], c0[0], c0[1], c1[0], c1[1], bl[0], bl[1]);
+                    mma16(o[2 * g + 1], c0[2], c0[3], c1[2], c1[3], bh[0], bh[1]);
+                    if constexpr (REST) mma16(o[2 * g + 1], c0[2], c0[3], c1[2], c1[3], bl[0], bl[1]);
+                }
             }
         }
+
+        l[0] += ls[0], l[1] += ls[1];
 
         // the stage is read: it may be written again
         __syncwarp();

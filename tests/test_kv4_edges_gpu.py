@@ -6,7 +6,7 @@ import torch
 
 import kv4_util as U
 import spindle_b200 as sg
-from test_kv4_gpu import TYPES, case, check, ints
+from test_kv4_gpu import TYPES, U24, case, check, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -247,3 +247,41 @@ def test_plan_refuses_what_it_would_overwrite(dev):
     plan.ring = torch.arange(4, dtype=torch.int32, device=dev)
     sg.kv4_plan(plan, buf[0:2], buf[2:4], buf[12:16].view(2, 2), plan.ring, buf[4:6])
     assert plan.seq.tolist() == [0, 0]
+
+
+def flat_tail(dev, n, k, heads, d, sink_v):
+    """A key 2^k ahead (for q = e_0) of n - 1 equal ones: cache, tables of one row, and the two keys and values in 64 bits
+    as the cache holds them.  All positions after the first page lie in one block."""
+    page = 64
+    cache = sg.Kv4Cache(2, heads, d, page, device=dev)
+    g = torch.Generator(device=dev).manual_seed(2)
+    key = torch.randn(2, heads, d, device=dev, generator=g)
+    v = torch.randn(2, heads, d, device=dev, generator=g).abs() + 0.5
+    key[0] = key[1]
+    key[0, :, 0] += 8.0
+    v[0] = v[0] if sink_v is None else sink_v
+    rows = [torch.cat([t[:1], t[1:].expand(2 * page - 1, heads, d)]) for t in (key, v)]
+    sg.kv4_append(cache, *rows, torch.arange(2 * page, dtype=torch.int32, device=dev))
+    tables = torch.ones(1, (n + page - 1) // page, dtype=torch.int32, device=dev)
+    tables[:, 0] = 0
+    kk, vv = (t.double() for t in sg.kv4_read(cache, ints([0, page], dev), dtype=torch.float32))
+    scale = torch.tensor(k * 0.6931471805599453 / (kk[0, 0, 0] - kk[1, 0, 0]).item(), dtype=torch.float32).item()
+    w = torch.exp(scale * (kk[1, :, 0] - kk[0, :, 0]))[:, None] * (n - 1)   # of all the equal ones, by heads
+    return cache, tables, scale, (vv[0] + w * vv[1]) / (1 + w), scale * kk[0, :, 0] + torch.log1p(w[:, 0]), vv
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n,k", [(1024, 10), (4096, 12), (16384, 14)])
+def test_attention_f32_first_token_and_a_flat_tail(dev, n, k, d):
+    # a first key that weighs as much as all the others together, and a request per warp, so that one running sum takes
+    # all of it: n / 16 rounded additions of values, n / 32 of weights, half a unit in the last place each, and some
+    # for the scores, weights and products
+    heads, n_req = 2, 1024
+    cache, tables, scale, want, wl, vv = flat_tail(dev, n, k, heads, d, None)
+    q = torch.zeros(n_req, heads, d, device=dev)
+    q[:, :, 0] = 1.0
+    cu, seq = torch.arange(n_req + 1, dtype=torch.int32, device=dev), torch.full((n_req,), n, dtype=torch.int32, device=dev)
+    lse = torch.empty(n_req, heads, device=dev)
+    out = sg.kv4_attention(cache, q, cu, seq, tables.repeat(n_req, 1), scale=scale, max_new=1, lse=lse)
+    assert ((out.double() - want).abs() / vv.amax()).max() <= (n / 16 + n / 32 + 64) * U24
+    assert (lse.double() - wl).abs().max() <= (n / 32 + 64) * U24
