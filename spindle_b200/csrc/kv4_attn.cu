@@ -29,13 +29,13 @@
 // with the scales applied in f32 to the small results, and q and its sums as f16
 // rounding and, in a second product, the rounding of what that left (about 22 bits
 // together; a 16-bit q is exact after scaling by a power of two).  The weights p are
-// held the same way (for bf16 without the rest).  For 16-bit types the V values are
-// made in f16, one rounding each.  For f32
+// held the same way (for bf16 without the rest), with as many bits as f16 has above
+// 2^-24.  For 16-bit types the V values are made in f16, one rounding each.  For f32
 //   sum_t p_t v_t = sum_t (p_t s_tg) (c_t - 8) + sum_t p_t (m_tg + 8 s_tg)
 // with p s and m + 8 s in two f16 parts again: around the middle of the codes the
 // long sums stay small, so that nothing of them cancels.  The tensor cores cut off
 // what does not fit a sum's f32, always towards zero, which over a long stretch of
-// small weights after a large one adds up to more than f32 has to lose (4.6e-5 after 4096 positions, 3.1e-6
+// small weights after a large one adds up to more than f32 has to lose (4.6e-5 after 4096 positions, 2.2e-6
 // now): so f32 sums the products of 16 positions apart and adds them by rounded f32 additions
 // (16 requests of 9 tokens: 36.7 -> 38.5 us).
 #include <cuda_bf16.h>
@@ -183,9 +183,15 @@ __device__ __forceinline__ void lds_codes(uint32_t (&w)[G], const uint8_t *row, 
 }
 
 constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
-// Weights are held as 2^P_SHIFT p with p below 2^LAG; in f32 the V scales are brought below 2^5, so that a
-// product stays inside f16's range above and keeps 30 bits below its largest.
-constexpr float P_SHIFT = 2.0f, LAG = 8.0f;
+// Weights are held as 2^P p with p at most 2^LAG, as far up in f16's range as they fit: f16 ends at 2^-24 below, and of a
+// weight 2^-k of the largest 25 + P - k bits are left (a long tail of small weights has one error, so it counts).
+// 16-bit types: 2^(P + LAG) is f16's largest power of two.  f32: the V scales are brought below 2, and the sums are
+// rescaled sooner for more bits below; a product of the two is below 2^15.
+template <typename T>
+struct Weights {
+    static constexpr float P = sizeof(T) == 4 ? 12.0f : 7.0f, LAG = sizeof(T) == 4 ? 2.0f : 8.0f;
+};
+constexpr int V_TOP = 1;  // f32: V scales below 2^V_TOP
 constexpr int ROWS = 8;
 constexpr uint32_t MAX_REQ = 1024;  // requests of one launch (their steps are in shared memory)
 constexpr uint32_t MAX_CTAS = 192;
@@ -251,6 +257,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
     using C = Cfg<T, D>;
     constexpr int G = L::G, TILES = C::TILES, STAGES = C::STAGES, STEP = C::STEP, WARPS = C::WARPS, THREADS = C::THREADS;
     constexpr bool Q32 = sizeof(T) == 4;
+    constexpr float P_SHIFT = Weights<T>::P, LAG = Weights<T>::LAG;
     constexpr int QR = Q32 ? 4 : 2;
     constexpr bool REST = !std::is_same<T, __nv_bfloat16>::value;  // what the weights' f16 rounding leaves is far below bf16
     extern __shared__ __align__(128) uint8_t smem[];
@@ -426,7 +433,8 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
     float l[2];
     int32_t lo_t[2], hi_t[2], full_lo = 0, full_hi = 0;  // positions [lo, hi) that a row sees; that all rows see
     int32_t kexp = 15;   // of group lane % G: V scales are multiplied by 2^kexp
-    uint32_t vlim2 = 0;  // and are at most this (f16x2)
+    uint32_t vlim2 = 0;  // and are at most this (f16x2), the f16 below 2^(V_TOP - kexp)
+    constexpr uint32_t VLIM15 = ((15 + V_TOP - 15) << 10) * 0x10001u - 0x10001u;
     uint32_t kmul[G];    // f16x2 of each group's 2^kexp
     uint32_t c_end = 0, c_seg = 0, phase = 0, stage = 0;
     int32_t t0 = 0, held_end = 0;  // the step's first position, the positions held
@@ -564,7 +572,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
                 lo_t[i] = __shfl_sync(~0u, lo_row, src);
                 m[i] = -INFINITY, sh[i] = 0.0f, l[i] = 0.0f;
             }
-            kexp = 15, vlim2 = 0x13FF13FFu;  // the f16 below 2^-10
+            kexp = 15, vlim2 = VLIM15;
 #pragma unroll
             for (int i = 0; i < 2 * G; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
             om[0] = om[1] = om[2] = om[3] = 0.0f;
@@ -678,15 +686,15 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
                 wmax = __vmaxu2(wmax, vw[k]);
             }
             if (__any_sync(~0u, wmax != vlim2)) {
-                const float2 v = unpack_h2(wmax);  // at least the limit, which is below 2^(5 - kexp)
+                const float2 v = unpack_h2(wmax);  // at least the limit, which is below 2^(V_TOP - kexp)
                 float vmax = fmaxf(v.x, v.y);
 #pragma unroll
                 for (int off = G; off < 32; off <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(~0u, vmax, off));
-                // 2^kexp times the largest scale is below 2^5 (kexp at most 15, f16's largest power of two)
-                const int k = min(kexp, 4 - ((int)(__float_as_uint(vmax) >> 23) - 127));
+                // 2^kexp times the largest scale is below 2^V_TOP (kexp at most 15, f16's largest power of two)
+                const int k = min(kexp, V_TOP - 1 - ((int)(__float_as_uint(vmax) >> 23) - 127));
                 vmax = __uint_as_float((uint32_t)(127 + k - kexp) << 23);
                 kexp = k;
-                vlim2 = (uint32_t)((15 + 5 - k) << 10) * 0x10001u - 0x10001u;  // the f16 below 2^(5 - k)
+                vlim2 = (uint32_t)((15 + V_TOP - k) << 10) * 0x10001u - 0x10001u;
 #pragma unroll
                 for (int g = 0; g < G; g++) {
                     const float f = __shfl_sync(~0u, vmax, g);

@@ -6,7 +6,7 @@ import torch
 
 import kv4_util as U
 import spindle_b200 as sg
-from test_kv4_gpu import TYPES, U24, case, check, ints
+from test_kv4_gpu import ROUND, TYPES, U24, case, check, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -285,3 +285,45 @@ def test_attention_f32_first_token_and_a_flat_tail(dev, n, k, d):
     out = sg.kv4_attention(cache, q, cu, seq, tables.repeat(n_req, 1), scale=scale, max_new=1, lse=lse)
     assert ((out.double() - want).abs() / vv.amax()).max() <= (n / 16 + n / 32 + 64) * U24
     assert (lse.double() - wl).abs().max() <= (n / 32 + 64) * U24
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [1, 900])
+@pytest.mark.parametrize("d,k", [(64, 12), (64, 16), (64, 20), (128, 16), (256, 20)])
+def test_attention_weights_far_below_the_largest(dev, dtype, d, k, new):
+    # the first key has nearly all the weight and a value of zeros: the result is the others' alone, each 2^-k of the
+    # largest.  A weight keeps 25 + 12 - k bits in f32, where its product with a scale is rounded once more, and at
+    # least 2^-12 in the 16-bit types (either kernel), besides V's rounding and the result's; scores below 32 in base
+    # 2 are known to three times 2^-20 times ln 2; n / 16 additions of values and n / 32 of weights in a warp at most.
+    # f32 sums (c - 8) s and m + 8 s apart: 8 / 15 of a group's span and a value, below 3 times the largest value
+    heads, group, n = 4, 8, 900 + new
+    cache, tables, scale, want, _, vv = flat_tail(dev, n, k, heads, d, 0.0)
+    q = torch.zeros(new, heads * group, d, device=dev, dtype=dtype)
+    q[..., 0] = 1.0
+    out = sg.kv4_attention(cache, q, ints([0, new], dev), ints([n], dev), tables, scale=scale)[-1]
+    share = (want / vv[1]).repeat_interleave(group, 0)                # of the weight that the others have
+    want = want.repeat_interleave(group, 0)
+    tol = 2.0 ** (k - 36) + 3 * 2.0 ** -20 + (n / 16 + n / 32 + 64) * U24
+    if dtype != torch.float32:
+        tol += 2.0 ** -12 + 2.0 ** -11 + ROUND[dtype]
+    assert ((out.double() - want).abs() <= tol * 3 * vv.amax() * share).all()
+
+
+def test_attention_f32_is_f32(dev):
+    # the root mean square of the errors in f32, where roundings meet in quadrature: scores that are off by
+    # sqrt(d) 2^-24 of sum |q k| (about 4), weights and their products by 2^-22 of the largest, sums by less
+    for heads, group, d, lens, news in [(2, 4, 64, [3000, 17], [1, 9]), (4, 8, 128, [5000, 900, 1], [1, 1, 1]), (8, 2, 128, [2050] * 4, [9] * 4),
+                                        (2, 4, 256, [700, 300], [200, 130]), (1, 7, 128, [70000], [2])]:
+        cache, tables, full, cu, seq, g = case(dev, lens, news, heads, d, 64, d)
+        q = torch.randn(sum(news), heads * group, d, device=dev, generator=g)
+        out = sg.kv4_attention(cache, q, cu, seq, tables, max_new=max(news)).double()
+        off, norm = 0.0, 0.0
+        for i, length in enumerate(lens):
+            a, b = cu[i].item(), cu[i + 1].item()
+            pos = torch.arange(length)
+            slots = (full[i][pos // 64] * 64 + pos % 64).int().to(dev)
+            k, v = (t.double() for t in sg.kv4_read(cache, slots, dtype=torch.float32))
+            want, _, _ = U.attention(q[a:b].double(), k, v, torch.arange(length - (b - a), length, device=dev),
+                                     torch.ones(length, dtype=torch.bool, device=dev), d ** -0.5, 0)
+            off, norm = off + (out[a:b] - want).pow(2).sum().item(), norm + want.pow(2).sum().item()
+        assert (off / norm) ** 0.5 <= 4 * d ** 0.5 * U24 + 2.0 ** -21, (d, lens, (off / norm) ** 0.5)
