@@ -114,7 +114,7 @@ struct Kv4AttnArgs {
     uint8_t *scratch;
     uint64_t block_bytes;  // of one block, all heads
     bool vec_q, vec_out;  // the rows allow 16-byte accesses
-    bool last;            // this launch's requests are the last ones
+    bool first, last;     // this launch's requests are the first ones, the last ones
     uint32_t head0, n_kv; // and its KV heads
 };
 

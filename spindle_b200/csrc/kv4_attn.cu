@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
 
     auto tiles_of = [&](const Req &r) { return ((uint32_t)r.nq * a.group + ROWS - 1) / ROWS; };
 
-    const uint32_t spare = !a.last ? a.n_tok : a.n_req ? (uint32_t)max(a.cu[a.n_req], 0) : 0;  // first token of no request
+    const uint32_t spare = !a.last ? a.n_tok : a.n_req ? min((uint32_t)max(a.cu[a.n_req], 0), a.n_tok) : 0;
 
     // steps before each request
     uint32_t total = 0;
@@ -311,11 +311,12 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
     if (tid == 0) pre[a.n_req] = total;
     __syncthreads();
 
-    // tokens of no request
-    if (spare < a.n_tok) {
-        const uint32_t rows = (a.n_tok - spare) * a.n_heads;
+    // tokens of no request: those before `lead` and those from `spare` on
+    const uint32_t lead = a.first && a.n_req ? min((uint32_t)reqs[0].tok0, a.n_tok) : 0;
+    if (lead || spare < a.n_tok) {
+        const uint32_t rows = (lead + a.n_tok - spare) * a.n_heads;
         for (uint32_t row = blockIdx.x * (WARPS + 1) + warp; row < rows; row += gridDim.x * (WARPS + 1)) {
-            const uint32_t t = spare + row / a.n_heads, h = row % a.n_heads;
+            const uint32_t i = row / a.n_heads, h = row % a.n_heads, t = i < lead ? i : spare + i - lead;
             if (h / a.group - a.head0 >= a.n_kv) continue;
             for (uint32_t d = lane; d < D; d += 32) ((T *)a.out)[t * a.o_tok + h * a.o_head + d] = Act<T>::put(0.0f);
             if (a.lse && lane == 0) a.lse[(uint64_t)t * a.n_heads + h] = -INFINITY;
@@ -987,7 +988,7 @@ sg_status launch(const Kv4AttnArgs &a0, int sms, cudaStream_t s, cudaError_t *er
             Kv4AttnArgs a = a0;
             a.n_req = a0.n_req - r0 < MAX_REQ ? a0.n_req - r0 : MAX_REQ;
             if (r0) a.cu += r0, a.seq += r0, a.tables += (uint64_t)r0 * a.ld_tables;
-            a.last = r0 + a.n_req == a0.n_req;
+            a.first = r0 == 0, a.last = r0 + a.n_req == a0.n_req;
             a.head0 = h0;
             a.n_kv = (uint32_t)(all - h0 < heads ? all - h0 : heads);
             fn<<<grid, Cfg<T, D>::THREADS, Cfg<T, D>::SMEM, s>>>(a);

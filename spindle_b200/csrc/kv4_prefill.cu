@@ -172,10 +172,12 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
     const uint32_t req = blockIdx.z, head = blockIdx.y;
 
     // tokens of no request: zeros, and no sum
-    if (a.last && req == 0) {
-        const uint32_t spare = min((uint32_t)max(a.cu[a.n_req], 0), a.n_tok), all = (a.n_tok - spare) * a.n_heads;
+    if ((a.first || a.last) && req == 0) {
+        const uint32_t lead = a.first ? min((uint32_t)max(a.cu[0], 0), a.n_tok) : 0;
+        const uint32_t spare = a.last ? min((uint32_t)max(a.cu[a.n_req], 0), a.n_tok) : a.n_tok, all = (lead + a.n_tok - spare) * a.n_heads;
         for (uint32_t r = (blockIdx.y * gridDim.x + blockIdx.x) * (C::THREADS / 32) + warp; r < all; r += gridDim.x * gridDim.y * (C::THREADS / 32)) {
-            const uint64_t t = spare + r / a.n_heads, h = r % a.n_heads;
+            const uint32_t i = r / a.n_heads;
+            const uint64_t t = i < lead ? i : spare + i - lead, h = r % a.n_heads;
             for (uint32_t d = lane; d < D; d += 32) ((T *)a.out)[t * a.o_tok + h * a.o_head + d] = from_f32<T>(0.0f);
             if (a.lse && lane == 0) a.lse[t * a.n_heads + h] = -INFINITY;
         }
@@ -605,7 +607,7 @@ cudaError_t launch(const Kv4AttnArgs &a, cudaStream_t s) {
     for (uint32_t r0 = 0; r0 < a.n_req; r0 += 32768) {
         Kv4AttnArgs b = a;
         b.n_req = a.n_req - r0 < 32768 ? a.n_req - r0 : 32768;
-        b.last = r0 + b.n_req == a.n_req;
+        b.first = r0 == 0, b.last = r0 + b.n_req == a.n_req;
         b.cu += r0, b.seq += r0, b.tables += (uint64_t)r0 * a.ld_tables;
         fn<<<dim3(tiles, a.c.heads, b.n_req), C::THREADS, C::SMEM, s>>>(b);
         if ((e = cudaGetLastError()) != cudaSuccess) return e;

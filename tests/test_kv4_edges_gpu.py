@@ -327,3 +327,20 @@ def test_attention_f32_is_f32(dev):
                                      torch.ones(length, dtype=torch.bool, device=dev), d ** -0.5, 0)
             off, norm = off + (out[a:b] - want).pow(2).sum().item(), norm + want.pow(2).sum().item()
         assert (off / norm) ** 0.5 <= 4 * d ** 0.5 * U24 + 2.0 ** -21, (d, lens, (off / norm) ** 0.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_tok,heads,group", [(9, 2, 4), (1500, 4, 8)])
+def test_attention_tokens_before_the_first_request(dev, dtype, n_tok, heads, group):
+    # a part of the requests: the tokens before and after theirs belong to none
+    lens = [300, 77, 40]
+    a, b, c = n_tok // 3, n_tok // 3 * 2, n_tok - 1
+    cache, tables, full, _, seq, g = case(dev, [max(l, n_tok) for l in lens[:2]], [1, 1], heads, 64, 16, 4)
+    cu = ints([a, b, c], dev)
+    q = torch.randn(n_tok, heads * group, 64, device=dev, generator=g).to(dtype)
+    out = torch.full_like(q, 7.0)
+    lse = torch.full((n_tok, heads * group), 7.0, device=dev)
+    sg.kv4_attention(cache, q, cu, seq, tables, out=out, lse=lse)
+    check(dev, cache, tables, full, cu, seq, q, 64 ** -0.5, 0, out, lse)
+    for none in (slice(0, a), slice(c, n_tok)):
+        assert (out[none] == 0).all() and torch.isneginf(lse[none]).all()
