@@ -186,6 +186,13 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
     // this CTA's rows; the requests' last tiles, which see most, come first
     const int32_t tok0 = max(a.cu[req], 0), nq = max(min(a.cu[req + 1], (int32_t)a.n_tok) - tok0, 0);
     const uint32_t rows = (uint32_t)nq * a.group, tile = gridDim.x - 1 - blockIdx.x, row0 = tile * (128 * NQ);
+    // rows of tokens past max_new, which no CTA has: not a number, rather than what was there before
+    if (blockIdx.x == 0)
+        for (uint32_t r = gridDim.x * (128 * NQ) + warp; r < rows; r += C::THREADS / 32) {
+            const uint64_t t = (uint64_t)tok0 + r / a.group, hq = head * a.group + r % a.group;
+            for (uint32_t d = lane; d < D; d += 32) ((T *)a.out)[t * a.o_tok + hq * a.o_head + d] = from_f32<T>(NAN);
+            if (a.lse && lane == 0) a.lse[t * a.n_heads + hq] = NAN;
+        }
     if (row0 >= rows) return;
     const uint32_t halves = min((uint32_t)NQ, (rows - row0 + 127) / 128);
     const int32_t seq = max(a.seq[req], 0);

@@ -222,7 +222,7 @@ def kv4_attention(cache, q, cu, seq, tables, scale=None, window=0, max_new=0, ou
     seq [n_req] int32 as kv4_plan makes them, tables int32 [n_req, width].  Token t
     of a request sees the positions up to its own, the last `window` of them if
     window > 0.  max_new: an upper bound of a request's new tokens, if the caller
-    knows one.  lse: optional float32 [n_tok, n_heads] to fill with the log of the
+    knows one (tokens past one that is too small may get NaN).  lse: optional float32 [n_tok, n_heads] to fill with the log of the
     softmax's sum.  Returns out, [n_tok, n_heads, head_dim] of q's type."""
     n = seq.numel()
     shape, stride = q.shape, q.stride()

@@ -344,3 +344,21 @@ def test_attention_tokens_before_the_first_request(dev, dtype, n_tok, heads, gro
     check(dev, cache, tables, full, cu, seq, q, 64 ** -0.5, 0, out, lse)
     for none in (slice(0, a), slice(c, n_tok)):
         assert (out[none] == 0).all() and torch.isneginf(lse[none]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_more_new_tokens_than_max_new(dev, dtype, d):
+    # a bound that is too small: every row is written, right up to the bound, and right or NaN past it
+    lens, news, heads, group = [700, 400], [600, 2], 4, 8
+    cache, tables, full, cu, seq, g = case(dev, lens, news, heads, d, 16, 8)
+    q = torch.randn(sum(news), heads * group, d, device=dev, generator=g).to(dtype)
+    right, rl = torch.empty_like(q), torch.empty(sum(news), heads * group, device=dev)
+    sg.kv4_attention(cache, q, cu, seq, tables, out=right, lse=rl)
+    for bound in (1, 100, 599):
+        out, lse = torch.full_like(q, 7.0), torch.full_like(rl, 7.0)
+        sg.kv4_attention(cache, q, cu, seq, tables, out=out, lse=lse, max_new=bound)
+        nan = torch.isnan(out)
+        assert torch.equal(nan[..., 0], torch.isnan(lse)) and torch.equal(nan, nan[..., :1].expand_as(nan))
+        assert not nan[:bound].any() and not nan[600:].any() if bound > 1 else not nan[:1].any()
+        assert torch.equal(out[~nan], right[~nan]) and torch.equal(lse[~nan[..., 0]], rl[~nan[..., 0]])
