@@ -517,7 +517,8 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
             }
             e = min(max(e, -100), 116);
             const float up = copysignf(__uint_as_float((uint32_t)(127 + 14 - e) << 23), a.scale);
-            const float cs_row = fabsf(a.scale) * LOG2E * __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+            // (above 0, so that a position that is not seen stays at minus infinity)
+            const float cs_row = fmaxf(fabsf(a.scale) * LOG2E * __uint_as_float((uint32_t)(127 - 14 + e) << 23), 0x1p-126f);
 #pragma unroll
             for (int g = 0; g < G; g++)
 #pragma unroll

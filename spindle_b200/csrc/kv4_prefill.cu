@@ -249,7 +249,8 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
         // q * 2^(6 - e) is below 2^7; the K operand is half of s c
         const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 116);
         const float up = copysignf(__uint_as_float((uint32_t)(127 + 6 - e) << 23), a.scale);
-        cs = fabsf(a.scale) * LOG2E * 2.0f * __uint_as_float((uint32_t)(127 - 6 + e) << 23);
+        // (above 0, so that a position that is not seen stays at minus infinity)
+        cs = fmaxf(fabsf(a.scale) * LOG2E * 2.0f * __uint_as_float((uint32_t)(127 - 6 + e) << 23), 0x1p-126f);
         uint8_t *dst = q_s + tid / 128 * C::Q_BYTES + tid % 128 / 8 * C::SBO_Q + tid % 8 * 16;
         float sum[G];
 #pragma unroll

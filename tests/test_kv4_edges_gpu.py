@@ -362,3 +362,19 @@ def test_attention_more_new_tokens_than_max_new(dev, dtype, d):
         assert torch.equal(nan[..., 0], torch.isnan(lse)) and torch.equal(nan, nan[..., :1].expand_as(nan))
         assert not nan[:bound].any() and not nan[600:].any() if bound > 1 else not nan[:1].any()
         assert torch.equal(out[~nan], right[~nan]) and torch.equal(lse[~nan[..., 0]], rl[~nan[..., 0]])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [1, 3, 700])
+def test_attention_tiny_scales(dev, dtype, new):
+    # scales so small that they and the smallest query's power of two leave f32's range: equal weights
+    heads, group, d, lens = 4, 8, 64, [new + 5, new, 800]
+    cache, tables, full, cu, seq, g = case(dev, lens, [new] * 3, heads, d, 16, new)
+    q = torch.randn(3 * new, heads * group, d, device=dev, generator=g)
+    q[0] = 0
+    q[1, ::2] *= 1e-30
+    q = q.to(dtype)
+    for scale in (1e-20, 1e-38, -1e-44):
+        lse = torch.empty(3 * new, heads * group, device=dev)
+        out = sg.kv4_attention(cache, q, cu, seq, tables, scale=scale, lse=lse, max_new=new)
+        check(dev, cache, tables, full, cu, seq, q, scale, 0, out, lse)
