@@ -221,7 +221,7 @@ def kv4_attention(cache, q, cu, seq, tables, scale=None, window=0, max_new=0, ou
     [n_tok, n_heads, head_dim] (float32, float16 or bfloat16), cu [n_req + 1] and
     seq [n_req] int32 as kv4_plan makes them, tables int32 [n_req, width].  Token t
     of a request sees the positions up to its own, the last `window` of them if
-    window > 0.  max_new: an upper bound of a request's new tokens, if the caller
+    window > 0.  scale None: 1 / sqrt(head_dim) (0: equal weights).  max_new: an upper bound of a request's new tokens, if the caller
     knows one (tokens past one that is too small may get NaN).  lse: optional float32 [n_tok, n_heads] to fill with the log of the
     softmax's sum.  Returns out, [n_tok, n_heads, head_dim] of q's type."""
     n = seq.numel()
@@ -244,7 +244,7 @@ def kv4_attention(cache, q, cu, seq, tables, scale=None, window=0, max_new=0, ou
         raise ValueError("scratch must be a contiguous tensor on q's device")
     a = SgKv4Attn(_type(q, "q"), shape[1], shape[0], n, q.data_ptr(), stride[0], stride[1], out.data_ptr(), ostride[0], ostride[1],
                   None if lse is None else lse.data_ptr(), _i32(cu, "cu", dev, n + 1), _i32(seq, "seq", dev), table, ld, width,
-                  0.0 if scale is None else scale, window, max_new, scratch.data_ptr(), scratch.numel())
+                  0.0 if scale is None else 1e-38 if -1e-38 < scale < 1e-38 else scale, window, max_new, scratch.data_ptr(), scratch.numel())
     st = _lib.load().sg_kv4_attention(cache._c, C.byref(a), _s(stream, q))
     if st:
         _lib.check(st, "kv4_attention")

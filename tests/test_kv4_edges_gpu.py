@@ -378,3 +378,12 @@ def test_attention_tiny_scales(dev, dtype, new):
         lse = torch.empty(3 * new, heads * group, device=dev)
         out = sg.kv4_attention(cache, q, cu, seq, tables, scale=scale, lse=lse, max_new=new)
         check(dev, cache, tables, full, cu, seq, q, scale, 0, out, lse)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_scale_of_zero(dev, dtype):
+    # not the default: every seen position weighs the same
+    cache, tables, full, cu, seq, g = case(dev, [100, 1], [1, 1], 2, 64, 16, 3)
+    q = torch.randn(2, 8, 64, device=dev, generator=g).to(dtype)
+    for zero in (0, 0.0, -0.0, 1e-60):
+        check(dev, cache, tables, full, cu, seq, q, 0.0, 0, sg.kv4_attention(cache, q, cu, seq, tables, scale=zero), None)
