@@ -12,7 +12,7 @@ for decoder.Decoder; the embedding is F32 or F16 rows.
 import torch
 
 from . import F16, F32, Moe, matmul_batch, moe_forward_batch, repack_tiled16
-from .kv4 import Kv4Cache, Kv4Plan, LogProbs, kv4_append, kv4_attention, kv4_attention_scratch, kv4_plan, logprobs
+from .kv4 import LOGPROBS_TOP_MAX, Kv4Cache, Kv4Plan, LogProbs, kv4_append, kv4_attention, kv4_attention_scratch, kv4_plan, logprobs
 
 BATCH = 128  # tokens of one batch GEMM or expert pass
 
@@ -80,8 +80,16 @@ class PagedDecoder:
         requests with tokens, in rising order, `requests` (list), `logits` [n, vocab]
         after their last token, `next` (greedy, int64) and `probs`, the LogProbs of
         the greedy tokens with `top` alternatives."""
-        new = [0] * self.n_req
+        new, end, vocab = [0] * self.n_req, set(end), self.cfg["vocab"]
+        # (all of it before the plan, which changes what the requests hold)
+        if not 0 <= top <= min(LOGPROBS_TOP_MAX, vocab):
+            raise ValueError("top must be 0 to %d" % min(LOGPROBS_TOP_MAX, vocab))
+        if any(not 0 <= r < self.n_req for r in end | set(tokens)):
+            raise ValueError("requests are numbered 0 to %d" % (self.n_req - 1))
+        tokens = {r: [int(t) for t in ts] for r, ts in tokens.items()}
         for r, ts in tokens.items():
+            if any(not 0 <= t < vocab for t in ts):
+                raise ValueError("request %d has a token outside the vocabulary" % r)
             if r in end:
                 raise ValueError("request %d cannot end and go on in one step" % r)
             if self.held[r] + len(ts) > self.cfg["max_seq"]:
