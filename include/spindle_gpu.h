@@ -610,7 +610,8 @@ SG_API sg_status sg_kv4_read(const sg_kv4 *c, int32_t type, const int32_t *d_slo
  * q's type; lse (optional, f32 [n_tok][n_heads]) = ln of the softmax's sum, for
  * joining with attention over other keys.  A token that sees nothing, or belongs
  * to no request, gets zeros and lse = -infinity.  q and out: element (t, h, d) at
- * [t * tok stride + h * head stride + d].  scale 0: 1 / sqrt(head_dim).  max_new:
+ * [t * tok stride + h * head stride + d].  width * page at most 2^31 - 1024.
+ * scale 0: 1 / sqrt(head_dim).  max_new:
  * an upper bound of a request's new tokens (0: n_tok); where it is too small, the
  * tokens past it may get NaN.  scratch:
  * sg_kv4_attention_scratch_bytes() bytes, 256-byte aligned, zeroed once by

@@ -2536,7 +2536,8 @@ sg_status sg_kv4_attention(const sg_kv4 *c, const sg_kv4_attn *p, void *stream) 
         p->n_req >= 1ull << 31 || !(p->scale - p->scale == 0.0f) ||
         (p->n_req && (!p->cu || !p->seq || (p->width && !p->tables))))
         return SG_ERR_INVALID;
-    if (p->width * c->page >= 1ull << 31 || p->width >= 1ull << 31 || (p->n_req > 1 && p->ld_tables < p->width))
+    // (positions in 32 bits, and the last step's end too)
+    if (p->width >= 1ull << 31 || p->width * c->page > (1ull << 31) - 1024 || (p->n_req > 1 && p->ld_tables < p->width))
         return SG_ERR_INVALID;
     if (!aligned(p->q, es) || !aligned(p->out, es) || !aligned(p->scratch, 256) || !aligned(p->lse, 4)) return SG_ERR_ALIGN;
     DevInfo *di;

@@ -62,3 +62,19 @@ def test_plan_refuses_overlapping_memory():
         for out, m in sizes.items():
             assert plan(**{out: at[read] + n - 4}) == 1, (read, out)
             assert plan(**{out: at[read] - m + 4}) == 1, (read, out)
+
+
+def test_attention_refuses_tables_to_the_end_of_31_bits():
+    # a step that begins below 2^31 may end past it
+    import ctypes as C
+
+    from spindle_b200 import _lib
+    L = _lib.load()
+    for page in (16, 64, 1024):
+        cache = _lib.SgKv4(128, 8, page, 4, 0x100000)
+        for past in (0, 16, 1024 - page):
+            if past % page:
+                continue
+            a = _lib.SgKv4Attn(1, 8, 1, 1, 0x100000, 1024, 128, 0x100000, 1024, 128, None, 0x100000, 0x100000, 0x100000, 1 << 28,
+                               ((1 << 31) - past) // page, 0.0, 0, 0, 0x100000, 1 << 30)
+            assert L.sg_kv4_attention(C.byref(cache), C.byref(a), None) == 1, (page, past)

@@ -387,3 +387,24 @@ def test_attention_scale_of_zero(dev, dtype):
     q = torch.randn(2, 8, 64, device=dev, generator=g).to(dtype)
     for zero in (0, 0.0, -0.0, 1e-60):
         check(dev, cache, tables, full, cu, seq, q, 0.0, 0, sg.kv4_attention(cache, q, cu, seq, tables, scale=zero), None)
+
+
+@pytest.mark.parametrize("dtype,new", [(torch.float32, 1), (torch.float16, 1), (torch.float32, 9), (torch.bfloat16, 9), (torch.float16, 900),
+                                       (torch.bfloat16, 900)])
+@pytest.mark.parametrize("d,window", [(64, 100), (128, 1000), (256, 37)])
+def test_attention_at_the_end_of_31_bits(dev, dtype, new, d, window):
+    # the longest table there is, its last two blocks held: offsets of table entries, positions and steps near 2^31
+    heads, group, page = 4, 8, 1024
+    n = (1 << 31) - 1024
+    cache = sg.Kv4Cache(2, heads, d, page, device=dev)
+    g = torch.Generator(device=dev).manual_seed(window)
+    k, v = (torch.randn(2 * page, heads, d, device=dev, generator=g) for _ in range(2))
+    slots = torch.arange(2 * page, dtype=torch.int32, device=dev)
+    sg.kv4_append(cache, k, v, slots)
+    tables = torch.full((1, n // page), -1, dtype=torch.int32, device=dev)
+    tables[0, -2:] = ints([0, 1], dev)
+    q = torch.randn(new, heads * group, d, device=dev, generator=g).to(dtype)
+    lse = torch.empty(new, heads * group, device=dev)
+    out = sg.kv4_attention(cache, q, ints([0, new], dev), ints([n], dev), tables, window=window, lse=lse)
+    check(dev, cache, ints([[0, 1]], dev), torch.tensor([[0, 1]]), ints([0, new], dev), ints([2 * page], dev), q, d ** -0.5, window, out, lse)
+    sg.device_status()
