@@ -195,7 +195,10 @@ constexpr int V_TOP = 1;  // f32: V scales below 2^V_TOP
 constexpr int ROWS = 8;
 constexpr uint32_t MAX_REQ = 1024;  // requests of one launch (their steps are in shared memory)
 constexpr uint32_t MAX_CTAS = 192;
-constexpr uint32_t MIN_WARPS = 7;   // warps that a CTA uses at least where the steps are few (264 steps: 13.0 us; 4: 13.6, 2: 15.0)
+// Warps that a CTA uses at least where the steps are few.  One token of 200, 600, 1037, 2000 and 4000 positions, 16 query
+// and 8 KV heads of 128 in f16, device time: 7.6, 12.6, 12.7, 11.3, 15.8 us; with 4 of them 12.0, 12.0, 13.3, 15.2, 15.8;
+// with 11 13.6, 13.5, 11.3, 14.2, 15.5.  (f32, heads of 64 and of 256, and four requests go the same way.)
+constexpr uint32_t MIN_WARPS = 7;
 
 template <typename T, int D>
 struct Cfg {

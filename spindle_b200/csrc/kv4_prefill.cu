@@ -632,13 +632,16 @@ cudaError_t kv4_prefill_launch(const Kv4AttnArgs &a, int32_t type, uint32_t d, c
 
 bool kv4_prefill_pays(const Kv4AttnArgs &a, int32_t type, uint32_t d, int sms) {
     if (type == SG_F32 || a.n_req == 0) return false;
-    // Rows (of all heads and requests) a wave of its CTAs from which this kernel is the faster one.  Measured in bf16
-    // over 500 to 8000 positions: heads of 128 at 6656 rows a wave 85 us against 65 in the streaming kernel, at 8192
-    // 126 against 143, at 13312 78 against 105; heads of 64 cross at the same place (69 against 46, 100 against 95, 60
-    // against 73); heads of 256, whose tiles are half as tall, at 5216 73 against 65 and at 6656 112 against 119.
+    // Rows (of all heads and requests) a wave of its CTAs from which this kernel is the faster one.  One request of 2000
+    // positions, 4 KV heads, groups of 8, streaming kernel / this one in us, bf16 (f16): heads of 128 at 5632 rows 63 / 74
+    // (66 / 74), at 6656 72 / 74 (76 / 74), at 8192 85 / 76 (91 / 76); of 8000 positions 190 / 230, 221 / 229, 270 / 227.
+    // Heads of 64: 6656 rows 48 / 59, 8192 56 / 60, 13312 84 / 61.  Heads of 256, whose tiles are half as tall: 4096 rows
+    // 91 / 101, 5632 119 / 100.  Over 150 shapes in f16 and bf16 (1 to 9 requests, 256 to 8000 positions, pages of 16 to
+    // 128, with and without a window) the kernel that these limits choose is 1.3 % (64), 0.3 % and 0 % slower than the
+    // faster of the two in the mean, at worst 19 %, 13 % and 0 %.
     const uint64_t per = d == 256 ? 128 : 256, rows = (uint64_t)a.n_tok * a.group;
     const uint64_t ctas = (rows / per + a.n_req) * a.c.heads, waves = (ctas + sms - 1) / sms;
-    return rows * a.c.heads > waves * (d == 256 ? 5700 : 7700);
+    return rows * a.c.heads > waves * (d == 64 ? 7700 : d == 128 ? 6500 : 4900);
 }
 
 }  // namespace sg
