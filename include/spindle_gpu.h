@@ -593,9 +593,9 @@ SG_API sg_status sg_kv4_plan(uint32_t page, uint32_t n_blocks, uint64_t n_req, c
  * row is left out; no two rows may have the same slot).  type SG_F32, SG_F16 or
  * SG_BF16; element (t, h, d) of K at d_k[t * k_tok + h * k_head + d], V likewise.
  * Values are clamped to f16's finite range and NaN counts as 0, so that the cache
- * holds numbers that are finite in f16 only; d_nonfinite (optional) counts the groups that had an
- * infinity or a NaN.  sg_kv4_read gives back the values of given slots as
- * [n_tok][n_kv_heads][head_dim] of `type`, 16-byte aligned, zeros for no slot. */
+ * holds numbers that are finite in f16 only; d_nonfinite (optional) counts the
+ * groups that had an infinity or a NaN.  sg_kv4_read gives back the values of given
+ * slots as [n_tok][n_kv_heads][head_dim] of `type`, 16-byte aligned, zeros for no slot. */
 SG_API sg_status sg_kv4_append(const sg_kv4 *c, int32_t type, const void *d_k, uint64_t k_tok, uint64_t k_head,
                                const void *d_v, uint64_t v_tok, uint64_t v_head, const int32_t *d_slots, uint64_t n_tok,
                                int32_t *d_nonfinite, void *stream);
@@ -611,10 +611,13 @@ SG_API sg_status sg_kv4_read(const sg_kv4 *c, int32_t type, const int32_t *d_slo
  * joining with attention over other keys.  A token that sees nothing, or belongs
  * to no request, gets zeros and lse = -infinity.  q and out: element (t, h, d) at
  * [t * tok stride + h * head stride + d].  width * page at most 2^31 - 1024.
- * scale 0: 1 / sqrt(head_dim).  max_new:
- * an upper bound of a request's new tokens (0: n_tok); where it is too small, the
- * tokens past it may get NaN.  scratch:
- * sg_kv4_attention_scratch_bytes() bytes, 256-byte aligned, zeroed once by
+ * scale 0: 1 / sqrt(head_dim).  max_new: an upper bound of a request's new tokens
+ * (0: n_tok); where it is too small, the tokens past it may get NaN.
+ * Maxima, sums and lse are f32.  For a 16-bit q the values of V are rounded to f16
+ * (2^-11 of them at most), and for bf16, or in calls of many tokens, the softmax's
+ * weights too; for f32 the query, the weights and their products with V's scales are
+ * held to about 22 bits each, weights to 2^-37 of the largest at best.
+ * scratch: sg_kv4_attention_scratch_bytes() bytes, 256-byte aligned, zeroed once by
  * sg_kv4_attention_scratch_init; calls that overlap on the GPU need one each. */
 typedef struct {
     int32_t type;                     /* of q and out: SG_F32, SG_F16 or SG_BF16 */

@@ -37,7 +37,8 @@ struct Kv4Tile {
 };
 
 // The codes of a word as f16 pairs, c - OFF of the nibbles (0, 4), (1, 5), (2, 6), (3, 7): a nibble in the lowest
-// mantissa bits of 1024, or four bits up in those of 64, less that number.  The masks and numbers are kept in registers
+// mantissa bits of 1024, or four bits up in those of 64, less that number (the well-known way to turn small integers into
+// floating point by their mantissa bits).  The masks and numbers are kept in registers
 // that the compiler does not see through, so that mask and insertion are one instruction (which takes one immediate).
 struct Kv4Codes {
     uint32_t k0, k1, m0, m1;

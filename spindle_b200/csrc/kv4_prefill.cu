@@ -11,9 +11,12 @@
 //     its weights are there: the tensor cores work for one tile while the weights
 //     of the other are made.
 // The scores are as good as f32: with K values m + s c (16-bit s and m, a code c)
-// s c goes in as its f16 rounding and the exact rest, and the minima as 16 more
-// columns against the sums of the query's groups (f16 rounding and rest).  V
-// values and weights are rounded to f16 once each.
+// s c goes in as its f16 rounding and the exact rest (down to f16's last bit, 2^-25 of
+// a K value), and the minima as 16 more columns against the sums of the query's
+// groups (f16 rounding and rest).  V values and weights are rounded to f16 once each,
+// the weights without the rest that the streaming kernel keeps for f16: a second
+// product of every weight would be half as much again of the products, for results that
+// are rounded to f16 or bf16 after it.
 //
 // Two chunks of 1024 and 768 tokens against up to 8100 positions, 32 query and 4 KV heads of 128, bf16: 374 us, 500
 // TFLOP/s of the 186 GFLOP that attention has (30 % of the measured matrix rate; with the rests of K and the minima

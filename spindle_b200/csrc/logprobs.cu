@@ -207,7 +207,7 @@ struct Shared {
     Sum sum[WARPS], all[8];
     uint32_t ahead[WARPS], all_ahead[8];
     uint32_t gmax[GROUPS];
-    uint32_t count, threshold, found;
+    uint32_t count, threshold;
     uint32_t warp_count[WARPS];
     union {
         uint64_t cand[CAP];
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
     sum = join_lanes<32>(sum);
     ahead = __reduce_add_sync(~0u, ahead);
     if (lane == 0) s.sum[warp] = sum, s.ahead[warp] = ahead;
-    if (tid == 0) s.count = 0, s.found = 0, s.threshold = 0;
+    if (tid == 0) s.count = 0, s.threshold = 0;
     if (a.top) {
         float g = tmax;
 #pragma unroll
