@@ -13,10 +13,11 @@
 // The scores are as good as f32: with K values m + s c (16-bit s and m, a code c)
 // s c goes in as its f16 rounding and the exact rest (down to f16's last bit, 2^-25 of
 // a K value), and the minima as 16 more columns against the sums of the query's
-// groups (f16 rounding and rest).  V values and weights are rounded to f16 once each,
-// the weights without the rest that the streaming kernel keeps for f16: a second
-// product of every weight would be half as much again of the products, for results that
-// are rounded to f16 or bf16 after it.
+// groups (f16 rounding and rest).  Weights are rounded to f16 once, without the rest
+// that the streaming kernel keeps for f16: TMEM has no room for it.  V values are rounded
+// to f16 once for bf16; for f16 they go in as rounding and rest, since V's rounding,
+// the weights' and the result's together were 1.5 times the result's alone (3.1e-4
+// against 2.1e-4 of it, root mean square; without V's 2.2e-4 to 2.5e-4).
 //
 // Two chunks of 1024 and 768 tokens against up to 8100 positions, 32 query and 4 KV heads of 128, bf16: 374 us, 500
 // TFLOP/s of the 186 GFLOP that attention has (30 % of the measured matrix rate; with the rests of K and the minima
@@ -36,20 +37,27 @@ namespace {
 constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
 constexpr float P_SHIFT = 6.0f, LAG = 8.0f;  // weights are held as 2^6 p, p below 2^8: inside f16's range
 
-template <int D>
+template <typename T, int D>
 struct Pre {
     static constexpr int G = D / 32;
+    static constexpr bool VREST = std::is_same<T, __half>::value;  // V as f16 rounding and rest
     // Products of 128 rows by 128 positions run at twice the rate of those by 64 (73 cycles against 59); what a head of
     // 256 leaves of the shared memory and of TMEM is one tile of rows and 64 positions.
     static constexpr int NQ = D == 256 ? 1 : 2, NK = D == 256 ? 64 : 128;
     static constexpr int ND = 256;                                  // threads that make operands
+    // V's rest takes the place of V's second buffer where there is no room for both (heads of 128, 8000 positions, a wave
+    // of CTAs: 274 us against 228 without a rest; with both and 96 positions a step 301).
+    static constexpr uint32_t VBUFS = D >= 128 && VREST ? 1 : 2;
+    // With one buffer of V the first of a thread's groups is made while the buffer is still read: heads of 128 274 us
+    // against 291; heads of 256 397 against 385, so there it is not.
+    static constexpr bool EARLY = VBUFS == 1 && D == 128;
     static constexpr int THREADS = 128 * NQ + ND + 32;
     static constexpr int GV = NK * G / ND;                          // groups of V that one of them makes
     static constexpr int KI = NK * 4 * (G == 8 ? 2 : 1) / ND;       // items of K: a position's part of four groups (two)
     static constexpr uint32_t SBO_Q = (D / 8 + 2) * 128, SBO_K = D / 8 * 128, SBO_M = 256, SBO_V = NK * 16 + 16;
     static constexpr uint32_t Q_BYTES = 16 * SBO_Q;                 // 128 rows
-    static constexpr uint32_t K_BYTES = NK / 8 * SBO_K, M_BYTES = NK / 8 * SBO_M, V_BYTES = D / 8 * SBO_V;
-    static constexpr uint32_t K_AT = NQ * Q_BYTES, M_AT = K_AT + 2 * K_BYTES, V_AT = M_AT + M_BYTES, BAR_AT = V_AT + 2 * V_BYTES;
+    static constexpr uint32_t K_BYTES = NK / 8 * SBO_K, M_BYTES = NK / 8 * SBO_M, V_BYTES = D / 8 * SBO_V, VBUF_BYTES = V_BYTES * (VREST ? 2 : 1);
+    static constexpr uint32_t K_AT = NQ * Q_BYTES, M_AT = K_AT + 2 * K_BYTES, V_AT = M_AT + M_BYTES, BAR_AT = V_AT + VBUFS * VBUF_BYTES;
     static constexpr uint32_t SMEM = BAR_AT + 256;
     // TMEM columns: scores, whose place the weights take (two f16 a column), and sums
     static constexpr uint32_t S_COL = 0, O_COL = 256;
@@ -126,6 +134,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
+__device__ __forceinline__ float2 unpack2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -158,10 +167,12 @@ __device__ __forceinline__ void ldg_words(uint32_t (&w)[N], const uint8_t *p) {
 }  // namespace
 
 template <typename T, int D>
-__global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
+__global__ void __launch_bounds__(Pre<T, D>::THREADS, 1) kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
     using L = Kv4Tile<D>;
-    using C = Pre<D>;
+    using C = Pre<T, D>;
     constexpr int G = C::G, NQ = C::NQ, NK = C::NK, ND = C::ND, GV = C::GV, KI = C::KI;
+    constexpr bool VREST = C::VREST;
+    constexpr uint32_t VBUFS = C::VBUFS;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *q_s = smem;
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::BAR_AT);
@@ -300,8 +311,8 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
         // step i: for each tile of rows the sums of step i - 1, then the scores of step i in the weights' place
 #pragma unroll 1
         for (uint32_t i = 0; i <= n && n; i++) {
-            const uint32_t b = (i - 1) & 1;
-            if (i) wait(&v_full[b], (i - 1) >> 1 & 1);
+            const uint32_t b = (i - 1) % VBUFS;
+            if (i) wait(&v_full[b], (i - 1) / VBUFS & 1);
 #pragma unroll 1
             for (uint32_t h = 0; h < halves; h++) {
                 if (i) {
@@ -310,9 +321,13 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
                     fence_after();
                     if (elect_one() && !*dead) {
                         const uint32_t d = tm + C::O_COL + h * D, p = tm + C::S_COL + h * NK;
-                        const uint64_t vd = v_desc + b * (C::V_BYTES >> 4);
+                        const uint64_t vd = v_desc + b * (C::VBUF_BYTES >> 4);
 #pragma unroll
                         for (uint32_t c = 0; c < NK / 16; c++) mma_ts(d, p + c * 8, vd + c * 16, idesc(D), c ? 1u : i - 1);
+                        if constexpr (VREST) {
+#pragma unroll
+                            for (uint32_t c = 0; c < NK / 16; c++) mma_ts(d, p + c * 8, vd + (C::V_BYTES >> 4) + c * 16, idesc(D), 1u);
+                        }
                         if (h + 1 == halves) commit(&v_free[b]);
                         commit(&pv_done[h]);
                     }
@@ -404,9 +419,9 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
             if (n > 1) entries_k(1), entries_v(1);
         }
         for (uint32_t i = 0; i < n; i++) {
-            const uint32_t b = i & 1;
+            const uint32_t b = i % VBUFS;
             wait(k_free, (i & 1) ^ 1);
-            uint8_t *k_hi = smem + C::K_AT, *k_lo = k_hi + C::K_BYTES, *k_m = smem + C::M_AT, *v_t = smem + C::V_AT + b * C::V_BYTES;
+            uint8_t *k_hi = smem + C::K_AT, *k_lo = k_hi + C::K_BYTES, *k_m = smem + C::M_AT, *v_t = smem + C::V_AT + b * C::VBUF_BYTES;
             const int32_t t = (k0 + (int32_t)i) * NK;
 #pragma unroll
             for (int j = 0; j < KI; j++) {
@@ -454,10 +469,10 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
                 load_k(i + 1);
                 if (i + 2 < n) entries_k(i + 2);
             }
-            wait(&v_free[b], (i >> 1 & 1) ^ 1);
+            if (!C::EARLY) wait(&v_free[b], (i / VBUFS & 1) ^ 1);
 #pragma unroll
             for (int g = 0; g < GV; g++) {
-                uint32_t val[4][4];
+                uint32_t val[4][4], low[VREST ? 4 : 1][4];
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
                     const int32_t p = t + (int32_t)tb * 8 + 2 * q;
@@ -466,12 +481,25 @@ __global__ void __launch_bounds__(Pre<D>::THREADS, 1) kv4_prefill_kernel(const _
                     uint32_t c[4];
                     codes.get<0>(vr[q][g], c);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) val[k][q] = hfma2(c[k], s, m);
+                    for (int k = 0; k < 4; k++) {
+                        if constexpr (VREST) {
+                            const float2 cf = unpack2(c[k]), sf = unpack2(s), mf = unpack2(m);
+                            const float v0 = fmaf(cf.x, sf.x, mf.x), v1 = fmaf(cf.y, sf.y, mf.y);
+                            val[k][q] = pack2(v0, v1);
+                            const float2 h = unpack2(val[k][q]);
+                            low[k][q] = pack2(v0 - h.x, v1 - h.y);
+                        } else {
+                            val[k][q] = hfma2(c[k], s, m);
+                        }
+                    }
                 }
+                if (C::EARLY && g == 0) wait(&v_free[b], (i / VBUFS & 1) ^ 1);
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const uint32_t d = 32 * (gq * GV + g) + 4 * x8 + k;
-                    *reinterpret_cast<uint4 *>(v_t + (d >> 3) * C::SBO_V + tb * 128 + (d & 7) * 16) = make_uint4(val[k][0], val[k][1], val[k][2], val[k][3]);
+                    uint4 *at = reinterpret_cast<uint4 *>(v_t + (d >> 3) * C::SBO_V + tb * 128 + (d & 7) * 16);
+                    *at = make_uint4(val[k][0], val[k][1], val[k][2], val[k][3]);
+                    if constexpr (VREST) at[C::V_BYTES / 16] = make_uint4(low[k][0], low[k][1], low[k][2], low[k][3]);
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -604,7 +632,7 @@ namespace {
 
 template <typename T, int D>
 cudaError_t launch(const Kv4AttnArgs &a, cudaStream_t s) {
-    using C = Pre<D>;
+    using C = Pre<T, D>;
     auto fn = kv4_prefill_kernel<T, D>;
     static bool ready[64];
     int dev = 0;
@@ -636,15 +664,16 @@ cudaError_t kv4_prefill_launch(const Kv4AttnArgs &a, int32_t type, uint32_t d, c
 bool kv4_prefill_pays(const Kv4AttnArgs &a, int32_t type, uint32_t d, int sms) {
     if (type == SG_F32 || a.n_req == 0) return false;
     // Rows (of all heads and requests) a wave of its CTAs from which this kernel is the faster one.  One request of 2000
-    // positions, 4 KV heads, groups of 8, streaming kernel / this one in us, bf16 (f16): heads of 128 at 5632 rows 63 / 74
-    // (66 / 74), at 6656 72 / 74 (76 / 74), at 8192 85 / 76 (91 / 76); of 8000 positions 190 / 230, 221 / 229, 270 / 227.
-    // Heads of 64: 6656 rows 48 / 59, 8192 56 / 60, 13312 84 / 61.  Heads of 256, whose tiles are half as tall: 4096 rows
-    // 91 / 101, 5632 119 / 100.  Over 150 shapes in f16 and bf16 (1 to 9 requests, 256 to 8000 positions, pages of 16 to
-    // 128, with and without a window) the kernel that these limits choose is 1.3 % (64), 0.3 % and 0 % slower than the
-    // faster of the two in the mean, at worst 19 %, 13 % and 0 %.
+    // positions, 4 KV heads, groups of 8, streaming kernel / this one in us, bf16 (f16): heads of 128 at 5632 rows 63 / 73
+    // (66 / 85), at 6656 72 / 74 (77 / 86), at 8192 85 / 74 (91 / 86); of 8000 positions 190 / 228 (205 / 276), 221 / 228
+    // (238 / 277), 270 / 226 (291 / 275).  Heads of 64: 6656 rows 48 / 58 (49 / 60), 8192 57 / 58 (58 / 62), 13312 84 / 58
+    // (88 / 62).  Heads of 256, whose tiles are half as tall: 4096 rows 91 / 101 (93 / 111), 5632 119 / 100 (121 / 112).
+    // Over 260 shapes in both types (1 to 9 requests, 256 to 8000 positions, pages of 16 to 128, with and without a window)
+    // the kernel that these limits choose is 0.9 % (64), 0.2 % and 0 % slower than the faster of the two in the mean, at
+    // worst 19 %, 19 % and 0 %.
     const uint64_t per = d == 256 ? 128 : 256, rows = (uint64_t)a.n_tok * a.group;
     const uint64_t ctas = (rows / per + a.n_req) * a.c.heads, waves = (ctas + sms - 1) / sms;
-    return rows * a.c.heads > waves * (d == 64 ? 7700 : d == 128 ? 6500 : 4900);
+    return rows * a.c.heads > waves * (d == 64 ? 7700 : d == 128 ? 6850 : 4900);
 }
 
 }  // namespace sg

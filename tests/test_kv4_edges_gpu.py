@@ -408,3 +408,24 @@ def test_attention_at_the_end_of_31_bits(dev, dtype, new, d, window):
     out = sg.kv4_attention(cache, q, ints([0, new], dev), ints([n], dev), tables, window=window, lse=lse)
     check(dev, cache, ints([[0, 1]], dev), torch.tensor([[0, 1]]), ints([0, new], dev), ints([2 * page], dev), q, d ** -0.5, window, out, lse)
     sg.device_status()
+
+
+@pytest.mark.parametrize("d,length,new", [(64, 2000, 900), (128, 3000, 700), (128, 8000, 300), (256, 1500, 700)])
+def test_attention_f16_many_rows_keeps_its_bits(dev, d, length, new):
+    # the root mean square error of a 16-bit result: a rounding to 11 bits is 2.1e-4 of a value (2^-10 / sqrt(12), over
+    # mantissas from 1 to 2), and besides the result's there is the weights', in quadrature, where a few of them count
+    # (the scale) and V has mean 0.  V's rounding would be a third: 3.6e-4
+    heads, group, page = 4, 8, 32
+    cache = sg.Kv4Cache((length + page - 1) // page, heads, d, page, device=dev)
+    g = torch.Generator(device=dev).manual_seed(d)
+    slots = torch.arange(length, dtype=torch.int32, device=dev)
+    sg.kv4_append(cache, *(torch.randn(length, heads, d, device=dev, generator=g) for _ in range(2)), slots)
+    tables = torch.arange(cache.n_blocks, dtype=torch.int32, device=dev)[None]
+    q = torch.randn(new, heads * group, d, device=dev, generator=g).half()
+    scale = 3 * d ** -0.5
+    out = sg.kv4_attention(cache, q, ints([0, new], dev), ints([length], dev), tables, scale=scale).double()
+    k, v = (t.double() for t in sg.kv4_read(cache, slots, dtype=torch.float32))
+    want, _, _ = U.attention(q.double(), k, v, torch.arange(length - new, length, device=dev), torch.ones(length, dtype=torch.bool, device=dev),
+                             scale, 0)
+    off = ((out - want).norm() / want.norm()).item()
+    assert off <= 2 ** 0.5 * 2.1e-4, off
