@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(KV4_PLAN_THREADS) kv4_plan_kernel(const __grid
 // f16 where m + 15 s >= 65520, which is infinity in f16, so that the cache holds
 // finite numbers only; groups that had an infinity or a NaN are counted.  Every
 // step is one rounded f32 operation, so the codes can be reproduced bit for bit.
-// What bounds it is the arithmetic (19 instructions a value by the counters), hence sixteen
+// What bounds it is the arithmetic (20 instructions a value by the counters), hence sixteen
 // values a lane: the place of a row in the cache is worked out half as often.
 // 24001 rows of 8 heads of 128 in bf16: 44 us, 2.9 TB/s (45 % of the measured copy rate); 32 rows are a launch.
 

@@ -6,7 +6,7 @@
 // pair) of one request and KV head, and goes over the positions NK at a time:
 //   - 128 threads per tile: a thread per row takes its scores from TMEM, keeps the
 //     running maximum and sum, and puts its weights, in f16, where the scores were;
-//   - ND threads turn the codes into f16 operands in shared memory (K, and V twice);
+//   - ND threads turn the codes into f16 operands in shared memory (K, and V twice or with its rest);
 //   - one thread issues the tensor products, a tile's sums and its next scores when
 //     its weights are there: the tensor cores work for one tile while the weights
 //     of the other are made.
@@ -16,10 +16,10 @@
 // groups (f16 rounding and rest).  Weights are rounded to f16 once, without the rest
 // that the streaming kernel keeps for f16: TMEM has no room for it.  V values are rounded
 // to f16 once for bf16; for f16 they go in as rounding and rest, since V's rounding,
-// the weights' and the result's together were 1.5 times the result's alone (3.1e-4
-// against 2.1e-4 of it, root mean square; without V's 2.2e-4 to 2.5e-4).
+// the weights' and the result's together were 1.5 to 1.6 times the result's alone
+// (3.1e-4 to 3.3e-4 against 2.1e-4 of it, root mean square; without V's 2.4e-4 to 2.9e-4).
 //
-// Two chunks of 1024 and 768 tokens against up to 8100 positions, 32 query and 4 KV heads of 128, bf16: 374 us, 500
+// Two chunks of 1024 and 768 tokens against up to 8100 positions, 32 query and 4 KV heads of 128, bf16: 370 us, 500
 // TFLOP/s of the 186 GFLOP that attention has (30 % of the measured matrix rate; with the rests of K and the minima
 // the products are 1.56 times that).  A step of 128 positions takes a tile 6100 cycles, of which its own thread-per-row
 // work is 3600 and the products of both tiles 3700; the last wave of CTAs is part empty (224 CTAs on 148 SMs).
