@@ -613,9 +613,9 @@ SG_API sg_status sg_kv4_read(const sg_kv4 *c, int32_t type, const int32_t *d_slo
  * [t * tok stride + h * head stride + d].  width * page at most 2^31 - 1024.
  * scale 0: 1 / sqrt(head_dim).  max_new: an upper bound of a request's new tokens
  * (0: n_tok); where it is too small, the tokens past it may get NaN.
- * Maxima, sums and lse are f32.  For a 16-bit q the values of V are rounded to f16
- * (2^-11 of them at most), and for bf16, or in calls of many tokens, the softmax's
- * weights too; for f32 the query, the weights and their products with V's scales are
+ * Maxima, sums and lse are f32.  For an f16 q either the values of V or, in calls of
+ * many tokens, the softmax's weights are rounded to f16 (2^-11 of them at most), for
+ * bf16 both; for f32 the query, the weights and their products with V's scales are
  * held to about 22 bits each, weights to 2^-37 of the largest at best.
  * scratch: sg_kv4_attention_scratch_bytes() bytes, 256-byte aligned, zeroed once by
  * sg_kv4_attention_scratch_init; calls that overlap on the GPU need one each. */
