@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
     // (8 rows), so that a lane of quad `quad` has rows 2 quad and 2 quad + 1 of every result.
     uint32_t qb[2 * G][QR], qs[G == 8 ? 2 : 1];
     float o[2 * G][4], om[4];
-    float m[2], sh[2], cs[2];  // the weights' reference and its shift; what a score is multiplied by
+    float m[2], nm[2], cs[2];  // the weights' reference (a score), its negative (0 for none); what a score is multiplied by
     float l[2];
     int32_t lo_t[2], hi_t[2], full_lo = 0, full_hi = 0;  // positions [lo, hi) that a row sees; that all rows see
     int32_t kexp = 15;   // of group lane % G: V scales are multiplied by 2^kexp
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
                 cs[i] = __shfl_sync(~0u, cs_row, src);
                 hi_t[i] = __shfl_sync(~0u, hi_row, src);
                 lo_t[i] = __shfl_sync(~0u, lo_row, src);
-                m[i] = -INFINITY, sh[i] = 0.0f, l[i] = 0.0f;
+                m[i] = -INFINITY, nm[i] = 0.0f, l[i] = 0.0f;
             }
             kexp = 15, vlim2 = VLIM15;
 #pragma unroll
@@ -663,21 +663,20 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
             top[r] = fmaxf(s[0][r], s[0][2 + r]);
 #pragma unroll
             for (int i = 1; i < TILES; i++) top[r] = fmaxf(top[r], fmaxf(s[i][r], s[i][2 + r]));
-            top[r] *= cs[r];
-            behind |= top[r] > m[r] + LAG;
+            behind |= (top[r] - m[r]) * cs[r] > LAG;
         }
         if (__any_sync(~0u, behind)) {
 #pragma unroll
             for (int r = 0; r < 2; r++) {
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) top[r] = fmaxf(top[r], __shfl_xor_sync(~0u, top[r], off));
-                const float mm = fmaxf(m[r], top[r]), f = m[r] == mm ? 1.0f : ex2(m[r] - mm);
+                const float mm = fmaxf(m[r], top[r]), f = m[r] == mm ? 1.0f : ex2((m[r] - mm) * cs[r]);
                 m[r] = mm;
 #pragma unroll
                 for (int i = 0; i < 2 * G; i++) o[i][r] *= f, o[i][2 + r] *= f;
                 om[r] *= f, om[2 + r] *= f;
                 l[r] *= f;
-                sh[r] = mm == -INFINITY ? 0.0f : P_SHIFT - mm;
+                nm[r] = mm == -INFINITY ? 0.0f : -mm;
             }
         }
 
@@ -720,7 +719,8 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
             uint32_t ph[2], pl[2];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const float p0 = ex2(fmaf(s[i][2 * j], cs[0], sh[0])), p1 = ex2(fmaf(s[i][2 * j + 1], cs[1], sh[1]));
+                const float2 t = kv4_exponents(s[i][2 * j], s[i][2 * j + 1], make_float2(nm[0], nm[1]), make_float2(cs[0], cs[1]), P_SHIFT);
+                const float p0 = ex2(t.x), p1 = ex2(t.y);
                 ls[0] = i + j ? ls[0] + p0 : p0, ls[1] = i + j ? ls[1] + p1 : p1;
                 ph[j] = pack_h2(p0, p1);
                 if constexpr (REST) {
@@ -824,7 +824,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
 #pragma unroll
                     for (int g = 0; g < G; g++)
                         *reinterpret_cast<float4 *>(part + tr * D + g * 32 + gid * 4) = make_float4(r[g][i][0], r[g][i][1], r[g][i][2], r[g][i][3]);
-                    if (gid == 0) part[ROWS * D + tr] = m[i], part[ROWS * D + ROWS + tr] = l[i];
+                    if (gid == 0) part[ROWS * D + tr] = m[i] * cs[i], part[ROWS * D + ROWS + tr] = l[i];
                     continue;
                 }
                 const uint32_t row = seg.tile * ROWS + tr, tok = row / a.group, hq = seg.head * a.group + row % a.group;
@@ -834,7 +834,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
                 const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
 #pragma unroll
                 for (int g = 0; g < G; g++) put4(out + g * 32, r[g][i][0] * inv, r[g][i][1] * inv, r[g][i][2] * inv, r[g][i][3] * inv, a.vec_out);
-                if (a.lse && gid == 0) a.lse[t * a.n_heads + hq] = lse_of(m[i], l[i]);
+                if (a.lse && gid == 0) a.lse[t * a.n_heads + hq] = lse_of(m[i] * cs[i], l[i]);
             }
             if (++c_seg == C::SEGS) c_seg = 0;
         }

@@ -547,11 +547,10 @@ __global__ void __launch_bounds__(Pre<T, D>::THREADS, 1) kv4_prefill_kernel(cons
                 for (int k = 2; k < 32; k += 2) t1 = fmaxf(t1, __uint_as_float(s[k])), t2 = fmaxf(t2, __uint_as_float(s[k + 1]));
                 top = fmaxf(top, fmaxf(t1, t2));
             }
-            top *= cs;
             // the reference of the weights follows the maximum when that is 2^LAG above it
-            const bool up = top > m + LAG;
+            const bool up = (top - m) * cs > LAG;
             if (__any_sync(~0u, up)) {
-                const float f = up ? ex2(m - top) : 1.0f;
+                const float f = up ? ex2((m - top) * cs) : 1.0f;
                 if (up) m = top, l *= f;
                 if (i) {
 #pragma unroll 1
@@ -566,7 +565,7 @@ __global__ void __launch_bounds__(Pre<T, D>::THREADS, 1) kv4_prefill_kernel(cons
                     }
                 }
             }
-            const float shift = m == -INFINITY ? 0.0f : P_SHIFT - m;
+            const float nm = m == -INFINITY ? 0.0f : -m;
             float l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
             for (int c = 0; c < NK; c += 32) {
@@ -576,7 +575,8 @@ __global__ void __launch_bounds__(Pre<T, D>::THREADS, 1) kv4_prefill_kernel(cons
                 masked(s, c);
 #pragma unroll
                 for (int k = 0; k < 32; k += 2) {
-                    const float p0 = ex2(fmaf(__uint_as_float(s[k]), cs, shift)), p1 = ex2(fmaf(__uint_as_float(s[k + 1]), cs, shift));
+                    const float2 t = kv4_exponents(__uint_as_float(s[k]), __uint_as_float(s[k + 1]), make_float2(nm, nm), make_float2(cs, cs), P_SHIFT);
+                    const float p0 = ex2(t.x), p1 = ex2(t.y);
                     l0 += p0, l1 += p1;
                     p[k / 2] = pack2(p0, p1);
                 }
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(Pre<T, D>::THREADS, 1) kv4_prefill_kernel(cons
                 }
             }
         }
-        if (live && a.lse) a.lse[t * a.n_heads + hq] = l == 0.0f ? -INFINITY : (m - P_SHIFT + log2f(l)) * LN2;
+        if (live && a.lse) a.lse[t * a.n_heads + hq] = l == 0.0f ? -INFINITY : (m * cs - P_SHIFT + log2f(l)) * LN2;
     }
     fence_before();
     __syncthreads();

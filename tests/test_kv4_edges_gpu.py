@@ -429,3 +429,29 @@ def test_attention_f16_many_rows_keeps_its_bits(dev, d, length, new):
                              scale, 0)
     off = ((out - want).norm() / want.norm()).item()
     assert off <= 2 ** 0.5 * 2.1e-4, off
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [1, 7, 900])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("big", [1.0, 30.0, 1000.0, 3e4])
+def test_attention_huge_scores(dev, dtype, new, d, big):
+    # keys of infinities (held as f16's largest numbers) and large queries: scores of 1e5 to 1e10, whose last f32 bit is
+    # worth more than a power of two of a weight.  The results are means of values all the same
+    heads, group, length = 4, 8, 1000
+    cache = sg.Kv4Cache(63, heads, d, 16, device=dev)
+    g = torch.Generator(device=dev).manual_seed(d + new)
+    k = torch.randn(length, heads, d, device=dev, generator=g)
+    k[::3] *= 2e4
+    k[5::50] = float("inf")
+    k[6::70] = -float("inf")
+    k[7::40, :, ::2] = float("inf")
+    v = torch.randn(length, heads, d, device=dev, generator=g)
+    sg.kv4_append(cache, k, v, torch.arange(length, dtype=torch.int32, device=dev))
+    tables = torch.arange(63, dtype=torch.int32, device=dev)[None]
+    q = (torch.randn(new, heads * group, d, device=dev, generator=g) * big).clamp(-65504, 65504).to(dtype)
+    lse = torch.empty(new, heads * group, device=dev)
+    out = sg.kv4_attention(cache, q, ints([0, new], dev), ints([length], dev), tables, lse=lse)
+    check(dev, cache, tables, tables.cpu(), ints([0, new], dev), ints([length], dev), q, d ** -0.5, 0, out, lse)
+    top = sg.kv4_read(cache, torch.arange(length, dtype=torch.int32, device=dev), dtype=torch.float32)[1].abs().amax()
+    assert (out.abs() <= top * 1.05).all()
