@@ -68,17 +68,6 @@ struct Kv4Codes {
     }
 };
 
-// The exponents of two weights in base 2, (s - m) scale + shift: the difference to the reference m first, which is exact
-// near the maximum, so that no weight passes its bound however large the scores.
-__device__ __forceinline__ float2 kv4_exponents(float s0, float s1, float2 minus_m, float2 scale, float shift) {
-    float2 d;
-    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 y, {%6, %7};\n"
-        " mov.b64 z, {%8, %8};\n fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(s0), "f"(s1), "f"(minus_m.x), "f"(minus_m.y), "f"(scale.x), "f"(scale.y), "f"(shift));
-    return d;
-}
-
 // A result in f16.  It is a mean of values that are finite in f16, so its true value is, but the weights' sum is 1 only up
 // to their rounding (2^-12 of it in the kernel for many rows): what that carries past the end of the range stays there.
 __device__ __forceinline__ __half kv4_f16(float v) {

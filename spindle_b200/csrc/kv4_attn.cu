@@ -719,8 +719,9 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1) kv4_attn_kernel(const _
             uint32_t ph[2], pl[2];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const float2 t = kv4_exponents(s[i][2 * j], s[i][2 * j + 1], make_float2(nm[0], nm[1]), make_float2(cs[0], cs[1]), P_SHIFT);
-                const float p0 = ex2(t.x), p1 = ex2(t.y);
+                // the difference to the reference first: exact near the maximum, so that no weight passes its bound however
+                // large the scores
+                const float p0 = ex2(fmaf(s[i][2 * j] + nm[0], cs[0], P_SHIFT)), p1 = ex2(fmaf(s[i][2 * j + 1] + nm[1], cs[1], P_SHIFT));
                 ls[0] = i + j ? ls[0] + p0 : p0, ls[1] = i + j ? ls[1] + p1 : p1;
                 ph[j] = pack_h2(p0, p1);
                 if constexpr (REST) {

@@ -141,6 +141,17 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// The exponents of two weights in base 2, (s - m) scale + shift: the difference to the reference m first, which is exact
+// near the maximum, so that no weight passes its bound however large the scores.
+__device__ __forceinline__ float2 exponents(float s0, float s1, float2 minus_m, float2 scale, float shift) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 y, {%6, %7};\n"
+        " mov.b64 z, {%8, %8};\n fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(s0), "f"(s1), "f"(minus_m.x), "f"(minus_m.y), "f"(scale.x), "f"(scale.y), "f"(shift));
+    return d;
+}
+
 template <typename T>
 __device__ __forceinline__ float to_f32(T v) {
     if constexpr (std::is_same<T, __half>::value) return __half2float(v);
@@ -575,7 +586,7 @@ __global__ void __launch_bounds__(Pre<T, D>::THREADS, 1) kv4_prefill_kernel(cons
                 masked(s, c);
 #pragma unroll
                 for (int k = 0; k < 32; k += 2) {
-                    const float2 t = kv4_exponents(__uint_as_float(s[k]), __uint_as_float(s[k + 1]), make_float2(nm, nm), make_float2(cs, cs), P_SHIFT);
+                    const float2 t = exponents(__uint_as_float(s[k]), __uint_as_float(s[k + 1]), make_float2(nm, nm), make_float2(cs, cs), P_SHIFT);
                     const float p0 = ex2(t.x), p1 = ex2(t.y);
                     l0 += p0, l1 += p1;
                     p[k / 2] = pack2(p0, p1);
