@@ -13,9 +13,9 @@
 // scratch, where the last CTA to arrive joins them, always in position order.
 //
 // Measured (device time): one token each of 64 requests of 2048 to 8192 positions, 32 query and 4 KV heads of 128,
-// bf16: 58 us, 3.7 TB/s (57 % of the measured copy rate); one request of 131071 positions, 32 and 8 heads, f16: 53
-// us, 3.2 TB/s; 1037 positions: 13 us; 16 requests of 9 tokens at 2050 positions in f32: 36 us.  What bounds it is
-// issuing instructions: by the counters 720 (bf16), 740 (f16) and 890 (f32) for 32 positions of eight rows, starts and
+// bf16: 59 us, 3.6 TB/s (56 % of the measured copy rate); one request of 131071 positions, 32 and 8 heads, f16: 54
+// us, 3.1 TB/s; 1037 positions: 13 us; 16 requests of 9 tokens at 2050 positions in f32: 36 us.  What bounds it is
+// issuing instructions: by the counters 730 (bf16), 750 (f16) and 890 (f32) for 32 positions of eight rows, starts and
 // joins included.  A call that has almost nothing to read (1037 positions) shows what starting and joining take.
 //
 // Arithmetic.  All products are m16n8k16 f16 tensor operations with f32 sums, the
