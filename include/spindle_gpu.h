@@ -52,7 +52,7 @@ typedef int32_t sg_status;
 #define SG_Q8_0 8
 #define SG_Q4_K 12
 #define SG_Q6_K 14
-#define SG_BF16 30 /* activations of the paged cache and log-probability calls only */
+#define SG_BF16 30 /* activations of the paged cache, log-probability and 4-bit matrix calls only */
 
 /* Weight layouts (sg_mat.layout).  GGUF: the file's rows, verbatim.
  * TILED16: the same bytes permuted once at upload by sg_repack_tiled16 so that
@@ -655,6 +655,86 @@ SG_API sg_status sg_kv4_attention(const sg_kv4 *c, const sg_kv4_attn *a, void *s
 SG_API sg_status sg_logprobs(int32_t type, const void *d_logits, uint64_t ld, uint64_t rows, uint64_t vocab,
                              const int32_t *d_tokens, float *d_logprob, float *d_entropy, int32_t *d_rank, uint64_t top,
                              int32_t *d_top_ids, float *d_top_logprobs, void *stream);
+
+/* ---- Microscaled 4-bit matrices, and tokens sorted by expert ---------------------
+ *
+ * A matrix that the tensor cores multiply as it is: 32 values along a row are
+ * c * 2^s, s of 8 bits and 32 codes c of 4 bits (sign, and one of 0 0.5 1 1.5 2 3 4
+ * 6), 17 bytes per 32 values.  s is floor(log2(top)) - 2 for the largest magnitude
+ * top, one more where top is 1.75 times a power of two or above, at least -127; codes
+ * are rounded to nearest, ties to the even code.  A group with an infinity or a NaN
+ * is NaN, all 32 values.  rms error of normally distributed values 11 % of their
+ * standard deviation.
+ *
+ * `experts` matrices of rows x cols (1: a plain matrix), cols a multiple of 32, in
+ * tiles of 128 rows by 256 columns (padded with zeros).  data: sg_mx4_bytes(m)
+ * device bytes, 16-byte aligned. */
+typedef struct {
+    uint64_t experts, rows, cols;
+    uint8_t *data;
+} sg_mx4;
+/* 0 for a shape that is not supported. */
+SG_API uint64_t sg_mx4_bytes(const sg_mx4 *m);
+/* Quantizes d_x (SG_F32, SG_F16 or SG_BF16), element (e, r, c) at d_x[e * ld_expert +
+ * r * ld + c]; sg_mx4_dequantize gives the values back the same way (rounded to
+ * f16 where they are f16). */
+SG_API sg_status sg_mx4_quantize(const sg_mx4 *m, int32_t type, const void *d_x, uint64_t ld, uint64_t ld_expert,
+                                 void *stream);
+SG_API sg_status sg_mx4_dequantize(const sg_mx4 *m, int32_t type, void *d_out, uint64_t ld, uint64_t ld_expert,
+                                   void *stream);
+
+/* out[t, n] = sum over k of q(x)[t, k] w[n, k] for n_tok rows of x, each quantized
+ * as above on the way, whatever their number; with `up` (a matrix of w's shape)
+ * silu(that) * (the same with up).  w has one expert.  Products are exact and added
+ * in f32; the results are rounded once, to out_type.
+ * d_scratch: sg_mx4_scratch_bytes(w, n_tok, NULL) bytes (0 is possible), 128-byte
+ * aligned, for calls that may overlap on the GPU one each. */
+typedef struct sg_moe_plan_ sg_moe_plan;
+SG_API uint64_t sg_mx4_scratch_bytes(const sg_mx4 *w, uint64_t n_tok, const sg_moe_plan *plan);
+SG_API sg_status sg_mx4_matmul(const sg_mx4 *w, const sg_mx4 *up, int32_t type, const void *d_x, uint64_t ldx, uint64_t n_tok,
+                               int32_t out_type, void *d_out, uint64_t ldo, void *d_scratch, uint64_t scratch_bytes,
+                               void *stream);
+
+/* Tokens sorted by expert: n_tok tokens of n_used choices among n_expert, a (token,
+ * choice) pair having the number token * n_used + choice.  All device memory of the
+ * caller's, written by sg_moe_route or sg_moe_sort and read by sg_mx4_experts and
+ * sg_moe_combine, which rely on what is written there:
+ *   ids, weights [n_tok * n_used]: the experts (-1: none) and their weights;
+ *   first [n_expert + 1]: the first sorted place of each expert;
+ *   order [n_tok * n_used]: the pair at each place, -1 past first[n_expert]; pairs of
+ *     one expert stand in rising order;
+ *   place [n_tok * n_used]: the place of each pair, -1 for none;
+ *   work: sg_moe_plan_work_bytes(n_tok, n_expert) bytes.
+ * n_used <= SG_MOE_MAX_USED, n_expert <= 1024, n_tok * n_used < 2^31. */
+struct sg_moe_plan_ {
+    uint64_t n_tok, n_used, n_expert;
+    int32_t *ids;
+    float *weights;
+    int32_t *first, *order, *place, *work;
+};
+SG_API uint64_t sg_moe_plan_work_bytes(uint64_t n_tok, uint64_t n_expert);
+/* The n_used largest of each token's n_expert logits (element (t, e) at d_logits[t *
+ * ld + e]), equal ones by rising number, and their softmax: over the chosen ones (norm)
+ * or over all.  prune as in sg_moe (applied to the chosen ones; those dropped are -1).
+ * A logit of minus infinity is never chosen: where fewer are left, the rest are -1 with
+ * weight 0.  A NaN counts as the largest and makes the token's weights NaN, as an
+ * infinity does.  sg_moe_sort takes ids and weights as they stand in the plan; ids
+ * outside 0..n_expert-1 become -1 with weight 0; a token may have an expert twice. */
+SG_API sg_status sg_moe_route(int32_t type, const void *d_logits, uint64_t ld, int32_t norm, float prune, const sg_moe_plan *plan,
+                              void *stream);
+SG_API sg_status sg_moe_sort(const sg_moe_plan *plan, void *stream);
+
+/* The products of each expert with its tokens: row s of out (rows = w->rows) is that of
+ * sorted place s.  w (and up, as in sg_mx4_matmul) has plan->n_expert experts.
+ * gather: d_x has a row per token; otherwise a row per sorted place.  Rows of out past
+ * first[n_expert] are left as they were.  d_scratch: sg_mx4_scratch_bytes(w, 0, plan). */
+SG_API sg_status sg_mx4_experts(const sg_mx4 *w, const sg_mx4 *up, const sg_moe_plan *plan, int32_t type, const void *d_x,
+                                uint64_t ldx, int32_t gather, int32_t out_type, void *d_out, uint64_t ldo,
+                                void *d_scratch, uint64_t scratch_bytes, void *stream);
+/* out[t] = sum over j of weights[t, j] * y[place[t, j]], dim columns, in f32 in the
+ * order of j and rounded once; zeros for a token without any. */
+SG_API sg_status sg_moe_combine(const sg_moe_plan *plan, int32_t type, const void *d_y, uint64_t ldy, uint64_t dim, int32_t out_type,
+                                void *d_out, uint64_t ldo, void *stream);
 
 /* ---- the reference's synthetic benchmark kernels ----------------------------
  * Prototypes driven by the reference's early benchmark (main.rs), not by its

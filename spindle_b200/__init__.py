@@ -13,7 +13,9 @@ Host-side mirror of the reference's kernel API (WiseHax/spindle 1.1.0, src/):
   moe_forward_batch        smollm_chat.rs:928-1174
 and, beyond the reference, what serving many requests needs (kv4.py): Kv4Cache,
 kv4_plan, kv4_append, kv4_read, kv4_attention (a paged KV cache in 4 bits) and
-logprobs.
+logprobs; and matrices that the tensor cores multiply in 4 bits (mx4.py): Mx4,
+mx4_quantize, mx4_dequantize, mx4_matmul, and for experts MoePlan, moe_route,
+moe_sort, mx4_experts, moe_combine.
 Every call goes through the C ABI of include/spindle_gpu.h (libspindle_b200.so);
 torch tensors are only the device-memory plumbing.  There is no CPU path: a
 missing library or a failed call raises.
@@ -437,3 +439,7 @@ def decode_choice(choice):
 # ---- paged 4-bit KV cache and token log probabilities (serving many requests)
 from .kv4 import (Kv4Cache, Kv4Plan, LogProbs, kv4_append, kv4_attention, kv4_attention_scratch, kv4_plan, kv4_read,  # noqa: E402,F401
                   logprobs)
+
+# ---- microscaled 4-bit matrices and experts' products on them
+from .mx4 import (MoePlan, Mx4, moe_combine, moe_route, moe_sort, mx4_dequantize, mx4_experts, mx4_matmul, mx4_quantize,  # noqa: E402,F401
+                  mx4_scratch)

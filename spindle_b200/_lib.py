@@ -77,6 +77,16 @@ class SgKv4Attn(C.Structure):
                 ("max_new", C.c_uint64), ("scratch", C.c_void_p), ("scratch_bytes", C.c_uint64)]
 
 
+class SgMx4(C.Structure):
+    _fields_ = [("experts", C.c_uint64), ("rows", C.c_uint64), ("cols", C.c_uint64), ("data", C.c_void_p)]
+
+
+class SgMoePlan(C.Structure):
+    _fields_ = [("n_tok", C.c_uint64), ("n_used", C.c_uint64), ("n_expert", C.c_uint64), ("ids", C.c_void_p),
+                ("weights", C.c_void_p), ("first", C.c_void_p), ("order", C.c_void_p), ("place", C.c_void_p),
+                ("work", C.c_void_p)]
+
+
 P, U64, I32 = C.c_void_p, C.c_uint64, C.c_int32
 
 # name -> (restype, argtypes); every function the header declares.
@@ -158,6 +168,16 @@ SIGNATURES = {
     "sg_kv4_attention_scratch_init": (I32, [P, U64, P]),
     "sg_kv4_attention": (I32, [C.POINTER(SgKv4), C.POINTER(SgKv4Attn), P]),
     "sg_logprobs": (I32, [I32, P, U64, U64, U64, P, P, P, P, U64, P, P, P]),
+    "sg_mx4_bytes": (U64, [C.POINTER(SgMx4)]),
+    "sg_mx4_quantize": (I32, [C.POINTER(SgMx4), I32, P, U64, U64, P]),
+    "sg_mx4_dequantize": (I32, [C.POINTER(SgMx4), I32, P, U64, U64, P]),
+    "sg_mx4_scratch_bytes": (U64, [C.POINTER(SgMx4), U64, C.POINTER(SgMoePlan)]),
+    "sg_mx4_matmul": (I32, [C.POINTER(SgMx4), C.POINTER(SgMx4), I32, P, U64, U64, I32, P, U64, P, U64, P]),
+    "sg_moe_plan_work_bytes": (U64, [U64, U64]),
+    "sg_moe_route": (I32, [I32, P, U64, I32, C.c_float, C.POINTER(SgMoePlan), P]),
+    "sg_moe_sort": (I32, [C.POINTER(SgMoePlan), P]),
+    "sg_mx4_experts": (I32, [C.POINTER(SgMx4), C.POINTER(SgMx4), C.POINTER(SgMoePlan), I32, P, U64, I32, I32, P, U64, P, U64, P]),
+    "sg_moe_combine": (I32, [C.POINTER(SgMoePlan), I32, P, U64, U64, I32, P, U64, P]),
     "sg_forward_batch": (I32, [P, P, U64, P, P, P, U64, U64, P, U64, P, P]),
 }
 

@@ -16,6 +16,7 @@
 #include "kernels.cuh"
 #include "kv4.cuh"
 #include "logprobs.cuh"
+#include "mx4.cuh"
 #include "moe.cuh"
 #include "decode.cuh"
 #include "gemv_float.cuh"
@@ -2578,6 +2579,209 @@ sg_status sg_logprobs(int32_t type, const void *d_logits, uint64_t ld, uint64_t 
     cudaError_t e = cudaSuccess;
     sg_status st = logprobs_launch(a, type, di->sms, (cudaStream_t)stream, &e);
     return st == SG_ERR_CUDA ? cuda_fail(e, "logprobs") : st;
+}
+
+}  // extern "C"
+
+// ---- microscaled 4-bit matrices, tokens sorted by expert --------------------------
+
+namespace {
+
+sg_status check_mx4(const sg_mx4 *m, bool data) {
+    if (!m) return SG_ERR_INVALID;
+    if (!m->experts || !m->rows || !m->cols || m->cols % 32 || m->cols >= 1ull << 31 || m->rows >= 1ull << 31 || m->experts >= 1ull << 31)
+        return SG_ERR_SHAPE;
+    // (rows of all tiles in 31 bits, bytes in 63)
+    if (m->experts * align_up(m->rows, MX4_ROWS) >= 1ull << 31) return SG_ERR_SHAPE;
+    if (!data) return SG_OK;
+    if (!m->data) return SG_ERR_INVALID;
+    return aligned(m->data, 16) ? SG_OK : SG_ERR_ALIGN;
+}
+
+uint32_t mx4_nk(const sg_mx4 *m) { return (uint32_t)((m->cols + MX4_COLS - 1) / MX4_COLS); }
+uint64_t mx4_expert_bytes(const sg_mx4 *m) { return align_up(m->rows, MX4_ROWS) / MX4_ROWS * mx4_nk(m) * MX4_TILE; }
+// rows of cols elements ld apart: whether every eight of them are 16-byte aligned
+bool rows16(const void *p, uint64_t ld, uint32_t es) { return aligned(p, 16) && !(ld & (16 / es - 1)); }
+
+sg_status check_plan(const sg_moe_plan *p) {
+    if (!p) return SG_ERR_INVALID;
+    if (!p->n_used || p->n_used > MOE_SORT_MAX_USED || !p->n_expert || p->n_expert > MOE_SORT_MAX_EXPERTS) return SG_ERR_SHAPE;
+    if (p->n_tok >= 1ull << 31 || p->n_tok * p->n_used >= 1ull << 31) return SG_ERR_SHAPE;
+    if (!p->first || !p->work || (p->n_tok && (!p->ids || !p->weights || !p->order || !p->place))) return SG_ERR_INVALID;
+    return SG_OK;
+}
+// CTAs that sort: a stretch of 64 tokens or more each
+uint32_t sort_ctas(uint64_t n_tok) {
+    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(128, (n_tok + MOE_SORT_TOKENS - 1) / MOE_SORT_TOKENS));
+}
+// plan->work: first tiles for tiles of 32, 64 and 128 rows, then the stretches' counts
+int32_t *plan_tiles(const sg_moe_plan *p, uint32_t shift) { return p->work + (shift - 5) * (p->n_expert + 1); }
+
+// How a product of n_tok rows is run: rows of x a tile, tiles of x, tiles of tokens (of experts: at most that many).
+struct Mx4Plan {
+    uint32_t shift;
+    uint64_t x_tiles, token_tiles;
+};
+Mx4Plan mx4_plan(uint64_t n_tok, const sg_moe_plan *plan) {
+    const uint64_t pairs = plan ? plan->n_tok * plan->n_used : n_tok, groups = plan ? std::min(plan->n_expert, pairs) : 1;
+    if (!pairs) return {5, 0, 0};
+    const uint32_t shift = pairs / groups <= 32 ? 5 : 7;
+    const uint64_t rows = 1ull << shift, tiles = (pairs + groups * (rows - 1)) / rows;
+    return {shift, tiles, tiles};
+}
+uint64_t mx4_scratch(const sg_mx4 *w, const Mx4Plan &p) { return p.x_tiles * mx4_nk(w) * mx4_tile_bytes(1u << p.shift); }
+
+// What matmul and experts have in common: the quantized rows of x, then the products.
+sg_status mx4_product(const sg_mx4 *w, const sg_mx4 *up, const sg_moe_plan *plan, bool gather, int32_t type, const void *d_x, uint64_t ldx,
+                      uint64_t n_tok, int32_t out_type, void *d_out, uint64_t ldo, void *d_scratch, uint64_t scratch_bytes, cudaStream_t s) {
+    const uint32_t es = act_bytes(type), eo = act_bytes(out_type);
+    if (!es || !eo) return SG_ERR_DTYPE;
+    if (!plan && n_tok >= 1ull << 31) return SG_ERR_INVALID;
+    const uint64_t pairs = plan ? plan->n_tok * plan->n_used : n_tok;
+    if (!pairs) return SG_OK;
+    const uint64_t x_rows = plan ? (gather ? plan->n_tok : pairs) : n_tok;
+    if (!d_x || !d_out || (x_rows > 1 && ldx < w->cols) || (pairs > 1 && ldo < w->rows)) return SG_ERR_INVALID;
+    const Mx4Plan mp = mx4_plan(n_tok, plan);
+    if (!d_scratch || scratch_bytes < mx4_scratch(w, mp)) return SG_ERR_INVALID;
+    if (!aligned(d_x, es) || !aligned(d_out, eo) || !aligned(d_scratch, 128)) return SG_ERR_ALIGN;
+    DevInfo *di;
+    if (sg_status st = dev_info(&di)) return st;
+    const uint32_t nk = mx4_nk(w), feat_tiles = (uint32_t)(align_up(w->rows, MX4_ROWS) / MX4_ROWS);
+    if (mp.token_tiles * feat_tiles >= 1ull << 27) return SG_ERR_SHAPE;  // (CTAs of a launch, eight a tile at most)
+    Mx4QuantArgs q = {};
+    q.x = d_x, q.ld = ldx, q.out = (uint8_t *)d_scratch;
+    q.cols = (uint32_t)w->cols, q.nk = nk, q.tile_shift = mp.shift, q.n_rows = x_rows;
+    q.rows = (uint32_t)x_rows, q.tile_rows = (uint32_t)x_rows;
+    q.vec = rows16(d_x, ldx, es);
+    Mx4GemmArgs g = {};
+    g.w = w->data, g.up = up ? up->data : nullptr, g.x = (const uint8_t *)d_scratch;
+    g.out = d_out, g.ldo = ldo, g.expert_bytes = mx4_expert_bytes(w), g.type = out_type;
+    g.feats = (uint32_t)w->rows, g.nk = nk, g.feat_tiles = feat_tiles, g.n_tok = n_tok;
+    if (plan) {
+        q.n_used = (uint32_t)plan->n_used, q.ids = plan->ids, q.place = plan->place, q.order = gather ? nullptr : plan->order;
+        q.first = g.first = plan->first, q.tiles = g.tiles = plan_tiles(plan, mp.shift);
+        g.n_expert = (uint32_t)plan->n_expert;
+    }
+    CK(mx4_quantize_launch(q, type, di->sms, s));
+    CK(mx4_gemm_launch(g, mp.shift, mp.token_tiles, di->sms, s));
+    return SG_OK;
+}
+
+sg_status check_product(const sg_mx4 *w, const sg_mx4 *up, uint64_t experts) {
+    if (sg_status st = check_mx4(w, true)) return st;
+    if (w->experts != experts) return SG_ERR_SHAPE;
+    if (!up) return SG_OK;
+    if (sg_status st = check_mx4(up, true)) return st;
+    return up->experts == w->experts && up->rows == w->rows && up->cols == w->cols ? SG_OK : SG_ERR_SHAPE;
+}
+
+MoeSortArgs sort_args(const sg_moe_plan *p) {
+    MoeSortArgs a = {};
+    a.n_tok = (uint32_t)p->n_tok, a.n_expert = (uint32_t)p->n_expert, a.n_used = (uint32_t)p->n_used, a.ctas = sort_ctas(p->n_tok);
+    a.ids = p->ids, a.weights = p->weights, a.first = p->first, a.order = p->order, a.place = p->place;
+    a.tiles = p->work, a.counts = p->work + 3 * (p->n_expert + 1);
+    return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t sg_mx4_bytes(const sg_mx4 *m) { return check_mx4(m, false) ? 0 : m->experts * mx4_expert_bytes(m); }
+
+sg_status sg_mx4_quantize(const sg_mx4 *m, int32_t type, const void *d_x, uint64_t ld, uint64_t ld_expert, void *stream) {
+    if (sg_status st = check_mx4(m, true)) return st;
+    const uint32_t es = act_bytes(type);
+    if (!es) return SG_ERR_DTYPE;
+    if (!d_x || (m->rows > 1 && ld < m->cols)) return SG_ERR_INVALID;
+    if (!aligned(d_x, es)) return SG_ERR_ALIGN;
+    DevInfo *di;
+    if (sg_status st = dev_info(&di)) return st;
+    Mx4QuantArgs q = {};
+    q.x = d_x, q.ld = ld, q.ld_expert = ld_expert, q.out = m->data;
+    q.cols = (uint32_t)m->cols, q.nk = mx4_nk(m), q.tile_shift = 7;
+    q.rows = (uint32_t)m->rows, q.tile_rows = (uint32_t)align_up(m->rows, MX4_ROWS);
+    q.n_rows = m->experts * q.tile_rows;
+    q.vec = rows16(d_x, m->rows > 1 ? ld : 0, es) && (m->experts == 1 || rows16(d_x, ld_expert, es));
+    CK(mx4_quantize_launch(q, type, di->sms, (cudaStream_t)stream));
+    return SG_OK;
+}
+
+sg_status sg_mx4_dequantize(const sg_mx4 *m, int32_t type, void *d_out, uint64_t ld, uint64_t ld_expert, void *stream) {
+    if (sg_status st = check_mx4(m, true)) return st;
+    const uint32_t es = act_bytes(type);
+    if (!es) return SG_ERR_DTYPE;
+    if (!d_out || (m->rows > 1 && ld < m->cols)) return SG_ERR_INVALID;
+    if (!aligned(d_out, es)) return SG_ERR_ALIGN;
+    DevInfo *di;
+    if (sg_status st = dev_info(&di)) return st;
+    Mx4ReadArgs r = {m->data, d_out, ld, ld_expert, (uint32_t)m->rows, (uint32_t)m->cols, mx4_nk(m),
+                     (uint32_t)align_up(m->rows, MX4_ROWS), m->experts * m->rows,
+                     rows16(d_out, m->rows > 1 ? ld : 0, es) && (m->experts == 1 || rows16(d_out, ld_expert, es))};
+    CK(mx4_dequantize_launch(r, type, di->sms, (cudaStream_t)stream));
+    return SG_OK;
+}
+
+uint64_t sg_mx4_scratch_bytes(const sg_mx4 *w, uint64_t n_tok, const sg_moe_plan *plan) {
+    if (check_mx4(w, false) || n_tok >= 1ull << 31) return 0;
+    if (plan && (!plan->n_used || !plan->n_expert || plan->n_tok >= 1ull << 31 || plan->n_used > MOE_SORT_MAX_USED)) return 0;
+    return mx4_scratch(w, mx4_plan(n_tok, plan));
+}
+
+sg_status sg_mx4_matmul(const sg_mx4 *w, const sg_mx4 *up, int32_t type, const void *d_x, uint64_t ldx, uint64_t n_tok, int32_t out_type,
+                        void *d_out, uint64_t ldo, void *d_scratch, uint64_t scratch_bytes, void *stream) {
+    if (sg_status st = check_product(w, up, 1)) return st;
+    return mx4_product(w, up, nullptr, false, type, d_x, ldx, n_tok, out_type, d_out, ldo, d_scratch, scratch_bytes, (cudaStream_t)stream);
+}
+
+uint64_t sg_moe_plan_work_bytes(uint64_t n_tok, uint64_t n_expert) {
+    if (!n_expert || n_expert > MOE_SORT_MAX_EXPERTS || n_tok >= 1ull << 31) return 0;
+    const uint32_t ctas = sort_ctas(n_tok);
+    return 4 * (3 * (n_expert + 1) + (ctas > 1 ? ctas * n_expert : 0));
+}
+
+sg_status sg_moe_route(int32_t type, const void *d_logits, uint64_t ld, int32_t norm, float prune, const sg_moe_plan *plan, void *stream) {
+    if (sg_status st = check_plan(plan)) return st;
+    const uint32_t es = act_bytes(type);
+    if (!es) return SG_ERR_DTYPE;
+    if (plan->n_tok && !d_logits) return SG_ERR_INVALID;
+    if (plan->n_tok > 1 && ld < plan->n_expert) return SG_ERR_INVALID;
+    if (!aligned(d_logits, es)) return SG_ERR_ALIGN;
+    MoeSortArgs a = sort_args(plan);
+    a.logits = plan->n_tok ? d_logits : nullptr, a.ld = ld, a.norm = norm, a.prune = prune;
+    CK(moe_sort_launch(a, type, (cudaStream_t)stream));
+    return SG_OK;
+}
+
+sg_status sg_moe_sort(const sg_moe_plan *plan, void *stream) {
+    if (sg_status st = check_plan(plan)) return st;
+    CK(moe_sort_launch(sort_args(plan), SG_F32, (cudaStream_t)stream));
+    return SG_OK;
+}
+
+sg_status sg_mx4_experts(const sg_mx4 *w, const sg_mx4 *up, const sg_moe_plan *plan, int32_t type, const void *d_x, uint64_t ldx,
+                         int32_t gather, int32_t out_type, void *d_out, uint64_t ldo, void *d_scratch, uint64_t scratch_bytes, void *stream) {
+    if (sg_status st = check_plan(plan)) return st;
+    if (sg_status st = check_product(w, up, plan->n_expert)) return st;
+    return mx4_product(w, up, plan, gather != 0, type, d_x, ldx, 0, out_type, d_out, ldo, d_scratch, scratch_bytes, (cudaStream_t)stream);
+}
+
+sg_status sg_moe_combine(const sg_moe_plan *plan, int32_t type, const void *d_y, uint64_t ldy, uint64_t dim, int32_t out_type, void *d_out,
+                         uint64_t ldo, void *stream) {
+    if (sg_status st = check_plan(plan)) return st;
+    const uint32_t es = act_bytes(type), eo = act_bytes(out_type);
+    if (!es || !eo) return SG_ERR_DTYPE;
+    if (!dim || dim >= 1ull << 31) return SG_ERR_SHAPE;
+    if (!plan->n_tok) return SG_OK;
+    const uint64_t pairs = plan->n_tok * plan->n_used;
+    if (!d_y || !d_out || (pairs > 1 && ldy < dim) || (plan->n_tok > 1 && ldo < dim)) return SG_ERR_INVALID;
+    if (!aligned(d_y, es) || !aligned(d_out, eo)) return SG_ERR_ALIGN;
+    DevInfo *di;
+    if (sg_status st = dev_info(&di)) return st;
+    const MoeCombineArgs a = {d_y, ldy, ldo, d_out, plan->place, plan->weights, plan->n_tok, (uint32_t)plan->n_used, (uint32_t)dim,
+                              (uint32_t)pairs, dim % 8 == 0 && rows16(d_y, ldy, es) && rows16(d_out, ldo, eo)};
+    CK(moe_combine_launch(a, type, out_type, di->sms, (cudaStream_t)stream));
+    return SG_OK;
 }
 
 }  // extern "C"
