@@ -2663,7 +2663,8 @@ sg_status mx4_product(const sg_mx4 *w, const sg_mx4 *up, const sg_moe_plan *plan
         g.n_expert = (uint32_t)plan->n_expert;
     }
     CK(mx4_quantize_launch(q, type, di->sms, s));
-    CK(mx4_gemm_launch(g, mp.shift, mp.token_tiles, di->sms, s));
+    g.vec = rows16(d_out, ldo, eo);
+    CK(mp.shift == 7 ? mx4_many_launch(g, mp.token_tiles, di->sms, s) : mx4_gemm_launch(g, mp.shift, mp.token_tiles, di->sms, s));
     return SG_OK;
 }
 

@@ -76,7 +76,9 @@ struct Mx4GemmArgs {
     uint64_t n_tok;                // rows of x, where they are one matrix
     const int32_t *first, *tiles;  // experts: the first sorted place of each, its first tile of x (n_expert + 1 each)
     uint32_t n_expert;
+    bool vec;                      // out allows 16-byte stores of eight features
 };
+cudaError_t mx4_many_launch(const Mx4GemmArgs &a, uint64_t token_tiles, int sms, cudaStream_t s);
 cudaError_t mx4_gemm_launch(const Mx4GemmArgs &a, uint32_t tile_shift, uint64_t token_tiles, int sms, cudaStream_t s);
 
 // The choice of experts and the sorting of its pairs.

@@ -10,15 +10,13 @@
 // tiles are fewer than the SMs, the CTAs of a cluster share a tile's columns and add their sums
 // over distributed shared memory, in rank order.
 #include <cooperative_groups.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
-#include "mx4.cuh"
-#include "tiled_block.cuh"
+#include "mx4_tc.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace sg {
+using namespace mx4;
 using namespace tiled;
 
 namespace {
@@ -44,52 +42,6 @@ struct Cfg {
     static_assert(WANT <= 512 && STAGES >= 2, "TMEM");
     static_assert((STAGES * STAGE) >= (DUAL ? 2 : 1) * 128 * (NT < 128 ? NT : 1) * 4, "partial sums");
 };
-
-// K-major operand, 128-byte swizzle: groups of 8 rows 1024 bytes apart, version 1 (bits 46-47), layout 2 (61-63).
-__device__ __forceinline__ uint64_t desc_operand(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-// Scales, no swizzle: groups of 8 rows of 16 bytes, 128 bytes apart.
-__device__ __forceinline__ uint64_t desc_scales(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(128u >> 4) << 32) | (1ull << 46);
-}
-// kind::mxf4: E2M1 x E2M1 (bits 7-9, 10-12 = 1), N >> 3 at bit 17, scales UE8M0 (bit 23), M >> 4 at bit 24; the half of a
-// scale word's four bytes at bits 29-30 (w) and 4-5 (x).
-__device__ __forceinline__ uint32_t idesc(uint32_t n, uint32_t half) {
-    return (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24) | ((2 * half) << 29) | ((2 * half) << 4);
-}
-__device__ __forceinline__ void mma(uint32_t d, uint64_t w, uint64_t x, uint32_t id, uint32_t sw, uint32_t sx, uint32_t add) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
-        "l"(w), "l"(x), "r"(id), "r"(sw), "r"(sx), "r"(add)
-        : "memory");
-}
-// 32 rows of 16 bytes to four columns of all 128 lanes
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t saddr) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc_scales(saddr)) : "memory");
-}
-__device__ __forceinline__ void commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// 16 columns of this thread's lane
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(addr)
-        : "memory");
-#pragma unroll
-    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
-}
-
-__device__ __forceinline__ float silu_times(float g, float u) { return g / (1.0f + expf(-g)) * u; }
 
 // A result of feature f of row t
 __device__ __forceinline__ void put(const Mx4GemmArgs &a, uint64_t t, uint32_t f, float v) {
@@ -158,8 +110,7 @@ __global__ void __launch_bounds__(THREADS) mx4_gemm_kernel(const __grid_constant
         fence_mbar_init();
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(C::COLS) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tmem_alloc<1>(slot, C::COLS);
     }
     fence_before();
     __syncthreads();
@@ -208,23 +159,23 @@ __global__ void __launch_bounds__(THREADS) mx4_gemm_kernel(const __grid_constant
             const uint32_t st = smem_u32(smem + HDR + s * C::STAGE), sc = tmem + C::SUMS + s * C::SC, sx = sc + 8 * (DUAL ? 2 : 1);
 #pragma unroll
             for (uint32_t h = 0; h < 2; h++) {
-                copy_scales(sc + 4 * h, st + MX4_ROWS * 128 + 512 * h);
-                if (DUAL) copy_scales(sc + 8 + 4 * h, st + MX4_TILE + MX4_ROWS * 128 + 512 * h);
+                copy_scales<1>(sc + 4 * h, st + MX4_ROWS * 128 + 512 * h);
+                if (DUAL) copy_scales<1>(sc + 8 + 4 * h, st + MX4_TILE + MX4_ROWS * 128 + 512 * h);
 #pragma unroll
                 for (uint32_t t = 0; t < C::XT; t++)
-                    copy_scales(sx + 4 * C::XT * h + 4 * t, st + C::W_BYTES + NT * 128 + t * MX4_SCALES + 512 * h);
+                    copy_scales<1>(sx + 4 * C::XT * h + 4 * t, st + C::W_BYTES + NT * 128 + t * MX4_SCALES + 512 * h);
             }
             // a product has 64 columns: 32 bytes of a row, half of a word of four scales
 #pragma unroll
             for (uint32_t q = 0; q < 4; q++) {
-                const uint32_t h = q >> 1, id = idesc(n, q & 1), add = i > 0 || q > 0;
+                const uint32_t h = q >> 1, id = idesc(128, n, q & 1), add = i > 0 || q > 0;
                 const uint64_t x = desc_operand(st + C::W_BYTES + 32 * q);
-                mma(tmem, desc_operand(st + 32 * q), x, id, sc + 4 * h, sx + 4 * C::XT * h, add);
-                if (DUAL) mma(tmem + NT, desc_operand(st + MX4_TILE + 32 * q), x, id, sc + 8 + 4 * h, sx + 4 * C::XT * h, add);
+                mma<1>(tmem, desc_operand(st + 32 * q), x, id, sc + 4 * h, sx + 4 * C::XT * h, add);
+                if (DUAL) mma<1>(tmem + NT, desc_operand(st + MX4_TILE + 32 * q), x, id, sc + 8 + 4 * h, sx + 4 * C::XT * h, add);
             }
-            commit(&empty[s]);
+            commit<1>(&empty[s]);
         }
-        if (ok) commit(done);
+        if (ok) commit<1>(done);
     }
     if (warp >= 2) {
         ok = mbar_wait_bounded(done, 0, 2 * WAIT_LIMIT_NS);
@@ -279,7 +230,7 @@ __global__ void __launch_bounds__(THREADS) mx4_gemm_kernel(const __grid_constant
     __syncthreads();
     if (warp == 1) {
         fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLS) : "memory");
+        tmem_free<1>(tmem, C::COLS);
     }
 }
 
