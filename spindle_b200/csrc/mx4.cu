@@ -19,20 +19,23 @@ template <> __device__ __forceinline__ float narrow<float>(float v) { return v; 
 template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Eight values of a row from column c on.
+// Eight values of a row, as they are loaded and as numbers.
+template <typename T>
+struct Raw {
+    uint4 w[8 * sizeof(T) / 16];
+};
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
+__device__ __forceinline__ void load8(const T *p, bool there, Raw<T> &r) {
+#pragma unroll
+    for (uint32_t i = 0; i < 8 * sizeof(T) / 16; i++) r.w[i] = make_uint4(0, 0, 0, 0);
+    if (!there) return;
     if constexpr (VEC) {
-        constexpr int N = 16 / sizeof(T);
-        uint4 w[8 / N];
 #pragma unroll
-        for (int i = 0; i < 8 / N; i++) w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
-        const T *t = reinterpret_cast<const T *>(w);
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = widen(t[i]);
+        for (uint32_t i = 0; i < 8 * sizeof(T) / 16; i++) r.w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
     } else {
+        T *t = reinterpret_cast<T *>(r.w);
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = widen(p[i]);
+        for (int i = 0; i < 8; i++) t[i] = p[i];
     }
 }
 
@@ -49,122 +52,154 @@ __device__ __forceinline__ uint32_t codes8(const float (&y)[8]) {
 }
 
 // Four lanes have the 32 values of a block: each gets its eight codes, all its scale byte.
-__device__ __forceinline__ uint32_t quantize8(const float (&v)[8], uint32_t &scale) {
+template <typename T>
+__device__ __forceinline__ uint32_t quantize8(const Raw<T> &raw, uint32_t &scale) {
+    const T *t = reinterpret_cast<const T *>(raw.w);
+    float v[8];
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);  // an infinity or a NaN: the largest
+    for (int i = 0; i < 8; i++) {
+        v[i] = widen(t[i]);
+        top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);  // an infinity or a NaN: the largest
+    }
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     // the exponent of the largest, one more from 1.75 times a power of two on, less 2
     const int e = max((int)((top + 0x200000u) >> 23) - 2, 0);
-    const bool bad = top >= 0x7F800000u;
-    scale = bad ? 255u : (uint32_t)e;
-    const float f = __uint_as_float((uint32_t)(254 - e) << 23);  // 2^(127 - e), e at most 253
-    float y[8];
+    scale = top >= 0x7F800000u ? 255u : (uint32_t)e;              // (all 32 are NaN then, whatever their codes)
+    const float f = __uint_as_float((uint32_t)(254 - e) << 23);  // 2^(127 - e), e at most 254
 #pragma unroll
-    for (int i = 0; i < 8; i++) y[i] = bad ? 0.0f : v[i] * f;
-    return codes8(y);
+    for (int i = 0; i < 8; i++) v[i] *= f;
+    return codes8(v);
 }
 
-// Where a quantized row goes: its tiles along the columns and its place in them.
-struct Dest {
-    uint8_t *tile;
-    uint32_t row;
-};
+// A warp takes 1024 columns of a row: its lanes eight values of each of four tiles, all loads at once, four lanes a block of
+// 32.  What bounds it: instructions (about 90 for a lane's eight values) next to reading x; a token that goes to several
+// experts is read and quantized once.
+constexpr uint32_t QUANT_TILES = 4;
 
-// A warp takes a row's 256 columns of a tile: four lanes a block of 32.  What bounds it: reading x (and, where a token goes
-// to several experts, writing its copies; it is read and quantized once for all of them).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(MX4_QUANT_THREADS) mx4_quantize_kernel(const __grid_constant__ Mx4QuantArgs a) {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, chunk = lane >> 2;
-    const uint64_t items = a.n_rows * a.nk, step = (uint64_t)gridDim.x * (MX4_QUANT_THREADS / 32);
-    const uint32_t tile_bytes = mx4_tile_bytes(1u << a.tile_shift), mask = (1u << a.tile_shift) - 1;
-    for (uint64_t at = (uint64_t)blockIdx.x * (MX4_QUANT_THREADS / 32) + warp; at < items; at += step) {
-        const uint64_t i = at / a.nk;
-        const uint32_t kt = (uint32_t)(at - i * a.nk), col = kt * MX4_COLS + lane * 8;
-        const T *src = static_cast<const T *>(a.x);
-        bool there = col < a.cols;
-        if (a.n_used) src += i * a.ld;
-        else {
-            const uint64_t e = i / a.tile_rows, r = i - e * a.tile_rows;
-            src += e * a.ld_expert + r * a.ld;
-            there = there && r < a.rows;
-        }
-        float v[8] = {};
-        if (there) load8<T, VEC>(src + col, v);
-        uint32_t scale;
-        const uint32_t w = quantize8(v, scale);
-        // the scale bytes of four blocks make a word
-        uint32_t s4 = (there ? scale : 0u) << (8 * (chunk & 3));
-        s4 |= __shfl_xor_sync(0xffffffffu, s4, 4);
-        s4 |= __shfl_xor_sync(0xffffffffu, s4, 8);
-        auto put = [&](uint64_t row) {
-            uint8_t *t = a.out + ((row >> a.tile_shift) * a.nk + kt) * tile_bytes;
-            const uint32_t r = (uint32_t)row & mask;
-            *reinterpret_cast<uint32_t *>(t + mx4_code_at(r, chunk) + 4 * (lane & 3)) = w;
-            if ((lane & 15) == 0) *reinterpret_cast<uint32_t *>(t + (mask + 1) * 128 + mx4_scale_at(r, chunk)) = s4;
-        };
-        if (!a.n_used) put(i);
-        else if (a.order) {
-            const int32_t pair = __ldg(a.order + i);
-            if (pair >= 0) {
-                const int32_t e = __ldg(a.ids + pair);
-                put(((uint64_t)__ldg(a.tiles + e) << a.tile_shift) + (i - __ldg(a.first + e)));
+    const uint32_t tile_bytes = mx4_tile_bytes(1u << a.tile_shift), mask = (1u << a.tile_shift) - 1, rows_at_once = gridDim.x * (MX4_QUANT_THREADS / 32);
+    for (uint32_t kt0 = blockIdx.y * QUANT_TILES; kt0 < a.nk; kt0 += gridDim.y * QUANT_TILES)
+        for (uint64_t i = blockIdx.x * (MX4_QUANT_THREADS / 32) + warp; i < a.n_rows; i += rows_at_once) {
+            const T *src = static_cast<const T *>(a.x);
+            bool row_there = true;
+            if (a.n_used) src += i * a.ld;
+            else {
+                const uint32_t e = (uint32_t)i / a.tile_rows, r = (uint32_t)i - e * a.tile_rows;
+                src += e * a.ld_expert + r * a.ld;
+                row_there = r < a.rows;
             }
-        } else {
-            for (uint32_t j = 0; j < a.n_used; j++) {
-                const uint64_t pair = i * a.n_used + j;
-                const int32_t p = __ldg(a.place + pair);
-                if (p < 0) continue;
-                const int32_t e = __ldg(a.ids + pair);
-                put(((uint64_t)__ldg(a.tiles + e) << a.tile_shift) + (p - __ldg(a.first + e)));
+            Raw<T> raw[QUANT_TILES];
+#pragma unroll
+            for (uint32_t u = 0; u < QUANT_TILES; u++) {
+                const uint32_t col = (kt0 + u) * MX4_COLS + lane * 8;
+                load8<T, VEC>(src + col, row_there && col < a.cols, raw[u]);
+            }
+            uint32_t w[QUANT_TILES], s4[QUANT_TILES];
+#pragma unroll
+            for (uint32_t u = 0; u < QUANT_TILES; u++) {
+                uint32_t scale;
+                w[u] = quantize8(raw[u], scale);
+                // the scale bytes of four blocks make a word
+                const bool there = row_there && (kt0 + u) * MX4_COLS + lane * 8 < a.cols;
+                s4[u] = (there ? scale : 0u) << (8 * (chunk & 3));
+                s4[u] |= __shfl_xor_sync(0xffffffffu, s4[u], 4);
+                s4[u] |= __shfl_xor_sync(0xffffffffu, s4[u], 8);
+            }
+            auto put = [&](uint64_t row) {
+                uint8_t *t = a.out + ((row >> a.tile_shift) * a.nk + kt0) * tile_bytes;
+                const uint32_t r = (uint32_t)row & mask, code_at = mx4_code_at(r, chunk) + 4 * (lane & 3);
+                const uint32_t scale_at = (mask + 1) * 128 + mx4_scale_at(r, chunk);
+#pragma unroll
+                for (uint32_t u = 0; u < QUANT_TILES; u++) {
+                    if (kt0 + u >= a.nk) break;
+                    *reinterpret_cast<uint32_t *>(t + u * tile_bytes + code_at) = w[u];
+                    if ((lane & 15) == 0) *reinterpret_cast<uint32_t *>(t + u * tile_bytes + scale_at) = s4[u];
+                }
+            };
+            if (!a.n_used) put(i);
+            else if (a.order) {
+                const int32_t pair = __ldg(a.order + i);
+                if (pair >= 0) {
+                    const int32_t e = __ldg(a.ids + pair);
+                    put(((uint64_t)__ldg(a.tiles + e) << a.tile_shift) + (i - __ldg(a.first + e)));
+                }
+            } else {
+                // (lane j looks the j-th place up)
+                int64_t row = -1;
+                if (lane < a.n_used) {
+                    const int32_t p = __ldg(a.place + i * a.n_used + lane);
+                    if (p >= 0) {
+                        const int32_t e = __ldg(a.ids + i * a.n_used + lane);
+                        row = ((int64_t)__ldg(a.tiles + e) << a.tile_shift) + (p - __ldg(a.first + e));
+                    }
+                }
+                for (uint32_t j = 0; j < a.n_used; j++) {
+                    const int64_t to = __shfl_sync(0xffffffffu, row, j);
+                    if (to >= 0) put(to);
+                }
             }
         }
-    }
     grid_launch_dependents();
 }
 
-// The value of a code's 4 bits.
-__device__ __forceinline__ float code_value(uint32_t c) {
-    const uint32_t m = c & 7;
-    // 0 and 0.5 below the first exponent, then 1 + the last bit's half
-    const float v = m < 2 ? 0.5f * m : __uint_as_float((126u + (m >> 1)) << 23 | (m & 1) << 22);
-    return c & 8 ? -v : v;
+// The values of two codes.
+__device__ __forceinline__ float2 values2(uint32_t byte) {
+    uint32_t h;
+    asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %1;\n cvt.rn.f16x2.e2m1x2 %0, a;\n}" : "=r"(h) : "r"(byte));
+    return __half22float2(*reinterpret_cast<const __half2 *>(&h));
 }
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(MX4_QUANT_THREADS) mx4_dequantize_kernel(const __grid_constant__ Mx4ReadArgs a) {
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, chunk = lane >> 2;
-    const uint64_t items = a.n_rows * a.nk, step = (uint64_t)gridDim.x * (MX4_QUANT_THREADS / 32);
-    for (uint64_t at = (uint64_t)blockIdx.x * (MX4_QUANT_THREADS / 32) + warp; at < items; at += step) {
-        const uint64_t i = at / a.nk, e = i / a.rows, r = i - e * a.rows, row = e * a.tile_rows + r;
-        const uint32_t kt = (uint32_t)(at - i * a.nk), col = kt * MX4_COLS + lane * 8, in = (uint32_t)row % MX4_ROWS;
-        if (col >= a.cols) continue;
-        const uint8_t *t = a.data + (row / MX4_ROWS * a.nk + kt) * MX4_TILE;
-        const uint32_t w = __ldg(reinterpret_cast<const uint32_t *>(t + mx4_code_at(in, chunk) + 4 * (lane & 3)));
-        const float s = mx4_scale(__ldg(t + MX4_ROWS * 128 + mx4_scale_at(in, chunk)));
-        T v[8];
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, chunk = lane >> 2, rows_at_once = gridDim.x * (MX4_QUANT_THREADS / 32);
+    for (uint32_t kt0 = blockIdx.y * QUANT_TILES; kt0 < a.nk; kt0 += gridDim.y * QUANT_TILES)
+        for (uint64_t i = blockIdx.x * (MX4_QUANT_THREADS / 32) + warp; i < a.n_rows; i += rows_at_once) {
+            const uint32_t e = (uint32_t)i / a.rows, r = (uint32_t)i - e * a.rows, row = e * a.tile_rows + r, in = row % MX4_ROWS;
+            const uint8_t *t = a.data + ((uint64_t)(row / MX4_ROWS) * a.nk + kt0) * MX4_TILE;
+            T *o = static_cast<T *>(a.out) + e * a.ld_expert + r * a.ld + kt0 * MX4_COLS + lane * 8;
+            uint32_t w[QUANT_TILES], sc[QUANT_TILES];
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = narrow<T>(code_value(w >> (4 * k) & 15) * s);
-        T *o = static_cast<T *>(a.out) + e * a.ld_expert + r * a.ld + col;
-        if constexpr (VEC) {
+            for (uint32_t u = 0; u < QUANT_TILES; u++)
+                if (kt0 + u < a.nk) {
+                    w[u] = __ldg(reinterpret_cast<const uint32_t *>(t + u * MX4_TILE + mx4_code_at(in, chunk) + 4 * (lane & 3)));
+                    sc[u] = __ldg(t + u * MX4_TILE + MX4_ROWS * 128 + mx4_scale_at(in, chunk));
+                }
 #pragma unroll
-            for (uint32_t k = 0; k < 8 * sizeof(T) / 16; k++) reinterpret_cast<uint4 *>(o)[k] = reinterpret_cast<const uint4 *>(v)[k];
-        } else {
+            for (uint32_t u = 0; u < QUANT_TILES; u++) {
+                if ((kt0 + u) * MX4_COLS + lane * 8 >= a.cols) break;
+                const float s = mx4_scale(sc[u]);
+                Raw<T> raw;
+                T *v = reinterpret_cast<T *>(raw.w);
 #pragma unroll
-            for (int k = 0; k < 8; k++) o[k] = v[k];
+                for (int k = 0; k < 4; k++) {
+                    const float2 f = values2(w[u] >> (8 * k));
+                    v[2 * k] = narrow<T>(f.x * s), v[2 * k + 1] = narrow<T>(f.y * s);
+                }
+                if constexpr (VEC) {
+#pragma unroll
+                    for (uint32_t k = 0; k < 8 * sizeof(T) / 16; k++) reinterpret_cast<uint4 *>(o + u * MX4_COLS)[k] = raw.w[k];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) o[u * MX4_COLS + k] = v[k];
+                }
+            }
         }
-    }
 }
 
-uint32_t row_grid(uint64_t items, int sms) {
-    const uint64_t want = (items + MX4_QUANT_THREADS / 32 - 1) / (MX4_QUANT_THREADS / 32);
-    return (uint32_t)(want < (uint64_t)sms * 16 ? want : (uint64_t)sms * 16);
+// CTAs of eight rows, by stretches of 1024 columns; eight of them an SM at most, which go on to further rows.
+dim3 row_grid(uint64_t rows, uint32_t nk, int sms) {
+    const uint32_t parts = (nk + QUANT_TILES - 1) / QUANT_TILES, y = parts < 1024 ? parts : 1024;
+    const uint64_t want = (rows + MX4_QUANT_THREADS / 32 - 1) / (MX4_QUANT_THREADS / 32), most = ((uint64_t)sms * 8 + y - 1) / y;
+    return dim3((uint32_t)(want < most ? want : most), y);
 }
 
 template <typename T>
 cudaError_t quantize_as(const Mx4QuantArgs &a, int sms, cudaStream_t s) {
-    const uint32_t grid = row_grid(a.n_rows * a.nk, sms);
+    const dim3 grid = row_grid(a.n_rows, a.nk, sms);
     if (a.vec) mx4_quantize_kernel<T, true><<<grid, MX4_QUANT_THREADS, 0, s>>>(a);
     else mx4_quantize_kernel<T, false><<<grid, MX4_QUANT_THREADS, 0, s>>>(a);
     return cudaGetLastError();
@@ -172,7 +207,7 @@ cudaError_t quantize_as(const Mx4QuantArgs &a, int sms, cudaStream_t s) {
 
 template <typename T>
 cudaError_t dequantize_as(const Mx4ReadArgs &a, int sms, cudaStream_t s) {
-    const uint32_t grid = row_grid(a.n_rows * a.nk, sms);
+    const dim3 grid = row_grid(a.n_rows, a.nk, sms);
     if (a.vec) mx4_dequantize_kernel<T, true><<<grid, MX4_QUANT_THREADS, 0, s>>>(a);
     else mx4_dequantize_kernel<T, false><<<grid, MX4_QUANT_THREADS, 0, s>>>(a);
     return cudaGetLastError();

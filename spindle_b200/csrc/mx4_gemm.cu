@@ -159,11 +159,11 @@ __global__ void __launch_bounds__(THREADS) mx4_gemm_kernel(const __grid_constant
             const uint32_t st = smem_u32(smem + HDR + s * C::STAGE), sc = tmem + C::SUMS + s * C::SC, sx = sc + 8 * (DUAL ? 2 : 1);
 #pragma unroll
             for (uint32_t h = 0; h < 2; h++) {
-                copy_scales<1>(sc + 4 * h, st + MX4_ROWS * 128 + 512 * h);
-                if (DUAL) copy_scales<1>(sc + 8 + 4 * h, st + MX4_TILE + MX4_ROWS * 128 + 512 * h);
+                copy_scales<1>(sc + 4 * h, desc_scales(st + MX4_ROWS * 128 + 512 * h));
+                if (DUAL) copy_scales<1>(sc + 8 + 4 * h, desc_scales(st + MX4_TILE + MX4_ROWS * 128 + 512 * h));
 #pragma unroll
                 for (uint32_t t = 0; t < C::XT; t++)
-                    copy_scales<1>(sx + 4 * C::XT * h + 4 * t, st + C::W_BYTES + NT * 128 + t * MX4_SCALES + 512 * h);
+                    copy_scales<1>(sx + 4 * C::XT * h + 4 * t, desc_scales(st + C::W_BYTES + NT * 128 + t * MX4_SCALES + 512 * h));
             }
             // a product has 64 columns: 32 bytes of a row, half of a word of four scales
 #pragma unroll

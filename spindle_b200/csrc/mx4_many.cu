@@ -42,7 +42,7 @@ struct Cfg {
 };
 
 struct Shared {
-    uint64_t full[8], peer[8], empty[8], sums_full, sums_empty;
+    uint64_t full[8], empty[8], sums_full, sums_empty;
     uint32_t tmem;
 };
 
@@ -66,10 +66,12 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity) {
         if (globaltimer_ns() - t0 > WAIT_LIMIT_NS) return false;
     }
 }
-// Arrives at the barrier of the pair's CTA `rank` that lies where bar does here.
+// Arrives at the barrier of the pair's CTA `rank` that lies where bar does here.  Relaxed: what it tells of are bulk copies
+// and TMEM loads, whose end this thread has seen; nothing that it wrote itself is handed over.  (With release each arrival
+// takes 500 ns, which made a stage of the pipeline 640 to 800 ns long instead of 330.)
 __device__ __forceinline__ void arrive_at(uint64_t *bar, uint32_t rank) {
     asm volatile(
-        "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n}" ::"r"(smem_u32(bar)),
+        "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [a];\n}" ::"r"(smem_u32(bar)),
         "r"(rank)
         : "memory");
 }
@@ -123,7 +125,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
         return;  // (the whole grid alike)
     }
     if (tid == 0) {
-        for (uint32_t i = 0; i < C::STAGES; i++) mbar_init(&sh.full[i], 3), mbar_init(&sh.peer[i], 1), mbar_init(&sh.empty[i], 1);
+        for (uint32_t i = 0; i < C::STAGES; i++) mbar_init(&sh.full[i], rank ? 3 : 4), mbar_init(&sh.empty[i], 1);
         mbar_init(&sh.sums_full, 1);
         mbar_init(&sh.sums_empty, 2 * EPI_WARPS);
         fence_mbar_init();
@@ -182,91 +184,106 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
 
     bool ok = true;
     if (warp < 3) {
-        if (lane == 0) {
-            uint32_t s = 0, turn = 0, issued = 0;
-            if (warp) grid_dependency_wait();  // x comes from the launch before
-            for (uint64_t i = me; i < tiles && ok; i += pairs) {
-                const Tile t = tile_at(i);
-                const uint32_t n = (t.rows + 31) & ~31u, half = n / 2, r0 = rank * half;  // this CTA's tokens: r0 .. r0 + half
-                const uint32_t ft = min(2 * t.fp + rank, a.feat_tiles - 1);
-                const uint64_t w_at = (uint64_t)t.e * a.expert_bytes + (uint64_t)ft * a.nk * MX4_TILE, next = (uint64_t)a.nk * MX4_TILE;
-                const uint8_t *x = a.x + (uint64_t)t.x_tile * next;
-                // rows of the first of them in its tile of 128, and what is left of it
-                const uint32_t in = r0 & 127u, part = min(half, 128 - in), xts = C::XT == 2 && n > 128 ? 2 : 1;
-                const uint8_t *xr = x + (r0 >> 7) * next;
-                for (uint32_t k = 0; k < a.nk; k++) {
-                    if (turn) ok = wait(&sh.empty[s], (turn - 1) & 1);
-                    if (!ok) break;
-                    uint8_t *st = smem + HDR + s * C::STAGE;
-                    const uint64_t at = (uint64_t)k * MX4_TILE;
-                    if (warp == 0) {
-                        mbar_arrive_expect_tx(&sh.full[s], C::W_BYTES);
-                        bulk_g2s(st, a.w + w_at + at, MX4_TILE, &sh.full[s]);
-                        if (DUAL) bulk_g2s(st + MX4_TILE, a.up + w_at + at, MX4_TILE, &sh.full[s]);
-                    } else if (warp == 1) {
-                        mbar_arrive_expect_tx(&sh.full[s], half * 128);
-                        bulk_g2s(st + C::W_BYTES, xr + at + in * 128, part * 128, &sh.full[s]);
-                        if (part < half) bulk_g2s(st + C::W_BYTES + part * 128, xr + next + at, (half - part) * 128, &sh.full[s]);
-                    } else {
-                        mbar_arrive_expect_tx(&sh.full[s], xts * MX4_SCALES);
-                        for (uint32_t j = 0; j < xts; j++)
-                            bulk_g2s(st + C::W_BYTES + C::X_BYTES + j * MX4_SCALES, x + j * next + at + MX4_ROWS * 128, MX4_SCALES, &sh.full[s]);
+        uint32_t s = 0, turn = 0, issued = 0;
+        if (warp) grid_dependency_wait();  // x comes from the launch before
+        for (uint64_t i = me; i < tiles && ok; i += pairs) {
+            const Tile t = tile_at(i);
+            const uint32_t n = (t.rows + 31) & ~31u, half = n / 2, r0 = rank * half;  // this CTA's tokens: r0 .. r0 + half
+            const uint32_t ft = min(2 * t.fp + rank, a.feat_tiles - 1);
+            const uint64_t w_at = (uint64_t)t.e * a.expert_bytes + (uint64_t)ft * a.nk * MX4_TILE, next = (uint64_t)a.nk * MX4_TILE;
+            const uint8_t *w = a.w + w_at, *up = DUAL ? a.up + w_at : nullptr, *x = a.x + (uint64_t)t.x_tile * next;
+            // rows from the first of them on in its tile of 128, and what is left of it
+            const uint32_t in = r0 & 127u, part = min(half, 128 - in), xts = C::XT == 2 && n > 128 ? 2 : 1;
+            const uint8_t *xr = x + (r0 >> 7) * next + in * 128, *xr2 = x + next;
+            if (warp == 2) x += MX4_ROWS * 128;
+            for (uint32_t k = 0; k < a.nk; k++) {
+                if (turn) ok = wait(&sh.empty[s], (turn - 1) & 1);
+                if (!ok) break;
+                uint8_t *st = smem + HDR + s * C::STAGE;
+                uint64_t *full = &sh.full[s];
+                if (warp == 0) {
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(full, C::W_BYTES);
+                        bulk_g2s(st, w, MX4_TILE, full);
+                        if (DUAL) bulk_g2s(st + MX4_TILE, up, MX4_TILE, full);
                     }
-                    issued = min(issued + 1, C::STAGES);
+                    w += MX4_TILE, up += MX4_TILE;
+                } else if (warp == 1) {
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(full, half * 128);
+                        bulk_g2s(st + C::W_BYTES, xr, part * 128, full);
+                        if (part < half) bulk_g2s(st + C::W_BYTES + part * 128, xr2, (half - part) * 128, full);
+                    }
+                    xr += MX4_TILE, xr2 += MX4_TILE;
+                } else {
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(full, xts * MX4_SCALES);
+                        bulk_g2s(st + C::W_BYTES + C::X_BYTES, x, MX4_SCALES, full);
+                        if (xts == 2) bulk_g2s(st + C::W_BYTES + C::X_BYTES + MX4_SCALES, x + next, MX4_SCALES, full);
+                    }
+                    x += MX4_TILE;
+                }
+                __syncwarp();
+                issued = min(issued + 1, C::STAGES);
+                if (++s == C::STAGES) s = 0, turn++;
+            }
+        }
+        if (!ok && warp == 0)  // the copies in flight end before the memory is given up
+            for (; issued; issued--) {
+                const bool back = s == 0;
+                s = back ? C::STAGES - 1 : s - 1;
+                turn -= back;
+                mbar_wait_bounded(&sh.full[s], turn & 1, WAIT_LIMIT_NS);
+            }
+    } else if (warp == 3) {
+        uint32_t s = 0, turn = 0, count = 0;
+        if (rank) {  // the other CTA's operands are there: the first one is told
+            for (uint64_t i = me; i < tiles && ok; i += pairs)
+                for (uint32_t k = 0; k < a.nk; k++) {
+                    ok = wait(&sh.full[s], turn & 1);
+                    if (!ok) break;
+                    if (elect_one()) arrive_at(&sh.full[s], 0);
+                    __syncwarp();
                     if (++s == C::STAGES) s = 0, turn++;
                 }
-            }
-            if (!ok && warp == 0)  // the copies in flight end before the memory is given up
-                for (; issued; issued--) {
-                    const bool back = s == 0;
-                    s = back ? C::STAGES - 1 : s - 1;
-                    turn -= back;
-                    mbar_wait_bounded(&sh.full[s], turn & 1, WAIT_LIMIT_NS);
-                }
-        }
-    } else if (warp == 3) {
-        if (lane == 0) {
-            uint32_t s = 0, turn = 0, count = 0;
+        } else {
+            // what changes in a descriptor from stage to stage is its address
+            const uint32_t base = smem_u32(smem + HDR);
+            const uint64_t w_desc = desc_operand(base), x_desc = desc_operand(base + C::W_BYTES);
+            const uint64_t ws_desc = desc_scales(base + MX4_ROWS * 128), xs_desc = desc_scales(base + C::W_BYTES + C::X_BYTES);
             for (uint64_t i = me; i < tiles && ok; i += pairs, count++) {
-                if (rank) {  // the other CTA's operands are there: the first one is told
-                    for (uint32_t k = 0; k < a.nk; k++) {
-                        ok = wait(&sh.full[s], turn & 1);
-                        if (!ok) break;
-                        arrive_at(&sh.peer[s], 0);
-                        if (++s == C::STAGES) s = 0, turn++;
-                    }
-                    continue;
-                }
-                const Tile t = tile_at(i);
-                const uint32_t n = (t.rows + 31) & ~31u;
+                const uint32_t n = (tile_at(i).rows + 31) & ~31u, id = idesc(256, n, 0);
                 if (count) ok = wait(&sh.sums_empty, (count - 1) & 1);
                 if (!ok) break;
                 fence_after();
                 for (uint32_t k = 0; k < a.nk; k++) {
-                    ok = wait(&sh.full[s], turn & 1) && wait(&sh.peer[s], turn & 1);
+                    ok = wait(&sh.full[s], turn & 1);
                     if (!ok) break;
                     fence_after();
-                    const uint32_t st = smem_u32(smem + HDR + s * C::STAGE), xs = st + C::W_BYTES + C::X_BYTES;
-                    const uint32_t sc = tmem + C::SUMS + s * C::SC, sx = sc + 8 * (DUAL ? 2 : 1);
+                    const uint32_t at = (s * C::STAGE) >> 4, sc = tmem + C::SUMS + s * C::SC, sx = sc + 8 * (DUAL ? 2 : 1);
+                    if (elect_one()) {
 #pragma unroll
-                    for (uint32_t h = 0; h < 2; h++) {
-                        copy_scales<2>(sc + 4 * h, st + MX4_ROWS * 128 + 512 * h);
-                        if (DUAL) copy_scales<2>(sc + 8 + 4 * h, st + MX4_TILE + MX4_ROWS * 128 + 512 * h);
+                        for (uint32_t h = 0; h < 2; h++) {
+                            copy_scales<2>(sc + 4 * h, ws_desc + at + 32 * h);
+                            if (DUAL) copy_scales<2>(sc + 8 + 4 * h, ws_desc + at + (MX4_TILE >> 4) + 32 * h);
 #pragma unroll
-                        for (uint32_t j = 0; j < C::XT; j++) copy_scales<2>(sx + 4 * C::XT * h + 4 * j, xs + j * MX4_SCALES + 512 * h);
+                            for (uint32_t j = 0; j < C::XT; j++) copy_scales<2>(sx + 4 * C::XT * h + 4 * j, xs_desc + at + j * (MX4_SCALES >> 4) + 32 * h);
+                        }
+                        // a product has 64 columns: 32 bytes of a row, half of a word of four scales
+#pragma unroll
+                        for (uint32_t q = 0; q < 4; q++) {
+                            const uint32_t h = q >> 1, iq = id | (q & 1 ? idesc(0, 0, 1) ^ idesc(0, 0, 0) : 0u), add = k > 0 || q > 0;
+                            mma<2>(tmem, w_desc + at + 2 * q, x_desc + at + 2 * q, iq, sc + 4 * h, sx + 4 * C::XT * h, add);
+                            if (DUAL)
+                                mma<2>(tmem + 128, w_desc + at + (MX4_TILE >> 4) + 2 * q, x_desc + at + 2 * q, iq, sc + 8 + 4 * h, sx + 4 * h, add);
+                        }
+                        commit<2>(&sh.empty[s]);
                     }
-                    // a product has 64 columns: 32 bytes of a row, half of a word of four scales
-#pragma unroll
-                    for (uint32_t q = 0; q < 4; q++) {
-                        const uint32_t h = q >> 1, id = idesc(256, n, q & 1), add = k > 0 || q > 0;
-                        const uint64_t x = desc_operand(st + C::W_BYTES + 32 * q);
-                        mma<2>(tmem, desc_operand(st + 32 * q), x, id, sc + 4 * h, sx + 4 * C::XT * h, add);
-                        if (DUAL) mma<2>(tmem + 128, desc_operand(st + MX4_TILE + 32 * q), x, id, sc + 8 + 4 * h, sx + 4 * h, add);
-                    }
-                    commit<2>(&sh.empty[s]);
+                    __syncwarp();
                     if (++s == C::STAGES) s = 0, turn++;
                 }
-                if (ok) commit<2>(&sh.sums_full);
+                if (ok && elect_one()) commit<2>(&sh.sums_full);
+                __syncwarp();
             }
         }
     } else {
@@ -288,7 +305,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
             }
             fence_before();
             __syncwarp();
-            if (lane == 0) arrive_at(&sh.sums_empty, 0);
+            if (elect_one()) arrive_at(&sh.sums_empty, 0);
+            __syncwarp();
             if (t.rows <= from) continue;
             const uint32_t f0 = (2 * t.fp + rank) * MX4_ROWS + 32 * q;
             if (f0 >= a.feats) continue;

@@ -41,9 +41,9 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
 }
 // 32 rows of 16 bytes to four columns of all 128 lanes (of a pair: each CTA's own)
 template <int G>
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t saddr) {
-    if constexpr (G == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc_scales(saddr)) : "memory");
-    else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc_scales(saddr)) : "memory");
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
+    if constexpr (G == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 // The barrier (of a pair: of both CTAs) is arrived at when everything issued before is done.
 template <int G>
@@ -107,6 +107,14 @@ __device__ __forceinline__ void tmem_ld64(uint32_t addr, float *v) {
         : "memory");
 #pragma unroll
     for (int i = 0; i < 64; i++) v[i] = __uint_as_float(r[i]);
+}
+
+// One lane of a converged warp.  (Copies, products and arrivals under this cost their warp half of what they cost under
+// lane == 0: about 20 ns instead of 44 a bulk copy.)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
 }
 
 __device__ __forceinline__ float silu_times(float g, float u) { return g / (1.0f + expf(-g)) * u; }
