@@ -10,7 +10,7 @@
 //     tokens, the tokens' scales (both halves': the scales of all columns stand in each CTA);
 //   - one thread of the pair's first CTA issues scales' copies to TMEM and products for both; the
 //     other CTA's tells it when its operands are there;
-//   - eight warps take the sums out of TMEM into registers, at once, so that the next tile's products
+//   - sixteen warps take the sums out of TMEM into registers, at once, so that the next tile's products
 //     can begin, then round them and write them by way of shared memory, 16 bytes a lane.
 #include <cooperative_groups.h>
 
@@ -24,27 +24,39 @@ using namespace tiled;
 
 namespace {
 
-constexpr uint32_t EPI_WARPS = 8, FIRST_EPI = 4, THREADS = 32 * (FIRST_EPI + EPI_WARPS);
+constexpr uint32_t EPI_WARPS = 16, FIRST_EPI = 4, THREADS = 32 * (FIRST_EPI + EPI_WARPS);
 constexpr uint32_t MAX_E = MOE_SORT_MAX_EXPERTS;
-constexpr uint32_t HDR = 1024 + (MAX_E + 4) * 4 / 1024 * 1024 + 1024;  // barriers and TMEM base; the experts' first tiles
-constexpr uint32_t OUT_ROW = 144;                                      // a token's 32 features of a warp, and padding
-constexpr uint32_t OUT_BYTES = 32 * OUT_ROW;
+constexpr uint32_t HDR = 1024 + 3 * 4 * MAX_E;   // barriers and TMEM base; what is looked up of the experts
+constexpr uint32_t GROUPS = EPI_WARPS / 4;       // four warps take a piece of 16 tokens, 32 features each
+constexpr uint32_t OUT_ROW = MX4_ROWS * 2 + 16;  // 16-bit results of a token in shared memory, and padding
+constexpr uint32_t OUT_BYTES = 2 * 16 * OUT_ROW; // two such pieces, or one of f32
+static_assert(OUT_BYTES >= 16 * (MX4_ROWS * 4 + 16), "a piece of f32");
 
 template <bool DUAL>
 struct Cfg {
-    static constexpr uint32_t NT = DUAL ? 128 : 256, XT = NT / 128;
+    // Two buffers of sums where TMEM has room for them beside the scales: the products of a tile run while the results of the
+    // one before are taken (32760 places, 768 columns to 2048: 60 us; with tiles of 256 tokens and one buffer 63).  Gate and up of 96 tokens
+    // would fit twice too, but then each brings its weights for fewer tokens.
+    static constexpr uint32_t NT = DUAL ? 128 : 192, XT = DUAL ? 1 : 2, BUFS = DUAL ? 1 : 2;
     static constexpr uint32_t W_BYTES = MX4_TILE * (DUAL ? 2 : 1), X_BYTES = NT / 2 * 128, XS_BYTES = XT * MX4_SCALES;
     static constexpr uint32_t STAGE = W_BYTES + X_BYTES + XS_BYTES;
     static constexpr uint32_t STAGES = DUAL ? 4 : 5;
-    static constexpr uint32_t OUT_AT = HDR + STAGES * STAGE, SMEM = OUT_AT + EPI_WARPS * OUT_BYTES;
-    static constexpr uint32_t SUMS = 256, SC = 8 * ((DUAL ? 2 : 1) + XT), COLS = 512;
-    static_assert(SUMS + STAGES * SC <= COLS && SMEM <= 227 * 1024 && STAGE % 1024 == 0, "shapes");
+    static constexpr uint32_t PIECES = NT / 16 / GROUPS;
+    static constexpr uint32_t OUT_AT = HDR + STAGES * STAGE, SMEM = OUT_AT + GROUPS * OUT_BYTES;
+    static constexpr uint32_t SUMS = NT * (DUAL ? 2 : BUFS), SC = 8 * ((DUAL ? 2 : 1) + XT), COLS = 512;
+    static_assert(SUMS + STAGES * SC <= COLS && SMEM <= 227 * 1024 && STAGE % 1024 == 0 && NT % (16 * GROUPS) == 0, "shapes");
 };
 
 struct Shared {
-    uint64_t full[8], empty[8], sums_full, sums_empty;
-    uint32_t tmem;
+    uint64_t full[8], empty[8], sums_full[2], sums_empty[2];
+    uint32_t tmem, n_rows;
 };
+// Of each expert: how many tiles end with it, its first sorted place, its first tile of x (a lookup from global memory took
+// every role 0.7 us a tile).
+struct Experts {
+    uint32_t upto[MAX_E], first[MAX_E], x_tile[MAX_E];
+};
+static_assert(sizeof(Shared) <= 1024 && sizeof(Experts) == HDR - 1024, "places");
 
 __device__ __forceinline__ bool try_wait_cluster(uint64_t *bar, uint32_t parity) {
     uint32_t ok;
@@ -78,35 +90,59 @@ __device__ __forceinline__ void arrive_at(uint64_t *bar, uint32_t rank) {
 
 // A tile: up to NT rows of x, those of one expert, from row row0 of the output on.
 struct Tile {
-    uint32_t e, x_tile, rows, fp;
+    uint32_t e, x_tile, in, rows, fp;  // (x: from row `in` of its tile x_tile on)
     uint64_t row0;
 };
 
-template <typename T> __device__ __forceinline__ T narrow(float v);
-template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ uint32_t pack(__half, float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack(__nv_bfloat16, float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
 
-// 32 tokens of 32 features, a feature a lane, to rows of the output; n of the tokens are there.
+// A piece of 16 tokens (n of them are there) by 128 features from f0 on, of which a warp has 32 in v as tmem_ld32x16 gives
+// them, to rows of the output from `row` on: by way of shared memory, where the four warps' features of a token come
+// together.  16-bit results go there eight by eight, turned over on the way (stmatrix), to one of two places in turn, so that
+// one barrier a piece will do.
 template <typename T>
-__device__ __forceinline__ void put32(const Mx4GemmArgs &a, uint8_t *buf, const float *v, uint64_t row, uint32_t n, uint32_t f0, uint32_t lane) {
-    T *out = static_cast<T *>(a.out);
-    if (a.vec && f0 + 32 <= a.feats) {
+__device__ __forceinline__ void put_piece(const Mx4GemmArgs &a, uint8_t *buf, const float *v, uint64_t row, uint32_t n, uint32_t f0, uint32_t warp,
+                                          uint32_t lane, uint32_t group) {
+    constexpr uint32_t ROW = MX4_ROWS * sizeof(T) + 16, PER = MX4_ROWS * sizeof(T) / 16, ES = 16 / sizeof(T);
+    if constexpr (sizeof(T) == 2) {
+        const uint32_t at = smem_u32(buf) + (lane & 7) * ROW + (32 * warp + 8 * (lane >> 3)) * 2;
 #pragma unroll
-        for (uint32_t j = 0; j < 32; j++) *reinterpret_cast<T *>(buf + j * OUT_ROW + lane * sizeof(T)) = narrow<T>(v[j]);
-        __syncwarp();
-        constexpr uint32_t PER = 2 * sizeof(T), AT_ONCE = 32 / PER;  // lanes a token
-#pragma unroll
-        for (uint32_t j = 0; j < 32; j += AT_ONCE) {
-            const uint32_t t = j + lane / PER, c = lane % PER;
-            const uint4 w = *reinterpret_cast<const uint4 *>(buf + t * OUT_ROW + 16 * c);
-            if (t < n) *reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(out + (row + t) * a.ldo + f0) + 16 * c) = w;
+        for (uint32_t b = 0; b < 2; b++) {
+            const float *lo = v + 4 * b, *hi = v + 8 + 4 * b;
+            asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at + 8 * b * ROW), "r"(pack(T(), lo[0], lo[1])),
+                         "r"(pack(T(), lo[2], lo[3])), "r"(pack(T(), hi[0], hi[1])), "r"(pack(T(), hi[2], hi[3]))
+                         : "memory");
         }
-        __syncwarp();
-    } else if (f0 + lane < a.feats) {
+    } else {
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");  // the piece before has been read
+        float *at = reinterpret_cast<float *>(buf + 2 * (lane & 3) * ROW) + 32 * warp + (lane >> 2);
 #pragma unroll
-        for (uint32_t j = 0; j < 32; j++)
-            if (j < n) out[(row + j) * a.ldo + f0 + lane] = narrow<T>(v[j]);
+        for (uint32_t b = 0; b < 2; b++)
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++)  // (token 8 b + 2 (lane % 4) + i % 2, feature 8 (i / 2) + lane / 4 of the warp's)
+                at[(8 * b + (i & 1)) * (ROW / 4) + 8 * (i >> 1)] = v[(i >> 2) * 8 + 4 * b + (i & 3)];
+    }
+    asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+    T *out = static_cast<T *>(a.out);
+#pragma unroll
+    for (uint32_t i = 0; i < 16 * PER / 128; i++) {
+        const uint32_t at = i * 128 + 32 * warp + lane, t = at / PER, c = at % PER, f = f0 + c * ES;
+        if (t < n && f < a.feats) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(buf + t * ROW + 16 * c);
+            T *o = out + (row + t) * a.ldo + f;
+            if (a.vec && f + ES <= a.feats) *reinterpret_cast<uint4 *>(o) = w;
+            else
+#pragma unroll
+                for (uint32_t j = 0; j < ES; j++)
+                    if (f + j < a.feats) o[j] = reinterpret_cast<const T *>(&w)[j];
+        }
     }
 }
 
@@ -115,7 +151,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
     using C = Cfg<DUAL>;
     extern __shared__ __align__(1024) uint8_t smem[];
     Shared &sh = *reinterpret_cast<Shared *>(smem);
-    uint32_t *upto = reinterpret_cast<uint32_t *>(smem + 1024);  // experts: tiles of the ones up to each
+    Experts &ex = *reinterpret_cast<Experts *>(smem + 1024);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = cluster.block_rank();
@@ -126,8 +162,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
     }
     if (tid == 0) {
         for (uint32_t i = 0; i < C::STAGES; i++) mbar_init(&sh.full[i], rank ? 3 : 4), mbar_init(&sh.empty[i], 1);
-        mbar_init(&sh.sums_full, 1);
-        mbar_init(&sh.sums_empty, 2 * EPI_WARPS);
+        for (uint32_t i = 0; i < 2; i++) mbar_init(&sh.sums_full[i], 1), mbar_init(&sh.sums_empty[i], 2 * EPI_WARPS);
         fence_mbar_init();
     }
     if (warp == 3) tmem_alloc<2>(&sh.tmem, C::COLS);
@@ -137,13 +172,19 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
             uint32_t before = 0;
             for (uint32_t base = 0; base < a.n_expert; base += 32) {
                 const uint32_t i = base + lane;
-                uint32_t n = i < a.n_expert ? ((uint32_t)__ldg(a.first + i + 1) - (uint32_t)__ldg(a.first + i) + C::NT - 1) / C::NT : 0;
+                const uint32_t f0 = i < a.n_expert ? (uint32_t)__ldg(a.first + i) : 0, f1 = i < a.n_expert ? (uint32_t)__ldg(a.first + i + 1) : 0;
+                uint32_t n = (f1 - f0 + C::NT - 1) / C::NT;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const uint32_t v = __shfl_up_sync(0xffffffffu, n, o);
                     if (lane >= (uint32_t)o) n += v;
                 }
-                if (i < a.n_expert) upto[i] = before + n;
+                if (i < a.n_expert) {
+                    ex.upto[i] = before + n;
+                    ex.first[i] = f0;
+                    ex.x_tile[i] = (uint32_t)__ldg(a.tiles + i);
+                    if (i + 1 == a.n_expert) sh.n_rows = f1;
+                }
                 before += __shfl_sync(0xffffffffu, n, 31);
             }
         }
@@ -152,31 +193,33 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
     __syncthreads();
     cluster.sync();
     fence_after();
-    token_tiles = a.first ? upto[a.n_expert - 1] : (uint32_t)((a.n_tok + C::NT - 1) / C::NT);
+    token_tiles = a.first ? ex.upto[a.n_expert - 1] : (uint32_t)((a.n_tok + C::NT - 1) / C::NT);
     const uint32_t tmem = sh.tmem, pairs = gridDim.x / 2, me = blockIdx.x / 2;
     const uint32_t fps = (a.feat_tiles + 1) / 2;
-    const uint64_t tiles = (uint64_t)token_tiles * fps;
+    const uint32_t tiles = token_tiles * fps;
 
-    auto tile_at = [&](uint64_t i) {
+    auto tile_at = [&](uint32_t i) {
         Tile t;
-        const uint32_t tt = (uint32_t)(i / fps);
-        t.fp = (uint32_t)(i - (uint64_t)tt * fps);
+        const uint32_t tt = i / fps;
+        t.fp = i - tt * fps;
         if (a.first) {
             uint32_t lo = 0, hi = a.n_expert - 1;  // the first expert whose tiles reach past tt
             while (lo < hi) {
                 const uint32_t mid = (lo + hi) / 2;
-                if (upto[mid] > tt) hi = mid;
+                if (ex.upto[mid] > tt) hi = mid;
                 else lo = mid + 1;
             }
-            const uint32_t k = tt - (lo ? upto[lo - 1] : 0), f0 = (uint32_t)__ldg(a.first + lo), n = (uint32_t)__ldg(a.first + lo + 1) - f0;
+            const uint32_t k = tt - (lo ? ex.upto[lo - 1] : 0), f0 = ex.first[lo], n = (lo + 1 < a.n_expert ? ex.first[lo + 1] : sh.n_rows) - f0;
             t.e = lo;
-            t.x_tile = (uint32_t)__ldg(a.tiles + lo) + k * C::XT;
+            t.x_tile = ex.x_tile[lo] + k * C::NT / 128;
+            t.in = k * C::NT % 128;
             t.rows = min(n - k * C::NT, C::NT);
             t.row0 = f0 + k * C::NT;
         } else {
             t.e = 0;
-            t.x_tile = tt * C::XT;
             t.row0 = (uint64_t)tt * C::NT;
+            t.x_tile = (uint32_t)(t.row0 / 128);
+            t.in = (uint32_t)(t.row0 % 128);
             t.rows = (uint32_t)(a.n_tok - t.row0 < C::NT ? a.n_tok - t.row0 : C::NT);
         }
         return t;
@@ -186,14 +229,14 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
     if (warp < 3) {
         uint32_t s = 0, turn = 0, issued = 0;
         if (warp) grid_dependency_wait();  // x comes from the launch before
-        for (uint64_t i = me; i < tiles && ok; i += pairs) {
+        for (uint32_t i = me; i < tiles && ok; i += pairs) {
             const Tile t = tile_at(i);
-            const uint32_t n = (t.rows + 31) & ~31u, half = n / 2, r0 = rank * half;  // this CTA's tokens: r0 .. r0 + half
+            const uint32_t n = (t.rows + 31) & ~31u, half = n / 2, r0 = t.in + rank * half;  // this CTA's tokens: r0 .. r0 + half
             const uint32_t ft = min(2 * t.fp + rank, a.feat_tiles - 1);
             const uint64_t w_at = (uint64_t)t.e * a.expert_bytes + (uint64_t)ft * a.nk * MX4_TILE, next = (uint64_t)a.nk * MX4_TILE;
             const uint8_t *w = a.w + w_at, *up = DUAL ? a.up + w_at : nullptr, *x = a.x + (uint64_t)t.x_tile * next;
             // rows from the first of them on in its tile of 128, and what is left of it
-            const uint32_t in = r0 & 127u, part = min(half, 128 - in), xts = C::XT == 2 && n > 128 ? 2 : 1;
+            const uint32_t in = r0 & 127u, part = min(half, 128 - in), xts = C::XT == 2 && t.in + n > 128 ? 2 : 1;
             const uint8_t *xr = x + (r0 >> 7) * next + in * 128, *xr2 = x + next;
             if (warp == 2) x += MX4_ROWS * 128;
             for (uint32_t k = 0; k < a.nk; k++) {
@@ -238,7 +281,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
     } else if (warp == 3) {
         uint32_t s = 0, turn = 0, count = 0;
         if (rank) {  // the other CTA's operands are there: the first one is told
-            for (uint64_t i = me; i < tiles && ok; i += pairs)
+            for (uint32_t i = me; i < tiles && ok; i += pairs)
                 for (uint32_t k = 0; k < a.nk; k++) {
                     ok = wait(&sh.full[s], turn & 1);
                     if (!ok) break;
@@ -251,9 +294,10 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
             const uint32_t base = smem_u32(smem + HDR);
             const uint64_t w_desc = desc_operand(base), x_desc = desc_operand(base + C::W_BYTES);
             const uint64_t ws_desc = desc_scales(base + MX4_ROWS * 128), xs_desc = desc_scales(base + C::W_BYTES + C::X_BYTES);
-            for (uint64_t i = me; i < tiles && ok; i += pairs, count++) {
-                const uint32_t n = (tile_at(i).rows + 31) & ~31u, id = idesc(256, n, 0);
-                if (count) ok = wait(&sh.sums_empty, (count - 1) & 1);
+            for (uint32_t i = me; i < tiles && ok; i += pairs, count++) {
+                const Tile t = tile_at(i);
+                const uint32_t n = (t.rows + 31) & ~31u, id = idesc(256, n, 0), b = count % C::BUFS, sums = tmem + b * C::NT;
+                if (count >= C::BUFS) ok = wait(&sh.sums_empty[b], (count / C::BUFS - 1) & 1);
                 if (!ok) break;
                 fence_after();
                 for (uint32_t k = 0; k < a.nk; k++) {
@@ -273,54 +317,69 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
 #pragma unroll
                         for (uint32_t q = 0; q < 4; q++) {
                             const uint32_t h = q >> 1, iq = id | (q & 1 ? idesc(0, 0, 1) ^ idesc(0, 0, 0) : 0u), add = k > 0 || q > 0;
-                            mma<2>(tmem, w_desc + at + 2 * q, x_desc + at + 2 * q, iq, sc + 4 * h, sx + 4 * C::XT * h, add);
+                            mma<2>(sums, w_desc + at + 2 * q, x_desc + at + 2 * q, iq, sc + 4 * h, sx + 4 * C::XT * h + t.in / 32, add);
                             if (DUAL)
-                                mma<2>(tmem + 128, w_desc + at + (MX4_TILE >> 4) + 2 * q, x_desc + at + 2 * q, iq, sc + 8 + 4 * h, sx + 4 * h, add);
+                                mma<2>(sums + C::NT, w_desc + at + (MX4_TILE >> 4) + 2 * q, x_desc + at + 2 * q, iq, sc + 8 + 4 * h, sx + 4 * h, add);
                         }
                         commit<2>(&sh.empty[s]);
                     }
                     __syncwarp();
                     if (++s == C::STAGES) s = 0, turn++;
                 }
-                if (ok && elect_one()) commit<2>(&sh.sums_full);
+                if (ok && elect_one()) commit<2>(&sh.sums_full[b]);
                 __syncwarp();
             }
         }
     } else {
-        const uint32_t q = warp & 3, g = (warp - FIRST_EPI) >> 2;  // lanes 32 q on; which half of the tokens
-        uint8_t *buf = smem + C::OUT_AT + (warp - FIRST_EPI) * OUT_BYTES;
-        constexpr uint32_t HALF = C::NT / 2;
-        uint32_t count = 0;
-        for (uint64_t i = me; i < tiles; i += pairs, count++) {
+        // lanes 32 q on; of the tile's pieces of 16 tokens every GROUPS-th from the g-th on
+        const uint32_t q = warp & 3, g = (warp - FIRST_EPI) >> 2;
+        uint8_t *buf = smem + C::OUT_AT + g * OUT_BYTES;
+        constexpr uint32_t APART = 16 * GROUPS;
+        uint32_t count = 0, turn = 0;
+        for (uint32_t i = me; i < tiles; i += pairs, count++) {
             const Tile t = tile_at(i);
-            ok = __all_sync(0xffffffffu, wait(&sh.sums_full, count & 1));
-            if (!ok) break;
-            fence_after();
-            float v[128];
-            const uint32_t from = g * HALF, at = tmem + ((32 * q) << 16) + from;
-            if (t.rows > from) {
-                tmem_ld64(at, v);
-                if (DUAL) tmem_ld64(at + 128, v + 64);
-                else if (t.rows > from + 64) tmem_ld64(at + 64, v + 64);
+            const uint32_t b = count % C::BUFS;
+            // one warp of a group waits, the others for it; they go on together, or not at all
+            uint32_t bad = q == 0 && !wait(&sh.sums_full[b], (count / C::BUFS) & 1);
+            asm volatile("{\n .reg .pred p, r;\n setp.ne.u32 p, %0, 0;\n barrier.cta.red.or.pred r, %1, 128, p;\n selp.u32 %0, 1, 0, r;\n}"
+                         : "+r"(bad)
+                         : "r"(1 + g)
+                         : "memory");
+            if (bad) {
+                ok = false;
+                break;
             }
+            fence_after();
+            float v[16 * C::PIECES * (DUAL ? 2 : 1)];  // the sums of the pieces, then those of `up`
+            const uint32_t at = tmem + b * C::NT + ((32 * q) << 16) + 16 * g;
+#pragma unroll
+            for (uint32_t c = 0; c < C::PIECES; c++)
+                if (t.rows > APART * c + 16 * g) {
+                    tmem_ld32x16(at + APART * c, v + 16 * c);
+                    if (DUAL) tmem_ld32x16(at + C::NT + APART * c, v + 16 * (C::PIECES + c));
+                }
+#pragma unroll
+            for (uint32_t c = 0; c < C::PIECES * (DUAL ? 2 : 1); c++) tmem_wait(v + 16 * c);
             fence_before();
             __syncwarp();
-            if (elect_one()) arrive_at(&sh.sums_empty, 0);
+            if (elect_one()) arrive_at(&sh.sums_empty[b], 0);
             __syncwarp();
-            if (t.rows <= from) continue;
-            const uint32_t f0 = (2 * t.fp + rank) * MX4_ROWS + 32 * q;
+            const uint32_t f0 = (2 * t.fp + rank) * MX4_ROWS;
             if (f0 >= a.feats) continue;
-            if (DUAL) {
 #pragma unroll
-                for (int j = 0; j < 64; j++) v[j] = silu_times(v[j], v[64 + j]);
-            }
+            for (uint32_t c = 0; c < C::PIECES; c++)
+                if (t.rows > APART * c + 16 * g) {
+                    const uint32_t from = APART * c + 16 * g, n = t.rows - from;
+                    float *p = v + 16 * c;
+                    if (DUAL) {
 #pragma unroll
-            for (uint32_t c = 0; c < HALF; c += 32)
-                if (t.rows > from + c) {
-                    const uint32_t n = t.rows - from - c;
-                    if (a.type == SG_F32) put32<float>(a, buf, v + c, t.row0 + from + c, n, f0, lane);
-                    else if (a.type == SG_F16) put32<__half>(a, buf, v + c, t.row0 + from + c, n, f0, lane);
-                    else put32<__nv_bfloat16>(a, buf, v + c, t.row0 + from + c, n, f0, lane);
+                        for (int j = 0; j < 16; j++) p[j] = silu_times(p[j], p[16 * C::PIECES + j]);
+                    }
+                    uint8_t *to = buf + (turn & 1) * (OUT_BYTES / 2);
+                    if (a.type == SG_F32) put_piece<float>(a, buf, p, t.row0 + from, n, f0, q, lane, g);
+                    else if (a.type == SG_F16) put_piece<__half>(a, to, p, t.row0 + from, n, f0, q, lane, g);
+                    else put_piece<__nv_bfloat16>(a, to, p, t.row0 + from, n, f0, q, lane, g);
+                    turn++;
                 }
         }
     }

@@ -86,27 +86,24 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
 #pragma unroll
     for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
 }
-// 64 columns
-__device__ __forceinline__ void tmem_ld64(uint32_t addr, float *v) {
-    uint32_t r[64];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
-        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-        : "r"(addr)
-        : "memory");
+// 32 lanes from the address's on, 16 columns: of each eight columns b and 16 lanes h a thread gets two of the lane (thread / 4)
+// in v[8 h + 4 b] and the next, columns 8 b + 2 (thread % 4) on, and the same of the lane 8 further in v[8 h + 4 b + 2] and the
+// next.  They are there after tmem_wait of the same registers (which are its operands, so that no use of them can move in
+// between).
+__device__ __forceinline__ void tmem_ld32x16(uint32_t addr, float *v) {
 #pragma unroll
-    for (int i = 0; i < 64; i++) v[i] = __uint_as_float(r[i]);
+    for (uint32_t h = 0; h < 2; h++, v += 8)
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                     : "r"(addr + ((16 * h) << 16))
+                     : "memory");
+}
+__device__ __forceinline__ void tmem_wait(float *v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]),
+                   "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+                 :
+                 : "memory");
 }
 
 // One lane of a converged warp.  (Copies, products and arrivals under this cost their warp half of what they cost under
@@ -117,7 +114,18 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
-__device__ __forceinline__ float silu_times(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// silu(g) * u, by E = exp(-|g|), at most 1: the logistic function of g is 1 or E (of a negative g) over 1 + E.  The exponent
+// |g| log2(e) is taken with its rest, so that E of a far g is off by little more than ex2's 2 units (|g| 1.3e-8 of it); below
+// 2^-126 it is 0.  13 instructions, two of them on the unit that has 16 lanes an SM (with expf and a division 60: a tile's
+// gates took three times as long as its products).
+__device__ __forceinline__ float silu_times(float g, float u) {
+    const float a = fminf(fabsf(g), 200.0f), t = a * -1.44269504f, rest = fmaf(a, -1.44269504f, -t);
+    float e, q;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    e = fmaf(e, rest * 0.693147181f, e);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.0f + e));
+    return (g < 0.0f ? e : 1.0f) * (q * (g * u));
+}
 
 }  // namespace mx4
 }  // namespace sg
