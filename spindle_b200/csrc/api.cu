@@ -2598,6 +2598,8 @@ sg_status check_mx4(const sg_mx4 *m, bool data) {
     return aligned(m->data, 16) ? SG_OK : SG_ERR_ALIGN;
 }
 
+// Tiles of 128 features and 128 tokens from which on the kernel for many tokens is taken: @@
+constexpr uint64_t MX4_MANY_TILES = 120;
 uint32_t mx4_nk(const sg_mx4 *m) { return (uint32_t)((m->cols + MX4_COLS - 1) / MX4_COLS); }
 uint64_t mx4_expert_bytes(const sg_mx4 *m) { return align_up(m->rows, MX4_ROWS) / MX4_ROWS * mx4_nk(m) * MX4_TILE; }
 // rows of cols elements ld apart: whether every eight of them are 16-byte aligned
@@ -2617,17 +2619,19 @@ uint32_t sort_ctas(uint64_t n_tok) {
 // plan->work: first tiles for tiles of 32, 64 and 128 rows, then the stretches' counts
 int32_t *plan_tiles(const sg_moe_plan *p, uint32_t shift) { return p->work + (shift - 5) * (p->n_expert + 1); }
 
-// How a product of n_tok rows is run: rows of x a tile, tiles of x, tiles of tokens (of experts: at most that many).
+// How a product of n_tok rows is run: rows of x a tile (1 << shift), tiles of x; tiles of tokens (of experts: at most that
+// many) and which kernel.
 struct Mx4Plan {
     uint32_t shift;
     uint64_t x_tiles, token_tiles;
+    bool many;
 };
-Mx4Plan mx4_plan(uint64_t n_tok, const sg_moe_plan *plan) {
+Mx4Plan mx4_plan(const sg_mx4 *w, uint64_t n_tok, const sg_moe_plan *plan) {
     const uint64_t pairs = plan ? plan->n_tok * plan->n_used : n_tok, groups = plan ? std::min(plan->n_expert, pairs) : 1;
-    if (!pairs) return {5, 0, 0};
+    if (!pairs) return {5, 0, 0, false};
     const uint32_t shift = pairs / groups <= 32 ? 5 : 7;
     const uint64_t rows = 1ull << shift, tiles = (pairs + groups * (rows - 1)) / rows;
-    return {shift, tiles, tiles};
+    return {shift, tiles, tiles, shift == 7 && tiles * (align_up(w->rows, MX4_ROWS) / MX4_ROWS) >= MX4_MANY_TILES};
 }
 uint64_t mx4_scratch(const sg_mx4 *w, const Mx4Plan &p) { return p.x_tiles * mx4_nk(w) * mx4_tile_bytes(1u << p.shift); }
 
@@ -2641,7 +2645,7 @@ sg_status mx4_product(const sg_mx4 *w, const sg_mx4 *up, const sg_moe_plan *plan
     if (!pairs) return SG_OK;
     const uint64_t x_rows = plan ? (gather ? plan->n_tok : pairs) : n_tok;
     if (!d_x || !d_out || (x_rows > 1 && ldx < w->cols) || (pairs > 1 && ldo < w->rows)) return SG_ERR_INVALID;
-    const Mx4Plan mp = mx4_plan(n_tok, plan);
+    const Mx4Plan mp = mx4_plan(w, n_tok, plan);
     if (!d_scratch || scratch_bytes < mx4_scratch(w, mp)) return SG_ERR_INVALID;
     if (!aligned(d_x, es) || !aligned(d_out, eo) || !aligned(d_scratch, 128)) return SG_ERR_ALIGN;
     DevInfo *di;
@@ -2652,7 +2656,7 @@ sg_status mx4_product(const sg_mx4 *w, const sg_mx4 *up, const sg_moe_plan *plan
     q.x = d_x, q.ld = ldx, q.out = (uint8_t *)d_scratch;
     q.cols = (uint32_t)w->cols, q.nk = nk, q.tile_shift = mp.shift, q.n_rows = x_rows;
     q.rows = (uint32_t)x_rows, q.tile_rows = (uint32_t)x_rows;
-    q.vec = rows16(d_x, ldx, es);
+    q.vec = rows16(d_x, ldx, es), q.early = true;
     Mx4GemmArgs g = {};
     g.w = w->data, g.up = up ? up->data : nullptr, g.x = (const uint8_t *)d_scratch;
     g.out = d_out, g.ldo = ldo, g.expert_bytes = mx4_expert_bytes(w), g.type = out_type;
@@ -2664,7 +2668,7 @@ sg_status mx4_product(const sg_mx4 *w, const sg_mx4 *up, const sg_moe_plan *plan
     }
     CK(mx4_quantize_launch(q, type, di->sms, s));
     g.vec = rows16(d_out, ldo, eo);
-    CK(mp.shift == 7 ? mx4_many_launch(g, mp.token_tiles, di->sms, s) : mx4_gemm_launch(g, mp.shift, mp.token_tiles, di->sms, s));
+    CK(mp.many ? mx4_many_launch(g, mp.token_tiles, di->sms, s) : mx4_few_launch(g, mp.shift, mp.token_tiles, di->sms, s));
     return SG_OK;
 }
 
@@ -2726,7 +2730,7 @@ sg_status sg_mx4_dequantize(const sg_mx4 *m, int32_t type, void *d_out, uint64_t
 uint64_t sg_mx4_scratch_bytes(const sg_mx4 *w, uint64_t n_tok, const sg_moe_plan *plan) {
     if (check_mx4(w, false) || n_tok >= 1ull << 31) return 0;
     if (plan && (!plan->n_used || !plan->n_expert || plan->n_tok >= 1ull << 31 || plan->n_used > MOE_SORT_MAX_USED)) return 0;
-    return mx4_scratch(w, mx4_plan(n_tok, plan));
+    return mx4_scratch(w, mx4_plan(w, n_tok, plan));
 }
 
 sg_status sg_mx4_matmul(const sg_mx4 *w, const sg_mx4 *up, int32_t type, const void *d_x, uint64_t ldx, uint64_t n_tok, int32_t out_type,

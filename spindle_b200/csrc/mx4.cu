@@ -82,6 +82,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(MX4_QUANT_THREADS) mx4_quantize_kernel(const __grid_constant__ Mx4QuantArgs a) {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, chunk = lane >> 2;
     const uint32_t tile_bytes = mx4_tile_bytes(1u << a.tile_shift), mask = (1u << a.tile_shift) - 1, rows_at_once = gridDim.x * (MX4_QUANT_THREADS / 32);
+    if (a.early) grid_launch_dependents();
     for (uint32_t kt0 = blockIdx.y * QUANT_TILES; kt0 < a.nk; kt0 += gridDim.y * QUANT_TILES)
         for (uint64_t i = blockIdx.x * (MX4_QUANT_THREADS / 32) + warp; i < a.n_rows; i += rows_at_once) {
             const T *src = static_cast<const T *>(a.x);
@@ -143,7 +144,6 @@ __global__ void __launch_bounds__(MX4_QUANT_THREADS) mx4_quantize_kernel(const _
                 }
             }
         }
-    grid_launch_dependents();
 }
 
 // The values of two codes.

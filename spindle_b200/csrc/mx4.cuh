@@ -51,6 +51,7 @@ struct Mx4QuantArgs {
     uint32_t n_used;
     const int32_t *ids, *place, *order, *first, *tiles;
     bool vec;                      // x allows 16-byte loads
+    bool early;                    // the next launch may begin at once: it waits for this one before it reads what is written here
 };
 constexpr uint32_t MX4_QUANT_THREADS = 256;
 cudaError_t mx4_quantize_launch(const Mx4QuantArgs &a, int32_t type, int sms, cudaStream_t s);
@@ -79,7 +80,7 @@ struct Mx4GemmArgs {
     bool vec;                      // out allows 16-byte stores of eight features
 };
 cudaError_t mx4_many_launch(const Mx4GemmArgs &a, uint64_t token_tiles, int sms, cudaStream_t s);
-cudaError_t mx4_gemm_launch(const Mx4GemmArgs &a, uint32_t tile_shift, uint64_t token_tiles, int sms, cudaStream_t s);
+cudaError_t mx4_few_launch(const Mx4GemmArgs &a, uint32_t tile_shift, uint64_t token_tiles, int sms, cudaStream_t s);
 
 // The choice of experts and the sorting of its pairs.
 constexpr uint32_t MOE_SORT_MAX_EXPERTS = 1024, MOE_SORT_MAX_USED = 16, MOE_SORT_TOKENS = 64;

@@ -25,12 +25,8 @@ using namespace tiled;
 namespace {
 
 constexpr uint32_t EPI_WARPS = 16, FIRST_EPI = 4, THREADS = 32 * (FIRST_EPI + EPI_WARPS);
-constexpr uint32_t MAX_E = MOE_SORT_MAX_EXPERTS;
-constexpr uint32_t HDR = 1024 + 3 * 4 * MAX_E;   // barriers and TMEM base; what is looked up of the experts
+constexpr uint32_t HDR = 1024 + EXPERTS_BYTES;     // barriers and TMEM base; what is looked up of the experts
 constexpr uint32_t GROUPS = EPI_WARPS / 4;       // four warps take a piece of 16 tokens, 32 features each
-constexpr uint32_t OUT_ROW = MX4_ROWS * 2 + 16;  // 16-bit results of a token in shared memory, and padding
-constexpr uint32_t OUT_BYTES = 2 * 16 * OUT_ROW; // two such pieces, or one of f32
-static_assert(OUT_BYTES >= 16 * (MX4_ROWS * 4 + 16), "a piece of f32");
 
 template <bool DUAL>
 struct Cfg {
@@ -49,35 +45,10 @@ struct Cfg {
 
 struct Shared {
     uint64_t full[8], empty[8], sums_full[2], sums_empty[2];
-    uint32_t tmem, n_rows;
+    uint32_t tmem;
 };
-// Of each expert: how many tiles end with it, its first sorted place, its first tile of x (a lookup from global memory took
-// every role 0.7 us a tile).
-struct Experts {
-    uint32_t upto[MAX_E], first[MAX_E], x_tile[MAX_E];
-};
-static_assert(sizeof(Shared) <= 1024 && sizeof(Experts) == HDR - 1024, "places");
+static_assert(sizeof(Shared) <= 1024 && sizeof(Experts) <= EXPERTS_BYTES, "places");
 
-__device__ __forceinline__ bool try_wait_cluster(uint64_t *bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// Bounded: a wait that does not end is recorded, and everybody goes home.
-__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity) {
-    for (int i = 0; i < 16; i++)
-        if (try_wait_cluster(bar, parity)) return true;
-    const uint64_t t0 = globaltimer_ns();
-    for (;;) {
-        for (int i = 0; i < 64; i++)
-            if (try_wait_cluster(bar, parity)) return true;
-        if (globaltimer_ns() - t0 > WAIT_LIMIT_NS) return false;
-    }
-}
 // Arrives at the barrier of the pair's CTA `rank` that lies where bar does here.  Relaxed: what it tells of are bulk copies
 // and TMEM loads, whose end this thread has seen; nothing that it wrote itself is handed over.  (With release each arrival
 // takes 500 ns, which made a stage of the pipeline 640 to 800 ns long instead of 330.)
@@ -86,64 +57,6 @@ __device__ __forceinline__ void arrive_at(uint64_t *bar, uint32_t rank) {
         "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [a];\n}" ::"r"(smem_u32(bar)),
         "r"(rank)
         : "memory");
-}
-
-// A tile: up to NT rows of x, those of one expert, from row row0 of the output on.
-struct Tile {
-    uint32_t e, x_tile, in, rows, fp;  // (x: from row `in` of its tile x_tile on)
-    uint64_t row0;
-};
-
-__device__ __forceinline__ uint32_t pack(__half, float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ uint32_t pack(__nv_bfloat16, float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
-// A piece of 16 tokens (n of them are there) by 128 features from f0 on, of which a warp has 32 in v as tmem_ld32x16 gives
-// them, to rows of the output from `row` on: by way of shared memory, where the four warps' features of a token come
-// together.  16-bit results go there eight by eight, turned over on the way (stmatrix), to one of two places in turn, so that
-// one barrier a piece will do.
-template <typename T>
-__device__ __forceinline__ void put_piece(const Mx4GemmArgs &a, uint8_t *buf, const float *v, uint64_t row, uint32_t n, uint32_t f0, uint32_t warp,
-                                          uint32_t lane, uint32_t group) {
-    constexpr uint32_t ROW = MX4_ROWS * sizeof(T) + 16, PER = MX4_ROWS * sizeof(T) / 16, ES = 16 / sizeof(T);
-    if constexpr (sizeof(T) == 2) {
-        const uint32_t at = smem_u32(buf) + (lane & 7) * ROW + (32 * warp + 8 * (lane >> 3)) * 2;
-#pragma unroll
-        for (uint32_t b = 0; b < 2; b++) {
-            const float *lo = v + 4 * b, *hi = v + 8 + 4 * b;
-            asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at + 8 * b * ROW), "r"(pack(T(), lo[0], lo[1])),
-                         "r"(pack(T(), lo[2], lo[3])), "r"(pack(T(), hi[0], hi[1])), "r"(pack(T(), hi[2], hi[3]))
-                         : "memory");
-        }
-    } else {
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");  // the piece before has been read
-        float *at = reinterpret_cast<float *>(buf + 2 * (lane & 3) * ROW) + 32 * warp + (lane >> 2);
-#pragma unroll
-        for (uint32_t b = 0; b < 2; b++)
-#pragma unroll
-            for (uint32_t i = 0; i < 8; i++)  // (token 8 b + 2 (lane % 4) + i % 2, feature 8 (i / 2) + lane / 4 of the warp's)
-                at[(8 * b + (i & 1)) * (ROW / 4) + 8 * (i >> 1)] = v[(i >> 2) * 8 + 4 * b + (i & 3)];
-    }
-    asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
-    T *out = static_cast<T *>(a.out);
-#pragma unroll
-    for (uint32_t i = 0; i < 16 * PER / 128; i++) {
-        const uint32_t at = i * 128 + 32 * warp + lane, t = at / PER, c = at % PER, f = f0 + c * ES;
-        if (t < n && f < a.feats) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(buf + t * ROW + 16 * c);
-            T *o = out + (row + t) * a.ldo + f;
-            if (a.vec && f + ES <= a.feats) *reinterpret_cast<uint4 *>(o) = w;
-            else
-#pragma unroll
-                for (uint32_t j = 0; j < ES; j++)
-                    if (f + j < a.feats) o[j] = reinterpret_cast<const T *>(&w)[j];
-        }
-    }
 }
 
 template <bool DUAL>
@@ -166,64 +79,19 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
         fence_mbar_init();
     }
     if (warp == 3) tmem_alloc<2>(&sh.tmem, C::COLS);
-    uint32_t token_tiles;
-    if (a.first) {
-        if (warp == 0) {
-            uint32_t before = 0;
-            for (uint32_t base = 0; base < a.n_expert; base += 32) {
-                const uint32_t i = base + lane;
-                const uint32_t f0 = i < a.n_expert ? (uint32_t)__ldg(a.first + i) : 0, f1 = i < a.n_expert ? (uint32_t)__ldg(a.first + i + 1) : 0;
-                uint32_t n = (f1 - f0 + C::NT - 1) / C::NT;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint32_t v = __shfl_up_sync(0xffffffffu, n, o);
-                    if (lane >= (uint32_t)o) n += v;
-                }
-                if (i < a.n_expert) {
-                    ex.upto[i] = before + n;
-                    ex.first[i] = f0;
-                    ex.x_tile[i] = (uint32_t)__ldg(a.tiles + i);
-                    if (i + 1 == a.n_expert) sh.n_rows = f1;
-                }
-                before += __shfl_sync(0xffffffffu, n, 31);
-            }
-        }
-    }
+    if (a.first && warp == 0) find_experts(a, ex, C::NT, lane);
     fence_before();
     __syncthreads();
     cluster.sync();
     fence_after();
-    token_tiles = a.first ? ex.upto[a.n_expert - 1] : (uint32_t)((a.n_tok + C::NT - 1) / C::NT);
+    const uint32_t token_tiles = a.first ? ex.upto[a.n_expert - 1] : (uint32_t)((a.n_tok + C::NT - 1) / C::NT);
     const uint32_t tmem = sh.tmem, pairs = gridDim.x / 2, me = blockIdx.x / 2;
     const uint32_t fps = (a.feat_tiles + 1) / 2;
     const uint32_t tiles = token_tiles * fps;
 
-    auto tile_at = [&](uint32_t i) {
-        Tile t;
-        const uint32_t tt = i / fps;
-        t.fp = i - tt * fps;
-        if (a.first) {
-            uint32_t lo = 0, hi = a.n_expert - 1;  // the first expert whose tiles reach past tt
-            while (lo < hi) {
-                const uint32_t mid = (lo + hi) / 2;
-                if (ex.upto[mid] > tt) hi = mid;
-                else lo = mid + 1;
-            }
-            const uint32_t k = tt - (lo ? ex.upto[lo - 1] : 0), f0 = ex.first[lo], n = (lo + 1 < a.n_expert ? ex.first[lo + 1] : sh.n_rows) - f0;
-            t.e = lo;
-            t.x_tile = ex.x_tile[lo] + k * C::NT / 128;
-            t.in = k * C::NT % 128;
-            t.rows = min(n - k * C::NT, C::NT);
-            t.row0 = f0 + k * C::NT;
-        } else {
-            t.e = 0;
-            t.row0 = (uint64_t)tt * C::NT;
-            t.x_tile = (uint32_t)(t.row0 / 128);
-            t.in = (uint32_t)(t.row0 % 128);
-            t.rows = (uint32_t)(a.n_tok - t.row0 < C::NT ? a.n_tok - t.row0 : C::NT);
-        }
-        return t;
-    };
+    // (the feature pairs of a token tile follow each other: an expert's weights are read once, by neighbours)
+    auto tile_at = [&](uint32_t i) { return tile_of<C::NT, 128>(a, ex, i / fps); };
+    auto pair_of = [&](uint32_t i) { return i % fps; };
 
     bool ok = true;
     if (warp < 3) {
@@ -232,7 +100,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
         for (uint32_t i = me; i < tiles && ok; i += pairs) {
             const Tile t = tile_at(i);
             const uint32_t n = (t.rows + 31) & ~31u, half = n / 2, r0 = t.in + rank * half;  // this CTA's tokens: r0 .. r0 + half
-            const uint32_t ft = min(2 * t.fp + rank, a.feat_tiles - 1);
+            const uint32_t ft = min(2 * pair_of(i) + rank, a.feat_tiles - 1);
             const uint64_t w_at = (uint64_t)t.e * a.expert_bytes + (uint64_t)ft * a.nk * MX4_TILE, next = (uint64_t)a.nk * MX4_TILE;
             const uint8_t *w = a.w + w_at, *up = DUAL ? a.up + w_at : nullptr, *x = a.x + (uint64_t)t.x_tile * next;
             // rows from the first of them on in its tile of 128, and what is left of it
@@ -364,7 +232,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
             __syncwarp();
             if (elect_one()) arrive_at(&sh.sums_empty[b], 0);
             __syncwarp();
-            const uint32_t f0 = (2 * t.fp + rank) * MX4_ROWS;
+            const uint32_t f0 = (2 * pair_of(i) + rank) * MX4_ROWS;
             if (f0 >= a.feats) continue;
 #pragma unroll
             for (uint32_t c = 0; c < C::PIECES; c++)

@@ -127,5 +127,147 @@ __device__ __forceinline__ float silu_times(float g, float u) {
     return (g < 0.0f ? e : 1.0f) * (q * (g * u));
 }
 
+// ---- what the kernels have in common ----
+
+constexpr uint32_t MAX_E = MOE_SORT_MAX_EXPERTS;
+constexpr uint32_t OUT_ROW = MX4_ROWS * 2 + 16;   // 16-bit results of a token in shared memory, and padding
+constexpr uint32_t OUT_BYTES = 2 * 16 * OUT_ROW;  // two pieces of 16 tokens, or one of f32
+static_assert(OUT_BYTES >= 16 * (MX4_ROWS * 4 + 16), "a piece of f32");
+
+__device__ __forceinline__ bool try_wait_cluster(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Bounded: a wait that does not end is recorded, and everybody goes home.
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity) {
+    for (int i = 0; i < 16; i++)
+        if (try_wait_cluster(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    for (;;) {
+        for (int i = 0; i < 64; i++)
+            if (try_wait_cluster(bar, parity)) return true;
+        if (globaltimer_ns() - t0 > WAIT_LIMIT_NS) return false;
+    }
+}
+// Of each expert: how many tiles end with it, its first sorted place, its first tile of x (a lookup from global memory took
+// every role 0.7 us a tile).
+struct Experts {
+    uint32_t upto[MAX_E], first[MAX_E], x_tile[MAX_E], n_rows;
+};
+constexpr uint32_t EXPERTS_BYTES = 3 * 4 * MAX_E + 1024;
+
+// A tile: up to NT rows of x (from row `in` of its tile x_tile on), those of one expert, to rows of the output from row0 on.
+struct Tile {
+    uint32_t e, x_tile, in, rows;
+    uint64_t row0;
+};
+
+// The experts' lookups for tiles of NT tokens, by one warp; the number of tiles of all.  rows: of x a tile of it has.
+__device__ __forceinline__ void find_experts(const Mx4GemmArgs &a, Experts &ex, uint32_t nt, uint32_t lane) {
+    uint32_t before = 0;
+    for (uint32_t base = 0; base < a.n_expert; base += 32) {
+        const uint32_t i = base + lane;
+        const uint32_t f0 = i < a.n_expert ? (uint32_t)__ldg(a.first + i) : 0, f1 = i < a.n_expert ? (uint32_t)__ldg(a.first + i + 1) : 0;
+        uint32_t n = (f1 - f0 + nt - 1) / nt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, n, o);
+            if (lane >= (uint32_t)o) n += v;
+        }
+        if (i < a.n_expert) {
+            ex.upto[i] = before + n;
+            ex.first[i] = f0;
+            ex.x_tile[i] = (uint32_t)__ldg(a.tiles + i);
+            if (i + 1 == a.n_expert) ex.n_rows = f1;
+        }
+        before += __shfl_sync(0xffffffffu, n, 31);
+    }
+}
+
+// The tt-th tile of NT tokens, x in tiles of XROWS rows.
+template <uint32_t NT, uint32_t XROWS>
+__device__ __forceinline__ Tile tile_of(const Mx4GemmArgs &a, const Experts &ex, uint32_t tt) {
+    Tile t;
+    if (a.first) {
+        uint32_t lo = 0, hi = a.n_expert - 1;  // the first expert whose tiles reach past tt
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (ex.upto[mid] > tt) hi = mid;
+            else lo = mid + 1;
+        }
+        const uint32_t r = (tt - (lo ? ex.upto[lo - 1] : 0)) * NT, f0 = ex.first[lo], n = (lo + 1 < a.n_expert ? ex.first[lo + 1] : ex.n_rows) - f0;
+        t.e = lo;
+        t.x_tile = ex.x_tile[lo] + r / XROWS;
+        t.in = r % XROWS;
+        t.rows = min(n - r, NT);
+        t.row0 = f0 + r;
+    } else {
+        t.e = 0;
+        t.row0 = (uint64_t)tt * NT;
+        t.x_tile = (uint32_t)(t.row0 / XROWS);
+        t.in = (uint32_t)(t.row0 % XROWS);
+        t.rows = (uint32_t)(a.n_tok - t.row0 < NT ? a.n_tok - t.row0 : NT);
+    }
+    return t;
+}
+
+__device__ __forceinline__ uint32_t pack(__half, float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack(__nv_bfloat16, float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// A piece of 16 tokens (n of them are there) by 128 features from f0 on, of which a warp has 32 in v as tmem_ld32x16 gives
+// them, to rows of the output from `row` on: by way of shared memory, where the four warps' features of a token come
+// together.  16-bit results go there eight by eight, turned over on the way (stmatrix), to one of two places in turn, so that
+// one barrier a piece will do.
+template <typename T>
+__device__ __forceinline__ void put_piece(const Mx4GemmArgs &a, uint8_t *buf, const float *v, uint64_t row, uint32_t n, uint32_t f0, uint32_t warp,
+                                          uint32_t lane, uint32_t group) {
+    constexpr uint32_t ROW = MX4_ROWS * sizeof(T) + 16, PER = MX4_ROWS * sizeof(T) / 16, ES = 16 / sizeof(T);
+    if constexpr (sizeof(T) == 2) {
+        const uint32_t at = smem_u32(buf) + (lane & 7) * ROW + (32 * warp + 8 * (lane >> 3)) * 2;
+#pragma unroll
+        for (uint32_t b = 0; b < 2; b++) {
+            const float *lo = v + 4 * b, *hi = v + 8 + 4 * b;
+            asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at + 8 * b * ROW), "r"(pack(T(), lo[0], lo[1])),
+                         "r"(pack(T(), lo[2], lo[3])), "r"(pack(T(), hi[0], hi[1])), "r"(pack(T(), hi[2], hi[3]))
+                         : "memory");
+        }
+    } else {
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");  // the piece before has been read
+        float *at = reinterpret_cast<float *>(buf + 2 * (lane & 3) * ROW) + 32 * warp + (lane >> 2);
+#pragma unroll
+        for (uint32_t b = 0; b < 2; b++)
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++)  // (token 8 b + 2 (lane % 4) + i % 2, feature 8 (i / 2) + lane / 4 of the warp's)
+                at[(8 * b + (i & 1)) * (ROW / 4) + 8 * (i >> 1)] = v[(i >> 2) * 8 + 4 * b + (i & 3)];
+    }
+    asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+    T *out = static_cast<T *>(a.out);
+#pragma unroll
+    for (uint32_t i = 0; i < 16 * PER / 128; i++) {
+        const uint32_t at = i * 128 + 32 * warp + lane, t = at / PER, c = at % PER, f = f0 + c * ES;
+        if (t < n && f < a.feats) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(buf + t * ROW + 16 * c);
+            T *o = out + (row + t) * a.ldo + f;
+            if (a.vec && f + ES <= a.feats) *reinterpret_cast<uint4 *>(o) = w;
+            else
+#pragma unroll
+                for (uint32_t j = 0; j < ES; j++)
+                    if (f + j < a.feats) o[j] = reinterpret_cast<const T *>(&w)[j];
+        }
+    }
+}
+
+
 }  // namespace mx4
 }  // namespace sg
