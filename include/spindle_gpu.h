@@ -704,7 +704,7 @@ SG_API sg_status sg_mx4_matmul(const sg_mx4 *w, const sg_mx4 *up, int32_t type, 
  *   order [n_tok * n_used]: the pair at each place, -1 past first[n_expert]; pairs of
  *     one expert stand in rising order;
  *   place [n_tok * n_used]: the place of each pair, -1 for none;
- *   work: sg_moe_plan_work_bytes(n_tok, n_expert) bytes.
+ *   work: sg_moe_plan_work_bytes(n_tok, n_expert) bytes, 16-byte aligned.
  * n_used <= SG_MOE_MAX_USED, n_expert <= 1024, n_tok * n_used < 2^31. */
 struct sg_moe_plan_ {
     uint64_t n_tok, n_used, n_expert;

@@ -2610,12 +2610,15 @@ sg_status check_plan(const sg_moe_plan *p) {
     if (!p->n_used || p->n_used > MOE_SORT_MAX_USED || !p->n_expert || p->n_expert > MOE_SORT_MAX_EXPERTS) return SG_ERR_SHAPE;
     if (p->n_tok >= 1ull << 31 || p->n_tok * p->n_used >= 1ull << 31) return SG_ERR_SHAPE;
     if (!p->first || !p->work || (p->n_tok && (!p->ids || !p->weights || !p->order || !p->place))) return SG_ERR_INVALID;
-    return SG_OK;
+    return aligned(p->work, 16) ? SG_OK : SG_ERR_ALIGN;
 }
-// CTAs that sort: a stretch of 64 tokens or more each
-uint32_t sort_ctas(uint64_t n_tok) {
-    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(128, (n_tok + MOE_SORT_TOKENS - 1) / MOE_SORT_TOKENS));
+// Tokens whose experts a CTA chooses: a step's all, otherwise 16, one a warp, or as many more as make 512 CTAs.
+uint32_t sort_stretch(uint64_t n_tok) {
+    if (n_tok <= MOE_SORT_GROUP) return MOE_SORT_GROUP;
+    return (uint32_t)std::max<uint64_t>(16, align_up((n_tok + 511) / 512, 16));
 }
+uint32_t sort_stretches(uint64_t n_tok) { return (uint32_t)std::max<uint64_t>(1, (n_tok + sort_stretch(n_tok) - 1) / sort_stretch(n_tok)); }
+uint64_t counts_at(uint64_t n_expert) { return align_up(3 * (n_expert + 1), 4); }
 // plan->work: first tiles for tiles of 32, 64 and 128 rows, then the stretches' counts
 int32_t *plan_tiles(const sg_moe_plan *p, uint32_t shift) { return p->work + (shift - 5) * (p->n_expert + 1); }
 
@@ -2682,9 +2685,10 @@ sg_status check_product(const sg_mx4 *w, const sg_mx4 *up, uint64_t experts) {
 
 MoeSortArgs sort_args(const sg_moe_plan *p) {
     MoeSortArgs a = {};
-    a.n_tok = (uint32_t)p->n_tok, a.n_expert = (uint32_t)p->n_expert, a.n_used = (uint32_t)p->n_used, a.ctas = sort_ctas(p->n_tok);
+    a.n_tok = (uint32_t)p->n_tok, a.n_expert = (uint32_t)p->n_expert, a.n_used = (uint32_t)p->n_used;
+    a.stretch = sort_stretch(p->n_tok), a.stretches = sort_stretches(p->n_tok);
     a.ids = p->ids, a.weights = p->weights, a.first = p->first, a.order = p->order, a.place = p->place;
-    a.tiles = p->work, a.counts = p->work + 3 * (p->n_expert + 1);
+    a.tiles = p->work, a.counts = p->work + counts_at(p->n_expert), a.counts_ld = (uint32_t)align_up(p->n_expert, 4);
     return a;
 }
 
@@ -2741,8 +2745,9 @@ sg_status sg_mx4_matmul(const sg_mx4 *w, const sg_mx4 *up, int32_t type, const v
 
 uint64_t sg_moe_plan_work_bytes(uint64_t n_tok, uint64_t n_expert) {
     if (!n_expert || n_expert > MOE_SORT_MAX_EXPERTS || n_tok >= 1ull << 31) return 0;
-    const uint32_t ctas = sort_ctas(n_tok);
-    return 4 * (3 * (n_expert + 1) + (ctas > 1 ? ctas * n_expert : 0));
+    if (n_tok <= MOE_SORT_GROUP) return 4 * 3 * (n_expert + 1);
+    // (up to 512 stretches, of fewer tokens than n_tok as well)
+    return 4 * (counts_at(n_expert) + std::min<uint64_t>(512 / MOE_SORT_JOIN, (n_tok + 16 * MOE_SORT_JOIN - 1) / (16 * MOE_SORT_JOIN)) * align_up(n_expert, 4));
 }
 
 sg_status sg_moe_route(int32_t type, const void *d_logits, uint64_t ld, int32_t norm, float prune, const sg_moe_plan *plan, void *stream) {

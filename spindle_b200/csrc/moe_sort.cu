@@ -2,17 +2,22 @@
 // router's logits, the stable sort of the (token, choice) pairs by expert, and the weighted sum
 // of the experts' results.
 //
-// The sort is a counting sort: a CTA per stretch of tokens counts its experts, a second launch
-// adds up the counts of the stretches before its own (all of them, for the places of the experts)
-// and gives each pair its place by counting the bits of the pairs before it with the same expert.
-// What bounds it: a step of a few tokens, the chain of dependent steps in one CTA; a prompt,
-// the logits' bytes.
+// The sort is a counting sort: a CTA per stretch of tokens (one a warp) chooses and counts their
+// experts, four of them together make a row of counts; a second launch adds up the rows before its
+// own (all of them, for the places of the experts) and gives each pair its place by counting the bits of the pairs before it
+// with the same expert.  A step of up to 64 tokens is one CTA's work.  What bounds it: the chain of
+// dependent steps, launches among them.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "mx4.cuh"
+#include "tiled_block.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace sg {
+using namespace tiled;
 
 namespace {
 
@@ -50,10 +55,9 @@ __device__ __forceinline__ int32_t choose(const MoeSortArgs &a, uint32_t t, uint
     uint32_t key[R];
 #pragma unroll
     for (int i = 0; i < R; i++) key[i] = lane + 32 * i < a.n_expert ? key_of(widen(x[lane + 32 * i])) : 0;
-    float top = 0.0f, mine = 0.0f, all = 0.0f;
+    uint32_t mine_key = 0, top_key = 0, found = 0;
     int32_t id = -1;
-    uint32_t found = 0;
-    for (uint32_t j = 0; j < a.n_used; j++) {
+    for (; found < a.n_used; found++) {
         uint32_t best = key[0], at = 0;
 #pragma unroll
         for (int i = 1; i < R; i++)
@@ -62,20 +66,19 @@ __device__ __forceinline__ int32_t choose(const MoeSortArgs &a, uint32_t t, uint
         if (most == 0) break;
         // equal ones: the lowest number
         const uint32_t e = __reduce_min_sync(0xffffffffu, best == most ? lane + 32 * at : 0xFFFFFFFFu);
-        if (j == 0) {
-            top = value_of(most);
-            if (!a.norm) {
-#pragma unroll
-                for (int i = 0; i < R; i++)
-                    if (key[i]) all += expf(value_of(key[i]) - top);
-                all = warp_sum(all);
-            }
-        }
-        if (lane == j) id = (int32_t)e, mine = expf(value_of(most) - top);
+        if (found == 0) top_key = most;
+        if (lane == found) id = (int32_t)e, mine_key = most;
 #pragma unroll
         for (int i = 0; i < R; i++)
             if (lane + 32 * i == e) key[i] = 0;
-        found++;
+    }
+    const float top = found ? value_of(top_key) : 0.0f;
+    float mine = id < 0 ? 0.0f : expf(value_of(mine_key) - top), all = 0.0f;
+    if (!a.norm) {  // the sum over the others too
+#pragma unroll
+        for (int i = 0; i < R; i++)
+            if (key[i]) all += expf(value_of(key[i]) - top);
+        all = warp_sum(all + mine);
     }
     // pruning, as the framework's one-token layer does it
     uint32_t keep = found;
@@ -98,74 +101,77 @@ __device__ __forceinline__ int32_t choose(const MoeSortArgs &a, uint32_t t, uint
     return id;
 }
 
-struct Stretch {
-    uint32_t t0, t1;
-};
-__device__ __forceinline__ Stretch stretch(const MoeSortArgs &a, uint32_t cta) {
-    const uint32_t groups = (a.n_tok + MOE_SORT_TOKENS - 1) / MOE_SORT_TOKENS;
-    const uint32_t g0 = (uint32_t)((uint64_t)groups * cta / a.ctas), g1 = (uint32_t)((uint64_t)groups * (cta + 1) / a.ctas);
-    return {g0 * MOE_SORT_TOKENS, min(g1 * MOE_SORT_TOKENS, a.n_tok)};
-}
-
-// Inclusive sum over the CTA of one value a thread (sums: WARPS words).
-__device__ __forceinline__ uint32_t cta_scan(uint32_t v, uint32_t *sums) {
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+// Exclusive sums of f(e) over the experts, by one warp: put(e, sum before e), and the sum of all.
+template <typename F, typename P>
+__device__ __forceinline__ uint32_t warp_sums(uint32_t n, uint32_t lane, F f, P put) {
+    uint32_t before = 0;
+    for (uint32_t base = 0; base < n; base += 128) {  // four experts a lane
+        uint32_t v[4], sum = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= (uint32_t)o) v += u;
-    }
-    if (lane == 31) sums[warp] = v;
-    __syncthreads();
-    uint32_t w = lane < WARPS ? sums[lane] : 0;
-#pragma unroll
-    for (int o = 1; o < (int)WARPS; o <<= 1) {
-        const uint32_t u = __shfl_up_sync(0xffffffffu, w, o);
-        if (lane >= (uint32_t)o) w += u;
-    }
-    const uint32_t before = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
-    __syncthreads();
-    return v + (warp ? before : 0);
-}
-
-// Places of the pairs of this CTA's tokens.  at: the first place of each expert here, on entry its counts in the stretches
-// before; total: the counts of all.  mask: zeroed, n_expert rows of n_used * 2 words.
-__device__ __forceinline__ void place_pairs(const MoeSortArgs &a, uint32_t cta, uint32_t *at, const uint32_t *total, uint32_t *mask, uint32_t *sums) {
-    const uint32_t tid = threadIdx.x, E = a.n_expert;
-    // thread i has experts 2 i and 2 i + 1
-    const uint32_t e0 = 2 * tid, c0 = e0 < E ? total[e0] : 0, c1 = e0 + 1 < E ? total[e0 + 1] : 0;
-    const uint32_t upto = cta_scan(c0 + c1, sums);
-    if (e0 < E) at[e0] += upto - c1 - c0;
-    if (e0 + 1 < E) at[e0 + 1] += upto - c1;
-    if (cta == 0) {
-        if (e0 < E) a.first[e0] = (int32_t)(upto - c1 - c0);
-        if (e0 + 1 < E) a.first[e0 + 1] = (int32_t)(upto - c1);
-        if (tid == THREADS - 1) a.first[E] = (int32_t)upto;
-#pragma unroll
-        for (uint32_t k = 0; k < 3; k++) {
-            const uint32_t r = (32u << k) - 1, n0 = (c0 + r) >> (5 + k), n1 = (c1 + r) >> (5 + k);
-            const uint32_t u = cta_scan(n0 + n1, sums);
-            int32_t *tiles = a.tiles + (uint64_t)k * (E + 1);
-            if (e0 < E) tiles[e0] = (int32_t)(u - n1 - n0);
-            if (e0 + 1 < E) tiles[e0 + 1] = (int32_t)(u - n1);
-            if (tid == THREADS - 1) tiles[E] = (int32_t)u;
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t e = base + 4 * lane + i;
+            v[i] = e < n ? f(e) : 0;
+            sum += v[i];
         }
+        uint32_t upto = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= (uint32_t)o) upto += u;
+        }
+        uint32_t at = before + upto - sum;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t e = base + 4 * lane + i;
+            if (e < n) put(e, at);
+            at += v[i];
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    if (tid == THREADS - 1) sums[WARPS] = upto;
+    return before;
+}
+
+// Shared memory: the first place of each expert for the pairs here, the counts of all, bits of a group's pairs, all pairs.
+struct Tables {
+    uint32_t *at, *total, *mask, *all;
+};
+// (a word more than the bits need: rows that begin in different banks)
+__host__ __device__ constexpr uint32_t mask_words(uint32_t used) { return MOE_SORT_GROUP * used / 32 + 1; }
+__host__ __device__ constexpr uint32_t sort_smem(uint32_t experts, uint32_t used) { return (2 * experts + experts * mask_words(used) + 1) * 4; }
+__device__ __forceinline__ Tables tables(const MoeSortArgs &a, uint32_t *sm) { return {sm, sm + a.n_expert, sm + 2 * a.n_expert, sm + sort_smem(a.n_expert, a.n_used) / 4 - 1}; }
+
+// Places of the pairs of the tokens t0 .. t1.  at: on entry the experts' counts in the tokens before; total: those of all.
+// mask: zeroed.  first: this CTA writes what all have in common.
+__device__ __forceinline__ void place_pairs(const MoeSortArgs &a, const Tables &m, uint32_t t0, uint32_t t1, bool first) {
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, E = a.n_expert;
+    const uint32_t *total = m.total;
+    if (warp == 0) {
+        const uint32_t all = warp_sums(E, lane, [&](uint32_t e) { return total[e]; }, [&](uint32_t e, uint32_t v) {
+            m.at[e] += v;
+            if (first) a.first[e] = (int32_t)v;
+        });
+        if (lane == 0) *m.all = all;
+        if (first && lane == 0) a.first[E] = (int32_t)all;
+    } else if (warp < 4 && first) {  // tiles of 32, 64 and 128 rows
+        const uint32_t shift = warp + 4, r = (1u << shift) - 1;
+        int32_t *tiles = a.tiles + (uint64_t)(warp - 1) * (E + 1);
+        const uint32_t all = warp_sums(E, lane, [&](uint32_t e) { return (total[e] + r) >> shift; }, [&](uint32_t e, uint32_t v) { tiles[e] = (int32_t)v; });
+        if (lane == 0) tiles[E] = (int32_t)all;
+    }
     __syncthreads();
-    const uint64_t pairs = (uint64_t)a.n_tok * a.n_used;
-    for (uint64_t s = sums[WARPS] + (uint64_t)cta * THREADS + tid; s < pairs; s += (uint64_t)a.ctas * THREADS) a.order[s] = -1;
-    const uint32_t words = MOE_SORT_TOKENS * a.n_used / 32;
-    const Stretch st = stretch(a, cta);
-    for (uint32_t t = st.t0; t < st.t1; t += MOE_SORT_TOKENS) {
-        const uint32_t n = min(MOE_SORT_TOKENS, st.t1 - t) * a.n_used;  // pairs, at most 1024
+    // places that no pair has
+    const uint64_t pairs = (uint64_t)a.n_tok * a.n_used, ctas = (a.stretches + MOE_SORT_JOIN - 1) / MOE_SORT_JOIN;
+    for (uint64_t s = *m.all + (uint64_t)blockIdx.x * THREADS + tid; s < pairs; s += ctas * THREADS) a.order[s] = -1;
+    const uint32_t words = mask_words(a.n_used);
+    for (uint32_t t = t0; t < t1; t += MOE_SORT_GROUP) {
+        const uint32_t n = min(MOE_SORT_GROUP, t1 - t) * a.n_used;  // pairs, at most 1024
         const uint64_t p0 = (uint64_t)t * a.n_used;
         int32_t e[2] = {-1, -1};
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const uint32_t p = tid + THREADS * i;
             if (p < n) e[i] = a.ids[p0 + p];
-            if (e[i] >= 0) atomicOr(&mask[e[i] * words + p / 32], 1u << (p & 31));
+            if (e[i] >= 0) atomicOr(&m.mask[e[i] * words + p / 32], 1u << (p & 31));
         }
         __syncthreads();
         uint32_t rank[2] = {}, count[2] = {};
@@ -173,90 +179,115 @@ __device__ __forceinline__ void place_pairs(const MoeSortArgs &a, uint32_t cta, 
         for (int i = 0; i < 2; i++) {
             const uint32_t p = tid + THREADS * i;
             if (e[i] >= 0) {
-                const uint32_t *m = mask + e[i] * words;
-                for (uint32_t w = 0; w < words; w++) {
-                    const uint32_t b = m[w];
+                const uint32_t *w = m.mask + e[i] * words;
+                for (uint32_t k = 0; k < words - 1; k++) {
+                    const uint32_t b = w[k];
                     count[i] += __popc(b);
-                    rank[i] += __popc(w < p / 32 ? b : w == p / 32 ? b & ((1u << (p & 31)) - 1) : 0);
+                    rank[i] += __popc(k < p / 32 ? b : k == p / 32 ? b & ((1u << (p & 31)) - 1) : 0);
                 }
-                const uint32_t s = at[e[i]] + rank[i];
+                const uint32_t s = m.at[e[i]] + rank[i];
                 a.order[s] = (int32_t)(p0 + p);
                 a.place[p0 + p] = (int32_t)s;
             } else if (p < n) a.place[p0 + p] = -1;
         }
-        if (t + MOE_SORT_TOKENS < st.t1) {
+        if (t + MOE_SORT_GROUP < t1) {
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < 2; i++)
                 if (e[i] >= 0) {
-                    if (rank[i] == 0) at[e[i]] += count[i];
-                    mask[e[i] * words + (tid + THREADS * i) / 32] = 0;
+                    if (rank[i] == 0) m.at[e[i]] += count[i];
+                    m.mask[e[i] * words + (tid + THREADS * i) / 32] = 0;
                 }
             __syncthreads();
         }
     }
 }
 
-__host__ __device__ constexpr uint32_t sort_smem(uint32_t experts, uint32_t used) {
-    return (2 * experts + WARPS + 1 + experts * (MOE_SORT_TOKENS * used / 32)) * 4;
-}
-
-// Choices (or the given ones, those outside 0..n_expert - 1 as none) and the counts of this stretch; a single CTA goes on to the places.
+// Choices (or the given ones, those outside 0..n_expert - 1 as none) of a.stretch tokens, and their counts; a single CTA goes
+// on to the places.
 template <typename T, int R>
-__global__ void __launch_bounds__(THREADS) moe_choose_kernel(const __grid_constant__ MoeSortArgs a) {
+__global__ void __launch_bounds__(THREADS, R <= 8 ? 4 : 2) moe_choose_kernel(const __grid_constant__ MoeSortArgs a) {
     extern __shared__ uint32_t sm[];
-    uint32_t *at = sm, *count = sm + a.n_expert, *sums = count + a.n_expert, *mask = sums + WARPS + 1;
+    const Tables m = tables(a, sm);
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    const uint32_t clear = a.ctas == 1 ? sort_smem(a.n_expert, a.n_used) / 4 : 2 * a.n_expert;
+    const bool alone = gridDim.x == 1;
+    const uint32_t clear = alone ? sort_smem(a.n_expert, a.n_used) / 4 : 2 * a.n_expert;
     for (uint32_t i = tid; i < clear; i += THREADS) sm[i] = 0;
     __syncthreads();
-    const Stretch st = stretch(a, blockIdx.x);
+    if (!alone) grid_launch_dependents();  // (the next launch clears its memory meanwhile)
+    const uint32_t t0 = (uint32_t)min((uint64_t)blockIdx.x * a.stretch, (uint64_t)a.n_tok), t1 = min(t0 + a.stretch, a.n_tok);
     if (a.logits) {
-        for (uint32_t t = st.t0 + warp; t < st.t1; t += WARPS) {
+        for (uint32_t t = t0 + warp; t < t1; t += WARPS) {
             float w;
             const int32_t id = choose<T, R>(a, t, lane, w);
             if (lane < a.n_used) {
                 a.ids[(uint64_t)t * a.n_used + lane] = id;
                 a.weights[(uint64_t)t * a.n_used + lane] = w;
-                if (id >= 0) atomicAdd(&count[id], 1u);
+                if (id >= 0) atomicAdd(&m.total[id], 1u);
             }
         }
     } else {
-        const uint64_t p1 = (uint64_t)st.t1 * a.n_used;
-        for (uint64_t p = (uint64_t)st.t0 * a.n_used + tid; p < p1; p += THREADS) {
+        const uint64_t p1 = (uint64_t)t1 * a.n_used;
+        for (uint64_t p = (uint64_t)t0 * a.n_used + tid; p < p1; p += THREADS) {
             const int32_t id = a.ids[p];
-            if (id >= 0 && (uint32_t)id < a.n_expert) atomicAdd(&count[id], 1u);
+            if (id >= 0 && (uint32_t)id < a.n_expert) atomicAdd(&m.total[id], 1u);
             else a.ids[p] = -1, a.weights[p] = 0.0f;
         }
     }
-    __syncthreads();
-    if (a.ctas == 1) place_pairs(a, 0, at, count, mask, sums);
-    else
-        for (uint32_t e = tid; e < a.n_expert; e += THREADS) a.counts[(uint64_t)blockIdx.x * a.n_expert + e] = (int32_t)count[e];
+    if (alone) {
+        __syncthreads();
+        place_pairs(a, m, t0, t1, true);
+        return;
+    }
+    // the counts of a cluster's stretches are one row
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const uint32_t rank = cluster.block_rank();
+    for (uint32_t e = rank + MOE_SORT_JOIN * tid; e < a.counts_ld; e += MOE_SORT_JOIN * THREADS) {
+        uint32_t n = 0;
+        if (e < a.n_expert)
+#pragma unroll
+            for (uint32_t r = 0; r < MOE_SORT_JOIN; r++) n += *cluster.map_shared_rank(m.total + e, r);
+        a.counts[(uint64_t)(blockIdx.x / MOE_SORT_JOIN) * a.counts_ld + e] = (int32_t)n;
+    }
+    cluster.sync();
 }
 
+// A CTA places the pairs of MOE_SORT_JOIN stretches, a row of counts: first the sums of all rows, and of those before its own.
 __global__ void __launch_bounds__(THREADS) moe_place_kernel(const __grid_constant__ MoeSortArgs a) {
     extern __shared__ uint32_t sm[];
-    uint32_t *at = sm, *total = sm + a.n_expert, *sums = total + a.n_expert, *mask = sums + WARPS + 1;
+    const Tables m = tables(a, sm);
     const uint32_t tid = threadIdx.x;
     for (uint32_t i = tid; i < sort_smem(a.n_expert, a.n_used) / 4; i += THREADS) sm[i] = 0;
     __syncthreads();
-    // the stretches in as many shares as the threads allow, an expert a thread
-    const uint32_t shares = max(1u, THREADS / a.n_expert), share = tid / a.n_expert;
-    if (share < shares)
-        for (uint32_t e = tid - share * a.n_expert; e < a.n_expert; e += THREADS) {
-            uint32_t all = 0, before = 0;
-#pragma unroll 8
-            for (uint32_t c = share; c < a.ctas; c += shares) {
-                const uint32_t n = (uint32_t)__ldg(a.counts + (uint64_t)c * a.n_expert + e);
-                all += n;
-                before += c < blockIdx.x ? n : 0;
+    grid_dependency_wait();
+    // four experts a thread, as many rows at once as the threads allow, eight loads in flight
+    const uint32_t per = a.counts_ld / 4, shares = THREADS / per, share = tid / per, c = tid - share * per, rows = gridDim.x;
+    if (share < shares) {
+        uint32_t all[4] = {}, before[4] = {};
+        for (uint32_t i0 = share; i0 < rows; i0 += 8 * shares) {
+            int4 v[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8; k++)
+                v[k] = i0 + k * shares < rows ? *(reinterpret_cast<const int4 *>(a.counts + (uint64_t)(i0 + k * shares) * a.counts_ld) + c) : make_int4(0, 0, 0, 0);
+#pragma unroll
+            for (uint32_t k = 0; k < 8; k++) {
+                const bool b = i0 + k * shares < blockIdx.x;
+                const uint32_t n[4] = {(uint32_t)v[k].x, (uint32_t)v[k].y, (uint32_t)v[k].z, (uint32_t)v[k].w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) all[j] += n[j], before[j] += b ? n[j] : 0;
             }
-            atomicAdd(&total[e], all);
-            atomicAdd(&at[e], before);
         }
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++)
+            if (4 * c + k < a.n_expert) {
+                if (all[k]) atomicAdd(&m.total[4 * c + k], all[k]);
+                if (before[k]) atomicAdd(&m.at[4 * c + k], before[k]);
+            }
+    }
     __syncthreads();
-    place_pairs(a, blockIdx.x, at, total, mask, sums);
+    const uint64_t t0 = (uint64_t)blockIdx.x * MOE_SORT_JOIN * a.stretch, n = a.n_tok;
+    place_pairs(a, m, (uint32_t)min(t0, n), (uint32_t)min(t0 + MOE_SORT_JOIN * a.stretch, n), blockIdx.x == 0);
 }
 
 // out[t] = sum over j of weights[t, j] y[place[t, j]], in the order of j, in f32.  A thread has eight columns of a token and
@@ -327,8 +358,18 @@ cudaError_t choose_as(const MoeSortArgs &a, uint32_t smem, cudaStream_t s) {
     static bool ready[64];
     cudaError_t e = big_smem(moe_choose_kernel<T, R>, smem, ready);
     if (e != cudaSuccess) return e;
-    moe_choose_kernel<T, R><<<a.ctas, THREADS, smem, s>>>(a);
-    return cudaGetLastError();
+    cudaLaunchConfig_t c = {};
+    const uint32_t cluster = a.stretches == 1 ? 1 : MOE_SORT_JOIN;
+    c.gridDim = dim3((a.stretches + cluster - 1) / cluster * cluster);
+    c.blockDim = dim3(THREADS);
+    c.dynamicSmemBytes = smem;
+    c.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {cluster, 1, 1};
+    c.attrs = at;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, moe_choose_kernel<T, R>, a);
 }
 template <typename T>
 cudaError_t choose_of(const MoeSortArgs &a, uint32_t smem, cudaStream_t s) {
@@ -351,13 +392,22 @@ cudaError_t combine_from(const MoeCombineArgs &a, int32_t o, int sms, cudaStream
 }  // namespace
 
 cudaError_t moe_sort_launch(const MoeSortArgs &a, int32_t type, cudaStream_t s) {
-    const uint32_t smem = sort_smem(a.n_expert, a.n_used), first = a.ctas == 1 ? smem : 2 * a.n_expert * 4;
+    const uint32_t smem = sort_smem(a.n_expert, a.n_used), first = a.stretches == 1 ? smem : 2 * a.n_expert * 4;
     cudaError_t e = type == SG_F32 ? choose_of<float>(a, first, s) : type == SG_F16 ? choose_of<__half>(a, first, s) : choose_of<__nv_bfloat16>(a, first, s);
-    if (e != cudaSuccess || a.ctas == 1) return e;
+    if (e != cudaSuccess || a.stretches == 1) return e;
     static bool ready[64];
     if ((e = big_smem(moe_place_kernel, smem, ready)) != cudaSuccess) return e;
-    moe_place_kernel<<<a.ctas, THREADS, smem, s>>>(a);
-    return cudaGetLastError();
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3((a.stretches + MOE_SORT_JOIN - 1) / MOE_SORT_JOIN);
+    c.blockDim = dim3(THREADS);
+    c.dynamicSmemBytes = smem;
+    c.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = at;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, moe_place_kernel, a);
 }
 
 cudaError_t moe_combine_launch(const MoeCombineArgs &a, int32_t type, int32_t out_type, int sms, cudaStream_t s) {

@@ -83,18 +83,22 @@ cudaError_t mx4_many_launch(const Mx4GemmArgs &a, uint64_t token_tiles, int sms,
 cudaError_t mx4_few_launch(const Mx4GemmArgs &a, uint32_t tile_shift, uint64_t token_tiles, int sms, cudaStream_t s);
 
 // The choice of experts and the sorting of its pairs.
-constexpr uint32_t MOE_SORT_MAX_EXPERTS = 1024, MOE_SORT_MAX_USED = 16, MOE_SORT_TOKENS = 64;
+constexpr uint32_t MOE_SORT_MAX_EXPERTS = 1024, MOE_SORT_MAX_USED = 16;
+constexpr uint32_t MOE_SORT_GROUP = 64;   // tokens whose pairs are ranked at a time
+constexpr uint32_t MOE_SORT_JOIN = 4;     // stretches that make a row of counts, and whose pairs a CTA places
 struct MoeSortArgs {
     const void *logits;            // null: ids are given
     uint64_t ld;
-    uint32_t n_tok, n_expert, n_used, ctas;
+    uint32_t n_tok, n_expert, n_used;
+    uint32_t stretch, stretches;   // tokens a CTA chooses for, and how many such
     int32_t norm;
     float prune;
     int32_t *ids;
     float *weights;
     int32_t *first, *order, *place;
     int32_t *tiles;                // [3][n_expert + 1]: the same for tiles of 32, 64 and 128 rows
-    int32_t *counts;               // [ctas][n_expert]
+    int32_t *counts;               // [a row for MOE_SORT_JOIN stretches][counts_ld]
+    uint32_t counts_ld;            // n_expert, up to the next multiple of four
 };
 cudaError_t moe_sort_launch(const MoeSortArgs &a, int32_t type, cudaStream_t s);
 
