@@ -2619,24 +2619,24 @@ uint32_t sort_stretch(uint64_t n_tok) {
 }
 uint32_t sort_stretches(uint64_t n_tok) { return (uint32_t)std::max<uint64_t>(1, (n_tok + sort_stretch(n_tok) - 1) / sort_stretch(n_tok)); }
 uint64_t counts_at(uint64_t n_expert) { return align_up(3 * (n_expert + 1), 4); }
-// plan->work: first tiles for tiles of 32, 64 and 128 rows, then the stretches' counts
-int32_t *plan_tiles(const sg_moe_plan *p, uint32_t shift) { return p->work + (shift - 5) * (p->n_expert + 1); }
+// plan->work: first tiles for tiles of 32, 128 and 192 rows, then the counts
+int32_t *plan_tiles(const sg_moe_plan *p, uint32_t rows) { return p->work + (rows == 32 ? 0 : rows == 128 ? 1 : 2) * (p->n_expert + 1); }
 
-// How a product of n_tok rows is run: rows of x a tile (1 << shift), tiles of x; tiles of tokens (of experts: at most that
-// many) and which kernel.
+// How a product of n_tok rows is run: rows of a tile of x, how many tiles (of experts: at most that many), which kernel.
 struct Mx4Plan {
-    uint32_t shift;
-    uint64_t x_tiles, token_tiles;
+    uint32_t x_rows;
+    uint64_t tiles;
     bool many;
 };
-Mx4Plan mx4_plan(const sg_mx4 *w, uint64_t n_tok, const sg_moe_plan *plan) {
+Mx4Plan mx4_plan(const sg_mx4 *w, bool up, uint64_t n_tok, const sg_moe_plan *plan) {
     const uint64_t pairs = plan ? plan->n_tok * plan->n_used : n_tok, groups = plan ? std::min(plan->n_expert, pairs) : 1;
-    if (!pairs) return {5, 0, 0, false};
-    const uint32_t shift = pairs / groups <= 32 ? 5 : 7;
-    const uint64_t rows = 1ull << shift, tiles = (pairs + groups * (rows - 1)) / rows;
-    return {shift, tiles, tiles, shift == 7 && tiles * (align_up(w->rows, MX4_ROWS) / MX4_ROWS) >= MX4_MANY_TILES};
+    if (!pairs) return {32, 0, false};
+    auto tiles = [&](uint64_t rows) { return (pairs + groups * (rows - 1)) / rows; };
+    if (pairs / groups <= 32) return {32, tiles(32), false};
+    if (tiles(128) * (align_up(w->rows, MX4_ROWS) / MX4_ROWS) < MX4_MANY_TILES) return {128, tiles(128), false};
+    return {up ? 128u : 192u, tiles(up ? 128 : 192), true};
 }
-uint64_t mx4_scratch(const sg_mx4 *w, const Mx4Plan &p) { return p.x_tiles * mx4_nk(w) * mx4_tile_bytes(1u << p.shift); }
+uint64_t mx4_scratch(const sg_mx4 *w, const Mx4Plan &p) { return p.tiles * mx4_nk(w) * mx4_tile_bytes(p.x_rows); }
 
 // What matmul and experts have in common: the quantized rows of x, then the products.
 sg_status mx4_product(const sg_mx4 *w, const sg_mx4 *up, const sg_moe_plan *plan, bool gather, int32_t type, const void *d_x, uint64_t ldx,
@@ -2648,16 +2648,16 @@ sg_status mx4_product(const sg_mx4 *w, const sg_mx4 *up, const sg_moe_plan *plan
     if (!pairs) return SG_OK;
     const uint64_t x_rows = plan ? (gather ? plan->n_tok : pairs) : n_tok;
     if (!d_x || !d_out || (x_rows > 1 && ldx < w->cols) || (pairs > 1 && ldo < w->rows)) return SG_ERR_INVALID;
-    const Mx4Plan mp = mx4_plan(w, n_tok, plan);
+    const Mx4Plan mp = mx4_plan(w, up, n_tok, plan);
     if (!d_scratch || scratch_bytes < mx4_scratch(w, mp)) return SG_ERR_INVALID;
     if (!aligned(d_x, es) || !aligned(d_out, eo) || !aligned(d_scratch, 128)) return SG_ERR_ALIGN;
     DevInfo *di;
     if (sg_status st = dev_info(&di)) return st;
     const uint32_t nk = mx4_nk(w), feat_tiles = (uint32_t)(align_up(w->rows, MX4_ROWS) / MX4_ROWS);
-    if (mp.token_tiles * feat_tiles >= 1ull << 27) return SG_ERR_SHAPE;  // (CTAs of a launch, eight a tile at most)
+    if (mp.tiles * feat_tiles >= 1ull << 27 || mp.tiles * mp.x_rows >= 1ull << 32) return SG_ERR_SHAPE;  // (CTAs of a launch, eight a tile at most)
     Mx4QuantArgs q = {};
     q.x = d_x, q.ld = ldx, q.out = (uint8_t *)d_scratch;
-    q.cols = (uint32_t)w->cols, q.nk = nk, q.tile_shift = mp.shift, q.n_rows = x_rows;
+    q.cols = (uint32_t)w->cols, q.nk = nk, q.x_rows = mp.x_rows, q.n_rows = x_rows;
     q.rows = (uint32_t)x_rows, q.tile_rows = (uint32_t)x_rows;
     q.vec = rows16(d_x, ldx, es), q.early = true;
     Mx4GemmArgs g = {};
@@ -2666,12 +2666,12 @@ sg_status mx4_product(const sg_mx4 *w, const sg_mx4 *up, const sg_moe_plan *plan
     g.feats = (uint32_t)w->rows, g.nk = nk, g.feat_tiles = feat_tiles, g.n_tok = n_tok;
     if (plan) {
         q.n_used = (uint32_t)plan->n_used, q.ids = plan->ids, q.place = plan->place, q.order = gather ? nullptr : plan->order;
-        q.first = g.first = plan->first, q.tiles = g.tiles = plan_tiles(plan, mp.shift);
+        q.first = g.first = plan->first, q.tiles = plan_tiles(plan, mp.x_rows);
         g.n_expert = (uint32_t)plan->n_expert;
     }
     CK(mx4_quantize_launch(q, type, di->sms, s));
     g.vec = rows16(d_out, ldo, eo);
-    CK(mp.many ? mx4_many_launch(g, mp.token_tiles, di->sms, s) : mx4_few_launch(g, mp.shift, mp.token_tiles, di->sms, s));
+    CK(mp.many ? mx4_many_launch(g, mp.tiles, di->sms, s) : mx4_few_launch(g, mp.x_rows, mp.tiles, di->sms, s));
     return SG_OK;
 }
 
@@ -2708,7 +2708,7 @@ sg_status sg_mx4_quantize(const sg_mx4 *m, int32_t type, const void *d_x, uint64
     if (sg_status st = dev_info(&di)) return st;
     Mx4QuantArgs q = {};
     q.x = d_x, q.ld = ld, q.ld_expert = ld_expert, q.out = m->data;
-    q.cols = (uint32_t)m->cols, q.nk = mx4_nk(m), q.tile_shift = 7;
+    q.cols = (uint32_t)m->cols, q.nk = mx4_nk(m), q.x_rows = MX4_ROWS;
     q.rows = (uint32_t)m->rows, q.tile_rows = (uint32_t)align_up(m->rows, MX4_ROWS);
     q.n_rows = m->experts * q.tile_rows;
     q.vec = rows16(d_x, m->rows > 1 ? ld : 0, es) && (m->experts == 1 || rows16(d_x, ld_expert, es));
@@ -2734,7 +2734,7 @@ sg_status sg_mx4_dequantize(const sg_mx4 *m, int32_t type, void *d_out, uint64_t
 uint64_t sg_mx4_scratch_bytes(const sg_mx4 *w, uint64_t n_tok, const sg_moe_plan *plan) {
     if (check_mx4(w, false) || n_tok >= 1ull << 31) return 0;
     if (plan && (!plan->n_used || !plan->n_expert || plan->n_tok >= 1ull << 31 || plan->n_used > MOE_SORT_MAX_USED)) return 0;
-    return mx4_scratch(w, mx4_plan(w, n_tok, plan));
+    return std::max(mx4_scratch(w, mx4_plan(w, false, n_tok, plan)), mx4_scratch(w, mx4_plan(w, true, n_tok, plan)));
 }
 
 sg_status sg_mx4_matmul(const sg_mx4 *w, const sg_mx4 *up, int32_t type, const void *d_x, uint64_t ldx, uint64_t n_tok, int32_t out_type,

@@ -152,10 +152,10 @@ __device__ __forceinline__ void place_pairs(const MoeSortArgs &a, const Tables &
         });
         if (lane == 0) *m.all = all;
         if (first && lane == 0) a.first[E] = (int32_t)all;
-    } else if (warp < 4 && first) {  // tiles of 32, 64 and 128 rows
-        const uint32_t shift = warp + 4, r = (1u << shift) - 1;
+    } else if (warp < 4 && first) {  // tiles of 32, 128 and 192 rows
+        const uint32_t rows = warp == 1 ? 32 : warp == 2 ? 128 : 192;
         int32_t *tiles = a.tiles + (uint64_t)(warp - 1) * (E + 1);
-        const uint32_t all = warp_sums(E, lane, [&](uint32_t e) { return (total[e] + r) >> shift; }, [&](uint32_t e, uint32_t v) { tiles[e] = (int32_t)v; });
+        const uint32_t all = warp_sums(E, lane, [&](uint32_t e) { return (total[e] + rows - 1) / rows; }, [&](uint32_t e, uint32_t v) { tiles[e] = (int32_t)v; });
         if (lane == 0) tiles[E] = (int32_t)all;
     }
     __syncthreads();

@@ -2,6 +2,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "mx4.cuh"
 #include "tiled_block.cuh"
 
@@ -10,10 +12,6 @@ using namespace tiled;
 
 namespace {
 
-template <typename T> __device__ __forceinline__ float widen(T v);
-template <> __device__ __forceinline__ float widen<float>(float v) { return v; }
-template <> __device__ __forceinline__ float widen<__half>(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float widen<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <typename T> __device__ __forceinline__ T narrow(float v);
 template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
@@ -51,40 +49,75 @@ __device__ __forceinline__ uint32_t codes8(const float (&y)[8]) {
     return w;
 }
 
+// The bits of the largest of eight magnitudes as f32 (an infinity or a NaN: at least 0x7F800000).  16-bit magnitudes are
+// compared as they are, two at a time.
+__device__ __forceinline__ uint32_t top8(const Raw<float> &r) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(r.w);
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) top = max(top, w[i] & 0x7FFFFFFFu);
+    return top;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t top8(const Raw<T> &r) {
+    const uint32_t m = 0x7FFF7FFFu, t = __vimax3_u16x2(__vimax3_u16x2(r.w[0].x & m, r.w[0].y & m, r.w[0].z & m), r.w[0].w & m, 0u);
+    const uint32_t most = max(t >> 16, t & 0xFFFFu);
+    return std::is_same<T, __nv_bfloat16>::value ? most << 16 : __float_as_uint(__half2float(__ushort_as_half((unsigned short)most)));
+}
+// The eight values times a power of two f.
+__device__ __forceinline__ void scaled8(const Raw<float> &r, float f, float (&y)[8]) {
+    const float *v = reinterpret_cast<const float *>(r.w);
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] = v[i] * f;
+}
+__device__ __forceinline__ void scaled8(const Raw<__half> &r, float f, float (&y)[8]) {
+    const __half2 *v = reinterpret_cast<const __half2 *>(r.w);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 t = __half22float2(v[i]);
+        y[2 * i] = t.x * f, y[2 * i + 1] = t.y * f;
+    }
+}
+__device__ __forceinline__ void scaled8(const Raw<__nv_bfloat16> &r, float f, float (&y)[8]) {
+    const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) y[2 * i] = __uint_as_float(w[i] << 16) * f, y[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u) * f;
+}
+
 // Four lanes have the 32 values of a block: each gets its eight codes, all its scale byte.
 template <typename T>
 __device__ __forceinline__ uint32_t quantize8(const Raw<T> &raw, uint32_t &scale) {
-    const T *t = reinterpret_cast<const T *>(raw.w);
-    float v[8];
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        v[i] = widen(t[i]);
-        top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);  // an infinity or a NaN: the largest
-    }
+    uint32_t top = top8(raw);
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     // the exponent of the largest, one more from 1.75 times a power of two on, less 2
     const int e = max((int)((top + 0x200000u) >> 23) - 2, 0);
     scale = top >= 0x7F800000u ? 255u : (uint32_t)e;              // (all 32 are NaN then, whatever their codes)
-    const float f = __uint_as_float((uint32_t)(254 - e) << 23);  // 2^(127 - e), e at most 254
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] *= f;
-    return codes8(v);
+    float y[8];
+    scaled8(raw, __uint_as_float((uint32_t)(254 - e) << 23), y);  // times 2^(127 - e), e at most 254
+    return codes8(y);
 }
 
 // A warp takes 1024 columns of a row: its lanes eight values of each of four tiles, all loads at once, four lanes a block of
-// 32.  What bounds it: instructions (about 90 for a lane's eight values) next to reading x; a token that goes to several
-// experts is read and quantized once.
+// 32.  A token that goes to several experts is read and quantized once.  What bounds it: instructions (about 50 for a lane's
+// eight values) next to reading x.
 constexpr uint32_t QUANT_TILES = 4;
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(MX4_QUANT_THREADS) mx4_quantize_kernel(const __grid_constant__ Mx4QuantArgs a) {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, chunk = lane >> 2;
-    const uint32_t tile_bytes = mx4_tile_bytes(1u << a.tile_shift), mask = (1u << a.tile_shift) - 1, rows_at_once = gridDim.x * (MX4_QUANT_THREADS / 32);
+    const uint32_t tile_bytes = mx4_tile_bytes(a.x_rows), half = mx4_scale_bytes(a.x_rows) / 2, rows_at_once = gridDim.x * (MX4_QUANT_THREADS / 32);
     if (a.early) grid_launch_dependents();
-    for (uint32_t kt0 = blockIdx.y * QUANT_TILES; kt0 < a.nk; kt0 += gridDim.y * QUANT_TILES)
-        for (uint64_t i = blockIdx.x * (MX4_QUANT_THREADS / 32) + warp; i < a.n_rows; i += rows_at_once) {
+    // a row's place among the tiles, from its place among the sorted ones
+    auto row_of = [&](int32_t pair, uint32_t place) {
+        const int32_t e = __ldg(a.ids + pair);
+        return (int64_t)__ldg(a.tiles + e) * a.x_rows + (place - (uint32_t)__ldg(a.first + e));
+    };
+    for (uint32_t kt0 = blockIdx.y * QUANT_TILES; kt0 < a.nk; kt0 += gridDim.y * QUANT_TILES) {
+        const uint32_t tiles = min(QUANT_TILES, a.nk - kt0);
+        uint32_t turn = 0;
+        int64_t ahead = -1;
+        for (uint64_t i = blockIdx.x * (MX4_QUANT_THREADS / 32) + warp; i < a.n_rows; i += rows_at_once, turn = (turn + 1) & 31) {
             const T *src = static_cast<const T *>(a.x);
             bool row_there = true;
             if (a.n_used) src += i * a.ld;
@@ -99,51 +132,48 @@ __global__ void __launch_bounds__(MX4_QUANT_THREADS) mx4_quantize_kernel(const _
                 const uint32_t col = (kt0 + u) * MX4_COLS + lane * 8;
                 load8<T, VEC>(src + col, row_there && col < a.cols, raw[u]);
             }
-            uint32_t w[QUANT_TILES], s4[QUANT_TILES];
-#pragma unroll
-            for (uint32_t u = 0; u < QUANT_TILES; u++) {
-                uint32_t scale;
-                w[u] = quantize8(raw[u], scale);
-                // the scale bytes of four blocks make a word
-                const bool there = row_there && (kt0 + u) * MX4_COLS + lane * 8 < a.cols;
-                s4[u] = (there ? scale : 0u) << (8 * (chunk & 3));
-                s4[u] |= __shfl_xor_sync(0xffffffffu, s4[u], 4);
-                s4[u] |= __shfl_xor_sync(0xffffffffu, s4[u], 8);
-            }
-            auto put = [&](uint64_t row) {
-                uint8_t *t = a.out + ((row >> a.tile_shift) * a.nk + kt0) * tile_bytes;
-                const uint32_t r = (uint32_t)row & mask, code_at = mx4_code_at(r, chunk) + 4 * (lane & 3);
-                const uint32_t scale_at = (mask + 1) * 128 + mx4_scale_at(r, chunk);
-#pragma unroll
-                for (uint32_t u = 0; u < QUANT_TILES; u++) {
-                    if (kt0 + u >= a.nk) break;
-                    *reinterpret_cast<uint32_t *>(t + u * tile_bytes + code_at) = w[u];
-                    if ((lane & 15) == 0) *reinterpret_cast<uint32_t *>(t + u * tile_bytes + scale_at) = s4[u];
+            // where it goes: of sorted rows the lanes look up the places of this one and the warp's next 31, of a token's
+            // those of its pairs
+            if (a.order) {
+                if (turn == 0) {
+                    const uint64_t j = i + (uint64_t)lane * rows_at_once;
+                    const int32_t pair = j < a.n_rows ? __ldg(a.order + j) : -1;
+                    ahead = pair < 0 ? -1 : row_of(pair, (uint32_t)j);
                 }
+            } else if (a.n_used) {
+                const int32_t p = lane < a.n_used ? __ldg(a.place + i * a.n_used + lane) : -1;
+                ahead = p < 0 ? -1 : row_of((int32_t)(i * a.n_used + lane), (uint32_t)p);
+            }
+            uint32_t w[QUANT_TILES], scale[QUANT_TILES];
+#pragma unroll
+            for (uint32_t u = 0; u < QUANT_TILES; u++)
+                if (u < tiles) {
+                    w[u] = quantize8(raw[u], scale[u]);
+                    if (!row_there || (kt0 + u) * MX4_COLS + lane * 8 >= a.cols) scale[u] = 0;
+                }
+            auto put = [&](uint64_t row) {
+                const uint32_t tile = (uint32_t)row / a.x_rows, r = (uint32_t)row - tile * a.x_rows;  // (rows are below 2^32)
+                uint8_t *t = a.out + ((uint64_t)tile * a.nk + kt0) * tile_bytes;
+                const uint32_t code_at = mx4_code_at(r, chunk) + 4 * (lane & 3);
+                const uint32_t scale_at = a.x_rows * 128 + mx4_scale_at(r, chunk, half);
+#pragma unroll
+                for (uint32_t u = 0; u < QUANT_TILES; u++)
+                    if (u < tiles) {
+                        *reinterpret_cast<uint32_t *>(t + u * tile_bytes + code_at) = w[u];
+                        if ((lane & 3) == 0) t[u * tile_bytes + scale_at] = (uint8_t)scale[u];
+                    }
             };
             if (!a.n_used) put(i);
             else if (a.order) {
-                const int32_t pair = __ldg(a.order + i);
-                if (pair >= 0) {
-                    const int32_t e = __ldg(a.ids + pair);
-                    put(((uint64_t)__ldg(a.tiles + e) << a.tile_shift) + (i - __ldg(a.first + e)));
-                }
-            } else {
-                // (lane j looks the j-th place up)
-                int64_t row = -1;
-                if (lane < a.n_used) {
-                    const int32_t p = __ldg(a.place + i * a.n_used + lane);
-                    if (p >= 0) {
-                        const int32_t e = __ldg(a.ids + i * a.n_used + lane);
-                        row = ((int64_t)__ldg(a.tiles + e) << a.tile_shift) + (p - __ldg(a.first + e));
-                    }
-                }
+                const int64_t to = __shfl_sync(0xffffffffu, ahead, turn);
+                if (to >= 0) put(to);
+            } else
                 for (uint32_t j = 0; j < a.n_used; j++) {
-                    const int64_t to = __shfl_sync(0xffffffffu, row, j);
+                    const int64_t to = __shfl_sync(0xffffffffu, ahead, j);
                     if (to >= 0) put(to);
                 }
-            }
         }
+    }
 }
 
 // The values of two codes.

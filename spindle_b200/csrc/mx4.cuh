@@ -12,8 +12,9 @@
 //           tcgen05.cp spreads over TMEM as the tensor cores take scales.
 // So one bulk copy of 17408 contiguous bytes brings a stage of an operand, without a
 // tensor map.  Rows past the last are zeros in a matrix; columns past the last are too
-// (codes 0, scale byte 0).  Quantized activations have the same form with 32, 64 or 128
-// rows a tile (codes of that many rows, then the same 1024 bytes of scales).
+// (codes 0, scale byte 0).  Quantized activations have the same form with 32, 128 or 192
+// rows a tile (codes of that many rows, then the scales; of 192 rows a half's are two such
+// blocks, the second of rows 128 on).
 #pragma once
 
 #include "common.cuh"
@@ -21,14 +22,16 @@
 namespace sg {
 
 constexpr uint32_t MX4_ROWS = 128, MX4_COLS = 256;             // of a tile
-constexpr uint32_t MX4_SCALES = 1024;                          // bytes of a tile's scales
-__host__ __device__ constexpr uint32_t mx4_tile_bytes(uint32_t rows) { return rows * 128 + MX4_SCALES; }
+constexpr uint32_t MX4_SCALES = 1024;                          // bytes of a tile's scales, of up to 128 rows
+__host__ __device__ constexpr uint32_t mx4_scale_bytes(uint32_t rows) { return rows > 128 ? 2 * MX4_SCALES : MX4_SCALES; }
+__host__ __device__ constexpr uint32_t mx4_tile_bytes(uint32_t rows) { return rows * 128 + mx4_scale_bytes(rows); }
 constexpr uint32_t MX4_TILE = mx4_tile_bytes(MX4_ROWS);
 
 // In a tile: the byte of a row's chunk of 32 codes, and of its scale (after the codes).
 __host__ __device__ __forceinline__ uint32_t mx4_code_at(uint32_t row, uint32_t chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
-__host__ __device__ __forceinline__ uint32_t mx4_scale_at(uint32_t row, uint32_t chunk) {
-    return (chunk >> 2) * 512 + (row & 31) * 16 + ((row >> 5) << 2) + (chunk & 3);
+// (half: bytes of a half of the columns, 512 for up to 128 rows)
+__host__ __device__ __forceinline__ uint32_t mx4_scale_at(uint32_t row, uint32_t chunk, uint32_t half = 512) {
+    return (chunk >> 2) * half + (row >> 7) * 512 + (row & 31) * 16 + ((row >> 5 & 3) << 2) + (chunk & 3);
 }
 
 // 2^(s - 127) of a scale byte; 255 is NaN.
@@ -42,7 +45,7 @@ struct Mx4QuantArgs {
     uint64_t ld, ld_expert;        // in elements
     uint8_t *out;
     uint32_t cols, nk;             // nk: tiles along the columns
-    uint32_t tile_shift;           // rows a tile: 1 << tile_shift
+    uint32_t x_rows;               // rows of a tile
     uint64_t n_rows;               // rows that are read; of a matrix: all rows of its tiles
     // a matrix of several experts (n_used 0): rows each, and rows of its tiles each
     uint32_t rows, tile_rows;
@@ -75,12 +78,12 @@ struct Mx4GemmArgs {
     uint32_t feats, nk;            // rows of w, tiles along its columns
     uint32_t feat_tiles;
     uint64_t n_tok;                // rows of x, where they are one matrix
-    const int32_t *first, *tiles;  // experts: the first sorted place of each, its first tile of x (n_expert + 1 each)
+    const int32_t *first;          // experts: the first sorted place of each (n_expert + 1)
     uint32_t n_expert;
     bool vec;                      // out allows 16-byte stores of eight features
 };
 cudaError_t mx4_many_launch(const Mx4GemmArgs &a, uint64_t token_tiles, int sms, cudaStream_t s);
-cudaError_t mx4_few_launch(const Mx4GemmArgs &a, uint32_t tile_shift, uint64_t token_tiles, int sms, cudaStream_t s);
+cudaError_t mx4_few_launch(const Mx4GemmArgs &a, uint32_t x_rows, uint64_t token_tiles, int sms, cudaStream_t s);
 
 // The choice of experts and the sorting of its pairs.
 constexpr uint32_t MOE_SORT_MAX_EXPERTS = 1024, MOE_SORT_MAX_USED = 16;
@@ -96,7 +99,7 @@ struct MoeSortArgs {
     int32_t *ids;
     float *weights;
     int32_t *first, *order, *place;
-    int32_t *tiles;                // [3][n_expert + 1]: the same for tiles of 32, 64 and 128 rows
+    int32_t *tiles;                // [3][n_expert + 1]: the same for tiles of 32, 128 and 192 rows
     int32_t *counts;               // [a row for MOE_SORT_JOIN stretches][counts_ld]
     uint32_t counts_ld;            // n_expert, up to the next multiple of four
 };

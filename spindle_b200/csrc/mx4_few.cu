@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_few_kernel(const __grid_consta
     // (a part of a cluster has its one tile: the launch makes no more)
     const uint32_t tiles = (a.first ? ex.upto[a.n_expert - 1] : (uint32_t)((a.n_tok + NT - 1) / NT)) * a.feat_tiles, me = blockIdx.x / parts;
     const uint32_t k0 = a.nk * part / parts, k1 = a.nk * (part + 1) / parts;
-    auto tile_at = [&](uint32_t i) { return tile_of<NT, NT>(a, ex, i / a.feat_tiles); };
+    auto tile_at = [&](uint32_t i) { return tile_of<NT>(a, ex, i / a.feat_tiles); };
 
     bool ok = true;
     if (warp < 2) {
@@ -285,13 +285,13 @@ cudaError_t launch_as(const Mx4GemmArgs &a, uint32_t grid, uint32_t parts, cudaS
 
 }  // namespace
 
-cudaError_t mx4_few_launch(const Mx4GemmArgs &a, uint32_t tile_shift, uint64_t token_tiles, int sms, cudaStream_t s) {
+cudaError_t mx4_few_launch(const Mx4GemmArgs &a, uint32_t x_rows, uint64_t token_tiles, int sms, cudaStream_t s) {
     const uint64_t tiles = token_tiles * a.feat_tiles;
     // few tiles: their columns in 2, 4 or 8 parts, while a part has four stages or more
     uint32_t parts = 1;
     while (parts < 8 && tiles * parts * 2 <= (uint64_t)sms && a.nk >= parts * 8) parts *= 2;
     const uint32_t grid = parts > 1 ? (uint32_t)tiles * parts : (uint32_t)(tiles < (uint64_t)sms ? tiles : sms);
-    if (tile_shift == 5) return a.up ? launch_as<32, true>(a, grid, parts, s) : launch_as<32, false>(a, grid, parts, s);
+    if (x_rows == 32) return a.up ? launch_as<32, true>(a, grid, parts, s) : launch_as<32, false>(a, grid, parts, s);
     return a.up ? launch_as<128, true>(a, grid, parts, s) : launch_as<128, false>(a, grid, parts, s);
 }
 

@@ -33,8 +33,8 @@ struct Cfg {
     // Two buffers of sums where TMEM has room for them beside the scales: the products of a tile run while the results of the
     // one before are taken (32760 places, 768 columns to 2048: 60 us; with tiles of 256 tokens and one buffer 63).  Gate and up of 96 tokens
     // would fit twice too, but then each brings its weights for fewer tokens.
-    static constexpr uint32_t NT = DUAL ? 128 : 192, XT = DUAL ? 1 : 2, BUFS = DUAL ? 1 : 2;
-    static constexpr uint32_t W_BYTES = MX4_TILE * (DUAL ? 2 : 1), X_BYTES = NT / 2 * 128, XS_BYTES = XT * MX4_SCALES;
+    static constexpr uint32_t NT = DUAL ? 128 : 192, XT = DUAL ? 1 : 2, BUFS = DUAL ? 1 : 2, X_TILE = mx4_tile_bytes(NT);
+    static constexpr uint32_t W_BYTES = MX4_TILE * (DUAL ? 2 : 1), X_BYTES = NT / 2 * 128, XS_BYTES = mx4_scale_bytes(NT);
     static constexpr uint32_t STAGE = W_BYTES + X_BYTES + XS_BYTES;
     static constexpr uint32_t STAGES = DUAL ? 4 : 5;
     static constexpr uint32_t PIECES = NT / 16 / GROUPS;
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
     const uint32_t tiles = token_tiles * fps;
 
     // (the feature pairs of a token tile follow each other: an expert's weights are read once, by neighbours)
-    auto tile_at = [&](uint32_t i) { return tile_of<C::NT, 128>(a, ex, i / fps); };
+    auto tile_at = [&](uint32_t i) { return tile_of<C::NT>(a, ex, i / fps); };
     auto pair_of = [&](uint32_t i) { return i % fps; };
 
     bool ok = true;
@@ -99,14 +99,11 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
         if (warp) grid_dependency_wait();  // x comes from the launch before
         for (uint32_t i = me; i < tiles && ok; i += pairs) {
             const Tile t = tile_at(i);
-            const uint32_t n = (t.rows + 31) & ~31u, half = n / 2, r0 = t.in + rank * half;  // this CTA's tokens: r0 .. r0 + half
+            const uint32_t half = ((t.rows + 31) & ~31u) / 2;  // this CTA's tokens: from rank * half on
             const uint32_t ft = min(2 * pair_of(i) + rank, a.feat_tiles - 1);
-            const uint64_t w_at = (uint64_t)t.e * a.expert_bytes + (uint64_t)ft * a.nk * MX4_TILE, next = (uint64_t)a.nk * MX4_TILE;
-            const uint8_t *w = a.w + w_at, *up = DUAL ? a.up + w_at : nullptr, *x = a.x + (uint64_t)t.x_tile * next;
-            // rows from the first of them on in its tile of 128, and what is left of it
-            const uint32_t in = r0 & 127u, part = min(half, 128 - in), xts = C::XT == 2 && t.in + n > 128 ? 2 : 1;
-            const uint8_t *xr = x + (r0 >> 7) * next + in * 128, *xr2 = x + next;
-            if (warp == 2) x += MX4_ROWS * 128;
+            const uint64_t w_at = (uint64_t)t.e * a.expert_bytes + (uint64_t)ft * a.nk * MX4_TILE;
+            const uint8_t *w = a.w + w_at, *up = DUAL ? a.up + w_at : nullptr, *x = a.x + (uint64_t)t.x_tile * a.nk * C::X_TILE;
+            x += warp == 1 ? rank * half * 128 : C::NT * 128;
             for (uint32_t k = 0; k < a.nk; k++) {
                 if (turn) ok = wait(&sh.empty[s], (turn - 1) & 1);
                 if (!ok) break;
@@ -119,20 +116,13 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
                         if (DUAL) bulk_g2s(st + MX4_TILE, up, MX4_TILE, full);
                     }
                     w += MX4_TILE, up += MX4_TILE;
-                } else if (warp == 1) {
-                    if (elect_one()) {
-                        mbar_arrive_expect_tx(full, half * 128);
-                        bulk_g2s(st + C::W_BYTES, xr, part * 128, full);
-                        if (part < half) bulk_g2s(st + C::W_BYTES + part * 128, xr2, (half - part) * 128, full);
-                    }
-                    xr += MX4_TILE, xr2 += MX4_TILE;
                 } else {
                     if (elect_one()) {
-                        mbar_arrive_expect_tx(full, xts * MX4_SCALES);
-                        bulk_g2s(st + C::W_BYTES + C::X_BYTES, x, MX4_SCALES, full);
-                        if (xts == 2) bulk_g2s(st + C::W_BYTES + C::X_BYTES + MX4_SCALES, x + next, MX4_SCALES, full);
+                        const uint32_t bytes = warp == 1 ? half * 128 : C::XS_BYTES;
+                        mbar_arrive_expect_tx(full, bytes);
+                        bulk_g2s(st + C::W_BYTES + (warp == 1 ? 0 : C::X_BYTES), x, bytes, full);
                     }
-                    x += MX4_TILE;
+                    x += C::X_TILE;
                 }
                 __syncwarp();
                 issued = min(issued + 1, C::STAGES);
@@ -179,13 +169,13 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
                             copy_scales<2>(sc + 4 * h, ws_desc + at + 32 * h);
                             if (DUAL) copy_scales<2>(sc + 8 + 4 * h, ws_desc + at + (MX4_TILE >> 4) + 32 * h);
 #pragma unroll
-                            for (uint32_t j = 0; j < C::XT; j++) copy_scales<2>(sx + 4 * C::XT * h + 4 * j, xs_desc + at + j * (MX4_SCALES >> 4) + 32 * h);
+                            for (uint32_t j = 0; j < C::XT; j++) copy_scales<2>(sx + 4 * C::XT * h + 4 * j, xs_desc + at + 32 * (C::XT * h + j));
                         }
                         // a product has 64 columns: 32 bytes of a row, half of a word of four scales
 #pragma unroll
                         for (uint32_t q = 0; q < 4; q++) {
                             const uint32_t h = q >> 1, iq = id | (q & 1 ? idesc(0, 0, 1) ^ idesc(0, 0, 0) : 0u), add = k > 0 || q > 0;
-                            mma<2>(sums, w_desc + at + 2 * q, x_desc + at + 2 * q, iq, sc + 4 * h, sx + 4 * C::XT * h + t.in / 32, add);
+                            mma<2>(sums, w_desc + at + 2 * q, x_desc + at + 2 * q, iq, sc + 4 * h, sx + 4 * C::XT * h, add);
                             if (DUAL)
                                 mma<2>(sums + C::NT, w_desc + at + (MX4_TILE >> 4) + 2 * q, x_desc + at + 2 * q, iq, sc + 8 + 4 * h, sx + 4 * h, add);
                         }

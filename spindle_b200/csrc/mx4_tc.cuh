@@ -154,20 +154,20 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity) {
         if (globaltimer_ns() - t0 > WAIT_LIMIT_NS) return false;
     }
 }
-// Of each expert: how many tiles end with it, its first sorted place, its first tile of x (a lookup from global memory took
+// Of each expert: how many tiles end with it and its first sorted place (a lookup from global memory took
 // every role 0.7 us a tile).
 struct Experts {
-    uint32_t upto[MAX_E], first[MAX_E], x_tile[MAX_E], n_rows;
+    uint32_t upto[MAX_E], first[MAX_E], n_rows;
 };
-constexpr uint32_t EXPERTS_BYTES = 3 * 4 * MAX_E + 1024;
+constexpr uint32_t EXPERTS_BYTES = 2 * 4 * MAX_E + 1024;
 
-// A tile: up to NT rows of x (from row `in` of its tile x_tile on), those of one expert, to rows of the output from row0 on.
+// A tile: up to NT rows of x, a tile of it, those of one expert, to rows of the output from row0 on.
 struct Tile {
-    uint32_t e, x_tile, in, rows;
+    uint32_t e, x_tile, rows;
     uint64_t row0;
 };
 
-// The experts' lookups for tiles of NT tokens, by one warp; the number of tiles of all.  rows: of x a tile of it has.
+// The experts' lookups for tiles of nt tokens, by one warp.
 __device__ __forceinline__ void find_experts(const Mx4GemmArgs &a, Experts &ex, uint32_t nt, uint32_t lane) {
     uint32_t before = 0;
     for (uint32_t base = 0; base < a.n_expert; base += 32) {
@@ -182,15 +182,14 @@ __device__ __forceinline__ void find_experts(const Mx4GemmArgs &a, Experts &ex, 
         if (i < a.n_expert) {
             ex.upto[i] = before + n;
             ex.first[i] = f0;
-            ex.x_tile[i] = (uint32_t)__ldg(a.tiles + i);
             if (i + 1 == a.n_expert) ex.n_rows = f1;
         }
         before += __shfl_sync(0xffffffffu, n, 31);
     }
 }
 
-// The tt-th tile of NT tokens, x in tiles of XROWS rows.
-template <uint32_t NT, uint32_t XROWS>
+// The tt-th tile of NT tokens, as x lies in memory.
+template <uint32_t NT>
 __device__ __forceinline__ Tile tile_of(const Mx4GemmArgs &a, const Experts &ex, uint32_t tt) {
     Tile t;
     if (a.first) {
@@ -202,15 +201,13 @@ __device__ __forceinline__ Tile tile_of(const Mx4GemmArgs &a, const Experts &ex,
         }
         const uint32_t r = (tt - (lo ? ex.upto[lo - 1] : 0)) * NT, f0 = ex.first[lo], n = (lo + 1 < a.n_expert ? ex.first[lo + 1] : ex.n_rows) - f0;
         t.e = lo;
-        t.x_tile = ex.x_tile[lo] + r / XROWS;
-        t.in = r % XROWS;
+        t.x_tile = tt;
         t.rows = min(n - r, NT);
         t.row0 = f0 + r;
     } else {
         t.e = 0;
         t.row0 = (uint64_t)tt * NT;
-        t.x_tile = (uint32_t)(t.row0 / XROWS);
-        t.in = (uint32_t)(t.row0 % XROWS);
+        t.x_tile = tt;
         t.rows = (uint32_t)(a.n_tok - t.row0 < NT ? a.n_tok - t.row0 : NT);
     }
     return t;
