@@ -2598,8 +2598,6 @@ sg_status check_mx4(const sg_mx4 *m, bool data) {
     return aligned(m->data, 16) ? SG_OK : SG_ERR_ALIGN;
 }
 
-// Tiles of 128 features and 128 tokens from which on the kernel for many tokens is taken: @@
-constexpr uint64_t MX4_MANY_TILES = 120;
 uint32_t mx4_nk(const sg_mx4 *m) { return (uint32_t)((m->cols + MX4_COLS - 1) / MX4_COLS); }
 uint64_t mx4_expert_bytes(const sg_mx4 *m) { return align_up(m->rows, MX4_ROWS) / MX4_ROWS * mx4_nk(m) * MX4_TILE; }
 // rows of cols elements ld apart: whether every eight of them are 16-byte aligned
@@ -2618,9 +2616,9 @@ uint32_t sort_stretch(uint64_t n_tok) {
     return (uint32_t)std::max<uint64_t>(16, align_up((n_tok + 511) / 512, 16));
 }
 uint32_t sort_stretches(uint64_t n_tok) { return (uint32_t)std::max<uint64_t>(1, (n_tok + sort_stretch(n_tok) - 1) / sort_stretch(n_tok)); }
-uint64_t counts_at(uint64_t n_expert) { return align_up(3 * (n_expert + 1), 4); }
-// plan->work: first tiles for tiles of 32, 128 and 192 rows, then the counts
-int32_t *plan_tiles(const sg_moe_plan *p, uint32_t rows) { return p->work + (rows == 32 ? 0 : rows == 128 ? 1 : 2) * (p->n_expert + 1); }
+uint64_t counts_at(uint64_t n_expert) { return align_up(4 * (n_expert + 1), 4); }
+// plan->work: first tiles for tiles of 32, 128, 192 and 256 rows, then the counts
+int32_t *plan_tiles(const sg_moe_plan *p, uint32_t rows) { return p->work + (rows == 32 ? 0 : rows / 64 - 1) * (p->n_expert + 1); }
 
 // How a product of n_tok rows is run: rows of a tile of x, how many tiles (of experts: at most that many), which kernel.
 struct Mx4Plan {
@@ -2628,15 +2626,35 @@ struct Mx4Plan {
     uint64_t tiles;
     bool many;
 };
-Mx4Plan mx4_plan(const sg_mx4 *w, bool up, uint64_t n_tok, const sg_moe_plan *plan) {
+Mx4Plan mx4_plan(const sg_mx4 *w, bool up, uint64_t n_tok, const sg_moe_plan *plan, int sms) {
     const uint64_t pairs = plan ? plan->n_tok * plan->n_used : n_tok, groups = plan ? std::min(plan->n_expert, pairs) : 1;
     if (!pairs) return {32, 0, false};
+    const uint64_t feat_tiles = align_up(w->rows, MX4_ROWS) / MX4_ROWS, nk = mx4_nk(w);
     auto tiles = [&](uint64_t rows) { return (pairs + groups * (rows - 1)) / rows; };
     if (pairs / groups <= 32) return {32, tiles(32), false};
-    if (tiles(128) * (align_up(w->rows, MX4_ROWS) / MX4_ROWS) < MX4_MANY_TILES) return {128, tiles(128), false};
-    return {up ? 128u : 192u, tiles(up ? 128 : 192), true};
+    // As long as each tile of 128 features and tokens has an SM of its own, the kernel for few tokens (33 rows of 14336 to
+    // 4096: 12.5 us against 18.8 in the other; 128 rows of 14336 to 14336: 26.9 against 28.9; 192 rows: 38.7 against 31.0).
+    if (tiles(128) * feat_tiles <= (uint64_t)sms) return {128, tiles(128), false};
+    if (up) return {128, tiles(128), true};
+    // Tiles of 256 tokens bring fewer bytes for their products, those of 192 have their results taken behind them, and fill
+    // the last round of pairs of SMs better or worse: a stage and what a tile has on top, 400 and 600 ns against 335 and 100
+    // (4096 x 4096 x 14336: 104 us against 105; 2048 x 14336 x 4096: 62 against 68; 1000 x 4096 x 14336: 35 against 33;
+    // 4096 x 768 x 4096: 19.3 against 18.9).  Of experts, whose tiles are part empty, 256 from 2048 columns on (32768 places,
+    // 128 experts, 2048 to 768: 58 against 60; 768 to 2048: 68 against 66; 64 experts, 1024 to 1024: 41 against 39).
+    auto rounds = [&](uint64_t rows) { return (tiles(rows) * ((feat_tiles + 1) / 2) + sms / 2 - 1) / (sms / 2); };
+    const uint64_t wide = plan ? (nk >= 8 ? 256 : 192) : rounds(256) * (40 * nk + 60) < rounds(192) * (33 * nk + 10) ? 256 : 192;
+    return {(uint32_t)wide, tiles(wide), true};
 }
 uint64_t mx4_scratch(const sg_mx4 *w, const Mx4Plan &p) { return p.tiles * mx4_nk(w) * mx4_tile_bytes(p.x_rows); }
+// Whatever of the plans it will be.
+uint64_t mx4_scratch_most(const sg_mx4 *w, uint64_t n_tok, const sg_moe_plan *plan) {
+    const uint64_t pairs = plan ? plan->n_tok * plan->n_used : n_tok, groups = plan ? std::min(plan->n_expert, pairs) : 1;
+    if (!pairs) return 0;
+    uint64_t most = 0;
+    for (uint32_t rows : {32u, 128u, 192u, 256u})
+        if ((rows == 32) == (pairs / groups <= 32)) most = std::max(most, mx4_scratch(w, {rows, (pairs + groups * (rows - 1)) / rows, false}));
+    return most;
+}
 
 // What matmul and experts have in common: the quantized rows of x, then the products.
 sg_status mx4_product(const sg_mx4 *w, const sg_mx4 *up, const sg_moe_plan *plan, bool gather, int32_t type, const void *d_x, uint64_t ldx,
@@ -2648,12 +2666,12 @@ sg_status mx4_product(const sg_mx4 *w, const sg_mx4 *up, const sg_moe_plan *plan
     if (!pairs) return SG_OK;
     const uint64_t x_rows = plan ? (gather ? plan->n_tok : pairs) : n_tok;
     if (!d_x || !d_out || (x_rows > 1 && ldx < w->cols) || (pairs > 1 && ldo < w->rows)) return SG_ERR_INVALID;
-    const Mx4Plan mp = mx4_plan(w, up, n_tok, plan);
-    if (!d_scratch || scratch_bytes < mx4_scratch(w, mp)) return SG_ERR_INVALID;
+    if (!d_scratch || scratch_bytes < mx4_scratch_most(w, n_tok, plan)) return SG_ERR_INVALID;
     if (!aligned(d_x, es) || !aligned(d_out, eo) || !aligned(d_scratch, 128)) return SG_ERR_ALIGN;
     DevInfo *di;
     if (sg_status st = dev_info(&di)) return st;
     const uint32_t nk = mx4_nk(w), feat_tiles = (uint32_t)(align_up(w->rows, MX4_ROWS) / MX4_ROWS);
+    const Mx4Plan mp = mx4_plan(w, up, n_tok, plan, di->sms);
     if (mp.tiles * feat_tiles >= 1ull << 27 || mp.tiles * mp.x_rows >= 1ull << 32) return SG_ERR_SHAPE;  // (CTAs of a launch, eight a tile at most)
     Mx4QuantArgs q = {};
     q.x = d_x, q.ld = ldx, q.out = (uint8_t *)d_scratch;
@@ -2671,7 +2689,7 @@ sg_status mx4_product(const sg_mx4 *w, const sg_mx4 *up, const sg_moe_plan *plan
     }
     CK(mx4_quantize_launch(q, type, di->sms, s));
     g.vec = rows16(d_out, ldo, eo);
-    CK(mp.many ? mx4_many_launch(g, mp.tiles, di->sms, s) : mx4_few_launch(g, mp.x_rows, mp.tiles, di->sms, s));
+    CK(mp.many ? mx4_many_launch(g, mp.x_rows, mp.tiles, di->sms, s) : mx4_few_launch(g, mp.x_rows, mp.tiles, di->sms, s));
     return SG_OK;
 }
 
@@ -2734,7 +2752,7 @@ sg_status sg_mx4_dequantize(const sg_mx4 *m, int32_t type, void *d_out, uint64_t
 uint64_t sg_mx4_scratch_bytes(const sg_mx4 *w, uint64_t n_tok, const sg_moe_plan *plan) {
     if (check_mx4(w, false) || n_tok >= 1ull << 31) return 0;
     if (plan && (!plan->n_used || !plan->n_expert || plan->n_tok >= 1ull << 31 || plan->n_used > MOE_SORT_MAX_USED)) return 0;
-    return std::max(mx4_scratch(w, mx4_plan(w, false, n_tok, plan)), mx4_scratch(w, mx4_plan(w, true, n_tok, plan)));
+    return mx4_scratch_most(w, n_tok, plan);
 }
 
 sg_status sg_mx4_matmul(const sg_mx4 *w, const sg_mx4 *up, int32_t type, const void *d_x, uint64_t ldx, uint64_t n_tok, int32_t out_type,
@@ -2745,7 +2763,7 @@ sg_status sg_mx4_matmul(const sg_mx4 *w, const sg_mx4 *up, int32_t type, const v
 
 uint64_t sg_moe_plan_work_bytes(uint64_t n_tok, uint64_t n_expert) {
     if (!n_expert || n_expert > MOE_SORT_MAX_EXPERTS || n_tok >= 1ull << 31) return 0;
-    if (n_tok <= MOE_SORT_GROUP) return 4 * 3 * (n_expert + 1);
+    if (n_tok <= MOE_SORT_GROUP) return 4 * 4 * (n_expert + 1);
     // (up to 512 stretches, of fewer tokens than n_tok as well)
     return 4 * (counts_at(n_expert) + std::min<uint64_t>(512 / MOE_SORT_JOIN, (n_tok + 16 * MOE_SORT_JOIN - 1) / (16 * MOE_SORT_JOIN)) * align_up(n_expert, 4));
 }

@@ -152,8 +152,8 @@ __device__ __forceinline__ void place_pairs(const MoeSortArgs &a, const Tables &
         });
         if (lane == 0) *m.all = all;
         if (first && lane == 0) a.first[E] = (int32_t)all;
-    } else if (warp < 4 && first) {  // tiles of 32, 128 and 192 rows
-        const uint32_t rows = warp == 1 ? 32 : warp == 2 ? 128 : 192;
+    } else if (warp < 5 && first) {  // tiles of 32, 128, 192 and 256 rows
+        const uint32_t rows = warp == 1 ? 32 : warp == 2 ? 128 : warp == 3 ? 192 : 256;
         int32_t *tiles = a.tiles + (uint64_t)(warp - 1) * (E + 1);
         const uint32_t all = warp_sums(E, lane, [&](uint32_t e) { return (total[e] + rows - 1) / rows; }, [&](uint32_t e, uint32_t v) { tiles[e] = (int32_t)v; });
         if (lane == 0) tiles[E] = (int32_t)all;

@@ -12,9 +12,9 @@
 //           tcgen05.cp spreads over TMEM as the tensor cores take scales.
 // So one bulk copy of 17408 contiguous bytes brings a stage of an operand, without a
 // tensor map.  Rows past the last are zeros in a matrix; columns past the last are too
-// (codes 0, scale byte 0).  Quantized activations have the same form with 32, 128 or 192
-// rows a tile (codes of that many rows, then the scales; of 192 rows a half's are two such
-// blocks, the second of rows 128 on).
+// (codes 0, scale byte 0).  Quantized activations have the same form with 32, 128, 192 or
+// 256 rows a tile (codes of that many rows, then the scales; of more than 128 rows a half's are
+// two such blocks, the second of rows 128 on).
 #pragma once
 
 #include "common.cuh"
@@ -82,7 +82,7 @@ struct Mx4GemmArgs {
     uint32_t n_expert;
     bool vec;                      // out allows 16-byte stores of eight features
 };
-cudaError_t mx4_many_launch(const Mx4GemmArgs &a, uint64_t token_tiles, int sms, cudaStream_t s);
+cudaError_t mx4_many_launch(const Mx4GemmArgs &a, uint32_t x_rows, uint64_t token_tiles, int sms, cudaStream_t s);
 cudaError_t mx4_few_launch(const Mx4GemmArgs &a, uint32_t x_rows, uint64_t token_tiles, int sms, cudaStream_t s);
 
 // The choice of experts and the sorting of its pairs.
@@ -99,7 +99,7 @@ struct MoeSortArgs {
     int32_t *ids;
     float *weights;
     int32_t *first, *order, *place;
-    int32_t *tiles;                // [3][n_expert + 1]: the same for tiles of 32, 128 and 192 rows
+    int32_t *tiles;                // [4][n_expert + 1]: the same for tiles of 32, 128, 192 and 256 rows
     int32_t *counts;               // [a row for MOE_SORT_JOIN stretches][counts_ld]
     uint32_t counts_ld;            // n_expert, up to the next multiple of four
 };

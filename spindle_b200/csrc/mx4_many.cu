@@ -28,18 +28,19 @@ constexpr uint32_t EPI_WARPS = 16, FIRST_EPI = 4, THREADS = 32 * (FIRST_EPI + EP
 constexpr uint32_t HDR = 1024 + EXPERTS_BYTES;     // barriers and TMEM base; what is looked up of the experts
 constexpr uint32_t GROUPS = EPI_WARPS / 4;       // four warps take a piece of 16 tokens, 32 features each
 
-template <bool DUAL>
+// Up to NT tokens a tile; DUAL: gate and up.
+template <uint32_t N, bool D>
 struct Cfg {
-    // Two buffers of sums where TMEM has room for them beside the scales: the products of a tile run while the results of the
-    // one before are taken (32760 places, 768 columns to 2048: 60 us; with tiles of 256 tokens and one buffer 63).  Gate and up of 96 tokens
-    // would fit twice too, but then each brings its weights for fewer tokens.
-    static constexpr uint32_t NT = DUAL ? 128 : 192, XT = DUAL ? 1 : 2, BUFS = DUAL ? 1 : 2, X_TILE = mx4_tile_bytes(NT);
+    static constexpr uint32_t NT = N, XT = (NT + 127) / 128, X_TILE = mx4_tile_bytes(NT);
+    static constexpr bool DUAL = D;
     static constexpr uint32_t W_BYTES = MX4_TILE * (DUAL ? 2 : 1), X_BYTES = NT / 2 * 128, XS_BYTES = mx4_scale_bytes(NT);
     static constexpr uint32_t STAGE = W_BYTES + X_BYTES + XS_BYTES;
     static constexpr uint32_t STAGES = DUAL ? 4 : 5;
     static constexpr uint32_t PIECES = NT / 16 / GROUPS;
     static constexpr uint32_t OUT_AT = HDR + STAGES * STAGE, SMEM = OUT_AT + GROUPS * OUT_BYTES;
-    static constexpr uint32_t SUMS = NT * (DUAL ? 2 : BUFS), SC = 8 * ((DUAL ? 2 : 1) + XT), COLS = 512;
+    // TMEM: sums, in two buffers in turn where there is room beside the scales
+    static constexpr uint32_t SC = 8 * ((DUAL ? 2 : 1) + XT), COLS = 512, ONE = NT * (DUAL ? 2 : 1), BUFS = 2 * ONE + STAGES * SC <= COLS ? 2 : 1;
+    static constexpr uint32_t SUMS = ONE * BUFS;
     static_assert(SUMS + STAGES * SC <= COLS && SMEM <= 227 * 1024 && STAGE % 1024 == 0 && NT % (16 * GROUPS) == 0, "shapes");
 };
 
@@ -59,9 +60,9 @@ __device__ __forceinline__ void arrive_at(uint64_t *bar, uint32_t rank) {
         : "memory");
 }
 
-template <bool DUAL>
+template <typename C>
 __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_constant__ Mx4GemmArgs a) {
-    using C = Cfg<DUAL>;
+    constexpr bool DUAL = C::DUAL;
     extern __shared__ __align__(1024) uint8_t smem[];
     Shared &sh = *reinterpret_cast<Shared *>(smem);
     Experts &ex = *reinterpret_cast<Experts *>(smem + 1024);
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
             const uint64_t ws_desc = desc_scales(base + MX4_ROWS * 128), xs_desc = desc_scales(base + C::W_BYTES + C::X_BYTES);
             for (uint32_t i = me; i < tiles && ok; i += pairs, count++) {
                 const Tile t = tile_at(i);
-                const uint32_t n = (t.rows + 31) & ~31u, id = idesc(256, n, 0), b = count % C::BUFS, sums = tmem + b * C::NT;
+                const uint32_t n = (t.rows + 31) & ~31u, id = idesc(256, n, 0), b = count % C::BUFS, sums = tmem + b * C::ONE;
                 if (count >= C::BUFS) ok = wait(&sh.sums_empty[b], (count / C::BUFS - 1) & 1);
                 if (!ok) break;
                 fence_after();
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
             }
             fence_after();
             float v[16 * C::PIECES * (DUAL ? 2 : 1)];  // the sums of the pieces, then those of `up`
-            const uint32_t at = tmem + b * C::NT + ((32 * q) << 16) + 16 * g;
+            const uint32_t at = tmem + b * C::ONE + ((32 * q) << 16) + 16 * g;
 #pragma unroll
             for (uint32_t c = 0; c < C::PIECES; c++)
                 if (t.rows > APART * c + 16 * g) {
@@ -251,10 +252,9 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
     }
 }
 
-template <bool DUAL>
+template <typename C>
 cudaError_t launch_as(const Mx4GemmArgs &a, uint64_t tiles, int sms, cudaStream_t s) {
-    using C = Cfg<DUAL>;
-    auto fn = mx4_many_kernel<DUAL>;
+    auto fn = mx4_many_kernel<C>;
     static bool ready[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -281,9 +281,10 @@ cudaError_t launch_as(const Mx4GemmArgs &a, uint64_t tiles, int sms, cudaStream_
 
 }  // namespace
 
-cudaError_t mx4_many_launch(const Mx4GemmArgs &a, uint64_t token_tiles, int sms, cudaStream_t s) {
+cudaError_t mx4_many_launch(const Mx4GemmArgs &a, uint32_t x_rows, uint64_t token_tiles, int sms, cudaStream_t s) {
     const uint64_t tiles = token_tiles * ((a.feat_tiles + 1) / 2);
-    return a.up ? launch_as<true>(a, tiles, sms, s) : launch_as<false>(a, tiles, sms, s);
+    if (a.up) return launch_as<Cfg<128, true>>(a, tiles, sms, s);
+    return x_rows == 256 ? launch_as<Cfg<256, false>>(a, tiles, sms, s) : launch_as<Cfg<192, false>>(a, tiles, sms, s);
 }
 
 }  // namespace sg

@@ -48,28 +48,34 @@ class Mx4:
         return n
 
 
-def _matrix(m, t, what):
+def _matrix(m, t, what, dev):
     """Row and expert stride of t, a tensor of m's shape ([rows, cols], or [experts, rows, cols])."""
     shape, stride = t.shape, t.stride()
-    if len(shape) == 2 and m.experts == 1:
-        shape, stride = (1,) + tuple(shape), (0,) + tuple(stride)
-    if tuple(shape) != (m.experts, m.rows, m.cols) or stride[2] != 1 or t.get_device() != m.dev:
+    if len(shape) == 2:
+        rows, cols = shape
+        ok, strides = m.experts == 1, (stride[0], 0)
+    elif len(shape) == 3:
+        experts, rows, cols = shape
+        ok, strides = experts == m.experts, (stride[1], stride[0])
+    else:
+        ok = False
+    if not ok or rows != m.rows or cols != m.cols or stride[-1] != 1 or t.get_device() != dev or m.dev != dev:
         raise ValueError("%s must be a tensor of the matrix's shape with contiguous rows on its CUDA device" % what)
-    return stride[1], stride[0]
+    return strides
 
 
 def mx4_quantize(x, out=None, stream=None):
     """The Mx4 of x [rows, cols] or [experts, rows, cols] (float32, float16 or
     bfloat16, contiguous rows any distance apart), or into out."""
-    _dev(x, "x")
-    if x.dim() not in (2, 3):
-        raise ValueError("x must be [rows, cols] or [experts, rows, cols]")
-    kind = _type(x, "x")
+    dev, kind = _dev(x, "x"), _type(x, "x")
     if out is None:
+        shape = x.shape
+        if len(shape) not in (2, 3):
+            raise ValueError("x must be [rows, cols] or [experts, rows, cols]")
+        size = (shape[-2], shape[-1], shape[0] if len(shape) == 3 else 1)
         with _on(stream):
-            out = Mx4(x.shape[-2], x.shape[-1], x.shape[0] if x.dim() == 3 else 1, data=torch.empty(
-                Mx4.bytes_for(x.shape[-2], x.shape[-1], x.shape[0] if x.dim() == 3 else 1), dtype=torch.uint8, device=x.device))
-    ld, le = _matrix(out, x, "x")
+            out = Mx4(*size, data=torch.empty(Mx4.bytes_for(*size), dtype=torch.uint8, device=x.device))
+    ld, le = _matrix(out, x, "x", dev)
     st = _lib.load().sg_mx4_quantize(out._c, kind, x.data_ptr(), ld, le, _s(stream, x))
     if st:
         _lib.check(st, "mx4_quantize")
@@ -79,11 +85,10 @@ def mx4_quantize(x, out=None, stream=None):
 def mx4_dequantize(m, out=None, dtype=torch.float32, stream=None):
     """The values of m, [rows, cols] ([experts, rows, cols] if it has several) of
     dtype, or into out."""
-    _dev(m.data, "m")
     if out is None:
         with _on(stream):
             out = torch.empty(*((m.experts,) if m.experts > 1 else ()), m.rows, m.cols, dtype=dtype, device=m.data.device)
-    ld, le = _matrix(m, out, "out")
+    ld, le = _matrix(m, out, "out", _dev(out, "out"))
     st = _lib.load().sg_mx4_dequantize(m._c, _type(out, "out"), out.data_ptr(), ld, le, _s(stream, out))
     if st:
         _lib.check(st, "mx4_dequantize")
@@ -99,36 +104,36 @@ def mx4_scratch(w, rows, stream=None):
         return torch.empty(n, dtype=torch.uint8, device=w.data.device)
 
 
-def _product(x, w, up, out, dtype, rows, scratch, key, stream):
-    """What the two products have in common: arguments of the call."""
-    dev = _dev(x, "x")
-    shape, stride = x.shape, x.stride()
+def _product(x, shape, w, up, out, dtype, rows, scratch, key, stream):
+    """What the two products have in common: the arguments of the call from x on."""
+    dev, stride = _dev(x, "x"), x.stride()
     if len(shape) != 2 or shape[1] != w.cols or (stride[1] != 1 and shape[0]) or dev != w.dev:
         raise ValueError("x must be a tensor [rows, %d] with contiguous rows on the matrix's CUDA device" % w.cols)
-    if up is not None and ((up.experts, up.rows, up.cols) != (w.experts, w.rows, w.cols) or up.dev != dev):
+    if up is not None and (up.experts != w.experts or up.rows != w.rows or up.cols != w.cols or up.dev != dev):
         raise ValueError("up must be a matrix of w's shape on the same CUDA device")
-    kind = _type(x, "x")
     if out is None:
         with _on(stream):
             out = torch.empty(rows, w.rows, dtype=dtype or x.dtype, device=x.device)
+    n, feats = out.shape
     so = out.stride()
-    if out.shape != (rows, w.rows) or (so[1] != 1 and w.rows > 1 and rows) or out.get_device() != dev or (dtype or out.dtype) is not out.dtype:
+    if (n != rows or feats != w.rows or (so[1] != 1 and feats > 1 and rows) or out.get_device() != dev or
+            (dtype is not None and dtype is not out.dtype)):
         raise ValueError("out must be a tensor [%d, %d] with contiguous rows on x's device" % (rows, w.rows))
     if scratch is None:
         scratch = mx4_scratch(w, key, stream)
-    elif not scratch.is_contiguous() or scratch.get_device() != dev:
-        raise ValueError("scratch must be a contiguous tensor on x's device")
-    return kind, stride[0], _type(out, "out"), out, so[0], scratch
+    elif scratch.dtype is not torch.uint8 or not scratch.is_contiguous() or scratch.get_device() != dev:
+        raise ValueError("scratch must be a contiguous uint8 tensor on x's device")
+    return out, (_type(x, "x"), x.data_ptr(), stride[0]), (_type(out, "out"), out.data_ptr(), so[0], scratch.data_ptr(), scratch.numel(), _s(stream, x))
 
 
 def mx4_matmul(x, w, up=None, out=None, dtype=None, scratch=None, stream=None):
     """x w^T for x [rows, w.cols] (float32, float16 or bfloat16), its rows quantized as
     w is, whatever their number; with up silu(x w^T) * (x up^T).  Returns out
     [rows, w.rows] of dtype (x's if None)."""
-    rows = x.shape[0]
-    kind, ldx, okind, out, ldo, scratch = _product(x, w, up, out, dtype, rows, scratch, rows, stream)
-    st = _lib.load().sg_mx4_matmul(w._c, None if up is None else up._c, kind, x.data_ptr(), ldx, rows, okind, out.data_ptr(), ldo,
-                                   scratch.data_ptr(), scratch.numel() * scratch.element_size(), _s(stream, x))
+    shape = x.shape
+    rows = shape[0]
+    out, xs, rest = _product(x, shape, w, up, out, dtype, rows, scratch, rows, stream)
+    st = _lib.load().sg_mx4_matmul(w._c, None if up is None else up._c, *xs, rows, *rest)
     if st:
         _lib.check(st, "mx4_matmul")
     return out
@@ -215,16 +220,15 @@ def mx4_experts(x, w, plan, up=None, gather=None, out=None, dtype=None, scratch=
     with up silu(x w^T) * (x up^T).  x has a row per token (gather; the default where up
     is given) or per sorted place.  Rows past plan.first[-1] are left as they were."""
     gather = up is not None if gather is None else gather
-    rows = plan.n_tok * plan.n_used
+    rows, shape = plan.n_tok * plan.n_used, x.shape
     if w.experts != plan.n_expert:
         raise ValueError("the plan has %d experts, the matrix %d" % (plan.n_expert, w.experts))
-    if x.shape[0] != (plan.n_tok if gather else rows):
+    if shape[0] != (plan.n_tok if gather else rows):
         raise ValueError("x must have a row per %s" % ("token" if gather else "sorted place"))
-    kind, ldx, okind, out, ldo, scratch = _product(x, w, up, out, dtype, rows, scratch, plan, stream)
     if plan.dev != w.dev:
         raise ValueError("the plan must lie on the same CUDA device")
-    st = _lib.load().sg_mx4_experts(w._c, None if up is None else up._c, plan._c, kind, x.data_ptr(), ldx, int(gather), okind,
-                                    out.data_ptr(), ldo, scratch.data_ptr(), scratch.numel() * scratch.element_size(), _s(stream, x))
+    out, xs, rest = _product(x, shape, w, up, out, dtype, rows, scratch, plan, stream)
+    st = _lib.load().sg_mx4_experts(w._c, None if up is None else up._c, plan._c, *xs, 1 if gather else 0, *rest)
     if st:
         _lib.check(st, "mx4_experts")
     return out
@@ -233,18 +237,19 @@ def mx4_experts(x, w, plan, up=None, gather=None, out=None, dtype=None, scratch=
 def moe_combine(y, plan, out=None, dtype=None, stream=None):
     """The weighted sums of the experts' results (sg_moe_combine): y [n * n_used, dim],
     a row per sorted place, to out [n, dim] of dtype (y's if None)."""
-    dev = _dev(y, "y")
-    shape, stride = y.shape, y.stride()
+    dev, shape, stride = _dev(y, "y"), y.shape, y.stride()
     if len(shape) != 2 or shape[0] != plan.n_tok * plan.n_used or (stride[1] != 1 and shape[1] > 1) or plan.dev != dev:
         raise ValueError("y must be a tensor [%d, dim] with contiguous rows on the plan's CUDA device" % (plan.n_tok * plan.n_used))
-    kind = _type(y, "y")
+    dim = shape[1]
     if out is None:
         with _on(stream):
-            out = torch.empty(plan.n_tok, shape[1], dtype=dtype or y.dtype, device=y.device)
+            out = torch.empty(plan.n_tok, dim, dtype=dtype or y.dtype, device=y.device)
+    n, cols = out.shape
     so = out.stride()
-    if out.shape != (plan.n_tok, shape[1]) or (so[1] != 1 and shape[1] > 1) or out.get_device() != dev or (dtype or out.dtype) is not out.dtype:
-        raise ValueError("out must be a tensor [%d, %d] with contiguous rows on y's device" % (plan.n_tok, shape[1]))
-    st = _lib.load().sg_moe_combine(plan._c, kind, y.data_ptr(), stride[0], shape[1], _type(out, "out"), out.data_ptr(), so[0], _s(stream, y))
+    if (n != plan.n_tok or cols != dim or (so[1] != 1 and dim > 1) or out.get_device() != dev or
+            (dtype is not None and dtype is not out.dtype)):
+        raise ValueError("out must be a tensor [%d, %d] with contiguous rows on y's device" % (plan.n_tok, dim))
+    st = _lib.load().sg_moe_combine(plan._c, _type(y, "y"), y.data_ptr(), stride[0], dim, _type(out, "out"), out.data_ptr(), so[0], _s(stream, y))
     if st:
         _lib.check(st, "moe_combine")
     return out
