@@ -173,21 +173,25 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_few_kernel(const __grid_consta
             }
             fence_after();
             const uint32_t at = tmem + b * NT * (DUAL ? 2 : 1) + ((32 * q) << 16), f0 = i % a.feat_tiles * MX4_ROWS;
-            for (uint32_t c = 0; c < t.rows; c += 16) {
-                float v[16], u[16];
-                tmem_ld32x16(at + c, v);
-                if (DUAL) tmem_ld32x16(at + NT + c, u);
-                tmem_wait(v);
-                if (DUAL) {
-                    tmem_wait(u);
+            auto put = [&](auto type) {
+                const Out<decltype(type)> o(a, t.row0, f0, q, lane);
+                for (uint32_t c = 0; c < t.rows; c += 16) {
+                    float v[16], u[16];
+                    tmem_ld32x16(at + c, v);
+                    if (DUAL) tmem_ld32x16(at + NT + c, u);
+                    tmem_wait(v);
+                    if (DUAL) {
+                        tmem_wait(u);
 #pragma unroll
-                    for (int j = 0; j < 16; j++) v[j] = silu_times(v[j], u[j]);
+                        for (int j = 0; j < 16; j++) v[j] = silu_times(v[j], u[j]);
+                    }
+                    put_piece(a, o, sizeof(type) == 2 ? buf + (turn & 1) * (OUT_BYTES / 2) : buf, v, c, t.rows - c, q, lane, 0);
+                    turn++;
                 }
-                uint8_t *to = buf + (turn++ & 1) * (OUT_BYTES / 2);
-                if (a.type == SG_F32) put_piece<float>(a, buf, v, t.row0 + c, t.rows - c, f0, q, lane, 0);
-                else if (a.type == SG_F16) put_piece<__half>(a, to, v, t.row0 + c, t.rows - c, f0, q, lane, 0);
-                else put_piece<__nv_bfloat16>(a, to, v, t.row0 + c, t.rows - c, f0, q, lane, 0);
-            }
+            };
+            if (a.type == SG_F32) put(float());
+            else if (a.type == SG_F16) put(__half());
+            else put(__nv_bfloat16());
             fence_before();
             __syncwarp();
             if (elect_one()) arrive(&sh.sums_empty[b]);

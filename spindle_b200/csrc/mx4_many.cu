@@ -60,7 +60,7 @@ __device__ __forceinline__ void arrive_at(uint64_t *bar, uint32_t rank) {
         : "memory");
 }
 
-template <typename C>
+template <typename C, typename T>
 __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_constant__ Mx4GemmArgs a) {
     constexpr bool DUAL = C::DUAL;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -225,19 +225,17 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
             __syncwarp();
             const uint32_t f0 = (2 * pair_of(i) + rank) * MX4_ROWS;
             if (f0 >= a.feats) continue;
+            const Out<T> o(a, t.row0, f0, q, lane);
 #pragma unroll
             for (uint32_t c = 0; c < C::PIECES; c++)
                 if (t.rows > APART * c + 16 * g) {
-                    const uint32_t from = APART * c + 16 * g, n = t.rows - from;
+                    const uint32_t from = APART * c + 16 * g;
                     float *p = v + 16 * c;
                     if (DUAL) {
 #pragma unroll
                         for (int j = 0; j < 16; j++) p[j] = silu_times(p[j], p[16 * C::PIECES + j]);
                     }
-                    uint8_t *to = buf + (turn & 1) * (OUT_BYTES / 2);
-                    if (a.type == SG_F32) put_piece<float>(a, buf, p, t.row0 + from, n, f0, q, lane, g);
-                    else if (a.type == SG_F16) put_piece<__half>(a, to, p, t.row0 + from, n, f0, q, lane, g);
-                    else put_piece<__nv_bfloat16>(a, to, p, t.row0 + from, n, f0, q, lane, g);
+                    put_piece(a, o, sizeof(T) == 2 ? buf + (turn & 1) * (OUT_BYTES / 2) : buf, p, from, t.rows - from, q, lane, g);
                     turn++;
                 }
         }
@@ -252,9 +250,9 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
     }
 }
 
-template <typename C>
+template <typename C, typename T>
 cudaError_t launch_as(const Mx4GemmArgs &a, uint64_t tiles, int sms, cudaStream_t s) {
-    auto fn = mx4_many_kernel<C>;
+    auto fn = mx4_many_kernel<C, T>;
     static bool ready[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -279,12 +277,17 @@ cudaError_t launch_as(const Mx4GemmArgs &a, uint64_t tiles, int sms, cudaStream_
     return cudaLaunchKernelEx(&c, fn, a);
 }
 
+template <typename C>
+cudaError_t launch_type(const Mx4GemmArgs &a, uint64_t tiles, int sms, cudaStream_t s) {
+    return a.type == SG_F32 ? launch_as<C, float>(a, tiles, sms, s) : a.type == SG_F16 ? launch_as<C, __half>(a, tiles, sms, s) : launch_as<C, __nv_bfloat16>(a, tiles, sms, s);
+}
+
 }  // namespace
 
 cudaError_t mx4_many_launch(const Mx4GemmArgs &a, uint32_t x_rows, uint64_t token_tiles, int sms, cudaStream_t s) {
     const uint64_t tiles = token_tiles * ((a.feat_tiles + 1) / 2);
-    if (a.up) return launch_as<Cfg<128, true>>(a, tiles, sms, s);
-    return x_rows == 256 ? launch_as<Cfg<256, false>>(a, tiles, sms, s) : launch_as<Cfg<192, false>>(a, tiles, sms, s);
+    if (a.up) return launch_type<Cfg<128, true>>(a, tiles, sms, s);
+    return x_rows == 256 ? launch_type<Cfg<256, false>>(a, tiles, sms, s) : launch_type<Cfg<192, false>>(a, tiles, sms, s);
 }
 
 }  // namespace sg

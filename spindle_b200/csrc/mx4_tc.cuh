@@ -188,16 +188,17 @@ __device__ __forceinline__ void find_experts(const Mx4GemmArgs &a, Experts &ex, 
     }
 }
 
-// The tt-th tile of NT tokens, as x lies in memory.
+// The tt-th tile of NT tokens (there has to be one), as x lies in memory; by a whole warp.
 template <uint32_t NT>
 __device__ __forceinline__ Tile tile_of(const Mx4GemmArgs &a, const Experts &ex, uint32_t tt) {
     Tile t;
     if (a.first) {
-        uint32_t lo = 0, hi = a.n_expert - 1;  // the first expert whose tiles reach past tt
-        while (lo < hi) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (ex.upto[mid] > tt) hi = mid;
-            else lo = mid + 1;
+        // the first expert whose tiles reach past tt, 32 at a time
+        uint32_t lo = 0;
+        for (uint32_t base = 0; base < a.n_expert; base += 32) {
+            const uint32_t i = base + (threadIdx.x & 31u), before = __ballot_sync(0xffffffffu, i < a.n_expert && ex.upto[i] <= tt);
+            lo += __popc(before);
+            if (before != 0xffffffffu) break;
         }
         const uint32_t r = (tt - (lo ? ex.upto[lo - 1] : 0)) * NT, f0 = ex.first[lo], n = (lo + 1 < a.n_expert ? ex.first[lo + 1] : ex.n_rows) - f0;
         t.e = lo;
@@ -222,49 +223,66 @@ __device__ __forceinline__ uint32_t pack(__nv_bfloat16, float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// A piece of 16 tokens (n of them are there) by 128 features from f0 on, of which a warp has 32 in v as tmem_ld32x16 gives
-// them, to rows of the output from `row` on: by way of shared memory, where the four warps' features of a token come
+// Where a thread's part of a tile's results goes, of a token 128 features from f0 on: 16 bytes of every eighth token (of f32:
+// fourth), from row `row` of the output on.
+template <typename T>
+struct Out {
+    static constexpr uint32_t ROW = MX4_ROWS * sizeof(T) + 16, PER = MX4_ROWS * sizeof(T) / 16, ES = 16 / sizeof(T), STEP = 128 / PER;
+    T *at;
+    uint32_t left;  // features from there on; at least ES: 16-byte stores
+    static __device__ __forceinline__ uint32_t token(uint32_t warp, uint32_t lane) { return (32 * warp + lane) / PER; }
+    static __device__ __forceinline__ uint32_t chunk(uint32_t warp, uint32_t lane) { return (32 * warp + lane) % PER; }
+    __device__ __forceinline__ Out(const Mx4GemmArgs &a, uint64_t row, uint32_t f0, uint32_t warp, uint32_t lane) {
+        const uint32_t f = f0 + chunk(warp, lane) * ES;
+        at = static_cast<T *>(a.out) + (row + token(warp, lane)) * a.ldo + f;
+        left = f < a.feats ? a.feats - f : 0;
+    }
+};
+
+// A piece of 16 tokens (n of them are there, the first of them the tile's `from`th) by 128 features, of which a warp has 32 in
+// v as tmem_ld32x16 gives them, to the output by way of shared memory, where the four warps' features of a token come
 // together.  16-bit results go there eight by eight, turned over on the way (stmatrix), to one of two places in turn, so that
 // one barrier a piece will do.
 template <typename T>
-__device__ __forceinline__ void put_piece(const Mx4GemmArgs &a, uint8_t *buf, const float *v, uint64_t row, uint32_t n, uint32_t f0, uint32_t warp,
+__device__ __forceinline__ void put_piece(const Mx4GemmArgs &a, const Out<T> &o, uint8_t *buf, const float *v, uint32_t from, uint32_t n, uint32_t warp,
                                           uint32_t lane, uint32_t group) {
-    constexpr uint32_t ROW = MX4_ROWS * sizeof(T) + 16, PER = MX4_ROWS * sizeof(T) / 16, ES = 16 / sizeof(T);
+    using O = Out<T>;
     if constexpr (sizeof(T) == 2) {
-        const uint32_t at = smem_u32(buf) + (lane & 7) * ROW + (32 * warp + 8 * (lane >> 3)) * 2;
+        const uint32_t at = smem_u32(buf) + (lane & 7) * O::ROW + (32 * warp + 8 * (lane >> 3)) * 2;
 #pragma unroll
         for (uint32_t b = 0; b < 2; b++) {
             const float *lo = v + 4 * b, *hi = v + 8 + 4 * b;
-            asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at + 8 * b * ROW), "r"(pack(T(), lo[0], lo[1])),
+            asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at + 8 * b * O::ROW), "r"(pack(T(), lo[0], lo[1])),
                          "r"(pack(T(), lo[2], lo[3])), "r"(pack(T(), hi[0], hi[1])), "r"(pack(T(), hi[2], hi[3]))
                          : "memory");
         }
     } else {
         asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");  // the piece before has been read
-        float *at = reinterpret_cast<float *>(buf + 2 * (lane & 3) * ROW) + 32 * warp + (lane >> 2);
+        float *at = reinterpret_cast<float *>(buf + 2 * (lane & 3) * O::ROW) + 32 * warp + (lane >> 2);
 #pragma unroll
         for (uint32_t b = 0; b < 2; b++)
 #pragma unroll
             for (uint32_t i = 0; i < 8; i++)  // (token 8 b + 2 (lane % 4) + i % 2, feature 8 (i / 2) + lane / 4 of the warp's)
-                at[(8 * b + (i & 1)) * (ROW / 4) + 8 * (i >> 1)] = v[(i >> 2) * 8 + 4 * b + (i & 3)];
+                at[(8 * b + (i & 1)) * (O::ROW / 4) + 8 * (i >> 1)] = v[(i >> 2) * 8 + 4 * b + (i & 3)];
     }
     asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
-    T *out = static_cast<T *>(a.out);
+    const uint32_t token = O::token(warp, lane);
+    const uint8_t *mine = buf + token * O::ROW + 16 * O::chunk(warp, lane);
+    T *to = o.at + from * a.ldo;
+    const bool whole = a.vec && o.left >= O::ES;
 #pragma unroll
-    for (uint32_t i = 0; i < 16 * PER / 128; i++) {
-        const uint32_t at = i * 128 + 32 * warp + lane, t = at / PER, c = at % PER, f = f0 + c * ES;
-        if (t < n && f < a.feats) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(buf + t * ROW + 16 * c);
-            T *o = out + (row + t) * a.ldo + f;
-            if (a.vec && f + ES <= a.feats) *reinterpret_cast<uint4 *>(o) = w;
-            else
+    for (uint32_t t = 0; t < 16; t += O::STEP, to += O::STEP * a.ldo) {
+        if (token + t >= n) break;
+        const uint4 w = *reinterpret_cast<const uint4 *>(mine + t * O::ROW);
+        if (whole) *reinterpret_cast<uint4 *>(to) = w;
+        else {
+            const T *e = reinterpret_cast<const T *>(&w);
 #pragma unroll
-                for (uint32_t j = 0; j < ES; j++)
-                    if (f + j < a.feats) o[j] = reinterpret_cast<const T *>(&w)[j];
+            for (uint32_t j = 0; j < O::ES; j++)
+                if (j < o.left) to[j] = e[j];
         }
     }
 }
-
 
 }  // namespace mx4
 }  // namespace sg
