@@ -2,7 +2,10 @@
 grow and end between steps, on the paged operators (kv4_plan, kv4_append,
 kv4_attention, logprobs) and the framework's own projections (matmul_batch),
 feed-forward layers (moe_forward_batch) and LM head.  The weights are named as
-for decoder.Decoder; the embedding is F32 or F16 rows.
+for decoder.Decoder; the embedding is F32 or F16 rows.  A matrix that is given as
+an Mx4, or as F32 or F16 rows (which become one), is multiplied in microscaled 4
+bits (mx4_matmul), all tokens of a step in one call; a layer's experts too, sorted by
+expert (moe_route, mx4_experts, moe_combine).
 
     p = PagedDecoder(cfg, weights, dtypes, device, n_req=8, n_blocks=512)
     out = p.step({0: prompt_a, 3: prompt_b})        # tokens of the requests that go on
@@ -13,8 +16,28 @@ import torch
 
 from . import F16, F32, Moe, matmul_batch, moe_forward_batch, repack_tiled16
 from .kv4 import LOGPROBS_TOP_MAX, Kv4Cache, Kv4Plan, LogProbs, kv4_append, kv4_attention, kv4_attention_scratch, kv4_plan, logprobs
+from .mx4 import MoePlan, Mx4, moe_combine, moe_route, mx4_experts, mx4_matmul, mx4_quantize
 
 BATCH = 128  # tokens of one batch GEMM or expert pass
+
+
+class Mx4Ffn:
+    """A feed-forward layer in microscaled 4 bits: silu(x gate) * (x up), down; with a
+    router a mixture of experts (moe: n_expert, n_used, norm, prune), n_max tokens at
+    a time."""
+
+    def __init__(self, gate, up, down, router=None, moe=None, n_max=0):
+        self.gate, self.up, self.down, self.router, self.moe = gate, up, down, router, moe
+        if (gate.experts, gate.rows, gate.cols) != (up.experts, up.rows, up.cols) or (down.experts, down.cols) != (gate.experts, gate.rows):
+            raise ValueError("gate, up and down do not fit together")
+        if moe:
+            self.plan = MoePlan(n_max, moe["n_used"], moe["n_expert"], device=gate.data.device)
+
+    def __call__(self, x):
+        if not self.moe:
+            return mx4_matmul(mx4_matmul(x, self.gate, up=self.up), self.down)
+        p = moe_route(x @ self.router.T, self.plan, norm=self.moe.get("norm", True), prune=self.moe.get("prune", 0.0))
+        return moe_combine(mx4_experts(mx4_experts(x, self.gate, p, up=self.up), self.down, p), p)
 
 
 class PagedDecoder:
@@ -31,13 +54,31 @@ class PagedDecoder:
             raise ValueError("the embedding must be F32 or F16 rows")
         self.embed = weights["embed"].view(torch.float32 if dtypes["embed"] == F32 else torch.float16).view(c["vocab"], dim)
 
+        def mx4(name, *shape):
+            """The matrix (or a layer's experts) if it is one in microscaled 4 bits, else None."""
+            w = weights[name]
+            if isinstance(w, Mx4):
+                if (w.experts, w.rows, w.cols) != ((1,) + shape)[-3:]:
+                    raise ValueError("%s must be a matrix %s" % (name, shape))
+                return w
+            if dtypes[name] not in (F32, F16):
+                return None
+            return mx4_quantize(w.view(torch.float32 if dtypes[name] == F32 else torch.float16).view(*shape))
+
         def mat(name, rows, cols):
-            return repack_tiled16(dtypes[name], weights[name], rows, cols)
+            return mx4(name, rows, cols) or repack_tiled16(dtypes[name], weights[name], rows, cols)
 
         self.layers = []
         for i in range(c["n_layers"]):
             p, moe = "l%d." % i, c.get("moe")
-            if moe:
+            names = [p + k + ("_exps" if moe else "") for k in ("gate", "up", "down")]
+            ff, each = (moe["n_ff"], (moe["n_expert"],)) if moe else (c["n_ff"], ())
+            in4 = [mx4(names[0], *each, ff, dim), mx4(names[1], *each, ff, dim), mx4(names[2], *each, dim, ff)]
+            if any(m is not None for m in in4):
+                if any(m is None for m in in4):
+                    raise ValueError("gate, up and down of a layer are all in microscaled 4 bits or none of them")
+                ffn = Mx4Ffn(*in4, router=weights[p + "router"].float().view(moe["n_expert"], dim) if moe else None, moe=moe, n_max=max_tokens)
+            elif moe:
                 ffn = Moe.pack(weights[p + "router"].float(), weights[p + "gate_exps"], weights[p + "up_exps"],
                                weights[p + "down_exps"], dtypes[p + "gate_exps"], dtypes[p + "down_exps"], moe["n_expert"],
                                moe["n_used"], dim, moe["n_ff"], norm=moe.get("norm", True), moe_prune=moe.get("prune", 0.0))
@@ -60,6 +101,8 @@ class PagedDecoder:
         return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + self.cfg["rms_eps"]) * w
 
     def _mm(self, m, x):
+        if isinstance(m, Mx4):
+            return mx4_matmul(x, m)
         t, mat = m
         out = torch.empty(x.shape[0], mat.rows, dtype=torch.float32, device=x.device)
         for a in range(0, x.shape[0], BATCH):
@@ -128,9 +171,12 @@ class PagedDecoder:
             o = kv4_attention(y["cache"], q.contiguous(), p.cu, p.seq, self.tables, scale=scale, max_new=most, scratch=self.scratch)
             x = x + self._mm(y["wo"], o.view(n, -1)) * c.get("residual_scale", 1.0)
             h = self._norm(x, w("ffn_norm")).contiguous()
-            f = torch.empty_like(x)
-            for a in range(0, n, BATCH):
-                moe_forward_batch(y["ffn"], h[a:a + BATCH], out=f[a:a + BATCH])
+            if isinstance(y["ffn"], Mx4Ffn):
+                f = y["ffn"](h)
+            else:
+                f = torch.empty_like(x)
+                for a in range(0, n, BATCH):
+                    moe_forward_batch(y["ffn"], h[a:a + BATCH], out=f[a:a + BATCH])
             x = x + f * c.get("residual_scale", 1.0)
         last = torch.tensor([sum(new[q] for q in go if q <= r) - 1 for r in go], device=self.dev)
         logits = self._mm(self.head, self._norm(x[last], self.w["out_norm"]).contiguous())
@@ -138,28 +184,8 @@ class PagedDecoder:
         return {"requests": go, "logits": logits, "next": nxt, "probs": logprobs(logits, nxt.int(), top=top, out=LogProbs(len(go), top, self.dev))}
 
 
-def main():
-    """A few requests of a small random model, served together."""
-    from . import Q4_K, Q6_K, quantize_weights
-    dev = torch.device("cuda")
-    g = torch.Generator(device=dev).manual_seed(0)
-    cfg = dict(dim=512, n_heads=8, n_kv_heads=2, head_dim=64, n_layers=2, vocab=1024, max_seq=512, n_ff=768, rope_theta=1e6,
-               rms_eps=1e-6, rope_neox=True)
-    dim, w, dt = cfg["dim"], {}, {}
-
-    def mat(name, rows, cols, kind):
-        w[name], dt[name] = quantize_weights(kind, torch.randn(rows, cols, device=dev, generator=g) * 0.05), kind
-
-    w["embed"], dt["embed"] = torch.randn(cfg["vocab"], dim, device=dev, generator=g).half().view(torch.uint8), F16
-    mat("head", cfg["vocab"], dim, Q6_K)
-    w["out_norm"] = torch.ones(dim, device=dev)
-    for i in range(cfg["n_layers"]):
-        p = "l%d." % i
-        w[p + "attn_norm"], w[p + "ffn_norm"] = torch.ones(dim, device=dev), torch.ones(dim, device=dev)
-        for name, rows, cols in (("wq", 512, dim), ("wk", 128, dim), ("wv", 128, dim), ("wo", dim, 512), ("gate", 768, dim), ("up", 768, dim),
-                                 ("down", dim, 768)):
-            mat(p + name, rows, cols, Q4_K)
-    d = PagedDecoder(cfg, w, dt, dev, n_req=4, n_blocks=64, page=16)
+def serve(d):
+    """A few requests served together, printed."""
     out = d.step({0: list(range(5, 45)), 2: [7, 8, 9]}, top=3)
     for step in range(8):
         ids = out["next"].tolist()
@@ -171,6 +197,37 @@ def main():
         if step == 5:
             del nxt[2]                 # and one ends
         out = d.step(nxt, end=[2] if step == 5 else [], top=3)
+
+
+def main():
+    """Two small random models: K-quants, and a mixture of experts in microscaled 4 bits."""
+    from . import Q4_K, Q6_K, quantize_weights
+    dev = torch.device("cuda")
+    g = torch.Generator(device=dev).manual_seed(0)
+    dense = dict(dim=512, n_heads=8, n_kv_heads=2, head_dim=64, n_layers=2, vocab=1024, max_seq=512, n_ff=768, rope_theta=1e6,
+                 rms_eps=1e-6, rope_neox=True)
+    for cfg in (dense, dict(dense, moe=dict(n_expert=16, n_used=4, n_ff=256))):
+        dim, w, dt = cfg["dim"], {}, {}
+
+        def mat(name, kind, *shape):
+            x = torch.randn(*shape, device=dev, generator=g) * 0.05
+            w[name], dt[name] = (mx4_quantize(x), None) if cfg.get("moe") else (quantize_weights(kind, x), kind)  # noqa: B023
+
+        w["embed"], dt["embed"] = torch.randn(cfg["vocab"], dim, device=dev, generator=g).half().view(torch.uint8), F16
+        mat("head", Q6_K, cfg["vocab"], dim)
+        w["out_norm"] = torch.ones(dim, device=dev)
+        for i in range(cfg["n_layers"]):
+            p, moe = "l%d." % i, cfg.get("moe")
+            w[p + "attn_norm"], w[p + "ffn_norm"] = torch.ones(dim, device=dev), torch.ones(dim, device=dev)
+            for name, rows, cols in (("wq", 512, dim), ("wk", 128, dim), ("wv", 128, dim), ("wo", dim, 512)):
+                mat(p + name, Q4_K, rows, cols)
+            ff, each, s = (moe["n_ff"], (moe["n_expert"],), "_exps") if moe else (cfg["n_ff"], (), "")
+            for name, rows, cols in (("gate", ff, dim), ("up", ff, dim), ("down", dim, ff)):
+                mat(p + name + s, Q4_K, *each, rows, cols)
+            if moe:
+                w[p + "router"] = torch.randn(moe["n_expert"], dim, device=dev, generator=g) * 0.05
+        print("experts in microscaled 4 bits:" if cfg.get("moe") else "K-quants:")
+        serve(PagedDecoder(cfg, w, dt, dev, n_req=4, n_blocks=64, page=16))
 
 
 if __name__ == "__main__":
