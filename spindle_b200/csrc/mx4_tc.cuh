@@ -170,21 +170,27 @@ struct Tile {
 // The experts' lookups for tiles of nt tokens, by one warp.
 __device__ __forceinline__ void find_experts(const Mx4GemmArgs &a, Experts &ex, uint32_t nt, uint32_t lane) {
     uint32_t before = 0;
-    for (uint32_t base = 0; base < a.n_expert; base += 32) {
-        const uint32_t i = base + lane;
-        const uint32_t f0 = i < a.n_expert ? (uint32_t)__ldg(a.first + i) : 0, f1 = i < a.n_expert ? (uint32_t)__ldg(a.first + i + 1) : 0;
-        uint32_t n = (f1 - f0 + nt - 1) / nt;
+    for (uint32_t base = 0; base < a.n_expert; base += 128) {  // four experts a lane
+        uint32_t f[5], n[4], upto = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < 5; k++) f[k] = (uint32_t)__ldg(a.first + min(base + 4 * lane + k, a.n_expert));
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) upto += n[k] = (f[k + 1] - f[k] + nt - 1) / nt;
+        const uint32_t mine = upto;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t v = __shfl_up_sync(0xffffffffu, n, o);
-            if (lane >= (uint32_t)o) n += v;
+            const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= (uint32_t)o) upto += v;
         }
-        if (i < a.n_expert) {
-            ex.upto[i] = before + n;
-            ex.first[i] = f0;
-            if (i + 1 == a.n_expert) ex.n_rows = f1;
+        uint32_t at = before + upto - mine;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) {
+            const uint32_t e = base + 4 * lane + k;
+            at += n[k];
+            if (e < a.n_expert) ex.upto[e] = at, ex.first[e] = f[k];
+            if (e + 1 == a.n_expert) ex.n_rows = f[k + 1];
         }
-        before += __shfl_sync(0xffffffffu, n, 31);
+        before += __shfl_sync(0xffffffffu, upto, 31);
     }
 }
 
