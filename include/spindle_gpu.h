@@ -686,7 +686,7 @@ SG_API sg_status sg_mx4_dequantize(const sg_mx4 *m, int32_t type, void *d_out, u
 /* out[t, n] = sum over k of q(x)[t, k] w[n, k] for n_tok rows of x, each quantized
  * as above on the way, whatever their number; with `up` (a matrix of w's shape)
  * silu(that) * (the same with up).  w has one expert.  Products are exact and added
- * in f32; the results are rounded once, to out_type.
+ * in f32; the results are rounded once, to out_type.  d_out may be d_x.
  * d_scratch: sg_mx4_scratch_bytes(w, n_tok, NULL) bytes (0 is possible), 128-byte
  * aligned, for calls that may overlap on the GPU one each. */
 typedef struct sg_moe_plan_ sg_moe_plan;
@@ -732,7 +732,7 @@ SG_API sg_status sg_mx4_experts(const sg_mx4 *w, const sg_mx4 *up, const sg_moe_
                                 uint64_t ldx, int32_t gather, int32_t out_type, void *d_out, uint64_t ldo,
                                 void *d_scratch, uint64_t scratch_bytes, void *stream);
 /* out[t] = sum over j of weights[t, j] * y[place[t, j]], dim columns, in f32 in the
- * order of j and rounded once; zeros for a token without any. */
+ * order of j and rounded once; zeros for a token without any.  d_out must not overlap d_y. */
 SG_API sg_status sg_moe_combine(const sg_moe_plan *plan, int32_t type, const void *d_y, uint64_t ldy, uint64_t dim, int32_t out_type,
                                 void *d_out, uint64_t ldo, void *stream);
 

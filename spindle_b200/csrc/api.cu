@@ -2804,6 +2804,8 @@ sg_status sg_moe_combine(const sg_moe_plan *plan, int32_t type, const void *d_y,
     const uint64_t pairs = plan->n_tok * plan->n_used;
     if (!d_y || !d_out || (pairs > 1 && ldy < dim) || (plan->n_tok > 1 && ldo < dim)) return SG_ERR_INVALID;
     if (!aligned(d_y, es) || !aligned(d_out, eo)) return SG_ERR_ALIGN;
+    // (a token's sum is written while others still read theirs)
+    if (overlap(d_y, ((pairs - 1) * ldy + dim) * es, d_out, ((plan->n_tok - 1) * ldo + dim) * eo)) return SG_ERR_INVALID;
     DevInfo *di;
     if (sg_status st = dev_info(&di)) return st;
     const MoeCombineArgs a = {d_y, ldy, ldo, d_out, plan->place, plan->weights, plan->n_tok, (uint32_t)plan->n_used, (uint32_t)dim,

@@ -81,6 +81,22 @@ def test_sort_of_given_ids(dev, n, e, k):
         check_sort(p, ids, e)
 
 
+def test_nothing_to_sort(dev):
+    p = sg.moe_route(torch.zeros(0, 32, device=dev), sg.MoePlan(10, 4, 32, device=dev))
+    assert p.ids.shape == (0, 4) and p.first.tolist() == [0] * 33
+    w = sg.mx4_quantize(rand(dev, 32, 64, 64))
+    assert sg.mx4_experts(torch.zeros(0, 64, device=dev), w, p).shape == (0, 64)
+    assert sg.moe_combine(torch.zeros(0, 64, device=dev), p).shape == (0, 64)
+    # tokens without any expert: no product, zeros back
+    p = sg.moe_route(torch.full((5, 32), float("-inf"), device=dev), sg.MoePlan(10, 4, 32, device=dev))
+    x = rand(dev, 5, 64)
+    y = torch.full((20, 64), 7.0, device=dev)
+    sg.mx4_experts(x, w, p, gather=True, out=y)
+    assert (y == 7).all() and sg.moe_combine(y, p).count_nonzero() == 0 and (p.order == -1).all()
+    with pytest.raises(sg.SgError):
+        sg.moe_combine(y, p, out=y[:5])           # over its own input
+
+
 def test_plans_are_used_again(dev):
     p = sg.MoePlan(3000, 4, 32, device=dev)
     for n in (3000, 5, 0, 64, 2999):

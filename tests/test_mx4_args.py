@@ -86,6 +86,8 @@ def test_sort_refusals():
     assert comb(t=8) == DTYPE and comb(ot=8) == DTYPE and comb(dim=0) == SHAPE and comb(ldy=63) == INVALID and comb(ldo=63) == INVALID
     assert comb(y=None) == INVALID and comb(o=None) == INVALID and comb(y=AT + 2) == ALIGN
     assert comb(p=plan(n_tok=0), y=None, o=None) == OK
+    # 8 rows of y, 4 of out: no byte in common
+    assert comb(o=AT + 8 * 256 - 4) == INVALID and comb(o=AT - 4 * 256 + 4) == INVALID
 
 
 def test_host_tensors():

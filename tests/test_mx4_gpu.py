@@ -142,6 +142,50 @@ def test_matmul_of_zeros_and_far_scales(dev, rows):
     assert U.close(sg.mx4_matmul(x * 2.0 ** 90, sg.mx4_quantize(w * 2.0 ** -100)), want, bound)
 
 
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_matmul_at_the_ends_of_the_scales(dev, rows):
+    # scale bytes down to 0 (2^-127) and up to 252: products of the smallest and the largest, and of the smallest alone
+    x, w = rand(dev, rows, 256, seed=8), rand(dev, 140, 256, seed=9) * 0.0625
+    for a, b in ((-124, 120), (-123, 126), (120, -124), (-80, -60)):
+        xs, ws = x * 2.0 ** a, w * 2.0 ** b
+        want, bound = U.product(U.quantized(xs), U.quantized(ws))
+        # (results below f32's normal numbers may be cut off)
+        assert U.close(sg.mx4_matmul(xs, sg.mx4_quantize(ws)), want, bound + 2.0 ** -126)
+
+
+def test_matmul_into_its_own_rows(dev):
+    for rows in (1, 40, 300):
+        x, W = rand(dev, rows, 256, seed=rows), sg.mx4_quantize(rand(dev, 256, 256, seed=1) * 0.06)
+        want = sg.mx4_matmul(x, W)
+        assert sg.mx4_matmul(x, W, out=x) is x and torch.equal(x, want)
+
+
+def test_matmul_past_two_to_the_31(dev):
+    # more than 2^31 results, and rows that begin past 2^32 bytes
+    rows, n = 17001, 130000
+    x, w = rand(dev, rows, 64, seed=1), rand(dev, n, 64, seed=2) * 0.125
+    y = sg.mx4_matmul(x, sg.mx4_quantize(w), dtype=torch.float16)
+    for r in ([0, 1, 5000], [8191, 8192, 16519, 16520], [16800, 16999, 17000]):
+        for f in (slice(0, 300), slice(65000, 65300), slice(n - 300, n)):
+            want, bound = U.product(U.quantized(x[r]), U.quantized(w[f]))
+            assert U.close(y[r, f], want, bound)
+    del y
+    torch.cuda.empty_cache()
+
+
+def test_dequantize_past_two_to_the_31(dev):
+    rows, cols = 70001, 32768
+    x = torch.zeros(rows, cols, dtype=torch.float16, device=dev)
+    some = [0, 65535, 65536, 65537, 70000]
+    x[some] = rand(dev, len(some), cols, seed=3).half()
+    m = sg.mx4_quantize(x)
+    want = U.quantized(x[some])
+    y = sg.mx4_dequantize(m, out=x)
+    assert torch.equal(y[some].double(), want) and y[1:65535:100].count_nonzero() == 0
+    del x, y, m
+    torch.cuda.empty_cache()
+
+
 def test_matmul_empty_and_refusals(dev):
     W = sg.mx4_quantize(rand(dev, 64, 256))
     assert sg.mx4_matmul(torch.zeros(0, 256, device=dev), W).shape == (0, 64)
