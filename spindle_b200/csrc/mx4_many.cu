@@ -41,6 +41,7 @@ struct Cfg {
     // TMEM: sums, in two buffers in turn where there is room beside the scales
     static constexpr uint32_t SC = 8 * ((DUAL ? 2 : 1) + XT), COLS = 512, ONE = NT * (DUAL ? 2 : 1), BUFS = 2 * ONE + STAGES * SC <= COLS ? 2 : 1;
     static constexpr uint32_t SUMS = ONE * BUFS;
+    static_assert(DUAL ? PIECES == 2 : PIECES == 3 || PIECES == 4, "what tmem_ld32x32 and so on are for");
     static_assert(SUMS + STAGES * SC <= COLS && SMEM <= 227 * 1024 && STAGE % 1024 == 0 && NT % (16 * GROUPS) == 0, "shapes");
 };
 
@@ -190,10 +191,9 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
             }
         }
     } else {
-        // lanes 32 q on; of the tile's pieces of 16 tokens every GROUPS-th from the g-th on
+        // lanes 32 q on; a quarter of the tile's pieces of 16 tokens
         const uint32_t q = warp & 3, g = (warp - FIRST_EPI) >> 2;
         uint8_t *buf = smem + C::OUT_AT + g * OUT_BYTES;
-        constexpr uint32_t APART = 16 * GROUPS;
         uint32_t count = 0, turn = 0;
         for (uint32_t i = me; i < tiles; i += pairs, count++) {
             const Tile t = tile_at(i);
@@ -210,13 +210,25 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
             }
             fence_after();
             float v[16 * C::PIECES * (DUAL ? 2 : 1)];  // the sums of the pieces, then those of `up`
-            const uint32_t at = tmem + b * C::ONE + ((32 * q) << 16) + 16 * g;
-#pragma unroll
-            for (uint32_t c = 0; c < C::PIECES; c++)
-                if (t.rows > APART * c + 16 * g) {
-                    tmem_ld32x16(at + APART * c, v + 16 * c);
-                    if (DUAL) tmem_ld32x16(at + C::NT + APART * c, v + 16 * (C::PIECES + c));
+            // of a full tile a group takes neighbouring pieces, of another every GROUPS-th
+            const bool full = t.rows == C::NT;
+            const uint32_t apart = full ? 16 : 16 * GROUPS, first = full ? 16 * C::PIECES * g : 16 * g;
+            const uint32_t at = tmem + b * C::ONE + ((32 * q) << 16) + first;
+            if (full) {
+                if constexpr (C::PIECES == 4) tmem_ld32x64(at, v);
+                else {
+                    tmem_ld32x32(at, v);
+                    if constexpr (C::PIECES == 3) tmem_ld32x16(at + 32, v + 32);
                 }
+                if (DUAL) tmem_ld32x32(at + C::NT, v + 32);
+            } else {
+#pragma unroll
+                for (uint32_t c = 0; c < C::PIECES; c++)
+                    if (t.rows > apart * c + first) {
+                        tmem_ld32x16(at + apart * c, v + 16 * c);
+                        if (DUAL) tmem_ld32x16(at + C::NT + apart * c, v + 16 * (C::PIECES + c));
+                    }
+            }
 #pragma unroll
             for (uint32_t c = 0; c < C::PIECES * (DUAL ? 2 : 1); c++) tmem_wait(v + 16 * c);
             fence_before();
@@ -228,8 +240,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
             const Out<T> o(a, t.row0, f0, q, lane);
 #pragma unroll
             for (uint32_t c = 0; c < C::PIECES; c++)
-                if (t.rows > APART * c + 16 * g) {
-                    const uint32_t from = APART * c + 16 * g;
+                if (t.rows > apart * c + first) {
+                    const uint32_t from = apart * c + first;
                     float *p = v + 16 * c;
                     if (DUAL) {
 #pragma unroll

@@ -98,6 +98,31 @@ __device__ __forceinline__ void tmem_ld32x16(uint32_t addr, float *v) {
                      : "r"(addr + ((16 * h) << 16))
                      : "memory");
 }
+// The same for 32 and for 64 columns, a piece of 16 of them after the other in v.  (Four pieces one by one take 450 ns a tile,
+// which the next tile's products wait for where there is one buffer of sums.)
+__device__ __forceinline__ void tmem_ld32x32(uint32_t addr, float *v) {
+#pragma unroll
+    for (uint32_t h = 0; h < 2; h++, v += 8)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+            : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+              "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23])
+            : "r"(addr + ((16 * h) << 16))
+            : "memory");
+}
+__device__ __forceinline__ void tmem_ld32x64(uint32_t addr, float *v) {
+#pragma unroll
+    for (uint32_t h = 0; h < 2; h++, v += 8)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+            "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+            : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+              "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+              "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]),
+              "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55])
+            : "r"(addr + ((16 * h) << 16))
+            : "memory");
+}
 __device__ __forceinline__ void tmem_wait(float *v) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]),
