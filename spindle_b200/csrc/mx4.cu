@@ -103,8 +103,9 @@ __device__ __forceinline__ uint2 quantize16(const Raw<T> &raw, uint32_t &scale) 
 }
 
 // A warp takes 1024 columns of a row, 512 at a time, all loads at once: a lane has sixteen values, two lanes a block of 32.
-// A token that goes to several experts is read and quantized once.  What bounds it: instructions (about 75 for a lane's
-// sixteen values) next to reading x.
+// A token that goes to several experts is read and quantized once.  What bounds it: instructions (80 for a lane's sixteen
+// values, the issue slots 63 % busy) next to reading x (8191 x 4096 bf16: 18.2 us, 5.7 TB/s read and written; with eight
+// values a lane 21.5).
 constexpr uint32_t QUANT_TILES = 4, STEPS = QUANT_TILES / 2;
 
 template <typename T, bool VEC>

@@ -8,6 +8,9 @@
 // issues the products; four warps write the results.  Where the tiles are fewer than the SMs, the
 // CTAs of a cluster take a part of the columns each and add their sums over distributed shared
 // memory, in rank order.
+// One row of 4096 to 14336 (31 MB of weights, 4.8 us): 10.3 us, 8.1 with its quantizing launch in a graph;
+// 33 rows of 14336 to 4096 (32 MB): 12.6, 10.4 in a graph: launches, the first copies' way and the last
+// sums; the copies between go at 5 to 6 TB/s.  Gate and up of 16 tokens' 8 of 128 experts (131 MB, 20 us): 27 us.
 #include <cooperative_groups.h>
 
 #include "mx4_tc.cuh"
