@@ -2608,7 +2608,8 @@ sg_status check_plan(const sg_moe_plan *p) {
     if (!p->n_used || p->n_used > MOE_SORT_MAX_USED || !p->n_expert || p->n_expert > MOE_SORT_MAX_EXPERTS) return SG_ERR_SHAPE;
     if (p->n_tok >= 1ull << 31 || p->n_tok * p->n_used >= 1ull << 31) return SG_ERR_SHAPE;
     if (!p->first || !p->work || (p->n_tok && (!p->ids || !p->weights || !p->order || !p->place))) return SG_ERR_INVALID;
-    return aligned(p->work, 16) ? SG_OK : SG_ERR_ALIGN;
+    const bool words = aligned(p->ids, 4) && aligned(p->weights, 4) && aligned(p->first, 4) && aligned(p->order, 4) && aligned(p->place, 4);
+    return words && aligned(p->work, 16) ? SG_OK : SG_ERR_ALIGN;
 }
 // Tokens whose experts a CTA chooses: a step's all, otherwise 16, one a warp, or as many more as make 512 CTAs.
 uint32_t sort_stretch(uint64_t n_tok) {

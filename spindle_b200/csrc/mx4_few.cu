@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_few_kernel(const __grid_consta
         }
     } else if (warp >= FIRST_EPI && me < tiles) {
         // the stages have been read: this part's sums take their place, [tokens][128 features], gate then up
-        ok = __all_sync(0xffffffffu, wait(&sh.sums_full[0], 0));
+        ok = wait(&sh.sums_full[0], 0);
         fence_after();
         const uint32_t q = warp & 3, n = tile_at(me).rows;
         float *mine = reinterpret_cast<float *>(smem + HDR) + 32 * q + (lane >> 2);

@@ -168,15 +168,15 @@ __device__ __forceinline__ bool try_wait_cluster(uint64_t *bar, uint32_t parity)
         : "memory");
     return ok != 0;
 }
-// Bounded: a wait that does not end is recorded, and everybody goes home.
+// By a whole warp, which goes on together.  Bounded: a wait that does not end is recorded, and everybody goes home.
 __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity) {
     for (int i = 0; i < 16; i++)
-        if (try_wait_cluster(bar, parity)) return true;
+        if (__all_sync(0xffffffffu, try_wait_cluster(bar, parity))) return true;
     const uint64_t t0 = globaltimer_ns();
     for (;;) {
         for (int i = 0; i < 64; i++)
-            if (try_wait_cluster(bar, parity)) return true;
-        if (globaltimer_ns() - t0 > WAIT_LIMIT_NS) return false;
+            if (__all_sync(0xffffffffu, try_wait_cluster(bar, parity))) return true;
+        if (__any_sync(0xffffffffu, globaltimer_ns() - t0 > WAIT_LIMIT_NS)) return false;
     }
 }
 // Of each expert: how many tiles end with it and its first sorted place (a lookup from global memory took

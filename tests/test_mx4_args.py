@@ -80,6 +80,7 @@ def test_sort_refusals():
     assert route(p=plan(n_tok=1 << 30, n_used=2)) == SHAPE
     assert route(t=8) == DTYPE and route(x=None) == INVALID and route(ld=7) == INVALID and route(x=AT + 2) == ALIGN
     for k in ("ids", "weights", "first", "order", "place", "work"):
+        assert route(p=plan(**{k: AT + 2})) == ALIGN and L.sg_moe_sort(C.byref(plan(**{k: AT + 2})), None) == ALIGN
         assert route(p=plan(**{k: None})) == INVALID and L.sg_moe_sort(C.byref(plan(**{k: None})), None) == INVALID
     assert L.sg_moe_plan_work_bytes(10, 0) == 0 and L.sg_moe_plan_work_bytes(10, 1025) == 0 and L.sg_moe_plan_work_bytes(10, 8) == 4 * 36
     comb = lambda p=plan(), t=0, y=AT, ldy=64, dim=64, ot=0, o=AT, ldo=64: L.sg_moe_combine(C.byref(p), t, y, ldy, dim, ot, o, ldo, None)  # noqa: E731
