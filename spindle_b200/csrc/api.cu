@@ -2689,7 +2689,7 @@ sg_status mx4_product(const sg_mx4 *w, const sg_mx4 *up, const sg_moe_plan *plan
         g.n_expert = (uint32_t)plan->n_expert;
     }
     CK(mx4_quantize_launch(q, type, di->sms, s));
-    g.vec = rows16(d_out, ldo, eo);
+    g.vec = rows16(d_out, pairs > 1 ? ldo : 0, eo), g.pairs = eo == 2 && aligned(d_out, 4) && !(ldo & 1);
     CK(mp.many ? mx4_many_launch(g, mp.x_rows, mp.tiles, di->sms, s) : mx4_few_launch(g, mp.x_rows, mp.tiles, di->sms, s));
     return SG_OK;
 }

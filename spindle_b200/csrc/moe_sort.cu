@@ -291,55 +291,74 @@ __global__ void __launch_bounds__(THREADS) moe_place_kernel(const __grid_constan
     place_pairs(a, m, (uint32_t)min(t0, n), (uint32_t)min(t0 + MOE_SORT_JOIN * a.stretch, n), blockIdx.x == 0);
 }
 
-// out[t] = sum over j of weights[t, j] y[place[t, j]], in the order of j, in f32.  A thread has eight columns of a token and
-// its loads of up to eight experts' rows in flight.  What bounds it: reading y (8191 x 8 rows of 2048 bf16: 50 us, 6.0 TB/s).
-template <typename T, typename O, bool VEC>
+// out[t] = sum over j of weights[t, j] y[place[t, j]], in the order of j, in f32.  A thread takes eight columns of a token, an
+// item, with its loads of J experts' rows in flight.  With one slot or two, two items at a time (52592 rows of 1192 bf16, a row a
+// token: eight slots, one item 125 us; one slot, one item 64, two 54, four 66; with four slots two are slower, 30.1 against 29.1).
+// What bounds it: reading y (8191 x 8 rows of 2048 bf16: 50 us, 6.0 TB/s; x 4: 29 us, 5.8 TB/s).
+constexpr int combine_items(bool vec, int slots) { return vec && slots <= 2 ? 2 : 1; }
+
+template <typename T, typename O, bool VEC, int J>
 __global__ void __launch_bounds__(256) moe_combine_kernel(const __grid_constant__ MoeCombineArgs a) {
+    constexpr int ITEMS = combine_items(VEC, J), N = 16 / sizeof(T);
     const uint32_t per = (a.dim + 7) / 8;
-    const uint64_t items = a.n_tok * per, step = (uint64_t)gridDim.x * 256;
-    for (uint64_t it = (uint64_t)blockIdx.x * 256 + threadIdx.x; it < items; it += step) {
-        const uint64_t t = it / per;
-        const uint32_t col = (uint32_t)(it - t * per) * 8, n = min(8u, a.dim - col);
-        float sum[8] = {};
-        for (uint32_t j0 = 0; j0 < a.n_used; j0 += 8) {
-            constexpr int N = 16 / sizeof(T);
-            uint4 v[8][8 / N];
-            float w[8];
+    const uint64_t items = a.n_tok * per, step = (uint64_t)gridDim.x * (256 * ITEMS);
+    for (uint64_t first = (uint64_t)blockIdx.x * (256 * ITEMS) + threadIdx.x; first < items; first += step) {
+        uint64_t t[ITEMS];
+        uint32_t col[ITEMS], n[ITEMS];
 #pragma unroll
-            for (uint32_t j = 0; j < 8; j++) {
-                w[j] = 0.0f;
-                int32_t p = -1;
-                if (j0 + j < a.n_used) p = __ldg(a.place + t * a.n_used + j0 + j);
-                const bool there = p >= 0 && (uint32_t)p < a.n_places;
-                if (there) w[j] = __ldg(a.weights + t * a.n_used + j0 + j);
-                const T *y = static_cast<const T *>(a.y) + (uint64_t)(there ? p : 0) * a.ldy + col;
-                if constexpr (VEC) {
-#pragma unroll
-                    for (int i = 0; i < 8 / N; i++) v[j][i] = there ? __ldg(reinterpret_cast<const uint4 *>(y) + i) : make_uint4(0, 0, 0, 0);
-                } else {
-                    T *to = reinterpret_cast<T *>(v[j]);
-#pragma unroll
-                    for (uint32_t i = 0; i < 8; i++) to[i] = there && i < n ? y[i] : narrow<T>(0.0f);
-                }
-            }
-#pragma unroll
-            for (uint32_t j = 0; j < 8; j++) {
-                const T *y = reinterpret_cast<const T *>(v[j]);
-#pragma unroll
-                for (int i = 0; i < 8; i++) sum[i] = fmaf(w[j], widen(y[i]), sum[i]);
-            }
+        for (int i = 0; i < ITEMS; i++) {
+            const uint64_t it = first + i * 256;
+            t[i] = it / per;
+            col[i] = (uint32_t)(it - t[i] * per) * 8;
+            n[i] = it < items ? min(8u, a.dim - col[i]) : 0;
         }
-        O *o = static_cast<O *>(a.out) + t * a.ldo + col;
-        if constexpr (VEC) {
-            O r[8];
+        float sum[ITEMS][8] = {};
+        for (uint32_t j0 = 0; j0 < a.n_used; j0 += J) {
+            uint4 v[ITEMS][J][8 / N];
+            float w[ITEMS][J];
 #pragma unroll
-            for (int i = 0; i < 8; i++) r[i] = narrow<O>(sum[i]);
+            for (int i = 0; i < ITEMS; i++)
 #pragma unroll
-            for (uint32_t i = 0; i < 8 * sizeof(O) / 16; i++) reinterpret_cast<uint4 *>(o)[i] = reinterpret_cast<const uint4 *>(r)[i];
-        } else {
+                for (uint32_t j = 0; j < J; j++) {
+                    w[i][j] = 0.0f;
+                    int32_t p = -1;
+                    if (n[i] && j0 + j < a.n_used) p = __ldg(a.place + t[i] * a.n_used + j0 + j);
+                    const bool there = p >= 0 && (uint32_t)p < a.n_places;
+                    if (there) w[i][j] = __ldg(a.weights + t[i] * a.n_used + j0 + j);
+                    const T *y = static_cast<const T *>(a.y) + (uint64_t)(there ? p : 0) * a.ldy + col[i];
+                    if constexpr (VEC) {
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i++)
-                if (i < n) o[i] = narrow<O>(sum[i]);
+                        for (int c = 0; c < 8 / N; c++) v[i][j][c] = there ? __ldg(reinterpret_cast<const uint4 *>(y) + c) : make_uint4(0, 0, 0, 0);
+                    } else {
+                        T *to = reinterpret_cast<T *>(v[i][j]);
+#pragma unroll
+                        for (uint32_t c = 0; c < 8; c++) to[c] = there && c < n[i] ? y[c] : narrow<T>(0.0f);
+                    }
+                }
+#pragma unroll
+            for (int i = 0; i < ITEMS; i++)
+#pragma unroll
+                for (uint32_t j = 0; j < J; j++) {
+                    const T *y = reinterpret_cast<const T *>(v[i][j]);
+#pragma unroll
+                    for (int c = 0; c < 8; c++) sum[i][c] = fmaf(w[i][j], widen(y[c]), sum[i][c]);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+            if (!n[i]) break;
+            O *o = static_cast<O *>(a.out) + t[i] * a.ldo + col[i];
+            if constexpr (VEC) {
+                O r[8];
+#pragma unroll
+                for (int c = 0; c < 8; c++) r[c] = narrow<O>(sum[i][c]);
+#pragma unroll
+                for (uint32_t c = 0; c < 8 * sizeof(O) / 16; c++) reinterpret_cast<uint4 *>(o)[c] = reinterpret_cast<const uint4 *>(r)[c];
+            } else {
+#pragma unroll
+                for (uint32_t c = 0; c < 8; c++)
+                    if (c < n[i]) o[c] = narrow<O>(sum[i][c]);
+            }
         }
     }
 }
@@ -377,13 +396,24 @@ cudaError_t choose_of(const MoeSortArgs &a, uint32_t smem, cudaStream_t s) {
     return a.n_expert <= 128 ? choose_as<T, 4>(a, smem, s) : a.n_expert <= 256 ? choose_as<T, 8>(a, smem, s) : choose_as<T, 32>(a, smem, s);
 }
 
+template <typename T, typename O, bool VEC, int J>
+cudaError_t combine_slots(const MoeCombineArgs &a, int sms, cudaStream_t s) {
+    constexpr int PER = 256 * combine_items(VEC, J);
+    const uint64_t want = (a.n_tok * ((a.dim + 7) / 8) + PER - 1) / PER;
+    const uint32_t grid = (uint32_t)(want < (uint64_t)sms * 32 ? want : (uint64_t)sms * 32);
+    moe_combine_kernel<T, O, VEC, J><<<grid, 256, 0, s>>>(a);
+    return cudaGetLastError();
+}
+template <typename T, typename O, bool VEC>
+cudaError_t combine_vec(const MoeCombineArgs &a, int sms, cudaStream_t s) {
+    return a.n_used == 1   ? combine_slots<T, O, VEC, 1>(a, sms, s)
+           : a.n_used == 2 ? combine_slots<T, O, VEC, 2>(a, sms, s)
+           : a.n_used <= 4 ? combine_slots<T, O, VEC, 4>(a, sms, s)
+                           : combine_slots<T, O, VEC, 8>(a, sms, s);
+}
 template <typename T, typename O>
 cudaError_t combine_as(const MoeCombineArgs &a, int sms, cudaStream_t s) {
-    const uint64_t want = (a.n_tok * ((a.dim + 7) / 8) + 255) / 256;
-    const uint32_t grid = (uint32_t)(want < (uint64_t)sms * 32 ? want : (uint64_t)sms * 32);
-    if (a.vec) moe_combine_kernel<T, O, true><<<grid, 256, 0, s>>>(a);
-    else moe_combine_kernel<T, O, false><<<grid, 256, 0, s>>>(a);
-    return cudaGetLastError();
+    return a.vec ? combine_vec<T, O, true>(a, sms, s) : combine_vec<T, O, false>(a, sms, s);
 }
 template <typename T>
 cudaError_t combine_from(const MoeCombineArgs &a, int32_t o, int sms, cudaStream_t s) {

@@ -80,7 +80,7 @@ struct Mx4GemmArgs {
     uint64_t n_tok;                // rows of x, where they are one matrix
     const int32_t *first;          // experts: the first sorted place of each (n_expert + 1)
     uint32_t n_expert;
-    bool vec;                      // out allows 16-byte stores of eight features
+    bool vec, pairs;               // out's rows allow 16-byte stores; 16-bit rows that allow 4-byte ones
 };
 cudaError_t mx4_many_launch(const Mx4GemmArgs &a, uint32_t x_rows, uint64_t token_tiles, int sms, cudaStream_t s);
 cudaError_t mx4_few_launch(const Mx4GemmArgs &a, uint32_t x_rows, uint64_t token_tiles, int sms, cudaStream_t s);

@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_few_kernel(const __grid_consta
             fence_after();
             const uint32_t at = tmem + b * NT * (DUAL ? 2 : 1) + ((32 * q) << 16), f0 = i % a.feat_tiles * MX4_ROWS;
             auto put = [&](auto type) {
-                const Out<decltype(type)> o(a, t.row0, f0, q, lane);
+                const Out<decltype(type), 2> o(a, t.row0, f0, q, lane);
                 for (uint32_t c = 0; c < t.rows; c += 16) {
                     float v[16], u[16];
                     tmem_ld32x16(at + c, v);

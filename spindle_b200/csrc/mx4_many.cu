@@ -68,7 +68,7 @@ __device__ __forceinline__ void arrive_at(uint64_t *bar, uint32_t rank) {
         : "memory");
 }
 
-template <typename C, typename T>
+template <typename C, typename T, bool VEC>
 __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_constant__ Mx4GemmArgs a) {
     constexpr bool DUAL = C::DUAL;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
             __syncwarp();
             const uint32_t f0 = (2 * pair_of(i) + rank) * MX4_ROWS;
             if (f0 >= a.feats) continue;
-            const Out<T> o(a, t.row0, f0, q, lane);
+            const Out<T, VEC> o(a, t.row0, f0, q, lane);
 #pragma unroll
             for (uint32_t c = 0; c < C::PIECES; c++)
                 if (t.rows > apart * c + first) {
@@ -269,9 +269,9 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_many_kernel(const __grid_const
     }
 }
 
-template <typename C, typename T>
+template <typename C, typename T, bool VEC>
 cudaError_t launch_as(const Mx4GemmArgs &a, uint64_t tiles, int sms, cudaStream_t s) {
-    auto fn = mx4_many_kernel<C, T>;
+    auto fn = mx4_many_kernel<C, T, VEC>;
     static bool ready[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -296,9 +296,13 @@ cudaError_t launch_as(const Mx4GemmArgs &a, uint64_t tiles, int sms, cudaStream_
     return cudaLaunchKernelEx(&c, fn, a);
 }
 
+template <typename C, typename T>
+cudaError_t launch_vec(const Mx4GemmArgs &a, uint64_t tiles, int sms, cudaStream_t s) {
+    return a.vec ? launch_as<C, T, true>(a, tiles, sms, s) : launch_as<C, T, false>(a, tiles, sms, s);
+}
 template <typename C>
 cudaError_t launch_type(const Mx4GemmArgs &a, uint64_t tiles, int sms, cudaStream_t s) {
-    return a.type == SG_F32 ? launch_as<C, float>(a, tiles, sms, s) : a.type == SG_F16 ? launch_as<C, __half>(a, tiles, sms, s) : launch_as<C, __nv_bfloat16>(a, tiles, sms, s);
+    return a.type == SG_F32 ? launch_vec<C, float>(a, tiles, sms, s) : a.type == SG_F16 ? launch_vec<C, __half>(a, tiles, sms, s) : launch_vec<C, __nv_bfloat16>(a, tiles, sms, s);
 }
 
 }  // namespace

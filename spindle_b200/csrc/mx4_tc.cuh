@@ -254,19 +254,22 @@ __device__ __forceinline__ uint32_t pack(__nv_bfloat16, float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// Where a thread's part of a tile's results goes, of a token 128 features from f0 on: 16 bytes of every eighth token (of f32:
-// fourth), from row `row` of the output on.
-template <typename T>
+// Where a thread's part of a tile's results goes, of a token 128 features from f0 on, from row `row` of the output on: 16
+// bytes of every eighth token (of f32: fourth); where the rows do not allow such stores, whatever their size, the warp's
+// lanes beside one another in every fourth token, words of 4 bytes or, for 16-bit rows that begin between words, values.
+// (1586 rows of 8320 columns to 6971 in bf16: eight stores of a value a lane, lanes 16 bytes apart 81 us, so 49.)
+// VEC: known to be so (1), not to be so (0), or found out (2).
+template <typename T, int VEC>
 struct Out {
     static constexpr uint32_t ROW = MX4_ROWS * sizeof(T) + 16, PER = MX4_ROWS * sizeof(T) / 16, ES = 16 / sizeof(T), STEP = 128 / PER;
     T *at;
-    uint32_t left;  // features from there on; at least ES: 16-byte stores
-    static __device__ __forceinline__ uint32_t token(uint32_t warp, uint32_t lane) { return (32 * warp + lane) / PER; }
-    static __device__ __forceinline__ uint32_t chunk(uint32_t warp, uint32_t lane) { return (32 * warp + lane) % PER; }
+    uint32_t left;  // features from there on
+    static __device__ __forceinline__ bool vec(const Mx4GemmArgs &a) { return VEC == 2 ? a.vec : VEC == 1; }
+    static __device__ __forceinline__ uint32_t token(const Mx4GemmArgs &a, uint32_t warp, uint32_t lane) { return vec(a) ? (32 * warp + lane) / PER : warp; }
     __device__ __forceinline__ Out(const Mx4GemmArgs &a, uint64_t row, uint32_t f0, uint32_t warp, uint32_t lane) {
-        const uint32_t f = f0 + chunk(warp, lane) * ES;
-        at = static_cast<T *>(a.out) + (row + token(warp, lane)) * a.ldo + f;
-        left = f < a.feats ? a.feats - f : 0;
+        const uint32_t f = vec(a) ? (32 * warp + lane) % PER * ES : lane * (a.pairs ? 2 : 1);
+        at = static_cast<T *>(a.out) + (row + token(a, warp, lane)) * a.ldo + f0 + f;
+        left = f0 + f < a.feats ? a.feats - f0 - f : 0;
     }
 };
 
@@ -274,10 +277,10 @@ struct Out {
 // v as tmem_ld32x16 gives them, to the output by way of shared memory, where the four warps' features of a token come
 // together.  16-bit results go there eight by eight, turned over on the way (stmatrix), to one of two places in turn, so that
 // one barrier a piece will do.
-template <typename T>
-__device__ __forceinline__ void put_piece(const Mx4GemmArgs &a, const Out<T> &o, uint8_t *buf, const float *v, uint32_t from, uint32_t n, uint32_t warp,
+template <typename T, int VEC>
+__device__ __forceinline__ void put_piece(const Mx4GemmArgs &a, const Out<T, VEC> &o, uint8_t *buf, const float *v, uint32_t from, uint32_t n, uint32_t warp,
                                           uint32_t lane, uint32_t group) {
-    using O = Out<T>;
+    using O = Out<T, VEC>;
     if constexpr (sizeof(T) == 2) {
         const uint32_t at = smem_u32(buf) + (lane & 7) * O::ROW + (32 * warp + 8 * (lane >> 3)) * 2;
 #pragma unroll
@@ -297,20 +300,42 @@ __device__ __forceinline__ void put_piece(const Mx4GemmArgs &a, const Out<T> &o,
                 at[(8 * b + (i & 1)) * (O::ROW / 4) + 8 * (i >> 1)] = v[(i >> 2) * 8 + 4 * b + (i & 3)];
     }
     asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
-    const uint32_t token = O::token(warp, lane);
-    const uint8_t *mine = buf + token * O::ROW + 16 * O::chunk(warp, lane);
+    const uint32_t token = O::token(a, warp, lane);
     T *to = o.at + from * a.ldo;
-    const bool whole = a.vec && o.left >= O::ES;
+    if (O::vec(a)) {
+        const uint8_t *mine = buf + token * O::ROW + (32 * warp + lane) % O::PER * 16;
 #pragma unroll
-    for (uint32_t t = 0; t < 16; t += O::STEP, to += O::STEP * a.ldo) {
-        if (token + t >= n) break;
-        const uint4 w = *reinterpret_cast<const uint4 *>(mine + t * O::ROW);
-        if (whole) *reinterpret_cast<uint4 *>(to) = w;
-        else {
-            const T *e = reinterpret_cast<const T *>(&w);
+        for (uint32_t t = 0; t < 16; t += O::STEP, to += O::STEP * a.ldo) {
+            if (token + t >= n) break;
+            const uint4 w = *reinterpret_cast<const uint4 *>(mine + t * O::ROW);
+            if (o.left >= O::ES) *reinterpret_cast<uint4 *>(to) = w;
+            else {
+                const T *e = reinterpret_cast<const T *>(&w);
 #pragma unroll
-            for (uint32_t j = 0; j < O::ES; j++)
-                if (j < o.left) to[j] = e[j];
+                for (uint32_t j = 0; j < O::ES; j++)
+                    if (j < o.left) to[j] = e[j];
+            }
+        }
+    } else if (sizeof(T) == 2 && a.pairs) {
+        const uint8_t *mine = buf + token * O::ROW + 4 * lane;
+#pragma unroll
+        for (uint32_t t = 0; t < 16; t += 4, to += 4 * a.ldo) {
+            if (token + t >= n) break;
+#pragma unroll
+            for (uint32_t j = 0; j < 2; j++) {
+                const uint32_t w = *reinterpret_cast<const uint32_t *>(mine + t * O::ROW + 128 * j);
+                if (o.left > 64 * j + 1) *reinterpret_cast<uint32_t *>(to + 64 * j) = w;
+                else if (o.left > 64 * j) to[64 * j] = reinterpret_cast<const T *>(&w)[0];
+            }
+        }
+    } else {
+        const T *mine = reinterpret_cast<const T *>(buf + token * O::ROW) + lane;
+#pragma unroll
+        for (uint32_t t = 0; t < 16; t += 4, to += 4 * a.ldo) {
+            if (token + t >= n) break;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++)
+                if (o.left > 32 * j) to[32 * j] = mine[t * (O::ROW / sizeof(T)) + 32 * j];
         }
     }
 }

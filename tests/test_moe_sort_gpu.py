@@ -192,6 +192,25 @@ def test_combine(dev, dim, k):
                 assert (out[:, 0] == 7).all() and (out[:, -1] == 7).all() and (out[4, 1:-1] == 0).all()
 
 
+@pytest.mark.parametrize("n,dim", [(1, 8), (3, 1000), (701, 1192)])
+@pytest.mark.parametrize("k", [1, 2, 4, 5, 8, 16])
+def test_combine_whole_rows(dev, n, dim, k):
+    # rows of 16-byte words, several of them a thread where a token has few
+    ids = torch.randint(-1, 20, (n, k), dtype=torch.int32, device=dev, generator=torch.Generator(device=dev).manual_seed(k))
+    p = sg.moe_sort(ids, rand(dev, n, k, seed=5), sg.MoePlan(n, k, 20, device=dev))
+    base = rand(dev, n * k, dim, seed=6)
+    base[int(p.first[-1]):] = float("nan")
+    place = p.place.long()
+    for dtype in TYPES:
+        y = base.to(dtype)
+        z = torch.where(place[..., None] < 0, 0.0, y[place.clamp(min=0)].double() * p.weights[..., None].double())
+        for ot in TYPES:
+            out = torch.full((n + 1, dim + 8), 7.0, dtype=ot, device=dev)
+            sg.moe_combine(y, p, out=out[:-1, :dim])
+            assert U.close(out[:-1, :dim], z.sum(1), z.abs().sum(1) * (k * 2.0 ** -24))
+            assert (out[-1] == 7).all() and (out[:, dim:] == 7).all()
+
+
 def test_captured_layer(dev):
     # route, experts and back in one graph, replayed with other tokens
     n, e, k, dim, ff = 24, 16, 4, 256, 128

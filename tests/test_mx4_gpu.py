@@ -118,6 +118,22 @@ def test_matmul_strides(dev, rows):
     sg.device_status()
 
 
+@pytest.mark.parametrize("rows", [2, 200, 600])
+@pytest.mark.parametrize("n", [1, 127, 258, 301])
+def test_matmul_rows_of_results(dev, rows, n):
+    # rows of results that begin on 16 bytes, on 4, on 2, and alternate
+    x, w = rand(dev, rows, 320, seed=rows), rand(dev, n, 320, seed=n) * 0.05
+    W = sg.mx4_quantize(w)
+    want, bound = U.product(U.quantized(x), U.quantized(w))
+    for dtype in TYPES:
+        for off, ld in ((0, 320), (2, 320), (0, 314), (1, 320), (1, 313), (3, 314)):
+            out = torch.full((rows + 1, ld), 7.0, dtype=dtype, device=dev)
+            assert U.close(sg.mx4_matmul(x, W, out=out[:-1, off:off + n]), want, bound)
+            out[:-1, off:off + n] = 7.0
+            assert (out == 7).all()
+    sg.device_status()
+
+
 @pytest.mark.parametrize("rows", [1, 4, 16, 40, 300])
 def test_matmul_nonfinite_rows_stay_apart(dev, rows):
     x, w = rand(dev, rows, 512, seed=5), rand(dev, 200, 512, seed=6)
