@@ -13,6 +13,7 @@ OK = 0
 STATUS = {0: "ok", 1: "invalid argument", 2: "unsupported dtype", 3: "unsupported shape",
           4: "misaligned device pointer", 5: "CUDA error", 6: "NCCL error", 7: "device wait timed out",
           8: "out of memory", 9: "request above the static scratch limit"}
+ERR_CUDA = 5
 
 
 class SgError(RuntimeError):
@@ -210,6 +211,6 @@ def load(build_if_missing=True):
 def check(status, what):
     if status != OK:
         detail = ""
-        if status == 5 and _lib is not None:
+        if status == ERR_CUDA and _lib is not None:
             detail = _lib.sg_last_error_string().decode(errors="replace")
         raise SgError(status, what, detail)

@@ -175,8 +175,6 @@ def _plan(plan, n, t):
         raise ValueError("the plan is made for %d tokens" % plan.max_tokens)
     if plan.dev != _dev(t, "the tokens' tensor"):
         raise ValueError("the plan must lie on the same CUDA device")
-    if plan.n_tok != n:
-        plan._tokens(n)
 
 
 def moe_route(logits, plan, norm=True, prune=0.0, stream=None):
@@ -187,10 +185,17 @@ def moe_route(logits, plan, norm=True, prune=0.0, stream=None):
     shape, stride = logits.shape, logits.stride()
     if len(shape) != 2 or shape[1] != plan.n_expert or (stride[1] != 1 and shape[1] > 1):
         raise ValueError("logits must be a tensor [n, %d] with contiguous rows" % plan.n_expert)
-    kind = _type(logits, "logits")
-    _plan(plan, shape[0], logits)
-    st = _lib.load().sg_moe_route(kind, logits.data_ptr(), stride[0], int(bool(norm)), prune, plan._c, _s(stream, logits))
+    kind, n, was = _type(logits, "logits"), shape[0], plan.n_tok
+    _plan(plan, n, logits)
+    args = kind, logits.data_ptr(), stride[0], int(bool(norm)), float(prune), plan._c, _s(stream, logits)
+    if was != n:
+        plan._tokens(n)
+    st = _lib.load().sg_moe_route(*args)
     if st:
+        # the arrays on the device and the number of tokens belong together (the products take tiles and rows from the ones, the
+        # sizes of what they read and write from the other): of a call that is refused they stay as they are, one that fails on
+        # the way leaves no tokens
+        plan._tokens(0 if st == _lib.ERR_CUDA else was)
         _lib.check(st, "moe_route")
     return plan
 
@@ -203,12 +208,20 @@ def moe_sort(ids, weights, plan, stream=None):
         raise ValueError("ids and weights must be int32 and float32 tensors [n, %d] of one CUDA device" % plan.n_used)
     _plan(plan, n, ids)
     _i32(ids, "ids", plan.dev)
-    with _on(stream):
-        if n and ids.data_ptr() != plan.ids.data_ptr():
-            plan.ids.copy_(ids)
-        if n and weights.data_ptr() != plan.weights.data_ptr():
-            plan.weights.copy_(weights)
-    st = _lib.load().sg_moe_sort(plan._c, _s(stream, ids))
+    handle = _s(stream, ids)
+    if plan.n_tok != n:
+        plan._tokens(n)
+    st = _lib.ERR_CUDA
+    try:
+        with _on(stream):
+            if n and ids.data_ptr() != plan.ids.data_ptr():
+                plan.ids.copy_(ids)
+            if n and weights.data_ptr() != plan.weights.data_ptr():
+                plan.weights.copy_(weights)
+        st = _lib.load().sg_moe_sort(plan._c, handle)
+    finally:
+        if st:  # (the ids have been written, or some of them)
+            plan._tokens(0)
     if st:
         _lib.check(st, "moe_sort")
     return plan

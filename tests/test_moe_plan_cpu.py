@@ -1,0 +1,112 @@
+"""What a plan of tokens sorted by expert holds after calls that are refused: on the CPU, the
+library's answers given by the test (nothing is launched)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from spindle_b200 import _lib, mx4
+
+INVALID, ALIGN, CUDA = 1, 4, 5
+
+
+class HostPlan(mx4.MoePlan):
+    """A plan in host memory."""
+
+    def __init__(self, max_tokens, n_used, n_expert):
+        self.max_tokens, self.n_used, self.n_expert, self.dev = max_tokens, n_used, n_expert, -1
+        n = max_tokens * n_used
+        self._ids, self._order, self._place = (torch.arange(n, dtype=torch.int32) for _ in range(3))
+        self._weights = torch.zeros(n)
+        self.desc = _lib.SgMoePlan(0, n_used, n_expert, *[t.data_ptr() for t in (self._ids, self._weights, self._ids, self._order, self._place)], None)
+        self._c = C.byref(self.desc)
+        self._tokens(0)
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    """The library in the place of which every call has the status that the test sets, and the tokens that the calls were
+    made for."""
+    class Lib:
+        status, tokens = 0, []
+
+        def sg_moe_route(self, *a):
+            Lib.tokens.append(plan_of(a[5]))
+            return Lib.status
+
+        def sg_moe_sort(self, *a):
+            Lib.tokens.append(plan_of(a[0]))
+            return Lib.status
+
+    def plan_of(ref):
+        return ref._obj.n_tok
+    Lib.tokens = []
+    monkeypatch.setattr(mx4._lib, "load", Lib)
+    monkeypatch.setattr(mx4, "_dev", lambda t, what: -1)
+    monkeypatch.setattr(mx4, "_s", lambda stream, t: stream and stream.cuda_stream)
+    return Lib
+
+
+def state(p):
+    return p.n_tok, p.desc.n_tok, p.ids.tolist(), p.order.tolist(), p.place.tolist(), p.weights.tolist()
+
+
+def filled(lib, n=6, most=10):
+    lib.status = 0
+    p = HostPlan(most, 2, 8)
+    mx4.moe_sort(torch.full((n, 2), 3, dtype=torch.int32), torch.ones(n, 2), p)
+    assert state(p)[:2] == (n, n) and p.ids.shape == (n, 2)
+    return p
+
+
+@pytest.mark.parametrize("n", [3, 9])
+def test_a_refused_sort_leaves_the_plan(lib, n):
+    ids, w = torch.zeros(n, 2, dtype=torch.int32), torch.zeros(n, 2)
+    wrong = [(TypeError, (ids.long(), w)), (TypeError, (torch.zeros(2, n, dtype=torch.int32).T, w)), (ValueError, (ids, w.double())),
+             (ValueError, (ids, w[:, :1])), (ValueError, (torch.zeros(11, 2, dtype=torch.int32), torch.zeros(11, 2)))]
+    for error, args in wrong:
+        p = filled(lib)
+        before, calls = state(p), len(lib.tokens)
+        with pytest.raises(error):
+            mx4.moe_sort(*args, p)
+        assert state(p) == before and len(lib.tokens) == calls
+
+
+@pytest.mark.parametrize("n", [3, 9])
+def test_a_refused_route_leaves_the_plan(lib, n):
+    p = filled(lib)
+    before = state(p)
+    for x in (torch.zeros(n, 7), torch.zeros(8, n).T, torch.zeros(11, 8)):
+        with pytest.raises(ValueError):
+            mx4.moe_route(x, p)
+        assert state(p) == before
+    with pytest.raises(TypeError):
+        mx4.moe_route(torch.zeros(n, 8, dtype=torch.float64), p)
+    with pytest.raises(ValueError):
+        mx4.moe_route(torch.zeros(n, 8), p, prune="none")
+    with pytest.raises(AttributeError):
+        mx4.moe_sort(torch.zeros(n, 2, dtype=torch.int32), torch.zeros(n, 2), p, stream="none")
+    assert state(p) == before
+    for status in (INVALID, ALIGN):  # refused by the library: rows one over the other, or between words
+        lib.status = status
+        with pytest.raises(_lib.SgError):
+            mx4.moe_route(torch.zeros(1, 8).expand(n, 8), p)
+        assert lib.tokens[-1] == n and state(p) == before
+
+
+@pytest.mark.parametrize("n", [3, 9])
+def test_a_call_that_failed_leaves_an_empty_plan(lib, n):
+    # a launch that failed may have written some of the plan's arrays: it holds no tokens then
+    for call in (lambda p: mx4.moe_route(torch.zeros(n, 8), p), lambda p: mx4.moe_sort(torch.zeros(n, 2, dtype=torch.int32), torch.zeros(n, 2), p)):
+        p = filled(lib)
+        lib.status = CUDA
+        with pytest.raises(_lib.SgError):
+            call(p)
+        assert lib.tokens[-1] == n and p.n_tok == p.desc.n_tok == 0 and p.ids.shape == (0, 2)
+
+
+def test_calls_set_the_tokens(lib):
+    p = filled(lib)
+    for n in (9, 0, 3):
+        assert mx4.moe_route(torch.zeros(n, 8), p) is p and state(p)[:2] == (n, n) and lib.tokens[-1] == n and p.order.shape == (2 * n,)
+        assert mx4.moe_sort(torch.zeros(n, 2, dtype=torch.int32), torch.zeros(n, 2), p) is p and lib.tokens[-1] == n

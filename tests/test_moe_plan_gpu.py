@@ -1,0 +1,33 @@
+"""Plans of tokens sorted by expert on the GPU: what they hold after refused calls, and their use
+for steps of other sizes."""
+import pytest
+import torch
+
+import spindle_b200 as sg
+
+pytestmark = pytest.mark.gpu
+
+
+def rand(dev, *shape, seed=0):
+    return torch.randn(*shape, device=dev, generator=torch.Generator(device=dev).manual_seed(seed))
+
+
+@pytest.mark.parametrize("n,other", [(300, 5), (5, 300), (70, 69)])
+def test_refused_calls_leave_the_plan(dev, n, other):
+    e, k = 12, 3
+    x, w = rand(dev, n, 64, seed=1), sg.mx4_quantize(rand(dev, e, 40, 64, seed=2))
+    p = sg.moe_route(rand(dev, n, e, seed=3), sg.MoePlan(400, k, e, device=dev))
+    held = [t.clone() for t in (p.ids, p.weights, p.first, p.order, p.place)]
+    want = sg.moe_combine(sg.mx4_experts(x, w, p, gather=True), p)
+    ids, logits = torch.zeros(other, k, dtype=torch.int32, device=dev), rand(dev, other + 1, e + 1, seed=4)
+    for call in (lambda: sg.moe_sort(ids.long(), ids.float(), p), lambda: sg.moe_sort(ids.T.contiguous().T, ids.float(), p),
+                 lambda: sg.moe_sort(ids, ids.double(), p), lambda: sg.moe_route(logits[:other], p), lambda: sg.moe_route(logits[:other, :e].double(), p),
+                 lambda: sg.moe_route(logits[:1, :e].expand(other, e), p),                       # rows one over the other
+                 lambda: sg.moe_route(torch.zeros(401, e, device=dev), p), lambda: sg.moe_route(logits[:other, :e], p, prune="none")):
+        with pytest.raises((TypeError, ValueError, sg.SgError)):
+            call()
+        assert p.n_tok == n and p.ids.shape == (n, k) and p.order.shape == (n * k,)
+        for t, was in zip((p.ids, p.weights, p.first, p.order, p.place), held):
+            assert torch.equal(t, was)
+        assert torch.equal(sg.moe_combine(sg.mx4_experts(x, w, p, gather=True), p), want)
+    sg.device_status()
