@@ -95,17 +95,24 @@ def mx4_dequantize(m, out=None, dtype=torch.float32, stream=None):
     return out
 
 
+def _scratch_bytes(w, rows, desc):
+    return _lib.load().sg_mx4_scratch_bytes(w._c, rows, desc)
+
+
 def mx4_scratch(w, rows, stream=None):
-    """Scratch of mx4_matmul for that many rows, or of mx4_experts (rows: its MoePlan):
-    kept by the caller, one for calls that may overlap on the GPU."""
-    L = _lib.load()
-    n = L.sg_mx4_scratch_bytes(w._c, 0, rows._c) if isinstance(rows, MoePlan) else L.sg_mx4_scratch_bytes(w._c, rows, None)
+    """Scratch of mx4_matmul for up to that many rows, or of mx4_experts for a MoePlan
+    (rows), whatever it holds, up to its max_tokens: kept by the caller, one for calls
+    that may overlap on the GPU."""
+    if isinstance(rows, MoePlan):
+        n = _scratch_bytes(w, 0, C.byref(SgMoePlan(rows.max_tokens, rows.n_used, rows.n_expert)))
+    else:
+        n = _scratch_bytes(w, rows, None)
     with _on(stream):
         return torch.empty(n, dtype=torch.uint8, device=w.data.device)
 
 
-def _product(x, shape, w, up, out, dtype, rows, scratch, key, stream):
-    """What the two products have in common: the arguments of the call from x on."""
+def _product(x, shape, w, up, out, dtype, rows, scratch, plan, stream):
+    """What the two products have in common: the arguments of the call from x on (plan: an expert's, or None)."""
     dev, stride = _dev(x, "x"), x.stride()
     if len(shape) != 2 or shape[1] != w.cols or (stride[1] != 1 and shape[0]) or dev != w.dev:
         raise ValueError("x must be a tensor [rows, %d] with contiguous rows on the matrix's CUDA device" % w.cols)
@@ -120,7 +127,8 @@ def _product(x, shape, w, up, out, dtype, rows, scratch, key, stream):
             (dtype is not None and dtype is not out.dtype)):
         raise ValueError("out must be a tensor [%d, %d] with contiguous rows on x's device" % (rows, w.rows))
     if scratch is None:
-        scratch = mx4_scratch(w, key, stream)
+        with _on(stream):  # (of a plan, for the tokens that it holds)
+            scratch = torch.empty(_scratch_bytes(w, rows, None) if plan is None else _scratch_bytes(w, 0, plan._c), dtype=torch.uint8, device=x.device)
     elif scratch.dtype is not torch.uint8 or not scratch.is_contiguous() or scratch.get_device() != dev:
         raise ValueError("scratch must be a contiguous uint8 tensor on x's device")
     return out, (_type(x, "x"), x.data_ptr(), stride[0]), (_type(out, "out"), out.data_ptr(), so[0], scratch.data_ptr(), scratch.numel(), _s(stream, x))
@@ -132,7 +140,7 @@ def mx4_matmul(x, w, up=None, out=None, dtype=None, scratch=None, stream=None):
     [rows, w.rows] of dtype (x's if None)."""
     shape = x.shape
     rows = shape[0]
-    out, xs, rest = _product(x, shape, w, up, out, dtype, rows, scratch, rows, stream)
+    out, xs, rest = _product(x, shape, w, up, out, dtype, rows, scratch, None, stream)
     st = _lib.load().sg_mx4_matmul(w._c, None if up is None else up._c, *xs, rows, *rest)
     if st:
         _lib.check(st, "mx4_matmul")

@@ -110,3 +110,19 @@ def test_calls_set_the_tokens(lib):
     for n in (9, 0, 3):
         assert mx4.moe_route(torch.zeros(n, 8), p) is p and state(p)[:2] == (n, n) and lib.tokens[-1] == n and p.order.shape == (2 * n,)
         assert mx4.moe_sort(torch.zeros(n, 2, dtype=torch.int32), torch.zeros(n, 2), p) is p and lib.tokens[-1] == n
+
+
+@pytest.mark.parametrize("e,k,rows,cols", [(1, 1, 100, 64), (8, 2, 300, 512), (60, 6, 129, 1024), (128, 8, 768, 2048), (1000, 16, 40, 96)])
+def test_scratch_grows_with_the_tokens(e, k, rows, cols):
+    # what is made for the largest step serves every smaller one
+    L, m = _lib.load(), _lib.SgMx4(e, rows, cols, None)
+    last = 0
+    for n in list(range(0, 700)) + list(range(700, 20000, 37)):
+        size = L.sg_mx4_scratch_bytes(C.byref(m), 0, C.byref(_lib.SgMoePlan(n, k, e)))
+        assert size >= last
+        last = size
+    one, last = _lib.SgMx4(1, rows, cols, None), 0
+    for n in range(0, 3000):
+        size = L.sg_mx4_scratch_bytes(C.byref(one), n, None)
+        assert size >= last
+        last = size

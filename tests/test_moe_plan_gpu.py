@@ -31,3 +31,19 @@ def test_refused_calls_leave_the_plan(dev, n, other):
             assert torch.equal(t, was)
         assert torch.equal(sg.moe_combine(sg.mx4_experts(x, w, p, gather=True), p), want)
     sg.device_status()
+
+
+@pytest.mark.parametrize("e,k,most", [(8, 2, 700), (128, 8, 600)])
+def test_one_scratch_for_all_steps(dev, e, k, most):
+    # made beside the plan, before any step; kept as the steps grow and shrink
+    w = sg.mx4_quantize(rand(dev, e, 200, 320, seed=2))
+    p = sg.MoePlan(most, k, e, device=dev)
+    scratch, rows = sg.mx4_scratch(w, p), sg.mx4_scratch(sg.mx4_quantize(rand(dev, 200, 320)), most)
+    for n in (0, 5, most, 33, 300, 1):
+        x = rand(dev, n, 320, seed=n)
+        sg.moe_route(rand(dev, n, e, seed=n + 1), p)
+        assert torch.equal(sg.mx4_experts(x, w, p, gather=True, scratch=scratch), sg.mx4_experts(x, w, p, gather=True))
+        assert sg.mx4_scratch(w, p).numel() == scratch.numel()
+        W = sg.mx4_quantize(rand(dev, 200, 320, seed=3))
+        assert torch.equal(sg.mx4_matmul(x, W, scratch=rows), sg.mx4_matmul(x, W))
+    sg.device_status()
