@@ -141,15 +141,16 @@ __device__ __forceinline__ bool elect_one() {
 
 // silu(g) * u, by E = exp(-|g|), at most 1: the logistic function of g is 1 or E (of a negative g) over 1 + E.  The exponent
 // |g| log2(e) is taken with its rest, so that E of a far g is off by little more than ex2's 2 units (|g| 1.3e-8 of it); below
-// 2^-126 it is 0.  13 instructions, two of them on the unit that has 16 lanes an SM (with expf and a division 60: a tile's
-// gates took three times as long as its products).
+// 2^-126 (g under -87.3) it is 0, and so is the result.  The function multiplies g before u does: g u alone can pass f32's
+// range where the result is small.  13 instructions, two of them on the unit that has 16 lanes an SM (with expf and a division
+// 60: a tile's gates took three times as long as its products).
 __device__ __forceinline__ float silu_times(float g, float u) {
     const float a = fminf(fabsf(g), 200.0f), t = a * -1.44269504f, rest = fmaf(a, -1.44269504f, -t);
     float e, q;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
     e = fmaf(e, rest * 0.693147181f, e);
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.0f + e));
-    return (g < 0.0f ? e : 1.0f) * (q * (g * u));
+    return (g < 0.0f ? e : 1.0f) * q * g * u;
 }
 
 // ---- what the kernels have in common ----
