@@ -694,6 +694,11 @@ SG_API uint64_t sg_mx4_scratch_bytes(const sg_mx4 *w, uint64_t n_tok, const sg_m
 SG_API sg_status sg_mx4_matmul(const sg_mx4 *w, const sg_mx4 *up, int32_t type, const void *d_x, uint64_t ldx, uint64_t n_tok,
                                int32_t out_type, void *d_out, uint64_t ldo, void *d_scratch, uint64_t scratch_bytes,
                                void *stream);
+/* How a product of n_tok rows (or of a plan's tokens) is run on the current device: *many
+ * 1 by the kernel on pairs of SMs, 0 by the one for few tokens; *rows tokens a tile.
+ * dual: with `up`.  Nothing is launched. */
+SG_API sg_status sg_mx4_tile(const sg_mx4 *w, int32_t dual, uint64_t n_tok, const sg_moe_plan *plan, int32_t *many,
+                             int32_t *rows);
 
 /* Tokens sorted by expert: n_tok tokens of n_used choices among n_expert, a (token,
  * choice) pair having the number token * n_used + choice.  All device memory of the

@@ -174,6 +174,7 @@ SIGNATURES = {
     "sg_mx4_dequantize": (I32, [C.POINTER(SgMx4), I32, P, U64, U64, P]),
     "sg_mx4_scratch_bytes": (U64, [C.POINTER(SgMx4), U64, C.POINTER(SgMoePlan)]),
     "sg_mx4_matmul": (I32, [C.POINTER(SgMx4), C.POINTER(SgMx4), I32, P, U64, U64, I32, P, U64, P, U64, P]),
+    "sg_mx4_tile": (I32, [C.POINTER(SgMx4), I32, U64, C.POINTER(SgMoePlan), C.POINTER(I32), C.POINTER(I32)]),
     "sg_moe_plan_work_bytes": (U64, [U64, U64]),
     "sg_moe_route": (I32, [I32, P, U64, I32, C.c_float, C.POINTER(SgMoePlan), P]),
     "sg_moe_sort": (I32, [C.POINTER(SgMoePlan), P]),

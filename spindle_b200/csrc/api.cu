@@ -2756,6 +2756,17 @@ uint64_t sg_mx4_scratch_bytes(const sg_mx4 *w, uint64_t n_tok, const sg_moe_plan
     return mx4_scratch_most(w, n_tok, plan);
 }
 
+sg_status sg_mx4_tile(const sg_mx4 *w, int32_t dual, uint64_t n_tok, const sg_moe_plan *plan, int32_t *many, int32_t *rows) {
+    if (sg_status st = check_mx4(w, false)) return st;
+    if (!many || !rows || n_tok >= 1ull << 31) return SG_ERR_INVALID;
+    if (plan && (!plan->n_used || !plan->n_expert || plan->n_tok >= 1ull << 31 || plan->n_used > MOE_SORT_MAX_USED)) return SG_ERR_SHAPE;
+    DevInfo *di;
+    if (sg_status st = dev_info(&di)) return st;
+    const Mx4Plan p = mx4_plan(w, dual != 0, n_tok, plan, di->sms);
+    *many = p.many, *rows = (int32_t)p.x_rows;
+    return SG_OK;
+}
+
 sg_status sg_mx4_matmul(const sg_mx4 *w, const sg_mx4 *up, int32_t type, const void *d_x, uint64_t ldx, uint64_t n_tok, int32_t out_type,
                         void *d_out, uint64_t ldo, void *d_scratch, uint64_t scratch_bytes, void *stream) {
     if (sg_status st = check_product(w, up, 1)) return st;

@@ -126,3 +126,14 @@ def test_scratch_grows_with_the_tokens(e, k, rows, cols):
         size = L.sg_mx4_scratch_bytes(C.byref(one), n, None)
         assert size >= last
         last = size
+
+
+def test_tile_refusals():
+    L, many, rows = _lib.load(), C.c_int32(), C.c_int32()
+    mat, plan = _lib.SgMx4(8, 64, 256, None), _lib.SgMoePlan(4, 2, 8)
+    call = lambda m=mat, n=4, p=None, a=many, b=rows: L.sg_mx4_tile(C.byref(m), 0, n, p and C.byref(p), a and C.byref(a), b and C.byref(b))  # noqa: E731
+    assert L.sg_mx4_tile(None, 0, 4, None, C.byref(many), C.byref(rows)) == INVALID
+    assert call(a=None) == INVALID and call(b=None) == INVALID and call(n=1 << 31) == INVALID
+    assert call(m=_lib.SgMx4(8, 64, 100, None)) == 3
+    for p in (_lib.SgMoePlan(4, 0, 8), _lib.SgMoePlan(4, 17, 8), _lib.SgMoePlan(4, 2, 0), _lib.SgMoePlan(1 << 31, 2, 8)):
+        assert call(p=p) == 3
