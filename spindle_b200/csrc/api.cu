@@ -2627,19 +2627,12 @@ struct Mx4Plan {
     uint64_t tiles;
     bool many;
 };
-// Whether tiles have 32 tokens: those of one matrix, or of an expert on average, are few.  Tiles of more waste no weights on
-// experts that have more than the average, and their kernel takes longer for the small ones.  Five mixtures (8 to 256 experts,
-// matrices of 0.5 to 29 million values), gate and up, and down, the larger tiles against 32 (geometric means): 16 places on
-// average 1.02, of an uneven router (its experts' logits 1.5 apart) 1.00; 24: 1.00 and 0.94; 28: 0.99 and 0.90; 32: 0.97 and
-// 0.90; the same experts for all tokens: 16: 0.93, 28: 0.79.  (128 experts, 2048 to 768, uneven: 768 to 2048 at 32 29 us against
-// 37; 60 experts, 1408 to 2048, even: 35 against 33.)
-bool mx4_tiles_of_32(uint64_t pairs, uint64_t groups) { return pairs <= 32 || pairs / groups <= 24; }
 Mx4Plan mx4_plan(const sg_mx4 *w, bool up, uint64_t n_tok, const sg_moe_plan *plan, int sms) {
     const uint64_t pairs = plan ? plan->n_tok * plan->n_used : n_tok, groups = plan ? std::min(plan->n_expert, pairs) : 1;
     if (!pairs) return {32, 0, false};
     const uint64_t feat_tiles = align_up(w->rows, MX4_ROWS) / MX4_ROWS, nk = mx4_nk(w);
     auto tiles = [&](uint64_t rows) { return (pairs + groups * (rows - 1)) / rows; };
-    if (mx4_tiles_of_32(pairs, groups)) return {32, tiles(32), false};
+    if (pairs / groups <= 32) return {32, tiles(32), false};
     // As long as each tile of 128 features and tokens has an SM of its own, the kernel for few tokens (33 rows of 14336 to
     // 4096: 12.5 us against 18.8 in the other; 128 rows of 14336 to 14336: 26.9 against 28.9; 192 rows: 38.7 against 31.0).
     if (tiles(128) * feat_tiles <= (uint64_t)sms) return {128, tiles(128), false};
@@ -2660,7 +2653,7 @@ uint64_t mx4_scratch_most(const sg_mx4 *w, uint64_t n_tok, const sg_moe_plan *pl
     if (!pairs) return 0;
     uint64_t most = 0;
     for (uint32_t rows : {32u, 128u, 192u, 256u})
-        if ((rows == 32) == mx4_tiles_of_32(pairs, groups)) most = std::max(most, mx4_scratch(w, {rows, (pairs + groups * (rows - 1)) / rows, false}));
+        if ((rows == 32) == (pairs / groups <= 32)) most = std::max(most, mx4_scratch(w, {rows, (pairs + groups * (rows - 1)) / rows, false}));
     return most;
 }
 
