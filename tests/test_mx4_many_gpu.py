@@ -133,3 +133,20 @@ def test_many_nonfinite_rows_stay_apart(dev, dual):
     nan[::3] = nan[1::30] = True
     nan[:, 17] = True
     assert torch.equal(y.isnan(), nan)
+
+
+# places of an expert on average up to 32 and from 33 on; experts of all numbers of tokens, tiles of 32 in part and several
+@pytest.mark.parametrize("n,e,k,tile_of", [(256, 16, 2, (0, 32)), (264, 16, 2, (0, 128)), (16, 128, 2, (0, 32)), (1024, 64, 2, (0, 32)), (1056, 64, 2, (1, 192)),
+                                           (32, 1, 1, (0, 32)), (33, 1, 1, (0, 128))])
+@pytest.mark.parametrize("uneven", [0.0, 2.0])
+def test_few_places_an_expert(dev, n, e, k, tile_of, uneven):
+    dim, ff = 288, 200
+    x, w = rand(dev, n, dim, seed=n), rand(dev, e, ff, dim, seed=3) * dim ** -0.5
+    W = sg.mx4_quantize(w)
+    p = sg.moe_route(rand(dev, n, e, seed=1) + uneven * rand(dev, e, seed=2), sg.MoePlan(n, k, e, device=dev))
+    assert tile(W, p) == tile_of
+    y, first, wq = sg.mx4_experts(x, W, p, gather=True), p.first.tolist(), U.quantized(w)
+    xq = U.quantized(x)[p.order.long() // k]
+    for i in range(e):
+        assert U.close(y[first[i]:first[i + 1]], *U.product(xq[first[i]:first[i + 1]], wq[i]))
+    sg.device_status()
