@@ -54,6 +54,9 @@ class PagedDecoder:
             raise ValueError("the embedding must be F32 or F16 rows")
         self.embed = weights["embed"].view(torch.float32 if dtypes["embed"] == F32 else torch.float16).view(c["vocab"], dim)
 
+        def dtype(name):  # (of `up` gate's, where it has none of its own)
+            return dtypes[name if name in dtypes or ".up" not in name else name.replace(".up", ".gate")]
+
         def mx4(name, *shape):
             """The matrix (or a layer's experts) if it is one in microscaled 4 bits, else None."""
             w = weights[name]
@@ -61,9 +64,9 @@ class PagedDecoder:
                 if (w.experts, w.rows, w.cols) != ((1,) + shape)[-3:]:
                     raise ValueError("%s must be a matrix %s" % (name, shape))
                 return w
-            if dtypes[name] not in (F32, F16):
+            if dtype(name) not in (F32, F16):
                 return None
-            return mx4_quantize(w.view(torch.float32 if dtypes[name] == F32 else torch.float16).view(*shape))
+            return mx4_quantize(w.view(torch.float32 if dtype(name) == F32 else torch.float16).view(*shape))
 
         def mat(name, rows, cols):
             return mx4(name, rows, cols) or repack_tiled16(dtypes[name], weights[name], rows, cols)
