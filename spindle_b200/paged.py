@@ -3,15 +3,19 @@ grow and end between steps, on the paged operators (kv4_plan, kv4_append,
 kv4_attention, logprobs) and the framework's own projections (matmul_batch),
 feed-forward layers (moe_forward_batch) and LM head.  The weights are named as
 for decoder.Decoder; the embedding is F32 or F16 rows.  A matrix that is given as
-an Mx4, or as F32 or F16 rows (which become one), is multiplied in microscaled 4
-bits (mx4_matmul), all tokens of a step in one call; a layer's experts too, sorted by
-expert (moe_route, mx4_experts, moe_combine).
+an Mx4 is multiplied in microscaled 4 bits, weights and activations (mx4_matmul), all
+tokens of a step in one call; a layer's experts too, sorted by expert (moe_route,
+mx4_experts, moe_combine).  F32 and F16 rows become an Mx4 where the caller asks for it
+(mx4=True); in a model without K-quants they do unless the caller forbids it
+(mx4=False), with a warning.
 
     p = PagedDecoder(cfg, weights, dtypes, device, n_req=8, n_blocks=512)
     out = p.step({0: prompt_a, 3: prompt_b})        # tokens of the requests that go on
     out = p.step({0: [token], 3: [token]}, end=[5]) # and requests that end
 
 `python -m spindle_b200.paged` runs it on a small random model."""
+import warnings
+
 import torch
 
 from . import F16, F32, Moe, matmul_batch, moe_forward_batch, repack_tiled16
@@ -42,9 +46,11 @@ class Mx4Ffn:
 
 class PagedDecoder:
     """n_req request rows over n_blocks blocks of `page` positions a layer; each
-    request at most max_seq positions (cfg)."""
+    request at most max_seq positions (cfg).  mx4: whether matrices of F32 or F16 rows
+    become Mx4 ones (about 16 % rms off a product); None: where no matrix is a K-quant.
+    dtypes needs no entry for an Mx4, nor for `up` (gate's then)."""
 
-    def __init__(self, cfg, weights, dtypes, device, n_req, n_blocks, page=64, max_tokens=4096):
+    def __init__(self, cfg, weights, dtypes, device, n_req, n_blocks, page=64, max_tokens=4096, mx4=None):
         c = self.cfg = dict(cfg)
         self.dev, self.n_req, self.n_blocks, self.page, self.max_tokens = device, n_req, n_blocks, page, max_tokens
         dim, hd = c["dim"], c["head_dim"]
@@ -54,33 +60,40 @@ class PagedDecoder:
             raise ValueError("the embedding must be F32 or F16 rows")
         self.embed = weights["embed"].view(torch.float32 if dtypes["embed"] == F32 else torch.float16).view(c["vocab"], dim)
 
-        def dtype(name):  # (of `up` gate's, where it has none of its own)
-            return dtypes[name if name in dtypes or ".up" not in name else name.replace(".up", ".gate")]
+        def dtype(name):
+            return None if isinstance(weights[name], Mx4) else dtypes[name if name in dtypes or ".up" not in name else name.replace(".up", ".gate")]
+        ffn_names = ["gate_exps", "up_exps", "down_exps"] if c.get("moe") else ["gate", "up", "down"]
+        kinds = {n: dtype(n) for n in ["head"] + ["l%d.%s" % (i, n) for i in range(c["n_layers"]) for n in ["wq", "wk", "wv", "wo"] + ffn_names]}
+        rows = [n for n, k in kinds.items() if k in (F32, F16)]
+        if rows and not mx4:
+            if mx4 is False or any(k not in (None, F32, F16) for k in kinds.values()):
+                raise ValueError("%s: F32 or F16 rows, which are served in microscaled 4 bits; that is asked for by mx4=True" % rows[0])
+            warnings.warn("F32 and F16 matrices are served in microscaled 4 bits, weights and activations (mx4=True asks for it, mx4=False forbids it)",
+                          stacklevel=2)
 
-        def mx4(name, *shape):
+        def in4(name, *shape):
             """The matrix (or a layer's experts) if it is one in microscaled 4 bits, else None."""
             w = weights[name]
             if isinstance(w, Mx4):
                 if (w.experts, w.rows, w.cols) != ((1,) + shape)[-3:]:
                     raise ValueError("%s must be a matrix %s" % (name, shape))
                 return w
-            if dtype(name) not in (F32, F16):
+            if kinds[name] not in (F32, F16):
                 return None
-            return mx4_quantize(w.view(torch.float32 if dtype(name) == F32 else torch.float16).view(*shape))
+            return mx4_quantize(w.view(torch.float32 if kinds[name] == F32 else torch.float16).view(*shape))
 
         def mat(name, rows, cols):
-            return mx4(name, rows, cols) or repack_tiled16(dtypes[name], weights[name], rows, cols)
+            return in4(name, rows, cols) or repack_tiled16(dtypes[name], weights[name], rows, cols)
 
         self.layers = []
         for i in range(c["n_layers"]):
             p, moe = "l%d." % i, c.get("moe")
-            names = [p + k + ("_exps" if moe else "") for k in ("gate", "up", "down")]
             ff, each = (moe["n_ff"], (moe["n_expert"],)) if moe else (c["n_ff"], ())
-            in4 = [mx4(names[0], *each, ff, dim), mx4(names[1], *each, ff, dim), mx4(names[2], *each, dim, ff)]
-            if any(m is not None for m in in4):
-                if any(m is None for m in in4):
+            mats = [in4(p + n, *each, *s) for n, s in zip(ffn_names, ((ff, dim), (ff, dim), (dim, ff)))]
+            if any(m is not None for m in mats):
+                if any(m is None for m in mats):
                     raise ValueError("gate, up and down of a layer are all in microscaled 4 bits or none of them")
-                ffn = Mx4Ffn(*in4, router=weights[p + "router"].float().view(moe["n_expert"], dim) if moe else None, moe=moe, n_max=max_tokens)
+                ffn = Mx4Ffn(*mats, router=weights[p + "router"].float().view(moe["n_expert"], dim) if moe else None, moe=moe, n_max=max_tokens)
             elif moe:
                 ffn = Moe.pack(weights[p + "router"].float(), weights[p + "gate_exps"], weights[p + "up_exps"],
                                weights[p + "down_exps"], dtypes[p + "gate_exps"], dtypes[p + "down_exps"], moe["n_expert"],

@@ -75,3 +75,52 @@ def test_up_needs_no_dtype(made, cfg):
     w, dt = model(cfg, lambda n: Q6_K if "down" in n else Q4_K)
     make(cfg, w, {n: k for n, k in dt.items() if ".up" not in n})
     assert made[0] == ("pack", Q4_K, Q6_K)
+
+
+@pytest.mark.parametrize("kind", [F16, F32])
+@pytest.mark.parametrize("name", ["head", "l0.wq", "l1.wo", "ffn"])
+@pytest.mark.parametrize("cfg", [CFG, MOE], ids=["dense", "moe"])
+def test_rows_in_a_model_of_k_quants(made, cfg, name, kind):
+    # one matrix of F16 or F32 rows (or a layer's three): 4 bits are asked for, or it is refused before anything is made
+    names = [n for n in shapes(cfg) if n.startswith(("l1.gate", "l1.up", "l1.down"))] if name == "ffn" else [name]
+    w, dt = model(cfg, lambda n: kind if n in names else Q4_K)
+    for kw in ({}, dict(mx4=None), dict(mx4=False)):
+        with pytest.raises(ValueError, match="mx4=True"):
+            paged.PagedDecoder(cfg, w, dt, torch.device("cpu"), n_req=1, n_blocks=8, **kw)
+        assert made == []
+    # beside matrices that the caller made into 4 bits as well
+    w2, dt2 = model(cfg, lambda n: kind if n in names else "mx4" if n.startswith("l0") else Q4_K)
+    with pytest.raises(ValueError, match="mx4=True"):
+        paged.PagedDecoder(cfg, w2, dt2, torch.device("cpu"), n_req=1, n_blocks=8)
+    assert made == []
+    make(cfg, w, dt, mx4=True)
+
+
+@pytest.mark.parametrize("cfg", [CFG, MOE], ids=["dense", "moe"])
+def test_a_model_of_rows(made, cfg):
+    w, dt = model(cfg, lambda n: F16)
+    with pytest.warns(UserWarning, match="4 bits"):
+        make(cfg, w, dt)
+    n = len(made)
+    assert ("mx4", torch.float16) in made and ("ffn4",) in made
+    with pytest.raises(ValueError, match="mx4=True"):
+        paged.PagedDecoder(cfg, w, dt, torch.device("cpu"), n_req=1, n_blocks=8, mx4=False)
+    assert len(made) == n
+
+
+@pytest.mark.parametrize("kw", [{}, dict(mx4=False), dict(mx4=True)])
+@pytest.mark.parametrize("cfg", [CFG, MOE], ids=["dense", "moe"])
+def test_what_the_caller_made_stays(made, cfg, kw, recwarn):
+    # Mx4s, with K-quants beside them or without, need no entry in dtypes
+    for kind in (lambda n: "mx4", lambda n: "mx4" if n.startswith(("l0.gate", "l0.up", "l0.down")) else Q4_K):
+        make(cfg, *model(cfg, kind), **kw)
+        assert made[0] == ("ffn4",) and not any(m[0] == "mx4" for m in made)
+    w, dt = model(cfg, lambda n: Q4_K)
+    make(cfg, w, dt, **kw)
+    assert not recwarn.list
+
+
+def test_up_of_another_kind(made):
+    w, dt = model(CFG, lambda n: F16 if n == "l0.up" else Q4_K)
+    with pytest.raises(ValueError):
+        paged.PagedDecoder(CFG, w, dt, torch.device("cpu"), n_req=1, n_blocks=8, mx4=True)
