@@ -25,6 +25,20 @@ from .mx4 import MoePlan, Mx4, moe_combine, moe_route, mx4_experts, mx4_matmul, 
 BATCH = 128  # tokens of one batch GEMM or expert pass
 
 
+def _router_logits(x, router):
+    """x router^T in whole f32, as the K-quant layers' router has it, whatever torch's switches for faster f32 products say:
+    a logit off by TF32's 2^-11 chooses other experts."""
+    m = torch.backends.cuda.matmul
+    was = m.fp32_precision
+    if was in ("ieee", "none"):
+        return x @ router.T
+    m.fp32_precision = "ieee"
+    try:
+        return x @ router.T
+    finally:
+        m.fp32_precision = was
+
+
 class Mx4Ffn:
     """A feed-forward layer in microscaled 4 bits: silu(x gate) * (x up), down; with a
     router a mixture of experts (moe: n_expert, n_used, norm, prune), n_max tokens at
@@ -40,7 +54,7 @@ class Mx4Ffn:
     def __call__(self, x):
         if not self.moe:
             return mx4_matmul(mx4_matmul(x, self.gate, up=self.up), self.down)
-        p = moe_route(x @ self.router.T, self.plan, norm=self.moe.get("norm", True), prune=self.moe.get("prune", 0.0))
+        p = moe_route(_router_logits(x, self.router), self.plan, norm=self.moe.get("norm", True), prune=self.moe.get("prune", 0.0))
         return moe_combine(mx4_experts(mx4_experts(x, self.gate, p, up=self.up), self.down, p), p)
 
 

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import spindle_b200 as sg
-from spindle_b200.paged import PagedDecoder
+from spindle_b200.paged import Mx4Ffn, PagedDecoder
 from test_paged_gpu import DENSE, MOE, model
 
 pytestmark = pytest.mark.gpu
@@ -26,3 +26,22 @@ def test_a_head_of_rows(dev, cfg):
     a, b = (PagedDecoder(cfg, w, d, dev, n_req=1, n_blocks=16).step({0: toks})["logits"] for d in (dt, {k: v for k, v in dt.items() if k not in names}))
     assert torch.equal(a, b)
     sg.device_status()
+
+
+@pytest.mark.parametrize("n", [3, 300])
+def test_the_router_is_whole_f32(dev, n):
+    # torch's switch for TF32 products changes no token's experts, and is left as it was
+    g = torch.Generator(device=dev).manual_seed(n)
+    dim, ff, e = 512, 64, 64
+    gate, up, down = (sg.mx4_quantize(torch.randn(e, a, b, device=dev, generator=g) * b ** -0.5) for a, b in ((ff, dim), (ff, dim), (dim, ff)))
+    x, router = torch.randn(n, dim, device=dev, generator=g), torch.randn(e, dim, device=dev, generator=g)
+    ffn = Mx4Ffn(gate, up, down, router=router, moe=dict(n_expert=e, n_used=8, n_ff=ff), n_max=n)
+    want, weights = ffn(x), ffn.plan.weights.clone()
+    m = torch.backends.cuda.matmul
+    was = m.fp32_precision
+    try:
+        for on in ("tf32", "ieee"):
+            m.fp32_precision = on
+            assert torch.equal(ffn(x), want) and torch.equal(ffn.plan.weights, weights) and m.fp32_precision == on
+    finally:
+        m.fp32_precision = was
