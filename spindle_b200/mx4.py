@@ -222,10 +222,9 @@ def moe_sort(ids, weights, plan, stream=None):
     st = _lib.ERR_CUDA
     try:
         with _on(stream):
-            if n and ids.data_ptr() != plan.ids.data_ptr():
-                plan.ids.copy_(ids)
-            if n and weights.data_ptr() != plan.weights.data_ptr():
-                plan.weights.copy_(weights)
+            for t, to in ((ids, plan.ids), (weights, plan.weights)):
+                if n and not (t.data_ptr() == to.data_ptr() and t.is_contiguous()):  # (rows of the plan's own array: by way of others)
+                    to.copy_(t.clone() if t.untyped_storage().data_ptr() == to.untyped_storage().data_ptr() else t)
         st = _lib.load().sg_moe_sort(plan._c, handle)
     finally:
         if st:  # (the ids have been written, or some of them)

@@ -137,3 +137,13 @@ def test_tile_refusals():
     assert call(m=_lib.SgMx4(8, 64, 100, None)) == 3
     for p in (_lib.SgMoePlan(4, 0, 8), _lib.SgMoePlan(4, 17, 8), _lib.SgMoePlan(4, 2, 0), _lib.SgMoePlan(1 << 31, 2, 8)):
         assert call(p=p) == 3
+
+
+def test_sort_of_the_plans_own_arrays(lib):
+    # rows of what the plan holds already, in another order or without some
+    for pick in (lambda t: t[:3], lambda t: t[2:], lambda t: t[::2], lambda t: t[1:4]):
+        p = HostPlan(12, 2, 8)
+        ids, w = torch.arange(20, dtype=torch.int32).view(10, 2) % 8, torch.rand(10, 2)
+        mx4.moe_sort(ids, w, p)
+        mx4.moe_sort(pick(p.ids).contiguous() if pick(p.ids).stride(0) != 2 else pick(p.ids), pick(p.weights), p)
+        assert torch.equal(p.ids, pick(ids)) and torch.equal(p.weights, pick(w)) and p.n_tok == pick(ids).shape[0]

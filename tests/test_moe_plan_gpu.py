@@ -47,3 +47,15 @@ def test_one_scratch_for_all_steps(dev, e, k, most):
         W = sg.mx4_quantize(rand(dev, 200, 320, seed=3))
         assert torch.equal(sg.mx4_matmul(x, W, scratch=rows), sg.mx4_matmul(x, W))
     sg.device_status()
+
+
+@pytest.mark.parametrize("n,first", [(6000, 1), (6000, 2999), (90, 37)])
+def test_sort_of_the_plans_own_arrays(dev, n, first):
+    ids = torch.randint(-1, 16, (n, 4), dtype=torch.int32, device=dev, generator=torch.Generator(device=dev).manual_seed(1))
+    w = rand(dev, n, 4, seed=2)
+    a, b = (sg.moe_sort(ids, w, sg.MoePlan(n, 4, 16, device=dev)) for _ in range(2))
+    sg.moe_sort(a.ids[first:], a.weights[first:], a)
+    sg.moe_sort(ids[first:].clone(), b.weights[first:].clone(), b)
+    for x, y in ((a.ids, b.ids), (a.weights, b.weights), (a.first, b.first), (a.order, b.order), (a.place, b.place)):
+        assert torch.equal(x, y)
+    assert torch.equal(a.ids, ids[first:])
