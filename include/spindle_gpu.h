@@ -677,7 +677,7 @@ typedef struct {
 SG_API uint64_t sg_mx4_bytes(const sg_mx4 *m);
 /* Quantizes d_x (SG_F32, SG_F16 or SG_BF16), element (e, r, c) at d_x[e * ld_expert +
  * r * ld + c]; sg_mx4_dequantize gives the values back the same way (rounded to
- * f16 where they are f16). */
+ * f16 where they are f16; rows of two experts must not overlap). */
 SG_API sg_status sg_mx4_quantize(const sg_mx4 *m, int32_t type, const void *d_x, uint64_t ld, uint64_t ld_expert,
                                  void *stream);
 SG_API sg_status sg_mx4_dequantize(const sg_mx4 *m, int32_t type, void *d_out, uint64_t ld, uint64_t ld_expert,

@@ -2746,6 +2746,8 @@ sg_status sg_mx4_dequantize(const sg_mx4 *m, int32_t type, void *d_out, uint64_t
     const uint32_t es = act_bytes(type);
     if (!es) return SG_ERR_DTYPE;
     if (!d_out || (m->rows > 1 && ld < m->cols)) return SG_ERR_INVALID;
+    // (no value is written twice: an expert's rows behind those of the one before, or all experts' between two rows)
+    if (m->experts > 1 && ld_expert < (m->rows - 1) * ld + m->cols && (ld_expert < m->cols || ld < (m->experts - 1) * ld_expert + m->cols)) return SG_ERR_INVALID;
     if (!aligned(d_out, es)) return SG_ERR_ALIGN;
     DevInfo *di;
     if (sg_status st = dev_info(&di)) return st;

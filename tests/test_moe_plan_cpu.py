@@ -147,3 +147,11 @@ def test_sort_of_the_plans_own_arrays(lib):
         mx4.moe_sort(ids, w, p)
         mx4.moe_sort(pick(p.ids).contiguous() if pick(p.ids).stride(0) != 2 else pick(p.ids), pick(p.weights), p)
         assert torch.equal(p.ids, pick(ids)) and torch.equal(p.weights, pick(w)) and p.n_tok == pick(ids).shape[0]
+
+
+def test_read_back_refuses_rows_over_one_another():
+    # element (e, r, c) at e * ld_expert + r * ld + c: two experts' would be the same
+    L, at = _lib.load(), 0x100000
+    call = lambda e, r, ld, le: L.sg_mx4_dequantize(C.byref(_lib.SgMx4(e, r, 64, at)), 0, at, ld, le, None)  # noqa: E731
+    for e, r, ld, le in ((2, 4, 64, 0), (2, 4, 64, 255), (2, 4, 100, 63), (3, 4, 191, 64), (3, 1, 64, 63), (2, 4, 128, 100)):
+        assert call(e, r, ld, le) == INVALID

@@ -59,3 +59,15 @@ def test_sort_of_the_plans_own_arrays(dev, n, first):
     for x, y in ((a.ids, b.ids), (a.weights, b.weights), (a.first, b.first), (a.order, b.order), (a.place, b.place)):
         assert torch.equal(x, y)
     assert torch.equal(a.ids, ids[first:])
+
+
+def test_read_back_between_rows(dev):
+    # an expert's rows behind the other's, and all experts' between two rows
+    x = rand(dev, 3, 70, 96, seed=1)
+    m = sg.mx4_quantize(x)
+    want = sg.mx4_dequantize(m)
+    for out in (torch.full((3, 75, 100), 7.0, device=dev)[:, :70, :96], torch.full((70, 3, 99), 7.0, device=dev).transpose(0, 1)[:, :, :96],
+                torch.full((70, 3, 96), 7.0, device=dev).transpose(0, 1)):
+        assert torch.equal(sg.mx4_dequantize(m, out=out), want)
+    with pytest.raises(sg.SgError):
+        sg.mx4_dequantize(m, out=torch.zeros(1, 70, 96, device=dev).expand(3, 70, 96))
