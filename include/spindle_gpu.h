@@ -710,6 +710,8 @@ SG_API sg_status sg_mx4_tile(const sg_mx4 *w, int32_t dual, uint64_t n_tok, cons
  *     one expert stand in rising order;
  *   place [n_tok * n_used]: the place of each pair, -1 for none;
  *   work: sg_moe_plan_work_bytes(n_tok, n_expert) bytes, 16-byte aligned.
+ * n_tok has to be that of the call that filled the arrays last, a replayed graph's as
+ * well; with another one results are not defined, but nothing outside is read or written.
  * n_used <= SG_MOE_MAX_USED, n_expert <= 1024, n_tok * n_used < 2^31. */
 struct sg_moe_plan_ {
     uint64_t n_tok, n_used, n_expert;

@@ -2692,7 +2692,7 @@ sg_status mx4_product(const sg_mx4 *w, const sg_mx4 *up, const sg_moe_plan *plan
     if (plan) {
         q.n_used = (uint32_t)plan->n_used, q.ids = plan->ids, q.place = plan->place, q.order = gather ? nullptr : plan->order;
         q.first = g.first = plan->first, q.tiles = plan_tiles(plan, mp.x_rows);
-        g.n_expert = (uint32_t)plan->n_expert;
+        q.n_expert = g.n_expert = (uint32_t)plan->n_expert, q.n_pairs = g.n_places = (uint32_t)pairs, q.out_rows = mp.tiles * mp.x_rows;
     }
     CK(mx4_quantize_launch(q, type, di->sms, s));
     g.vec = rows16(d_out, pairs > 1 ? ldo : 0, eo), g.pairs = eo == 2 && aligned(d_out, 4) && !(ldo & 1);

@@ -114,10 +114,13 @@ __global__ void __launch_bounds__(MX4_QUANT_THREADS) mx4_quantize_kernel(const _
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, side = lane >> 4, chunk = lane >> 1 & 7u, part = lane & 1u;
     const uint32_t tile_bytes = mx4_tile_bytes(a.x_rows), half = mx4_scale_bytes(a.x_rows) / 2, rows_at_once = gridDim.x * (MX4_QUANT_THREADS / 32);
     if (a.early) grid_launch_dependents();
-    // a row's place among the tiles, from its place among the sorted ones
-    auto row_of = [&](int32_t pair, uint32_t place) {
-        const int32_t e = __ldg(a.ids + pair);
-        return (int64_t)__ldg(a.tiles + e) * a.x_rows + (place - (uint32_t)__ldg(a.first + e));
+    // a row's place among the tiles, from its place among the sorted ones (-1: none; a plan that was filled anew for other tokens
+    // than the host counts, by a replayed graph, leads nowhere outside)
+    auto row_of = [&](int32_t pair, uint32_t place) -> int64_t {
+        const uint32_t e = (uint32_t)pair < a.n_pairs ? (uint32_t)__ldg(a.ids + pair) : a.n_expert;
+        if (e >= a.n_expert) return -1;
+        const uint64_t row = (uint64_t)(uint32_t)__ldg(a.tiles + e) * a.x_rows + (place - (uint32_t)__ldg(a.first + e));
+        return row < a.out_rows ? (int64_t)row : -1;
     };
     for (uint32_t kt0 = blockIdx.y * QUANT_TILES; kt0 < a.nk; kt0 += gridDim.y * QUANT_TILES) {
         const uint32_t kt = kt0 + side, col = kt * MX4_COLS + (lane & 15u) * 16;

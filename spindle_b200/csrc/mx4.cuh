@@ -53,6 +53,8 @@ struct Mx4QuantArgs {
     // places of the pairs i * n_used + 0..
     uint32_t n_used;
     const int32_t *ids, *place, *order, *first, *tiles;
+    uint32_t n_pairs, n_expert;    // what the host knows of them: nothing is read or written past these and out_rows
+    uint64_t out_rows;             // rows of the tiles that out has room for
     bool vec;                      // x allows 16-byte loads
     bool early;                    // the next launch may begin at once: it waits for this one before it reads what is written here
 };
@@ -78,8 +80,8 @@ struct Mx4GemmArgs {
     uint32_t feats, nk;            // rows of w, tiles along its columns
     uint32_t feat_tiles;
     uint64_t n_tok;                // rows of x, where they are one matrix
-    const int32_t *first;          // experts: the first sorted place of each (n_expert + 1)
-    uint32_t n_expert;
+    const int32_t *first;          // experts: the first sorted place of each (n_expert + 1), at most n_places
+    uint32_t n_expert, n_places;
     bool vec, pairs;               // out's rows allow 16-byte stores; 16-bit rows that allow 4-byte ones
 };
 cudaError_t mx4_many_launch(const Mx4GemmArgs &a, uint32_t x_rows, uint64_t token_tiles, int sms, cudaStream_t s);

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import spindle_b200 as sg
+from spindle_b200.mx4 import _scratch_bytes
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +72,43 @@ def test_read_back_between_rows(dev):
         assert torch.equal(sg.mx4_dequantize(m, out=out), want)
     with pytest.raises(sg.SgError):
         sg.mx4_dequantize(m, out=torch.zeros(1, 70, 96, device=dev).expand(3, 70, 96))
+
+
+@pytest.mark.parametrize("e,k,many,few,ff", [(16, 2, 3000, 40, 200), (16, 2, 3000, 2500, 200), (64, 4, 2000, 300, 1300), (4, 1, 900, 1, 64)])
+def test_a_plan_filled_by_a_replayed_graph(dev, e, k, many, few, ff):
+    # a graph sorts other numbers of tokens into the plan than the last call did that the host made: what the products give is
+    # not defined then, but they write into their rows and scratch only
+    dim = 320
+    w, v, d = (sg.mx4_quantize(rand(dev, e, a, b, seed=s) * 0.05) for a, b, s in ((ff, dim, 1), (ff, dim, 2), (dim, ff // 32 * 32, 3)))
+    p = sg.MoePlan(many, k, e, device=dev)
+    skew = rand(dev, e, seed=4) * 2
+    graphs = {}
+    for n in (many, few):
+        logits = rand(dev, n, e, seed=n) + skew
+        sg.moe_route(logits, p)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            sg.moe_route(logits, p)
+        graphs[n] = g, logits
+    for n, other in ((few, many), (many, few)):
+        sg.moe_route(graphs[n][1], p)
+        graphs[other][0].replay()                 # p.n_tok is n, the arrays hold other tokens
+        rows, x = n * k, rand(dev, n, dim, seed=5)
+        h = rand(dev, n * k, ff // 32 * 32, seed=6)
+        for m, call in ((w, lambda o, s: sg.mx4_experts(x, w, p, up=v, out=o, scratch=s)),           # noqa: B023
+                        (w, lambda o, s: sg.mx4_experts(x, w, p, gather=True, out=o, scratch=s)),    # noqa: B023
+                        (d, lambda o, s: sg.mx4_experts(h, d, p, out=o, scratch=s))):                # noqa: B023
+            size = _scratch_bytes(m, 0, p._c)
+            out, scratch = torch.full((rows + 4000, m.rows), 7.0, device=dev), torch.full((size + (1 << 22),), 0x5A, dtype=torch.uint8, device=dev)
+            call(out[:rows], scratch[:size])
+            assert (out[rows:] == 7).all() and (scratch[size:] == 0x5A).all()
+        y = torch.full((n + 4000, dim), 7.0, device=dev)
+        sg.moe_combine(rand(dev, rows, dim, seed=7), p, out=y[:n])
+        assert (y[n:] == 7).all()
+        # filled for its own tokens again, all is as it was
+        graphs[n][0].replay()
+        got = sg.mx4_experts(x, w, p, gather=True)
+        q = sg.moe_route(graphs[n][1], sg.MoePlan(n, k, e, device=dev))
+        assert torch.equal(sg.moe_combine(got, p), sg.moe_combine(sg.mx4_experts(x, w, q, gather=True), q))
+    sg.device_status()
