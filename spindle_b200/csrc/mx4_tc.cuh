@@ -150,7 +150,7 @@ __device__ __forceinline__ float silu_times(float g, float u) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
     e = fmaf(e, rest * 0.693147181f, e);
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.0f + e));
-    return (g < 0.0f ? e : 1.0f) * q * g * u;
+    return (g < 0.0f ? e : 1.0f) * g * q * u;
 }
 
 // ---- what the kernels have in common ----
