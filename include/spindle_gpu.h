@@ -663,7 +663,8 @@ SG_API sg_status sg_logprobs(int32_t type, const void *d_logits, uint64_t ld, ui
  * 6), 17 bytes per 32 values.  s is floor(log2(top)) - 2 for the largest magnitude
  * top, one more where top is 1.75 times a power of two or above, at least -127; codes
  * are rounded to nearest, ties to the even code.  A group with an infinity or a NaN
- * is NaN, all 32 values.  rms error of normally distributed values 11 % of their
+ * is NaN, all 32 values; values from 1.75 * 2^127 on become 2^128, an infinity in f32.
+ * rms error of normally distributed values 11 % of their
  * standard deviation.
  *
  * `experts` matrices of rows x cols (1: a plain matrix), cols a multiple of 32, in
@@ -685,8 +686,10 @@ SG_API sg_status sg_mx4_dequantize(const sg_mx4 *m, int32_t type, void *d_out, u
 
 /* out[t, n] = sum over k of q(x)[t, k] w[n, k] for n_tok rows of x, each quantized
  * as above on the way, whatever their number; with `up` (a matrix of w's shape)
- * silu(that) * (the same with up).  w has one expert.  Products are exact and added
- * in f32; the results are rounded once, to out_type.  d_out may be d_x.
+ * silu(that) * (the same with up); silu is 0 below -87.3.  w has one expert.  Products
+ * are exact and added in f32 by the tensor cores, 64 columns at a time, which may cut a
+ * sum off where they do not round it (a unit in its last place each time); the results
+ * are rounded once, to out_type.  d_out may be d_x.
  * d_scratch: sg_mx4_scratch_bytes(w, n_tok, NULL) bytes (0 is possible), 128-byte
  * aligned, for calls that may overlap on the GPU one each. */
 typedef struct sg_moe_plan_ sg_moe_plan;
