@@ -294,7 +294,8 @@ __global__ void __launch_bounds__(THREADS) moe_place_kernel(const __grid_constan
 // out[t] = sum over j of weights[t, j] y[place[t, j]], in the order of j, in f32.  A thread takes eight columns of a token, an
 // item, with its loads of J experts' rows in flight.  With one slot or two, two items at a time (52592 rows of 1192 bf16, a row a
 // token: eight slots, one item 125 us; one slot, one item 64, two 54, four 66; with four slots two are slower, 30.1 against 29.1).
-// What bounds it: reading y (8191 x 8 rows of 2048 bf16: 50 us, 6.0 TB/s; x 4: 29 us, 5.8 TB/s).
+// What bounds it: reading y (8191 x 8 rows of 2048 bf16: 50 us, 6.0 TB/s; x 4: 29 us, 5.8 TB/s; rows that do not begin on 16
+// bytes, value by value: 98 us).
 constexpr int combine_items(bool vec, int slots) { return vec && slots <= 2 ? 2 : 1; }
 
 template <typename T, typename O, bool VEC, int J>

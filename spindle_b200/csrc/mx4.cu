@@ -103,9 +103,9 @@ __device__ __forceinline__ uint2 quantize16(const Raw<T> &raw, uint32_t &scale) 
 }
 
 // A warp takes 1024 columns of a row, 512 at a time, all loads at once: a lane has sixteen values, two lanes a block of 32.
-// A token that goes to several experts is read and quantized once.  What bounds it: instructions (80 for a lane's sixteen
-// values, the issue slots 63 % busy) next to reading x (8191 x 4096 bf16: 18.2 us, 5.7 TB/s read and written; with eight
-// values a lane 21.5).
+// A token that goes to several experts is read and quantized once.  What bounds it: instructions (160 for a lane's sixteen
+// values, the issue slots 63 % busy) next to reading x (8191 x 4096 bf16: 18.2 us, 85 MB read and written at 4.7 TB/s; with eight
+// values a lane 21.5).  Rows that do not begin on 16 bytes are loaded value by value: 41 us, f32 73 instead of 29.
 constexpr uint32_t QUANT_TILES = 4, STEPS = QUANT_TILES / 2;
 
 template <typename T, bool VEC>
@@ -190,7 +190,8 @@ __device__ __forceinline__ float2 values2(uint32_t byte) {
 }
 
 // Eight values a lane of each of four tiles: a lane's 16-bit results are one 16-byte store beside its neighbours' (sixteen, as
-// above, would be two with gaps: 22 us for 8191 x 4096 to bf16 against 15).
+// above, would be two with gaps: 22 us for 8191 x 4096 to bf16 against 15; value by value, to rows that do not begin on 16 bytes,
+// 108).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(MX4_QUANT_THREADS) mx4_dequantize_kernel(const __grid_constant__ Mx4ReadArgs a) {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, chunk = lane >> 2, rows_at_once = gridDim.x * (MX4_QUANT_THREADS / 32);
